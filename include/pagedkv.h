@@ -378,6 +378,108 @@ int pkv_add_rms_norm_split(void *hidden, const void *partials, int32_t splits, c
  * pkv_linear ([splits][rows][2 * inter] FP32); inter a multiple of 8. */
 int pkv_silu_mul_split(const void *partials, int32_t splits, void *out, int32_t rows, int32_t inter, void *stream);
 
+/* ---- 8-bit decode path -------------------------------------------------------
+ * E4M3 codes with FP32 scales.  Scales made by these functions are powers of
+ * two, 2^e with the smallest e in [-15, 8] that brings the block's largest
+ * finite magnitude to 448 or less; every stored value is then an FP16 number.
+ * A value that is not finite is stored as NaN.  No counterpart in the reference
+ * (it keeps FP16 weights, activations and cache); each function is the 8-bit
+ * form of the FP16 function named beside it. */
+
+/* 8-bit rows: codes [rows][width] contiguous, scales [rows][ceil(width / 128)],
+ * one per 128 values (the last group may be shorter); width a multiple of 8.
+ *
+ * pkv_add_rms_norm with an 8-bit output: v = hidden + delta (delta may be null),
+ * residual = fp16(v) when delta is given (residual may be hidden itself),
+ * codes/scales of v * rsqrt(mean(v^2) + eps) * weight, FP32 throughout and
+ * rounded once.  hidden, delta, residual [rows][dim] contiguous, weight [dim],
+ * 16-byte aligned; dim a multiple of 8 up to 8192. */
+int pkv_fp8_add_rms_norm(const void *hidden, const void *delta, const void *weight, void *residual, void *codes,
+                         void *scales, int32_t rows, int32_t dim, float eps, void *stream);
+
+/* Rows of FP16 x (x_stride elements apart) to 8-bit rows; with silu_pairs, of
+ * silu(x[r][c]) * x[r][width + c] (pkv_silu_mul), FP32 and rounded once. */
+int pkv_fp8_quantize(const void *x, int64_t x_stride, int32_t silu_pairs, int32_t rows, int32_t width, void *codes,
+                     void *scales, void *stream);
+
+/* The FP16 numbers that 8-bit rows stand for (rows of out out_stride apart). */
+int pkv_fp8_to_half(const void *codes, const void *scales, int32_t rows, int32_t width, void *out, int64_t out_stride,
+                    void *stream);
+
+/* The 8-bit form of pkv_linear, any number of rows:
+ *   out[m][n] = fp16( sum_b x_scales[m][b] * w_scales[n / 128][b] * sum_{k in block b} x[m][k] * w[n][k] )
+ * x E4M3 [rows][k] with rows x_stride apart (a multiple of 16), x_scales
+ * [rows][ceil(k / 128)]; w E4M3 [n][k] contiguous, w_scales
+ * [ceil(n / 128)][ceil(k / 128)]; any FP32 scales.  k a multiple of 16, x and w
+ * 16-byte aligned, out rows out_stride elements apart.  FP32 sums, one rounding;
+ * the result does not depend on timing.  Allocates nothing. */
+int pkv_fp8_linear(const void *x, int64_t x_stride, const void *x_scales, const void *w, const void *w_scales,
+                   int32_t rows, int32_t n, int32_t k, void *out, int64_t out_stride, int32_t *error_flag,
+                   void *stream);
+
+/* 8-bit KV cache: key_codes [layers][num_blocks][4][16][64], value_codes
+ * [layers][num_blocks][4][64][16] (V tiles are transposed), key_scales and
+ * value_scales FP32 [layers][num_blocks][4]; all 16-byte aligned.
+ *
+ * pkv_append_kv into it: as there, for pool layers layer_begin .. + layer_count
+ * of the cache.  RoPE is computed in FP32 and rounded once (K to its code, the
+ * query to FP16).  The tokens written to one block in one call must be
+ * consecutive in the list and in the block, which the slots of a request's
+ * consecutive positions are.  A block's slot 0 sets its scale; a later slot
+ * raises it where it needs more, and the block's codes are rounded again to it.
+ * Codes at slots that are not listed, and past the listed ones, stay. */
+int pkv_fp8_append_kv(void *key_codes, void *value_codes, void *key_scales, void *value_scales, int32_t layers,
+                      int32_t num_blocks, int32_t layer_begin, int32_t layer_count, const void *key, const void *value,
+                      int64_t src_layer_stride, int64_t src_token_stride, const int32_t *slots,
+                      const int32_t *positions, int32_t tokens, const void *rope_table, const void *query_in,
+                      int64_t q_layer_stride, int64_t q_token_stride, void *query_out, int64_t q_out_layer_stride,
+                      int64_t q_out_token_stride, int32_t *error_flag, void *stream);
+
+/* K and V of `count` blocks (device int32) at `layer` as FP16: K [count][16][4][64]
+ * at out, V the same at out + kv_stride elements. */
+int pkv_fp8_read_blocks(const void *key_codes, const void *value_codes, const void *key_scales,
+                        const void *value_scales, int32_t layers, int32_t num_blocks, int32_t layer,
+                        const int32_t *blocks, int32_t count, void *out, int64_t kv_stride, int32_t *error_flag,
+                        void *stream);
+
+/* pkv_prefill_attention over the 8-bit cache: same arguments and result over the
+ * values that the cache holds.  The workspace (16-byte aligned, 16388 bytes for
+ * each of the ceil((start + tokens) / 16) blocks) needs no initialisation. */
+int pkv_fp8_prefill_attention(const void *key_codes, const void *value_codes, const void *key_scales,
+                              const void *value_scales, int32_t layers, int32_t num_blocks, int32_t layer,
+                              const void *query, int64_t query_stride, const int32_t *blocks, int32_t start,
+                              int32_t tokens, void *out, int64_t out_stride, void *workspace, int64_t workspace_bytes,
+                              int32_t *error_flag, void *stream);
+
+/* Grid and workspace of the two functions below on `device`. */
+int pkv_fp8_decode_plan(int32_t device, int32_t batch, int32_t total_blocks, int32_t *out_grid,
+                        int64_t *out_workspace_bytes);
+
+/* pkv_decode_attention over the 8-bit cache: query (rotated), lengths, prefix,
+ * flat and out as there; a row without blocks (prefix[b + 1] == prefix[b]) or
+ * without valid tokens gives zeros.  grid and workspace from
+ * pkv_fp8_decode_plan for the same batch and total_blocks; the workspace (16-byte
+ * aligned) needs no initialisation, and launches that share one must not overlap
+ * on the GPU. */
+int pkv_fp8_decode_attention(const void *key_codes, const void *value_codes, const void *key_scales,
+                             const void *value_scales, int32_t layers, int32_t num_blocks, int32_t layer,
+                             const void *query, int64_t query_stride, const int32_t *lengths, const int32_t *prefix,
+                             const int32_t *flat, int32_t batch, int32_t total_blocks, int32_t grid, void *out,
+                             int64_t out_stride, void *workspace, int64_t workspace_bytes, int32_t *error_flag,
+                             void *stream);
+
+/* pkv_decode_layer over the 8-bit cache: the new token of every row (position
+ * lengths[b] - 1, in the row's last block) has its K rotated and K and V written
+ * as pkv_fp8_append_kv does, its query rotated, and attends to all lengths[b]
+ * tokens.  query, key and value unrotated, rows query_stride / kv_stride apart.
+ * No two rows may share a last block. */
+int pkv_fp8_decode_layer(void *key_codes, void *value_codes, void *key_scales, void *value_scales, int32_t layers,
+                         int32_t num_blocks, int32_t layer, const void *query, int64_t query_stride, const void *key,
+                         const void *value, int64_t kv_stride, const void *rope_table, const int32_t *lengths,
+                         const int32_t *prefix, const int32_t *flat, int32_t batch, int32_t total_blocks, int32_t grid,
+                         void *out, int64_t out_stride, void *workspace, int64_t workspace_bytes, int32_t *error_flag,
+                         void *stream);
+
 #ifdef __cplusplus
 }
 #endif

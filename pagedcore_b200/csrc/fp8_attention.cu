@@ -1,0 +1,691 @@
+// Batched one-token attention over the 8-bit KV cache (layout: fp8_cache.cuh):
+//   out[b, h] = sum_t softmax_t(q[b, h] . K[t, h / 8] / 8) V[t, h / 8]
+// over the lengths[b] tokens that row b's block table lists, K and V being the
+// cache's codes times their block's scale.
+//
+// Work split, as in the FP16 kernel: the batch's block tables form one flat
+// list, CTA g streams piece g of it (equal pieces), warp w serves KV head w and
+// its eight query heads.  A row that one piece holds is written directly; the
+// others leave (m, l, O) partials at index row + piece (unique: along the
+// pieces the pairs form a monotone staircase) that a second kernel, launched
+// as its programmatic dependent, merges in piece order.
+//
+// Data movement: every warp runs its own ring of stages of up to four blocks
+// (64 tokens): per block one bulk copy each for the 1 KiB K tile, the 1 KiB V
+// tile and the two 16-byte scale rows.  V tiles lie 1056 bytes apart, so the
+// 16-byte reads below are free of bank conflicts.
+//
+// Math: mma.sync m16n8k16 on FP16 operands made from codes in registers
+// (E4M3 to FP16 is exact), FP32 sums:
+//   S^T[16 tok x 8 heads]  = K[16 x 64] . Q^T[64 x 8]
+//   O^T[64 dims x 8 heads] += V^T[64 x 16] . P^T[16 x 8]
+// The summed indices may be taken in any order, so each lane reads 16
+// consecutive codes: in the first product lane (g, t) holds dims 16 t .. +15 of
+// two tokens of block g / 2, in the second all 16 tokens of block t for dims
+// g + 8 i; MMA j of either covers tokens 4 j .. 4 j + 3 of the four blocks, and the
+// S^T accumulator becomes the P^T operand with two 8 x 8 transposes.
+//
+// Scales: K's multiplies the score.  V's, 2^e of the token's block, goes into
+// the exponent: the weight is w = 2^(s + e - M + 15) with M the running maximum
+// of s + e, so the largest contribution, not the largest probability, sits at
+// 2^15 and blocks of very different magnitude lose nothing; the normaliser adds
+// w * 2^-e, in FP32.  w is rounded to FP16 (2^-11 of each weight, below the
+// 2^-4 of the codes that it multiplies); scores, maxima, normaliser and sums
+// are FP32.
+
+#include <cuda_fp16.h>
+#include <cuda_runtime.h>
+#include <stdint.h>
+
+#include <mutex>
+#include <string>
+#include <unordered_map>
+
+#include "fp8_cache.cuh"
+#include "pdl.h"
+#include "ptx.cuh"
+#include "status.h"
+
+namespace pkv::fp8 {
+int check_cache(const void *key_codes, const void *value_codes, const void *key_scales, const void *value_scales,
+                int32_t layers, int32_t num_blocks, int32_t layer_begin, int32_t layer_count);
+int launch_decode_append(const Cache &cache, int32_t layer, const void *key, const void *value, int64_t kv_stride,
+                         const void *rope_table, const void *query, int64_t query_stride, void *query_out,
+                         const int32_t *lengths, const int32_t *prefix, const int32_t *flat, int32_t batch,
+                         int32_t total_blocks, int32_t *error_flag, cudaStream_t stream);
+}
+
+namespace {
+
+constexpr int kDim = PKV_HEAD_DIM;
+constexpr int kHeads = PKV_KV_HEADS;
+constexpr int kQueryHeads = PKV_QUERY_HEADS;
+constexpr int kGroup = kQueryHeads / kHeads;
+constexpr int kSlots = PKV_BLOCK_TOKENS;
+constexpr int kTile = pkv::fp8::kTileBytes;
+constexpr int kWarps = kHeads;
+constexpr int kThreads = kWarps * 32;
+constexpr int kChunk = 4;     // blocks per stage
+constexpr int kStages = 3;
+constexpr int kValuePitch = kTile + 32;
+constexpr int kValueAt = kChunk * kTile;
+constexpr int kScaleAt = kValueAt + kChunk * kValuePitch;   // K then V scale rows, 16 bytes a block
+constexpr int kStageBytes = kScaleAt + 2 * kChunk * 16;
+constexpr int kBlockTraffic = 2 * kTile + 32;
+constexpr int kSmem = kWarps * kStages * kStageBytes;
+constexpr uint32_t kWaitPolls = 1u << 24;
+constexpr float kScaleLog2 = 0.125f * 1.4426950408889634f;  // 64^-0.5 * log2(e)
+constexpr float kWeightShift = 15.0f;
+constexpr float kLowest = -1e30f;  // below every finite score
+constexpr int kPartial = kQueryHeads * (kDim + 2);  // floats of a partial
+
+struct Args {
+    pkv::fp8::Cache cache;
+    int32_t layer;
+    const __half *query;
+    int64_t query_stride;
+    const int32_t *lengths;
+    const int32_t *prefix;
+    const int32_t *flat;
+    int32_t batch;
+    int32_t total;
+    int32_t grid;
+    __half *out;
+    int64_t out_stride;
+    float *part_o;   // [batch + grid][32][64]
+    float *part_ml;  // [batch + grid][32][2]
+    int32_t *error_flag;
+};
+
+// Piece g covers blocks [g * total / grid, (g + 1) * total / grid).
+__host__ __device__ __forceinline__ int piece_begin(int g, int total, int grid) {
+    return static_cast<int>(static_cast<int64_t>(g) * total / grid);
+}
+
+__device__ __forceinline__ int piece_of(int block, int total, int grid) {
+    return static_cast<int>(((static_cast<int64_t>(block) + 1) * grid - 1) / total);
+}
+
+__device__ __forceinline__ void bulk_load(uint32_t dst, const void *src, uint32_t bytes, uint32_t bar,
+                                          uint64_t policy) {
+    asm volatile(
+        "cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes.L2::cache_hint [%0], [%1], %2, [%3], %4;"
+        ::"r"(dst), "l"(src), "r"(bytes), "r"(bar), "l"(policy)
+        : "memory");
+}
+
+__device__ __forceinline__ uint4 lds128(uint32_t addr) {
+    uint4 v;
+    asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(addr));
+    return v;
+}
+
+__device__ __forceinline__ float lds32(uint32_t addr) {
+    float v;
+    asm volatile("ld.shared.f32 %0, [%1];" : "=f"(v) : "r"(addr));
+    return v;
+}
+
+__device__ __forceinline__ float max8(float v) {
+    v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, 4));
+    v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, 8));
+    return fmaxf(v, __shfl_xor_sync(0xffffffffu, v, 16));
+}
+
+__device__ __forceinline__ float sum8(float v) {
+    v += __shfl_xor_sync(0xffffffffu, v, 4);
+    v += __shfl_xor_sync(0xffffffffu, v, 8);
+    return v + __shfl_xor_sync(0xffffffffu, v, 16);
+}
+
+__device__ __forceinline__ uint32_t word(const uint4 &v, int i) {
+    return i == 0 ? v.x : i == 1 ? v.y : i == 2 ? v.z : v.w;
+}
+
+// The low `keep` (0 .. 16) bytes of v.
+__device__ __forceinline__ uint4 keep_bytes(const uint4 &v, int keep) {
+    uint32_t m[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const int k = min(max(keep - 4 * i, 0), 4);
+        m[i] = k == 4 ? 0xffffffffu : (1u << (8 * k)) - 1u;
+    }
+    return make_uint4(v.x & m[0], v.y & m[1], v.z & m[2], v.w & m[3]);
+}
+
+// Rows of the block list: where each ends.  32 rows from `base` in registers.
+struct Rows {
+    int base, last, length;
+};
+
+__device__ __forceinline__ Rows load_rows(const Args &a, int base, int lane) {
+    const int r = base + lane;
+    return Rows{base, r < a.batch ? a.prefix[r + 1] : INT32_MAX, r < a.batch ? a.lengths[r] : 0};
+}
+
+// The first row at or after `row` that has blocks past `block`, with its window.
+__device__ __forceinline__ int advance_row(const Args &a, Rows &w, int row, int block, int lane) {
+    while (true) {
+        if (row - w.base >= 32) w = load_rows(a, row, lane);
+        const unsigned past = __ballot_sync(0xffffffffu, w.base + lane >= row && w.last > block);
+        if (past != 0) return w.base + __ffs(past) - 1;
+        row = w.base + 32;
+    }
+}
+
+__device__ __forceinline__ void load_query(const Args &a, int row, int head, int t, uint32_t (&q)[8]) {
+    const uint4 *src = reinterpret_cast<const uint4 *>(a.query + row * a.query_stride + head * kDim + 16 * t);
+    const uint4 x = src[0], y = src[1];
+    q[0] = x.x, q[1] = x.y, q[2] = x.z, q[3] = x.w;
+    q[4] = y.x, q[5] = y.y, q[6] = y.z, q[7] = y.w;
+}
+
+__global__ void __launch_bounds__(kThreads, 2) fp8_decode_kernel(const __grid_constant__ Args a) {
+    extern __shared__ __align__(16) uint8_t smem[];
+    __shared__ __align__(8) uint64_t barriers[kWarps * kStages];
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int g = lane >> 2, t = lane & 3;
+    const uint32_t ring = pkv::smem_addr(smem) + warp * kStages * kStageBytes;
+    const uint32_t bar0 = pkv::smem_addr(&barriers[warp * kStages]);
+    if (lane == 0) {
+        for (int s = 0; s < kStages; ++s) pkv::mbar_init(bar0 + 8 * s, 1);
+        pkv::fence_barrier_init();
+    }
+    __syncwarp();
+    pkv::pdl_wait();
+    pkv::pdl_launch_dependents();
+
+    // Rows without blocks: zeros.
+    for (int b = blockIdx.x * kThreads + threadIdx.x; b < a.batch; b += a.grid * kThreads) {
+        if (a.prefix[b + 1] <= a.prefix[b]) {
+            for (int i = 0; i < kQueryHeads * kDim; ++i) a.out[b * a.out_stride + i] = __float2half_rn(0.f);
+        }
+    }
+    const int begin = piece_begin(blockIdx.x, a.total, a.grid);
+    const int end = piece_begin(blockIdx.x + 1, a.total, a.grid);
+    if (begin >= end) return;
+
+    const uint64_t policy = pkv::l2_policy_evict_first();
+    // First row with blocks past `begin`, by a 32-way search over prefix[1 ..].
+    int lo = 0, hi = a.batch - 1;
+    while (hi > lo) {
+        const int step = (hi - lo + 32) / 32;
+        const int probe = min(lo + lane * step + step - 1, hi);
+        const unsigned past = __ballot_sync(0xffffffffu, a.prefix[probe + 1] > begin);
+        const int which = past != 0 ? __ffs(past) - 1 : 31;
+        lo = min(lo + which * step, hi);
+        hi = min(lo + step - 1, hi);
+    }
+
+    // Fetch cursor: the next block to copy, the row it belongs to, and the ids
+    // of the list's next 64 blocks (32 at a time, one window ahead).
+    Rows fetch_rows = load_rows(a, lo, lane);
+    int fetch_row = advance_row(a, fetch_rows, lo, begin, lane);
+    int fetch_end = __shfl_sync(0xffffffffu, fetch_rows.last, fetch_row - fetch_rows.base);
+    int fetch = begin;
+    int ids_base = begin;
+    int ids = begin + lane < end ? a.flat[begin + lane] : 0;
+    int ids_next = begin + 32 + lane < end ? a.flat[begin + 32 + lane] : 0;
+    int fetched = 0;
+
+    const int64_t layer_tile = pkv::fp8::tile_index(a.cache, a.layer, 0, 0);
+    // Copy the next chunk into stage `fetched % kStages`.
+    const auto issue = [&]() {
+        if (fetch >= end) return;
+        if (fetch >= fetch_end) {
+            fetch_row = advance_row(a, fetch_rows, fetch_row + 1, fetch, lane);
+            fetch_end = __shfl_sync(0xffffffffu, fetch_rows.last, fetch_row - fetch_rows.base);
+        }
+        const int n = min(kChunk, min(fetch_end, end) - fetch);
+        if (fetch - ids_base >= 32) {
+            ids = ids_next;
+            ids_base += 32;
+            const int ahead = ids_base + 32 + lane;
+            ids_next = ahead < end ? a.flat[ahead] : 0;
+        }
+        const int at = fetch - ids_base + (lane & 3);
+        const int near = __shfl_sync(0xffffffffu, ids, at & 31);
+        const int far = __shfl_sync(0xffffffffu, ids_next, at & 31);
+        int block = at < 32 ? near : far;
+        const int stage = fetched % kStages;
+        const uint32_t dst = ring + stage * kStageBytes, bar = bar0 + 8 * stage;
+        const bool mine = (lane & 3) < n;
+        if (mine && (block < 0 || block >= a.cache.num_blocks)) {
+            // Reported; block 0 is read in its place (inside the cache).
+            atomicOr(a.error_flag, PKV_DEVICE_BAD_BLOCK);
+            block = 0;
+        }
+        if (lane == 0) pkv::mbar_arrive_expect_tx(bar, n * kBlockTraffic);
+        __syncwarp();
+        if (mine && lane < 16) {
+            const int j = lane & 3;
+            const int64_t tile = layer_tile + static_cast<int64_t>(block) * kHeads;
+            if (lane < 4) {
+                bulk_load(dst + j * kTile, a.cache.key_codes + (tile + warp) * kTile, kTile, bar, policy);
+            } else if (lane < 8) {
+                bulk_load(dst + kValueAt + j * kValuePitch, a.cache.value_codes + (tile + warp) * kTile, kTile, bar, policy);
+            } else if (lane < 12) {
+                bulk_load(dst + kScaleAt + j * 16, a.cache.key_scales + tile, 16, bar, policy);
+            } else {
+                bulk_load(dst + kScaleAt + (kChunk + j) * 16, a.cache.value_scales + tile, 16, bar, policy);
+            }
+        }
+        fetch += n;
+        ++fetched;
+    };
+    for (int s = 0; s < kStages; ++s) issue();
+
+    Rows rows = load_rows(a, lo, lane);
+    int row = advance_row(a, rows, lo, begin, lane);
+    bool beyond = row >= a.batch;  // prefix[batch] and total_blocks disagree
+    int row_first = 0;
+    uint32_t q[8];
+    if (!beyond) {
+        row_first = a.prefix[row];
+        load_query(a, row, warp * kGroup + g, t, q);
+    }
+
+    int consumed = 0;
+    bool failed = false;
+    int i = begin;
+    while (i < end && !beyond) {
+        const int row_last = __shfl_sync(0xffffffffu, rows.last, row - rows.base);
+        const int length = __shfl_sync(0xffffffffu, rows.length, row - rows.base);
+        const int seg_end = min(end, row_last);
+        // The next row's query is loaded while this row streams.
+        uint32_t q_next[8];
+        int row_next = row;
+        Rows rows_next = rows;
+        if (row_last < end) {
+            row_next = advance_row(a, rows_next, row + 1, row_last, lane);
+            beyond = row_next >= a.batch;
+            if (!beyond) load_query(a, row_next, warp * kGroup + g, t, q_next);
+        }
+
+        float m0 = kLowest, m1 = kLowest, l0 = 0.f, l1 = 0.f;
+        float o[4][4];
+#pragma unroll
+        for (int mt = 0; mt < 4; ++mt) o[mt][0] = o[mt][1] = o[mt][2] = o[mt][3] = 0.f;
+
+        while (i < seg_end) {
+            const int n = min(kChunk, seg_end - i);
+            const int stage = consumed % kStages;
+            const uint32_t src = ring + stage * kStageBytes;
+            if (!failed && !pkv::mbar_wait_bounded(bar0 + 8 * stage, (consumed / kStages) & 1, kWaitPolls)) failed = true;
+            failed = __any_sync(0xffffffffu, failed);
+            if (failed) break;
+            const int tokens = min(max(length - (i - row_first) * kSlots, 0), n * kSlots);  // valid ones of the chunk
+
+            // Scores: lane's rows are tokens 4 j + (g & 1) and 4 j + 2 + (g & 1) of block g / 2.
+            float s[4][4];
+            const uint32_t k_at = src + (g >> 1) * kTile + (g & 1) * kDim + 16 * t;
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                const uint4 a0 = lds128(k_at + 4 * j * kDim);
+                const uint4 a1 = lds128(k_at + (4 * j + 2) * kDim);
+                s[j][0] = s[j][1] = s[j][2] = s[j][3] = 0.f;
+#pragma unroll
+                for (int ks = 0; ks < 4; ++ks) {
+                    const uint32_t x = word(a0, ks), y = word(a1, ks);
+                    pkv::mma_f16_16816(s[j], pkv::fp8::decode2(x), pkv::fp8::decode2(y), pkv::fp8::decode2(x >> 16),
+                                       pkv::fp8::decode2(y >> 16), q[2 * ks], q[2 * ks + 1]);
+                }
+            }
+            const float key_scale = lds32(src + kScaleAt + (g >> 1) * 16 + warp * 4) * kScaleLog2;
+            const float value_scale = lds32(src + kScaleAt + (kChunk + (g >> 1)) * 16 + warp * 4);
+            const int ve = ((__float_as_int(value_scale) >> 23) & 0xff) - 127;
+            const float shift = static_cast<float>(ve);
+            const float unscale = pkv::fp8::exp2_int(-ve);
+            // Blocks past n hold an earlier chunk's bytes: their tokens are masked below.
+            const bool whole = tokens == kChunk * kSlots;
+            float top0 = kLowest, top1 = kLowest;
+            const int held = tokens - (g >> 1) * kSlots;  // valid tokens from block g / 2 on
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                s[j][0] = fmaf(s[j][0], key_scale, shift);
+                s[j][1] = fmaf(s[j][1], key_scale, shift);
+                s[j][2] = fmaf(s[j][2], key_scale, shift);
+                s[j][3] = fmaf(s[j][3], key_scale, shift);
+                if (!whole) {
+                    const int token = 4 * j + (g & 1);
+                    if (token >= held) s[j][0] = s[j][1] = -INFINITY;
+                    if (token + 2 >= held) s[j][2] = s[j][3] = -INFINITY;
+                }
+                top0 = fmaxf(top0, fmaxf(s[j][0], s[j][2]));
+                top1 = fmaxf(top1, fmaxf(s[j][1], s[j][3]));
+            }
+            top0 = fmaxf(m0, max8(top0));
+            top1 = fmaxf(m1, max8(top1));
+            const float alpha0 = pkv::exp2_approx(m0 - top0);
+            const float alpha1 = pkv::exp2_approx(m1 - top1);
+            m0 = top0;
+            m1 = top1;
+            const float base0 = kWeightShift - m0, base1 = kWeightShift - m1;
+            float add0 = 0.f, add1 = 0.f;
+            uint32_t p[4][2];
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                const float w0 = pkv::exp2_approx(s[j][0] + base0);
+                const float w1 = pkv::exp2_approx(s[j][1] + base1);
+                const float w2 = pkv::exp2_approx(s[j][2] + base0);
+                const float w3 = pkv::exp2_approx(s[j][3] + base1);
+                add0 += w0 + w2;
+                add1 += w1 + w3;
+                p[j][0] = pkv::movmatrix_trans(pkv::pack_half2(__floats2half2_rn(w0, w1)));
+                p[j][1] = pkv::movmatrix_trans(pkv::pack_half2(__floats2half2_rn(w2, w3)));
+            }
+            // A block whose tokens are all masked adds nothing, whatever its scale row holds.
+            if (!whole && held <= 0) add0 = add1 = 0.f;
+            else {
+                add0 *= unscale;
+                add1 *= unscale;
+            }
+            l0 = fmaf(l0, alpha0, add0);
+            l1 = fmaf(l1, alpha1, add1);
+#pragma unroll
+            for (int mt = 0; mt < 4; ++mt) {
+                o[mt][0] *= alpha0;
+                o[mt][1] *= alpha1;
+                o[mt][2] *= alpha0;
+                o[mt][3] *= alpha1;
+                uint4 v0 = lds128(src + kValueAt + t * kValuePitch + (16 * mt + g) * 16);
+                uint4 v1 = lds128(src + kValueAt + t * kValuePitch + (16 * mt + 8 + g) * 16);
+                if (!whole) {  // weight 0 times NaN is NaN
+                    const int keep = tokens - t * kSlots;
+                    v0 = keep_bytes(v0, keep);
+                    v1 = keep_bytes(v1, keep);
+                }
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    const uint32_t x = word(v0, j), y = word(v1, j);
+                    pkv::mma_f16_16816(o[mt], pkv::fp8::decode2(x), pkv::fp8::decode2(y), pkv::fp8::decode2(x >> 16),
+                                       pkv::fp8::decode2(y >> 16), p[j][0], p[j][1]);
+                }
+            }
+            // The stage is free: every lane has read it (the reads are ordered
+            // before the copies by the fence and the warp barrier).
+            pkv::fence_proxy_async_smem();
+            __syncwarp();
+            i += n;
+            ++consumed;
+            issue();
+        }
+        if (failed) break;
+
+        l0 = sum8(l0);
+        l1 = sum8(l1);
+        const int head0 = warp * kGroup + 2 * t;
+        if (row_first >= begin && row_last <= end) {
+            // Normalise and round; a row whose every token is masked is zeros.
+            __half *dst = a.out + row * a.out_stride;
+#pragma unroll
+            for (int mt = 0; mt < 4; ++mt) {
+                const int d = 16 * mt + g;
+                dst[head0 * kDim + d] = __float2half_rn(l0 == 0.f ? 0.f : __fdiv_rn(o[mt][0], l0));
+                dst[(head0 + 1) * kDim + d] = __float2half_rn(l1 == 0.f ? 0.f : __fdiv_rn(o[mt][1], l1));
+                dst[head0 * kDim + d + 8] = __float2half_rn(l0 == 0.f ? 0.f : __fdiv_rn(o[mt][2], l0));
+                dst[(head0 + 1) * kDim + d + 8] = __float2half_rn(l1 == 0.f ? 0.f : __fdiv_rn(o[mt][3], l1));
+            }
+        } else {
+            const int64_t index = static_cast<int64_t>(row) + blockIdx.x;
+            float *po = a.part_o + index * kQueryHeads * kDim;
+#pragma unroll
+            for (int mt = 0; mt < 4; ++mt) {
+                const int d = 16 * mt + g;
+                po[head0 * kDim + d] = o[mt][0];
+                po[(head0 + 1) * kDim + d] = o[mt][1];
+                po[head0 * kDim + d + 8] = o[mt][2];
+                po[(head0 + 1) * kDim + d + 8] = o[mt][3];
+            }
+            if (g == 0) {
+                *reinterpret_cast<float4 *>(a.part_ml + index * kQueryHeads * 2 + head0 * 2) = make_float4(m0, l0, m1, l1);
+            }
+        }
+        if (row_last < end) {
+            row = row_next;
+            rows = rows_next;
+            row_first = row_last;
+#pragma unroll
+            for (int x = 0; x < 8; ++x) q[x] = q_next[x];
+        }
+    }
+    if (failed || beyond) {
+        if (lane == 0) atomicOr(a.error_flag, failed ? PKV_DEVICE_WAIT_TIMEOUT : PKV_DEVICE_BAD_BLOCK);
+        // No copy may land after the CTA has left.
+        for (int c = consumed; c < fetched; ++c) {
+            pkv::mbar_wait_bounded(bar0 + 8 * (c % kStages), (c / kStages) & 1, kWaitPolls);
+        }
+    }
+}
+
+// Merge of the rows that several pieces hold: a warp per (row, two heads), 16
+// lanes a head and four dims a lane, pieces in order, four loaded at a time.
+constexpr int kMergeThreads = 256;
+
+__global__ void __launch_bounds__(kMergeThreads) fp8_merge_kernel(const __grid_constant__ Args a) {
+    const int pair = blockIdx.x * (kMergeThreads / 32) + (threadIdx.x >> 5);
+    const int lane = threadIdx.x & 31;
+    const int row = pair / (kQueryHeads / 2);
+    const int head = 2 * (pair % (kQueryHeads / 2)) + (lane >> 4);
+    const int dim = 4 * (lane & 15);
+    pkv::pdl_launch_dependents();
+    pkv::pdl_wait();
+    if (row >= a.batch) return;
+    const int first_block = a.prefix[row], last_block = a.prefix[row + 1] - 1;
+    if (last_block < first_block) return;
+    if (first_block < 0 || last_block >= a.total) {  // prefix and total_blocks disagree
+        if (lane == 0) atomicOr(a.error_flag, PKV_DEVICE_BAD_BLOCK);
+        return;
+    }
+    const int first = piece_of(first_block, a.total, a.grid), last = piece_of(last_block, a.total, a.grid);
+    if (first == last) return;
+    float M = kLowest, L = 0.f, A[4] = {0.f, 0.f, 0.f, 0.f};
+    constexpr int kBatch = 4;
+    for (int c0 = first; c0 <= last; c0 += kBatch) {
+        float2 ml[kBatch];
+        float4 v[kBatch];
+#pragma unroll
+        for (int j = 0; j < kBatch; ++j) {
+            if (c0 + j <= last) {
+                const int64_t index = (static_cast<int64_t>(row) + c0 + j) * kQueryHeads + head;
+                ml[j] = *reinterpret_cast<const float2 *>(a.part_ml + index * 2);
+                v[j] = *reinterpret_cast<const float4 *>(a.part_o + index * kDim + dim);
+            }
+        }
+#pragma unroll
+        for (int j = 0; j < kBatch; ++j) {
+            if (c0 + j <= last) {
+                const float top = fmaxf(M, ml[j].x);
+                const float x = pkv::exp2_approx(M - top), y = pkv::exp2_approx(ml[j].x - top);
+                M = top;
+                L = fmaf(L, x, ml[j].y * y);
+                A[0] = fmaf(A[0], x, v[j].x * y);
+                A[1] = fmaf(A[1], x, v[j].y * y);
+                A[2] = fmaf(A[2], x, v[j].z * y);
+                A[3] = fmaf(A[3], x, v[j].w * y);
+            }
+        }
+    }
+#pragma unroll
+    for (int d = 0; d < 4; ++d) A[d] = L == 0.f ? 0.f : __fdiv_rn(A[d], L);
+    __half2 *dst = reinterpret_cast<__half2 *>(a.out + row * a.out_stride + head * kDim + dim);
+    dst[0] = __floats2half2_rn(A[0], A[1]);
+    dst[1] = __floats2half2_rn(A[2], A[3]);
+}
+
+// The rotated queries of pkv_fp8_decode_layer, then the partials.
+constexpr int64_t kQueryRowBytes = kQueryHeads * kDim * 2;
+
+int64_t workspace_of(int64_t batch, int64_t grid) {
+    return batch * kQueryRowBytes + (grid > 1 ? (batch + grid) * kPartial * 4 : 0);
+}
+
+struct DeviceInfo {
+    int sms = 0;
+    int ctas_per_sm = 0;
+};
+
+int device_info(int device, DeviceInfo *info) {
+    static std::mutex mutex;
+    static std::unordered_map<int, DeviceInfo> cache;
+    std::lock_guard<std::mutex> lock(mutex);
+    auto it = cache.find(device);
+    if (it != cache.end()) {
+        *info = it->second;
+        return PKV_OK;
+    }
+    int previous = 0;
+    cudaGetDevice(&previous);
+    DeviceInfo d;
+    cudaError_t e = cudaSetDevice(device);
+    if (e == cudaSuccess) e = cudaDeviceGetAttribute(&d.sms, cudaDevAttrMultiProcessorCount, device);
+    if (e == cudaSuccess) e = cudaFuncSetAttribute(fp8_decode_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem);
+    if (e == cudaSuccess) {
+        e = cudaFuncSetAttribute(fp8_decode_kernel, cudaFuncAttributePreferredSharedMemoryCarveout,
+                                 cudaSharedmemCarveoutMaxShared);
+    }
+    if (e == cudaSuccess) {
+        // The merge keeps the split kernel's partition of L1 and shared memory.
+        e = cudaFuncSetAttribute(fp8_merge_kernel, cudaFuncAttributePreferredSharedMemoryCarveout,
+                                 cudaSharedmemCarveoutMaxShared);
+    }
+    if (e == cudaSuccess) e = cudaOccupancyMaxActiveBlocksPerMultiprocessor(&d.ctas_per_sm, fp8_decode_kernel, kThreads, kSmem);
+    cudaSetDevice(previous);
+    if (e != cudaSuccess) return pkv::fail(PKV_CUDA_ERROR, std::string("fp8 decode: ") + cudaGetErrorString(e));
+    if (d.ctas_per_sm < 1) d.ctas_per_sm = 1;
+    cache.emplace(device, d);
+    *info = d;
+    return PKV_OK;
+}
+
+}  // namespace
+
+extern "C" int pkv_fp8_decode_plan(int32_t device, int32_t batch, int32_t total_blocks, int32_t *out_grid,
+                                   int64_t *out_workspace_bytes) {
+    pkv::clear_error();
+    if (out_grid == nullptr || out_workspace_bytes == nullptr || batch < 1 || total_blocks < 0) {
+        return pkv::fail(PKV_VALUE_ERROR, "fp8 decode plan: needs a nonempty batch");
+    }
+    DeviceInfo info;
+    const int rc = device_info(device, &info);
+    if (rc) return rc;
+    // One piece per resident CTA; with few blocks one per chunk, so that no CTA is without work.
+    const int slots = info.sms * info.ctas_per_sm;
+    const int chunks = (total_blocks + kChunk - 1) / kChunk;
+    const int grid = chunks < 1 ? 1 : chunks < slots ? chunks : slots;
+    *out_grid = grid;
+    *out_workspace_bytes = workspace_of(batch, grid);
+    return PKV_OK;
+}
+
+namespace {
+
+// The attention of pkv_fp8_decode_attention, with the append of pkv_fp8_decode_layer before it when `key` is given.
+int decode(const pkv::fp8::Cache &cache, int32_t layer, const void *query, int64_t query_stride, const void *key,
+           const void *value, int64_t kv_stride, const void *rope_table, const int32_t *lengths, const int32_t *prefix,
+           const int32_t *flat, int32_t batch, int32_t total_blocks, int32_t grid, void *out, int64_t out_stride,
+           void *workspace, int64_t workspace_bytes, int32_t *error_flag, cudaStream_t stream) {
+    int rc = pkv::fp8::check_cache(cache.key_codes, cache.value_codes, cache.key_scales, cache.value_scales,
+                                   cache.layers, cache.num_blocks, layer, 1);
+    if (rc) return rc;
+    if (query == nullptr || lengths == nullptr || prefix == nullptr || (flat == nullptr && total_blocks > 0) ||
+        out == nullptr || error_flag == nullptr) {
+        return pkv::fail(PKV_VALUE_ERROR, "fp8 decode: null pointer argument");
+    }
+    if (batch < 1 || total_blocks < 0 || grid < 1 || (grid > 1 && grid > total_blocks)) {
+        return pkv::fail(PKV_VALUE_ERROR, "fp8 decode: batch, block count or grid out of range");
+    }
+    if ((reinterpret_cast<uintptr_t>(query) & 15) || (reinterpret_cast<uintptr_t>(out) & 15) || query_stride % 8 ||
+        out_stride % 8 || query_stride < kQueryHeads * kDim || out_stride < kQueryHeads * kDim) {
+        return pkv::fail(PKV_VALUE_ERROR, "fp8 decode: rows must be 16-byte aligned, 2048 or more values apart in multiples of 8");
+    }
+    const int64_t slots = static_cast<int64_t>(batch) + grid;
+    if (workspace == nullptr || (reinterpret_cast<uintptr_t>(workspace) & 15) ||
+        workspace_bytes < workspace_of(batch, grid)) {
+        return pkv::fail(PKV_VALUE_ERROR, "fp8 decode: the workspace is too small (see pkv_fp8_decode_plan)");
+    }
+    int device = 0;
+    cudaError_t e = cudaGetDevice(&device);
+    if (e != cudaSuccess) return pkv::fail(PKV_CUDA_ERROR, std::string("cudaGetDevice: ") + cudaGetErrorString(e));
+    DeviceInfo info;
+    if ((rc = device_info(device, &info))) return rc;
+    if (key != nullptr) {
+        rc = pkv::fp8::launch_decode_append(cache, layer, key, value, kv_stride, rope_table, query, query_stride, workspace,
+                                            lengths, prefix, flat, batch, total_blocks, error_flag, stream);
+        if (rc) return rc;
+        query = workspace;
+        query_stride = kQueryHeads * kDim;
+    }
+    float *const partials = reinterpret_cast<float *>(static_cast<uint8_t *>(workspace) + batch * kQueryRowBytes);
+    Args a;
+    a.cache = cache;
+    a.layer = layer;
+    a.query = static_cast<const __half *>(query);
+    a.query_stride = query_stride;
+    a.lengths = lengths;
+    a.prefix = prefix;
+    a.flat = flat;
+    a.batch = batch;
+    a.total = total_blocks;
+    a.grid = grid;
+    a.out = static_cast<__half *>(out);
+    a.out_stride = out_stride;
+    a.part_o = partials;
+    a.part_ml = partials + slots * kQueryHeads * kDim;
+    a.error_flag = error_flag;
+    cudaLaunchConfig_t config = {};
+    config.gridDim = dim3(grid);
+    config.blockDim = dim3(kThreads);
+    config.dynamicSmemBytes = kSmem;
+    config.stream = stream;
+    cudaLaunchAttribute attribute[1];
+    attribute[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attribute[0].val.programmaticStreamSerializationAllowed = 1;
+    config.attrs = attribute;
+    config.numAttrs = 1;
+    e = cudaLaunchKernelEx(&config, fp8_decode_kernel, a);
+    if (e == cudaSuccess && grid > 1) {
+        const int64_t warps = static_cast<int64_t>(batch) * (kQueryHeads / 2);
+        e = pkv::launch_pdl(fp8_merge_kernel, dim3(static_cast<unsigned>((warps * 32 + kMergeThreads - 1) / kMergeThreads)),
+                            dim3(kMergeThreads), config.stream, a);
+    }
+    if (e != cudaSuccess) return pkv::fail(PKV_CUDA_ERROR, std::string("fp8 decode launch failed: ") + cudaGetErrorString(e));
+    return PKV_OK;
+}
+
+pkv::fp8::Cache cache_of(const void *key_codes, const void *value_codes, const void *key_scales,
+                         const void *value_scales, int32_t layers, int32_t num_blocks) {
+    return {static_cast<uint8_t *>(const_cast<void *>(key_codes)), static_cast<uint8_t *>(const_cast<void *>(value_codes)),
+            static_cast<float *>(const_cast<void *>(key_scales)), static_cast<float *>(const_cast<void *>(value_scales)),
+            layers, num_blocks};
+}
+
+}  // namespace
+
+extern "C" int pkv_fp8_decode_attention(const void *key_codes, const void *value_codes, const void *key_scales,
+                                        const void *value_scales, int32_t layers, int32_t num_blocks, int32_t layer,
+                                        const void *query, int64_t query_stride, const int32_t *lengths,
+                                        const int32_t *prefix, const int32_t *flat, int32_t batch, int32_t total_blocks,
+                                        int32_t grid, void *out, int64_t out_stride, void *workspace,
+                                        int64_t workspace_bytes, int32_t *error_flag, void *stream) {
+    pkv::clear_error();
+    return decode(cache_of(key_codes, value_codes, key_scales, value_scales, layers, num_blocks), layer, query,
+                  query_stride, nullptr, nullptr, 0, nullptr, lengths, prefix, flat, batch, total_blocks, grid, out,
+                  out_stride, workspace, workspace_bytes, error_flag, static_cast<cudaStream_t>(stream));
+}
+
+extern "C" int pkv_fp8_decode_layer(void *key_codes, void *value_codes, void *key_scales, void *value_scales,
+                                    int32_t layers, int32_t num_blocks, int32_t layer, const void *query,
+                                    int64_t query_stride, const void *key, const void *value, int64_t kv_stride,
+                                    const void *rope_table, const int32_t *lengths, const int32_t *prefix,
+                                    const int32_t *flat, int32_t batch, int32_t total_blocks, int32_t grid, void *out,
+                                    int64_t out_stride, void *workspace, int64_t workspace_bytes, int32_t *error_flag,
+                                    void *stream) {
+    pkv::clear_error();
+    if (key == nullptr || value == nullptr || rope_table == nullptr) {
+        return pkv::fail(PKV_VALUE_ERROR, "fp8 decode layer: key, value and rope_table are required");
+    }
+    return decode(cache_of(key_codes, value_codes, key_scales, value_scales, layers, num_blocks), layer, query,
+                  query_stride, key, value, kv_stride, rope_table, lengths, prefix, flat, batch, total_blocks, grid, out,
+                  out_stride, workspace, workspace_bytes, error_flag, static_cast<cudaStream_t>(stream));
+}
