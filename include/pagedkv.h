@@ -457,10 +457,12 @@ int pkv_fp8_decode_plan(int32_t device, int32_t batch, int32_t total_blocks, int
 
 /* pkv_decode_attention over the 8-bit cache: query (rotated), lengths, prefix,
  * flat and out as there; a row without blocks (prefix[b + 1] == prefix[b]) or
- * without valid tokens gives zeros.  grid and workspace from
- * pkv_fp8_decode_plan for the same batch and total_blocks; the workspace (16-byte
- * aligned) needs no initialisation, and launches that share one must not overlap
- * on the GPU. */
+ * without valid tokens gives zeros.  The batch's blocks are prefix[batch], read
+ * on the device; total_blocks is the room of flat, which it must not exceed, so
+ * a captured launch serves any batch within it.  grid: the plan's for this
+ * batch and block count, or any other; workspace (16-byte aligned, of at least
+ * the plan's bytes for that grid: 4096 * batch + 8448 * (batch + grid)) needs no
+ * initialisation, and launches that share one must not overlap on the GPU. */
 int pkv_fp8_decode_attention(const void *key_codes, const void *value_codes, const void *key_scales,
                              const void *value_scales, int32_t layers, int32_t num_blocks, int32_t layer,
                              const void *query, int64_t query_stride, const int32_t *lengths, const int32_t *prefix,
@@ -472,7 +474,8 @@ int pkv_fp8_decode_attention(const void *key_codes, const void *value_codes, con
  * lengths[b] - 1, in the row's last block) has its K rotated and K and V written
  * as pkv_fp8_append_kv does, its query rotated, and attends to all lengths[b]
  * tokens.  query, key and value unrotated, rows query_stride / kv_stride apart.
- * No two rows may share a last block. */
+ * A row without blocks is left alone, its output too.  No two rows may share a
+ * last block. */
 int pkv_fp8_decode_layer(void *key_codes, void *value_codes, void *key_scales, void *value_scales, int32_t layers,
                          int32_t num_blocks, int32_t layer, const void *query, int64_t query_stride, const void *key,
                          const void *value, int64_t kv_stride, const void *rope_table, const int32_t *lengths,

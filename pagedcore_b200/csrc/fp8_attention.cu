@@ -88,8 +88,9 @@ struct Args {
     const int32_t *prefix;
     const int32_t *flat;
     int32_t batch;
-    int32_t total;
+    int32_t capacity;  // of flat; the batch's blocks are prefix[batch]
     int32_t grid;
+    int32_t clear;     // rows without blocks give zeros (else they are left alone)
     __half *out;
     int64_t out_stride;
     float *part_o;   // [batch + grid][32][64]
@@ -153,6 +154,21 @@ __device__ __forceinline__ uint4 keep_bytes(const uint4 &v, int keep) {
     return make_uint4(v.x & m[0], v.y & m[1], v.z & m[2], v.w & m[3]);
 }
 
+// The batch's block count, from the device so that a captured launch serves changing batches.
+__device__ __forceinline__ int total_blocks(const Args &a) {
+    const int total = a.prefix[a.batch];
+    if (total >= 0 && total <= a.capacity) return total;
+    atomicOr(a.error_flag, PKV_DEVICE_BAD_BLOCK);
+    return 0;
+}
+
+// Pieces of a list of `total` blocks: at most one per CTA and per chunk, so
+// none is empty.  (A captured launch has a CTA for every resident slot.)
+__host__ __device__ __forceinline__ int pieces_of(int total, int grid) {
+    const int chunks = (total + kChunk - 1) / kChunk;
+    return chunks < 1 ? 1 : chunks < grid ? chunks : grid;
+}
+
 // Rows of the block list: where each ends.  32 rows from `base` in registers.
 struct Rows {
     int base, last, length;
@@ -196,14 +212,16 @@ __global__ void __launch_bounds__(kThreads, 2) fp8_decode_kernel(const __grid_co
     pkv::pdl_launch_dependents();
 
     // Rows without blocks: zeros.
-    for (int b = blockIdx.x * kThreads + threadIdx.x; b < a.batch; b += a.grid * kThreads) {
+    for (int b = blockIdx.x * kThreads + threadIdx.x; a.clear && b < a.batch; b += a.grid * kThreads) {
         if (a.prefix[b + 1] <= a.prefix[b]) {
             for (int i = 0; i < kQueryHeads * kDim; ++i) a.out[b * a.out_stride + i] = __float2half_rn(0.f);
         }
     }
-    const int begin = piece_begin(blockIdx.x, a.total, a.grid);
-    const int end = piece_begin(blockIdx.x + 1, a.total, a.grid);
-    if (begin >= end) return;
+    const int total = total_blocks(a);
+    const int pieces = pieces_of(total, a.grid);
+    if (total == 0 || static_cast<int>(blockIdx.x) >= pieces) return;
+    const int begin = piece_begin(blockIdx.x, total, pieces);
+    const int end = piece_begin(blockIdx.x + 1, total, pieces);
 
     const uint64_t policy = pkv::l2_policy_evict_first();
     // First row with blocks past `begin`, by a 32-way search over prefix[1 ..].
@@ -277,7 +295,7 @@ __global__ void __launch_bounds__(kThreads, 2) fp8_decode_kernel(const __grid_co
 
     Rows rows = load_rows(a, lo, lane);
     int row = advance_row(a, rows, lo, begin, lane);
-    bool beyond = row >= a.batch;  // prefix[batch] and total_blocks disagree
+    bool beyond = row >= a.batch;  // prefix does not grow from row to row
     int row_first = 0;
     uint32_t q[8];
     if (!beyond) {
@@ -472,12 +490,10 @@ __global__ void __launch_bounds__(kMergeThreads) fp8_merge_kernel(const __grid_c
     pkv::pdl_wait();
     if (row >= a.batch) return;
     const int first_block = a.prefix[row], last_block = a.prefix[row + 1] - 1;
-    if (last_block < first_block) return;
-    if (first_block < 0 || last_block >= a.total) {  // prefix and total_blocks disagree
-        if (lane == 0) atomicOr(a.error_flag, PKV_DEVICE_BAD_BLOCK);
-        return;
-    }
-    const int first = piece_of(first_block, a.total, a.grid), last = piece_of(last_block, a.total, a.grid);
+    const int total = total_blocks(a);
+    if (last_block < first_block || first_block < 0 || last_block >= total) return;
+    const int pieces = pieces_of(total, a.grid);
+    const int first = piece_of(first_block, total, pieces), last = piece_of(last_block, total, pieces);
     if (first == last) return;
     float M = kLowest, L = 0.f, A[4] = {0.f, 0.f, 0.f, 0.f};
     constexpr int kBatch = 4;
@@ -569,10 +585,7 @@ extern "C" int pkv_fp8_decode_plan(int32_t device, int32_t batch, int32_t total_
     DeviceInfo info;
     const int rc = device_info(device, &info);
     if (rc) return rc;
-    // One piece per resident CTA; with few blocks one per chunk, so that no CTA is without work.
-    const int slots = info.sms * info.ctas_per_sm;
-    const int chunks = (total_blocks + kChunk - 1) / kChunk;
-    const int grid = chunks < 1 ? 1 : chunks < slots ? chunks : slots;
+    const int grid = pieces_of(total_blocks, info.sms * info.ctas_per_sm);  // at most one CTA per resident slot
     *out_grid = grid;
     *out_workspace_bytes = workspace_of(batch, grid);
     return PKV_OK;
@@ -592,7 +605,7 @@ int decode(const pkv::fp8::Cache &cache, int32_t layer, const void *query, int64
         out == nullptr || error_flag == nullptr) {
         return pkv::fail(PKV_VALUE_ERROR, "fp8 decode: null pointer argument");
     }
-    if (batch < 1 || total_blocks < 0 || grid < 1 || (grid > 1 && grid > total_blocks)) {
+    if (batch < 1 || total_blocks < 0 || grid < 1) {
         return pkv::fail(PKV_VALUE_ERROR, "fp8 decode: batch, block count or grid out of range");
     }
     if ((reinterpret_cast<uintptr_t>(query) & 15) || (reinterpret_cast<uintptr_t>(out) & 15) || query_stride % 8 ||
@@ -626,8 +639,9 @@ int decode(const pkv::fp8::Cache &cache, int32_t layer, const void *query, int64
     a.prefix = prefix;
     a.flat = flat;
     a.batch = batch;
-    a.total = total_blocks;
+    a.capacity = total_blocks;
     a.grid = grid;
+    a.clear = key == nullptr;
     a.out = static_cast<__half *>(out);
     a.out_stride = out_stride;
     a.part_o = partials;

@@ -232,6 +232,7 @@ __global__ void __launch_bounds__(kThreads) fp8_append_kernel(const __grid_const
     const int token = blockIdx.x;
     const int layer = blockIdx.y;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    if (a.lengths != nullptr && a.prefix[token + 1] <= a.prefix[token]) return;  // a row without blocks
 
     if (a.query_in != nullptr) {
         // A warp rotates four query heads: eight lanes a head, of which two hold

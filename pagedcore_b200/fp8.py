@@ -423,6 +423,11 @@ def decode_plan(device_index: int, batch: int, total_blocks: int) -> tuple[int, 
     return grid.value, workspace.value
 
 
+def decode_workspace_bytes(batch: int, grid: int) -> int:
+    """Workspace of a decode launch with ``grid`` pieces (rotated queries, then split partials)."""
+    return batch * _QUERY_HEADS * _HEAD_DIM * 2 + (batch + grid) * _QUERY_HEADS * (_HEAD_DIM + 2) * 4
+
+
 def _attention_rows(name: str, tensor: Tensor, shape: tuple[int, ...], device: torch.device) -> None:
     if tensor.shape != shape or tensor.dtype != torch.float16 or tensor.device != device:
         raise ValueError(f"{name} must be FP16 {list(shape)} on {device}")

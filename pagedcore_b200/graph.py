@@ -31,7 +31,7 @@ import torch
 from torch import Tensor
 
 from pagedcore_b200 import kernels
-from pagedcore_b200._lib import DECODE_EARLY_KV, check, lib
+from pagedcore_b200._lib import DECODE_EARLY_KV
 from pagedcore_b200.engine_types import RequestId
 from pagedcore_b200.kv_cache import KVAllocator
 
@@ -58,18 +58,6 @@ def _capturing(graph: torch.cuda.CUDAGraph, stream: torch.cuda.Stream) -> Iterat
     finally:
         if enabled:
             gc.enable()
-
-
-def _replay_args(allocator: KVAllocator, rows: int, grid: int) -> tuple:
-    """Fixed pkv_decode_layer arguments of the staged (padded) step, minus layer, I/O and stream.
-
-    With piece tables the kernels take the block count only as a bound and
-    ignore the arithmetic partition, so the upload's room and constants stand
-    in for them: the arguments repeat from step to step and key the graphs.
-    """
-    staged = allocator._staged
-    fixed = allocator._decode_layer_args(staged.staged_batch, rows, grid)
-    return (*fixed[:8], staged.flat_capacity, grid, 1, grid, 1, *fixed[13:16])
 
 
 class DecodeStepGraph:
@@ -116,23 +104,16 @@ class DecodeStepGraph:
 
     def _capture(self, args: tuple, query: Tensor, key: Tensor, value: Tensor, out: Tensor) -> torch.cuda.CUDAGraph:
         allocator = self.allocator
-        (pool, num_blocks, rope, lengths, prefix, flat, pieces, row_pieces, bound, grid, per_cta, big, tail, ws,
-         ws_bytes, err) = args
         side = torch.cuda.Stream(allocator.pool.device)
         side.wait_stream(allocator._stream)
         graph = torch.cuda.CUDAGraph()
         with _capturing(graph, side):
             for layer in range(_LAYERS):
-                q, k, v, o = query[layer], key[layer], value[layer], out[layer]
-                check(
-                    lib.pkv_decode_layer(
-                        pool, num_blocks, layer, q.data_ptr(), q.stride(0), k.data_ptr(), v.data_ptr(), k.stride(0),
-                        rope, lengths, prefix, flat, pieces, row_pieces, self.rows, bound, grid, per_cta, big, tail,
-                        # Layers after the first follow this graph's own combine, which
-                        # writes no pool data: they may start streaming early.
-                        o.data_ptr(), o.stride(0), ws, ws_bytes, err, DECODE_EARLY_KV if layer else 0,
-                        side.cuda_stream,
-                    )
+                allocator._launch_decode_layer(
+                    layer, query[layer], key[layer], value[layer], out[layer], self.rows, args,
+                    # Layers after the first follow this graph's own combine, which
+                    # writes no pool data: they may start streaming early.
+                    DECODE_EARLY_KV if layer else 0, side.cuda_stream,
                 )
         allocator._stream.wait_stream(side)
         self.captures += 1
@@ -150,7 +131,7 @@ class DecodeStepGraph:
         self._check(query, key, value, out)
         with allocator.append_decode(requests, layout=(self.rows, self.grid)):
             staged = allocator._staged
-            args = _replay_args(allocator, self.rows, self.grid)
+            args = allocator._replay_args(self.rows, self.grid)
             cache_key = (args, query.data_ptr(), key.data_ptr(), value.data_ptr(), out.data_ptr())
             graph = self._graphs.get(cache_key)
             if graph is None:
@@ -199,8 +180,6 @@ class DecoderStepGraph:
 
     def _capture(self, args: tuple) -> tuple[torch.cuda.CUDAGraph, Tensor]:
         allocator = self.allocator
-        (pool, num_blocks, rope, lengths, prefix, flat, pieces, row_pieces, bound, grid, per_cta, big, tail, ws,
-         ws_bytes, err) = args
         side = torch.cuda.Stream(allocator.pool.device)
         side.wait_stream(allocator._stream)
         out = self.attention
@@ -209,13 +188,7 @@ class DecoderStepGraph:
             # The previous kernel is a GEMM of this step, not a decode combine:
             # no early K/V (it would only save the launch, which a GEMM
             # predecessor does not overlap).
-            check(
-                lib.pkv_decode_layer(
-                    pool, num_blocks, layer, q.data_ptr(), q.stride(0), k.data_ptr(), v.data_ptr(), k.stride(0),
-                    rope, lengths, prefix, flat, pieces, row_pieces, self.rows, bound, grid, per_cta, big, tail,
-                    out.data_ptr(), out.stride(0), ws, ws_bytes, err, 0, side.cuda_stream,
-                )
-            )
+            allocator._launch_decode_layer(layer, q, k, v, out, self.rows, args, 0, side.cuda_stream)
             return out
 
         # One forward outside the capture first, with an attention stand-in
@@ -245,7 +218,7 @@ class DecoderStepGraph:
             raise ValueError("input_ids must be int64 [batch, 1] matching request IDs on the pool device")
         with allocator.append_decode(requests, layout=(self.rows, self.grid)):
             staged = allocator._staged
-            args = _replay_args(allocator, self.rows, self.grid)
+            args = allocator._replay_args(self.rows, self.grid)
             entry = self._graphs.get(args)
             if entry is None:
                 if len(self._graphs) >= self.max_graphs:

@@ -205,10 +205,9 @@ class PrefillAppend:
             rotated = query_in
         else:
             rotated = torch.empty((1, self.tokens, 32, 64), dtype=torch.float16, device=allocator._pool.device)
-        kernels.append_kv(
-            allocator._pool, key.reshape(1, self.tokens, 4, 64), value.reshape(1, self.tokens, 4, 64), self.slots,
-            layer_begin=layer, error_flag=allocator._error, positions=self.positions, rope_table=allocator._rope,
-            query_in=query_in, query_out=rotated,
+        allocator._write(
+            key.reshape(1, self.tokens, 4, 64), value.reshape(1, self.tokens, 4, 64), self.slots, layer,
+            positions=self.positions, query_in=query_in, query_out=rotated,
         )
         return rotated[0]
 
@@ -225,7 +224,7 @@ class PrefillAppend:
             raise ValueError("layer_index must identify one of the 22 decoder layers")
         if out is None:
             out = torch.empty(query.shape, dtype=torch.float16, device=allocator._pool.device)
-        return kernels.prefill_attention(allocator._pool, layer, query, self.blocks, self.start, out, allocator._error)
+        return allocator._attend_prompt(layer, query, self.blocks, self.start, out)
 
     @torch.inference_mode()
     def attend_split(self, layer: int, query: Tensor, out: Tensor | None = None) -> Tensor:
@@ -295,10 +294,14 @@ class KVAllocator:
             raise ValueError("KV pool must be contiguous FP16 [22, 2, blocks, 16, 4, 64] storage")
         if pool.device.type != "cuda":
             raise ValueError("KV pool must be CUDA storage: the B200 KV path has no CPU implementation")
+        self._setup(pool, pool.shape[2], validation, balance)
+
+    def _setup(self, pool, num_blocks: int, validation: str, balance: str) -> None:
+        """State over ``pool``, checked storage of ``num_blocks`` blocks on a CUDA device."""
         self._pool = pool
         self._worker = current_thread()
         self._stream = torch.cuda.current_stream(pool.device)
-        self._ledger = BlockLedger(pool.shape[2], validation)
+        self._ledger = BlockLedger(num_blocks, validation)
         self._handles: dict[RequestId, int] = {}
         self._next_handle = 1
         self._staged: _Staged | None = None
@@ -318,6 +321,45 @@ class KVAllocator:
         # Grid of every decode launch since the slot counters were last zeroed
         # (None: launches outside a measured step, or of mixed grids).
         self._window_grid: int | None = None
+
+    # -- the pool's kernels (an allocator over another storage replaces these) ---
+    def _write(
+        self, key: Tensor, value: Tensor, slots: Tensor, layer_begin: int, *, positions: Tensor | None = None,
+        query_in: Tensor | None = None, query_out: Tensor | None = None,
+    ) -> None:
+        """Scatter K/V [layers, tokens, 4, 64] at ``slots``; with ``positions`` K (and ``query_in``) rotated."""
+        kernels.append_kv(
+            self._pool, key, value, slots, layer_begin=layer_begin, error_flag=self._error, positions=positions,
+            rope_table=None if positions is None else self._rope, query_in=query_in, query_out=query_out,
+        )
+
+    def _attend_prompt(self, layer: int, query: Tensor, blocks: Tensor, start: int, out: Tensor) -> Tensor:
+        return kernels.prefill_attention(self._pool, layer, query, blocks, start, out, self._error)
+
+    def _launch_decode_layer(
+        self, layer: int, query: Tensor, key: Tensor, value: Tensor, out: Tensor, rows: int, fixed: tuple,
+        flags: int, stream: int,
+    ) -> None:
+        """The fused decode layer over ``rows`` rows, ``fixed`` from ``_decode_layer_args`` or ``_replay_args``."""
+        (pool, num_blocks, rope, lengths, prefix, flat, pieces, row_pieces, total, grid, per_cta, big, tail, ws,
+         ws_bytes, err) = fixed
+        check(
+            lib.pkv_decode_layer(
+                pool, num_blocks, layer, query.data_ptr(), query.stride(0), key.data_ptr(), value.data_ptr(),
+                key.stride(0), rope, lengths, prefix, flat, pieces, row_pieces, rows, total, grid, per_cta, big, tail,
+                out.data_ptr(), out.stride(0), ws, ws_bytes, err, flags, stream,
+            )
+        )
+
+    def _replay_args(self, rows: int, grid: int) -> tuple:
+        """Fixed launch arguments of the staged (padded) step, the same for every batch it is replayed on.
+
+        With piece tables the kernels take the block count only as a bound and
+        ignore the arithmetic partition, so the upload's room and constants stand
+        in for them: the arguments repeat from step to step and key the graphs.
+        """
+        fixed = self._decode_layer_args(self._staged.staged_batch, rows, grid)
+        return (*fixed[:8], self._staged.flat_capacity, grid, 1, grid, 1, *fixed[13:16])
 
     # -- plumbing -------------------------------------------------------------
     @property
@@ -496,13 +538,10 @@ class KVAllocator:
         if rotate:
             positions = np.arange(start, start + tokens, dtype=np.int32)
             meta = self._upload_i32(slots, positions)
-            kernels.append_kv(
-                self._pool, key, value, meta[:tokens], layer_begin=0, error_flag=self._error,
-                positions=meta[tokens:], rope_table=self._rope,
-            )
+            self._write(key, value, meta[:tokens], 0, positions=meta[tokens:])
         else:
             meta = self._upload_i32(slots)
-            kernels.append_kv(self._pool, key, value, meta, layer_begin=0, error_flag=self._error)
+            self._write(key, value, meta, 0)
         # Publish valid positions only after both K and V writes were issued.
         self._ledger.append_commit(handle, tokens)
 
@@ -554,13 +593,10 @@ class KVAllocator:
                 [np.arange(start, start + count, dtype=np.int32) for start, count in zip(starts, counts, strict=True)]
             )
             meta = self._upload_i32(slots, positions)
-            kernels.append_kv(
-                self._pool, key, value, meta[:total], layer_begin=0, error_flag=self._error,
-                positions=meta[total:], rope_table=self._rope,
-            )
+            self._write(key, value, meta[:total], 0, positions=meta[total:])
         else:
             meta = self._upload_i32(slots)
-            kernels.append_kv(self._pool, key, value, meta, layer_begin=0, error_flag=self._error)
+            self._write(key, value, meta, 0)
         # Publish every request only after the one launch was issued.
         self._ledger.append_commit_many(handles, counts)
 
@@ -671,10 +707,7 @@ class KVAllocator:
         ):
             raise ValueError("K and V must share FP16 [4, 64] on the pool device")
         row = staged.rows[request_id]
-        kernels.append_kv(
-            self._pool, key[None, None], value[None, None], staged.slots[row : row + 1],
-            layer_begin=layer, error_flag=self._error,
-        )
+        self._write(key[None, None], value[None, None], staged.slots[row : row + 1], layer)
         self._ledger.decode_mark(handle, layer)
 
     @torch.inference_mode()
@@ -709,17 +742,9 @@ class KVAllocator:
             if query.shape != (count, 32, 64) or query.dtype != torch.float16:
                 raise ValueError("query must be FP16 [batch, 32, 64]")
             query_out = torch.empty((1, count, 32, 64), dtype=torch.float16, device=self._pool.device)
-        kernels.append_kv(
-            self._pool,
-            key[None],
-            value[None],
-            staged.slots,
-            layer_begin=layer,
-            error_flag=self._error,
-            positions=staged.positions if rotate else None,
-            rope_table=self._rope if rotate else None,
-            query_in=None if query is None else query[None],
-            query_out=query_out,
+        self._write(
+            key[None], value[None], staged.slots, layer, positions=staged.positions if rotate else None,
+            query_in=None if query is None else query[None], query_out=query_out,
         )
         self._ledger.decode_mark(-1, layer)
         staged.written = layer + 1
@@ -767,15 +792,7 @@ class KVAllocator:
         if fixed is None:
             batch = self.staged_decode_batch()
             fixed = staged.launch_args = self._decode_layer_args(batch, count, batch.plan.grid)
-        pool_ptr, num_blocks, rope, lengths, prefix, flat, pieces, row_pieces, total, grid, per_cta, big, tail, ws, ws_bytes, \
-            err, stream = fixed
-        check(
-            lib.pkv_decode_layer(
-                pool_ptr, num_blocks, layer, query.data_ptr(), query.stride(0), key.data_ptr(), value.data_ptr(),
-                key.stride(0), rope, lengths, prefix, flat, pieces, row_pieces, count, total, grid, per_cta, big, tail,
-                out.data_ptr(), out.stride(0), ws, ws_bytes, err, 0, stream,
-            )
-        )
+        self._launch_decode_layer(layer, query, key, value, out, count, fixed, 0, self._stream.cuda_stream)
         self._ledger.decode_mark(-1, layer)
         staged.written = layer + 1
         return out
@@ -790,7 +807,7 @@ class KVAllocator:
             batch.total_blocks,
             grid, batch.plan.blocks_per_cta, *batch.plan.pieces(),
             0 if workspace is None else workspace.data_ptr(),
-            0 if workspace is None else workspace.numel() * 4, self._error.data_ptr(), self._stream.cuda_stream,
+            0 if workspace is None else workspace.numel() * 4, self._error.data_ptr(),
         )
 
     def staged_decode_batch(self) -> DecodeBatch:

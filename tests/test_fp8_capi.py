@@ -75,7 +75,7 @@ def test_attention() -> None:
 
     refused(lib.pkv_fp8_decode_attention, *decode(batch=0), message=b"out of range")
     refused(lib.pkv_fp8_decode_attention, *decode(total=-1), message=b"out of range")
-    refused(lib.pkv_fp8_decode_attention, *decode(grid=5), message=b"out of range")
+    refused(lib.pkv_fp8_decode_attention, *decode(grid=0), message=b"out of range")
     refused(lib.pkv_fp8_decode_attention, *decode(stride=2040), message=b"2048 or more")
     refused(lib.pkv_fp8_decode_attention, *decode(workspace=None), message=b"workspace")
     refused(lib.pkv_fp8_decode_attention, *decode(grid=4, size=4096), message=b"workspace")

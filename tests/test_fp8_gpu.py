@@ -440,6 +440,20 @@ def test_decode_attention(lengths) -> None:
     assert torch.equal(out, again)
 
 
+def test_decode_attention_does_not_depend_on_the_room_of_the_block_list() -> None:
+    """A launch sized for a larger batch (a captured one) cuts the list as one sized for this batch does."""
+    case = CacheCase(16, [300, 5, 64])
+    lengths, prefix, flat, total = case.batch()
+    query = randn(3, 3, 32, 64).half()
+    expected = fp8.decode_attention(case.cache, LAYER, query, lengths, prefix, flat, total, case.flag)
+    room = torch.cat((flat, torch.full((5000,), -7, dtype=torch.int32, device=case.device)))
+    out = fp8.decode_attention(case.cache, LAYER, query, lengths, prefix, room, room.numel(), case.flag)
+    assert int(case.flag.item()) == 0
+    assert torch.equal(out, expected)
+    fp8.decode_attention(case.cache, LAYER, query, lengths, prefix, flat, total - 1, case.flag)  # too little room
+    assert int(case.flag.item()) == 1
+
+
 def test_decode_attention_with_blocks_of_very_different_scale() -> None:
     """V's scale goes into the weights' exponent: tiny and huge blocks in one row lose nothing."""
     case = CacheCase(12, [300, 90], spread=4.0)
