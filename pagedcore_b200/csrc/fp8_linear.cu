@@ -48,13 +48,14 @@ constexpr int kWBytes = kTileRows * kKBlock;
 constexpr uint32_t kWaitPolls = 1u << 24;
 constexpr int kMaxCluster = 8;
 
+// The kernel for few rows: NT rows of x, at most 64.
 template <int NT>
 struct Shape {
-    static constexpr int kEpilogueWarps = NT >= 128 ? 8 : 4;
+    static constexpr int kEpilogueWarps = 4;
     static constexpr int kThreads = (kEpilogueWarps + 2) * 32;
-    static constexpr int kColumns = NT / (kEpilogueWarps / 4);  // of one epilogue warp
+    static constexpr int kColumns = NT;  // of one epilogue warp
     static constexpr int kStageBytes = kWBytes + NT * kKBlock;
-    static constexpr int kStages = NT >= 256 ? 4 : NT >= 128 ? 3 : 4;
+    static constexpr int kStages = 4;
     static constexpr int kTmemColumns = 2 * NT < 32 ? 32 : 2 * NT;
     // The ring, reused at the end for [NT][128] FP32 sums.
     static constexpr int kRing = kStages * kStageBytes;
@@ -72,7 +73,10 @@ struct LinearArgs {
     int32_t k_blocks;
     int32_t splits;   // CTAs of a cluster
     int32_t n_tiles;
-    int32_t vector_out;  // rows of out take 8-byte stores
+    int32_t m_tiles;     // many rows: tiles of 128 rows of x
+    int32_t tiles;       // many rows: all
+    int32_t w_blocks;    // ceil(n / 128)
+    int32_t vector_out;  // rows of out take 16-byte stores
     int32_t *error_flag;
 };
 
@@ -118,6 +122,22 @@ __device__ __forceinline__ float4 ld_cluster_f4(uint32_t addr) {
     return v;
 }
 
+// Four outputs of row m at column n (a multiple of 4), rounded to FP16.
+__device__ __forceinline__ void store4(const LinearArgs &a, int m, int n, const float4 &v) {
+    __half *dst = a.out + static_cast<int64_t>(m) * a.out_stride + n;
+    if (a.vector_out && n + 4 <= a.n) {
+        uint2 h;
+        h.x = pkv::pack_half2(__floats2half2_rn(v.x, v.y));
+        h.y = pkv::pack_half2(__floats2half2_rn(v.z, v.w));
+        *reinterpret_cast<uint2 *>(dst) = h;
+    } else {
+        if (n < a.n) dst[0] = __float2half_rn(v.x);
+        if (n + 1 < a.n) dst[1] = __float2half_rn(v.y);
+        if (n + 2 < a.n) dst[2] = __float2half_rn(v.z);
+        if (n + 3 < a.n) dst[3] = __float2half_rn(v.w);
+    }
+}
+
 template <int NT>
 __global__ void __launch_bounds__(Shape<NT>::kThreads, 1)
     fp8_linear_kernel(const __grid_constant__ CUtensorMap w_map, const __grid_constant__ CUtensorMap x_map,
@@ -131,10 +151,9 @@ __global__ void __launch_bounds__(Shape<NT>::kThreads, 1)
     const uint32_t raw = pkv::smem_addr(dyn_smem);
     const uint32_t base = (raw + 1023u) & ~1023u;
     const int split = static_cast<int>(blockIdx.x) % a.splits;  // rank in the cluster
-    const int tile = static_cast<int>(blockIdx.x) / a.splits;
-    const int n_tile = tile % a.n_tiles;
+    const int n_tile = static_cast<int>(blockIdx.x) / a.splits;
     const int n0 = n_tile * kTileRows;
-    const int m0 = tile / a.n_tiles * NT;
+    constexpr int m0 = 0;  // all rows are one tile
     const int kb_begin = static_cast<int>(static_cast<int64_t>(split) * a.k_blocks / a.splits);
     const int kb_end = static_cast<int>(static_cast<int64_t>(split + 1) * a.k_blocks / a.splits);
     const int count = kb_end - kb_begin;
@@ -226,22 +245,27 @@ __global__ void __launch_bounds__(Shape<NT>::kThreads, 1)
     } else {
         pkv::pdl_wait();
         constexpr int kEpilogueThreads = S::kEpilogueWarps * 32;
-        // Thread c < NT loads column c's scale, two K blocks ahead.
+        // Thread c < NT loads column c's scale two K blocks ahead; the two factors
+        // stay apart until they are used, so that nothing waits for a load.
         const int column = m0 + static_cast<int>(threadIdx.x);
         const bool loads = threadIdx.x < NT;
         const bool inside = loads && column < a.rows;
         const float *sx = a.x_scales + static_cast<int64_t>(inside ? column : 0) * a.k_blocks + kb_begin;
         const float *sw = a.w_scales + static_cast<int64_t>(n_tile) * a.k_blocks + kb_begin;
-        float f0 = inside ? sx[0] * sw[0] : 0.f;
-        float f1 = inside && count > 1 ? sx[1] * sw[1] : 0.f;
+        float x0 = inside ? sx[0] : 0.f, w0 = sw[0];
+        float x1 = inside && count > 1 ? sx[1] : 0.f, w1 = count > 1 ? sw[1] : 0.f;
         const int first = (warp >> 2) * S::kColumns;  // of this warp's columns
         const uint32_t lanes = static_cast<uint32_t>((warp & 3) * 32) << 16;
         bool ok = true;
         for (int i = 0; i < count; ++i) {
             const int buf = i & 1;
-            if (loads) factors[buf][threadIdx.x] = f0;
-            f0 = f1;
-            f1 = inside && i + 2 < count ? sx[i + 2] * sw[i + 2] : 0.f;
+            if (loads) factors[buf][threadIdx.x] = x0 * w0;
+            x0 = x1;
+            w0 = w1;
+            if (i + 2 < count) {
+                if (inside) x1 = sx[i + 2];
+                w1 = sw[i + 2];
+            }
             asm volatile("bar.sync 1, %0;" ::"n"(kEpilogueThreads) : "memory");
             if (ok) ok = wait_bounded(pkv::smem_addr(&tmem_full[buf]), (i >> 1) & 1, a.error_flag);
             ok = __all_sync(0xffffffffu, ok);
@@ -302,23 +326,290 @@ __global__ void __launch_bounds__(Shape<NT>::kThreads, 1)
                 v.x += u.x, v.y += u.y, v.z += u.z, v.w += u.w;
             }
         }
-        const int n = n0 + 4 * lane;
-        __half *dst = a.out + static_cast<int64_t>(m0 + c) * a.out_stride + n;
-        if (a.vector_out && n + 4 <= a.n) {
-            uint2 h;
-            h.x = pkv::pack_half2(__floats2half2_rn(v.x, v.y));
-            h.y = pkv::pack_half2(__floats2half2_rn(v.z, v.w));
-            *reinterpret_cast<uint2 *>(dst) = h;
-        } else {
-            if (n < a.n) dst[0] = __float2half_rn(v.x);
-            if (n + 1 < a.n) dst[1] = __float2half_rn(v.y);
-            if (n + 2 < a.n) dst[2] = __float2half_rn(v.z);
-            if (n + 3 < a.n) dst[3] = __float2half_rn(v.w);
-        }
+        store4(a, m0 + c, n0 + 4 * lane, v);
     }
     if (a.splits > 1) {  // no CTA leaves while another reads its sums
         cluster_arrive();
         cluster_wait();
+    }
+    if (warp == kMma) {
+        pkv::tc::fence_after_sync();
+        pkv::tc::tmem_dealloc(tmem, S::kTmemColumns);
+    }
+}
+
+// ---------------------------------------------------------------------------
+// Many rows: the rows of x are the MMA's M side (128 a tile), N weight rows its N
+// side.  Lane = row of x, so a thread's scale factor for a K block is one number,
+// sx[row] * sw[block of its 64 columns]: no factor goes through shared memory, and
+// the scaled sum is one packed FMA for two columns.  Each epilogue warp holds 64
+// columns in registers (N / 16 warps, four to twelve), enough warps to cover the
+// latency of the TMEM reads.  With one split the CTAs are persistent: the loads and
+// MMAs of the next tile run while the last one is rounded and stored.
+// ---------------------------------------------------------------------------
+template <int N>
+struct RowsShape {
+    static constexpr int kEpilogueWarps = N / 16;
+    static constexpr int kThreads = (kEpilogueWarps + 3) * 32;
+    static constexpr int kXBytes = kTileRows * kKBlock;
+    static constexpr int kStageBytes = kXBytes + N * kKBlock;
+    static constexpr int kStages = N == 192 ? 5 : N == 128 ? 6 : 8;
+    static constexpr int kBufferColumns = N > 128 ? 256 : N;
+    static constexpr int kTmemColumns = 2 * kBufferColumns;
+    static constexpr int kRing = kStages * kStageBytes;
+    static constexpr int kPitch = N + 4;  // floats between the rows of a cluster's sums (in the ring)
+    static_assert(kTileRows * kPitch * 4 <= kRing, "the sums fit the ring");
+    static constexpr int kStoreBytes = 32 * 64;  // a warp's staging: 32 rows of 32 FP16 values
+    static constexpr int kSmem = kRing + kEpilogueWarps * kStoreBytes + 1024;
+};
+
+// v[j] = p[at + j] for the indexes below `count`.
+__device__ __forceinline__ void load_group(const float *p, int at, int count, float (&v)[4]) {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) v[j] = at + j < count ? __ldg(p + at + j) : 0.f;
+}
+
+// acc[j] += (d[2 j], d[2 j + 1]) * f for 32 columns.
+__device__ __forceinline__ void add_scaled(uint64_t *acc, const uint32_t (&d)[32], uint64_t f) {
+#pragma unroll
+    for (int j = 0; j < 16; ++j) {
+        acc[j] = pkv::fma_f32x2(pkv::f32x2(__uint_as_float(d[2 * j]), __uint_as_float(d[2 * j + 1])), f, acc[j]);
+    }
+}
+
+template <int N>
+__global__ void __launch_bounds__(RowsShape<N>::kThreads, 1)
+    fp8_linear_rows_kernel(const __grid_constant__ CUtensorMap w_map, const __grid_constant__ CUtensorMap x_map,
+                           const LinearArgs a) {
+    using S = RowsShape<N>;
+    extern __shared__ uint8_t dyn_smem[];
+    __shared__ uint64_t full[S::kStages], empty[S::kStages], tmem_full[2], tmem_empty[2];
+    __shared__ uint32_t tmem_slot;
+
+    const uint32_t raw = pkv::smem_addr(dyn_smem);
+    const uint32_t base = (raw + 1023u) & ~1023u;
+    const int split = static_cast<int>(blockIdx.x) % a.splits;
+    const int first_tile = static_cast<int>(blockIdx.x) / a.splits;
+    const int tile_step = static_cast<int>(gridDim.x) / a.splits;
+    const int kb_begin = static_cast<int>(static_cast<int64_t>(split) * a.k_blocks / a.splits);
+    const int kb_end = static_cast<int>(static_cast<int64_t>(split + 1) * a.k_blocks / a.splits);
+    const int count = kb_end - kb_begin;
+    const int warp = threadIdx.x >> 5;
+    const int lane = threadIdx.x & 31;
+    constexpr int kProducer = S::kEpilogueWarps;
+    constexpr int kMma = S::kEpilogueWarps + 1;
+
+    if (warp == kMma) {
+        pkv::tc::tmem_alloc(pkv::smem_addr(&tmem_slot), S::kTmemColumns);
+        pkv::tc::tmem_relinquish();
+    }
+    if (threadIdx.x == kProducer * 32) {
+        for (int s = 0; s < S::kStages; ++s) {
+            pkv::mbar_init(pkv::smem_addr(&full[s]), 1);
+            pkv::mbar_init(pkv::smem_addr(&empty[s]), 1);
+        }
+        for (int b = 0; b < 2; ++b) {
+            pkv::mbar_init(pkv::smem_addr(&tmem_full[b]), 1);
+            pkv::mbar_init(pkv::smem_addr(&tmem_empty[b]), S::kEpilogueWarps);
+        }
+        pkv::fence_barrier_init();
+    }
+    pkv::tc::fence_before_sync();
+    __syncthreads();
+    pkv::tc::fence_after_sync();
+    const uint32_t tmem = tmem_slot;
+    pkv::pdl_launch_dependents();
+
+    uint64_t acc[32];  // this warp's 64 columns, two to a register pair
+
+    if (warp == kProducer) {
+        if (lane == 0) {
+            const uint64_t reused = pkv::l2_policy_evict_last();
+            int issued = 0;
+            bool ok = true;
+            for (int tile = first_tile; ok && tile < a.tiles; tile += tile_step) {
+                const int m0 = tile % a.m_tiles * kTileRows, n0 = tile / a.m_tiles * N;
+                for (int i = 0; i < count; ++i) {
+                    const int st = issued % S::kStages;
+                    if (issued >= S::kStages &&
+                        !wait_bounded(pkv::smem_addr(&empty[st]), ((issued / S::kStages) - 1) & 1, a.error_flag)) {
+                        ok = false;
+                        break;
+                    }
+                    const uint32_t dst = base + st * S::kStageBytes, bar = pkv::smem_addr(&full[st]);
+                    pkv::mbar_arrive_expect_tx(bar, S::kStageBytes);
+                    // The weight is no kernel's output: the first box goes out before the wait.
+                    pkv::tma_load_2d(dst + S::kXBytes, &w_map, (kb_begin + i) * kKBlock, n0, bar);
+                    if (issued == 0) pkv::pdl_wait();
+                    pkv::tma_load_2d_hint(dst, &x_map, (kb_begin + i) * kKBlock, m0, bar, reused);
+                    ++issued;
+                }
+            }
+            // No copy may land once the ring is reused or the CTA has left.
+            for (int i = max(0, issued - S::kStages); i < issued; ++i) {
+                pkv::mbar_wait_bounded(pkv::smem_addr(&full[i % S::kStages]), (i / S::kStages) & 1, kWaitPolls);
+            }
+        } else {
+            pkv::pdl_wait();
+        }
+        __syncwarp();
+    } else if (warp >= kMma) {
+        // Two issuing warps, one per TMEM buffer: each takes every other K block, so
+        // one's waits and issue (about 200 and 50 clocks each) run beside the other's MMAs.
+        pkv::pdl_wait();
+        if (lane == 0) {
+            constexpr uint32_t idesc = idesc_e4m3_f32(kTileRows, N);
+            int done = 0;
+            bool ok = true;
+            for (int tile = first_tile; ok && tile < a.tiles; tile += tile_step) {
+                for (int i = 0; i < count; ++i, ++done) {
+                    const int st = done % S::kStages;
+                    const int buf = done & 1;
+                    if (buf != warp - kMma) continue;
+                    ok = wait_bounded(pkv::smem_addr(&full[st]), (done / S::kStages) & 1, a.error_flag) &&
+                         (done < 2 || wait_bounded(pkv::smem_addr(&tmem_empty[buf]), ((done >> 1) - 1) & 1, a.error_flag));
+                    if (!ok) break;
+                    pkv::tc::fence_after_sync();
+                    const uint32_t src = base + st * S::kStageBytes;
+#pragma unroll
+                    for (int k = 0; k < kKBlock / 32; ++k) {
+                        mma_f8_ss(tmem + buf * S::kBufferColumns, pkv::tc::desc_k_major_sw128(src + 32 * k),
+                                  pkv::tc::desc_k_major_sw128(src + S::kXBytes + 32 * k), idesc, k > 0);
+                    }
+                    pkv::tc::commit(pkv::smem_addr(&empty[st]));
+                    pkv::tc::commit(pkv::smem_addr(&tmem_full[buf]));
+                }
+            }
+        }
+        __syncwarp();
+    } else {
+        pkv::pdl_wait();
+        const int quarter = warp & 3, first = (warp >> 2) * 64;  // TMEM lanes and columns of this warp
+        const uint32_t lanes = static_cast<uint32_t>(quarter * 32) << 16;
+        const uint32_t staging = base + S::kRing + warp * S::kStoreBytes;
+        int done = 0;
+        bool ok = true;
+        for (int tile = first_tile; tile < a.tiles; tile += tile_step) {
+            const int m0 = tile % a.m_tiles * kTileRows, n0 = tile / a.m_tiles * N;
+            const int row = m0 + quarter * 32 + lane;
+            const int block = min((n0 + first) / kTileRows, a.w_blocks - 1);  // columns past n are not stored
+            // Scales four K blocks at a time, a group ahead: no register is touched
+            // while its load is under way.
+            const float *sx = a.x_scales + static_cast<int64_t>(min(row, a.rows - 1)) * a.k_blocks + kb_begin;
+            const float *sw = a.w_scales + static_cast<int64_t>(block) * a.k_blocks + kb_begin;
+            float x_next[4], w_next[4];
+            load_group(sx, 0, count, x_next);
+            load_group(sw, 0, count, w_next);
+#pragma unroll
+            for (int c = 0; c < 32; ++c) acc[c] = 0;
+            for (int group = 0; group < count; group += 4) {
+                float f[4];
+#pragma unroll
+                for (int j = 0; j < 4; ++j) f[j] = x_next[j] * w_next[j];
+                load_group(sx, group + 4, count, x_next);
+                load_group(sw, group + 4, count, w_next);
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    if (group + j < count) {
+                        const int buf = done & 1;
+                        if (ok) ok = wait_bounded(pkv::smem_addr(&tmem_full[buf]), (done >> 1) & 1, a.error_flag);
+                        ok = __all_sync(0xffffffffu, ok);
+                        ++done;
+                        if (ok) {
+                            pkv::tc::fence_after_sync();
+                            const uint64_t f2 = pkv::f32x2(f[j], f[j]);
+                            const uint32_t src = tmem + lanes + buf * S::kBufferColumns + first;
+                            uint32_t d[2][32];
+                            pkv::tc::tmem_ld32(src, d[0]);
+                            pkv::tc::tmem_ld32(src + 32, d[1]);
+                            pkv::tc::tmem_wait_ld();
+                            pkv::tc::fence_before_sync();
+                            __syncwarp();
+                            if (lane == 0) pkv::mbar_arrive(pkv::smem_addr(&tmem_empty[buf]));
+                            add_scaled(acc, d[0], f2);
+                            add_scaled(acc + 16, d[1], f2);
+                        }
+                    }
+                }
+            }
+            if (a.splits == 1) {
+                // 32 columns at a time through the warp's own staging (16-byte chunk c of
+                // row r at chunk c ^ (r / 2 % 4): no bank conflicts), then 64 bytes a row.
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+#pragma unroll
+                    for (int c = 0; c < 4; ++c) {
+                        uint32_t w[4];
+#pragma unroll
+                        for (int j = 0; j < 4; ++j) {
+                            const float2 v = pkv::unpack_f32x2(acc[16 * h + 4 * c + j]);
+                            w[j] = pkv::pack_half2(__floats2half2_rn(v.x, v.y));
+                        }
+                        asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(staging + lane * 64 + ((c ^ ((lane >> 1) & 3)) << 4)),
+                                     "r"(w[0]), "r"(w[1]), "r"(w[2]), "r"(w[3])
+                                     : "memory");
+                    }
+                    __syncwarp();
+#pragma unroll
+                    for (int part = 0; part < 4; ++part) {
+                        const int r = part * 8 + (lane >> 2), c = lane & 3;
+                        uint32_t w[4];
+                        asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];"
+                                     : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3])
+                                     : "r"(staging + r * 64 + ((c ^ ((r >> 1) & 3)) << 4))
+                                     : "memory");
+                        const int m = m0 + quarter * 32 + r, n = n0 + first + 32 * h + 8 * c;
+                        if (m < a.rows && n < a.n) {
+                            __half *dst = a.out + static_cast<int64_t>(m) * a.out_stride + n;
+                            if (a.vector_out && n + 8 <= a.n) {
+                                *reinterpret_cast<uint4 *>(dst) = make_uint4(w[0], w[1], w[2], w[3]);
+                            } else {
+                                const __half *v = reinterpret_cast<const __half *>(w);
+#pragma unroll
+                                for (int j = 0; j < 8; ++j) {
+                                    if (n + j < a.n) dst[j] = v[j];
+                                }
+                            }
+                        }
+                    }
+                    __syncwarp();
+                }
+            }
+        }
+    }
+
+    if (a.splits > 1) {
+        // One tile per cluster: each CTA leaves its sums in its ring, and rank r adds
+        // and writes rows r, r + splits, ...
+        __syncthreads();  // every copy has landed and every MMA has been read (or given up on)
+        const int m0 = first_tile % a.m_tiles * kTileRows, n0 = first_tile / a.m_tiles * N;
+        if (warp < S::kEpilogueWarps) {
+            const uint32_t dst = base + (((warp & 3) * 32 + lane) * S::kPitch + (warp >> 2) * 64) * 4;
+#pragma unroll
+            for (int c = 0; c < 16; ++c) {
+                const float2 u = pkv::unpack_f32x2(acc[2 * c]), v = pkv::unpack_f32x2(acc[2 * c + 1]);
+                asm volatile("st.shared.v4.f32 [%0], {%1, %2, %3, %4};" ::"r"(dst + 16 * c), "f"(u.x), "f"(u.y),
+                             "f"(v.x), "f"(v.y)
+                             : "memory");
+            }
+        }
+        cluster_arrive();
+        cluster_wait();
+        for (int r = split + a.splits * warp; r < kTileRows && m0 + r < a.rows; r += a.splits * (S::kThreads / 32)) {
+            for (int c = 4 * lane; c < N && n0 + c < a.n; c += 128) {
+                const uint32_t at = base + (r * S::kPitch + c) * 4;
+                float4 v = ld_cluster_f4(map_to_rank(at, 0));
+                for (int s = 1; s < a.splits; ++s) {
+                    const float4 u = ld_cluster_f4(map_to_rank(at, s));
+                    v.x += u.x, v.y += u.y, v.z += u.z, v.w += u.w;
+                }
+                store4(a, m0 + r, n0 + c, v);
+            }
+        }
+        cluster_arrive();  // no CTA leaves while another reads its sums
+        cluster_wait();
+    } else {
+        __syncthreads();
     }
     if (warp == kMma) {
         pkv::tc::fence_after_sync();
@@ -386,50 +677,90 @@ int sm_count(int device) {
     return sms;
 }
 
-template <int NT>
-int launch(int device, const void *x, int64_t x_stride, const void *w, int32_t k, LinearArgs &args,
-           cudaStream_t stream) {
-    using S = Shape<NT>;
-    static std::atomic<int> prepared[kMaxDevices] = {};
-    if (device < 0 || device >= kMaxDevices || !prepared[device].load(std::memory_order_acquire)) {
-        const cudaError_t e =
-            cudaFuncSetAttribute(fp8_linear_kernel<NT>, cudaFuncAttributeMaxDynamicSharedMemorySize, S::kSmem);
-        if (e != cudaSuccess) {
-            return pkv::fail(PKV_CUDA_ERROR, std::string("fp8 linear: cudaFuncSetAttribute: ") + cudaGetErrorString(e));
-        }
-        if (device >= 0 && device < kMaxDevices) prepared[device].store(1, std::memory_order_release);
+// Raise a kernel's shared-memory limit once per device.
+int prepare(const void *kernel, int smem, int device, std::atomic<int> *prepared) {
+    const bool known = device >= 0 && device < kMaxDevices;
+    if (known && prepared[device].load(std::memory_order_acquire)) return PKV_OK;
+    const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+    if (e != cudaSuccess) {
+        return pkv::fail(PKV_CUDA_ERROR, std::string("fp8 linear: cudaFuncSetAttribute: ") + cudaGetErrorString(e));
     }
-    CUtensorMap w_map, x_map;
-    int rc = byte_matrix_map(w, static_cast<uint64_t>(args.n), static_cast<uint64_t>(k), static_cast<uint64_t>(k),
-                             kTileRows, &w_map);
-    if (rc) return rc;
-    rc = byte_matrix_map(x, static_cast<uint64_t>(args.rows), static_cast<uint64_t>(k), static_cast<uint64_t>(x_stride),
-                         NT, &x_map);
-    if (rc) return rc;
-    const int64_t tiles = static_cast<int64_t>(args.n_tiles) * ((args.rows + NT - 1) / NT);
-    // Split K while the cluster's CTAs still find free SMs and each keeps a K block.
-    int splits = 1;
-    const int sms = sm_count(device);
-    while (splits < kMaxCluster && tiles * splits * 2 <= sms + sms / 8 && args.k_blocks >= 2 * splits) splits *= 2;
-    if (tiles * splits > INT32_MAX) return pkv::fail(PKV_VALUE_ERROR, "fp8 linear: too many tiles");
-    args.splits = splits;
+    if (known) prepared[device].store(1, std::memory_order_release);
+    return PKV_OK;
+}
+
+using Kernel = void (*)(CUtensorMap, CUtensorMap, LinearArgs);
+
+int launch_kernel(Kernel kernel, int grid, int threads, int smem, const CUtensorMap &w_map, const CUtensorMap &x_map,
+                  const LinearArgs &args, cudaStream_t stream) {
     cudaLaunchConfig_t config = {};
-    config.gridDim = dim3(static_cast<unsigned>(tiles * splits));
-    config.blockDim = dim3(S::kThreads);
-    config.dynamicSmemBytes = S::kSmem;
+    config.gridDim = dim3(grid);
+    config.blockDim = dim3(threads);
+    config.dynamicSmemBytes = smem;
     config.stream = stream;
     cudaLaunchAttribute attributes[2];
     attributes[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
     attributes[0].val.programmaticStreamSerializationAllowed = 1;
     attributes[1].id = cudaLaunchAttributeClusterDimension;
-    attributes[1].val.clusterDim.x = static_cast<unsigned>(splits);
+    attributes[1].val.clusterDim.x = static_cast<unsigned>(args.splits);
     attributes[1].val.clusterDim.y = 1;
     attributes[1].val.clusterDim.z = 1;
     config.attrs = attributes;
-    config.numAttrs = splits > 1 ? 2 : 1;
-    const cudaError_t e = cudaLaunchKernelEx(&config, fp8_linear_kernel<NT>, w_map, x_map, args);
+    config.numAttrs = args.splits > 1 ? 2 : 1;
+    const cudaError_t e = cudaLaunchKernelEx(&config, kernel, w_map, x_map, args);
     if (e != cudaSuccess) return pkv::fail(PKV_CUDA_ERROR, std::string("fp8 linear launch failed: ") + cudaGetErrorString(e));
     return PKV_OK;
+}
+
+int operand_maps(const void *x, int64_t x_stride, int x_box, const void *w, int w_box, int32_t k, const LinearArgs &args,
+                 CUtensorMap *w_map, CUtensorMap *x_map) {
+    const int rc = byte_matrix_map(w, static_cast<uint64_t>(args.n), static_cast<uint64_t>(k), static_cast<uint64_t>(k),
+                                   static_cast<uint32_t>(w_box), w_map);
+    if (rc) return rc;
+    return byte_matrix_map(x, static_cast<uint64_t>(args.rows), static_cast<uint64_t>(k), static_cast<uint64_t>(x_stride),
+                           static_cast<uint32_t>(x_box), x_map);
+}
+
+// CTAs that share a tile's K blocks: as many as still find free SMs, each keeping a block.
+int row_splits(int64_t tiles, int k_blocks, int slots) {
+    int splits = 1;
+    while (splits < kMaxCluster && tiles * splits * 2 <= slots && k_blocks >= 2 * splits) splits *= 2;
+    return splits;
+}
+
+template <int NT>
+int launch_few(int device, const void *x, int64_t x_stride, const void *w, int32_t k, int sms, LinearArgs &args,
+               cudaStream_t stream) {
+    using S = Shape<NT>;
+    static std::atomic<int> prepared[kMaxDevices] = {};
+    int rc = prepare(reinterpret_cast<const void *>(fp8_linear_kernel<NT>), S::kSmem, device, prepared);
+    if (rc) return rc;
+    CUtensorMap w_map, x_map;
+    if ((rc = operand_maps(x, x_stride, NT, w, kTileRows, k, args, &w_map, &x_map))) return rc;
+    args.splits = row_splits(args.n_tiles, args.k_blocks, sms + sms / 8);
+    if (static_cast<int64_t>(args.n_tiles) * args.splits > INT32_MAX) {
+        return pkv::fail(PKV_VALUE_ERROR, "fp8 linear: too many tiles");
+    }
+    return launch_kernel(fp8_linear_kernel<NT>, args.n_tiles * args.splits, S::kThreads, S::kSmem, w_map, x_map, args, stream);
+}
+
+template <int N>
+int launch_rows(int device, const void *x, int64_t x_stride, const void *w, int32_t k, int sms, LinearArgs &args,
+                cudaStream_t stream) {
+    using S = RowsShape<N>;
+    static std::atomic<int> prepared[kMaxDevices] = {};
+    int rc = prepare(reinterpret_cast<const void *>(fp8_linear_rows_kernel<N>), S::kSmem, device, prepared);
+    if (rc) return rc;
+    CUtensorMap w_map, x_map;
+    if ((rc = operand_maps(x, x_stride, kTileRows, w, N, k, args, &w_map, &x_map))) return rc;
+    const int64_t m_tiles = (static_cast<int64_t>(args.rows) + kTileRows - 1) / kTileRows;
+    const int64_t tiles = m_tiles * ((static_cast<int64_t>(args.n) + N - 1) / N);
+    if (tiles > INT32_MAX / kMaxCluster) return pkv::fail(PKV_VALUE_ERROR, "fp8 linear: too many tiles");
+    args.m_tiles = static_cast<int32_t>(m_tiles);
+    args.tiles = static_cast<int32_t>(tiles);
+    args.splits = row_splits(tiles, args.k_blocks, sms);
+    const int64_t grid = args.splits > 1 ? tiles * args.splits : tiles < sms ? tiles : sms;
+    return launch_kernel(fp8_linear_rows_kernel<N>, static_cast<int>(grid), S::kThreads, S::kSmem, w_map, x_map, args, stream);
 }
 
 }  // namespace
@@ -464,12 +795,30 @@ extern "C" int pkv_fp8_linear(const void *x, int64_t x_stride, const void *x_sca
     args.k_blocks = (k + kKBlock - 1) / kKBlock;
     args.splits = 1;
     args.n_tiles = (n + kTileRows - 1) / kTileRows;
-    args.vector_out = (reinterpret_cast<uintptr_t>(out) & 7) == 0 && out_stride % 4 == 0;
+    args.m_tiles = 0;
+    args.tiles = 0;
+    args.w_blocks = args.n_tiles;
+    args.vector_out = (reinterpret_cast<uintptr_t>(out) & 15) == 0 && out_stride % 8 == 0;
     args.error_flag = error_flag;
     const auto s = static_cast<cudaStream_t>(stream);
-    if (rows <= 16) return launch<16>(device, x, x_stride, w, k, args, s);
-    if (rows <= 32) return launch<32>(device, x, x_stride, w, k, args, s);
-    if (rows <= 64) return launch<64>(device, x, x_stride, w, k, args, s);
-    if (rows <= 128) return launch<128>(device, x, x_stride, w, k, args, s);
-    return launch<256>(device, x, x_stride, w, k, args, s);
+    const int sms = sm_count(device);
+    if (rows <= 16) return launch_few<16>(device, x, x_stride, w, k, sms, args, s);
+    if (rows <= 32) return launch_few<32>(device, x, x_stride, w, k, sms, args, s);
+    if (rows <= 64) return launch_few<64>(device, x, x_stride, w, k, sms, args, s);
+    // Tile width by the time of the busiest SM: rounds of tiles times the tensor
+    // time of a K block, 2 N clocks (192 at N = 64, where reading x's tile from
+    // shared memory bounds it), over the splits that fill the SMs.
+    const int64_t m_tiles = (rows + kTileRows - 1) / kTileRows;
+    int best = 0;
+    int64_t best_cost = 0;
+    for (const int width : {192, 128, 64}) {
+        const int64_t tiles = m_tiles * ((n + width - 1) / width);
+        const int splits = row_splits(tiles, args.k_blocks, sms);
+        const int64_t rounds = (tiles * splits + sms - 1) / sms;
+        const int64_t cost = rounds * ((args.k_blocks + splits - 1) / splits) * (width == 64 ? 192 : 2 * width);
+        if (best == 0 || cost < best_cost) best = width, best_cost = cost;
+    }
+    if (best == 192) return launch_rows<192>(device, x, x_stride, w, k, sms, args, s);
+    if (best == 128) return launch_rows<128>(device, x, x_stride, w, k, sms, args, s);
+    return launch_rows<64>(device, x, x_stride, w, k, sms, args, s);
 }

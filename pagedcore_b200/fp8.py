@@ -17,7 +17,6 @@ Scales made here are powers of two, so every stored value is an FP16 number.
 
 from __future__ import annotations
 
-import contextlib
 import ctypes
 import functools
 from dataclasses import dataclass
@@ -40,36 +39,33 @@ def _groups(width: int) -> int:
     return -(-width // GROUP)
 
 
-def _device(*tensors: Tensor) -> torch.device:
-    """The CUDA device that every tensor is on."""
-    device = tensors[0].device
-    if device.type != "cuda":
+def _device(first: Tensor, *others: Tensor) -> int:
+    """Index of the CUDA device that every tensor is on."""
+    index = first.get_device()
+    if index < 0:
         raise ValueError("8-bit operators need CUDA tensors")
-    for tensor in tensors:
-        if tensor.device != device:
-            raise ValueError(f"every tensor must be on {device}")
-    return device
+    for tensor in others:
+        if tensor.get_device() != index:
+            raise ValueError(f"every tensor must be on cuda:{index}")
+    return index
 
 
-@contextlib.contextmanager
-def _switched(device: torch.device):
-    with torch.cuda.device(device):
-        yield
+def _call(index: int, function, *args) -> None:
+    """Launch on device ``index`` and its current stream, whatever the current device is.
+
+    The raw stream handle spares the Stream object that
+    ``torch.cuda.current_stream`` builds (2 us of a 5 us call).
+    """
+    if torch._C._cuda_getDevice() == index:
+        status = function(*args, torch._C._cuda_getCurrentRawStream(index))
+    else:
+        with torch.cuda.device(index):
+            status = function(*args, torch._C._cuda_getCurrentRawStream(index))
+    if status:
+        check(status)
 
 
-_SAME = contextlib.nullcontext()
-
-
-def _on(device: torch.device):
-    """Launch on ``device`` whatever the current device is."""
-    return _SAME if torch.cuda.current_device() == device.index else _switched(device)
-
-
-def _stream(device: torch.device) -> int:
-    return torch.cuda.current_stream(device).cuda_stream
-
-
-@dataclass(frozen=True, slots=True)
+@dataclass(slots=True)
 class Fp8Rows:
     """E4M3 codes [rows, width] and FP32 scales [rows, ceil(width / 128)]."""
 
@@ -82,24 +78,24 @@ class Fp8Rows:
 
     def to_half(self, out: Tensor | None = None) -> Tensor:
         """The values as FP16 [rows, width] (exact for scales made by this module)."""
-        _check_rows(self)
-        rows, width = self.codes.shape
-        device = _device(self.codes, self.scales)
+        rows, width = _check_rows(self)
+        index = _device(self.codes, self.scales)
         if not self.codes.is_contiguous():
             raise ValueError("to_half needs contiguous codes")
         if out is None:
-            out = torch.empty((rows, width), dtype=torch.float16, device=device)
-        elif out.shape != (rows, width) or out.dtype != torch.float16 or out.stride(1) != 1 or out.device != device:
-            raise ValueError(f"out must be FP16 [{rows}, {width}] with contiguous rows")
-        if rows == 0:
-            return out
-        with _on(device):
-            check(lib.pkv_fp8_to_half(self.codes.data_ptr(), self.scales.data_ptr(), rows, width, out.data_ptr(),
-                                      out.stride(0), _stream(device)))
+            out = torch.empty((rows, width), dtype=torch.float16, device=self.codes.device)
+            stride = width
+        else:
+            if out.shape != (rows, width) or out.dtype != torch.float16 or out.stride(1) != 1 or out.get_device() != index:
+                raise ValueError(f"out must be FP16 [{rows}, {width}] with contiguous rows")
+            stride = max(out.stride(0), width)
+        if rows:
+            _call(index, lib.pkv_fp8_to_half, self.codes.data_ptr(), self.scales.data_ptr(), rows, width,
+                  out.data_ptr(), stride)
         return out
 
 
-@dataclass(frozen=True, slots=True)
+@dataclass(slots=True)
 class Fp8Weight:
     """E4M3 codes [n, k] and FP32 scales [ceil(n / 128), ceil(k / 128)]."""
 
@@ -111,16 +107,14 @@ class Fp8Weight:
         return tuple(self.codes.shape)
 
 
-def _check_rows(x: Fp8Rows) -> None:
+def _check_rows(x: Fp8Rows) -> tuple[int, int]:
     codes, scales = x.codes, x.scales
-    if codes.ndim != 2 or codes.dtype != _CODES or (codes.numel() and codes.stride(1) != 1):
+    if codes.ndim != 2 or codes.dtype != _CODES or codes.stride(1) != 1:
         raise ValueError("8-bit rows must be E4M3 [rows, width] with contiguous rows")
-    if (
-        scales.shape != (codes.shape[0], _groups(codes.shape[1]))
-        or scales.dtype != torch.float32
-        or not scales.is_contiguous()
-    ):
+    rows, width = codes.shape
+    if scales.shape != (rows, _groups(width)) or scales.dtype != torch.float32 or not scales.is_contiguous():
         raise ValueError("8-bit rows need contiguous FP32 scales [rows, ceil(width / 128)]")
+    return rows, width
 
 
 def _empty_rows(rows: int, width: int, device: torch.device) -> Fp8Rows:
@@ -151,36 +145,34 @@ def add_rms_norm(
     """
     if hidden.ndim != 2:
         raise ValueError("hidden must be contiguous FP16 [rows, dim]")
-    rows, dim = hidden.shape
-    _half_matrix("hidden", hidden, (rows, dim))
+    rows, dim = shape = hidden.shape
+    _half_matrix("hidden", hidden, shape)
     _half_matrix("weight", weight, (dim,))
+    delta_ptr = residual_ptr = None
     if delta is None:
-        device = _device(hidden, weight)
-        delta_ptr = residual_ptr = None
+        index = _device(hidden, weight)
     else:
         if residual is None:
             residual = hidden
-        _half_matrix("delta", delta, (rows, dim))
-        _half_matrix("residual", residual, (rows, dim))
-        device = _device(hidden, weight, delta, residual)
+        else:
+            _half_matrix("residual", residual, shape)
+        _half_matrix("delta", delta, shape)
+        index = _device(hidden, weight, delta, residual)
         delta_ptr, residual_ptr = delta.data_ptr(), residual.data_ptr()
-    out = _empty_rows(rows, dim, device)
-    if rows == 0:
-        return out
-    with _on(device):
-        check(lib.pkv_fp8_add_rms_norm(hidden.data_ptr(), delta_ptr, weight.data_ptr(), residual_ptr,
-                                       out.codes.data_ptr(), out.scales.data_ptr(), rows, dim, eps, _stream(device)))
+    out = _empty_rows(rows, dim, hidden.device)
+    if rows:
+        _call(index, lib.pkv_fp8_add_rms_norm, hidden.data_ptr(), delta_ptr, weight.data_ptr(), residual_ptr,
+              out.codes.data_ptr(), out.scales.data_ptr(), rows, dim, eps)
     return out
 
 
 def _quantize(x: Tensor, width: int, silu_pairs: bool) -> Fp8Rows:
-    device = _device(x)
-    out = _empty_rows(x.shape[0], width, device)
-    if x.shape[0] == 0:
-        return out
-    with _on(device):
-        check(lib.pkv_fp8_quantize(x.data_ptr(), max(x.stride(0), x.shape[1]), silu_pairs, x.shape[0], width,
-                                   out.codes.data_ptr(), out.scales.data_ptr(), _stream(device)))
+    index = _device(x)
+    rows, columns = x.shape
+    out = _empty_rows(rows, width, x.device)
+    if rows:
+        _call(index, lib.pkv_fp8_quantize, x.data_ptr(), max(x.stride(0), columns), silu_pairs, rows, width,
+              out.codes.data_ptr(), out.scales.data_ptr())
     return out
 
 
@@ -221,34 +213,32 @@ def linear(x: Fp8Rows, weight: Fp8Weight, out: Tensor | None = None) -> Tensor:
     Any number of rows and any n; k a multiple of 16.  FP32 sums on the
     tensor cores, scaled block by block, rounded once.
     """
-    _check_rows(x)
-    (rows, k), (n, wk) = x.codes.shape, weight.codes.shape
-    if wk != k or weight.codes.dtype != _CODES or not weight.codes.is_contiguous():
+    rows, k = _check_rows(x)
+    codes, scales = weight.codes, weight.scales
+    if codes.ndim != 2 or codes.shape[1] != k or codes.dtype != _CODES or not codes.is_contiguous():
         raise ValueError(f"weight must be contiguous E4M3 [n, {k}]")
-    if (
-        weight.scales.shape != (_groups(n), _groups(k))
-        or weight.scales.dtype != torch.float32
-        or not weight.scales.is_contiguous()
-    ):
+    n = codes.shape[0]
+    if scales.shape != (_groups(n), _groups(k)) or scales.dtype != torch.float32 or not scales.is_contiguous():
         raise ValueError("weight needs contiguous FP32 scales [ceil(n / 128), ceil(k / 128)]")
-    device = _device(x.codes, x.scales, weight.codes, weight.scales)
+    index = _device(x.codes, x.scales, codes, scales)
     if out is None:
-        out = torch.empty((rows, n), dtype=torch.float16, device=device)
-    elif out.shape != (rows, n) or out.dtype != torch.float16 or out.stride(1) != 1 or out.device != device:
-        raise ValueError(f"out must be FP16 [{rows}, {n}] with contiguous rows")
-    if rows == 0:
-        return out
-    with _on(device):
-        check(lib.pkv_fp8_linear(x.codes.data_ptr(), max(x.codes.stride(0), k), x.scales.data_ptr(),
-                                 weight.codes.data_ptr(), weight.scales.data_ptr(), rows, n, k, out.data_ptr(),
-                                 max(out.stride(0), n), linear_error_flag(device).data_ptr(), _stream(device)))
+        out = torch.empty((rows, n), dtype=torch.float16, device=codes.device)
+        stride = n
+    else:
+        if out.shape != (rows, n) or out.dtype != torch.float16 or out.stride(1) != 1 or out.get_device() != index:
+            raise ValueError(f"out must be FP16 [{rows}, {n}] with contiguous rows")
+        stride = max(out.stride(0), n)
+    if rows:
+        _call(index, lib.pkv_fp8_linear, x.codes.data_ptr(), max(x.codes.stride(0), k), x.scales.data_ptr(),
+              codes.data_ptr(), scales.data_ptr(), rows, n, k, out.data_ptr(), stride,
+              linear_error_flag(codes.device).data_ptr())
     return out
 
 
 # -- the KV cache ------------------------------------------------------------------
 
 
-@dataclass(frozen=True, slots=True)
+@dataclass(slots=True)
 class Fp8Cache:
     """An 8-bit KV cache: E4M3 codes and FP32 scales.
 
@@ -263,21 +253,22 @@ class Fp8Cache:
     value_scales: Tensor
 
     def __post_init__(self) -> None:
-        codes = self.key_codes
-        if codes.ndim != 5 or codes.shape[2:] != (_KV_HEADS, _BLOCK_TOKENS, _HEAD_DIM):
+        keys, values, key_scales, value_scales = self.key_codes, self.value_codes, self.key_scales, self.value_scales
+        shape = keys.shape
+        if len(shape) != 5 or shape[2:] != (_KV_HEADS, _BLOCK_TOKENS, _HEAD_DIM):
             raise ValueError("key_codes must be E4M3 [layers, blocks, 4, 16, 64]")
-        layers, blocks = codes.shape[:2]
+        layers, blocks = shape[0], shape[1]
         if layers < 1 or blocks < 1:
             raise ValueError("an 8-bit cache needs at least one layer and one block")
-        if self.value_codes.shape != (layers, blocks, _KV_HEADS, _HEAD_DIM, _BLOCK_TOKENS):
+        if values.shape != (layers, blocks, _KV_HEADS, _HEAD_DIM, _BLOCK_TOKENS):
             raise ValueError("value_codes must be E4M3 [layers, blocks, 4, 64, 16]")
-        for tensor in (codes, self.value_codes):
-            if tensor.dtype != _CODES or not tensor.is_contiguous():
-                raise ValueError("cache codes must be contiguous E4M3 storage")
-        for tensor in (self.key_scales, self.value_scales):
-            if tensor.shape != (layers, blocks, _KV_HEADS) or tensor.dtype != torch.float32 or not tensor.is_contiguous():
+        if keys.dtype != _CODES or values.dtype != _CODES or not (keys.is_contiguous() and values.is_contiguous()):
+            raise ValueError("cache codes must be contiguous E4M3 storage")
+        scales = (layers, blocks, _KV_HEADS)
+        for tensor in (key_scales, value_scales):
+            if tensor.shape != scales or tensor.dtype != torch.float32 or not tensor.is_contiguous():
                 raise ValueError("cache scales must be contiguous FP32 [layers, blocks, 4]")
-        _device(codes, self.value_codes, self.key_scales, self.value_scales)
+        _device(keys, values, key_scales, value_scales)
 
     @classmethod
     def empty(cls, layers: int, blocks: int, device: str | torch.device = "cuda") -> Fp8Cache:
@@ -307,32 +298,38 @@ class Fp8Cache:
                 self.value_scales.data_ptr(), shape[0], shape[1])
 
 
-def _require(device: torch.device, dtype: torch.dtype, **tensors: Tensor) -> None:
-    for name, tensor in tensors.items():
-        if tensor.device != device or tensor.dtype != dtype:
-            raise ValueError(f"{name} must be {dtype} on {device}")
+def _half(name: str, tensor: Tensor, index: int) -> None:
+    if tensor.dtype != torch.float16 or tensor.get_device() != index:
+        raise ValueError(f"{name} must be FP16 on cuda:{index}")
 
 
-def _int_list(device: torch.device, name: str, tensor: Tensor, count: int) -> None:
-    if tensor.device != device or tensor.dtype != torch.int32 or not tensor.is_contiguous() or tensor.numel() < count:
-        raise ValueError(f"{name} must hold {count} contiguous int32 values on {device}")
+def _int_list(index: int, name: str, tensor: Tensor, count: int) -> int:
+    """Address of ``count`` or more int32 values on the device."""
+    if (
+        tensor.dtype != torch.int32
+        or tensor.numel() < count
+        or not tensor.is_contiguous()
+        or tensor.get_device() != index
+    ):
+        raise ValueError(f"{name} must hold {count} contiguous int32 values on cuda:{index}")
+    return tensor.data_ptr()
 
 
-def _check_flag(device: torch.device, error_flag: Tensor) -> None:
-    _int_list(device, "error_flag", error_flag, 1)
-
-
-def _check_rope(device: torch.device, table: Tensor) -> None:
-    _require(device, torch.float16, rope_table=table)
+def _check_rope(index: int, table: Tensor) -> int:
+    _half("rope_table", table, index)
     if table.shape != (2, 2048, 32) or not table.is_contiguous():
         raise ValueError("rope_table must be contiguous FP16 [2, 2048, 32]")
+    return table.data_ptr()
 
 
 def _rows_ok(tensor: Tensor) -> bool:
     """Inner [heads, 64] contiguous and rows 16-byte aligned."""
+    strides = tensor.stride()
     return (
-        tensor.stride()[-2:] == (_HEAD_DIM, 1)
-        and all(stride % 8 == 0 for stride in tensor.stride()[:-2])
+        strides[-1] == 1
+        and strides[-2] == _HEAD_DIM
+        and strides[0] % 8 == 0
+        and strides[-3] % 8 == 0
         and tensor.data_ptr() % 16 == 0
     )
 
@@ -357,61 +354,58 @@ def append_kv(
     which may be ``query`` itself).  The tokens of one block must be
     consecutive, in the list and in the block, as a request's positions are.
     """
-    device = cache.device
-    if key.ndim != 4 or key.shape[2:] != (_KV_HEADS, _HEAD_DIM) or value.shape != key.shape:
+    index = cache.key_codes.get_device()
+    shape = key.shape
+    if len(shape) != 4 or shape[2] != _KV_HEADS or shape[3] != _HEAD_DIM or value.shape != shape:
         raise ValueError("K and V must share FP16 [layers, tokens, 4, 64]")
-    _require(device, torch.float16, key=key, value=value)
-    layers, tokens = key.shape[:2]
-    _int_list(device, "slots", slots, tokens)
-    _check_flag(device, error_flag)
+    _half("key", key, index)
+    _half("value", value, index)
+    layers, tokens = shape[0], shape[1]
+    slots_ptr = _int_list(index, "slots", slots, tokens)
+    flag = _int_list(index, "error_flag", error_flag, 1)
     if (rope_table is None) != (positions is None) or (query is not None and rope_table is None):
         raise ValueError("rope_table goes with positions, query with both")
+    rope = positions_ptr = None
     if rope_table is not None:
-        _check_rope(device, rope_table)
-        _int_list(device, "positions", positions, tokens)
-    if layers == 0 or tokens == 0:
-        return query
-    if not (_rows_ok(key) and value.stride() == key.stride() and _rows_ok(value)):
-        key, value = key.contiguous(), value.contiguous()
+        rope = _check_rope(index, rope_table)
+        positions_ptr = _int_list(index, "positions", positions, tokens)
     q_ptr = out_ptr = None
     q_strides = out_strides = (0, 0)
     if query is not None:
         if query.shape != (layers, tokens, _QUERY_HEADS, _HEAD_DIM):
             raise ValueError("query must be FP16 [layers, tokens, 32, 64]")
-        _require(device, torch.float16, query=query)
+        _half("query", query, index)
         if query_out is None:
-            query_out = torch.empty(query.shape, dtype=torch.float16, device=device)
+            query_out = torch.empty(query.shape, dtype=torch.float16, device=query.device)
         elif query_out.shape != query.shape or not _rows_ok(query_out):
             raise ValueError("query_out must be FP16 [layers, tokens, 32, 64] with contiguous, 16-byte aligned rows")
-        _require(device, torch.float16, query_out=query_out)
+        else:
+            _half("query_out", query_out, index)
         if not _rows_ok(query):
             query = query.contiguous()
         q_ptr, out_ptr = query.data_ptr(), query_out.data_ptr()
         q_strides, out_strides = query.stride()[:2], query_out.stride()[:2]
-    with _on(device):
-        check(
-            lib.pkv_fp8_append_kv(
-                *cache._args(), layer_begin, layers, key.data_ptr(), value.data_ptr(), key.stride(0), key.stride(1),
-                slots.data_ptr(), None if positions is None else positions.data_ptr(), tokens,
-                None if rope_table is None else rope_table.data_ptr(), q_ptr, *q_strides, out_ptr, *out_strides,
-                error_flag.data_ptr(), _stream(device),
-            )
-        )
+    if layers == 0 or tokens == 0:
+        return query_out
+    if not (_rows_ok(key) and value.stride() == key.stride() and _rows_ok(value)):
+        key, value = key.contiguous(), value.contiguous()
+    layer_stride, token_stride = key.stride()[:2]
+    _call(index, lib.pkv_fp8_append_kv, *cache._args(), layer_begin, layers, key.data_ptr(), value.data_ptr(),
+          layer_stride, token_stride, slots_ptr, positions_ptr, tokens, rope, q_ptr, *q_strides, out_ptr, *out_strides,
+          flag)
     return query_out
 
 
 def read_blocks(cache: Fp8Cache, layer: int, blocks: Tensor, error_flag: Tensor) -> tuple[Tensor, Tensor]:
     """K and V of ``blocks`` (int32 [count]) at ``layer`` as FP16 [count, 16, 4, 64] each."""
-    device = cache.device
+    index = cache.key_codes.get_device()
     count = blocks.numel()
-    _int_list(device, "blocks", blocks, count)
-    _check_flag(device, error_flag)
-    out = torch.empty((2, count, _BLOCK_TOKENS, _KV_HEADS, _HEAD_DIM), dtype=torch.float16, device=device)
-    if count == 0:
-        return out[0], out[1]
-    with _on(device):
-        check(lib.pkv_fp8_read_blocks(*cache._args(), layer, blocks.data_ptr(), count, out.data_ptr(), out.stride(0),
-                                      error_flag.data_ptr(), _stream(device)))
+    blocks_ptr = _int_list(index, "blocks", blocks, count)
+    flag = _int_list(index, "error_flag", error_flag, 1)
+    out = torch.empty((2, count, _BLOCK_TOKENS, _KV_HEADS, _HEAD_DIM), dtype=torch.float16, device=blocks.device)
+    if count:
+        _call(index, lib.pkv_fp8_read_blocks, *cache._args(), layer, blocks_ptr, count, out.data_ptr(),
+              count * _BLOCK_TOKENS * _KV_HEADS * _HEAD_DIM, flag)
     return out[0], out[1]
 
 
@@ -428,44 +422,41 @@ def decode_workspace_bytes(batch: int, grid: int) -> int:
     return batch * _QUERY_HEADS * _HEAD_DIM * 2 + (batch + grid) * _QUERY_HEADS * (_HEAD_DIM + 2) * 4
 
 
-def _attention_rows(name: str, tensor: Tensor, shape: tuple[int, ...], device: torch.device) -> None:
-    if tensor.shape != shape or tensor.dtype != torch.float16 or tensor.device != device:
-        raise ValueError(f"{name} must be FP16 {list(shape)} on {device}")
+def _attention_rows(name: str, tensor: Tensor, shape: tuple[int, ...], index: int) -> None:
+    if tensor.shape != shape or tensor.dtype != torch.float16 or tensor.get_device() != index:
+        raise ValueError(f"{name} must be FP16 {list(shape)} on cuda:{index}")
 
 
-def _decode(cache, layer, query, new, rope_table, lengths, prefix, flat, total_blocks, error_flag, out) -> Tensor:
-    device = cache.device
-    if query.ndim != 3 or query.shape[0] < 1:
-        raise ValueError("query must be FP16 [batch, 32, 64] of a nonempty batch")
-    batch = query.shape[0]
-    _attention_rows("query", query, (batch, _QUERY_HEADS, _HEAD_DIM), device)
+def _query_and_out(query: Tensor, out: Tensor | None, index: int, rows: str) -> tuple[Tensor, int, Tensor, int]:
+    """Query and output [rows, 32, 64] as the kernels take them, with their row strides."""
+    shape = query.shape
+    if len(shape) != 3 or shape[0] < 1 or shape[1] != _QUERY_HEADS or shape[2] != _HEAD_DIM:
+        raise ValueError(f"query must be FP16 [{rows}, 32, 64] of a nonempty {rows}")
+    _half("query", query, index)
     if not _rows_ok(query) or query.stride(0) < _QUERY_HEADS * _HEAD_DIM:
         query = query.contiguous()
+    stride = max(query.stride(0), _QUERY_HEADS * _HEAD_DIM)  # of one row it may be anything
     if out is None:
-        out = torch.empty((batch, _QUERY_HEADS, _HEAD_DIM), dtype=torch.float16, device=device)
-    else:
-        _attention_rows("out", out, (batch, _QUERY_HEADS, _HEAD_DIM), device)
-        if not _rows_ok(out):
-            raise ValueError("out must be FP16 [batch, 32, 64] with contiguous, 16-byte aligned rows")
-    _int_list(device, "lengths", lengths, batch)
-    _int_list(device, "prefix", prefix, batch + 1)
-    _int_list(device, "flat", flat, total_blocks)
-    _check_flag(device, error_flag)
-    grid, workspace_bytes = decode_plan(device.index, batch, total_blocks)
-    workspace = torch.empty(workspace_bytes, dtype=torch.uint8, device=device)
-    tables = (lengths.data_ptr(), prefix.data_ptr(), flat.data_ptr(), batch, total_blocks, grid, out.data_ptr(),
-              max(out.stride(0), _QUERY_HEADS * _HEAD_DIM), workspace.data_ptr(), workspace_bytes,
-              error_flag.data_ptr())
-    query_stride = max(query.stride(0), _QUERY_HEADS * _HEAD_DIM)
-    with _on(device):
-        if new is None:
-            check(lib.pkv_fp8_decode_attention(*cache._args(), layer, query.data_ptr(), query_stride, *tables,
-                                               _stream(device)))
-        else:
-            key, value = new
-            check(lib.pkv_fp8_decode_layer(*cache._args(), layer, query.data_ptr(), query_stride, key.data_ptr(),
-                                           value.data_ptr(), key.stride(0), rope_table.data_ptr(), *tables,
-                                           _stream(device)))
+        return query, stride, torch.empty(shape, dtype=torch.float16, device=query.device), _QUERY_HEADS * _HEAD_DIM
+    _attention_rows("out", out, shape, index)
+    if not _rows_ok(out):
+        raise ValueError(f"out must be FP16 [{rows}, 32, 64] with contiguous, 16-byte aligned rows")
+    return query, stride, out, max(out.stride(0), _QUERY_HEADS * _HEAD_DIM)
+
+
+def _decode(cache, layer, query, new, lengths, prefix, flat, total_blocks, error_flag, out) -> Tensor:
+    index = cache.key_codes.get_device()
+    query, query_stride, out, out_stride = _query_and_out(query, out, index, "batch")
+    batch = query.shape[0]
+    grid, workspace_bytes = decode_plan(index, batch, total_blocks)
+    workspace = torch.empty(workspace_bytes, dtype=torch.uint8, device=query.device)
+    _call(
+        index, lib.pkv_fp8_decode_attention if new is None else lib.pkv_fp8_decode_layer, *cache._args(), layer,
+        query.data_ptr(), query_stride, *(new or ()), _int_list(index, "lengths", lengths, batch),
+        _int_list(index, "prefix", prefix, batch + 1), _int_list(index, "flat", flat, total_blocks), batch,
+        total_blocks, grid, out.data_ptr(), out_stride, workspace.data_ptr(), workspace_bytes,
+        _int_list(index, "error_flag", error_flag, 1),
+    )
     return out
 
 
@@ -486,7 +477,7 @@ def decode_attention(
     int32 [total_blocks] (the concatenated block tables) on the device.  A row
     without tokens gives zeros.
     """
-    return _decode(cache, layer, query, None, None, lengths, prefix, flat, total_blocks, error_flag, out)
+    return _decode(cache, layer, query, None, lengths, prefix, flat, total_blocks, error_flag, out)
 
 
 def decode_layer(
@@ -510,14 +501,15 @@ def decode_layer(
     rotated, and attends to all of the row's tokens.  No two rows may share
     a last block.
     """
-    device = cache.device
-    batch = query.shape[0]
-    _attention_rows("key", key, (batch, _KV_HEADS, _HEAD_DIM), device)
-    _attention_rows("value", value, (batch, _KV_HEADS, _HEAD_DIM), device)
-    _check_rope(device, rope_table)
+    index = cache.key_codes.get_device()
+    shape = (query.shape[0], _KV_HEADS, _HEAD_DIM)
+    _attention_rows("key", key, shape, index)
+    _attention_rows("value", value, shape, index)
+    rope = _check_rope(index, rope_table)
     if not (_rows_ok(key) and value.stride() == key.stride() and _rows_ok(value)):
         key, value = key.contiguous(), value.contiguous()
-    return _decode(cache, layer, query, (key, value), rope_table, lengths, prefix, flat, total_blocks, error_flag, out)
+    new = (key.data_ptr(), value.data_ptr(), key.stride(0), rope)
+    return _decode(cache, layer, query, new, lengths, prefix, flat, total_blocks, error_flag, out)
 
 
 _PREFILL_BLOCK_BYTES = 2 * _BLOCK_TOKENS * _KV_HEADS * _HEAD_DIM * 2 + 4  # an FP16 block and its table entry
@@ -537,29 +529,15 @@ def prefill_attention(
     Token t attends to positions 0 .. start + t through ``blocks`` (int32, the
     request's physical block per 16 positions).
     """
-    device = cache.device
-    if query.ndim != 3 or query.shape[0] < 1:
-        raise ValueError("query must be FP16 [tokens, 32, 64]")
+    index = cache.key_codes.get_device()
+    query, query_stride, out, out_stride = _query_and_out(query, out, index, "tokens")
     tokens = query.shape[0]
-    _attention_rows("query", query, (tokens, _QUERY_HEADS, _HEAD_DIM), device)
     if type(start) is not int or start < 0 or start + tokens > 2048:
         raise ValueError("the chunk must hold 1 or more tokens at positions below 2048")
     count = -(-(start + tokens) // _BLOCK_TOKENS)
-    _int_list(device, "blocks", blocks, count)
-    _check_flag(device, error_flag)
-    if not _rows_ok(query) or query.stride(0) < _QUERY_HEADS * _HEAD_DIM:
-        query = query.contiguous()
-    if out is None:
-        out = torch.empty((tokens, _QUERY_HEADS, _HEAD_DIM), dtype=torch.float16, device=device)
-    else:
-        _attention_rows("out", out, (tokens, _QUERY_HEADS, _HEAD_DIM), device)
-        if not _rows_ok(out):
-            raise ValueError("out must be FP16 [tokens, 32, 64] with contiguous, 16-byte aligned rows")
-    workspace = torch.empty(count * _PREFILL_BLOCK_BYTES, dtype=torch.uint8, device=device)
-    with _on(device):
-        check(lib.pkv_fp8_prefill_attention(*cache._args(), layer, query.data_ptr(),
-                                            max(query.stride(0), _QUERY_HEADS * _HEAD_DIM), blocks.data_ptr(), start,
-                                            tokens, out.data_ptr(), max(out.stride(0), _QUERY_HEADS * _HEAD_DIM),
-                                            workspace.data_ptr(), workspace.numel(), error_flag.data_ptr(),
-                                            _stream(device)))
+    blocks_ptr = _int_list(index, "blocks", blocks, count)
+    workspace = torch.empty(count * _PREFILL_BLOCK_BYTES, dtype=torch.uint8, device=query.device)
+    _call(index, lib.pkv_fp8_prefill_attention, *cache._args(), layer, query.data_ptr(), query_stride, blocks_ptr,
+          start, tokens, out.data_ptr(), out_stride, workspace.data_ptr(), count * _PREFILL_BLOCK_BYTES,
+          _int_list(index, "error_flag", error_flag, 1))
     return out
