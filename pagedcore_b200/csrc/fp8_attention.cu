@@ -66,7 +66,7 @@ constexpr int kTile = pkv::fp8::kTileBytes;
 constexpr int kWarps = kHeads;
 constexpr int kThreads = kWarps * 32;
 constexpr int kChunk = 4;     // blocks per stage
-constexpr int kStages = 3;
+constexpr int kStages = 2;
 constexpr int kValuePitch = kTile + 32;
 constexpr int kValueAt = kChunk * kTile;
 constexpr int kScaleAt = kValueAt + kChunk * kValuePitch;   // K then V scale rows, 16 bytes a block
@@ -91,6 +91,7 @@ struct Args {
     int32_t capacity;  // of flat; the batch's blocks are prefix[batch]
     int32_t grid;
     int32_t clear;     // rows without blocks give zeros (else they are left alone)
+    int32_t early;     // the kernel before this one writes, of what this one reads, only the queries and the rows' last blocks
     __half *out;
     int64_t out_stride;
     float *part_o;   // [batch + grid][32][64]
@@ -115,16 +116,12 @@ __device__ __forceinline__ void bulk_load(uint32_t dst, const void *src, uint32_
         : "memory");
 }
 
-__device__ __forceinline__ uint4 lds128(uint32_t addr) {
-    uint4 v;
-    asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(addr));
-    return v;
-}
-
-__device__ __forceinline__ float lds32(uint32_t addr) {
-    float v;
-    asm volatile("ld.shared.f32 %0, [%1];" : "=f"(v) : "r"(addr));
-    return v;
+// D = A(16x16, row) * B(16x8, col) + D, FP16 operands; free to move, unlike the volatile form.
+__device__ __forceinline__ void mma(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
+                                    uint32_t b1) {
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+        : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
 
 __device__ __forceinline__ float max8(float v) {
@@ -169,14 +166,15 @@ __host__ __device__ __forceinline__ int pieces_of(int total, int grid) {
     return chunks < 1 ? 1 : chunks < grid ? chunks : grid;
 }
 
-// Rows of the block list: where each ends.  32 rows from `base` in registers.
+// Rows of the block list: where each begins and ends.  32 rows from `base` in registers.
 struct Rows {
-    int base, last, length;
+    int base, first, last, length;
 };
 
 __device__ __forceinline__ Rows load_rows(const Args &a, int base, int lane) {
     const int r = base + lane;
-    return Rows{base, r < a.batch ? a.prefix[r + 1] : INT32_MAX, r < a.batch ? a.lengths[r] : 0};
+    if (r >= a.batch) return Rows{base, INT32_MAX, INT32_MAX, 0};
+    return Rows{base, a.prefix[r], a.prefix[r + 1], a.lengths[r]};
 }
 
 // The first row at or after `row` that has blocks past `block`, with its window.
@@ -196,54 +194,66 @@ __device__ __forceinline__ void load_query(const Args &a, int row, int head, int
     q[4] = y.x, q[5] = y.y, q[6] = y.z, q[7] = y.w;
 }
 
-__global__ void __launch_bounds__(kThreads, 2) fp8_decode_kernel(const __grid_constant__ Args a) {
+__global__ void __launch_bounds__(kThreads, 3) fp8_decode_kernel(const __grid_constant__ Args a) {
     extern __shared__ __align__(16) uint8_t smem[];
     __shared__ __align__(8) uint64_t barriers[kWarps * kStages];
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int g = lane >> 2, t = lane & 3;
-    const uint32_t ring = pkv::smem_addr(smem) + warp * kStages * kStageBytes;
+    uint8_t *const ring_tiles = smem + warp * kStages * kStageBytes;
+    const uint32_t ring = pkv::smem_addr(ring_tiles);
     const uint32_t bar0 = pkv::smem_addr(&barriers[warp * kStages]);
     if (lane == 0) {
         for (int s = 0; s < kStages; ++s) pkv::mbar_init(bar0 + 8 * s, 1);
         pkv::fence_barrier_init();
     }
     __syncwarp();
-    pkv::pdl_wait();
-    pkv::pdl_launch_dependents();
+    // Launched as a programmatic dependent: behind the append of the same layer
+    // (early) the tables and every block but the rows' last ones are ready, and only
+    // what the append writes is waited for.
+    bool ready = !a.early;
+    if (ready) pkv::pdl_wait();
 
+    // The piece, and a first cut of the rows: 32 samples of prefix, `step` rows apart.
+    int step = (a.batch + 31) / 32;
+    int sample = lane * step < a.batch ? a.prefix[min((lane + 1) * step, a.batch)] : INT32_MAX;
+    const int total = total_blocks(a);
+    const int pieces = pieces_of(total, a.grid);
     // Rows without blocks: zeros.
     for (int b = blockIdx.x * kThreads + threadIdx.x; a.clear && b < a.batch; b += a.grid * kThreads) {
         if (a.prefix[b + 1] <= a.prefix[b]) {
             for (int i = 0; i < kQueryHeads * kDim; ++i) a.out[b * a.out_stride + i] = __float2half_rn(0.f);
         }
     }
-    const int total = total_blocks(a);
-    const int pieces = pieces_of(total, a.grid);
-    if (total == 0 || static_cast<int>(blockIdx.x) >= pieces) return;
+    if (total == 0 || static_cast<int>(blockIdx.x) >= pieces) {
+        if (!ready) pkv::pdl_wait();
+        return;
+    }
     const int begin = piece_begin(blockIdx.x, total, pieces);
     const int end = piece_begin(blockIdx.x + 1, total, pieces);
-
-    const uint64_t policy = pkv::l2_policy_evict_first();
-    // First row with blocks past `begin`, by a 32-way search over prefix[1 ..].
-    int lo = 0, hi = a.batch - 1;
-    while (hi > lo) {
-        const int step = (hi - lo + 32) / 32;
-        const int probe = min(lo + lane * step + step - 1, hi);
-        const unsigned past = __ballot_sync(0xffffffffu, a.prefix[probe + 1] > begin);
-        const int which = past != 0 ? __ffs(past) - 1 : 31;
-        lo = min(lo + which * step, hi);
-        hi = min(lo + step - 1, hi);
-    }
-
-    // Fetch cursor: the next block to copy, the row it belongs to, and the ids
-    // of the list's next 64 blocks (32 at a time, one window ahead).
-    Rows fetch_rows = load_rows(a, lo, lane);
-    int fetch_row = advance_row(a, fetch_rows, lo, begin, lane);
-    int fetch_end = __shfl_sync(0xffffffffu, fetch_rows.last, fetch_row - fetch_rows.base);
-    int fetch = begin;
+    // The ids of the list's next 64 blocks (32 at a time, one window ahead).
     int ids_base = begin;
     int ids = begin + lane < end ? a.flat[begin + lane] : 0;
     int ids_next = begin + 32 + lane < end ? a.flat[begin + 32 + lane] : 0;
+
+    const uint64_t policy = pkv::l2_policy_evict_first();
+    // The first row with blocks past `begin`: the first sample past it, cut finer until
+    // the samples are rows.
+    int lo = 0;
+    while (true) {
+        const unsigned past = __ballot_sync(0xffffffffu, sample > begin);
+        lo += (past != 0 ? __ffs(past) - 1 : 31) * step;
+        if (step <= 32) break;
+        step = (step + 31) / 32;
+        sample = lo + lane * step < a.batch ? a.prefix[min(lo + (lane + 1) * step, a.batch)] : INT32_MAX;
+    }
+    Rows rows = load_rows(a, lo, lane);
+    int row = advance_row(a, rows, lo, begin, lane);
+
+    // Fetch cursor: the next block to copy and the row it belongs to.
+    Rows fetch_rows = rows;
+    int fetch_row = row;
+    int fetch_end = __shfl_sync(0xffffffffu, fetch_rows.last, fetch_row - fetch_rows.base);
+    int fetch = begin;
     int fetched = 0;
 
     const int64_t layer_tile = pkv::fp8::tile_index(a.cache, a.layer, 0, 0);
@@ -255,6 +265,10 @@ __global__ void __launch_bounds__(kThreads, 2) fp8_decode_kernel(const __grid_co
             fetch_end = __shfl_sync(0xffffffffu, fetch_rows.last, fetch_row - fetch_rows.base);
         }
         const int n = min(kChunk, min(fetch_end, end) - fetch);
+        if (!ready && fetch + n >= fetch_end) {  // the row's last block
+            pkv::pdl_wait();
+            ready = true;
+        }
         if (fetch - ids_base >= 32) {
             ids = ids_next;
             ids_base += 32;
@@ -292,16 +306,16 @@ __global__ void __launch_bounds__(kThreads, 2) fp8_decode_kernel(const __grid_co
         ++fetched;
     };
     for (int s = 0; s < kStages; ++s) issue();
-
-    Rows rows = load_rows(a, lo, lane);
-    int row = advance_row(a, rows, lo, begin, lane);
-    bool beyond = row >= a.batch;  // prefix does not grow from row to row
-    int row_first = 0;
-    uint32_t q[8];
-    if (!beyond) {
-        row_first = a.prefix[row];
-        load_query(a, row, warp * kGroup + g, t, q);
+    if (!ready) {
+        pkv::pdl_wait();
+        ready = true;
     }
+    pkv::pdl_launch_dependents();
+
+    bool beyond = row >= a.batch;  // prefix does not grow from row to row
+    int row_first = __shfl_sync(0xffffffffu, rows.first, row - rows.base);
+    uint32_t q[8];
+    if (!beyond) load_query(a, row, warp * kGroup + g, t, q);
 
     int consumed = 0;
     bool failed = false;
@@ -328,7 +342,7 @@ __global__ void __launch_bounds__(kThreads, 2) fp8_decode_kernel(const __grid_co
         while (i < seg_end) {
             const int n = min(kChunk, seg_end - i);
             const int stage = consumed % kStages;
-            const uint32_t src = ring + stage * kStageBytes;
+            const uint8_t *src = ring_tiles + stage * kStageBytes;
             if (!failed && !pkv::mbar_wait_bounded(bar0 + 8 * stage, (consumed / kStages) & 1, kWaitPolls)) failed = true;
             failed = __any_sync(0xffffffffu, failed);
             if (failed) break;
@@ -336,21 +350,39 @@ __global__ void __launch_bounds__(kThreads, 2) fp8_decode_kernel(const __grid_co
 
             // Scores: lane's rows are tokens 4 j + (g & 1) and 4 j + 2 + (g & 1) of block g / 2.
             float s[4][4];
-            const uint32_t k_at = src + (g >> 1) * kTile + (g & 1) * kDim + 16 * t;
+            const uint8_t *k_at = src + (g >> 1) * kTile + (g & 1) * kDim + 16 * t;
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
-                const uint4 a0 = lds128(k_at + 4 * j * kDim);
-                const uint4 a1 = lds128(k_at + (4 * j + 2) * kDim);
+                const uint4 a0 = *reinterpret_cast<const uint4 *>(k_at + 4 * j * kDim);
+                const uint4 a1 = *reinterpret_cast<const uint4 *>(k_at + (4 * j + 2) * kDim);
                 s[j][0] = s[j][1] = s[j][2] = s[j][3] = 0.f;
 #pragma unroll
                 for (int ks = 0; ks < 4; ++ks) {
                     const uint32_t x = word(a0, ks), y = word(a1, ks);
-                    pkv::mma_f16_16816(s[j], pkv::fp8::decode2(x), pkv::fp8::decode2(y), pkv::fp8::decode2(x >> 16),
-                                       pkv::fp8::decode2(y >> 16), q[2 * ks], q[2 * ks + 1]);
+                    mma(s[j], pkv::fp8::decode2(x), pkv::fp8::decode2(y), pkv::fp8::decode2(x >> 16),
+                        pkv::fp8::decode2(y >> 16), q[2 * ks], q[2 * ks + 1]);
                 }
             }
-            const float key_scale = lds32(src + kScaleAt + (g >> 1) * 16 + warp * 4) * kScaleLog2;
-            const float value_scale = lds32(src + kScaleAt + (kChunk + (g >> 1)) * 16 + warp * 4);
+            const float key_scale =
+                *reinterpret_cast<const float *>(src + kScaleAt + (g >> 1) * 16 + warp * 4) * kScaleLog2;
+            const float value_scale =
+                *reinterpret_cast<const float *>(src + kScaleAt + (kChunk + (g >> 1)) * 16 + warp * 4);
+            uint4 v[4][2];
+#pragma unroll
+            for (int mt = 0; mt < 4; ++mt) {
+                const uint8_t *v_at = src + kValueAt + t * kValuePitch + (16 * mt + g) * 16;
+                v[mt][0] = *reinterpret_cast<const uint4 *>(v_at);
+                v[mt][1] = *reinterpret_cast<const uint4 *>(v_at + 8 * 16);
+            }
+            // Every lane has read the stage (the fence orders the reads before the
+            // copies, the warp barrier the lanes): it is filled again while this
+            // chunk is worked on.
+            pkv::fence_proxy_async_smem();
+            __syncwarp();
+            i += n;
+            ++consumed;
+            issue();
+
             const int ve = ((__float_as_int(value_scale) >> 23) & 0xff) - 127;
             const float shift = static_cast<float>(ve);
             const float unscale = pkv::fp8::exp2_int(-ve);
@@ -406,27 +438,18 @@ __global__ void __launch_bounds__(kThreads, 2) fp8_decode_kernel(const __grid_co
                 o[mt][1] *= alpha1;
                 o[mt][2] *= alpha0;
                 o[mt][3] *= alpha1;
-                uint4 v0 = lds128(src + kValueAt + t * kValuePitch + (16 * mt + g) * 16);
-                uint4 v1 = lds128(src + kValueAt + t * kValuePitch + (16 * mt + 8 + g) * 16);
                 if (!whole) {  // weight 0 times NaN is NaN
                     const int keep = tokens - t * kSlots;
-                    v0 = keep_bytes(v0, keep);
-                    v1 = keep_bytes(v1, keep);
+                    v[mt][0] = keep_bytes(v[mt][0], keep);
+                    v[mt][1] = keep_bytes(v[mt][1], keep);
                 }
 #pragma unroll
                 for (int j = 0; j < 4; ++j) {
-                    const uint32_t x = word(v0, j), y = word(v1, j);
-                    pkv::mma_f16_16816(o[mt], pkv::fp8::decode2(x), pkv::fp8::decode2(y), pkv::fp8::decode2(x >> 16),
-                                       pkv::fp8::decode2(y >> 16), p[j][0], p[j][1]);
+                    const uint32_t x = word(v[mt][0], j), y = word(v[mt][1], j);
+                    mma(o[mt], pkv::fp8::decode2(x), pkv::fp8::decode2(y), pkv::fp8::decode2(x >> 16),
+                        pkv::fp8::decode2(y >> 16), p[j][0], p[j][1]);
                 }
             }
-            // The stage is free: every lane has read it (the reads are ordered
-            // before the copies by the fence and the warp barrier).
-            pkv::fence_proxy_async_smem();
-            __syncwarp();
-            i += n;
-            ++consumed;
-            issue();
         }
         if (failed) break;
 
@@ -476,57 +499,88 @@ __global__ void __launch_bounds__(kThreads, 2) fp8_decode_kernel(const __grid_co
     }
 }
 
-// Merge of the rows that several pieces hold: a warp per (row, two heads), 16
-// lanes a head and four dims a lane, pieces in order, four loaded at a time.
-constexpr int kMergeThreads = 256;
+// Merge of the rows that several pieces hold, sixteen lanes a head and four dims
+// a lane.  With few rows a CTA's eight warps deal out the pieces of one (row, two
+// heads) and the first warp merges the warps' results in order, so a row of 32
+// pieces is four dependent loads deep; with many rows a warp merges a row's few
+// pieces.
+constexpr int kMergeWarps = 8;
+constexpr int kMergeThreads = kMergeWarps * 32;
 
+struct Merge {
+    float M, L, A[4];
+
+    __device__ __forceinline__ void add(float m, float l, const float4 &v) {
+        const float top = fmaxf(M, m);
+        const float x = pkv::exp2_approx(M - top), y = pkv::exp2_approx(m - top);
+        M = top;
+        L = fmaf(L, x, l * y);
+        A[0] = fmaf(A[0], x, v.x * y);
+        A[1] = fmaf(A[1], x, v.y * y);
+        A[2] = fmaf(A[2], x, v.z * y);
+        A[3] = fmaf(A[3], x, v.w * y);
+    }
+};
+
+template <bool SPREAD>
 __global__ void __launch_bounds__(kMergeThreads) fp8_merge_kernel(const __grid_constant__ Args a) {
-    const int pair = blockIdx.x * (kMergeThreads / 32) + (threadIdx.x >> 5);
-    const int lane = threadIdx.x & 31;
+    __shared__ float part[kMergeWarps][32][6];
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int pair = SPREAD ? blockIdx.x : blockIdx.x * kMergeWarps + warp;
     const int row = pair / (kQueryHeads / 2);
     const int head = 2 * (pair % (kQueryHeads / 2)) + (lane >> 4);
     const int dim = 4 * (lane & 15);
     pkv::pdl_launch_dependents();
+    // The tables are older than the split kernel: it lets this one start only after
+    // its own wait for what came before.
+    int first = 0, last = 0;
+    if (row < a.batch) {
+        const int first_block = a.prefix[row], last_block = a.prefix[row + 1] - 1;
+        const int total = total_blocks(a);
+        if (last_block >= first_block && first_block >= 0 && last_block < total) {
+            const int pieces = pieces_of(total, a.grid);
+            first = piece_of(first_block, total, pieces);
+            last = piece_of(last_block, total, pieces);
+        }
+    }
     pkv::pdl_wait();
-    if (row >= a.batch) return;
-    const int first_block = a.prefix[row], last_block = a.prefix[row + 1] - 1;
-    const int total = total_blocks(a);
-    if (last_block < first_block || first_block < 0 || last_block >= total) return;
-    const int pieces = pieces_of(total, a.grid);
-    const int first = piece_of(first_block, total, pieces), last = piece_of(last_block, total, pieces);
     if (first == last) return;
-    float M = kLowest, L = 0.f, A[4] = {0.f, 0.f, 0.f, 0.f};
+    constexpr int kStep = SPREAD ? kMergeWarps : 1;
+    Merge merged{kLowest, 0.f, {0.f, 0.f, 0.f, 0.f}};
     constexpr int kBatch = 4;
-    for (int c0 = first; c0 <= last; c0 += kBatch) {
+    for (int c0 = first + (SPREAD ? warp : 0); c0 <= last; c0 += kBatch * kStep) {
         float2 ml[kBatch];
         float4 v[kBatch];
 #pragma unroll
         for (int j = 0; j < kBatch; ++j) {
-            if (c0 + j <= last) {
-                const int64_t index = (static_cast<int64_t>(row) + c0 + j) * kQueryHeads + head;
+            const int c = c0 + j * kStep;
+            if (c <= last) {
+                const int64_t index = (static_cast<int64_t>(row) + c) * kQueryHeads + head;
                 ml[j] = *reinterpret_cast<const float2 *>(a.part_ml + index * 2);
                 v[j] = *reinterpret_cast<const float4 *>(a.part_o + index * kDim + dim);
             }
         }
 #pragma unroll
         for (int j = 0; j < kBatch; ++j) {
-            if (c0 + j <= last) {
-                const float top = fmaxf(M, ml[j].x);
-                const float x = pkv::exp2_approx(M - top), y = pkv::exp2_approx(ml[j].x - top);
-                M = top;
-                L = fmaf(L, x, ml[j].y * y);
-                A[0] = fmaf(A[0], x, v[j].x * y);
-                A[1] = fmaf(A[1], x, v[j].y * y);
-                A[2] = fmaf(A[2], x, v[j].z * y);
-                A[3] = fmaf(A[3], x, v[j].w * y);
-            }
+            if (c0 + j * kStep <= last) merged.add(ml[j].x, ml[j].y, v[j]);
+        }
+    }
+    if constexpr (SPREAD) {
+        float *mine = part[warp][lane];
+        mine[0] = merged.M, mine[1] = merged.L;
+        mine[2] = merged.A[0], mine[3] = merged.A[1], mine[4] = merged.A[2], mine[5] = merged.A[3];
+        __syncthreads();
+        if (warp != 0) return;
+        for (int w = 1; w < kMergeWarps; ++w) {
+            const float *p = part[w][lane];
+            merged.add(p[0], p[1], make_float4(p[2], p[3], p[4], p[5]));
         }
     }
 #pragma unroll
-    for (int d = 0; d < 4; ++d) A[d] = L == 0.f ? 0.f : __fdiv_rn(A[d], L);
+    for (int d = 0; d < 4; ++d) merged.A[d] = merged.L == 0.f ? 0.f : __fdiv_rn(merged.A[d], merged.L);
     __half2 *dst = reinterpret_cast<__half2 *>(a.out + row * a.out_stride + head * kDim + dim);
-    dst[0] = __floats2half2_rn(A[0], A[1]);
-    dst[1] = __floats2half2_rn(A[2], A[3]);
+    dst[0] = __floats2half2_rn(merged.A[0], merged.A[1]);
+    dst[1] = __floats2half2_rn(merged.A[2], merged.A[3]);
 }
 
 // The rotated queries of pkv_fp8_decode_layer, then the partials.
@@ -562,7 +616,11 @@ int device_info(int device, DeviceInfo *info) {
     }
     if (e == cudaSuccess) {
         // The merge keeps the split kernel's partition of L1 and shared memory.
-        e = cudaFuncSetAttribute(fp8_merge_kernel, cudaFuncAttributePreferredSharedMemoryCarveout,
+        e = cudaFuncSetAttribute(fp8_merge_kernel<false>, cudaFuncAttributePreferredSharedMemoryCarveout,
+                                 cudaSharedmemCarveoutMaxShared);
+    }
+    if (e == cudaSuccess) {
+        e = cudaFuncSetAttribute(fp8_merge_kernel<true>, cudaFuncAttributePreferredSharedMemoryCarveout,
                                  cudaSharedmemCarveoutMaxShared);
     }
     if (e == cudaSuccess) e = cudaOccupancyMaxActiveBlocksPerMultiprocessor(&d.ctas_per_sm, fp8_decode_kernel, kThreads, kSmem);
@@ -642,6 +700,7 @@ int decode(const pkv::fp8::Cache &cache, int32_t layer, const void *query, int64
     a.capacity = total_blocks;
     a.grid = grid;
     a.clear = key == nullptr;
+    a.early = key != nullptr;
     a.out = static_cast<__half *>(out);
     a.out_stride = out_stride;
     a.part_o = partials;
@@ -659,9 +718,13 @@ int decode(const pkv::fp8::Cache &cache, int32_t layer, const void *query, int64
     config.numAttrs = 1;
     e = cudaLaunchKernelEx(&config, fp8_decode_kernel, a);
     if (e == cudaSuccess && grid > 1) {
-        const int64_t warps = static_cast<int64_t>(batch) * (kQueryHeads / 2);
-        e = pkv::launch_pdl(fp8_merge_kernel, dim3(static_cast<unsigned>((warps * 32 + kMergeThreads - 1) / kMergeThreads)),
-                            dim3(kMergeThreads), config.stream, a);
+        // A CTA per (row, two heads) while that is at most two waves of CTAs: beyond it rows
+        // have few pieces each and a warp merges them as fast.
+        const int64_t pairs = static_cast<int64_t>(batch) * (kQueryHeads / 2);
+        const bool spread = pairs <= 16 * info.sms;
+        const auto blocks = static_cast<unsigned>(spread ? pairs : (pairs + kMergeWarps - 1) / kMergeWarps);
+        e = pkv::launch_pdl(spread ? fp8_merge_kernel<true> : fp8_merge_kernel<false>, dim3(blocks), dim3(kMergeThreads),
+                            config.stream, a);
     }
     if (e != cudaSuccess) return pkv::fail(PKV_CUDA_ERROR, std::string("fp8 decode launch failed: ") + cudaGetErrorString(e));
     return PKV_OK;

@@ -227,37 +227,40 @@ __device__ void write_value(const AppendArgs &a, int layer, int head, int token,
 }
 
 __global__ void __launch_bounds__(kThreads) fp8_append_kernel(const __grid_constant__ AppendArgs a) {
-    pkv::pdl_launch_dependents();
+    // In this order: the decode attention behind it reads what is older than this
+    // kernel (the tables, the cache but for the blocks written here) before its own wait.
     pkv::pdl_wait();
+    pkv::pdl_launch_dependents();
     const int token = blockIdx.x;
     const int layer = blockIdx.y;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     if (a.lengths != nullptr && a.prefix[token + 1] <= a.prefix[token]) return;  // a row without blocks
 
     if (a.query_in != nullptr) {
-        // A warp rotates four query heads: eight lanes a head, of which two hold
-        // 16 dims and their partners each.
+        // Eight lanes a query head, eight dims a lane; the partner's dims (32 away)
+        // come from the lane four further.
         const int position = checked_position(a, token);
-        const int64_t in = layer * a.q_layer_stride + token * a.q_token_stride;
-        const int64_t out = layer * a.q_out_layer_stride + token * a.q_out_token_stride;
-        if (lane < 8) {
-            const int at = (4 * warp + (lane >> 1)) * kDim + 16 * (lane & 1);
-            float lo[16], hi[16];
-            load16(a.query_in + in + at, lo);
-            load16(a.query_in + in + at + kHalf, hi);
-            rotate16(a.rope, position, 16 * (lane & 1), lo, hi);
-            __align__(16) __half2 l[8], h[8];
+        const int chunk = lane & 7, at = (4 * warp + (lane >> 3)) * kDim + 8 * chunk;
+        const int64_t in = layer * a.q_layer_stride + token * a.q_token_stride + at;
+        const int64_t out = layer * a.q_out_layer_stride + token * a.q_out_token_stride + at;
+        const uint4 own = *reinterpret_cast<const uint4 *>(a.query_in + in);
+        const __half *factors = a.rope + position * kHalf + 8 * (chunk & 3);
+        const uint4 cos = *reinterpret_cast<const uint4 *>(factors);
+        const uint4 sin = *reinterpret_cast<const uint4 *>(factors + PKV_CONTEXT_LIMIT * kHalf);
+        const float sign = chunk < 4 ? -1.f : 1.f;
+        const uint32_t x[4] = {own.x, own.y, own.z, own.w}, c[4] = {cos.x, cos.y, cos.z, cos.w},
+                       s[4] = {sin.x, sin.y, sin.z, sin.w};
+        uint32_t r[4];
 #pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                l[i] = __floats2half2_rn(lo[2 * i], lo[2 * i + 1]);
-                h[i] = __floats2half2_rn(hi[2 * i], hi[2 * i + 1]);
-            }
-#pragma unroll
-            for (int i = 0; i < 2; ++i) {
-                reinterpret_cast<uint4 *>(a.query_out + out + at)[i] = reinterpret_cast<const uint4 *>(l)[i];
-                reinterpret_cast<uint4 *>(a.query_out + out + at + kHalf)[i] = reinterpret_cast<const uint4 *>(h)[i];
-            }
+        for (int i = 0; i < 4; ++i) {
+            const uint32_t p = __shfl_xor_sync(0xffffffffu, x[i], 4);
+            const float2 xf = __half22float2(*reinterpret_cast<const __half2 *>(&x[i]));
+            const float2 pf = __half22float2(*reinterpret_cast<const __half2 *>(&p));
+            const float2 cf = __half22float2(*reinterpret_cast<const __half2 *>(&c[i]));
+            const float2 sf = __half22float2(*reinterpret_cast<const __half2 *>(&s[i]));
+            r[i] = pkv::pack_half2(__floats2half2_rn(xf.x * cf.x + sign * pf.x * sf.x, xf.y * cf.y + sign * pf.y * sf.y));
         }
+        *reinterpret_cast<uint4 *>(a.query_out + out) = make_uint4(r[0], r[1], r[2], r[3]);
     }
 
     const int slot = slot_of(a, token);

@@ -354,8 +354,9 @@ struct RowsShape {
     static constexpr int kXBytes = kTileRows * kKBlock;
     static constexpr int kStageBytes = kXBytes + N * kKBlock;
     static constexpr int kStages = N == 192 ? 5 : N == 128 ? 6 : 8;
+    static constexpr int kBuffers = N > 128 ? 2 : 4;  // TMEM buffers
     static constexpr int kBufferColumns = N > 128 ? 256 : N;
-    static constexpr int kTmemColumns = 2 * kBufferColumns;
+    static constexpr int kTmemColumns = kBuffers * kBufferColumns;
     static constexpr int kRing = kStages * kStageBytes;
     static constexpr int kPitch = N + 4;  // floats between the rows of a cluster's sums (in the ring)
     static_assert(kTileRows * kPitch * 4 <= kRing, "the sums fit the ring");
@@ -383,7 +384,7 @@ __global__ void __launch_bounds__(RowsShape<N>::kThreads, 1)
                            const LinearArgs a) {
     using S = RowsShape<N>;
     extern __shared__ uint8_t dyn_smem[];
-    __shared__ uint64_t full[S::kStages], empty[S::kStages], tmem_full[2], tmem_empty[2];
+    __shared__ uint64_t full[S::kStages], empty[S::kStages], tmem_full[S::kBuffers], tmem_empty[S::kBuffers];
     __shared__ uint32_t tmem_slot;
 
     const uint32_t raw = pkv::smem_addr(dyn_smem);
@@ -408,7 +409,7 @@ __global__ void __launch_bounds__(RowsShape<N>::kThreads, 1)
             pkv::mbar_init(pkv::smem_addr(&full[s]), 1);
             pkv::mbar_init(pkv::smem_addr(&empty[s]), 1);
         }
-        for (int b = 0; b < 2; ++b) {
+        for (int b = 0; b < S::kBuffers; ++b) {
             pkv::mbar_init(pkv::smem_addr(&tmem_full[b]), 1);
             pkv::mbar_init(pkv::smem_addr(&tmem_empty[b]), S::kEpilogueWarps);
         }
@@ -454,7 +455,7 @@ __global__ void __launch_bounds__(RowsShape<N>::kThreads, 1)
         }
         __syncwarp();
     } else if (warp >= kMma) {
-        // Two issuing warps, one per TMEM buffer: each takes every other K block, so
+        // Two issuing warps: each takes every other K block, so
         // one's waits and issue (about 200 and 50 clocks each) run beside the other's MMAs.
         pkv::pdl_wait();
         if (lane == 0) {
@@ -464,10 +465,11 @@ __global__ void __launch_bounds__(RowsShape<N>::kThreads, 1)
             for (int tile = first_tile; ok && tile < a.tiles; tile += tile_step) {
                 for (int i = 0; i < count; ++i, ++done) {
                     const int st = done % S::kStages;
-                    const int buf = done & 1;
-                    if (buf != warp - kMma) continue;
+                    const int buf = done % S::kBuffers;
+                    if ((done & 1) != warp - kMma) continue;
                     ok = wait_bounded(pkv::smem_addr(&full[st]), (done / S::kStages) & 1, a.error_flag) &&
-                         (done < 2 || wait_bounded(pkv::smem_addr(&tmem_empty[buf]), ((done >> 1) - 1) & 1, a.error_flag));
+                         (done < S::kBuffers ||
+                          wait_bounded(pkv::smem_addr(&tmem_empty[buf]), (done / S::kBuffers - 1) & 1, a.error_flag));
                     if (!ok) break;
                     pkv::tc::fence_after_sync();
                     const uint32_t src = base + st * S::kStageBytes;
@@ -511,8 +513,8 @@ __global__ void __launch_bounds__(RowsShape<N>::kThreads, 1)
 #pragma unroll
                 for (int j = 0; j < 4; ++j) {
                     if (group + j < count) {
-                        const int buf = done & 1;
-                        if (ok) ok = wait_bounded(pkv::smem_addr(&tmem_full[buf]), (done >> 1) & 1, a.error_flag);
+                        const int buf = done % S::kBuffers;
+                        if (ok) ok = wait_bounded(pkv::smem_addr(&tmem_full[buf]), (done / S::kBuffers) & 1, a.error_flag);
                         ok = __all_sync(0xffffffffu, ok);
                         ++done;
                         if (ok) {
