@@ -435,11 +435,11 @@ int pkv_fp8_append_kv(void *key_codes, void *value_codes, void *key_scales, void
                       int64_t q_layer_stride, int64_t q_token_stride, void *query_out, int64_t q_out_layer_stride,
                       int64_t q_out_token_stride, int32_t *error_flag, void *stream);
 
-/* K and V of `count` blocks (device int32) at `layer` as FP16: K [count][16][4][64]
- * at out, V the same at out + kv_stride elements. */
+/* K and V of `count` blocks (device int32) at `layer` as FP16 [count][16][4][64]
+ * each, 16-byte aligned. */
 int pkv_fp8_read_blocks(const void *key_codes, const void *value_codes, const void *key_scales,
                         const void *value_scales, int32_t layers, int32_t num_blocks, int32_t layer,
-                        const int32_t *blocks, int32_t count, void *out, int64_t kv_stride, int32_t *error_flag,
+                        const int32_t *blocks, int32_t count, void *key_out, void *value_out, int32_t *error_flag,
                         void *stream);
 
 /* pkv_prefill_attention over the 8-bit cache: same arguments and result over the

@@ -124,7 +124,7 @@ SIGNATURES: dict[str, tuple[object, list[object]]] = {
     ),
     "pkv_fp8_read_blocks": (
         c_int,
-        [*_FP8_CACHE, c_int32, c_void_p, c_int32, c_void_p, c_int64, c_void_p, c_void_p],
+        [*_FP8_CACHE, c_int32, c_void_p, c_int32, c_void_p, c_void_p, c_void_p, c_void_p],
     ),
     "pkv_fp8_prefill_attention": (
         c_int,

@@ -282,16 +282,15 @@ __global__ void __launch_bounds__(kThreads) fp8_append_kernel(const __grid_const
     }
 }
 
-// K and V of `blocks` as FP16: element (kv, i, slot, head, dim) at
-// out + kv * kv_stride + ((i * 16 + slot) * 4 + head) * 64 + dim.  One CTA per
-// block: K code rows go straight across; V tiles turn around in shared memory.
-// index_out (nullable) receives 0 .. count - 1, the block table of `out` as a pool.
+// K and V of `blocks` as FP16, each [i][slot][head][dim].  One CTA per block: K code rows go straight across; V tiles turn around in shared memory.
+// index_out (nullable) receives 0 .. count - 1, the block table of the outputs as a pool.
 constexpr int kReadThreads = 256;
 constexpr int64_t kBlockValues = kSlots * kHeads * kDim;
 
 __global__ void __launch_bounds__(kReadThreads)
     fp8_read_kernel(const pkv::fp8::Cache cache, int layer, const int32_t *__restrict__ blocks,
-                    __half *__restrict__ out, int64_t kv_stride, int32_t *__restrict__ index_out, int32_t *error_flag) {
+                    __half *__restrict__ key_out, __half *__restrict__ value_out, int32_t *__restrict__ index_out,
+                    int32_t *error_flag) {
     __shared__ __align__(16) __half turned[kHeads][kSlots][kDim + 8];
     pkv::pdl_launch_dependents();
     pkv::pdl_wait();
@@ -310,7 +309,7 @@ __global__ void __launch_bounds__(kReadThreads)
         ks = cache.key_scales[tile];
         vs = cache.value_scales[tile];
     }
-    __half *dst = out + static_cast<int64_t>(blockIdx.x) * kSlots * kHeads * kDim;
+    const int64_t at = static_cast<int64_t>(blockIdx.x) * kBlockValues;
     const uint32_t kw[4] = {k.x, k.y, k.z, k.w}, vw[4] = {v.x, v.y, v.z, v.w};
     __align__(16) __half2 row[8];
 #pragma unroll
@@ -321,13 +320,13 @@ __global__ void __launch_bounds__(kReadThreads)
         turned[head][2 * i][part] = __float2half_rn(g.x * vs);  // part is the dim
         turned[head][2 * i + 1][part] = __float2half_rn(g.y * vs);
     }
-    uint4 *kd = reinterpret_cast<uint4 *>(dst + ((part >> 2) * kHeads + head) * kDim + (part & 3) * 16);
+    uint4 *kd = reinterpret_cast<uint4 *>(key_out + at + ((part >> 2) * kHeads + head) * kDim + (part & 3) * 16);
     kd[0] = reinterpret_cast<const uint4 *>(row)[0];
     kd[1] = reinterpret_cast<const uint4 *>(row)[1];
     __syncthreads();
     for (int i = threadIdx.x; i < kSlots * kHeads * kDim / 8; i += kReadThreads) {
         const int h = (i >> 3) & 3, slot = i >> 5, chunk = i & 7;
-        reinterpret_cast<uint4 *>(dst + kv_stride)[i] =
+        reinterpret_cast<uint4 *>(value_out + at)[i] =
             *reinterpret_cast<const uint4 *>(&turned[h][slot][8 * chunk]);
     }
 }
@@ -446,15 +445,15 @@ extern "C" int pkv_fp8_append_kv(void *key_codes, void *value_codes, void *key_s
 namespace {
 
 int read_blocks(const void *key_codes, const void *value_codes, const void *key_scales, const void *value_scales,
-                int32_t layers, int32_t num_blocks, int32_t layer, const int32_t *blocks, int32_t count, void *out,
-                int64_t kv_stride, int32_t *index_out, int32_t *error_flag, void *stream) {
+                int32_t layers, int32_t num_blocks, int32_t layer, const int32_t *blocks, int32_t count, void *key_out,
+                void *value_out, int32_t *index_out, int32_t *error_flag, void *stream) {
     const int rc = pkv::fp8::check_cache(key_codes, value_codes, key_scales, value_scales, layers, num_blocks, layer, 1);
     if (rc) return rc;
-    if (blocks == nullptr || out == nullptr || error_flag == nullptr || count < 0) {
-        return pkv::fail(PKV_VALUE_ERROR, "fp8 read: blocks, out and error_flag are required");
+    if (blocks == nullptr || key_out == nullptr || value_out == nullptr || error_flag == nullptr || count < 0) {
+        return pkv::fail(PKV_VALUE_ERROR, "fp8 read: blocks, outputs and error_flag are required");
     }
-    if (!aligned16(out) || kv_stride % 8 || kv_stride < static_cast<int64_t>(count) * kBlockValues) {
-        return pkv::fail(PKV_VALUE_ERROR, "fp8 read: out must be 16-byte aligned with K before V");
+    if (!aligned16(key_out) || !aligned16(value_out)) {
+        return pkv::fail(PKV_VALUE_ERROR, "fp8 read: the outputs must be 16-byte aligned");
     }
     if (count == 0) return PKV_OK;
     const pkv::fp8::Cache cache{static_cast<uint8_t *>(const_cast<void *>(key_codes)),
@@ -463,7 +462,7 @@ int read_blocks(const void *key_codes, const void *value_codes, const void *key_
                                 static_cast<float *>(const_cast<void *>(value_scales)), layers, num_blocks};
     const cudaError_t e =
         pkv::launch_pdl(fp8_read_kernel, dim3(count), dim3(kReadThreads), static_cast<cudaStream_t>(stream), cache,
-                        layer, blocks, static_cast<__half *>(out), kv_stride, index_out, error_flag);
+                        layer, blocks, static_cast<__half *>(key_out), static_cast<__half *>(value_out), index_out, error_flag);
     if (e != cudaSuccess) return pkv::fail(PKV_CUDA_ERROR, std::string("fp8 read launch failed: ") + cudaGetErrorString(e));
     return PKV_OK;
 }
@@ -472,11 +471,11 @@ int read_blocks(const void *key_codes, const void *value_codes, const void *key_
 
 extern "C" int pkv_fp8_read_blocks(const void *key_codes, const void *value_codes, const void *key_scales,
                                    const void *value_scales, int32_t layers, int32_t num_blocks, int32_t layer,
-                                   const int32_t *blocks, int32_t count, void *out, int64_t kv_stride,
+                                   const int32_t *blocks, int32_t count, void *key_out, void *value_out,
                                    int32_t *error_flag, void *stream) {
     pkv::clear_error();
-    return read_blocks(key_codes, value_codes, key_scales, value_scales, layers, num_blocks, layer, blocks, count, out,
-                       kv_stride, nullptr, error_flag, stream);
+    return read_blocks(key_codes, value_codes, key_scales, value_scales, layers, num_blocks, layer, blocks, count,
+                       key_out, value_out, nullptr, error_flag, stream);
 }
 
 // The request's blocks become an FP16 pool of one layer in the workspace (the
@@ -499,7 +498,8 @@ extern "C" int pkv_fp8_prefill_attention(const void *key_codes, const void *valu
     }
     int32_t *const table = reinterpret_cast<int32_t *>(static_cast<uint8_t *>(workspace) + pool_bytes);
     const int rc = read_blocks(key_codes, value_codes, key_scales, value_scales, layers, num_blocks, layer, blocks, count,
-                               workspace, count * kBlockValues, table, error_flag, stream);
+                               workspace, static_cast<__half *>(workspace) + count * kBlockValues, table, error_flag,
+                               stream);
     if (rc) return rc;
     return pkv_prefill_attention(workspace, count, 0, query, query_stride, table, start, tokens, out, out_stride,
                                  error_flag, stream);

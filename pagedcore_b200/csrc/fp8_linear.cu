@@ -81,7 +81,7 @@ struct LinearArgs {
 };
 
 __device__ __forceinline__ bool wait_bounded(uint32_t bar, uint32_t parity, int32_t *error_flag) {
-    if (pkv::mbar_wait_bounded(bar, parity, kWaitPolls)) return true;
+    if (pkv::mbar_test_wait(bar, parity) || pkv::mbar_wait_bounded(bar, parity, kWaitPolls)) return true;
     atomicOr(error_flag, PKV_DEVICE_WAIT_TIMEOUT);
     return false;
 }
@@ -117,8 +117,23 @@ __device__ __forceinline__ float4 ld_cluster_f4(uint32_t addr) {
     float4 v;
     asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];"
                  : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w)
-                 : "r"(addr)
-                 : "memory");
+                 : "r"(addr));
+    return v;
+}
+
+// The sum over the cluster's CTAs of the four FP32 values at `addr`, in rank
+// order; every rank's load is under way before the first is used.
+__device__ __forceinline__ float4 cluster_sum(uint32_t addr, int splits) {
+    float4 part[kMaxCluster];
+#pragma unroll
+    for (int s = 0; s < kMaxCluster; ++s) {
+        if (s < splits) part[s] = ld_cluster_f4(map_to_rank(addr, s));
+    }
+    float4 v = part[0];
+#pragma unroll
+    for (int s = 1; s < kMaxCluster; ++s) {
+        if (s < splits) v.x += part[s].x, v.y += part[s].y, v.z += part[s].z, v.w += part[s].w;
+    }
     return v;
 }
 
@@ -139,7 +154,7 @@ __device__ __forceinline__ void store4(const LinearArgs &a, int m, int n, const 
 }
 
 template <int NT>
-__global__ void __launch_bounds__(Shape<NT>::kThreads, 1)
+__global__ void __launch_bounds__(Shape<NT>::kThreads, 2)
     fp8_linear_kernel(const __grid_constant__ CUtensorMap w_map, const __grid_constant__ CUtensorMap x_map,
                       const LinearArgs a) {
     using S = Shape<NT>;
@@ -313,20 +328,15 @@ __global__ void __launch_bounds__(Shape<NT>::kThreads, 1)
     } else {
         __syncthreads();
     }
-    // Rank r adds and writes columns r, r + splits, ...: a warp a column, four weight rows a lane.
-    for (int c = split + a.splits * warp; c < NT && m0 + c < a.rows; c += a.splits * (S::kThreads / 32)) {
-        const uint32_t at = static_cast<uint32_t>((c * kTileRows + 4 * lane) * 4);
-        float4 v;
-        if (a.splits == 1) {
-            v = *reinterpret_cast<const float4 *>(reinterpret_cast<const uint8_t *>(sums) + at);
-        } else {
-            v = ld_cluster_f4(map_to_rank(base + at, 0));
-            for (int s = 1; s < a.splits; ++s) {
-                const float4 u = ld_cluster_f4(map_to_rank(base + at, s));
-                v.x += u.x, v.y += u.y, v.z += u.z, v.w += u.w;
-            }
-        }
-        store4(a, m0 + c, n0 + 4 * lane, v);
+    // Rank r adds and writes columns r, r + splits, ...: four weight rows a thread.
+    const int columns = min(NT, a.rows);
+    for (int item = threadIdx.x;; item += S::kThreads) {
+        const int c = split + a.splits * (item / (kTileRows / 4)), r = 4 * (item % (kTileRows / 4));
+        if (c >= columns) break;
+        const uint32_t at = static_cast<uint32_t>((c * kTileRows + r) * 4);
+        store4(a, m0 + c, n0 + r,
+               a.splits == 1 ? *reinterpret_cast<const float4 *>(reinterpret_cast<const uint8_t *>(sums) + at)
+                             : cluster_sum(base + at, a.splits));
     }
     if (a.splits > 1) {  // no CTA leaves while another reads its sums
         cluster_arrive();
@@ -375,6 +385,53 @@ __device__ __forceinline__ void add_scaled(uint64_t *acc, const uint32_t (&d)[32
 #pragma unroll
     for (int j = 0; j < 16; ++j) {
         acc[j] = pkv::fma_f32x2(pkv::f32x2(__uint_as_float(d[2 * j]), __uint_as_float(d[2 * j + 1])), f, acc[j]);
+    }
+}
+
+// A warp's 32 rows x 64 columns of sums (row = lane, `acc` two columns a pair)
+// rounded and stored at row m, column n: 32 columns at a time through the warp's
+// own 2 KiB of shared memory (16-byte chunk c of row r at chunk c ^ (r / 2 % 4): no
+// bank conflicts), then 64 bytes a row.
+__device__ __forceinline__ void store_rows(const LinearArgs &a, const uint64_t *acc, uint32_t staging, int m, int n,
+                                           int lane) {
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+#pragma unroll
+        for (int c = 0; c < 4; ++c) {
+            uint32_t w[4];
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                const float2 v = pkv::unpack_f32x2(acc[16 * h + 4 * c + j]);
+                w[j] = pkv::pack_half2(__floats2half2_rn(v.x, v.y));
+            }
+            asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(staging + lane * 64 + ((c ^ ((lane >> 1) & 3)) << 4)),
+                         "r"(w[0]), "r"(w[1]), "r"(w[2]), "r"(w[3])
+                         : "memory");
+        }
+        __syncwarp();
+#pragma unroll
+        for (int part = 0; part < 4; ++part) {
+            const int r = part * 8 + (lane >> 2), c = lane & 3;
+            uint32_t w[4];
+            asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];"
+                         : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3])
+                         : "r"(staging + r * 64 + ((c ^ ((r >> 1) & 3)) << 4))
+                         : "memory");
+            const int at = n + 32 * h + 8 * c;
+            if (m + r < a.rows && at < a.n) {
+                __half *dst = a.out + static_cast<int64_t>(m + r) * a.out_stride + at;
+                if (a.vector_out && at + 8 <= a.n) {
+                    *reinterpret_cast<uint4 *>(dst) = make_uint4(w[0], w[1], w[2], w[3]);
+                } else {
+                    const __half *v = reinterpret_cast<const __half *>(w);
+#pragma unroll
+                    for (int j = 0; j < 8; ++j) {
+                        if (at + j < a.n) dst[j] = v[j];
+                    }
+                }
+            }
+        }
+        __syncwarp();
     }
 }
 
@@ -535,54 +592,14 @@ __global__ void __launch_bounds__(RowsShape<N>::kThreads, 1)
                 }
             }
             if (a.splits == 1) {
-                // 32 columns at a time through the warp's own staging (16-byte chunk c of
-                // row r at chunk c ^ (r / 2 % 4): no bank conflicts), then 64 bytes a row.
-#pragma unroll
-                for (int h = 0; h < 2; ++h) {
-#pragma unroll
-                    for (int c = 0; c < 4; ++c) {
-                        uint32_t w[4];
-#pragma unroll
-                        for (int j = 0; j < 4; ++j) {
-                            const float2 v = pkv::unpack_f32x2(acc[16 * h + 4 * c + j]);
-                            w[j] = pkv::pack_half2(__floats2half2_rn(v.x, v.y));
-                        }
-                        asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(staging + lane * 64 + ((c ^ ((lane >> 1) & 3)) << 4)),
-                                     "r"(w[0]), "r"(w[1]), "r"(w[2]), "r"(w[3])
-                                     : "memory");
-                    }
-                    __syncwarp();
-#pragma unroll
-                    for (int part = 0; part < 4; ++part) {
-                        const int r = part * 8 + (lane >> 2), c = lane & 3;
-                        uint32_t w[4];
-                        asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];"
-                                     : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3])
-                                     : "r"(staging + r * 64 + ((c ^ ((r >> 1) & 3)) << 4))
-                                     : "memory");
-                        const int m = m0 + quarter * 32 + r, n = n0 + first + 32 * h + 8 * c;
-                        if (m < a.rows && n < a.n) {
-                            __half *dst = a.out + static_cast<int64_t>(m) * a.out_stride + n;
-                            if (a.vector_out && n + 8 <= a.n) {
-                                *reinterpret_cast<uint4 *>(dst) = make_uint4(w[0], w[1], w[2], w[3]);
-                            } else {
-                                const __half *v = reinterpret_cast<const __half *>(w);
-#pragma unroll
-                                for (int j = 0; j < 8; ++j) {
-                                    if (n + j < a.n) dst[j] = v[j];
-                                }
-                            }
-                        }
-                    }
-                    __syncwarp();
-                }
+                store_rows(a, acc, staging, m0 + quarter * 32, n0 + first, lane);
             }
         }
     }
 
     if (a.splits > 1) {
         // One tile per cluster: each CTA leaves its sums in its ring, and rank r adds
-        // and writes rows r, r + splits, ...
+        // and writes rows r, r + splits, ..., four columns a thread.
         __syncthreads();  // every copy has landed and every MMA has been read (or given up on)
         const int m0 = first_tile % a.m_tiles * kTileRows, n0 = first_tile / a.m_tiles * N;
         if (warp < S::kEpilogueWarps) {
@@ -597,16 +614,11 @@ __global__ void __launch_bounds__(RowsShape<N>::kThreads, 1)
         }
         cluster_arrive();
         cluster_wait();
-        for (int r = split + a.splits * warp; r < kTileRows && m0 + r < a.rows; r += a.splits * (S::kThreads / 32)) {
-            for (int c = 4 * lane; c < N && n0 + c < a.n; c += 128) {
-                const uint32_t at = base + (r * S::kPitch + c) * 4;
-                float4 v = ld_cluster_f4(map_to_rank(at, 0));
-                for (int s = 1; s < a.splits; ++s) {
-                    const float4 u = ld_cluster_f4(map_to_rank(at, s));
-                    v.x += u.x, v.y += u.y, v.z += u.z, v.w += u.w;
-                }
-                store4(a, m0 + r, n0 + c, v);
-            }
+        const int rows = min(kTileRows, a.rows - m0);
+        for (int item = threadIdx.x;; item += S::kThreads) {
+            const int r = split + a.splits * (item / (N / 4)), c = 4 * (item % (N / 4));
+            if (r >= rows) break;
+            if (n0 + c < a.n) store4(a, m0 + r, n0 + c, cluster_sum(base + (r * S::kPitch + c) * 4, a.splits));
         }
         cluster_arrive();  // no CTA leaves while another reads its sums
         cluster_wait();
@@ -616,6 +628,229 @@ __global__ void __launch_bounds__(RowsShape<N>::kThreads, 1)
     if (warp == kMma) {
         pkv::tc::fence_after_sync();
         pkv::tc::tmem_dealloc(tmem, S::kTmemColumns);
+    }
+}
+
+// ---------------------------------------------------------------------------
+// Many rows, large: pairs of CTAs (cta_group::2) on tiles of 256 rows of x by 256
+// weight rows.  Each CTA loads its own 128 rows of x and half of the weight rows and
+// holds the sums of its rows, so a K block costs an SM 32 KiB of L2 traffic for
+// 128 x 256 outputs, half of what the kernel above takes; that traffic is what
+// bounds the latter.  CTA 0 of a pair (the leader) issues the MMAs of both; the
+// barriers that it waits on (full, tmem_empty) live in its shared memory and the other
+// CTA's loads and epilogue signal them there, and its commits signal empty and
+// tmem_full in both.  Sixteen epilogue warps, 64 columns each; persistent.
+// ---------------------------------------------------------------------------
+struct PairShape {
+    static constexpr int kN = 256;
+    static constexpr int kEpilogueWarps = 16;
+    static constexpr int kThreads = (kEpilogueWarps + 3) * 32;
+    static constexpr int kXBytes = kTileRows * kKBlock;
+    static constexpr int kStageBytes = kXBytes + kN / 2 * kKBlock;
+    static constexpr int kStages = 6;
+    static constexpr int kStoreBytes = 32 * 64;
+    static constexpr int kRing = kStages * kStageBytes;
+    static constexpr int kSmem = kRing + kEpilogueWarps * kStoreBytes + 1024;
+};
+
+__device__ __forceinline__ void mma_f8_pair(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc, uint32_t idesc,
+                                            bool accumulate) {
+    const uint32_t acc = accumulate ? 1u : 0u;
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "setp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::2.kind::f8f6f4 [%0], %1, %2, %3, p;\n\t}"
+        ::"r"(d_tmem), "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(acc)
+        : "memory");
+}
+
+// The barrier at this offset in both CTAs of the pair receives one arrival once
+// the MMAs issued before have completed.
+__device__ __forceinline__ void commit_pair(uint32_t bar) {
+    asm volatile(
+        "tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(bar),
+        "h"(static_cast<uint16_t>(3))
+        : "memory");
+}
+
+// A box into this CTA's shared memory that completes on the leader's barrier (`bar`
+// in the cluster's address space); no multicast.
+__device__ __forceinline__ void tma_load_pair(uint32_t dst, const CUtensorMap *map, int32_t c0, int32_t c1,
+                                              uint32_t bar) {
+    asm volatile(
+        "cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes"
+        " [%0], [%1, {%2, %3}], [%4];" ::"r"(dst),
+        "l"(reinterpret_cast<uint64_t>(map)), "r"(c0), "r"(c1), "r"(bar)
+        : "memory");
+}
+
+__device__ __forceinline__ void arrive_cluster(uint32_t bar) {
+    asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
+}
+
+__global__ void __launch_bounds__(PairShape::kThreads, 1)
+    fp8_linear_pair_kernel(const __grid_constant__ CUtensorMap w_map, const __grid_constant__ CUtensorMap x_map,
+                           const LinearArgs a) {
+    using S = PairShape;
+    extern __shared__ uint8_t dyn_smem[];
+    __shared__ uint64_t full[S::kStages], empty[S::kStages], tmem_full[2], tmem_empty[2];
+    __shared__ uint32_t tmem_slot;
+
+    const uint32_t raw = pkv::smem_addr(dyn_smem);
+    const uint32_t base = (raw + 1023u) & ~1023u;  // the same offset in both CTAs
+    const int rank = static_cast<int>(blockIdx.x) & 1;
+    const int first_tile = static_cast<int>(blockIdx.x) >> 1;
+    const int tile_step = static_cast<int>(gridDim.x) >> 1;
+    const int count = a.k_blocks;
+    const int warp = threadIdx.x >> 5;
+    const int lane = threadIdx.x & 31;
+    constexpr int kProducer = S::kEpilogueWarps;
+    constexpr int kMma = S::kEpilogueWarps + 1;
+
+    if (warp == kMma) {
+        asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(pkv::smem_addr(&tmem_slot)),
+                     "r"(512)
+                     : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
+    }
+    if (threadIdx.x == kProducer * 32) {
+        for (int s = 0; s < S::kStages; ++s) {
+            pkv::mbar_init(pkv::smem_addr(&full[s]), 1);
+            pkv::mbar_init(pkv::smem_addr(&empty[s]), 1);
+        }
+        for (int b = 0; b < 2; ++b) {
+            pkv::mbar_init(pkv::smem_addr(&tmem_full[b]), 1);
+            pkv::mbar_init(pkv::smem_addr(&tmem_empty[b]), 2 * S::kEpilogueWarps);
+        }
+        pkv::fence_barrier_init();
+    }
+    pkv::tc::fence_before_sync();
+    cluster_arrive();  // both CTAs' barriers and TMEM are ready
+    cluster_wait();
+    pkv::tc::fence_after_sync();
+    const uint32_t tmem = tmem_slot;
+    pkv::pdl_launch_dependents();
+
+    if (warp == kProducer) {
+        pkv::pdl_wait();
+        if (lane == 0) {
+            int issued = 0;
+            bool ok = true;
+            for (int tile = first_tile; ok && tile < a.tiles; tile += tile_step) {
+                const int m0 = tile % a.m_tiles * 256 + rank * 128, n0 = tile / a.m_tiles * S::kN + rank * 128;
+                for (int i = 0; i < count; ++i) {
+                    const int st = issued % S::kStages;
+                    if (issued >= S::kStages &&
+                        !wait_bounded(pkv::smem_addr(&empty[st]), ((issued / S::kStages) - 1) & 1, a.error_flag)) {
+                        ok = false;
+                        break;
+                    }
+                    const uint32_t dst = base + st * S::kStageBytes;
+                    if (rank == 0) pkv::mbar_arrive_expect_tx(pkv::smem_addr(&full[st]), 2 * S::kStageBytes);
+                    const uint32_t bar = map_to_rank(pkv::smem_addr(&full[st]), 0);
+                    tma_load_pair(dst, &x_map, i * kKBlock, m0, bar);
+                    tma_load_pair(dst + S::kXBytes, &w_map, i * kKBlock, n0, bar);
+                    ++issued;
+                }
+            }
+            // No copy may land after the CTA has left: every stage has been multiplied
+            // (or, where a wait ran out, long since filled).
+            for (int i = max(0, issued - S::kStages); i < issued; ++i) {
+                wait_bounded(pkv::smem_addr(&empty[i % S::kStages]), (i / S::kStages) & 1, a.error_flag);
+            }
+        }
+        __syncwarp();
+    } else if (warp >= kMma) {
+        pkv::pdl_wait();
+        if (rank == 0 && lane == 0) {
+            constexpr uint32_t idesc = idesc_e4m3_f32(256, S::kN);
+            int done = 0;
+            bool ok = true;
+            for (int tile = first_tile; ok && tile < a.tiles; tile += tile_step) {
+                for (int i = 0; i < count; ++i, ++done) {
+                    const int st = done % S::kStages;
+                    const int buf = done & 1;
+                    if (buf != warp - kMma) continue;  // two issuing warps, one per TMEM buffer
+                    ok = wait_bounded(pkv::smem_addr(&full[st]), (done / S::kStages) & 1, a.error_flag) &&
+                         (done < 2 || wait_bounded(pkv::smem_addr(&tmem_empty[buf]), ((done >> 1) - 1) & 1, a.error_flag));
+                    if (!ok) break;
+                    pkv::tc::fence_after_sync();
+                    const uint32_t src = base + st * S::kStageBytes;
+#pragma unroll
+                    for (int k = 0; k < kKBlock / 32; ++k) {
+                        mma_f8_pair(tmem + buf * 256, pkv::tc::desc_k_major_sw128(src + 32 * k),
+                                    pkv::tc::desc_k_major_sw128(src + S::kXBytes + 32 * k), idesc, k > 0);
+                    }
+                    commit_pair(pkv::smem_addr(&empty[st]));
+                    commit_pair(pkv::smem_addr(&tmem_full[buf]));
+                }
+            }
+        }
+        __syncwarp();
+    } else {
+        pkv::pdl_wait();
+        const int quarter = warp & 3, first = (warp >> 2) * 64;
+        const uint32_t src = tmem + (static_cast<uint32_t>(quarter * 32) << 16) + first;
+        const uint32_t staging = base + S::kRing + warp * S::kStoreBytes;
+        const uint32_t empty0 = map_to_rank(pkv::smem_addr(&tmem_empty[0]), 0);
+        uint64_t acc[32];
+        int done = 0;
+        bool ok = true;
+        for (int tile = first_tile; tile < a.tiles; tile += tile_step) {
+            const int m0 = tile % a.m_tiles * 256 + rank * 128, n0 = tile / a.m_tiles * S::kN;
+            const float *sx = a.x_scales + static_cast<int64_t>(min(m0 + quarter * 32 + lane, a.rows - 1)) * count;
+            const float *sw = a.w_scales + static_cast<int64_t>(min((n0 + first) / kTileRows, a.w_blocks - 1)) * count;
+            // Scales two K blocks ahead, in registers of their own for even and odd blocks.
+            float x[2], w[2];
+            x[0] = __ldg(sx), w[0] = __ldg(sw);
+            x[1] = w[1] = 0.f;
+            if (count > 1) x[1] = __ldg(sx + 1), w[1] = __ldg(sw + 1);
+#pragma unroll
+            for (int c = 0; c < 32; ++c) acc[c] = 0;
+            for (int i = 0; i < count; i += 2) {
+#pragma unroll
+                for (int odd = 0; odd < 2; ++odd) {
+                    if (i + odd < count) {
+                        const int buf = done & 1;
+                        const float f = x[odd] * w[odd];
+                        const uint64_t f2 = pkv::f32x2(f, f);
+                        if (i + odd + 2 < count) x[odd] = __ldg(sx + i + odd + 2), w[odd] = __ldg(sw + i + odd + 2);
+                        if (ok) ok = wait_bounded(pkv::smem_addr(&tmem_full[buf]), (done >> 1) & 1, a.error_flag);
+                        ok = __all_sync(0xffffffffu, ok);
+                        ++done;
+                        if (ok) {
+                            pkv::tc::fence_after_sync();
+#pragma unroll
+                            for (int c = 0; c < 4; ++c) {
+                                uint32_t d[16];
+                                pkv::tc::tmem_ld16(src + buf * 256 + 16 * c, d);
+                                pkv::tc::tmem_wait_ld();
+                                if (c == 3) {
+                                    pkv::tc::fence_before_sync();
+                                    __syncwarp();
+                                    if (lane == 0) arrive_cluster(empty0 + 8 * buf);
+                                }
+#pragma unroll
+                                for (int j = 0; j < 8; ++j) {
+                                    acc[8 * c + j] = pkv::fma_f32x2(
+                                        pkv::f32x2(__uint_as_float(d[2 * j]), __uint_as_float(d[2 * j + 1])), f2,
+                                        acc[8 * c + j]);
+                                }
+                            }
+                        }
+                    }
+                }
+            }
+            store_rows(a, acc, staging, m0 + quarter * 32, n0 + first, lane);
+        }
+    }
+    __syncwarp();
+    pkv::tc::fence_before_sync();
+    cluster_arrive();  // neither CTA leaves while the other's MMAs or arrivals need it
+    cluster_wait();
+    if (warp == kMma) {
+        pkv::tc::fence_after_sync();
+        asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512) : "memory");
     }
 }
 
@@ -694,7 +929,7 @@ int prepare(const void *kernel, int smem, int device, std::atomic<int> *prepared
 using Kernel = void (*)(CUtensorMap, CUtensorMap, LinearArgs);
 
 int launch_kernel(Kernel kernel, int grid, int threads, int smem, const CUtensorMap &w_map, const CUtensorMap &x_map,
-                  const LinearArgs &args, cudaStream_t stream) {
+                  const LinearArgs &args, int cluster, cudaStream_t stream) {
     cudaLaunchConfig_t config = {};
     config.gridDim = dim3(grid);
     config.blockDim = dim3(threads);
@@ -704,11 +939,11 @@ int launch_kernel(Kernel kernel, int grid, int threads, int smem, const CUtensor
     attributes[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
     attributes[0].val.programmaticStreamSerializationAllowed = 1;
     attributes[1].id = cudaLaunchAttributeClusterDimension;
-    attributes[1].val.clusterDim.x = static_cast<unsigned>(args.splits);
+    attributes[1].val.clusterDim.x = static_cast<unsigned>(cluster);
     attributes[1].val.clusterDim.y = 1;
     attributes[1].val.clusterDim.z = 1;
     config.attrs = attributes;
-    config.numAttrs = args.splits > 1 ? 2 : 1;
+    config.numAttrs = cluster > 1 ? 2 : 1;
     const cudaError_t e = cudaLaunchKernelEx(&config, kernel, w_map, x_map, args);
     if (e != cudaSuccess) return pkv::fail(PKV_CUDA_ERROR, std::string("fp8 linear launch failed: ") + cudaGetErrorString(e));
     return PKV_OK;
@@ -724,11 +959,16 @@ int operand_maps(const void *x, int64_t x_stride, int x_box, const void *w, int 
 }
 
 // CTAs that share a tile's K blocks: as many as still find free SMs, each keeping a block.
-int row_splits(int64_t tiles, int k_blocks, int slots) {
+int row_splits(int64_t tiles, int k_blocks, int slots, int most) {
     int splits = 1;
-    while (splits < kMaxCluster && tiles * splits * 2 <= slots && k_blocks >= 2 * splits) splits *= 2;
+    while (splits < most && tiles * splits * 2 <= slots && k_blocks >= 2 * splits) splits *= 2;
     return splits;
 }
+
+// Largest cluster of the kernel for many rows, which takes a whole SM a CTA: clusters of
+// eight left SMs of a GPC idle and ran in two waves (128 x 2048 x 2048: 13.3 us, 8.0
+// with four).
+constexpr int kRowsCluster = 4;
 
 template <int NT>
 int launch_few(int device, const void *x, int64_t x_stride, const void *w, int32_t k, int sms, LinearArgs &args,
@@ -739,11 +979,12 @@ int launch_few(int device, const void *x, int64_t x_stride, const void *w, int32
     if (rc) return rc;
     CUtensorMap w_map, x_map;
     if ((rc = operand_maps(x, x_stride, NT, w, kTileRows, k, args, &w_map, &x_map))) return rc;
-    args.splits = row_splits(args.n_tiles, args.k_blocks, sms + sms / 8);
+    args.splits = row_splits(args.n_tiles, args.k_blocks, sms + sms / 8, kMaxCluster);
     if (static_cast<int64_t>(args.n_tiles) * args.splits > INT32_MAX) {
         return pkv::fail(PKV_VALUE_ERROR, "fp8 linear: too many tiles");
     }
-    return launch_kernel(fp8_linear_kernel<NT>, args.n_tiles * args.splits, S::kThreads, S::kSmem, w_map, x_map, args, stream);
+    return launch_kernel(fp8_linear_kernel<NT>, args.n_tiles * args.splits, S::kThreads, S::kSmem, w_map, x_map, args,
+                         args.splits, stream);
 }
 
 template <int N>
@@ -760,9 +1001,28 @@ int launch_rows(int device, const void *x, int64_t x_stride, const void *w, int3
     if (tiles > INT32_MAX / kMaxCluster) return pkv::fail(PKV_VALUE_ERROR, "fp8 linear: too many tiles");
     args.m_tiles = static_cast<int32_t>(m_tiles);
     args.tiles = static_cast<int32_t>(tiles);
-    args.splits = row_splits(tiles, args.k_blocks, sms);
+    args.splits = row_splits(tiles, args.k_blocks, sms, kRowsCluster);
     const int64_t grid = args.splits > 1 ? tiles * args.splits : tiles < sms ? tiles : sms;
-    return launch_kernel(fp8_linear_rows_kernel<N>, static_cast<int>(grid), S::kThreads, S::kSmem, w_map, x_map, args, stream);
+    return launch_kernel(fp8_linear_rows_kernel<N>, static_cast<int>(grid), S::kThreads, S::kSmem, w_map, x_map, args,
+                         args.splits, stream);
+}
+
+int launch_pairs(int device, const void *x, int64_t x_stride, const void *w, int32_t k, int sms, LinearArgs &args,
+                 cudaStream_t stream) {
+    using S = PairShape;
+    static std::atomic<int> prepared[kMaxDevices] = {};
+    int rc = prepare(reinterpret_cast<const void *>(fp8_linear_pair_kernel), S::kSmem, device, prepared);
+    if (rc) return rc;
+    CUtensorMap w_map, x_map;
+    if ((rc = operand_maps(x, x_stride, kTileRows, w, S::kN / 2, k, args, &w_map, &x_map))) return rc;
+    const int64_t m_tiles = (static_cast<int64_t>(args.rows) + 255) / 256;
+    const int64_t tiles = m_tiles * ((static_cast<int64_t>(args.n) + S::kN - 1) / S::kN);
+    if (tiles > INT32_MAX / 2) return pkv::fail(PKV_VALUE_ERROR, "fp8 linear: too many tiles");
+    args.m_tiles = static_cast<int32_t>(m_tiles);
+    args.tiles = static_cast<int32_t>(tiles);
+    const int64_t pairs = tiles < sms / 2 ? tiles : sms / 2;
+    return launch_kernel(fp8_linear_pair_kernel, static_cast<int>(2 * pairs), S::kThreads, S::kSmem, w_map, x_map, args, 2,
+                         stream);
 }
 
 }  // namespace
@@ -807,19 +1067,23 @@ extern "C" int pkv_fp8_linear(const void *x, int64_t x_stride, const void *x_sca
     if (rows <= 16) return launch_few<16>(device, x, x_stride, w, k, sms, args, s);
     if (rows <= 32) return launch_few<32>(device, x, x_stride, w, k, sms, args, s);
     if (rows <= 64) return launch_few<64>(device, x, x_stride, w, k, sms, args, s);
-    // Tile width by the time of the busiest SM: rounds of tiles times the tensor
-    // time of a K block, 2 N clocks (192 at N = 64, where reading x's tile from
-    // shared memory bounds it), over the splits that fill the SMs.
+    // Tile shape by the time of the busiest SM: rounds of tiles, times the K blocks of a
+    // CTA, times the clocks that a K block was measured to take (the chain of waits,
+    // TMEM reads and scaled sums, more than the MMAs' 2 N clocks): 700 / 800 / 1000 at
+    // N = 64 / 128 / 192, and 1100 for a pair's 256 x 256.
     const int64_t m_tiles = (rows + kTileRows - 1) / kTileRows;
-    int best = 0;
-    int64_t best_cost = 0;
-    for (const int width : {192, 128, 64}) {
-        const int64_t tiles = m_tiles * ((n + width - 1) / width);
-        const int splits = row_splits(tiles, args.k_blocks, sms);
+    const int64_t pair_rounds = (static_cast<int64_t>((rows + 255) / 256) * ((n + 255) / 256) + sms / 2 - 1) / (sms / 2);
+    int best = 256;
+    int64_t best_cost = pair_rounds * args.k_blocks * 1100;
+    constexpr int kWidths[3] = {192, 128, 64}, kClocks[3] = {1000, 800, 700};
+    for (int i = 0; i < 3; ++i) {
+        const int64_t tiles = m_tiles * ((n + kWidths[i] - 1) / kWidths[i]);
+        const int splits = row_splits(tiles, args.k_blocks, sms, kRowsCluster);
         const int64_t rounds = (tiles * splits + sms - 1) / sms;
-        const int64_t cost = rounds * ((args.k_blocks + splits - 1) / splits) * (width == 64 ? 192 : 2 * width);
-        if (best == 0 || cost < best_cost) best = width, best_cost = cost;
+        const int64_t cost = rounds * ((args.k_blocks + splits - 1) / splits) * kClocks[i];
+        if (cost < best_cost) best = kWidths[i], best_cost = cost;
     }
+    if (best == 256) return launch_pairs(device, x, x_stride, w, k, sms, args, s);
     if (best == 192) return launch_rows<192>(device, x, x_stride, w, k, sms, args, s);
     if (best == 128) return launch_rows<128>(device, x, x_stride, w, k, sms, args, s);
     return launch_rows<64>(device, x, x_stride, w, k, sms, args, s);

@@ -83,7 +83,7 @@ class Fp8Rows:
         if not self.codes.is_contiguous():
             raise ValueError("to_half needs contiguous codes")
         if out is None:
-            out = torch.empty((rows, width), dtype=torch.float16, device=self.codes.device)
+            out = self.codes.new_empty((rows, width), dtype=torch.float16)
             stride = width
         else:
             if out.shape != (rows, width) or out.dtype != torch.float16 or out.stride(1) != 1 or out.get_device() != index:
@@ -117,10 +117,10 @@ def _check_rows(x: Fp8Rows) -> tuple[int, int]:
     return rows, width
 
 
-def _empty_rows(rows: int, width: int, device: torch.device) -> Fp8Rows:
+def _empty_rows(x: Tensor, rows: int, width: int) -> Fp8Rows:
+    """Uninitialised 8-bit rows on the device of ``x``."""
     return Fp8Rows(
-        torch.empty((rows, width), dtype=_CODES, device=device),
-        torch.empty((rows, _groups(width)), dtype=torch.float32, device=device),
+        x.new_empty((rows, width), dtype=_CODES), x.new_empty((rows, _groups(width)), dtype=torch.float32)
     )
 
 
@@ -159,7 +159,7 @@ def add_rms_norm(
         _half_matrix("delta", delta, shape)
         index = _device(hidden, weight, delta, residual)
         delta_ptr, residual_ptr = delta.data_ptr(), residual.data_ptr()
-    out = _empty_rows(rows, dim, hidden.device)
+    out = _empty_rows(hidden, rows, dim)
     if rows:
         _call(index, lib.pkv_fp8_add_rms_norm, hidden.data_ptr(), delta_ptr, weight.data_ptr(), residual_ptr,
               out.codes.data_ptr(), out.scales.data_ptr(), rows, dim, eps)
@@ -169,7 +169,7 @@ def add_rms_norm(
 def _quantize(x: Tensor, width: int, silu_pairs: bool) -> Fp8Rows:
     index = _device(x)
     rows, columns = x.shape
-    out = _empty_rows(rows, width, x.device)
+    out = _empty_rows(x, rows, width)
     if rows:
         _call(index, lib.pkv_fp8_quantize, x.data_ptr(), max(x.stride(0), columns), silu_pairs, rows, width,
               out.codes.data_ptr(), out.scales.data_ptr())
@@ -222,7 +222,7 @@ def linear(x: Fp8Rows, weight: Fp8Weight, out: Tensor | None = None) -> Tensor:
         raise ValueError("weight needs contiguous FP32 scales [ceil(n / 128), ceil(k / 128)]")
     index = _device(x.codes, x.scales, codes, scales)
     if out is None:
-        out = torch.empty((rows, n), dtype=torch.float16, device=codes.device)
+        out = codes.new_empty((rows, n), dtype=torch.float16)
         stride = n
     else:
         if out.shape != (rows, n) or out.dtype != torch.float16 or out.stride(1) != 1 or out.get_device() != index:
@@ -376,7 +376,7 @@ def append_kv(
             raise ValueError("query must be FP16 [layers, tokens, 32, 64]")
         _half("query", query, index)
         if query_out is None:
-            query_out = torch.empty(query.shape, dtype=torch.float16, device=query.device)
+            query_out = torch.empty_like(query, memory_format=torch.contiguous_format)
         elif query_out.shape != query.shape or not _rows_ok(query_out):
             raise ValueError("query_out must be FP16 [layers, tokens, 32, 64] with contiguous, 16-byte aligned rows")
         else:
@@ -402,11 +402,12 @@ def read_blocks(cache: Fp8Cache, layer: int, blocks: Tensor, error_flag: Tensor)
     count = blocks.numel()
     blocks_ptr = _int_list(index, "blocks", blocks, count)
     flag = _int_list(index, "error_flag", error_flag, 1)
-    out = torch.empty((2, count, _BLOCK_TOKENS, _KV_HEADS, _HEAD_DIM), dtype=torch.float16, device=blocks.device)
+    key = blocks.new_empty((count, _BLOCK_TOKENS, _KV_HEADS, _HEAD_DIM), dtype=torch.float16)
+    value = torch.empty_like(key)
     if count:
-        _call(index, lib.pkv_fp8_read_blocks, *cache._args(), layer, blocks_ptr, count, out.data_ptr(),
-              count * _BLOCK_TOKENS * _KV_HEADS * _HEAD_DIM, flag)
-    return out[0], out[1]
+        _call(index, lib.pkv_fp8_read_blocks, *cache._args(), layer, blocks_ptr, count, key.data_ptr(),
+              value.data_ptr(), flag)
+    return key, value
 
 
 @functools.lru_cache(maxsize=4096)
@@ -437,7 +438,8 @@ def _query_and_out(query: Tensor, out: Tensor | None, index: int, rows: str) -> 
         query = query.contiguous()
     stride = max(query.stride(0), _QUERY_HEADS * _HEAD_DIM)  # of one row it may be anything
     if out is None:
-        return query, stride, torch.empty(shape, dtype=torch.float16, device=query.device), _QUERY_HEADS * _HEAD_DIM
+        out = torch.empty_like(query, memory_format=torch.contiguous_format)
+        return query, stride, out, _QUERY_HEADS * _HEAD_DIM
     _attention_rows("out", out, shape, index)
     if not _rows_ok(out):
         raise ValueError(f"out must be FP16 [{rows}, 32, 64] with contiguous, 16-byte aligned rows")
@@ -449,7 +451,7 @@ def _decode(cache, layer, query, new, lengths, prefix, flat, total_blocks, error
     query, query_stride, out, out_stride = _query_and_out(query, out, index, "batch")
     batch = query.shape[0]
     grid, workspace_bytes = decode_plan(index, batch, total_blocks)
-    workspace = torch.empty(workspace_bytes, dtype=torch.uint8, device=query.device)
+    workspace = query.new_empty((workspace_bytes + 1) // 2)
     _call(
         index, lib.pkv_fp8_decode_attention if new is None else lib.pkv_fp8_decode_layer, *cache._args(), layer,
         query.data_ptr(), query_stride, *(new or ()), _int_list(index, "lengths", lengths, batch),
@@ -536,7 +538,7 @@ def prefill_attention(
         raise ValueError("the chunk must hold 1 or more tokens at positions below 2048")
     count = -(-(start + tokens) // _BLOCK_TOKENS)
     blocks_ptr = _int_list(index, "blocks", blocks, count)
-    workspace = torch.empty(count * _PREFILL_BLOCK_BYTES, dtype=torch.uint8, device=query.device)
+    workspace = query.new_empty(count * _PREFILL_BLOCK_BYTES // 2)
     _call(index, lib.pkv_fp8_prefill_attention, *cache._args(), layer, query.data_ptr(), query_stride, blocks_ptr,
           start, tokens, out.data_ptr(), out_stride, workspace.data_ptr(), count * _PREFILL_BLOCK_BYTES,
           _int_list(index, "error_flag", error_flag, 1))

@@ -65,8 +65,8 @@ def test_cache() -> None:
     refused(lib.pkv_fp8_append_kv, *append(rope=P), message=b"positions")
     refused(lib.pkv_fp8_append_kv, *append(query=P, query_out=P), message=b"positions")
     refused(lib.pkv_fp8_append_kv, *append(rope=P, positions=P, query=P), message=b"an output")
-    refused(lib.pkv_fp8_read_blocks, *CACHE, 2, P, 1, P, 4096, P, None, message=b"layers out of range")
-    refused(lib.pkv_fp8_read_blocks, *CACHE, 0, P, 2, P, 4096, P, None, message=b"K before V")
+    refused(lib.pkv_fp8_read_blocks, *CACHE, 2, P, 1, P, P, P, None, message=b"layers out of range")
+    refused(lib.pkv_fp8_read_blocks, *CACHE, 0, P, 2, P, P + 8, P, None, message=b"16-byte")
 
 
 def test_attention() -> None:

@@ -188,7 +188,8 @@ def linear64(x, weight):
     "rows, n, k",
     [(1, 1, 16), (1, 128, 128), (1, 2560, 2048), (2, 300, 48), (7, 33, 2048), (16, 129, 144), (17, 128, 272),
      (32, 2048, 5632), (33, 200, 400), (64, 640, 2048), (65, 129, 1040), (128, 2048, 5632), (129, 500, 272),
-     (256, 2560, 2048), (257, 131, 512), (600, 300, 2048), (1000, 64, 16)],
+     (256, 2560, 2048), (257, 131, 512), (600, 300, 2048), (1000, 64, 16), (2047, 2048, 272), (700, 11264, 400),
+     (1500, 8200, 1040), (385, 7000, 2064)],
 )
 def test_linear(rows, n, k) -> None:
     x, weight = random_operands(rows + n + k, rows, n, k)
