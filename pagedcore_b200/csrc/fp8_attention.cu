@@ -10,10 +10,13 @@
 // pieces the pairs form a monotone staircase) that a second kernel, launched
 // as its programmatic dependent, merges in piece order.
 //
-// Data movement: every warp runs its own ring of stages of up to four blocks
-// (64 tokens): per block one bulk copy each for the 1 KiB K tile, the 1 KiB V
-// tile and the two 16-byte scale rows.  V tiles lie 1056 bytes apart, so the
-// 16-byte reads below are free of bank conflicts.
+// Data movement: a fifth warp fills a ring of stages of up to four blocks (64
+// tokens) for the whole CTA: per block one bulk copy each for the K tiles and the V
+// tiles of the four heads (4 KiB, contiguous) and for the two 16-byte scale rows.
+// (Copies of 1 KiB by each of the four warps were four times as many; a bulk copy
+// takes the SM about 13 clocks to issue, 1.4 us for the first chunk of 12 warps.)
+// V blocks lie 4128 bytes apart in a stage, so the 16-byte reads below are free of
+// bank conflicts.  Two stages and three CTAs an SM keep about 200 KB under way.
 //
 // Math: mma.sync m16n8k16 on FP16 operands made from codes in registers
 // (E4M3 to FP16 is exact), FP32 sums:
@@ -63,16 +66,18 @@ constexpr int kQueryHeads = PKV_QUERY_HEADS;
 constexpr int kGroup = kQueryHeads / kHeads;
 constexpr int kSlots = PKV_BLOCK_TOKENS;
 constexpr int kTile = pkv::fp8::kTileBytes;
-constexpr int kWarps = kHeads;
-constexpr int kThreads = kWarps * 32;
-constexpr int kChunk = 4;     // blocks per stage
+constexpr int kWarps = kHeads;        // consumers, one per KV head
+constexpr int kProducer = kWarps;     // the warp that fills the ring
+constexpr int kThreads = (kWarps + 1) * 32;
+constexpr int kChunk = 4;             // blocks per stage
 constexpr int kStages = 2;
-constexpr int kValuePitch = kTile + 32;
-constexpr int kValueAt = kChunk * kTile;
-constexpr int kScaleAt = kValueAt + kChunk * kValuePitch;   // K then V scale rows, 16 bytes a block
+constexpr int kBlockBytes = kHeads * kTile;
+constexpr int kValuePitch = kBlockBytes + 32;
+constexpr int kValueAt = kChunk * kBlockBytes;
+constexpr int kScaleAt = kValueAt + kChunk * kValuePitch;  // K then V scale rows, 16 bytes a block
 constexpr int kStageBytes = kScaleAt + 2 * kChunk * 16;
-constexpr int kBlockTraffic = 2 * kTile + 32;
-constexpr int kSmem = kWarps * kStages * kStageBytes;
+constexpr int kBlockTraffic = 2 * kBlockBytes + 32;
+constexpr int kSmem = kStages * kStageBytes;
 constexpr uint32_t kWaitPolls = 1u << 24;
 constexpr float kScaleLog2 = 0.125f * 1.4426950408889634f;  // 64^-0.5 * log2(e)
 constexpr float kWeightShift = 15.0f;
@@ -194,19 +199,99 @@ __device__ __forceinline__ void load_query(const Args &a, int row, int head, int
     q[4] = y.x, q[5] = y.y, q[6] = y.z, q[7] = y.w;
 }
 
+__device__ __forceinline__ bool wait_bounded(uint32_t bar, uint32_t parity) {
+    return pkv::mbar_test_wait(bar, parity) || pkv::mbar_wait_bounded(bar, parity, kWaitPolls);
+}
+
+// The producer warp: copies the blocks of [begin, end) chunk by chunk, a chunk
+// ending with its row.  `lo` is at most 32 rows before the piece's first; !ready:
+// rows' last blocks only after the grid before this one.
+__device__ __forceinline__ void fill_ring(const Args &a, int begin, int end, int lo, bool ready, int lane,
+                                          uint8_t *smem, uint64_t *full, uint64_t *empty) {
+    const uint64_t policy = pkv::l2_policy_evict_first();
+    const uint32_t ring = pkv::smem_addr(smem);
+    // The ids of the list's next 64 blocks, 32 at a time, a window ahead.
+    int ids_base = begin;
+    int ids = begin + lane < end ? a.flat[begin + lane] : 0;
+    int ids_next = begin + 32 + lane < end ? a.flat[begin + 32 + lane] : 0;
+    Rows rows = load_rows(a, lo, lane);
+    int row = advance_row(a, rows, lo, begin, lane);
+    int row_end = __shfl_sync(0xffffffffu, rows.last, row - rows.base);
+    const int64_t layer_tile = pkv::fp8::tile_index(a.cache, a.layer, 0, 0);
+    int issued = 0;
+    bool ok = true;
+    for (int at = begin; at < end;) {
+        if (at >= row_end) {
+            row = advance_row(a, rows, row + 1, at, lane);
+            row_end = __shfl_sync(0xffffffffu, rows.last, row - rows.base);
+        }
+        if (row >= a.batch) break;  // prefix does not grow from row to row: the consumers stop here too
+        const int n = min(kChunk, min(row_end, end) - at);
+        if (at - ids_base >= 32) {
+            ids = ids_next;
+            ids_base += 32;
+            const int ahead = ids_base + 32 + lane;
+            ids_next = ahead < end ? a.flat[ahead] : 0;
+        }
+        const int j = lane & 3;
+        const int offset = at - ids_base + j;
+        const int near = __shfl_sync(0xffffffffu, ids, offset & 31);
+        const int far = __shfl_sync(0xffffffffu, ids_next, offset & 31);
+        int block = offset < 32 ? near : far;
+        if (j < n && (block < 0 || block >= a.cache.num_blocks)) {
+            // Reported; block 0 is read in its place (inside the cache).
+            atomicOr(a.error_flag, PKV_DEVICE_BAD_BLOCK);
+            block = 0;
+        }
+        if (!ready && at + n >= row_end) {  // the row's last block
+            pkv::pdl_wait();
+            ready = true;
+        }
+        const int stage = issued % kStages;
+        if (issued >= kStages) {
+            ok = wait_bounded(pkv::smem_addr(&empty[stage]), (issued / kStages - 1) & 1);
+            ok = __all_sync(0xffffffffu, ok);
+            if (!ok) break;  // a consumer gave up
+        }
+        const uint32_t dst = ring + stage * kStageBytes, bar = pkv::smem_addr(&full[stage]);
+        if (lane == 0) pkv::mbar_arrive_expect_tx(bar, n * kBlockTraffic);
+        __syncwarp();
+        if (j < n && lane < 16) {
+            const int64_t tile = layer_tile + static_cast<int64_t>(block) * kHeads;
+            if (lane < 4) {
+                bulk_load(dst + j * kBlockBytes, a.cache.key_codes + tile * kTile, kBlockBytes, bar, policy);
+            } else if (lane < 8) {
+                bulk_load(dst + kValueAt + j * kValuePitch, a.cache.value_codes + tile * kTile, kBlockBytes, bar, policy);
+            } else if (lane < 12) {
+                bulk_load(dst + kScaleAt + j * 16, a.cache.key_scales + tile, 16, bar, policy);
+            } else {
+                bulk_load(dst + kScaleAt + (kChunk + j) * 16, a.cache.value_scales + tile, 16, bar, policy);
+            }
+        }
+        at += n;
+        ++issued;
+    }
+    if (!ok && lane == 0) atomicOr(a.error_flag, PKV_DEVICE_WAIT_TIMEOUT);
+    // No copy may land after the CTA has left.
+    for (int c = max(0, issued - kStages); c < issued; ++c) {
+        wait_bounded(pkv::smem_addr(&full[c % kStages]), (c / kStages) & 1);
+    }
+    if (!ready) pkv::pdl_wait();
+}
+
 __global__ void __launch_bounds__(kThreads, 3) fp8_decode_kernel(const __grid_constant__ Args a) {
     extern __shared__ __align__(16) uint8_t smem[];
-    __shared__ __align__(8) uint64_t barriers[kWarps * kStages];
+    __shared__ __align__(8) uint64_t full[kStages], empty[kStages];
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int g = lane >> 2, t = lane & 3;
-    uint8_t *const ring_tiles = smem + warp * kStages * kStageBytes;
-    const uint32_t ring = pkv::smem_addr(ring_tiles);
-    const uint32_t bar0 = pkv::smem_addr(&barriers[warp * kStages]);
-    if (lane == 0) {
-        for (int s = 0; s < kStages; ++s) pkv::mbar_init(bar0 + 8 * s, 1);
+    if (threadIdx.x == 0) {
+        for (int s = 0; s < kStages; ++s) {
+            pkv::mbar_init(pkv::smem_addr(&full[s]), 1);
+            pkv::mbar_init(pkv::smem_addr(&empty[s]), kWarps);
+        }
         pkv::fence_barrier_init();
     }
-    __syncwarp();
+    __syncthreads();
     // Launched as a programmatic dependent: behind the append of the same layer
     // (early) the tables and every block but the rows' last ones are ready, and only
     // what the append writes is waited for.
@@ -230,12 +315,6 @@ __global__ void __launch_bounds__(kThreads, 3) fp8_decode_kernel(const __grid_co
     }
     const int begin = piece_begin(blockIdx.x, total, pieces);
     const int end = piece_begin(blockIdx.x + 1, total, pieces);
-    // The ids of the list's next 64 blocks (32 at a time, one window ahead).
-    int ids_base = begin;
-    int ids = begin + lane < end ? a.flat[begin + lane] : 0;
-    int ids_next = begin + 32 + lane < end ? a.flat[begin + 32 + lane] : 0;
-
-    const uint64_t policy = pkv::l2_policy_evict_first();
     // The first row with blocks past `begin`: the first sample past it, cut finer until
     // the samples are rows.
     int lo = 0;
@@ -246,70 +325,13 @@ __global__ void __launch_bounds__(kThreads, 3) fp8_decode_kernel(const __grid_co
         step = (step + 31) / 32;
         sample = lo + lane * step < a.batch ? a.prefix[min(lo + (lane + 1) * step, a.batch)] : INT32_MAX;
     }
+    if (warp == kProducer) {
+        fill_ring(a, begin, end, lo, ready, lane, smem, full, empty);
+        return;
+    }
     Rows rows = load_rows(a, lo, lane);
     int row = advance_row(a, rows, lo, begin, lane);
-
-    // Fetch cursor: the next block to copy and the row it belongs to.
-    Rows fetch_rows = rows;
-    int fetch_row = row;
-    int fetch_end = __shfl_sync(0xffffffffu, fetch_rows.last, fetch_row - fetch_rows.base);
-    int fetch = begin;
-    int fetched = 0;
-
-    const int64_t layer_tile = pkv::fp8::tile_index(a.cache, a.layer, 0, 0);
-    // Copy the next chunk into stage `fetched % kStages`.
-    const auto issue = [&]() {
-        if (fetch >= end) return;
-        if (fetch >= fetch_end) {
-            fetch_row = advance_row(a, fetch_rows, fetch_row + 1, fetch, lane);
-            fetch_end = __shfl_sync(0xffffffffu, fetch_rows.last, fetch_row - fetch_rows.base);
-        }
-        const int n = min(kChunk, min(fetch_end, end) - fetch);
-        if (!ready && fetch + n >= fetch_end) {  // the row's last block
-            pkv::pdl_wait();
-            ready = true;
-        }
-        if (fetch - ids_base >= 32) {
-            ids = ids_next;
-            ids_base += 32;
-            const int ahead = ids_base + 32 + lane;
-            ids_next = ahead < end ? a.flat[ahead] : 0;
-        }
-        const int at = fetch - ids_base + (lane & 3);
-        const int near = __shfl_sync(0xffffffffu, ids, at & 31);
-        const int far = __shfl_sync(0xffffffffu, ids_next, at & 31);
-        int block = at < 32 ? near : far;
-        const int stage = fetched % kStages;
-        const uint32_t dst = ring + stage * kStageBytes, bar = bar0 + 8 * stage;
-        const bool mine = (lane & 3) < n;
-        if (mine && (block < 0 || block >= a.cache.num_blocks)) {
-            // Reported; block 0 is read in its place (inside the cache).
-            atomicOr(a.error_flag, PKV_DEVICE_BAD_BLOCK);
-            block = 0;
-        }
-        if (lane == 0) pkv::mbar_arrive_expect_tx(bar, n * kBlockTraffic);
-        __syncwarp();
-        if (mine && lane < 16) {
-            const int j = lane & 3;
-            const int64_t tile = layer_tile + static_cast<int64_t>(block) * kHeads;
-            if (lane < 4) {
-                bulk_load(dst + j * kTile, a.cache.key_codes + (tile + warp) * kTile, kTile, bar, policy);
-            } else if (lane < 8) {
-                bulk_load(dst + kValueAt + j * kValuePitch, a.cache.value_codes + (tile + warp) * kTile, kTile, bar, policy);
-            } else if (lane < 12) {
-                bulk_load(dst + kScaleAt + j * 16, a.cache.key_scales + tile, 16, bar, policy);
-            } else {
-                bulk_load(dst + kScaleAt + (kChunk + j) * 16, a.cache.value_scales + tile, 16, bar, policy);
-            }
-        }
-        fetch += n;
-        ++fetched;
-    };
-    for (int s = 0; s < kStages; ++s) issue();
-    if (!ready) {
-        pkv::pdl_wait();
-        ready = true;
-    }
+    if (!ready) pkv::pdl_wait();
     pkv::pdl_launch_dependents();
 
     bool beyond = row >= a.batch;  // prefix does not grow from row to row
@@ -342,15 +364,15 @@ __global__ void __launch_bounds__(kThreads, 3) fp8_decode_kernel(const __grid_co
         while (i < seg_end) {
             const int n = min(kChunk, seg_end - i);
             const int stage = consumed % kStages;
-            const uint8_t *src = ring_tiles + stage * kStageBytes;
-            if (!failed && !pkv::mbar_wait_bounded(bar0 + 8 * stage, (consumed / kStages) & 1, kWaitPolls)) failed = true;
+            const uint8_t *src = smem + stage * kStageBytes;
+            failed = !wait_bounded(pkv::smem_addr(&full[stage]), (consumed / kStages) & 1);
             failed = __any_sync(0xffffffffu, failed);
             if (failed) break;
             const int tokens = min(max(length - (i - row_first) * kSlots, 0), n * kSlots);  // valid ones of the chunk
 
             // Scores: lane's rows are tokens 4 j + (g & 1) and 4 j + 2 + (g & 1) of block g / 2.
             float s[4][4];
-            const uint8_t *k_at = src + (g >> 1) * kTile + (g & 1) * kDim + 16 * t;
+            const uint8_t *k_at = src + (g >> 1) * kBlockBytes + warp * kTile + (g & 1) * kDim + 16 * t;
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
                 const uint4 a0 = *reinterpret_cast<const uint4 *>(k_at + 4 * j * kDim);
@@ -370,18 +392,18 @@ __global__ void __launch_bounds__(kThreads, 3) fp8_decode_kernel(const __grid_co
             uint4 v[4][2];
 #pragma unroll
             for (int mt = 0; mt < 4; ++mt) {
-                const uint8_t *v_at = src + kValueAt + t * kValuePitch + (16 * mt + g) * 16;
+                const uint8_t *v_at = src + kValueAt + t * kValuePitch + warp * kTile + (16 * mt + g) * 16;
                 v[mt][0] = *reinterpret_cast<const uint4 *>(v_at);
                 v[mt][1] = *reinterpret_cast<const uint4 *>(v_at + 8 * 16);
             }
             // Every lane has read the stage (the fence orders the reads before the
-            // copies, the warp barrier the lanes): it is filled again while this
+            // copies, the warp barrier the lanes): it may be filled again while this
             // chunk is worked on.
             pkv::fence_proxy_async_smem();
             __syncwarp();
+            if (lane == 0) pkv::mbar_arrive(pkv::smem_addr(&empty[stage]));
             i += n;
             ++consumed;
-            issue();
 
             const int ve = ((__float_as_int(value_scale) >> 23) & 0xff) - 127;
             const float shift = static_cast<float>(ve);
@@ -490,12 +512,8 @@ __global__ void __launch_bounds__(kThreads, 3) fp8_decode_kernel(const __grid_co
             for (int x = 0; x < 8; ++x) q[x] = q_next[x];
         }
     }
-    if (failed || beyond) {
-        if (lane == 0) atomicOr(a.error_flag, failed ? PKV_DEVICE_WAIT_TIMEOUT : PKV_DEVICE_BAD_BLOCK);
-        // No copy may land after the CTA has left.
-        for (int c = consumed; c < fetched; ++c) {
-            pkv::mbar_wait_bounded(bar0 + 8 * (c % kStages), (c / kStages) & 1, kWaitPolls);
-        }
+    if ((failed || beyond) && lane == 0) {
+        atomicOr(a.error_flag, failed ? PKV_DEVICE_WAIT_TIMEOUT : PKV_DEVICE_BAD_BLOCK);
     }
 }
 
