@@ -7,7 +7,8 @@
 // power of two: only codes near the subnormals change).  Writing the same
 // token to the same slot twice leaves the same bytes.
 //
-// One CTA per token and layer, a warp per (K or V, head).  The warps of a token
+// A CTA takes one token of a layer (eight of a long list) with a warp per (K or V,
+// head); others, ahead of them in the grid, rotate the queries.  The warps of a token
 // that opens a run (the first token, or one whose slot does not follow the
 // previous token's within its block) write the whole run; the tokens of a run
 // are those that follow it slot by slot in the block.  K: lane (r, h) holds the
@@ -60,7 +61,11 @@ struct AppendArgs {
     const int32_t *prefix;
     const int32_t *flat;
     int32_t total_blocks;
+    int32_t q_ctas;  // CTAs that rotate queries, ahead of those that write K and V
+    int32_t span;    // tokens per CTA of the latter
 };
+
+constexpr int kQuerySpan = 4;  // tokens per CTA that rotates queries
 
 __device__ __forceinline__ float warp_max(float v) {
 #pragma unroll
@@ -148,6 +153,7 @@ __device__ void write_key(const AppendArgs &a, int layer, int head, int token, i
                           int lane) {
     const int64_t tile = pkv::fp8::tile_index(a.cache, layer + a.layer_begin, block, head);
     uint8_t *codes = a.cache.key_codes + tile * pkv::fp8::kTileBytes;
+    const float held_scale = first > 0 ? a.cache.key_scales[tile] : 0.f;
     const int r = lane >> 1, d = 16 * (lane & 1);
     const bool fresh = r >= first && r < first + run;
     float lo[16], hi[16];
@@ -163,7 +169,7 @@ __device__ void write_key(const AppendArgs &a, int layer, int head, int token, i
     }
     amax = warp_max(amax);
     int held;
-    const int e = tile_exponent(amax, first, a.cache.key_scales[tile], held);
+    const int e = tile_exponent(amax, first, held_scale, held);
     uint4 *row = reinterpret_cast<uint4 *>(codes + r * kDim + d);
     if (fresh) {
         const float inverse = pkv::fp8::exp2_int(-e);
@@ -183,6 +189,8 @@ __device__ void write_value(const AppendArgs &a, int layer, int head, int token,
                             int lane) {
     const int64_t tile = pkv::fp8::tile_index(a.cache, layer + a.layer_begin, block, head);
     uint4 *rows = reinterpret_cast<uint4 *>(a.cache.value_codes + tile * pkv::fp8::kTileBytes) + 2 * lane;
+    const float held_scale = first > 0 ? a.cache.value_scales[tile] : 0.f;
+    const uint4 stored[2] = {rows[0], rows[1]};
     const __half *src = a.value + layer * a.layer_stride + token * a.token_stride + head * kDim + 2 * lane;
     float v[2][kSlots];  // of dims 2 lane, 2 lane + 1 by slot
     float amax = 0.f;
@@ -198,13 +206,13 @@ __device__ void write_value(const AppendArgs &a, int layer, int head, int token,
     }
     amax = warp_max(amax);
     int held;
-    const int e = tile_exponent(amax, first, a.cache.value_scales[tile], held);
+    const int e = tile_exponent(amax, first, held_scale, held);
     const float inverse = pkv::fp8::exp2_int(-e);
     const bool largest = e == pkv::fp8::kMaxExponent;
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
         const uint4 fresh = encode16(v[i], inverse, largest);
-        uint4 codes = rows[i];
+        uint4 codes = stored[i];
         const uint32_t *f = reinterpret_cast<const uint32_t *>(&fresh);
         uint32_t *c = reinterpret_cast<uint32_t *>(&codes);
 #pragma unroll
@@ -226,30 +234,29 @@ __device__ void write_value(const AppendArgs &a, int layer, int head, int token,
     if (lane == 0) a.cache.value_scales[tile] = pkv::fp8::exp2_int(e);
 }
 
-__global__ void __launch_bounds__(kThreads) fp8_append_kernel(const __grid_constant__ AppendArgs a) {
-    // In this order: the decode attention behind it reads what is older than this
-    // kernel (the tables, the cache but for the blocks written here) before its own wait.
-    pkv::pdl_wait();
-    pkv::pdl_launch_dependents();
-    const int token = blockIdx.x;
-    const int layer = blockIdx.y;
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    if (a.lengths != nullptr && a.prefix[token + 1] <= a.prefix[token]) return;  // a row without blocks
-
-    if (a.query_in != nullptr) {
-        // Eight lanes a query head, eight dims a lane; the partner's dims (32 away)
-        // come from the lane four further.
-        const int position = checked_position(a, token);
-        const int chunk = lane & 7, at = (4 * warp + (lane >> 3)) * kDim + 8 * chunk;
-        const int64_t in = layer * a.q_layer_stride + token * a.q_token_stride + at;
-        const int64_t out = layer * a.q_out_layer_stride + token * a.q_out_token_stride + at;
-        const uint4 own = *reinterpret_cast<const uint4 *>(a.query_in + in);
-        const __half *factors = a.rope + position * kHalf + 8 * (chunk & 3);
-        const uint4 cos = *reinterpret_cast<const uint4 *>(factors);
-        const uint4 sin = *reinterpret_cast<const uint4 *>(factors + PKV_CONTEXT_LIMIT * kHalf);
-        const float sign = chunk < 4 ? -1.f : 1.f;
-        const uint32_t x[4] = {own.x, own.y, own.z, own.w}, c[4] = {cos.x, cos.y, cos.z, cos.w},
-                       s[4] = {sin.x, sin.y, sin.z, sin.w};
+// RoPE of kQuerySpan tokens' queries, four heads a warp: eight lanes a head, eight
+// dims a lane; the partner's dims (32 away) come from the lane four further.
+__device__ void rotate_queries(const AppendArgs &a, int layer, int begin, int warp, int lane) {
+    const int chunk = lane & 7, at = (4 * warp + (lane >> 3)) * kDim + 8 * chunk;
+    const float sign = chunk < 4 ? -1.f : 1.f;
+    uint4 own[kQuerySpan], cos[kQuerySpan], sin[kQuerySpan];
+    bool here[kQuerySpan];
+#pragma unroll
+    for (int j = 0; j < kQuerySpan; ++j) {
+        const int token = begin + j;
+        here[j] = token < a.tokens && (a.lengths == nullptr || a.prefix[token + 1] > a.prefix[token]);
+        own[j] = cos[j] = sin[j] = make_uint4(0, 0, 0, 0);
+        if (here[j]) {
+            own[j] = *reinterpret_cast<const uint4 *>(a.query_in + layer * a.q_layer_stride + token * a.q_token_stride + at);
+            const __half *factors = a.rope + checked_position(a, token) * kHalf + 8 * (chunk & 3);
+            cos[j] = *reinterpret_cast<const uint4 *>(factors);
+            sin[j] = *reinterpret_cast<const uint4 *>(factors + PKV_CONTEXT_LIMIT * kHalf);
+        }
+    }
+#pragma unroll
+    for (int j = 0; j < kQuerySpan; ++j) {
+        const uint32_t x[4] = {own[j].x, own[j].y, own[j].z, own[j].w}, c[4] = {cos[j].x, cos[j].y, cos[j].z, cos[j].w},
+                       s[4] = {sin[j].x, sin[j].y, sin[j].z, sin[j].w};
         uint32_t r[4];
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
@@ -260,25 +267,58 @@ __global__ void __launch_bounds__(kThreads) fp8_append_kernel(const __grid_const
             const float2 sf = __half22float2(*reinterpret_cast<const __half2 *>(&s[i]));
             r[i] = pkv::pack_half2(__floats2half2_rn(xf.x * cf.x + sign * pf.x * sf.x, xf.y * cf.y + sign * pf.y * sf.y));
         }
-        *reinterpret_cast<uint4 *>(a.query_out + out) = make_uint4(r[0], r[1], r[2], r[3]);
+        if (here[j]) {
+            const int64_t to = layer * a.q_out_layer_stride + (begin + j) * a.q_out_token_stride + at;
+            *reinterpret_cast<uint4 *>(a.query_out + to) = make_uint4(r[0], r[1], r[2], r[3]);
+        }
     }
+}
 
-    const int slot = slot_of(a, token);
-    if (slot < 0) {
-        if (threadIdx.x == 0) atomicOr(a.error_flag, PKV_DEVICE_BAD_BLOCK);
+// The grid for `tokens`: eight tokens a CTA (of a prompt every sixteenth opens a run) once there are enough CTAs to fill the SMs.
+dim3 append_grid(AppendArgs &a, int layers) {
+    a.q_ctas = a.query_in != nullptr ? (a.tokens + kQuerySpan - 1) / kQuerySpan : 0;
+    a.span = a.lengths == nullptr && a.tokens >= 512 ? 8 : 1;
+    return dim3(a.q_ctas + (a.tokens + a.span - 1) / a.span, layers);
+}
+
+__global__ void __launch_bounds__(kThreads, 3) fp8_append_kernel(const __grid_constant__ AppendArgs a) {
+    // In this order: the decode attention behind it reads what is older than this
+    // kernel (the tables, the cache but for the blocks written here) before its own wait.
+    pkv::pdl_wait();
+    pkv::pdl_launch_dependents();
+    const int layer = blockIdx.y;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    if (static_cast<int>(blockIdx.x) < a.q_ctas) {
+        rotate_queries(a, layer, blockIdx.x * kQuerySpan, warp, lane);
         return;
     }
-    const int first = slot % kSlots;
-    int run = 1;
-    if (a.lengths == nullptr) {
-        if (first != 0 && token > 0 && a.slots[token - 1] == slot - 1) return;  // written by its run's first token
-        const bool follows = lane < kSlots - first && token + lane < a.tokens && a.slots[token + lane] == slot + lane;
-        run = __ffs(~__ballot_sync(0xffffffffu, follows)) - 1;
-    }
-    if (warp < kHeads) {
-        write_key(a, layer, warp, token, run, slot / kSlots, first, lane);
-    } else {
-        write_value(a, layer, warp - kHeads, token, run, slot / kSlots, first, lane);
+    const int begin = (static_cast<int>(blockIdx.x) - a.q_ctas) * a.span;
+    // Slots of the tokens from begin - 1 on: a span's runs end 15 tokens past it.
+    const int near = begin - 1 + lane;
+    int slot_at = -1;
+    if (near >= 0 && near < a.tokens) slot_at = slot_of(a, near);
+    for (int j = 0; j < a.span && begin + j < a.tokens; ++j) {
+        const int token = begin + j;
+        if (a.lengths != nullptr && a.prefix[token + 1] <= a.prefix[token]) continue;  // a row without blocks
+        const int slot = __shfl_sync(0xffffffffu, slot_at, j + 1);
+        if (slot < 0) {
+            if (threadIdx.x == 0) atomicOr(a.error_flag, PKV_DEVICE_BAD_BLOCK);
+            continue;
+        }
+        const int first = slot % kSlots;
+        int run = 1;
+        if (a.lengths == nullptr) {
+            const int previous = __shfl_sync(0xffffffffu, slot_at, j);
+            if (first != 0 && token > 0 && previous == slot - 1) continue;  // written with its run's first token
+            const int ahead = lane - (j + 1);  // of this token
+            const bool follows = ahead >= 0 && ahead < kSlots - first && near < a.tokens && slot_at == slot + ahead;
+            run = __ffs(~(__ballot_sync(0xffffffffu, follows) >> (j + 1))) - 1;
+        }
+        if (warp < kHeads) {
+            write_key(a, layer, warp, token, run, slot / kSlots, first, lane);
+        } else {
+            write_value(a, layer, warp - kHeads, token, run, slot / kSlots, first, lane);
+        }
     }
 }
 
@@ -380,7 +420,7 @@ int launch_decode_append(const Cache &cache, int32_t layer, const void *key, con
     a.prefix = prefix;
     a.flat = flat;
     a.total_blocks = total_blocks;
-    const cudaError_t e = launch_pdl(fp8_append_kernel, dim3(batch, 1), dim3(kThreads), stream, a);
+    const cudaError_t e = launch_pdl(fp8_append_kernel, append_grid(a, 1), dim3(kThreads), stream, a);
     if (e != cudaSuccess) return fail(PKV_CUDA_ERROR, std::string("fp8 append launch failed: ") + cudaGetErrorString(e));
     return PKV_OK;
 }
@@ -436,7 +476,7 @@ extern "C" int pkv_fp8_append_kv(void *key_codes, void *value_codes, void *key_s
     a.prefix = nullptr;
     a.flat = nullptr;
     a.total_blocks = 0;
-    const cudaError_t e = pkv::launch_pdl(fp8_append_kernel, dim3(tokens, layer_count), dim3(kThreads),
+    const cudaError_t e = pkv::launch_pdl(fp8_append_kernel, append_grid(a, layer_count), dim3(kThreads),
                                           static_cast<cudaStream_t>(stream), a);
     if (e != cudaSuccess) return pkv::fail(PKV_CUDA_ERROR, std::string("fp8 append launch failed: ") + cudaGetErrorString(e));
     return PKV_OK;
