@@ -461,7 +461,7 @@ int pkv_fp8_decode_plan(int32_t device, int32_t batch, int32_t total_blocks, int
  * on the device; total_blocks is the room of flat, which it must not exceed, so
  * a captured launch serves any batch within it.  grid: the plan's for this
  * batch and block count, or any other; workspace (16-byte aligned, of at least
- * the plan's bytes for that grid: 4096 * batch + 8448 * (batch + grid)) needs no
+ * the plan's bytes for that grid: 8192 * batch + 8448 * (batch + grid)) needs no
  * initialisation, and launches that share one must not overlap on the GPU. */
 int pkv_fp8_decode_attention(const void *key_codes, const void *value_codes, const void *key_scales,
                              const void *value_scales, int32_t layers, int32_t num_blocks, int32_t layer,

@@ -68,6 +68,16 @@ __device__ __forceinline__ uint32_t decode2(uint32_t codes) {
     return r;
 }
 
+// Four codes to two such pairs (the halves of a register are operands of their own: no shift).
+__device__ __forceinline__ void decode4(uint32_t codes, uint32_t &low, uint32_t &high) {
+    asm("{\n\t.reg .b16 l, h;\n\t"
+        "mov.b32 {l, h}, %2;\n\t"
+        "cvt.rn.f16x2.e4m3x2 %0, l;\n\t"
+        "cvt.rn.f16x2.e4m3x2 %1, h;\n\t}"
+        : "=r"(low), "=r"(high)
+        : "r"(codes));
+}
+
 __device__ __forceinline__ float2 decode2f(uint32_t codes) {
     const uint32_t h = decode2(codes);
     return __half22float2(*reinterpret_cast<const __half2 *>(&h));

@@ -32,9 +32,11 @@
 // the exponent: the weight is w = 2^(s + e - M + 15) with M the running maximum
 // of s + e, so the largest contribution, not the largest probability, sits at
 // 2^15 and blocks of very different magnitude lose nothing; the normaliser adds
-// w * 2^-e, in FP32.  w is rounded to FP16 (2^-11 of each weight, below the
-// 2^-4 of the codes that it multiplies); scores, maxima, normaliser and sums
-// are FP32.
+// w * 2^-e, in FP32.  The weights go into the MMA as two FP16 numbers, hi = fp16(w)
+// and lo = fp16(w - hi), 2^-22 of the weight together (one alone is off by 2^-11,
+// which showed in the output), and so do the queries of the decode layer, rotated
+// in FP32; scores, maxima, normaliser and sums are FP32.  The second products are
+// free: the tensor pipe was 13 % busy without them.
 
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
@@ -53,7 +55,7 @@ namespace pkv::fp8 {
 int check_cache(const void *key_codes, const void *value_codes, const void *key_scales, const void *value_scales,
                 int32_t layers, int32_t num_blocks, int32_t layer_begin, int32_t layer_count);
 int launch_decode_append(const Cache &cache, int32_t layer, const void *key, const void *value, int64_t kv_stride,
-                         const void *rope_table, const void *query, int64_t query_stride, void *query_out,
+                         const void *rope_table, const void *query, int64_t query_stride, void *query_out, void *query_low,
                          const int32_t *lengths, const int32_t *prefix, const int32_t *flat, int32_t batch,
                          int32_t total_blocks, int32_t *error_flag, cudaStream_t stream);
 }
@@ -77,7 +79,8 @@ constexpr int kValueAt = kChunk * kBlockBytes;
 constexpr int kScaleAt = kValueAt + kChunk * kValuePitch;  // K then V scale rows, 16 bytes a block
 constexpr int kStageBytes = kScaleAt + 2 * kChunk * 16;
 constexpr int kBlockTraffic = 2 * kBlockBytes + 32;
-constexpr int kSmem = kStages * kStageBytes;
+constexpr int kLowAt = kStages * kStageBytes;  // SPLIT_Q: the low halves of the row's queries, 32 bytes a lane
+constexpr int kSmem = kLowAt + kWarps * 32 * 32;
 constexpr uint32_t kWaitPolls = 1u << 24;
 constexpr float kScaleLog2 = 0.125f * 1.4426950408889634f;  // 64^-0.5 * log2(e)
 constexpr float kWeightShift = 15.0f;
@@ -88,6 +91,7 @@ struct Args {
     pkv::fp8::Cache cache;
     int32_t layer;
     const __half *query;
+    const __half *query_low;  // SPLIT_Q: what FP16 left of each query value
     int64_t query_stride;
     const int32_t *lengths;
     const int32_t *prefix;
@@ -192,11 +196,36 @@ __device__ __forceinline__ int advance_row(const Args &a, Rows &w, int row, int 
     }
 }
 
-__device__ __forceinline__ void load_query(const Args &a, int row, int head, int t, uint32_t (&q)[8]) {
-    const uint4 *src = reinterpret_cast<const uint4 *>(a.query + row * a.query_stride + head * kDim + 16 * t);
+// A lane's 16 query dims of a head: the high halves to registers, the low ones to its
+// own 32 bytes of shared memory at `low`.
+template <bool SPLIT_Q>
+__device__ __forceinline__ void load_query(const Args &a, int row, int head, int t, uint32_t (&q)[8], uint32_t low) {
+    const int64_t at = row * a.query_stride + head * kDim + 16 * t;
+    const uint4 *src = reinterpret_cast<const uint4 *>(a.query + at);
     const uint4 x = src[0], y = src[1];
+    if (SPLIT_Q) {
+        const uint4 *rest = reinterpret_cast<const uint4 *>(a.query_low + at);
+        const uint4 u = rest[0], v = rest[1];
+        asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(low), "r"(u.x), "r"(u.y), "r"(u.z), "r"(u.w) : "memory");
+        asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(low + 16), "r"(v.x), "r"(v.y), "r"(v.z), "r"(v.w) : "memory");
+    }
     q[0] = x.x, q[1] = x.y, q[2] = x.z, q[3] = x.w;
     q[4] = y.x, q[5] = y.y, q[6] = y.z, q[7] = y.w;
+}
+
+// Bring the same into L1 ahead of the row (registers for a second row do not fit).
+template <bool SPLIT_Q>
+__device__ __forceinline__ void prefetch_query(const Args &a, int row, int head, int t) {
+    const int64_t at = row * a.query_stride + head * kDim + 16 * t;
+    asm volatile("prefetch.global.L1 [%0];" ::"l"(a.query + at));
+    if (SPLIT_Q) asm volatile("prefetch.global.L1 [%0];" ::"l"(a.query_low + at));
+}
+
+// Read where it is used (volatile): the eight registers of a whole row do not fit beside the rest.
+__device__ __forceinline__ uint2 lds64(uint32_t addr) {
+    uint2 v;
+    asm volatile("ld.shared.v2.u32 {%0, %1}, [%2];" : "=r"(v.x), "=r"(v.y) : "r"(addr));
+    return v;
 }
 
 __device__ __forceinline__ bool wait_bounded(uint32_t bar, uint32_t parity) {
@@ -279,6 +308,7 @@ __device__ __forceinline__ void fill_ring(const Args &a, int begin, int end, int
     if (!ready) pkv::pdl_wait();
 }
 
+template <bool SPLIT_Q>
 __global__ void __launch_bounds__(kThreads, 3) fp8_decode_kernel(const __grid_constant__ Args a) {
     extern __shared__ __align__(16) uint8_t smem[];
     __shared__ __align__(8) uint64_t full[kStages], empty[kStages];
@@ -337,7 +367,8 @@ __global__ void __launch_bounds__(kThreads, 3) fp8_decode_kernel(const __grid_co
     bool beyond = row >= a.batch;  // prefix does not grow from row to row
     int row_first = __shfl_sync(0xffffffffu, rows.first, row - rows.base);
     uint32_t q[8];
-    if (!beyond) load_query(a, row, warp * kGroup + g, t, q);
+    const uint32_t low = pkv::smem_addr(smem) + kLowAt + threadIdx.x * 32;
+    if (!beyond) load_query<SPLIT_Q>(a, row, warp * kGroup + g, t, q, low);
 
     int consumed = 0;
     bool failed = false;
@@ -346,14 +377,13 @@ __global__ void __launch_bounds__(kThreads, 3) fp8_decode_kernel(const __grid_co
         const int row_last = __shfl_sync(0xffffffffu, rows.last, row - rows.base);
         const int length = __shfl_sync(0xffffffffu, rows.length, row - rows.base);
         const int seg_end = min(end, row_last);
-        // The next row's query is loaded while this row streams.
-        uint32_t q_next[8];
+        // The next row's query is brought near while this row streams.
         int row_next = row;
         Rows rows_next = rows;
         if (row_last < end) {
             row_next = advance_row(a, rows_next, row + 1, row_last, lane);
             beyond = row_next >= a.batch;
-            if (!beyond) load_query(a, row_next, warp * kGroup + g, t, q_next);
+            if (!beyond) prefetch_query<SPLIT_Q>(a, row_next, warp * kGroup + g, t);
         }
 
         float m0 = kLowest, m1 = kLowest, l0 = 0.f, l1 = 0.f;
@@ -381,8 +411,14 @@ __global__ void __launch_bounds__(kThreads, 3) fp8_decode_kernel(const __grid_co
 #pragma unroll
                 for (int ks = 0; ks < 4; ++ks) {
                     const uint32_t x = word(a0, ks), y = word(a1, ks);
-                    mma(s[j], pkv::fp8::decode2(x), pkv::fp8::decode2(y), pkv::fp8::decode2(x >> 16),
-                        pkv::fp8::decode2(y >> 16), q[2 * ks], q[2 * ks + 1]);
+                    uint32_t k0, k1, k2, k3;
+                    pkv::fp8::decode4(x, k0, k2);
+                    pkv::fp8::decode4(y, k1, k3);
+                    mma(s[j], k0, k1, k2, k3, q[2 * ks], q[2 * ks + 1]);
+                    if (SPLIT_Q) {
+                        const uint2 half = lds64(low + 8 * ks);
+                        mma(s[j], k0, k1, k2, k3, half.x, half.y);
+                    }
                 }
             }
             const float key_scale =
@@ -434,7 +470,7 @@ __global__ void __launch_bounds__(kThreads, 3) fp8_decode_kernel(const __grid_co
             m1 = top1;
             const float base0 = kWeightShift - m0, base1 = kWeightShift - m1;
             float add0 = 0.f, add1 = 0.f;
-            uint32_t p[4][2];
+            uint32_t p[4][2], pl[4][2];
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
                 const float w0 = pkv::exp2_approx(s[j][0] + base0);
@@ -443,8 +479,12 @@ __global__ void __launch_bounds__(kThreads, 3) fp8_decode_kernel(const __grid_co
                 const float w3 = pkv::exp2_approx(s[j][3] + base1);
                 add0 += w0 + w2;
                 add1 += w1 + w3;
-                p[j][0] = pkv::movmatrix_trans(pkv::pack_half2(__floats2half2_rn(w0, w1)));
-                p[j][1] = pkv::movmatrix_trans(pkv::pack_half2(__floats2half2_rn(w2, w3)));
+                const __half2 h01 = __floats2half2_rn(w0, w1), h23 = __floats2half2_rn(w2, w3);
+                const float2 f01 = __half22float2(h01), f23 = __half22float2(h23);
+                p[j][0] = pkv::movmatrix_trans(pkv::pack_half2(h01));
+                p[j][1] = pkv::movmatrix_trans(pkv::pack_half2(h23));
+                pl[j][0] = pkv::movmatrix_trans(pkv::pack_half2(__floats2half2_rn(w0 - f01.x, w1 - f01.y)));
+                pl[j][1] = pkv::movmatrix_trans(pkv::pack_half2(__floats2half2_rn(w2 - f23.x, w3 - f23.y)));
             }
             // A block whose tokens are all masked adds nothing, whatever its scale row holds.
             if (!whole && held <= 0) add0 = add1 = 0.f;
@@ -468,8 +508,11 @@ __global__ void __launch_bounds__(kThreads, 3) fp8_decode_kernel(const __grid_co
 #pragma unroll
                 for (int j = 0; j < 4; ++j) {
                     const uint32_t x = word(v[mt][0], j), y = word(v[mt][1], j);
-                    mma(o[mt], pkv::fp8::decode2(x), pkv::fp8::decode2(y), pkv::fp8::decode2(x >> 16),
-                        pkv::fp8::decode2(y >> 16), p[j][0], p[j][1]);
+                    uint32_t v0, v1, v2, v3;
+                    pkv::fp8::decode4(x, v0, v2);
+                    pkv::fp8::decode4(y, v1, v3);
+                    mma(o[mt], v0, v1, v2, v3, p[j][0], p[j][1]);
+                    mma(o[mt], v0, v1, v2, v3, pl[j][0], pl[j][1]);
                 }
             }
         }
@@ -508,8 +551,7 @@ __global__ void __launch_bounds__(kThreads, 3) fp8_decode_kernel(const __grid_co
             row = row_next;
             rows = rows_next;
             row_first = row_last;
-#pragma unroll
-            for (int x = 0; x < 8; ++x) q[x] = q_next[x];
+            if (!beyond) load_query<SPLIT_Q>(a, row, warp * kGroup + g, t, q, low);
         }
     }
     if ((failed || beyond) && lane == 0) {
@@ -601,8 +643,8 @@ __global__ void __launch_bounds__(kMergeThreads) fp8_merge_kernel(const __grid_c
     dst[1] = __floats2half2_rn(merged.A[2], merged.A[3]);
 }
 
-// The rotated queries of pkv_fp8_decode_layer, then the partials.
-constexpr int64_t kQueryRowBytes = kQueryHeads * kDim * 2;
+// The rotated queries of pkv_fp8_decode_layer (all high halves, then all low ones), then the partials.
+constexpr int64_t kQueryRowBytes = 2 * kQueryHeads * kDim * 2;
 
 int64_t workspace_of(int64_t batch, int64_t grid) {
     return batch * kQueryRowBytes + (grid > 1 ? (batch + grid) * kPartial * 4 : 0);
@@ -612,6 +654,15 @@ struct DeviceInfo {
     int sms = 0;
     int ctas_per_sm = 0;
 };
+
+cudaError_t prepare_kernel(void (*kernel)(Args), int *ctas_per_sm) {
+    cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem);
+    if (e == cudaSuccess) {
+        e = cudaFuncSetAttribute(kernel, cudaFuncAttributePreferredSharedMemoryCarveout, cudaSharedmemCarveoutMaxShared);
+    }
+    if (e == cudaSuccess) e = cudaOccupancyMaxActiveBlocksPerMultiprocessor(ctas_per_sm, kernel, kThreads, kSmem);
+    return e;
+}
 
 int device_info(int device, DeviceInfo *info) {
     static std::mutex mutex;
@@ -627,11 +678,9 @@ int device_info(int device, DeviceInfo *info) {
     DeviceInfo d;
     cudaError_t e = cudaSetDevice(device);
     if (e == cudaSuccess) e = cudaDeviceGetAttribute(&d.sms, cudaDevAttrMultiProcessorCount, device);
-    if (e == cudaSuccess) e = cudaFuncSetAttribute(fp8_decode_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem);
-    if (e == cudaSuccess) {
-        e = cudaFuncSetAttribute(fp8_decode_kernel, cudaFuncAttributePreferredSharedMemoryCarveout,
-                                 cudaSharedmemCarveoutMaxShared);
-    }
+    int ctas[2] = {0, 0};
+    if (e == cudaSuccess) e = prepare_kernel(fp8_decode_kernel<false>, &ctas[0]);
+    if (e == cudaSuccess) e = prepare_kernel(fp8_decode_kernel<true>, &ctas[1]);
     if (e == cudaSuccess) {
         // The merge keeps the split kernel's partition of L1 and shared memory.
         e = cudaFuncSetAttribute(fp8_merge_kernel<false>, cudaFuncAttributePreferredSharedMemoryCarveout,
@@ -641,7 +690,7 @@ int device_info(int device, DeviceInfo *info) {
         e = cudaFuncSetAttribute(fp8_merge_kernel<true>, cudaFuncAttributePreferredSharedMemoryCarveout,
                                  cudaSharedmemCarveoutMaxShared);
     }
-    if (e == cudaSuccess) e = cudaOccupancyMaxActiveBlocksPerMultiprocessor(&d.ctas_per_sm, fp8_decode_kernel, kThreads, kSmem);
+    d.ctas_per_sm = ctas[0] < ctas[1] ? ctas[0] : ctas[1];
     cudaSetDevice(previous);
     if (e != cudaSuccess) return pkv::fail(PKV_CUDA_ERROR, std::string("fp8 decode: ") + cudaGetErrorString(e));
     if (d.ctas_per_sm < 1) d.ctas_per_sm = 1;
@@ -698,8 +747,11 @@ int decode(const pkv::fp8::Cache &cache, int32_t layer, const void *query, int64
     if (e != cudaSuccess) return pkv::fail(PKV_CUDA_ERROR, std::string("cudaGetDevice: ") + cudaGetErrorString(e));
     DeviceInfo info;
     if ((rc = device_info(device, &info))) return rc;
+    const __half *query_low = nullptr;
     if (key != nullptr) {
-        rc = pkv::fp8::launch_decode_append(cache, layer, key, value, kv_stride, rope_table, query, query_stride, workspace,
+        __half *const low = static_cast<__half *>(workspace) + static_cast<int64_t>(batch) * kQueryHeads * kDim;
+        query_low = low;
+        rc = pkv::fp8::launch_decode_append(cache, layer, key, value, kv_stride, rope_table, query, query_stride, workspace, low,
                                             lengths, prefix, flat, batch, total_blocks, error_flag, stream);
         if (rc) return rc;
         query = workspace;
@@ -710,6 +762,7 @@ int decode(const pkv::fp8::Cache &cache, int32_t layer, const void *query, int64
     a.cache = cache;
     a.layer = layer;
     a.query = static_cast<const __half *>(query);
+    a.query_low = query_low;
     a.query_stride = query_stride;
     a.lengths = lengths;
     a.prefix = prefix;
@@ -734,7 +787,7 @@ int decode(const pkv::fp8::Cache &cache, int32_t layer, const void *query, int64
     attribute[0].val.programmaticStreamSerializationAllowed = 1;
     config.attrs = attribute;
     config.numAttrs = 1;
-    e = cudaLaunchKernelEx(&config, fp8_decode_kernel, a);
+    e = cudaLaunchKernelEx(&config, key != nullptr ? fp8_decode_kernel<true> : fp8_decode_kernel<false>, a);
     if (e == cudaSuccess && grid > 1) {
         // A CTA per (row, two heads) while that is at most two waves of CTAs: beyond it rows
         // have few pieces each and a warp merges them as fast.

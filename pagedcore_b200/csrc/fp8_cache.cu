@@ -50,6 +50,7 @@ struct AppendArgs {
     const __half *rope;  // FP16 cos [2048][32], sin [2048][32], or null
     const __half *query_in;
     __half *query_out;
+    __half *query_low;  // nullable, laid out as query_out: what FP16 left of each value
     int64_t q_layer_stride;
     int64_t q_token_stride;
     int64_t q_out_layer_stride;
@@ -257,7 +258,7 @@ __device__ void rotate_queries(const AppendArgs &a, int layer, int begin, int wa
     for (int j = 0; j < kQuerySpan; ++j) {
         const uint32_t x[4] = {own[j].x, own[j].y, own[j].z, own[j].w}, c[4] = {cos[j].x, cos[j].y, cos[j].z, cos[j].w},
                        s[4] = {sin[j].x, sin[j].y, sin[j].z, sin[j].w};
-        uint32_t r[4];
+        uint32_t r[4], low[4];
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
             const uint32_t p = __shfl_xor_sync(0xffffffffu, x[i], 4);
@@ -265,11 +266,18 @@ __device__ void rotate_queries(const AppendArgs &a, int layer, int begin, int wa
             const float2 pf = __half22float2(*reinterpret_cast<const __half2 *>(&p));
             const float2 cf = __half22float2(*reinterpret_cast<const __half2 *>(&c[i]));
             const float2 sf = __half22float2(*reinterpret_cast<const __half2 *>(&s[i]));
-            r[i] = pkv::pack_half2(__floats2half2_rn(xf.x * cf.x + sign * pf.x * sf.x, xf.y * cf.y + sign * pf.y * sf.y));
+            const float2 y = make_float2(xf.x * cf.x + sign * pf.x * sf.x, xf.y * cf.y + sign * pf.y * sf.y);
+            const __half2 h = __floats2half2_rn(y.x, y.y);
+            const float2 f = __half22float2(h);
+            r[i] = pkv::pack_half2(h);
+            low[i] = pkv::pack_half2(__floats2half2_rn(y.x - f.x, y.y - f.y));
         }
         if (here[j]) {
             const int64_t to = layer * a.q_out_layer_stride + (begin + j) * a.q_out_token_stride + at;
             *reinterpret_cast<uint4 *>(a.query_out + to) = make_uint4(r[0], r[1], r[2], r[3]);
+            if (a.query_low != nullptr) {
+                *reinterpret_cast<uint4 *>(a.query_low + to) = make_uint4(low[0], low[1], low[2], low[3]);
+            }
         }
     }
 }
@@ -395,9 +403,10 @@ int check_cache(const void *key_codes, const void *value_codes, const void *key_
     return PKV_OK;
 }
 
-// The new token of every row of a staged batch at `layer`: K rotated and V written, Q rotated to query_out.
+// The new token of every row of a staged batch at `layer`: K rotated and V written, Q
+// rotated to query_out + query_low (FP16 numbers that add up to the FP32 value).
 int launch_decode_append(const Cache &cache, int32_t layer, const void *key, const void *value, int64_t kv_stride,
-                         const void *rope_table, const void *query, int64_t query_stride, void *query_out,
+                         const void *rope_table, const void *query, int64_t query_stride, void *query_out, void *query_low,
                          const int32_t *lengths, const int32_t *prefix, const int32_t *flat, int32_t batch,
                          int32_t total_blocks, int32_t *error_flag, cudaStream_t stream) {
     if (!aligned16(key) || !aligned16(value) || kv_stride % 8 || !aligned16(rope_table)) {
@@ -413,6 +422,7 @@ int launch_decode_append(const Cache &cache, int32_t layer, const void *key, con
     a.rope = static_cast<const __half *>(rope_table);
     a.query_in = static_cast<const __half *>(query);
     a.query_out = static_cast<__half *>(query_out);
+    a.query_low = static_cast<__half *>(query_low);
     a.q_token_stride = query_stride;
     a.q_out_token_stride = PKV_QUERY_HEADS * PKV_HEAD_DIM;
     a.error_flag = error_flag;
@@ -467,6 +477,7 @@ extern "C" int pkv_fp8_append_kv(void *key_codes, void *value_codes, void *key_s
     a.rope = static_cast<const __half *>(rope_table);
     a.query_in = static_cast<const __half *>(query_in);
     a.query_out = static_cast<__half *>(query_out);
+    a.query_low = nullptr;
     a.q_layer_stride = q_layer_stride;
     a.q_token_stride = q_token_stride;
     a.q_out_layer_stride = q_out_layer_stride;

@@ -420,7 +420,7 @@ def decode_plan(device_index: int, batch: int, total_blocks: int) -> tuple[int, 
 
 def decode_workspace_bytes(batch: int, grid: int) -> int:
     """Workspace of a decode launch with ``grid`` pieces (rotated queries, then split partials)."""
-    return batch * _QUERY_HEADS * _HEAD_DIM * 2 + (batch + grid) * _QUERY_HEADS * (_HEAD_DIM + 2) * 4
+    return 2 * batch * _QUERY_HEADS * _HEAD_DIM * 2 + (batch + grid) * _QUERY_HEADS * (_HEAD_DIM + 2) * 4
 
 
 def _attention_rows(name: str, tensor: Tensor, shape: tuple[int, ...], index: int) -> None:

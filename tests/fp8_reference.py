@@ -99,14 +99,17 @@ class CacheOracle:
         return self.values[table].transpose(1, 2).reshape(-1, 4, 64)[:length]
 
 
-def attend64(query: torch.Tensor, key: torch.Tensor, value: torch.Tensor):
+def attend64(query: torch.Tensor, key: torch.Tensor, value: torch.Tensor, weight_error: float = 2.0**-21):
     """One query [32, 64] over K/V [tokens, 4, 64] (float64): output [32, 64] and its error bound.
 
-    The kernels round each softmax weight to FP16 (2^-11), sum 64 exact
-    products per score in FP32 (65 roundings of the summed magnitudes, 2^-24
-    each, and as much again for truncation inside the tensor core; the scale,
-    the subtraction of the maximum and 2^x add 2^-20 and two roundings of the
-    score), and round the output to FP16.
+    A softmax weight is off by ``weight_error`` as the second product takes it
+    (2^-22 and the rounding of its low half in the decode kernels, 2^-11 in the
+    prompt kernel), and by the error of its score: 64 exact products summed in
+    FP32 (65 roundings of the summed magnitudes, 2^-24 each, twice over for two
+    halves of a query, and as much again for truncation inside the tensor
+    core; the scale, the subtraction of the maximum and 2^x add 2^-20 and two
+    roundings of the score).  The second product sums in FP32 likewise, and the
+    output is rounded to FP16.
     """
     if key.shape[0] == 0:
         zero = torch.zeros(32, 64, dtype=torch.float64, device=query.device)
@@ -117,6 +120,7 @@ def attend64(query: torch.Tensor, key: torch.Tensor, value: torch.Tensor):
     weights = torch.softmax(scores, -1)
     out = weights @ v
     magnitude = (q.abs() @ k.abs().transpose(1, 2) / 8).amax(-1, keepdim=True)
-    off = 2 * 65 * F32 * magnitude + 2.0**-20 + 4 * F32 * scores.abs().amax(-1, keepdim=True)
-    bound = HALF_FP16 * out.abs() + (HALF_FP16 + 2 * off) * (weights @ v.abs()) + 2.0**-25
+    off = 4 * 65 * F32 * magnitude + 2.0**-20 + 4 * F32 * scores.abs().amax(-1, keepdim=True)
+    off = off + 2 * key.shape[0] * F32  # the sums over tokens
+    bound = HALF_FP16 * out.abs() + (weight_error + 2 * off) * (weights @ v.abs()) + 2.0**-25
     return out.reshape(32, 64), bound.reshape(32, 64)

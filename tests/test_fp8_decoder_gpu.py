@@ -42,15 +42,14 @@ def context(allocator: Fp8KVAllocator, request: RequestId, layer: int) -> tuple[
     return torch.cat([k for k, _ in pages]).double(), torch.cat([v for _, v in pages]).double()
 
 
-def assert_attends(allocator, requests, layer: int, query64: torch.Tensor, out: torch.Tensor) -> None:
-    """out [B, 32, 64] is the attention of ``query64`` (rounded to FP16 on the way) over what the cache holds."""
+def assert_attends(allocator, requests, layer: int, query: torch.Tensor, out: torch.Tensor) -> None:
+    """out [B, 32, 64] is the attention of ``query`` (FP16, or rotated in 64 bits) over what the cache holds."""
     for row, request in enumerate(requests):
         key, value = context(allocator, request, layer)
-        query = query64[row].half()
-        exact, bound = attend64(query, key, value)
-        # The kernel's FP32 rotation may round to the neighbouring FP16 number: 2^-11 of each score's magnitude.
-        q, k = query.double().view(4, 8, 64), key.transpose(0, 1)
-        moved = 2 * 2.0**-10 * (q.abs() @ k.abs().transpose(1, 2) / 8).amax(-1, keepdim=True)
+        exact, bound = attend64(query[row], key, value)
+        # The kernel's rotation: three FP32 roundings and two FP16 halves, of magnitudes at most sqrt(2) of the query's.
+        q, k = query[row].double().abs().amax(-1, keepdim=True).expand(32, 64).reshape(4, 8, 64), key.transpose(0, 1)
+        moved = 2 * 2.0**-20 * (q @ k.abs().transpose(1, 2) / 8).amax(-1, keepdim=True)
         bound = bound + (moved * value.abs().amax(0)[:, None]).reshape(32, 64)
         assert bool(((out[row].double() - exact).abs() <= bound).all()), (row, layer)
 

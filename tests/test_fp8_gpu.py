@@ -502,7 +502,7 @@ def test_a_block_outside_the_cache_sets_the_flag() -> None:
 
 
 @pytest.mark.parametrize("lengths", [[1], [16, 17], [1, 15, 16, 48, 700, 65], [2048, 3]], ids=str)
-def test_decode_layer_is_the_append_and_the_attention(lengths) -> None:
+def test_decode_layer_writes_as_append_does_and_attends(lengths) -> None:
     whole, parts = (CacheCase(21, [n - 1 for n in lengths]) for _ in range(2))
     for case in (whole, parts):
         for row, length in enumerate(lengths):
@@ -516,13 +516,21 @@ def test_decode_layer_is_the_append_and_the_attention(lengths) -> None:
     slots = torch.tensor([parts.slots(row, n - 1, 1)[0] for row, n in enumerate(lengths)], dtype=torch.int32,
                          device=parts.device)
     positions = torch.tensor(lengths, dtype=torch.int32, device=parts.device) - 1
-    rotated = fp8.append_kv(parts.cache, key[None], value[None], slots, layer_begin=LAYER, error_flag=parts.flag,
-                            positions=positions, rope_table=parts.rope, query=query[None])
-    expected = fp8.decode_attention(parts.cache, LAYER, rotated[0], *parts.batch(), parts.flag)
-    assert torch.equal(out, expected)
+    fp8.append_kv(parts.cache, key[None], value[None], slots, layer_begin=LAYER, error_flag=parts.flag,
+                  positions=positions, rope_table=parts.rope)
     for name in ("key_codes", "value_codes", "key_scales", "value_scales"):
         assert torch.equal(getattr(whole.cache, name).view(torch.uint8), getattr(parts.cache, name).view(torch.uint8))
     assert int(whole.flag.item()) == 0
+    # The query is rotated in FP32 and kept as two FP16 numbers: 2^-22 of it, and the rotation's 3 roundings.
+    rotated = rope64(query, whole.rope, positions.long())
+    for row, length in enumerate(lengths):
+        blocks = torch.tensor(whole.tables[row], dtype=torch.int32, device=whole.device)
+        k, v = (t.reshape(-1, 4, 64)[:length].double() for t in fp8.read_blocks(whole.cache, LAYER, blocks, whole.flag))
+        exact, bound = attend64(rotated[row], k, v)
+        size = (query[row].double().abs() + query[row].double().abs().roll(32, -1)).view(4, 8, 64)
+        moved = (4 * F32 + 2.0**-22) * (size @ k.transpose(0, 1).abs().transpose(1, 2) / 8).amax(-1, keepdim=True)
+        bound = bound + (2 * moved * v.abs().amax(0)[:, None]).reshape(32, 64)
+        assert bool(((out[row].double() - exact).abs() <= bound).all()), length
 
 
 def test_decode_layer_flags_a_row_without_a_token() -> None:
@@ -544,7 +552,7 @@ def test_prefill_attention(start, tokens) -> None:
     assert int(case.flag.item()) == 0
     for t in {0, 1, tokens // 2, tokens - 1} & set(range(tokens)):
         exact, bound = attend64(query[t], case.key.tokens(case.tables[0], start + t + 1),
-                                case.value.tokens(case.tables[0], start + t + 1))
+                                case.value.tokens(case.tables[0], start + t + 1), HALF_FP16)
         assert bool(((out[t].double() - exact).abs() <= bound).all()), t
 
 
