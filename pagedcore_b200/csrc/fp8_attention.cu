@@ -42,9 +42,9 @@
 #include <cuda_runtime.h>
 #include <stdint.h>
 
-#include <mutex>
+#include <atomic>
+#include <initializer_list>
 #include <string>
-#include <unordered_map>
 
 #include "fp8_cache.cuh"
 #include "pdl.h"
@@ -664,38 +664,38 @@ cudaError_t prepare_kernel(void (*kernel)(Args), int *ctas_per_sm) {
     return e;
 }
 
+constexpr int kMaxDevices = 64;
+
+// SMs and resident CTAs of `device`, found out (and the kernels' attributes set) at its first use.
 int device_info(int device, DeviceInfo *info) {
-    static std::mutex mutex;
-    static std::unordered_map<int, DeviceInfo> cache;
-    std::lock_guard<std::mutex> lock(mutex);
-    auto it = cache.find(device);
-    if (it != cache.end()) {
-        *info = it->second;
+    static std::atomic<int> sms[kMaxDevices] = {}, ctas[kMaxDevices] = {};
+    const bool known = device >= 0 && device < kMaxDevices;
+    if (known && ctas[device].load(std::memory_order_acquire) > 0) {
+        info->sms = sms[device].load(std::memory_order_relaxed);
+        info->ctas_per_sm = ctas[device].load(std::memory_order_relaxed);
         return PKV_OK;
     }
-    int previous = 0;
-    cudaGetDevice(&previous);
-    DeviceInfo d;
-    cudaError_t e = cudaSetDevice(device);
-    if (e == cudaSuccess) e = cudaDeviceGetAttribute(&d.sms, cudaDevAttrMultiProcessorCount, device);
-    int ctas[2] = {0, 0};
-    if (e == cudaSuccess) e = prepare_kernel(fp8_decode_kernel<false>, &ctas[0]);
-    if (e == cudaSuccess) e = prepare_kernel(fp8_decode_kernel<true>, &ctas[1]);
-    if (e == cudaSuccess) {
-        // The merge keeps the split kernel's partition of L1 and shared memory.
-        e = cudaFuncSetAttribute(fp8_merge_kernel<false>, cudaFuncAttributePreferredSharedMemoryCarveout,
-                                 cudaSharedmemCarveoutMaxShared);
+    int previous = 0, plain = 0, split = 0;
+    cudaError_t e = cudaGetDevice(&previous);
+    if (e == cudaSuccess) e = cudaSetDevice(device);
+    if (e != cudaSuccess) return pkv::fail(PKV_CUDA_ERROR, std::string("fp8 decode: ") + cudaGetErrorString(e));
+    e = cudaDeviceGetAttribute(&info->sms, cudaDevAttrMultiProcessorCount, device);
+    if (e == cudaSuccess) e = prepare_kernel(fp8_decode_kernel<false>, &plain);
+    if (e == cudaSuccess) e = prepare_kernel(fp8_decode_kernel<true>, &split);
+    // The merge keeps the split kernel's partition of L1 and shared memory.
+    for (const auto merge : {fp8_merge_kernel<false>, fp8_merge_kernel<true>}) {
+        if (e == cudaSuccess) {
+            e = cudaFuncSetAttribute(merge, cudaFuncAttributePreferredSharedMemoryCarveout, cudaSharedmemCarveoutMaxShared);
+        }
     }
-    if (e == cudaSuccess) {
-        e = cudaFuncSetAttribute(fp8_merge_kernel<true>, cudaFuncAttributePreferredSharedMemoryCarveout,
-                                 cudaSharedmemCarveoutMaxShared);
-    }
-    d.ctas_per_sm = ctas[0] < ctas[1] ? ctas[0] : ctas[1];
     cudaSetDevice(previous);
     if (e != cudaSuccess) return pkv::fail(PKV_CUDA_ERROR, std::string("fp8 decode: ") + cudaGetErrorString(e));
-    if (d.ctas_per_sm < 1) d.ctas_per_sm = 1;
-    cache.emplace(device, d);
-    *info = d;
+    const int least = plain < split ? plain : split;
+    info->ctas_per_sm = least < 1 ? 1 : least;
+    if (known) {
+        sms[device].store(info->sms, std::memory_order_relaxed);
+        ctas[device].store(info->ctas_per_sm, std::memory_order_release);
+    }
     return PKV_OK;
 }
 

@@ -29,10 +29,7 @@
 #include <stdint.h>
 
 #include <atomic>
-#include <functional>
-#include <mutex>
 #include <string>
-#include <unordered_map>
 
 #include "pagedkv.h"
 #include "ptx.cuh"
@@ -137,6 +134,13 @@ __device__ __forceinline__ float4 cluster_sum(uint32_t addr, int splits) {
     return v;
 }
 
+// Bring a box into L2 (a hint: no data is used, so nothing has to be waited for first).
+__device__ __forceinline__ void tma_prefetch_2d(const CUtensorMap *map, int32_t c0, int32_t c1) {
+    asm volatile("cp.async.bulk.prefetch.tensor.2d.L2.global [%0, {%1, %2}];" ::"l"(reinterpret_cast<uint64_t>(map)),
+                 "r"(c0), "r"(c1)
+                 : "memory");
+}
+
 // Four outputs of row m at column n (a multiple of 4), rounded to FP16.
 __device__ __forceinline__ void store4(const LinearArgs &a, int m, int n, const float4 &v) {
     __half *dst = a.out + static_cast<int64_t>(m) * a.out_stride + n;
@@ -206,22 +210,15 @@ __global__ void __launch_bounds__(Shape<NT>::kThreads, 2)
         int issued = 0;
         if (lane == 0) {
             const uint64_t reused = pkv::l2_policy_evict_last();
-            // The weight is no kernel's output: the first stages' weight boxes go out before the wait.
-            const int early = min(count, S::kStages);
-            for (int i = 0; i < early; ++i) {
-                const uint32_t bar = pkv::smem_addr(&full[i]);
-                pkv::mbar_arrive_expect_tx(bar, S::kStageBytes);
-                pkv::tma_load_2d(base + i * S::kStageBytes, &w_map, (kb_begin + i) * kKBlock, n0, bar);
-            }
-            issued = early;
+            // The weight's first boxes start towards L2 while the kernel before this one ends.
+            for (int i = 0; i < min(count, S::kStages); ++i) tma_prefetch_2d(&w_map, (kb_begin + i) * kKBlock, n0);
             pkv::pdl_wait();
-            for (int i = 0; i < early; ++i) {
-                pkv::tma_load_2d_hint(base + i * S::kStageBytes + kWBytes, &x_map, (kb_begin + i) * kKBlock, m0,
-                                      pkv::smem_addr(&full[i]), reused);
-            }
-            for (int i = early; i < count; ++i) {
+            for (int i = 0; i < count; ++i) {
                 const int st = i % S::kStages;
-                if (!wait_bounded(pkv::smem_addr(&empty[st]), ((i / S::kStages) - 1) & 1, a.error_flag)) break;
+                if (i >= S::kStages &&
+                    !wait_bounded(pkv::smem_addr(&empty[st]), ((i / S::kStages) - 1) & 1, a.error_flag)) {
+                    break;
+                }
                 issued = i + 1;
                 const uint32_t bar = pkv::smem_addr(&full[st]);
                 pkv::mbar_arrive_expect_tx(bar, S::kStageBytes);
@@ -485,6 +482,12 @@ __global__ void __launch_bounds__(RowsShape<N>::kThreads, 1)
             const uint64_t reused = pkv::l2_policy_evict_last();
             int issued = 0;
             bool ok = true;
+            if (first_tile < a.tiles) {  // the weight's first boxes start towards L2 while the kernel before this one ends
+                for (int i = 0; i < min(count, S::kStages); ++i) {
+                    tma_prefetch_2d(&w_map, (kb_begin + i) * kKBlock, first_tile / a.m_tiles * N);
+                }
+            }
+            pkv::pdl_wait();
             for (int tile = first_tile; ok && tile < a.tiles; tile += tile_step) {
                 const int m0 = tile % a.m_tiles * kTileRows, n0 = tile / a.m_tiles * N;
                 for (int i = 0; i < count; ++i) {
@@ -496,9 +499,7 @@ __global__ void __launch_bounds__(RowsShape<N>::kThreads, 1)
                     }
                     const uint32_t dst = base + st * S::kStageBytes, bar = pkv::smem_addr(&full[st]);
                     pkv::mbar_arrive_expect_tx(bar, S::kStageBytes);
-                    // The weight is no kernel's output: the first box goes out before the wait.
                     pkv::tma_load_2d(dst + S::kXBytes, &w_map, (kb_begin + i) * kKBlock, n0, bar);
-                    if (issued == 0) pkv::pdl_wait();
                     pkv::tma_load_2d_hint(dst, &x_map, (kb_begin + i) * kKBlock, m0, bar, reused);
                     ++issued;
                 }
@@ -859,32 +860,10 @@ __global__ void __launch_bounds__(PairShape::kThreads, 1)
 // ---------------------------------------------------------------------------
 constexpr int kMaxDevices = 64;
 
-struct MapKey {
-    uintptr_t base;
-    uint64_t rows, cols, stride;
-    uint32_t box_rows;
-    bool operator==(const MapKey &o) const {
-        return base == o.base && rows == o.rows && cols == o.cols && stride == o.stride && box_rows == o.box_rows;
-    }
-};
-struct MapKeyHash {
-    size_t operator()(const MapKey &k) const {
-        return std::hash<uintptr_t>()(k.base) ^ (k.rows << 7) ^ (k.cols << 19) ^ (k.stride << 31) ^ k.box_rows;
-    }
-};
-
-// A map holds an address and a shape only, so one that is found again is the one that would be made.
+// Map of an 8-bit matrix (rows `stride` bytes apart) in boxes of box_rows x 128 bytes with
+// the 128-byte swizzle; what lies outside reads as zeros.
 int byte_matrix_map(const void *base, uint64_t rows, uint64_t cols, uint64_t stride, uint32_t box_rows,
                     CUtensorMap *out) {
-    static std::mutex mutex;
-    static std::unordered_map<MapKey, CUtensorMap, MapKeyHash> cache;
-    const MapKey key{reinterpret_cast<uintptr_t>(base), rows, cols, stride, box_rows};
-    std::lock_guard<std::mutex> lock(mutex);
-    auto it = cache.find(key);
-    if (it != cache.end()) {
-        *out = it->second;
-        return PKV_OK;
-    }
     const pkv::EncodeTiled encode = pkv::encode_fn();
     if (encode == nullptr) return pkv::fail(PKV_CUDA_ERROR, "cuTensorMapEncodeTiled is unavailable");
     const cuuint64_t dims[2] = {cols, rows};
@@ -897,8 +876,6 @@ int byte_matrix_map(const void *base, uint64_t rows, uint64_t cols, uint64_t str
     if (r != CUDA_SUCCESS) {
         return pkv::fail(PKV_CUDA_ERROR, "cuTensorMapEncodeTiled (8-bit matrix) failed with code " + std::to_string(int(r)));
     }
-    if (cache.size() > 4096) cache.clear();
-    cache.emplace(key, *out);
     return PKV_OK;
 }
 

@@ -73,12 +73,6 @@ __global__ void __launch_bounds__(kThreads) norm_kernel(const __half *__restrict
     __shared__ float partial[kThreads / 32];
     const int chunks = dim / kChunk;
     uint4 wraw[CHUNKS];
-#pragma unroll
-    for (int j = 0; j < CHUNKS; ++j) {
-        // The weight is no kernel's output: it is read before the wait.
-        const int c = threadIdx.x + j * kThreads;
-        if (c < chunks) wraw[j] = *reinterpret_cast<const uint4 *>(weight + c * kChunk);
-    }
     pkv::pdl_launch_dependents();
     pkv::pdl_wait();
     const int64_t base = static_cast<int64_t>(blockIdx.x) * dim;
@@ -88,6 +82,7 @@ __global__ void __launch_bounds__(kThreads) norm_kernel(const __half *__restrict
     for (int j = 0; j < CHUNKS; ++j) {
         const int c = threadIdx.x + j * kThreads;
         if (c < chunks) {
+            wraw[j] = *reinterpret_cast<const uint4 *>(weight + c * kChunk);
             unpack8(*reinterpret_cast<const uint4 *>(hidden + base + c * kChunk), v[j]);
             if (delta != nullptr) {
                 float d[kChunk];

@@ -33,6 +33,10 @@ _QUERY_HEADS = 32
 _HEAD_DIM = 64
 _BLOCK_TOKENS = 16
 _CODES = torch.float8_e4m3fn
+_HALF = torch.float16
+_FLOAT = torch.float32
+_INT = torch.int32
+_ROW = _QUERY_HEADS * _HEAD_DIM  # values of a query row
 
 
 def _groups(width: int) -> int:
@@ -83,10 +87,10 @@ class Fp8Rows:
         if not self.codes.is_contiguous():
             raise ValueError("to_half needs contiguous codes")
         if out is None:
-            out = self.codes.new_empty((rows, width), dtype=torch.float16)
+            out = self.codes.new_empty((rows, width), dtype=_HALF)
             stride = width
         else:
-            if out.shape != (rows, width) or out.dtype != torch.float16 or out.stride(1) != 1 or out.get_device() != index:
+            if out.shape != (rows, width) or out.dtype is not _HALF or out.stride(1) != 1 or out.get_device() != index:
                 raise ValueError(f"out must be FP16 [{rows}, {width}] with contiguous rows")
             stride = max(out.stride(0), width)
         if rows:
@@ -109,10 +113,10 @@ class Fp8Weight:
 
 def _check_rows(x: Fp8Rows) -> tuple[int, int]:
     codes, scales = x.codes, x.scales
-    if codes.ndim != 2 or codes.dtype != _CODES or codes.stride(1) != 1:
+    if codes.ndim != 2 or codes.dtype is not _CODES or codes.stride(1) != 1:
         raise ValueError("8-bit rows must be E4M3 [rows, width] with contiguous rows")
     rows, width = codes.shape
-    if scales.shape != (rows, _groups(width)) or scales.dtype != torch.float32 or not scales.is_contiguous():
+    if scales.shape != (rows, _groups(width)) or scales.dtype is not _FLOAT or not scales.is_contiguous():
         raise ValueError("8-bit rows need contiguous FP32 scales [rows, ceil(width / 128)]")
     return rows, width
 
@@ -120,12 +124,12 @@ def _check_rows(x: Fp8Rows) -> tuple[int, int]:
 def _empty_rows(x: Tensor, rows: int, width: int) -> Fp8Rows:
     """Uninitialised 8-bit rows on the device of ``x``."""
     return Fp8Rows(
-        x.new_empty((rows, width), dtype=_CODES), x.new_empty((rows, _groups(width)), dtype=torch.float32)
+        x.new_empty((rows, width), dtype=_CODES), x.new_empty((rows, _groups(width)), dtype=_FLOAT)
     )
 
 
 def _half_matrix(name: str, tensor: Tensor, shape: tuple[int, ...]) -> None:
-    if tensor.shape != shape or tensor.dtype != torch.float16 or not tensor.is_contiguous():
+    if tensor.shape != shape or tensor.dtype is not _HALF or not tensor.is_contiguous():
         raise ValueError(f"{name} must be contiguous FP16 {list(shape)}")
 
 
@@ -199,10 +203,13 @@ def quantize_weight(weight: Tensor) -> Fp8Weight:
     padded = torch.zeros((tall * GROUP, wide * GROUP), dtype=torch.float32, device=weight.device)
     padded[:n, :k] = weight.detach().float()
     blocks = padded.view(tall, GROUP, wide, GROUP)
-    mantissa, exponent = torch.frexp(blocks.abs().amax((1, 3)))
+    finite = blocks.isfinite()
+    mantissa, exponent = torch.frexp(torch.where(finite, blocks.abs(), 0.0).amax((1, 3)))
     exponent = (exponent - 9 + (mantissa > 0.875).int()).clamp(-15, 8)  # 448 = 0.875 * 2^9
     scales = torch.ldexp(torch.ones_like(mantissa), exponent)
-    scaled = (blocks / scales[:, None, :, None]).clamp(-448.0, 448.0).to(_CODES)
+    largest = torch.where(exponent == 8, 240.0, 448.0)[:, None, :, None]  # at 2^8 the values end inside FP16
+    scaled = torch.minimum(torch.maximum(blocks / scales[:, None, :, None], -largest), largest)
+    scaled = torch.where(finite, scaled, torch.nan).to(_CODES)
     codes = scaled.view(torch.uint8).reshape(tall * GROUP, wide * GROUP)[:n, :k].contiguous().view(_CODES)
     return Fp8Weight(codes, scales.contiguous())
 
@@ -215,17 +222,17 @@ def linear(x: Fp8Rows, weight: Fp8Weight, out: Tensor | None = None) -> Tensor:
     """
     rows, k = _check_rows(x)
     codes, scales = weight.codes, weight.scales
-    if codes.ndim != 2 or codes.shape[1] != k or codes.dtype != _CODES or not codes.is_contiguous():
+    if codes.ndim != 2 or codes.shape[1] != k or codes.dtype is not _CODES or not codes.is_contiguous():
         raise ValueError(f"weight must be contiguous E4M3 [n, {k}]")
     n = codes.shape[0]
-    if scales.shape != (_groups(n), _groups(k)) or scales.dtype != torch.float32 or not scales.is_contiguous():
+    if scales.shape != (_groups(n), _groups(k)) or scales.dtype is not _FLOAT or not scales.is_contiguous():
         raise ValueError("weight needs contiguous FP32 scales [ceil(n / 128), ceil(k / 128)]")
     index = _device(x.codes, x.scales, codes, scales)
     if out is None:
-        out = codes.new_empty((rows, n), dtype=torch.float16)
+        out = codes.new_empty((rows, n), dtype=_HALF)
         stride = n
     else:
-        if out.shape != (rows, n) or out.dtype != torch.float16 or out.stride(1) != 1 or out.get_device() != index:
+        if out.shape != (rows, n) or out.dtype is not _HALF or out.stride(1) != 1 or out.get_device() != index:
             raise ValueError(f"out must be FP16 [{rows}, {n}] with contiguous rows")
         stride = max(out.stride(0), n)
     if rows:
@@ -266,7 +273,7 @@ class Fp8Cache:
             raise ValueError("cache codes must be contiguous E4M3 storage")
         scales = (layers, blocks, _KV_HEADS)
         for tensor in (key_scales, value_scales):
-            if tensor.shape != scales or tensor.dtype != torch.float32 or not tensor.is_contiguous():
+            if tensor.shape != scales or tensor.dtype is not _FLOAT or not tensor.is_contiguous():
                 raise ValueError("cache scales must be contiguous FP32 [layers, blocks, 4]")
         _device(keys, values, key_scales, value_scales)
 
@@ -299,32 +306,30 @@ class Fp8Cache:
 
 
 def _half(name: str, tensor: Tensor, index: int) -> None:
-    if tensor.dtype != torch.float16 or tensor.get_device() != index:
+    if tensor.dtype is not _HALF or tensor.get_device() != index:
         raise ValueError(f"{name} must be FP16 on cuda:{index}")
 
 
 def _int_list(index: int, name: str, tensor: Tensor, count: int) -> int:
     """Address of ``count`` or more int32 values on the device."""
-    if (
-        tensor.dtype != torch.int32
-        or tensor.numel() < count
-        or not tensor.is_contiguous()
-        or tensor.get_device() != index
-    ):
-        raise ValueError(f"{name} must hold {count} contiguous int32 values on cuda:{index}")
-    return tensor.data_ptr()
+    if tensor.dtype is _INT and tensor.numel() >= count and tensor.get_device() == index and tensor.is_contiguous():
+        return tensor.data_ptr()
+    raise ValueError(f"{name} must hold {count} contiguous int32 values on cuda:{index}")
 
 
 def _check_rope(index: int, table: Tensor) -> int:
-    _half("rope_table", table, index)
-    if table.shape != (2, 2048, 32) or not table.is_contiguous():
-        raise ValueError("rope_table must be contiguous FP16 [2, 2048, 32]")
-    return table.data_ptr()
+    if (
+        table.dtype is _HALF
+        and table.get_device() == index
+        and table.shape == (2, 2048, 32)
+        and table.is_contiguous()
+    ):
+        return table.data_ptr()
+    raise ValueError(f"rope_table must be contiguous FP16 [2, 2048, 32] on cuda:{index}")
 
 
-def _rows_ok(tensor: Tensor) -> bool:
+def _rows_ok(tensor: Tensor, strides: tuple[int, ...]) -> bool:
     """Inner [heads, 64] contiguous and rows 16-byte aligned."""
-    strides = tensor.stride()
     return (
         strides[-1] == 1
         and strides[-2] == _HEAD_DIM
@@ -332,6 +337,15 @@ def _rows_ok(tensor: Tensor) -> bool:
         and strides[-3] % 8 == 0
         and tensor.data_ptr() % 16 == 0
     )
+
+
+def _aligned_pair(key: Tensor, value: Tensor) -> tuple[Tensor, Tensor, tuple[int, ...]]:
+    """K and V with common strides that the kernels take (copies where they are not), and those strides."""
+    strides = key.stride()
+    if not (value.stride() == strides and _rows_ok(key, strides) and value.data_ptr() % 16 == 0):
+        key, value = key.contiguous(), value.contiguous()
+        strides = key.stride()
+    return key, value, strides
 
 
 def append_kv(
@@ -377,19 +391,18 @@ def append_kv(
         _half("query", query, index)
         if query_out is None:
             query_out = torch.empty_like(query, memory_format=torch.contiguous_format)
-        elif query_out.shape != query.shape or not _rows_ok(query_out):
+        elif query_out.shape != query.shape or not _rows_ok(query_out, query_out.stride()):
             raise ValueError("query_out must be FP16 [layers, tokens, 32, 64] with contiguous, 16-byte aligned rows")
         else:
             _half("query_out", query_out, index)
-        if not _rows_ok(query):
+        if not _rows_ok(query, query.stride()):
             query = query.contiguous()
         q_ptr, out_ptr = query.data_ptr(), query_out.data_ptr()
         q_strides, out_strides = query.stride()[:2], query_out.stride()[:2]
     if layers == 0 or tokens == 0:
         return query_out
-    if not (_rows_ok(key) and value.stride() == key.stride() and _rows_ok(value)):
-        key, value = key.contiguous(), value.contiguous()
-    layer_stride, token_stride = key.stride()[:2]
+    key, value, strides = _aligned_pair(key, value)
+    layer_stride, token_stride = strides[0], strides[1]
     _call(index, lib.pkv_fp8_append_kv, *cache._args(), layer_begin, layers, key.data_ptr(), value.data_ptr(),
           layer_stride, token_stride, slots_ptr, positions_ptr, tokens, rope, q_ptr, *q_strides, out_ptr, *out_strides,
           flag)
@@ -402,7 +415,7 @@ def read_blocks(cache: Fp8Cache, layer: int, blocks: Tensor, error_flag: Tensor)
     count = blocks.numel()
     blocks_ptr = _int_list(index, "blocks", blocks, count)
     flag = _int_list(index, "error_flag", error_flag, 1)
-    key = blocks.new_empty((count, _BLOCK_TOKENS, _KV_HEADS, _HEAD_DIM), dtype=torch.float16)
+    key = blocks.new_empty((count, _BLOCK_TOKENS, _KV_HEADS, _HEAD_DIM), dtype=_HALF)
     value = torch.empty_like(key)
     if count:
         _call(index, lib.pkv_fp8_read_blocks, *cache._args(), layer, blocks_ptr, count, key.data_ptr(),
@@ -424,7 +437,7 @@ def decode_workspace_bytes(batch: int, grid: int) -> int:
 
 
 def _attention_rows(name: str, tensor: Tensor, shape: tuple[int, ...], index: int) -> None:
-    if tensor.shape != shape or tensor.dtype != torch.float16 or tensor.get_device() != index:
+    if tensor.shape != shape or tensor.dtype is not _HALF or tensor.get_device() != index:
         raise ValueError(f"{name} must be FP16 {list(shape)} on cuda:{index}")
 
 
@@ -434,16 +447,18 @@ def _query_and_out(query: Tensor, out: Tensor | None, index: int, rows: str) -> 
     if len(shape) != 3 or shape[0] < 1 or shape[1] != _QUERY_HEADS or shape[2] != _HEAD_DIM:
         raise ValueError(f"query must be FP16 [{rows}, 32, 64] of a nonempty {rows}")
     _half("query", query, index)
-    if not _rows_ok(query) or query.stride(0) < _QUERY_HEADS * _HEAD_DIM:
+    strides = query.stride()
+    if not _rows_ok(query, strides) or strides[0] < _ROW:
         query = query.contiguous()
-    stride = max(query.stride(0), _QUERY_HEADS * _HEAD_DIM)  # of one row it may be anything
+        strides = query.stride()
+    stride = max(strides[0], _ROW)  # of one row it may be anything
     if out is None:
-        out = torch.empty_like(query, memory_format=torch.contiguous_format)
-        return query, stride, out, _QUERY_HEADS * _HEAD_DIM
+        return query, stride, torch.empty_like(query, memory_format=torch.contiguous_format), _ROW
     _attention_rows("out", out, shape, index)
-    if not _rows_ok(out):
+    strides = out.stride()
+    if not _rows_ok(out, strides):
         raise ValueError(f"out must be FP16 [{rows}, 32, 64] with contiguous, 16-byte aligned rows")
-    return query, stride, out, max(out.stride(0), _QUERY_HEADS * _HEAD_DIM)
+    return query, stride, out, max(strides[0], _ROW)
 
 
 def _decode(cache, layer, query, new, lengths, prefix, flat, total_blocks, error_flag, out) -> Tensor:
@@ -508,9 +523,8 @@ def decode_layer(
     _attention_rows("key", key, shape, index)
     _attention_rows("value", value, shape, index)
     rope = _check_rope(index, rope_table)
-    if not (_rows_ok(key) and value.stride() == key.stride() and _rows_ok(value)):
-        key, value = key.contiguous(), value.contiguous()
-    new = (key.data_ptr(), value.data_ptr(), key.stride(0), rope)
+    key, value, strides = _aligned_pair(key, value)
+    new = (key.data_ptr(), value.data_ptr(), strides[0], rope)
     return _decode(cache, layer, query, new, lengths, prefix, flat, total_blocks, error_flag, out)
 
 

@@ -115,3 +115,14 @@ def test_quantize_weight_is_one_rounding_with_the_block_scale(n, k) -> None:
     assert torch.equal(result.scales.double(), scales)
     each = scales.repeat_interleave(128, 0)[:n].repeat_interleave(128, 1)[:, :k]
     assert torch.equal(result.codes.double() * each, round_e4m3(weight.double(), each))
+
+
+def test_quantize_weight_at_the_ends_of_the_range() -> None:
+    weight = torch.zeros(2, 144)
+    weight[0, :4] = torch.tensor([70000.0, -1.0, float("inf"), 3.0])
+    weight[1, 130:133] = torch.tensor([float("nan"), 2.0**-30, 0.0])
+    result = fp8.quantize_weight(weight)
+    assert result.scales.tolist() == [[256.0, 2.0**-15]]
+    values = result.codes.float() * torch.tensor([[256.0] * 128 + [2.0**-15] * 16])
+    assert values[0, 0] == 61440 and values[0, 2].isnan() and values[1, 130].isnan()
+    assert values[1, 131] == 0 and values[0, 3] == 3.0
