@@ -8,7 +8,7 @@
 // token to the same slot twice leaves the same bytes.
 //
 // A CTA takes one token of a layer (eight of a long list) with a warp per (K or V,
-// head); others, ahead of them in the grid, rotate the queries.  The warps of a token
+// head); others, behind them in the grid, rotate the queries.  The warps of a token
 // that opens a run (the first token, or one whose slot does not follow the
 // previous token's within its block) write the whole run; the tokens of a run
 // are those that follow it slot by slot in the block.  K: lane (r, h) holds the
@@ -62,8 +62,8 @@ struct AppendArgs {
     const int32_t *prefix;
     const int32_t *flat;
     int32_t total_blocks;
-    int32_t q_ctas;  // CTAs that rotate queries, ahead of those that write K and V
-    int32_t span;    // tokens per CTA of the latter
+    int32_t tile_ctas;  // CTAs that write K and V; those that rotate queries come after them in the grid
+    int32_t span;       // tokens per CTA of the former
 };
 
 constexpr int kQuerySpan = 4;  // tokens per CTA that rotates queries
@@ -284,9 +284,9 @@ __device__ void rotate_queries(const AppendArgs &a, int layer, int begin, int wa
 
 // The grid for `tokens`: eight tokens a CTA (of a prompt every sixteenth opens a run) once there are enough CTAs to fill the SMs.
 dim3 append_grid(AppendArgs &a, int layers) {
-    a.q_ctas = a.query_in != nullptr ? (a.tokens + kQuerySpan - 1) / kQuerySpan : 0;
     a.span = a.lengths == nullptr && a.tokens >= 512 ? 8 : 1;
-    return dim3(a.q_ctas + (a.tokens + a.span - 1) / a.span, layers);
+    a.tile_ctas = (a.tokens + a.span - 1) / a.span;
+    return dim3(a.tile_ctas + (a.query_in != nullptr ? (a.tokens + kQuerySpan - 1) / kQuerySpan : 0), layers);
 }
 
 __global__ void __launch_bounds__(kThreads, 3) fp8_append_kernel(const __grid_constant__ AppendArgs a) {
@@ -296,11 +296,11 @@ __global__ void __launch_bounds__(kThreads, 3) fp8_append_kernel(const __grid_co
     pkv::pdl_launch_dependents();
     const int layer = blockIdx.y;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    if (static_cast<int>(blockIdx.x) < a.q_ctas) {
-        rotate_queries(a, layer, blockIdx.x * kQuerySpan, warp, lane);
+    if (static_cast<int>(blockIdx.x) >= a.tile_ctas) {
+        rotate_queries(a, layer, (static_cast<int>(blockIdx.x) - a.tile_ctas) * kQuerySpan, warp, lane);
         return;
     }
-    const int begin = (static_cast<int>(blockIdx.x) - a.q_ctas) * a.span;
+    const int begin = static_cast<int>(blockIdx.x) * a.span;
     // Slots of the tokens from begin - 1 on: a span's runs end 15 tokens past it.
     const int near = begin - 1 + lane;
     int slot_at = -1;
