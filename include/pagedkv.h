@@ -423,7 +423,7 @@ int pkv_fp8_linear(const void *x, int64_t x_stride, const void *x_scales, const 
  *
  * pkv_append_kv into it: as there, for pool layers layer_begin .. + layer_count
  * of the cache.  RoPE is computed in FP32 and rounded once (K to its code, the
- * query to FP16).  The tokens written to one block in one call must be
+ * query to FP16), or with query_out_fp32 the query not at all (query_out FP32).  The tokens written to one block in one call must be
  * consecutive in the list and in the block, which the slots of a request's
  * consecutive positions are.  A block's slot 0 sets its scale; a later slot
  * raises it where it needs more, and the block's codes are rounded again to it.
@@ -432,8 +432,8 @@ int pkv_fp8_append_kv(void *key_codes, void *value_codes, void *key_scales, void
                       int32_t num_blocks, int32_t layer_begin, int32_t layer_count, const void *key, const void *value,
                       int64_t src_layer_stride, int64_t src_token_stride, const int32_t *slots,
                       const int32_t *positions, int32_t tokens, const void *rope_table, const void *query_in,
-                      int64_t q_layer_stride, int64_t q_token_stride, void *query_out, int64_t q_out_layer_stride,
-                      int64_t q_out_token_stride, int32_t *error_flag, void *stream);
+                      int64_t q_layer_stride, int64_t q_token_stride, void *query_out, int32_t query_out_fp32,
+                      int64_t q_out_layer_stride, int64_t q_out_token_stride, int32_t *error_flag, void *stream);
 
 /* K and V of `count` blocks (device int32) at `layer` as FP16 [count][16][4][64]
  * each, 16-byte aligned. */
@@ -443,13 +443,15 @@ int pkv_fp8_read_blocks(const void *key_codes, const void *value_codes, const vo
                         void *stream);
 
 /* pkv_prefill_attention over the 8-bit cache: same arguments and result over the
- * values that the cache holds.  The workspace (16-byte aligned, 16388 bytes for
- * each of the ceil((start + tokens) / 16) blocks) needs no initialisation. */
+ * values that the cache holds; the query FP16 or, with query_fp32, FP32 (taken
+ * as it is; rows query_stride values apart).  The workspace (16-byte aligned,
+ * 16388 bytes for each of the ceil((start + tokens) / 16) blocks) needs no
+ * initialisation. */
 int pkv_fp8_prefill_attention(const void *key_codes, const void *value_codes, const void *key_scales,
                               const void *value_scales, int32_t layers, int32_t num_blocks, int32_t layer,
-                              const void *query, int64_t query_stride, const int32_t *blocks, int32_t start,
-                              int32_t tokens, void *out, int64_t out_stride, void *workspace, int64_t workspace_bytes,
-                              int32_t *error_flag, void *stream);
+                              const void *query, int32_t query_fp32, int64_t query_stride, const int32_t *blocks,
+                              int32_t start, int32_t tokens, void *out, int64_t out_stride, void *workspace,
+                              int64_t workspace_bytes, int32_t *error_flag, void *stream);
 
 /* Grid and workspace of the two functions below on `device`. */
 int pkv_fp8_decode_plan(int32_t device, int32_t batch, int32_t total_blocks, int32_t *out_grid,

@@ -116,6 +116,7 @@ SIGNATURES: dict[str, tuple[object, list[object]]] = {
             c_int64,  # q_layer_stride
             c_int64,  # q_token_stride
             c_void_p,  # query_out
+            c_int32,  # query_out_fp32
             c_int64,  # q_out_layer_stride
             c_int64,  # q_out_token_stride
             c_void_p,  # error_flag
@@ -132,6 +133,7 @@ SIGNATURES: dict[str, tuple[object, list[object]]] = {
             *_FP8_CACHE,
             c_int32,  # layer
             c_void_p,  # query
+            c_int32,  # query_fp32
             c_int64,  # query_stride
             c_void_p,  # blocks
             c_int32,  # start

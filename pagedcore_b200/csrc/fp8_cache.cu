@@ -50,7 +50,8 @@ struct AppendArgs {
     const __half *rope;  // FP16 cos [2048][32], sin [2048][32], or null
     const __half *query_in;
     __half *query_out;
-    __half *query_low;  // nullable, laid out as query_out: what FP16 left of each value
+    __half *query_low;   // nullable, laid out as query_out: what FP16 left of each value
+    float *query_out32;  // in place of query_out: the rotated queries in FP32
     int64_t q_layer_stride;
     int64_t q_token_stride;
     int64_t q_out_layer_stride;
@@ -258,7 +259,7 @@ __device__ void rotate_queries(const AppendArgs &a, int layer, int begin, int wa
     for (int j = 0; j < kQuerySpan; ++j) {
         const uint32_t x[4] = {own[j].x, own[j].y, own[j].z, own[j].w}, c[4] = {cos[j].x, cos[j].y, cos[j].z, cos[j].w},
                        s[4] = {sin[j].x, sin[j].y, sin[j].z, sin[j].w};
-        uint32_t r[4], low[4];
+        float2 y[4];
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
             const uint32_t p = __shfl_xor_sync(0xffffffffu, x[i], 4);
@@ -266,18 +267,27 @@ __device__ void rotate_queries(const AppendArgs &a, int layer, int begin, int wa
             const float2 pf = __half22float2(*reinterpret_cast<const __half2 *>(&p));
             const float2 cf = __half22float2(*reinterpret_cast<const __half2 *>(&c[i]));
             const float2 sf = __half22float2(*reinterpret_cast<const __half2 *>(&s[i]));
-            const float2 y = make_float2(xf.x * cf.x + sign * pf.x * sf.x, xf.y * cf.y + sign * pf.y * sf.y);
-            const __half2 h = __floats2half2_rn(y.x, y.y);
+            y[i] = make_float2(xf.x * cf.x + sign * pf.x * sf.x, xf.y * cf.y + sign * pf.y * sf.y);
+        }
+        if (!here[j]) continue;
+        const int64_t to = layer * a.q_out_layer_stride + (begin + j) * a.q_out_token_stride + at;
+        if (a.query_out32 != nullptr) {
+            float4 *dst = reinterpret_cast<float4 *>(a.query_out32 + to);
+            dst[0] = make_float4(y[0].x, y[0].y, y[1].x, y[1].y);
+            dst[1] = make_float4(y[2].x, y[2].y, y[3].x, y[3].y);
+            continue;
+        }
+        uint32_t r[4], low[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const __half2 h = __floats2half2_rn(y[i].x, y[i].y);
             const float2 f = __half22float2(h);
             r[i] = pkv::pack_half2(h);
-            low[i] = pkv::pack_half2(__floats2half2_rn(y.x - f.x, y.y - f.y));
+            low[i] = pkv::pack_half2(__floats2half2_rn(y[i].x - f.x, y[i].y - f.y));
         }
-        if (here[j]) {
-            const int64_t to = layer * a.q_out_layer_stride + (begin + j) * a.q_out_token_stride + at;
-            *reinterpret_cast<uint4 *>(a.query_out + to) = make_uint4(r[0], r[1], r[2], r[3]);
-            if (a.query_low != nullptr) {
-                *reinterpret_cast<uint4 *>(a.query_low + to) = make_uint4(low[0], low[1], low[2], low[3]);
-            }
+        *reinterpret_cast<uint4 *>(a.query_out + to) = make_uint4(r[0], r[1], r[2], r[3]);
+        if (a.query_low != nullptr) {
+            *reinterpret_cast<uint4 *>(a.query_low + to) = make_uint4(low[0], low[1], low[2], low[3]);
         }
     }
 }
@@ -379,9 +389,23 @@ __global__ void __launch_bounds__(kReadThreads)
     }
 }
 
+pkv::fp8::Cache cache_of(const void *key_codes, const void *value_codes, const void *key_scales,
+                         const void *value_scales, int32_t layers, int32_t num_blocks) {
+    return {static_cast<uint8_t *>(const_cast<void *>(key_codes)), static_cast<uint8_t *>(const_cast<void *>(value_codes)),
+            static_cast<float *>(const_cast<void *>(key_scales)), static_cast<float *>(const_cast<void *>(value_scales)),
+            layers, num_blocks};
+}
+
 bool aligned16(const void *p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
 
 }  // namespace
+
+namespace pkv {
+int launch_prefill_attention_tc(const void *pool, int32_t num_blocks, int32_t layer, const void *query,
+                                bool query_fp32, int64_t query_stride, const int32_t *blocks, int32_t start,
+                                int32_t tokens, void *out, int64_t out_stride, int32_t *error_flag,
+                                cudaStream_t stream);
+}
 
 namespace pkv::fp8 {
 
@@ -442,8 +466,8 @@ extern "C" int pkv_fp8_append_kv(void *key_codes, void *value_codes, void *key_s
                                  const void *key, const void *value, int64_t src_layer_stride, int64_t src_token_stride,
                                  const int32_t *slots, const int32_t *positions, int32_t tokens, const void *rope_table,
                                  const void *query_in, int64_t q_layer_stride, int64_t q_token_stride, void *query_out,
-                                 int64_t q_out_layer_stride, int64_t q_out_token_stride, int32_t *error_flag,
-                                 void *stream) {
+                                 int32_t query_out_fp32, int64_t q_out_layer_stride, int64_t q_out_token_stride,
+                                 int32_t *error_flag, void *stream) {
     pkv::clear_error();
     int rc = pkv::fp8::check_cache(key_codes, value_codes, key_scales, value_scales, layers, num_blocks, layer_begin,
                                    layer_count);
@@ -463,7 +487,7 @@ extern "C" int pkv_fp8_append_kv(void *key_codes, void *value_codes, void *key_s
     }
     if (layer_count > 65535) return pkv::fail(PKV_VALUE_ERROR, "fp8 append: layers out of range");
     if (tokens == 0) return PKV_OK;
-    AppendArgs a;
+    AppendArgs a = {};
     a.cache = {static_cast<uint8_t *>(key_codes), static_cast<uint8_t *>(value_codes), static_cast<float *>(key_scales),
                static_cast<float *>(value_scales), layers, num_blocks};
     a.layer_begin = layer_begin;
@@ -476,7 +500,8 @@ extern "C" int pkv_fp8_append_kv(void *key_codes, void *value_codes, void *key_s
     a.tokens = tokens;
     a.rope = static_cast<const __half *>(rope_table);
     a.query_in = static_cast<const __half *>(query_in);
-    a.query_out = static_cast<__half *>(query_out);
+    a.query_out = query_out_fp32 ? nullptr : static_cast<__half *>(query_out);
+    a.query_out32 = query_out_fp32 ? static_cast<float *>(query_out) : nullptr;
     a.query_low = nullptr;
     a.q_layer_stride = q_layer_stride;
     a.q_token_stride = q_token_stride;
@@ -507,13 +532,10 @@ int read_blocks(const void *key_codes, const void *value_codes, const void *key_
         return pkv::fail(PKV_VALUE_ERROR, "fp8 read: the outputs must be 16-byte aligned");
     }
     if (count == 0) return PKV_OK;
-    const pkv::fp8::Cache cache{static_cast<uint8_t *>(const_cast<void *>(key_codes)),
-                                static_cast<uint8_t *>(const_cast<void *>(value_codes)),
-                                static_cast<float *>(const_cast<void *>(key_scales)),
-                                static_cast<float *>(const_cast<void *>(value_scales)), layers, num_blocks};
-    const cudaError_t e =
-        pkv::launch_pdl(fp8_read_kernel, dim3(count), dim3(kReadThreads), static_cast<cudaStream_t>(stream), cache,
-                        layer, blocks, static_cast<__half *>(key_out), static_cast<__half *>(value_out), index_out, error_flag);
+    const cudaError_t e = pkv::launch_pdl(
+        fp8_read_kernel, dim3(count), dim3(kReadThreads), static_cast<cudaStream_t>(stream),
+        cache_of(key_codes, value_codes, key_scales, value_scales, layers, num_blocks), layer, blocks,
+        static_cast<__half *>(key_out), static_cast<__half *>(value_out), index_out, error_flag);
     if (e != cudaSuccess) return pkv::fail(PKV_CUDA_ERROR, std::string("fp8 read launch failed: ") + cudaGetErrorString(e));
     return PKV_OK;
 }
@@ -529,18 +551,29 @@ extern "C" int pkv_fp8_read_blocks(const void *key_codes, const void *value_code
                        key_out, value_out, nullptr, error_flag, stream);
 }
 
-// The request's blocks become an FP16 pool of one layer in the workspace (the
-// values are FP16 numbers: nothing is rounded), which the tensor-core prompt
-// kernel attends to.  That kernel reads every block once for each 16 queries,
-// so the conversion is a small part: 3 MiB of traffic at 2048 tokens.
+// The request's blocks become an FP16 pool of one layer in the workspace (the values are
+// FP16 numbers: nothing is rounded), which the tensor-core prompt kernel attends to.  That
+// kernel reads every block once for each 16 queries, so the conversion is a small part: 2 us
+// at 2047 tokens.  (The prompt kernel's producers reading codes and converting them, every
+// block as often as there are 16 queries behind it: 74 to 85 us against 53 for the prompt of
+// 2047 tokens, and no better at one of 75 behind 601.)
 extern "C" int pkv_fp8_prefill_attention(const void *key_codes, const void *value_codes, const void *key_scales,
                                          const void *value_scales, int32_t layers, int32_t num_blocks, int32_t layer,
-                                         const void *query, int64_t query_stride, const int32_t *blocks, int32_t start,
-                                         int32_t tokens, void *out, int64_t out_stride, void *workspace,
-                                         int64_t workspace_bytes, int32_t *error_flag, void *stream) {
+                                         const void *query, int32_t query_fp32, int64_t query_stride,
+                                         const int32_t *blocks, int32_t start, int32_t tokens, void *out,
+                                         int64_t out_stride, void *workspace, int64_t workspace_bytes,
+                                         int32_t *error_flag, void *stream) {
     pkv::clear_error();
+    if (query == nullptr || blocks == nullptr || out == nullptr || error_flag == nullptr) {
+        return pkv::fail(PKV_VALUE_ERROR, "prefill attention: null pointer argument");
+    }
     if (tokens < 1 || start < 0 || static_cast<int64_t>(start) + tokens > PKV_CONTEXT_LIMIT) {
         return pkv::fail(PKV_VALUE_ERROR, "prefill attention: the chunk must hold 1 or more tokens at positions below 2048");
+    }
+    constexpr int64_t kRow = PKV_QUERY_HEADS * PKV_HEAD_DIM;
+    if (!aligned16(query) || !aligned16(out) || query_stride % 8 || out_stride % 8 || query_stride < kRow ||
+        out_stride < kRow) {
+        return pkv::fail(PKV_VALUE_ERROR, "prefill attention: rows must be 16-byte aligned, 2048 or more values apart in multiples of 8");
     }
     const int count = (start + tokens + kSlots - 1) / kSlots;
     const int64_t pool_bytes = static_cast<int64_t>(count) * 2 * kBlockValues * 2;
@@ -552,6 +585,6 @@ extern "C" int pkv_fp8_prefill_attention(const void *key_codes, const void *valu
                                workspace, static_cast<__half *>(workspace) + count * kBlockValues, table, error_flag,
                                stream);
     if (rc) return rc;
-    return pkv_prefill_attention(workspace, count, 0, query, query_stride, table, start, tokens, out, out_stride,
-                                 error_flag, stream);
+    return pkv::launch_prefill_attention_tc(workspace, count, 0, query, query_fp32 != 0, query_stride, table, start, tokens,
+                                            out, out_stride, error_flag, static_cast<cudaStream_t>(stream));
 }

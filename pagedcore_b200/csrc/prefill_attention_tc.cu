@@ -53,6 +53,13 @@
 // TMEM: S/P buffers at columns 0, 64, 128, O at 192 (256 columns, two CTAs
 // per SM).  Shared memory: Q (16 KiB) and the K and V rings.
 //
+// An FP32 query (SPLIT_Q; the 8-bit cache's rotated query) becomes two Q tiles, its FP16
+// value and what that leaves, and S takes both: four more MMAs a step, mostly hidden behind
+// the softmax (2047 tokens with their read: 43.4 us, with an FP16 query 41.0).  P stays one
+// FP16 number, a rounding of the output's own size: relative error 2.6e-4 to 2.9e-4 against
+// 2.0e-4 with nothing but the output rounded, 3.5e-4 to 4.2e-4 with the query rounded too.
+// (P as two FP16 numbers in a buffer's two halves and as many MMAs again: 52 us.)
+//
 // Block ids outside the pool set PKV_DEVICE_BAD_BLOCK and read as zeros.
 // Every wait is bounded: on a timeout the thread sets
 // PKV_DEVICE_WAIT_TIMEOUT, the CTA stops issuing work, waits (bounded) for
@@ -95,7 +102,9 @@ constexpr int kKCopyLag = 2;
 constexpr int kVCopyLag = 1;
 constexpr int kQBytes = kRows * kRowBytes;             // 16 KiB
 constexpr int kRingBytes = kStepBlocks * kBoxBytes;    // 8 KiB: one step's K (or V)
-constexpr int kSmemBytes = kQBytes + (kKStages + kVStages) * kRingBytes + 1024;  // + alignment slack
+// SPLIT_Q: a second Q tile, the low halves.  + alignment slack.
+template <bool SPLIT_Q>
+constexpr int kSmemBytes = (SPLIT_Q ? 2 : 1) * kQBytes + (kKStages + kVStages) * kRingBytes + 1024;
 constexpr int kSoftmaxWarps = 4;           // thread r of warps 0-3 owns row r (TMEM lane r)
 constexpr int kSoftmaxThreads = kSoftmaxWarps * 32;
 constexpr int kThreads = kSoftmaxThreads + 128;
@@ -138,6 +147,7 @@ struct TcArgs {
     int32_t start;
     int32_t tokens;
     int32_t *error_flag;
+    const float *query32;  // SPLIT_Q, in place of query
 };
 
 // Barriers of one CTA (8-byte mbarriers in static shared memory).
@@ -217,8 +227,43 @@ __device__ __forceinline__ void load_q_row(uint32_t q_smem, const TcArgs &a, con
     pkv::cp_async_commit();
 }
 
+// The same from an FP32 query: two FP16 numbers that add up to each value, the high
+// halves at q_smem and the low ones a tile further.
+__device__ __forceinline__ void load_q_row_split(uint32_t q_smem, const TcArgs &a, const Item &it, int r) {
+    const int t = min(it.t0 + (r >> 3), a.tokens - 1);
+    const float4 *src = reinterpret_cast<const float4 *>(a.query32 + static_cast<int64_t>(t) * a.query_stride +
+                                                         (it.kv * 8 + (r & 7)) * kHeadDim);
+    const uint32_t row = q_smem + (r >> 3) * 1024 + (r & 7) * kRowBytes;
+#pragma unroll
+    for (int c = 0; c < 8; ++c) {
+        const float4 x = src[2 * c], y = src[2 * c + 1];
+        const float v[8] = {x.x, x.y, x.z, x.w, y.x, y.y, y.z, y.w};
+        uint32_t high[4], low[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const __half2 h = __floats2half2_rn(v[2 * i], v[2 * i + 1]);
+            const float2 f = __half22float2(h);
+            high[i] = pkv::pack_half2(h);
+            low[i] = pack2(v[2 * i] - f.x, v[2 * i + 1] - f.y);
+        }
+        const uint32_t at = row + ((c ^ (r & 7)) << 4);
+        asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(at), "r"(high[0]), "r"(high[1]), "r"(high[2]), "r"(high[3]) : "memory");
+        asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(at + kQBytes), "r"(low[0]), "r"(low[1]), "r"(low[2]), "r"(low[3]) : "memory");
+    }
+}
+
+template <bool SPLIT_Q>
+__device__ __forceinline__ void load_q(uint32_t q_smem, const TcArgs &a, const Item &it, int r) {
+    if constexpr (SPLIT_Q) {
+        load_q_row_split(q_smem, a, it, r);
+    } else {
+        load_q_row(q_smem, a, it, r);
+    }
+}
+
 // At most 120 registers a thread: two CTAs of 256 threads then fit an SM
 // (the occupancy calculation gives one CTA at 125).
+template <bool SPLIT_Q>
 __global__ void __maxnreg__(120)
     prefill_tc_kernel(const TcArgs a) {
     extern __shared__ uint8_t dyn_smem[];
@@ -230,7 +275,7 @@ __global__ void __maxnreg__(120)
     const uint32_t raw = pkv::smem_addr(dyn_smem);
     const uint32_t base = (raw + 1023u) & ~1023u;  // 1024-aligned: swizzle atoms
     const uint32_t q_smem = base;
-    const uint32_t k_smem = base + kQBytes;                   // K ring, 8 KiB a stage
+    const uint32_t k_smem = base + (SPLIT_Q ? 2 : 1) * kQBytes;   // K ring, 8 KiB a stage
     const uint32_t v_smem = k_smem + kKStages * kRingBytes;   // V ring, 8 KiB a stage
 
     const int tiles = (a.tokens + kTileTokens - 1) / kTileTokens;
@@ -377,6 +422,13 @@ __global__ void __maxnreg__(120)
                         pkv::tc::mma_f16_ss(tmem + (g % kSBuffers) * kStepKeys, q_desc + 2 * k, k_desc + 2 * k, kIdescS,
                                             k > 0);
                     }
+                    if constexpr (SPLIT_Q) {  // the low halves, a tile (kQBytes / 16 on the descriptor) further
+#pragma unroll
+                        for (int k = 0; k < kHeadDim / 16; ++k) {
+                            pkv::tc::mma_f16_ss(tmem + (g % kSBuffers) * kStepKeys, q_desc + kQBytes / 16 + 2 * k,
+                                                k_desc + 2 * k, kIdescS, true);
+                        }
+                    }
                     pkv::tc::commit(bar_addr(bars.s_full[g % kSBuffers]));
                     pkv::tc::commit(bar_addr(bars.k_empty[st]));
                 }
@@ -437,7 +489,7 @@ __global__ void __maxnreg__(120)
         // The first item's Q tile; each later one is loaded during the last step
         // of the item before it, once every S MMA that read the tile has completed.
         if (item_of(0, cta, ctas) < items) {
-            load_q_row(q_smem, a, item_info(item_of(0, cta, ctas), tiles, a), r);
+            load_q<SPLIT_Q>(q_smem, a, item_info(item_of(0, cta, ctas), tiles, a), r);
             pkv::cp_async_wait<0>();
             pkv::fence_proxy_async_smem();  // generic-proxy copies -> the MMA's (async proxy) reads
             __syncwarp();
@@ -469,7 +521,7 @@ __global__ void __maxnreg__(120)
                 pkv::tc::tmem_wait_ld();
                 // s_full of the item's last step: every S MMA of the item has
                 // completed, so the next item's Q may replace this one's.
-                if (last && next < items) load_q_row(q_smem, a, item_info(next, tiles, a), r);
+                if (last && next < items) load_q<SPLIT_Q>(q_smem, a, item_info(next, tiles, a), r);
 
                 float s[64];
 #pragma unroll
@@ -516,7 +568,7 @@ __global__ void __maxnreg__(120)
                         const float lo = pkv::exp2_approx(x.x);
                         const float hi = pkv::exp2_approx(x.y);
                         l4[c & 3] = pkv::add_f32x2(l4[c & 3], pkv::f32x2(lo, hi));
-                        pr[c] = pkv::pack_half2(__floats2half2_rn(lo, hi));
+                        pr[c] = pack2(lo, hi);
                     }
                     pkv::tc::tmem_st16(sbuf + 16 * half, pr);
                 }
@@ -607,16 +659,18 @@ constexpr int kCtasPerSm = 2;
 
 // Per device, once: the kernel's dynamic shared-memory limit raised, and the
 // number of its CTAs that run at once (2 per SM) recorded in *ctas.
+template <bool SPLIT_Q>
 int prepare(int device, int *ctas) {
     static std::atomic<int> resident[kMaxDevices] = {};
     if (device >= 0 && device < kMaxDevices) {
         *ctas = resident[device].load(std::memory_order_acquire);
         if (*ctas > 0) return PKV_OK;
     }
-    cudaError_t e = cudaFuncSetAttribute(prefill_tc_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmemBytes);
+    cudaError_t e = cudaFuncSetAttribute(prefill_tc_kernel<SPLIT_Q>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                         kSmemBytes<SPLIT_Q>);
     if (e == cudaSuccess) {
         // All of the SM's unified L1/shared memory as shared memory: two CTAs' worth.
-        e = cudaFuncSetAttribute(prefill_tc_kernel, cudaFuncAttributePreferredSharedMemoryCarveout,
+        e = cudaFuncSetAttribute(prefill_tc_kernel<SPLIT_Q>, cudaFuncAttributePreferredSharedMemoryCarveout,
                                  cudaSharedmemCarveoutMaxShared);
     }
     if (e != cudaSuccess) {
@@ -629,7 +683,7 @@ int prepare(int device, int *ctas) {
         return pkv::fail(PKV_CUDA_ERROR, std::string("prefill attention: SM count query failed: ") +
                                              cudaGetErrorString(e));
     }
-    // Two CTAs fit an SM: 2 x (105 KiB + static) of shared memory, 2 x 256
+    // Two CTAs fit an SM: 2 x (at most 105 KiB + static) of shared memory, 2 x 256
     // columns of TMEM, 2 x 256 threads at 120 registers.
     const int per_sm = kCtasPerSm;
     *ctas = sms * per_sm;
@@ -637,23 +691,38 @@ int prepare(int device, int *ctas) {
     return PKV_OK;
 }
 
+template <bool SPLIT_Q>
+int launch(const TcArgs &args, cudaStream_t stream) {
+    int device = 0;
+    cudaError_t e = cudaGetDevice(&device);
+    if (e != cudaSuccess) return pkv::fail(PKV_CUDA_ERROR, std::string("cudaGetDevice: ") + cudaGetErrorString(e));
+    int resident = 0;
+    const int rc = prepare<SPLIT_Q>(device, &resident);
+    if (rc) return rc;
+    // One CTA per resident slot at most; each walks its share of the items.
+    const int items = (args.tokens + kTileTokens - 1) / kTileTokens * kKvHeads;
+    prefill_tc_kernel<SPLIT_Q><<<std::min(items, resident), kThreads, kSmemBytes<SPLIT_Q>, stream>>>(args);
+    e = cudaGetLastError();
+    if (e != cudaSuccess) {
+        return pkv::fail(PKV_CUDA_ERROR, std::string("prefill attention launch failed: ") + cudaGetErrorString(e));
+    }
+    return PKV_OK;
+}
+
 }  // namespace
 
 namespace pkv {
 
-// Launch of the tcgen05 prefill attention (arguments checked by the caller).
+// Launch of the tcgen05 prefill attention (arguments checked by the caller); the query FP16
+// or, with query_fp32, FP32.
 int launch_prefill_attention_tc(const void *pool, int32_t num_blocks, int32_t layer, const void *query,
-                                int64_t query_stride, const int32_t *blocks, int32_t start, int32_t tokens,
-                                void *out, int64_t out_stride, int32_t *error_flag, cudaStream_t stream) {
-    int device = 0;
-    cudaError_t e = cudaGetDevice(&device);
-    if (e != cudaSuccess) return fail(PKV_CUDA_ERROR, std::string("cudaGetDevice: ") + cudaGetErrorString(e));
-    int resident = 0;
-    int rc = prepare(device, &resident);
-    if (rc) return rc;
+                                bool query_fp32, int64_t query_stride, const int32_t *blocks, int32_t start,
+                                int32_t tokens, void *out, int64_t out_stride, int32_t *error_flag,
+                                cudaStream_t stream) {
     TcArgs args;
     args.pool = static_cast<const __half *>(pool);
-    args.query = static_cast<const __half *>(query);
+    args.query = query_fp32 ? nullptr : static_cast<const __half *>(query);
+    args.query32 = query_fp32 ? static_cast<const float *>(query) : nullptr;
     args.out = static_cast<__half *>(out);
     args.blocks = blocks;
     args.query_stride = query_stride;
@@ -663,14 +732,7 @@ int launch_prefill_attention_tc(const void *pool, int32_t num_blocks, int32_t la
     args.start = start;
     args.tokens = tokens;
     args.error_flag = error_flag;
-    // One CTA per resident slot at most; each walks its share of the items.
-    const int items = (tokens + kTileTokens - 1) / kTileTokens * kKvHeads;
-    prefill_tc_kernel<<<std::min(items, resident), kThreads, kSmemBytes, stream>>>(args);
-    e = cudaGetLastError();
-    if (e != cudaSuccess) {
-        return fail(PKV_CUDA_ERROR, std::string("prefill attention launch failed: ") + cudaGetErrorString(e));
-    }
-    return PKV_OK;
+    return query_fp32 ? launch<true>(args, stream) : launch<false>(args, stream);
 }
 
 }  // namespace pkv

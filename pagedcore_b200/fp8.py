@@ -364,8 +364,9 @@ def append_kv(
     """Write FP16 K/V [layers, tokens, 4, 64] into the cache at ``slots`` (int32 [tokens]).
 
     With ``rope_table`` K is rotated at ``positions`` first, and ``query``
-    [layers, tokens, 32, 64] is returned rotated (in ``query_out`` when given,
-    which may be ``query`` itself).  The tokens of one block must be
+    [layers, tokens, 32, 64] is returned rotated: in FP32, unrounded, for
+    ``prefill_attention``, or in FP16 in ``query_out`` when that is given
+    (which may be ``query`` itself).  The tokens of one block must be
     consecutive, in the list and in the block, as a request's positions are.
     """
     index = cache.key_codes.get_device()
@@ -390,7 +391,7 @@ def append_kv(
             raise ValueError("query must be FP16 [layers, tokens, 32, 64]")
         _half("query", query, index)
         if query_out is None:
-            query_out = torch.empty_like(query, memory_format=torch.contiguous_format)
+            query_out = torch.empty_like(query, dtype=_FLOAT, memory_format=torch.contiguous_format)
         elif query_out.shape != query.shape or not _rows_ok(query_out, query_out.stride()):
             raise ValueError("query_out must be FP16 [layers, tokens, 32, 64] with contiguous, 16-byte aligned rows")
         else:
@@ -404,7 +405,8 @@ def append_kv(
     key, value, strides = _aligned_pair(key, value)
     layer_stride, token_stride = strides[0], strides[1]
     _call(index, lib.pkv_fp8_append_kv, *cache._args(), layer_begin, layers, key.data_ptr(), value.data_ptr(),
-          layer_stride, token_stride, slots_ptr, positions_ptr, tokens, rope, q_ptr, *q_strides, out_ptr, *out_strides,
+          layer_stride, token_stride, slots_ptr, positions_ptr, tokens, rope, q_ptr, *q_strides, out_ptr,
+          query_out is not None and query_out.dtype is _FLOAT, *out_strides,
           flag)
     return query_out
 
@@ -441,19 +443,22 @@ def _attention_rows(name: str, tensor: Tensor, shape: tuple[int, ...], index: in
         raise ValueError(f"{name} must be FP16 {list(shape)} on cuda:{index}")
 
 
-def _query_and_out(query: Tensor, out: Tensor | None, index: int, rows: str) -> tuple[Tensor, int, Tensor, int]:
+def _query_and_out(
+    query: Tensor, out: Tensor | None, index: int, rows: str, fp32: bool = False
+) -> tuple[Tensor, int, Tensor, int]:
     """Query and output [rows, 32, 64] as the kernels take them, with their row strides."""
     shape = query.shape
     if len(shape) != 3 or shape[0] < 1 or shape[1] != _QUERY_HEADS or shape[2] != _HEAD_DIM:
         raise ValueError(f"query must be FP16 [{rows}, 32, 64] of a nonempty {rows}")
-    _half("query", query, index)
+    if not (fp32 and query.dtype is _FLOAT and query.get_device() == index):
+        _half("query", query, index)
     strides = query.stride()
     if not _rows_ok(query, strides) or strides[0] < _ROW:
         query = query.contiguous()
         strides = query.stride()
     stride = max(strides[0], _ROW)  # of one row it may be anything
     if out is None:
-        return query, stride, torch.empty_like(query, memory_format=torch.contiguous_format), _ROW
+        return query, stride, torch.empty_like(query, dtype=_HALF, memory_format=torch.contiguous_format), _ROW
     _attention_rows("out", out, shape, index)
     strides = out.stride()
     if not _rows_ok(out, strides):
@@ -540,20 +545,20 @@ def prefill_attention(
     error_flag: Tensor,
     out: Tensor | None = None,
 ) -> Tensor:
-    """``kernels.prefill_attention`` over the 8-bit cache: rotated FP16 query [T, 32, 64].
+    """``kernels.prefill_attention`` over the 8-bit cache: rotated query [T, 32, 64], FP16 or FP32.
 
     Token t attends to positions 0 .. start + t through ``blocks`` (int32, the
     request's physical block per 16 positions).
     """
     index = cache.key_codes.get_device()
-    query, query_stride, out, out_stride = _query_and_out(query, out, index, "tokens")
+    query, query_stride, out, out_stride = _query_and_out(query, out, index, "tokens", fp32=True)
     tokens = query.shape[0]
     if type(start) is not int or start < 0 or start + tokens > 2048:
         raise ValueError("the chunk must hold 1 or more tokens at positions below 2048")
     count = -(-(start + tokens) // _BLOCK_TOKENS)
     blocks_ptr = _int_list(index, "blocks", blocks, count)
-    workspace = query.new_empty(count * _PREFILL_BLOCK_BYTES // 2)
-    _call(index, lib.pkv_fp8_prefill_attention, *cache._args(), layer, query.data_ptr(), query_stride, blocks_ptr,
-          start, tokens, out.data_ptr(), out_stride, workspace.data_ptr(), count * _PREFILL_BLOCK_BYTES,
-          _int_list(index, "error_flag", error_flag, 1))
+    workspace = out.new_empty(count * _PREFILL_BLOCK_BYTES // 2)
+    _call(index, lib.pkv_fp8_prefill_attention, *cache._args(), layer, query.data_ptr(), query.dtype is _FLOAT,
+          query_stride, blocks_ptr, start, tokens, out.data_ptr(), out_stride, workspace.data_ptr(),
+          count * _PREFILL_BLOCK_BYTES, _int_list(index, "error_flag", error_flag, 1))
     return out

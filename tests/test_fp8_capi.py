@@ -53,7 +53,7 @@ def test_linear() -> None:
 
 def test_cache() -> None:
     def append(cache=CACHE, begin=0, count=1, stride=256, rope=None, positions=None, query=None, query_out=None):
-        return (*cache, begin, count, P, P, 0, stride, P, positions, 1, rope, query, 0, 0, query_out, 0, 0, P, None)
+        return (*cache, begin, count, P, P, 0, stride, P, positions, 1, rope, query, 0, 0, query_out, 0, 0, 0, P, None)
 
     refused(lib.pkv_fp8_append_kv, *append(cache=(P, None, P, P, 2, 8)), message=b"codes and scales")
     refused(lib.pkv_fp8_append_kv, *append(cache=(P + 8, P, P, P, 2, 8)), message=b"16-byte")
@@ -82,10 +82,14 @@ def test_attention() -> None:
     refused(lib.pkv_fp8_decode_attention, *decode(layer=2), message=b"layers out of range")
     refused(lib.pkv_fp8_decode_layer, *CACHE, 0, P, 2048, None, P, 256, P, P, P, P, 1, 4, 1, P, 2048, P, 1 << 20, P, None,
             message=b"key, value and rope_table")
-    refused(lib.pkv_fp8_prefill_attention, *CACHE, 0, P, 2048, P, 2040, 9, P, 2048, P, 1 << 24, P, None,
-            message=b"positions below 2048")
-    refused(lib.pkv_fp8_prefill_attention, *CACHE, 0, P, 2048, P, 0, 17, P, 2048, P, 2 * 16388 - 1, P, None,
-            message=b"workspace")
+    def prefill(layer=0, fp32=0, stride=2048, blocks=P, start=0, tokens=17, bytes=1 << 24):
+        return (*CACHE, layer, P, fp32, stride, blocks, start, tokens, P, 2048, P, bytes, P, None)
+
+    refused(lib.pkv_fp8_prefill_attention, *prefill(start=2040, tokens=9), message=b"positions below 2048")
+    refused(lib.pkv_fp8_prefill_attention, *prefill(bytes=2 * 16388 - 1), message=b"workspace")
+    refused(lib.pkv_fp8_prefill_attention, *prefill(fp32=1, stride=2044), message=b"2048 or more")
+    refused(lib.pkv_fp8_prefill_attention, *prefill(blocks=None), message=b"null pointer")
+    refused(lib.pkv_fp8_prefill_attention, *prefill(layer=2), message=b"layers out of range")
     out, size = ctypes.c_int32(), ctypes.c_int64()
     refused(lib.pkv_fp8_decode_plan, 0, 0, 4, ctypes.byref(out), ctypes.byref(size), message=b"nonempty batch")
 

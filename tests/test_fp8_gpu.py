@@ -543,17 +543,51 @@ def test_decode_layer_flags_a_row_without_a_token() -> None:
     assert torch.equal(case.cache.key_codes.view(torch.uint8)[LAYER, case.tables[0][0]], before)
 
 
-@pytest.mark.parametrize("start, tokens", [(0, 1), (0, 15), (0, 130), (7, 40), (100, 64), (2000, 48)])
-def test_prefill_attention(start, tokens) -> None:
+@pytest.mark.parametrize("start, tokens", [(0, 1), (0, 15), (0, 130), (7, 40), (100, 64), (601, 75), (2000, 48)])
+@pytest.mark.parametrize("dtype", [torch.float16, torch.float32])
+def test_prefill_attention(start, tokens, dtype) -> None:
     case = CacheCase(31, [start + tokens])
-    query = randn(32, tokens, 32, 64).half()
+    query = randn(32, tokens, 32, 64).to(dtype)
     blocks = case.batch()[2]
-    out = fp8.prefill_attention(case.cache, LAYER, query, blocks, start, case.flag)
+    wide = torch.full((tokens + 1, 40, 64), 3.0, dtype=torch.float16, device=case.device)
+    out = fp8.prefill_attention(case.cache, LAYER, query, blocks, start, case.flag, wide[:tokens, 4:36])
     assert int(case.flag.item()) == 0
     for t in {0, 1, tokens // 2, tokens - 1} & set(range(tokens)):
         exact, bound = attend64(query[t], case.key.tokens(case.tables[0], start + t + 1),
                                 case.value.tokens(case.tables[0], start + t + 1), HALF_FP16)
         assert bool(((out[t].double() - exact).abs() <= bound).all()), t
+    assert bool((wide[tokens] == 3).all()) and bool((wide[:, :4] == 3).all()) and bool((wide[:, 36:] == 3).all())
+    assert torch.equal(fp8.prefill_attention(case.cache, LAYER, query, blocks, start, case.flag), out)
+
+
+def test_prefill_attention_with_blocks_of_very_different_scale_and_a_bad_block() -> None:
+    case = CacheCase(33, [300], spread=4.0)
+    query = 2 * randn(34, 300, 32, 64).half()
+    blocks = case.batch()[2].clone()
+    out = fp8.prefill_attention(case.cache, LAYER, query, blocks, 0, case.flag)
+    for t in (0, 17, 200, 299):
+        exact, bound = attend64(query[t], case.key.tokens(case.tables[0], t + 1),
+                                case.value.tokens(case.tables[0], t + 1), HALF_FP16)
+        # FP16 weights end at 2^-24, the largest is 2^7 or more: half a step is 2^-32 of the largest V a token.
+        bound = bound + 300 * 2.0**-32 * case.value.tokens(case.tables[0], t + 1).abs().amax()
+        assert bool(((out[t].double() - exact).abs() <= bound).all()), t
+    blocks[3] = -1
+    fp8.prefill_attention(case.cache, LAYER, query, blocks, 0, case.flag)
+    assert int(case.flag.item()) == 1
+
+
+def test_append_returns_the_query_in_fp32_for_the_prompt() -> None:
+    case = CacheCase(35, [0], spare=4)
+    case.tables[0] += [case.free.pop() for _ in range(3)]
+    key, value, query = randn(1, 1, 40, 4, 64).half(), randn(2, 1, 40, 4, 64).half(), randn(3, 1, 40, 32, 64).half()
+    positions = torch.arange(40, device=case.device)
+    slots = torch.tensor(case.slots(0, 0, 40), dtype=torch.int32, device=case.device)
+    rotated = fp8.append_kv(case.cache, key, value, slots, layer_begin=LAYER, error_flag=case.flag,
+                            positions=positions.int(), rope_table=case.rope, query=query)
+    exact = rope64(query[0], case.rope, positions)
+    size = query[0].double().abs() + query[0].double().abs().roll(32, -1)
+    assert rotated.dtype is torch.float32
+    assert bool(((rotated[0].double() - exact).abs() <= 3 * F32 * size).all())
 
 
 def test_cache_refusals() -> None:
