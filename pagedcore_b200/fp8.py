@@ -69,6 +69,16 @@ def _call(index: int, function, *args) -> None:
         check(status)
 
 
+def _row_stride(name: str, tensor: Tensor, width: int) -> int:
+    """Row stride of a matrix whose rows must not overlap (one row's may be anything)."""
+    stride = tensor.stride(0)
+    if stride >= width:
+        return stride
+    if tensor.shape[0] > 1:
+        raise ValueError(f"the rows of {name} overlap")
+    return width
+
+
 @dataclass(slots=True)
 class Fp8Rows:
     """E4M3 codes [rows, width] and FP32 scales [rows, ceil(width / 128)]."""
@@ -92,7 +102,7 @@ class Fp8Rows:
         else:
             if out.shape != (rows, width) or out.dtype is not _HALF or out.stride(1) != 1 or out.get_device() != index:
                 raise ValueError(f"out must be FP16 [{rows}, {width}] with contiguous rows")
-            stride = max(out.stride(0), width)
+            stride = _row_stride("out", out, width)
         if rows:
             _call(index, lib.pkv_fp8_to_half, self.codes.data_ptr(), self.scales.data_ptr(), rows, width,
                   out.data_ptr(), stride)
@@ -175,7 +185,7 @@ def _quantize(x: Tensor, width: int, silu_pairs: bool) -> Fp8Rows:
     rows, columns = x.shape
     out = _empty_rows(x, rows, width)
     if rows:
-        _call(index, lib.pkv_fp8_quantize, x.data_ptr(), max(x.stride(0), columns), silu_pairs, rows, width,
+        _call(index, lib.pkv_fp8_quantize, x.data_ptr(), _row_stride("x", x, columns), silu_pairs, rows, width,
               out.codes.data_ptr(), out.scales.data_ptr())
     return out
 
@@ -228,15 +238,16 @@ def linear(x: Fp8Rows, weight: Fp8Weight, out: Tensor | None = None) -> Tensor:
     if scales.shape != (_groups(n), _groups(k)) or scales.dtype is not _FLOAT or not scales.is_contiguous():
         raise ValueError("weight needs contiguous FP32 scales [ceil(n / 128), ceil(k / 128)]")
     index = _device(x.codes, x.scales, codes, scales)
+    x_stride = _row_stride("x", x.codes, k)
     if out is None:
         out = codes.new_empty((rows, n), dtype=_HALF)
         stride = n
     else:
         if out.shape != (rows, n) or out.dtype is not _HALF or out.stride(1) != 1 or out.get_device() != index:
             raise ValueError(f"out must be FP16 [{rows}, {n}] with contiguous rows")
-        stride = max(out.stride(0), n)
+        stride = _row_stride("out", out, n)
     if rows:
-        _call(index, lib.pkv_fp8_linear, x.codes.data_ptr(), max(x.codes.stride(0), k), x.scales.data_ptr(),
+        _call(index, lib.pkv_fp8_linear, x.codes.data_ptr(), x_stride, x.scales.data_ptr(),
               codes.data_ptr(), scales.data_ptr(), rows, n, k, out.data_ptr(), stride,
               linear_error_flag(codes.device).data_ptr())
     return out
@@ -392,7 +403,12 @@ def append_kv(
         _half("query", query, index)
         if query_out is None:
             query_out = torch.empty_like(query, dtype=_FLOAT, memory_format=torch.contiguous_format)
-        elif query_out.shape != query.shape or not _rows_ok(query_out, query_out.stride()):
+        elif (
+            query_out.shape != query.shape
+            or not _rows_ok(query_out, query_out.stride())
+            or (tokens > 1 and query_out.stride(1) < _ROW)
+            or (layers > 1 and query_out.stride(0) < _ROW)
+        ):
             raise ValueError("query_out must be FP16 [layers, tokens, 32, 64] with contiguous, 16-byte aligned rows")
         else:
             _half("query_out", query_out, index)
@@ -463,7 +479,7 @@ def _query_and_out(
     strides = out.stride()
     if not _rows_ok(out, strides):
         raise ValueError(f"out must be FP16 [{rows}, 32, 64] with contiguous, 16-byte aligned rows")
-    return query, stride, out, max(strides[0], _ROW)
+    return query, stride, out, _row_stride("out", out, _ROW)
 
 
 def _decode(cache, layer, query, new, lengths, prefix, flat, total_blocks, error_flag, out) -> Tensor:
@@ -548,7 +564,8 @@ def prefill_attention(
     """``kernels.prefill_attention`` over the 8-bit cache: rotated query [T, 32, 64], FP16 or FP32.
 
     Token t attends to positions 0 .. start + t through ``blocks`` (int32, the
-    request's physical block per 16 positions).
+    request's physical block per 16 positions).  A V value that is NaN may also
+    reach tokens up to 63 positions before it (their weight for it is 0).
     """
     index = cache.key_codes.get_device()
     query, query_stride, out, out_stride = _query_and_out(query, out, index, "tokens", fp32=True)

@@ -107,6 +107,16 @@ def test_tensors_on_the_cpu_are_refused() -> None:
         fp8.linear(fp8.Fp8Rows(torch.zeros(2, 64).to(torch.float8_e4m3fn), torch.ones(2, 1)), weight)
 
 
+def test_rows_that_overlap_are_refused() -> None:
+    row = torch.zeros(1, 64)
+    assert fp8._row_stride("x", row, 64) == 64
+    assert fp8._row_stride("x", row[:, :32], 32) in (32, 64)
+    assert fp8._row_stride("x", torch.zeros(3, 80)[:, :64], 64) == 80
+    for overlapping in (row.expand(3, 64), torch.zeros(128).as_strided((3, 64), (32, 1))):
+        with pytest.raises(ValueError, match="overlap"):
+            fp8._row_stride("x", overlapping, 64)
+
+
 @pytest.mark.parametrize("n, k", [(1, 16), (130, 128), (300, 400)])
 def test_quantize_weight_is_one_rounding_with_the_block_scale(n, k) -> None:
     generator = torch.Generator().manual_seed(n)

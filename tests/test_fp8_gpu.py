@@ -590,6 +590,65 @@ def test_append_returns_the_query_in_fp32_for_the_prompt() -> None:
     assert bool(((rotated[0].double() - exact).abs() <= 3 * F32 * size).all())
 
 
+def test_rows_that_overlap_are_refused_or_copied() -> None:
+    x = randn(1, 1, 256).half()
+    rows, weight = fp8.quantize_rows(x.repeat(3, 1)), fp8.quantize_weight(randn(2, 64, 256))
+    with pytest.raises(ValueError, match="overlap"):
+        fp8.quantize_rows(x.expand(3, 256))
+    with pytest.raises(ValueError, match="overlap"):
+        fp8.linear(fp8.Fp8Rows(rows.codes[:1].expand(3, 256), rows.scales), weight)
+    with pytest.raises(ValueError, match="overlap"):
+        fp8.linear(rows, weight, torch.zeros(1, 64, dtype=torch.float16, device="cuda").expand(3, 64))
+    with pytest.raises(ValueError, match="overlap"):
+        rows.to_half(torch.zeros(1, 256, dtype=torch.float16, device="cuda").expand(3, 256))
+    case = CacheCase(36, [40])
+    query, blocks = randn(3, 1, 32, 64).half(), case.batch()[2]
+    attend = lambda q, out=None: fp8.prefill_attention(case.cache, LAYER, q, blocks, 30, case.flag, out)  # noqa: E731
+    assert torch.equal(attend(query.expand(3, 32, 64)), attend(query.repeat(3, 1, 1)))
+    with pytest.raises(ValueError, match="overlap"):
+        attend(query.repeat(3, 1, 1), torch.zeros(1, 32, 64, dtype=torch.float16, device="cuda").expand(3, 32, 64))
+
+
+def test_a_cache_past_32_bits_of_offset() -> None:
+    case = CacheCase(37, [0])
+    blocks = 2**20 + 32  # 4096 bytes of K codes a block: the last ones begin past 2^32
+    cache = fp8.Fp8Cache.empty(1, blocks, "cuda")
+    small = fp8.Fp8Cache.empty(1, 4, "cuda")
+    key, value, query = randn(1, 1, 40, 4, 64).half(), randn(2, 1, 40, 4, 64).half(), randn(3, 1, 40, 32, 64).half()
+    positions, results = torch.arange(40, dtype=torch.int32, device="cuda"), []
+    for pool, table in ((cache, [blocks - 1, blocks - 3, 2**19 + 1]), (small, [0, 1, 2])):
+        flat = torch.tensor(table, dtype=torch.int32, device="cuda")
+        slots = (flat[positions.long() // 16] * 16 + positions % 16).int()
+        rotated = fp8.append_kv(pool, key[:, :39], value[:, :39], slots[:39], layer_begin=0, error_flag=case.flag,
+                                positions=positions[:39], rope_table=case.rope, query=query[:, :39])
+        prompt = fp8.prefill_attention(pool, 0, rotated[0], flat, 0, case.flag)
+        lengths, prefix = (torch.tensor(x, dtype=torch.int32, device="cuda") for x in ([40], [0, 3]))
+        new = fp8.decode_layer(pool, 0, query[0, 39:], key[0, 39:], value[0, 39:], case.rope, lengths, prefix, flat, 3,
+                               case.flag)
+        read = [x.reshape(-1, 4, 64)[:40] for x in fp8.read_blocks(pool, 0, flat, case.flag)]
+        results.append((prompt, new, *read))
+    assert int(case.flag.item()) == 0
+    assert all(torch.equal(a, b) for a, b in zip(*results))
+
+
+def test_operators_on_another_stream_and_two_at_once() -> None:
+    case = CacheCase(38, [300, 40, 17])
+    lengths, prefix, flat = case.batch()[:3]
+    query, x, weight = randn(39, 3, 32, 64).half(), randn(40, 70, 256).half(), fp8.quantize_weight(randn(41, 200, 256))
+    total = flat.numel()
+    attend = lambda: fp8.decode_attention(case.cache, LAYER, query, lengths, prefix, flat, total, case.flag)  # noqa: E731
+    product = lambda: fp8.linear(fp8.quantize_rows(x), weight)  # noqa: E731
+    expected = attend(), product()
+    torch.cuda.synchronize()
+    streams, results = [torch.cuda.Stream() for _ in range(2)], []
+    for _ in range(20):
+        for stream in streams:
+            with torch.cuda.stream(stream):
+                results.append((attend(), product()))
+    torch.cuda.synchronize()
+    assert all(torch.equal(a, b) for pair in results for a, b in zip(pair, expected))
+
+
 def test_cache_refusals() -> None:
     case = CacheCase(41, [20])
     lengths, prefix, flat, total = case.batch()
