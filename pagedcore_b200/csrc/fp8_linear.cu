@@ -640,12 +640,21 @@ __global__ void __launch_bounds__(RowsShape<N>::kThreads, 1)
 // bounds the latter.  CTA 0 of a pair (the leader) issues the MMAs of both; the
 // barriers that it waits on (full, tmem_empty) live in its shared memory and the other
 // CTA's loads and epilogue signal them there, and its commits signal empty and
-// tmem_full in both.  Sixteen epilogue warps, 64 columns each; persistent.
+// tmem_full in both.  Sixteen epilogue warps, 64 columns each; persistent.  The epilogue
+// bounds it, so its warps take registers from the others' warpgroup: 32 columns are under
+// way at a time and nothing is spilled (2047 x 11264 x 2048: 49.9 us, 1.89 PFLOP/s; 16 at
+// a time within 96 registers 56.6, two 16s in turn 52.8, and 60.4 with the scales two
+// blocks ahead and spills).  Two halves of 128 columns with two TMEM buffers and an issuing
+// warp each: 58.0.
 // ---------------------------------------------------------------------------
 struct PairShape {
     static constexpr int kN = 256;
     static constexpr int kEpilogueWarps = 16;
-    static constexpr int kThreads = (kEpilogueWarps + 3) * 32;
+    static constexpr int kThreads = (kEpilogueWarps + 4) * 32;  // the last warp only gives up its registers
+    // Registers a thread: launched with, and how the warpgroups then share them.
+    static constexpr int kRegisters = 96, kEpilogueRegisters = 112, kOtherRegisters = 32;
+    static_assert(kEpilogueWarps * kEpilogueRegisters + 4 * kOtherRegisters <= (kEpilogueWarps + 4) * kRegisters,
+                  "an increase would wait for registers that the block was not launched with");
     static constexpr int kXBytes = kTileRows * kKBlock;
     static constexpr int kStageBytes = kXBytes + kN / 2 * kKBlock;
     static constexpr int kStages = 6;
@@ -732,63 +741,67 @@ __global__ void __launch_bounds__(PairShape::kThreads, 1)
     const uint32_t tmem = tmem_slot;
     pkv::pdl_launch_dependents();
 
-    if (warp == kProducer) {
-        pkv::pdl_wait();
-        if (lane == 0) {
-            int issued = 0;
-            bool ok = true;
-            for (int tile = first_tile; ok && tile < a.tiles; tile += tile_step) {
-                const int m0 = tile % a.m_tiles * 256 + rank * 128, n0 = tile / a.m_tiles * S::kN + rank * 128;
-                for (int i = 0; i < count; ++i) {
-                    const int st = issued % S::kStages;
-                    if (issued >= S::kStages &&
-                        !wait_bounded(pkv::smem_addr(&empty[st]), ((issued / S::kStages) - 1) & 1, a.error_flag)) {
-                        ok = false;
-                        break;
+    if (warp >= kProducer) {
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(S::kOtherRegisters));
+        if (warp == kProducer) {
+            pkv::pdl_wait();
+            if (lane == 0) {
+                int issued = 0;
+                bool ok = true;
+                for (int tile = first_tile; ok && tile < a.tiles; tile += tile_step) {
+                    const int m0 = tile % a.m_tiles * 256 + rank * 128, n0 = tile / a.m_tiles * S::kN + rank * 128;
+                    for (int i = 0; i < count; ++i) {
+                        const int st = issued % S::kStages;
+                        if (issued >= S::kStages &&
+                            !wait_bounded(pkv::smem_addr(&empty[st]), ((issued / S::kStages) - 1) & 1, a.error_flag)) {
+                            ok = false;
+                            break;
+                        }
+                        const uint32_t dst = base + st * S::kStageBytes;
+                        if (rank == 0) pkv::mbar_arrive_expect_tx(pkv::smem_addr(&full[st]), 2 * S::kStageBytes);
+                        const uint32_t bar = map_to_rank(pkv::smem_addr(&full[st]), 0);
+                        tma_load_pair(dst, &x_map, i * kKBlock, m0, bar);
+                        tma_load_pair(dst + S::kXBytes, &w_map, i * kKBlock, n0, bar);
+                        ++issued;
                     }
-                    const uint32_t dst = base + st * S::kStageBytes;
-                    if (rank == 0) pkv::mbar_arrive_expect_tx(pkv::smem_addr(&full[st]), 2 * S::kStageBytes);
-                    const uint32_t bar = map_to_rank(pkv::smem_addr(&full[st]), 0);
-                    tma_load_pair(dst, &x_map, i * kKBlock, m0, bar);
-                    tma_load_pair(dst + S::kXBytes, &w_map, i * kKBlock, n0, bar);
-                    ++issued;
+                }
+                // No copy may land after the CTA has left: every stage has been multiplied
+                // (or, where a wait ran out, long since filled).
+                for (int i = max(0, issued - S::kStages); i < issued; ++i) {
+                    wait_bounded(pkv::smem_addr(&empty[i % S::kStages]), (i / S::kStages) & 1, a.error_flag);
                 }
             }
-            // No copy may land after the CTA has left: every stage has been multiplied
-            // (or, where a wait ran out, long since filled).
-            for (int i = max(0, issued - S::kStages); i < issued; ++i) {
-                wait_bounded(pkv::smem_addr(&empty[i % S::kStages]), (i / S::kStages) & 1, a.error_flag);
-            }
-        }
-        __syncwarp();
-    } else if (warp >= kMma) {
-        pkv::pdl_wait();
-        if (rank == 0 && lane == 0) {
-            constexpr uint32_t idesc = idesc_e4m3_f32(256, S::kN);
-            int done = 0;
-            bool ok = true;
-            for (int tile = first_tile; ok && tile < a.tiles; tile += tile_step) {
-                for (int i = 0; i < count; ++i, ++done) {
-                    const int st = done % S::kStages;
-                    const int buf = done & 1;
-                    if (buf != warp - kMma) continue;  // two issuing warps, one per TMEM buffer
-                    ok = wait_bounded(pkv::smem_addr(&full[st]), (done / S::kStages) & 1, a.error_flag) &&
-                         (done < 2 || wait_bounded(pkv::smem_addr(&tmem_empty[buf]), ((done >> 1) - 1) & 1, a.error_flag));
-                    if (!ok) break;
-                    pkv::tc::fence_after_sync();
-                    const uint32_t src = base + st * S::kStageBytes;
+            __syncwarp();
+        } else {
+            pkv::pdl_wait();
+            if (rank == 0 && lane == 0 && warp < kMma + 2) {
+                constexpr uint32_t idesc = idesc_e4m3_f32(256, S::kN);
+                int done = 0;
+                bool ok = true;
+                for (int tile = first_tile; ok && tile < a.tiles; tile += tile_step) {
+                    for (int i = 0; i < count; ++i, ++done) {
+                        const int st = done % S::kStages;
+                        const int buf = done & 1;
+                        if (buf != warp - kMma) continue;  // two issuing warps, one per TMEM buffer
+                        ok = wait_bounded(pkv::smem_addr(&full[st]), (done / S::kStages) & 1, a.error_flag) &&
+                             (done < 2 || wait_bounded(pkv::smem_addr(&tmem_empty[buf]), ((done >> 1) - 1) & 1, a.error_flag));
+                        if (!ok) break;
+                        pkv::tc::fence_after_sync();
+                        const uint32_t src = base + st * S::kStageBytes;
 #pragma unroll
-                    for (int k = 0; k < kKBlock / 32; ++k) {
-                        mma_f8_pair(tmem + buf * 256, pkv::tc::desc_k_major_sw128(src + 32 * k),
-                                    pkv::tc::desc_k_major_sw128(src + S::kXBytes + 32 * k), idesc, k > 0);
+                        for (int k = 0; k < kKBlock / 32; ++k) {
+                            mma_f8_pair(tmem + buf * 256, pkv::tc::desc_k_major_sw128(src + 32 * k),
+                                        pkv::tc::desc_k_major_sw128(src + S::kXBytes + 32 * k), idesc, k > 0);
+                        }
+                        commit_pair(pkv::smem_addr(&empty[st]));
+                        commit_pair(pkv::smem_addr(&tmem_full[buf]));
                     }
-                    commit_pair(pkv::smem_addr(&empty[st]));
-                    commit_pair(pkv::smem_addr(&tmem_full[buf]));
                 }
             }
+            __syncwarp();
         }
-        __syncwarp();
     } else {
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(S::kEpilogueRegisters));
         pkv::pdl_wait();
         const int quarter = warp & 3, first = (warp >> 2) * 64;
         const uint32_t src = tmem + (static_cast<uint32_t>(quarter * 32) << 16) + first;
@@ -799,46 +812,34 @@ __global__ void __launch_bounds__(PairShape::kThreads, 1)
         bool ok = true;
         for (int tile = first_tile; tile < a.tiles; tile += tile_step) {
             const int m0 = tile % a.m_tiles * 256 + rank * 128, n0 = tile / a.m_tiles * S::kN;
-            const float *sx = a.x_scales + static_cast<int64_t>(min(m0 + quarter * 32 + lane, a.rows - 1)) * count;
-            const float *sw = a.w_scales + static_cast<int64_t>(min((n0 + first) / kTileRows, a.w_blocks - 1)) * count;
-            // Scales two K blocks ahead, in registers of their own for even and odd blocks.
-            float x[2], w[2];
-            x[0] = __ldg(sx), w[0] = __ldg(sw);
-            x[1] = w[1] = 0.f;
-            if (count > 1) x[1] = __ldg(sx + 1), w[1] = __ldg(sw + 1);
+            // Below 2^32: with more than one K block a row has 72 codes or more a scale.
+            uint32_t sx = static_cast<uint32_t>(min(m0 + quarter * 32 + lane, a.rows - 1)) * count;
+            uint32_t sw = static_cast<uint32_t>(min((n0 + first) / kTileRows, a.w_blocks - 1)) * count;
+            float x = __ldg(a.x_scales + sx), w = __ldg(a.w_scales + sw);  // a K block ahead
 #pragma unroll
             for (int c = 0; c < 32; ++c) acc[c] = 0;
-            for (int i = 0; i < count; i += 2) {
+#pragma unroll 1
+            for (int i = 1; i <= count; ++i) {
+                const float f = x * w;
+                const uint64_t f2 = pkv::f32x2(f, f);
+                if (i < count) x = __ldg(a.x_scales + ++sx), w = __ldg(a.w_scales + ++sw);
+                const int buf = done & 1;
+                if (ok) ok = wait_bounded(pkv::smem_addr(&tmem_full[buf]), (done >> 1) & 1, a.error_flag);
+                ok = __all_sync(0xffffffffu, ok);
+                ++done;
+                if (ok) {
+                    pkv::tc::fence_after_sync();
 #pragma unroll
-                for (int odd = 0; odd < 2; ++odd) {
-                    if (i + odd < count) {
-                        const int buf = done & 1;
-                        const float f = x[odd] * w[odd];
-                        const uint64_t f2 = pkv::f32x2(f, f);
-                        if (i + odd + 2 < count) x[odd] = __ldg(sx + i + odd + 2), w[odd] = __ldg(sw + i + odd + 2);
-                        if (ok) ok = wait_bounded(pkv::smem_addr(&tmem_full[buf]), (done >> 1) & 1, a.error_flag);
-                        ok = __all_sync(0xffffffffu, ok);
-                        ++done;
-                        if (ok) {
-                            pkv::tc::fence_after_sync();
-#pragma unroll
-                            for (int c = 0; c < 4; ++c) {
-                                uint32_t d[16];
-                                pkv::tc::tmem_ld16(src + buf * 256 + 16 * c, d);
-                                pkv::tc::tmem_wait_ld();
-                                if (c == 3) {
-                                    pkv::tc::fence_before_sync();
-                                    __syncwarp();
-                                    if (lane == 0) arrive_cluster(empty0 + 8 * buf);
-                                }
-#pragma unroll
-                                for (int j = 0; j < 8; ++j) {
-                                    acc[8 * c + j] = pkv::fma_f32x2(
-                                        pkv::f32x2(__uint_as_float(d[2 * j]), __uint_as_float(d[2 * j + 1])), f2,
-                                        acc[8 * c + j]);
-                                }
-                            }
+                    for (int c = 0; c < 2; ++c) {
+                        uint32_t d[32];
+                        pkv::tc::tmem_ld32(src + buf * 256 + 32 * c, d);
+                        pkv::tc::tmem_wait_ld();
+                        if (c == 1) {
+                            pkv::tc::fence_before_sync();
+                            __syncwarp();
+                            if (lane == 0) arrive_cluster(empty0 + 8 * buf);
                         }
+                        add_scaled(acc + 16 * c, d, f2);
                     }
                 }
             }
@@ -984,12 +985,28 @@ int launch_rows(int device, const void *x, int64_t x_stride, const void *w, int3
                          args.splits, stream);
 }
 
+// The pair kernel's warpgroups share out the registers it was planned to be launched with.
+int check_registers(int device) {
+    static std::atomic<int> checked[kMaxDevices] = {};
+    const bool known = device >= 0 && device < kMaxDevices;
+    if (known && checked[device].load(std::memory_order_acquire)) return PKV_OK;
+    cudaFuncAttributes attributes;
+    const cudaError_t e = cudaFuncGetAttributes(&attributes, reinterpret_cast<const void *>(fp8_linear_pair_kernel));
+    if (e != cudaSuccess) return pkv::fail(PKV_CUDA_ERROR, std::string("fp8 linear: cudaFuncGetAttributes: ") + cudaGetErrorString(e));
+    if (attributes.numRegs < PairShape::kRegisters) {
+        return pkv::fail(PKV_CUDA_ERROR, "fp8 linear: the pair kernel was compiled to fewer registers than its warps share out");
+    }
+    if (known) checked[device].store(1, std::memory_order_release);
+    return PKV_OK;
+}
+
 int launch_pairs(int device, const void *x, int64_t x_stride, const void *w, int32_t k, int sms, LinearArgs &args,
                  cudaStream_t stream) {
     using S = PairShape;
     static std::atomic<int> prepared[kMaxDevices] = {};
     int rc = prepare(reinterpret_cast<const void *>(fp8_linear_pair_kernel), S::kSmem, device, prepared);
     if (rc) return rc;
+    if ((rc = check_registers(device))) return rc;
     CUtensorMap w_map, x_map;
     if ((rc = operand_maps(x, x_stride, kTileRows, w, S::kN / 2, k, args, &w_map, &x_map))) return rc;
     const int64_t m_tiles = (static_cast<int64_t>(args.rows) + 255) / 256;
