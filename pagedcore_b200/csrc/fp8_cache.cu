@@ -299,7 +299,9 @@ dim3 append_grid(AppendArgs &a, int layers) {
     return dim3(a.tile_ctas + (a.query_in != nullptr ? (a.tokens + kQuerySpan - 1) / kQuerySpan : 0), layers);
 }
 
-__global__ void __launch_bounds__(kThreads, 3) fp8_append_kernel(const __grid_constant__ AppendArgs a) {
+// Two CTAs an SM: with the 80 registers that three leave, the write of a run spills
+// (2047 tokens with queries 10.2 us, 9.4 so; 8.6 and 7.0 without queries).
+__global__ void __launch_bounds__(kThreads, 2) fp8_append_kernel(const __grid_constant__ AppendArgs a) {
     // In this order: the decode attention behind it reads what is older than this
     // kernel (the tables, the cache but for the blocks written here) before its own wait.
     pkv::pdl_wait();
