@@ -11,11 +11,12 @@
 namespace pkv {
 
 template <typename... KernelArgs, typename... Args>
-cudaError_t launch_pdl(void (*kernel)(KernelArgs...), dim3 grid, dim3 block, cudaStream_t stream, Args... args) {
+cudaError_t launch_pdl_smem(void (*kernel)(KernelArgs...), dim3 grid, dim3 block, size_t smem, cudaStream_t stream,
+                            Args... args) {
     cudaLaunchConfig_t config = {};
     config.gridDim = grid;
     config.blockDim = block;
-    config.dynamicSmemBytes = 0;
+    config.dynamicSmemBytes = smem;
     config.stream = stream;
     cudaLaunchAttribute attribute[1];
     attribute[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
@@ -23,6 +24,11 @@ cudaError_t launch_pdl(void (*kernel)(KernelArgs...), dim3 grid, dim3 block, cud
     config.attrs = attribute;
     config.numAttrs = 1;
     return cudaLaunchKernelEx(&config, kernel, static_cast<KernelArgs>(args)...);
+}
+
+template <typename... KernelArgs, typename... Args>
+cudaError_t launch_pdl(void (*kernel)(KernelArgs...), dim3 grid, dim3 block, cudaStream_t stream, Args... args) {
+    return launch_pdl_smem(kernel, grid, block, 0, stream, args...);
 }
 
 }  // namespace pkv

@@ -75,6 +75,7 @@
 #include <string>
 
 #include "pagedkv.h"
+#include "pdl.h"
 #include "ptx.cuh"
 #include "status.h"
 #include "tcgen05.cuh"
@@ -287,8 +288,6 @@ __global__ void __maxnreg__(120)
     const int lane = threadIdx.x & 31;
 
     // ---- set-up ----------------------------------------------------------
-    // Every item reads the same block table (the chunk's request).
-    for (int j = threadIdx.x; j <= (written - 1) / kBlockTokens; j += kThreads) table[j] = a.blocks[j];
     if (warp == kMmaWarp) {
         pkv::tc::tmem_alloc(pkv::smem_addr(&tmem_slot), kTmemCols);
         pkv::tc::tmem_relinquish();
@@ -313,6 +312,9 @@ __global__ void __maxnreg__(120)
         abort_flag = 0;
         pkv::fence_barrier_init();
     }
+    if constexpr (SPLIT_Q) pkv::pdl_wait();  // a programmatic dependent of the read that fills its pool
+    // Every item reads the same block table (the chunk's request).
+    for (int j = threadIdx.x; j <= (written - 1) / kBlockTokens; j += kThreads) table[j] = a.blocks[j];
     pkv::tc::fence_before_sync();
     __syncthreads();
     pkv::tc::fence_after_sync();
@@ -701,8 +703,13 @@ int launch(const TcArgs &args, cudaStream_t stream) {
     if (rc) return rc;
     // One CTA per resident slot at most; each walks its share of the items.
     const int items = (args.tokens + kTileTokens - 1) / kTileTokens * kKvHeads;
-    prefill_tc_kernel<SPLIT_Q><<<std::min(items, resident), kThreads, kSmemBytes<SPLIT_Q>, stream>>>(args);
-    e = cudaGetLastError();
+    if constexpr (SPLIT_Q) {
+        e = pkv::launch_pdl_smem(prefill_tc_kernel<true>, dim3(std::min(items, resident)), dim3(kThreads), kSmemBytes<true>,
+                                 stream, args);
+    } else {
+        prefill_tc_kernel<false><<<std::min(items, resident), kThreads, kSmemBytes<false>, stream>>>(args);
+        e = cudaGetLastError();
+    }
     if (e != cudaSuccess) {
         return pkv::fail(PKV_CUDA_ERROR, std::string("prefill attention launch failed: ") + cudaGetErrorString(e));
     }
