@@ -97,7 +97,7 @@ class Fp8Rows:
         if not self.codes.is_contiguous():
             raise ValueError("to_half needs contiguous codes")
         if out is None:
-            out = self.codes.new_empty((rows, width), dtype=_HALF)
+            out = torch.empty_like(self.codes, dtype=_HALF)
             stride = width
         else:
             if out.shape != (rows, width) or out.dtype is not _HALF or out.stride(1) != 1 or out.get_device() != index:
@@ -133,8 +133,10 @@ def _check_rows(x: Fp8Rows) -> tuple[int, int]:
 
 def _empty_rows(x: Tensor, rows: int, width: int) -> Fp8Rows:
     """Uninitialised 8-bit rows on the device of ``x``."""
+    device = x.device  # sizes one by one: torch.empty takes a tuple 0.7 us slower
     return Fp8Rows(
-        x.new_empty((rows, width), dtype=_CODES), x.new_empty((rows, _groups(width)), dtype=_FLOAT)
+        torch.empty(rows, width, dtype=_CODES, device=device),
+        torch.empty(rows, -(-width // GROUP), dtype=_FLOAT, device=device),
     )
 
 
@@ -240,7 +242,7 @@ def linear(x: Fp8Rows, weight: Fp8Weight, out: Tensor | None = None) -> Tensor:
     index = _device(x.codes, x.scales, codes, scales)
     x_stride = _row_stride("x", x.codes, k)
     if out is None:
-        out = codes.new_empty((rows, n), dtype=_HALF)
+        out = torch.empty(rows, n, dtype=_HALF, device=codes.device)
         stride = n
     else:
         if out.shape != (rows, n) or out.dtype is not _HALF or out.stride(1) != 1 or out.get_device() != index:
@@ -433,7 +435,7 @@ def read_blocks(cache: Fp8Cache, layer: int, blocks: Tensor, error_flag: Tensor)
     count = blocks.numel()
     blocks_ptr = _int_list(index, "blocks", blocks, count)
     flag = _int_list(index, "error_flag", error_flag, 1)
-    key = blocks.new_empty((count, _BLOCK_TOKENS, _KV_HEADS, _HEAD_DIM), dtype=_HALF)
+    key = torch.empty(count, _BLOCK_TOKENS, _KV_HEADS, _HEAD_DIM, dtype=_HALF, device=blocks.device)
     value = torch.empty_like(key)
     if count:
         _call(index, lib.pkv_fp8_read_blocks, *cache._args(), layer, blocks_ptr, count, key.data_ptr(),
@@ -487,7 +489,7 @@ def _decode(cache, layer, query, new, lengths, prefix, flat, total_blocks, error
     query, query_stride, out, out_stride = _query_and_out(query, out, index, "batch")
     batch = query.shape[0]
     grid, workspace_bytes = decode_plan(index, batch, total_blocks)
-    workspace = query.new_empty((workspace_bytes + 1) // 2)
+    workspace = torch.empty((workspace_bytes + 1) // 2, dtype=_HALF, device=query.device)
     _call(
         index, lib.pkv_fp8_decode_attention if new is None else lib.pkv_fp8_decode_layer, *cache._args(), layer,
         query.data_ptr(), query_stride, *(new or ()), _int_list(index, "lengths", lengths, batch),
@@ -574,7 +576,7 @@ def prefill_attention(
         raise ValueError("the chunk must hold 1 or more tokens at positions below 2048")
     count = -(-(start + tokens) // _BLOCK_TOKENS)
     blocks_ptr = _int_list(index, "blocks", blocks, count)
-    workspace = out.new_empty(count * _PREFILL_BLOCK_BYTES // 2)
+    workspace = torch.empty(count * _PREFILL_BLOCK_BYTES // 2, dtype=_HALF, device=out.device)
     _call(index, lib.pkv_fp8_prefill_attention, *cache._args(), layer, query.data_ptr(), query.dtype is _FLOAT,
           query_stride, blocks_ptr, start, tokens, out.data_ptr(), out_stride, workspace.data_ptr(),
           count * _PREFILL_BLOCK_BYTES, _int_list(index, "error_flag", error_flag, 1))
