@@ -642,10 +642,12 @@ __global__ void __launch_bounds__(RowsShape<N>::kThreads, 1)
 // CTA's loads and epilogue signal them there, and its commits signal empty and
 // tmem_full in both.  Sixteen epilogue warps, 64 columns each; persistent.  The epilogue
 // bounds it, so its warps take registers from the others' warpgroup: 32 columns are under
-// way at a time and nothing is spilled (2047 x 11264 x 2048: 49.9 us, 1.89 PFLOP/s; 16 at
-// a time within 96 registers 56.6, two 16s in turn 52.8, and 60.4 with the scales two
-// blocks ahead and spills).  Two halves of 128 columns with two TMEM buffers and an issuing
-// warp each: 58.0.
+// way at a time and nothing is spilled, and bulk stores take the tile out while the next
+// one begins: 2047 x 11264 x 2048 in 49.3 us, 1.92 PFLOP/s, 2047 x 2048 x 5632 in 25.0.
+// (The first without the bulk stores 51.3; 16 columns at a time within 96 registers 56.6;
+// 60.4 with the scales two blocks ahead and spills.  With all 64 columns staged at once and
+// five stages the first takes 47.8, the second 26.5.  Two halves of 128 columns with two
+// TMEM buffers and an issuing warp each: 58.0.)
 // ---------------------------------------------------------------------------
 struct PairShape {
     static constexpr int kN = 256;
@@ -658,10 +660,50 @@ struct PairShape {
     static constexpr int kXBytes = kTileRows * kKBlock;
     static constexpr int kStageBytes = kXBytes + kN / 2 * kKBlock;
     static constexpr int kStages = 6;
-    static constexpr int kStoreBytes = 32 * 64;
+    static constexpr int kStoreBytes = 32 * 64;  // a warp's 32 rows of 64 FP16 values
     static constexpr int kRing = kStages * kStageBytes;
     static constexpr int kSmem = kRing + kEpilogueWarps * kStoreBytes + 1024;
 };
+
+// Every lane may write the warp's staging again.
+__device__ __forceinline__ void wait_staging(int lane) {
+    if (lane == 0) asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
+    __syncwarp();
+}
+
+// A warp's 32 rows x 64 columns of sums (row = lane, `acc` two columns a pair) as FP16, 32
+// columns at a time, in its staging (rows of 64 bytes with the 64-byte swizzle), from where
+// a bulk tensor store takes them, the second while the warp goes on.  The store leaves out
+// rows past the last, and columns in whole 16 bytes only.  The staging is free again after
+// wait_staging.
+__device__ __forceinline__ void store_rows_async(const CUtensorMap *map, const uint64_t *acc, uint32_t staging, int m,
+                                                 int n, int lane) {
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+        if (h) wait_staging(lane);
+#pragma unroll
+        for (int c = 0; c < 4; ++c) {
+            uint32_t w[4];
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                const float2 v = pkv::unpack_f32x2(acc[16 * h + 4 * c + j]);
+                w[j] = pkv::pack_half2(__floats2half2_rn(v.x, v.y));
+            }
+            asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(staging + lane * 64 + ((c ^ ((lane >> 1) & 3)) << 4)),
+                         "r"(w[0]), "r"(w[1]), "r"(w[2]), "r"(w[3])
+                         : "memory");
+        }
+        pkv::fence_proxy_async_smem();
+        __syncwarp();
+        if (lane == 0) {
+            asm volatile("cp.async.bulk.tensor.2d.global.shared::cta.bulk_group [%0, {%1, %2}], [%3];" ::"l"(
+                             reinterpret_cast<uint64_t>(map)),
+                         "r"(n + 32 * h), "r"(m), "r"(staging)
+                         : "memory");
+            asm volatile("cp.async.bulk.commit_group;" ::: "memory");
+        }
+    }
+}
 
 __device__ __forceinline__ void mma_f8_pair(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc, uint32_t idesc,
                                             bool accumulate) {
@@ -700,7 +742,7 @@ __device__ __forceinline__ void arrive_cluster(uint32_t bar) {
 
 __global__ void __launch_bounds__(PairShape::kThreads, 1)
     fp8_linear_pair_kernel(const __grid_constant__ CUtensorMap w_map, const __grid_constant__ CUtensorMap x_map,
-                           const LinearArgs a) {
+                           const __grid_constant__ CUtensorMap out_map, const LinearArgs a) {
     using S = PairShape;
     extern __shared__ uint8_t dyn_smem[];
     __shared__ uint64_t full[S::kStages], empty[S::kStages], tmem_full[2], tmem_empty[2];
@@ -805,7 +847,6 @@ __global__ void __launch_bounds__(PairShape::kThreads, 1)
         pkv::pdl_wait();
         const int quarter = warp & 3, first = (warp >> 2) * 64;
         const uint32_t src = tmem + (static_cast<uint32_t>(quarter * 32) << 16) + first;
-        const uint32_t staging = base + S::kRing + warp * S::kStoreBytes;
         const uint32_t empty0 = map_to_rank(pkv::smem_addr(&tmem_empty[0]), 0);
         uint64_t acc[32];
         int done = 0;
@@ -843,8 +884,22 @@ __global__ void __launch_bounds__(PairShape::kThreads, 1)
                     }
                 }
             }
-            store_rows(a, acc, staging, m0 + quarter * 32, n0 + first, lane);
+            // From the thread's index anew: kept from before they would spill in the loop above.
+            uint32_t thread;
+            asm volatile("mov.u32 %0, %%tid.x;" : "=r"(thread));
+            const int own = static_cast<int>(thread & 31), part = static_cast<int>(thread >> 5);
+            const int m = tile % a.m_tiles * 256 + rank * 128 + (part & 3) * 32, n = tile / a.m_tiles * S::kN + (part >> 2) * 64;
+            const uint32_t staging = base + S::kRing + part * S::kStoreBytes;
+            if (m < a.rows && n < a.n) {
+                wait_staging(own);
+                if (a.vector_out && (n + 64 <= a.n || a.n % 8 == 0)) {
+                    store_rows_async(&out_map, acc, staging, m, n, own);
+                } else {
+                    store_rows(a, acc, staging, m, n, own);
+                }
+            }
         }
+        if (lane == 0) asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
     }
     __syncwarp();
     pkv::tc::fence_before_sync();
@@ -880,6 +935,23 @@ int byte_matrix_map(const void *base, uint64_t rows, uint64_t cols, uint64_t str
     return PKV_OK;
 }
 
+// Map of the output (16-byte aligned rows) in swizzled boxes, to store from.
+int half_matrix_map(const LinearArgs &args, uint32_t box_columns, uint32_t box_rows, CUtensorMap *out) {
+    const pkv::EncodeTiled encode = pkv::encode_fn();
+    if (encode == nullptr) return pkv::fail(PKV_CUDA_ERROR, "cuTensorMapEncodeTiled is unavailable");
+    const cuuint64_t dims[2] = {static_cast<cuuint64_t>(args.n), static_cast<cuuint64_t>(args.rows)};
+    const cuuint64_t strides[1] = {static_cast<cuuint64_t>(args.out_stride) * 2};
+    const cuuint32_t box[2] = {box_columns, box_rows};
+    const cuuint32_t elem[2] = {1u, 1u};
+    const CUresult r = encode(out, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 2, args.out, dims, strides, box, elem,
+                              CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_64B,
+                              CU_TENSOR_MAP_L2_PROMOTION_NONE, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    if (r != CUDA_SUCCESS) {
+        return pkv::fail(PKV_CUDA_ERROR, "cuTensorMapEncodeTiled (output) failed with code " + std::to_string(int(r)));
+    }
+    return PKV_OK;
+}
+
 int sm_count(int device) {
     static std::atomic<int> cached[kMaxDevices] = {};
     if (device >= 0 && device < kMaxDevices) {
@@ -904,10 +976,9 @@ int prepare(const void *kernel, int smem, int device, std::atomic<int> *prepared
     return PKV_OK;
 }
 
-using Kernel = void (*)(CUtensorMap, CUtensorMap, LinearArgs);
-
-int launch_kernel(Kernel kernel, int grid, int threads, int smem, const CUtensorMap &w_map, const CUtensorMap &x_map,
-                  const LinearArgs &args, int cluster, cudaStream_t stream) {
+template <typename... KernelArgs>
+int launch_kernel(void (*kernel)(KernelArgs...), int grid, int threads, int smem, int cluster, cudaStream_t stream,
+                  const KernelArgs &...args) {
     cudaLaunchConfig_t config = {};
     config.gridDim = dim3(grid);
     config.blockDim = dim3(threads);
@@ -922,7 +993,7 @@ int launch_kernel(Kernel kernel, int grid, int threads, int smem, const CUtensor
     attributes[1].val.clusterDim.z = 1;
     config.attrs = attributes;
     config.numAttrs = cluster > 1 ? 2 : 1;
-    const cudaError_t e = cudaLaunchKernelEx(&config, kernel, w_map, x_map, args);
+    const cudaError_t e = cudaLaunchKernelEx(&config, kernel, args...);
     if (e != cudaSuccess) return pkv::fail(PKV_CUDA_ERROR, std::string("fp8 linear launch failed: ") + cudaGetErrorString(e));
     return PKV_OK;
 }
@@ -963,8 +1034,8 @@ int launch_few(int device, const void *x, int64_t x_stride, const void *w, int32
     if (static_cast<int64_t>(args.n_tiles) * args.splits > INT32_MAX) {
         return pkv::fail(PKV_VALUE_ERROR, "fp8 linear: too many tiles");
     }
-    return launch_kernel(fp8_linear_kernel<NT>, args.n_tiles * args.splits, S::kThreads, S::kSmem, w_map, x_map, args,
-                         args.splits, stream);
+    return launch_kernel(fp8_linear_kernel<NT>, args.n_tiles * args.splits, S::kThreads, S::kSmem, args.splits, stream,
+                         w_map, x_map, args);
 }
 
 template <int N>
@@ -983,8 +1054,8 @@ int launch_rows(int device, const void *x, int64_t x_stride, const void *w, int3
     args.tiles = static_cast<int32_t>(tiles);
     args.splits = row_splits(tiles, args.k_blocks, sms, kRowsCluster);
     const int64_t grid = args.splits > 1 ? tiles * args.splits : tiles < sms ? tiles : sms;
-    return launch_kernel(fp8_linear_rows_kernel<N>, static_cast<int>(grid), S::kThreads, S::kSmem, w_map, x_map, args,
-                         args.splits, stream);
+    return launch_kernel(fp8_linear_rows_kernel<N>, static_cast<int>(grid), S::kThreads, S::kSmem, args.splits, stream,
+                         w_map, x_map, args);
 }
 
 // The pair kernel's warpgroups share out the registers it was planned to be launched with.
@@ -1017,8 +1088,10 @@ int launch_pairs(int device, const void *x, int64_t x_stride, const void *w, int
     args.m_tiles = static_cast<int32_t>(m_tiles);
     args.tiles = static_cast<int32_t>(tiles);
     const int64_t pairs = tiles < sms / 2 ? tiles : sms / 2;
-    return launch_kernel(fp8_linear_pair_kernel, static_cast<int>(2 * pairs), S::kThreads, S::kSmem, w_map, x_map, args, 2,
-                         stream);
+    CUtensorMap out_map = x_map;  // of no use to outputs that a tensor map cannot describe
+    if (args.vector_out && (rc = half_matrix_map(args, 32, 32, &out_map))) return rc;
+    return launch_kernel(fp8_linear_pair_kernel, static_cast<int>(2 * pairs), S::kThreads, S::kSmem, 2, stream, w_map, x_map,
+                         out_map, args);
 }
 
 }  // namespace

@@ -211,6 +211,17 @@ def test_linear_takes_strided_rows_and_outputs() -> None:
     assert fp8.linear(fp8.Fp8Rows(x.codes[:0], x.scales[:0]), weight).shape == (0, 77)
 
 
+@pytest.mark.parametrize("n, width, first", [(8203, 8216, 8), (8203, 8216, 3), (8203, 8205, 0), (8200, 8216, 8)])
+def test_linear_of_many_rows_leaves_what_lies_beside_its_output(n, width, first) -> None:
+    rows = 1500  # tiles of 256 rows; 8203 columns end inside 16 bytes
+    x, weight = random_operands(8, rows, n, 1040)
+    expected = fp8.linear(x, weight)
+    out = torch.full((rows + 40, width), 9.0, dtype=torch.float16, device=expected.device)
+    fp8.linear(x, weight, out[:rows, first : first + n])
+    assert torch.equal(out[:rows, first : first + n], expected)
+    assert bool((out[rows:] == 9).all()) and bool((out[:, :first] == 9).all()) and bool((out[:, first + n :] == 9).all())
+
+
 def test_linear_keeps_rows_apart() -> None:
     x, weight = random_operands(6, 20, 256, 384)
     clean = fp8.linear(x, weight)
