@@ -37,6 +37,8 @@ _HALF = torch.float16
 _FLOAT = torch.float32
 _INT = torch.int32
 _ROW = _QUERY_HEADS * _HEAD_DIM  # values of a query row
+_current_device = torch._C._cuda_getDevice
+_raw_stream = torch._C._cuda_getCurrentRawStream
 
 
 def _groups(width: int) -> int:
@@ -60,11 +62,11 @@ def _call(index: int, function, *args) -> None:
     The raw stream handle spares the Stream object that
     ``torch.cuda.current_stream`` builds (2 us of a 5 us call).
     """
-    if torch._C._cuda_getDevice() == index:
-        status = function(*args, torch._C._cuda_getCurrentRawStream(index))
+    if _current_device() == index:
+        status = function(*args, _raw_stream(index))
     else:
         with torch.cuda.device(index):
-            status = function(*args, torch._C._cuda_getCurrentRawStream(index))
+            status = function(*args, _raw_stream(index))
     if status:
         check(status)
 
@@ -93,18 +95,19 @@ class Fp8Rows:
     def to_half(self, out: Tensor | None = None) -> Tensor:
         """The values as FP16 [rows, width] (exact for scales made by this module)."""
         rows, width = _check_rows(self)
-        index = _device(self.codes, self.scales)
-        if not self.codes.is_contiguous():
+        codes, scales = self.codes, self.scales
+        index = _device(codes, scales)
+        if not codes.is_contiguous():
             raise ValueError("to_half needs contiguous codes")
         if out is None:
-            out = torch.empty_like(self.codes, dtype=_HALF)
+            out = torch.empty_like(codes, dtype=_HALF)
             stride = width
         else:
             if out.shape != (rows, width) or out.dtype is not _HALF or out.stride(1) != 1 or out.get_device() != index:
                 raise ValueError(f"out must be FP16 [{rows}, {width}] with contiguous rows")
             stride = _row_stride("out", out, width)
         if rows:
-            _call(index, lib.pkv_fp8_to_half, self.codes.data_ptr(), self.scales.data_ptr(), rows, width,
+            _call(index, lib.pkv_fp8_to_half, codes.data_ptr(), scales.data_ptr(), rows, width,
                   out.data_ptr(), stride)
         return out
 
@@ -123,10 +126,11 @@ class Fp8Weight:
 
 def _check_rows(x: Fp8Rows) -> tuple[int, int]:
     codes, scales = x.codes, x.scales
-    if codes.ndim != 2 or codes.dtype is not _CODES or codes.stride(1) != 1:
+    shape = codes.shape
+    if len(shape) != 2 or codes.dtype is not _CODES or codes.stride(1) != 1:
         raise ValueError("8-bit rows must be E4M3 [rows, width] with contiguous rows")
-    rows, width = codes.shape
-    if scales.shape != (rows, _groups(width)) or scales.dtype is not _FLOAT or not scales.is_contiguous():
+    rows, width = shape
+    if scales.shape != (rows, -(-width // GROUP)) or scales.dtype is not _FLOAT or not scales.is_contiguous():
         raise ValueError("8-bit rows need contiguous FP32 scales [rows, ceil(width / 128)]")
     return rows, width
 
@@ -159,9 +163,10 @@ def add_rms_norm(
     is written as FP16 to ``residual`` (``hidden`` itself by default); the
     norm is taken of the unrounded sum, in FP32, and rounded once, to E4M3.
     """
-    if hidden.ndim != 2:
+    shape = hidden.shape
+    if len(shape) != 2:
         raise ValueError("hidden must be contiguous FP16 [rows, dim]")
-    rows, dim = shape = hidden.shape
+    rows, dim = shape
     _half_matrix("hidden", hidden, shape)
     _half_matrix("weight", weight, (dim,))
     delta_ptr = residual_ptr = None
@@ -234,9 +239,10 @@ def linear(x: Fp8Rows, weight: Fp8Weight, out: Tensor | None = None) -> Tensor:
     """
     rows, k = _check_rows(x)
     codes, scales = weight.codes, weight.scales
-    if codes.ndim != 2 or codes.shape[1] != k or codes.dtype is not _CODES or not codes.is_contiguous():
+    shape = codes.shape
+    if len(shape) != 2 or shape[1] != k or codes.dtype is not _CODES or not codes.is_contiguous():
         raise ValueError(f"weight must be contiguous E4M3 [n, {k}]")
-    n = codes.shape[0]
+    n = shape[0]
     if scales.shape != (_groups(n), _groups(k)) or scales.dtype is not _FLOAT or not scales.is_contiguous():
         raise ValueError("weight needs contiguous FP32 scales [ceil(n / 128), ceil(k / 128)]")
     index = _device(x.codes, x.scales, codes, scales)
