@@ -404,8 +404,8 @@ bool aligned16(const void *p) { return (reinterpret_cast<uintptr_t>(p) & 15u) ==
 
 namespace pkv {
 int launch_prefill_attention_tc(const void *pool, int32_t num_blocks, int32_t layer, const void *query,
-                                bool query_fp32, int64_t query_stride, const int32_t *blocks, int32_t start,
-                                int32_t tokens, void *out, int64_t out_stride, int32_t *error_flag,
+                                bool query_fp32, bool fine, int64_t query_stride, const int32_t *blocks,
+                                int32_t start, int32_t tokens, void *out, int64_t out_stride, int32_t *error_flag,
                                 cudaStream_t stream);
 }
 
@@ -587,6 +587,6 @@ extern "C" int pkv_fp8_prefill_attention(const void *key_codes, const void *valu
                                workspace, static_cast<__half *>(workspace) + count * kBlockValues, table, error_flag,
                                stream);
     if (rc) return rc;
-    return pkv::launch_prefill_attention_tc(workspace, count, 0, query, query_fp32 != 0, query_stride, table, start, tokens,
-                                            out, out_stride, error_flag, static_cast<cudaStream_t>(stream));
+    return pkv::launch_prefill_attention_tc(workspace, count, 0, query, query_fp32 != 0, true, query_stride, table, start,
+                                            tokens, out, out_stride, error_flag, static_cast<cudaStream_t>(stream));
 }

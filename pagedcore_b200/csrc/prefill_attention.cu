@@ -20,8 +20,8 @@
 
 namespace pkv {
 int launch_prefill_attention_tc(const void *pool, int32_t num_blocks, int32_t layer, const void *query,
-                                bool query_fp32, int64_t query_stride, const int32_t *blocks, int32_t start,
-                                int32_t tokens, void *out, int64_t out_stride, int32_t *error_flag,
+                                bool query_fp32, bool fine, int64_t query_stride, const int32_t *blocks,
+                                int32_t start, int32_t tokens, void *out, int64_t out_stride, int32_t *error_flag,
                                 cudaStream_t stream);
 }
 
@@ -48,6 +48,6 @@ extern "C" int pkv_prefill_attention(const void *pool, int32_t num_blocks, int32
         out_stride % 8 || query_stride < row || out_stride < row) {
         return pkv::fail(PKV_VALUE_ERROR, "prefill attention: misaligned tensor");
     }
-    return pkv::launch_prefill_attention_tc(pool, num_blocks, layer, query, false, query_stride, blocks, start,
-                                            tokens, out, out_stride, error_flag, static_cast<cudaStream_t>(stream));
+    return pkv::launch_prefill_attention_tc(pool, num_blocks, layer, query, false, false, query_stride, blocks,
+                                            start, tokens, out, out_stride, error_flag, static_cast<cudaStream_t>(stream));
 }

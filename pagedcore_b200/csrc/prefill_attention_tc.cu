@@ -55,10 +55,10 @@
 //
 // An FP32 query (SPLIT_Q; the 8-bit cache's rotated query) becomes two Q tiles, its FP16
 // value and what that leaves, and S takes both: four more MMAs a step, mostly hidden behind
-// the softmax (2047 tokens with their read: 43.4 us, with an FP16 query 41.0).  P stays one
-// FP16 number, a rounding of the output's own size: relative error 2.6e-4 to 2.9e-4 against
-// 2.0e-4 with nothing but the output rounded, 3.5e-4 to 4.2e-4 with the query rounded too.
-// (P as two FP16 numbers in a buffer's two halves and as many MMAs again: 52 us.)
+// the softmax.  Over the 8-bit cache (FINE) so does P: what the FP16 weights leave goes over
+// the second 32 columns of S_g's buffer, and P.V takes both, so that the output's own
+// rounding is the only one to FP16.  (One FP16 number for each weight was off by as much
+// again: relative error 2.9e-4 where the output's rounding alone gives 2.0e-4.)
 //
 // Block ids outside the pool set PKV_DEVICE_BAD_BLOCK and read as zeros.
 // Every wait is bounded: on a timeout the thread sets
@@ -264,7 +264,7 @@ __device__ __forceinline__ void load_q(uint32_t q_smem, const TcArgs &a, const I
 
 // At most 120 registers a thread: two CTAs of 256 threads then fit an SM
 // (the occupancy calculation gives one CTA at 125).
-template <bool SPLIT_Q>
+template <bool SPLIT_Q, bool FINE>
 __global__ void __maxnreg__(120)
     prefill_tc_kernel(const TcArgs a) {
     extern __shared__ uint8_t dyn_smem[];
@@ -312,7 +312,7 @@ __global__ void __maxnreg__(120)
         abort_flag = 0;
         pkv::fence_barrier_init();
     }
-    if constexpr (SPLIT_Q) pkv::pdl_wait();  // a programmatic dependent of the read that fills its pool
+    if constexpr (FINE) pkv::pdl_wait();  // a programmatic dependent of the read that fills its pool
     // Every item reads the same block table (the chunk's request).
     for (int j = threadIdx.x; j <= (written - 1) / kBlockTokens; j += kThreads) table[j] = a.blocks[j];
     pkv::tc::fence_before_sync();
@@ -471,6 +471,9 @@ __global__ void __maxnreg__(120)
                         // before it published P_g).
                         pkv::tc::mma_f16_ts(tmem + kTmemO, p_tmem + 8 * kb, v_desc + 128 * kb, kIdescO,
                                             j > 0 || kb > 0);
+                        if constexpr (FINE) {  // what the FP16 weights left
+                            pkv::tc::mma_f16_ts(tmem + kTmemO, p_tmem + kStepKeys / 2 + 8 * kb, v_desc + 128 * kb, kIdescO, true);
+                        }
                     }
                     pkv::tc::commit(bar_addr(bars.pv_done[g % kSBuffers]));
                     pkv::tc::commit(bar_addr(bars.v_empty[st]));
@@ -562,7 +565,7 @@ __global__ void __maxnreg__(120)
                 uint64_t l4[4] = {0, 0, 0, 0};  // FP32 pairs: 8 independent chains
 #pragma unroll
                 for (int half = 0; half < 2; ++half) {
-                    uint32_t pr[16];
+                    uint32_t pr[16], rest[16];
 #pragma unroll
                     for (int c = 0; c < 16; ++c) {
                         const int k = 32 * half + 2 * c;
@@ -570,9 +573,15 @@ __global__ void __maxnreg__(120)
                         const float lo = pkv::exp2_approx(x.x);
                         const float hi = pkv::exp2_approx(x.y);
                         l4[c & 3] = pkv::add_f32x2(l4[c & 3], pkv::f32x2(lo, hi));
-                        pr[c] = pack2(lo, hi);
+                        const __half2 p = __floats2half2_rn(lo, hi);
+                        pr[c] = pkv::pack_half2(p);
+                        if constexpr (FINE) {
+                            const float2 f = __half22float2(p);
+                            rest[c] = pack2(lo - f.x, hi - f.y);
+                        }
                     }
                     pkv::tc::tmem_st16(sbuf + 16 * half, pr);
+                    if constexpr (FINE) pkv::tc::tmem_st16(sbuf + kStepKeys / 2 + 16 * half, rest);
                 }
                 float l8[8];
 #pragma unroll
@@ -661,18 +670,18 @@ constexpr int kCtasPerSm = 2;
 
 // Per device, once: the kernel's dynamic shared-memory limit raised, and the
 // number of its CTAs that run at once (2 per SM) recorded in *ctas.
-template <bool SPLIT_Q>
+template <bool SPLIT_Q, bool FINE>
 int prepare(int device, int *ctas) {
     static std::atomic<int> resident[kMaxDevices] = {};
     if (device >= 0 && device < kMaxDevices) {
         *ctas = resident[device].load(std::memory_order_acquire);
         if (*ctas > 0) return PKV_OK;
     }
-    cudaError_t e = cudaFuncSetAttribute(prefill_tc_kernel<SPLIT_Q>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+    cudaError_t e = cudaFuncSetAttribute(prefill_tc_kernel<SPLIT_Q, FINE>, cudaFuncAttributeMaxDynamicSharedMemorySize,
                                          kSmemBytes<SPLIT_Q>);
     if (e == cudaSuccess) {
         // All of the SM's unified L1/shared memory as shared memory: two CTAs' worth.
-        e = cudaFuncSetAttribute(prefill_tc_kernel<SPLIT_Q>, cudaFuncAttributePreferredSharedMemoryCarveout,
+        e = cudaFuncSetAttribute(prefill_tc_kernel<SPLIT_Q, FINE>, cudaFuncAttributePreferredSharedMemoryCarveout,
                                  cudaSharedmemCarveoutMaxShared);
     }
     if (e != cudaSuccess) {
@@ -693,21 +702,21 @@ int prepare(int device, int *ctas) {
     return PKV_OK;
 }
 
-template <bool SPLIT_Q>
+template <bool SPLIT_Q, bool FINE>
 int launch(const TcArgs &args, cudaStream_t stream) {
     int device = 0;
     cudaError_t e = cudaGetDevice(&device);
     if (e != cudaSuccess) return pkv::fail(PKV_CUDA_ERROR, std::string("cudaGetDevice: ") + cudaGetErrorString(e));
     int resident = 0;
-    const int rc = prepare<SPLIT_Q>(device, &resident);
+    const int rc = prepare<SPLIT_Q, FINE>(device, &resident);
     if (rc) return rc;
     // One CTA per resident slot at most; each walks its share of the items.
     const int items = (args.tokens + kTileTokens - 1) / kTileTokens * kKvHeads;
-    if constexpr (SPLIT_Q) {
-        e = pkv::launch_pdl_smem(prefill_tc_kernel<true>, dim3(std::min(items, resident)), dim3(kThreads), kSmemBytes<true>,
-                                 stream, args);
+    if constexpr (FINE) {
+        e = pkv::launch_pdl_smem(prefill_tc_kernel<SPLIT_Q, FINE>, dim3(std::min(items, resident)), dim3(kThreads),
+                                 kSmemBytes<SPLIT_Q>, stream, args);
     } else {
-        prefill_tc_kernel<false><<<std::min(items, resident), kThreads, kSmemBytes<false>, stream>>>(args);
+        prefill_tc_kernel<SPLIT_Q, FINE><<<std::min(items, resident), kThreads, kSmemBytes<SPLIT_Q>, stream>>>(args);
         e = cudaGetLastError();
     }
     if (e != cudaSuccess) {
@@ -721,9 +730,10 @@ int launch(const TcArgs &args, cudaStream_t stream) {
 namespace pkv {
 
 // Launch of the tcgen05 prefill attention (arguments checked by the caller); the query FP16
-// or, with query_fp32, FP32.
+// or, with query_fp32, FP32.  fine: over the 8-bit cache's values, behind the kernel that
+// reads them, with weights that are not rounded to FP16 (query_fp32 needs it).
 int launch_prefill_attention_tc(const void *pool, int32_t num_blocks, int32_t layer, const void *query,
-                                bool query_fp32, int64_t query_stride, const int32_t *blocks, int32_t start,
+                                bool query_fp32, bool fine, int64_t query_stride, const int32_t *blocks, int32_t start,
                                 int32_t tokens, void *out, int64_t out_stride, int32_t *error_flag,
                                 cudaStream_t stream) {
     TcArgs args;
@@ -739,7 +749,8 @@ int launch_prefill_attention_tc(const void *pool, int32_t num_blocks, int32_t la
     args.start = start;
     args.tokens = tokens;
     args.error_flag = error_flag;
-    return query_fp32 ? launch<true>(args, stream) : launch<false>(args, stream);
+    if (query_fp32) return launch<true, true>(args, stream);
+    return fine ? launch<false, true>(args, stream) : launch<false, false>(args, stream);
 }
 
 }  // namespace pkv
