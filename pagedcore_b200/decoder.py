@@ -250,8 +250,9 @@ class BatchedDecoder:
         with allocator.prefill_append(request_id, tokens) as chunk:
 
             def attend(index: int, query: Tensor, key: Tensor, value: Tensor) -> Tensor:
-                # Q is rotated in place inside the fused projection's output.
-                return chunk.attend(index, chunk.write_layer(index, key, value, query, in_place=True))
+                # FP16 queries are rotated in place inside the fused projection's output.
+                in_place = allocator.prompt_query_dtype == torch.float16
+                return chunk.attend(index, chunk.write_layer(index, key, value, query, in_place=in_place))
 
             logits = self.forward(input_ids.view(tokens, 1), attend)
         return logits.view(1, tokens, -1)

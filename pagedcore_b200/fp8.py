@@ -384,8 +384,8 @@ def append_kv(
 
     With ``rope_table`` K is rotated at ``positions`` first, and ``query``
     [layers, tokens, 32, 64] is returned rotated: in FP32, unrounded, for
-    ``prefill_attention``, or in FP16 in ``query_out`` when that is given
-    (which may be ``query`` itself).  The tokens of one block must be
+    ``prefill_attention``, or in ``query_out``, FP16 (which may be ``query``
+    itself) or FP32.  The tokens of one block must be
     consecutive, in the list and in the block, as a request's positions are.
     """
     index = cache.key_codes.get_device()
@@ -417,9 +417,9 @@ def append_kv(
             or (tokens > 1 and query_out.stride(1) < _ROW)
             or (layers > 1 and query_out.stride(0) < _ROW)
         ):
-            raise ValueError("query_out must be FP16 [layers, tokens, 32, 64] with contiguous, 16-byte aligned rows")
-        else:
-            _half("query_out", query_out, index)
+            raise ValueError("query_out must be [layers, tokens, 32, 64] with contiguous, 16-byte aligned rows")
+        elif query_out.dtype not in (_HALF, _FLOAT) or query_out.get_device() != index:
+            raise ValueError(f"query_out must be FP16 or FP32 on cuda:{index}")
         if not _rows_ok(query, query.stride()):
             query = query.contiguous()
         q_ptr, out_ptr = query.data_ptr(), query_out.data_ptr()

@@ -190,6 +190,7 @@ class PrefillAppend:
     def write_layer(self, layer: int, key: Tensor, value: Tensor, query: Tensor, *, in_place: bool = False) -> Tensor:
         """Rotate K and write K/V [T, 4, 64] at `layer`; return Q [T, 32, 64] rotated.
 
+        The rotated Q has the allocator's ``prompt_query_dtype``.
         ``in_place=True`` rotates ``query`` itself (its [32, 64] rows must be
         contiguous; the token stride may be anything, e.g. a view of a fused
         Q/K/V projection) and returns it.
@@ -204,7 +205,9 @@ class PrefillAppend:
                 raise ValueError("in-place rotation needs query rows of contiguous [32, 64] heads")
             rotated = query_in
         else:
-            rotated = torch.empty((1, self.tokens, 32, 64), dtype=torch.float16, device=allocator._pool.device)
+            rotated = torch.empty(
+                (1, self.tokens, 32, 64), dtype=allocator.prompt_query_dtype, device=allocator._pool.device
+            )
         allocator._write(
             key.reshape(1, self.tokens, 4, 64), value.reshape(1, self.tokens, 4, 64), self.slots, layer,
             positions=self.positions, query_in=query_in, query_out=rotated,
@@ -279,6 +282,8 @@ class KVAllocator:
     Construct and use on the model worker thread; CUDA work stays on the
     stream current at construction.  Block reads borrow pool storage.
     """
+
+    prompt_query_dtype = torch.float16  # of the rotated prompt queries that its attention takes
 
     def __init__(self, pool: Tensor, *, validation: str = "full", balance: str = "rows") -> None:
         if (

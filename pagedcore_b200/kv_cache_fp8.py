@@ -7,7 +7,8 @@ traffic of a decode step.  The decoder functions, the step graphs and the
 scheduler take it in place of a ``KVAllocator``.
 
 What differs: K and V are rounded to E4M3 with a scale per block of 16 tokens
-and head (K rotated in FP32 and rounded once), ``read_block`` and
+and head (K rotated in FP32 and rounded once), a prompt chunk's rotated queries
+are FP32 (``prompt_query_dtype``) unless rotated in place, ``read_block`` and
 ``iter_layer_blocks`` return FP16 copies of what is stored instead of views,
 and a token that raises its block's scale may round the block's earlier codes
 again (an aborted step leaves a scale that it raised).
@@ -50,6 +51,8 @@ def allocate_fp8_kv_pool(config: PagedCoreConfig, *, device: str | torch.device 
 class Fp8KVAllocator(KVAllocator):
     """Assign blocks within an 8-bit cache of 22 layers."""
 
+    prompt_query_dtype = torch.float32  # rotated in FP32 and not rounded
+
     def __init__(self, pool: fp8.Fp8Cache, *, validation: str = "full") -> None:
         if not isinstance(pool, fp8.Fp8Cache) or pool.layers != _LAYERS:
             raise ValueError("KV pool must be an 8-bit cache of 22 layers")
@@ -69,8 +72,10 @@ class Fp8KVAllocator(KVAllocator):
         return fp8.prefill_attention(self._pool, layer, query, blocks, start, self._error, out)
 
     def attend(self, batch: DecodeBatch, query: Tensor, *, layer_index: int, out: Tensor | None = None) -> Tensor:
-        """Decode attention of FP16 query [B, 32, 64] over a :class:`DecodeBatch`."""
+        """Decode attention of FP16 query [B, 32, 64] over a :class:`DecodeBatch` (FP32 is rounded first)."""
         self._check_worker()
+        if query.dtype == torch.float32:
+            query = query.half()
         return fp8.decode_attention(
             self._pool, layer_index, query, batch.lengths, batch.prefix, batch.flat, batch.total_blocks, self._error,
             out,
