@@ -467,6 +467,15 @@ def _attention_rows(name: str, tensor: Tensor, shape: tuple[int, ...], index: in
         raise ValueError(f"{name} must be FP16 {list(shape)} on cuda:{index}")
 
 
+def _query_rows(query: Tensor) -> tuple[Tensor, int]:
+    """Query [rows, 32, 64] as the kernels take it (a copy where it is not), and its row stride."""
+    strides = query.stride()
+    if not _rows_ok(query, strides) or strides[0] < _ROW:
+        query = query.contiguous()
+        strides = query.stride()
+    return query, max(strides[0], _ROW)  # of one row it may be anything
+
+
 def _query_and_out(
     query: Tensor, out: Tensor | None, index: int, rows: str, fp32: bool = False
 ) -> tuple[Tensor, int, Tensor, int]:
@@ -476,11 +485,7 @@ def _query_and_out(
         raise ValueError(f"query must be FP16 [{rows}, 32, 64] of a nonempty {rows}")
     if not (fp32 and query.dtype is _FLOAT and query.get_device() == index):
         _half("query", query, index)
-    strides = query.stride()
-    if not _rows_ok(query, strides) or strides[0] < _ROW:
-        query = query.contiguous()
-        strides = query.stride()
-    stride = max(strides[0], _ROW)  # of one row it may be anything
+    query, stride = _query_rows(query)
     if out is None:
         return query, stride, torch.empty_like(query, dtype=_HALF, memory_format=torch.contiguous_format), _ROW
     _attention_rows("out", out, shape, index)

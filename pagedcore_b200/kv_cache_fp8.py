@@ -103,11 +103,13 @@ class Fp8KVAllocator(KVAllocator):
         flags: int, stream: int,
     ) -> None:
         cache, rope, lengths, prefix, flat, capacity, grid, workspace, workspace_bytes, error = fixed
+        out_stride = fp8._row_stride("out", out, 32 * 64)
+        query, query_stride = fp8._query_rows(query)
         check(
             lib.pkv_fp8_decode_layer(
-                *cache, layer, query.data_ptr(), max(query.stride(0), 32 * 64), key.data_ptr(), value.data_ptr(), key.stride(0),
-                rope, lengths, prefix, flat, rows, capacity, grid, out.data_ptr(), max(out.stride(0), 32 * 64), workspace,
-                workspace_bytes, error, stream,
+                *cache, layer, query.data_ptr(), query_stride, key.data_ptr(), value.data_ptr(), key.stride(0), rope,
+                lengths, prefix, flat, rows, capacity, grid, out.data_ptr(), out_stride, workspace, workspace_bytes,
+                error, stream,
             )
         )
 

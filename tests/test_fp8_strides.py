@@ -1,0 +1,100 @@
+"""Strides of the 8-bit allocator's decode calls: what reaches the kernels, and the results."""
+
+from __future__ import annotations
+
+import pytest
+import torch
+
+from pagedcore_b200 import kv_cache_fp8
+from pagedcore_b200.kv_cache_fp8 import Fp8KVAllocator
+
+ROW = 32 * 64
+
+
+class Library:
+    """Stands in for the native library: records what a decode layer is launched with."""
+
+    def pkv_fp8_decode_layer(self, *args) -> int:
+        names = ("query", "query_stride", "key", "value", "kv_stride")
+        self.call = dict(zip(names, args[7:12])) | {"out": args[19], "out_stride": args[20]}
+        return 0
+
+
+@pytest.fixture
+def launch(monkeypatch):
+    library = Library()
+    monkeypatch.setattr(kv_cache_fp8, "lib", library)
+    allocator = Fp8KVAllocator.__new__(Fp8KVAllocator)
+    fixed = ((0, 0, 0, 0, 22, 4), 0, 0, 0, 0, 4, 1, 0, 0, 0)
+
+    def run(query, key, value, out):
+        library.call = None
+        allocator._launch_decode_layer(0, query, key, value, out, query.shape[0], fixed, 0, 0)
+        return library.call
+
+    return run
+
+
+def half(*shape: int) -> torch.Tensor:
+    return torch.zeros(shape, dtype=torch.float16)
+
+
+def test_rows_as_they_are_reach_the_kernels_as_they_are(launch) -> None:
+    wide, out = half(4, 40, 64), half(4, 48, 64)
+    call = launch(wide[:, :32], wide[:, 32:36], wide[:, 36:], out[:, 8:40])
+    assert call == {"query": wide.data_ptr(), "query_stride": 2560, "key": wide[:, 32:].data_ptr(),
+                    "value": wide[:, 36:].data_ptr(), "kv_stride": 2560, "out": out[:, 8:].data_ptr(),
+                    "out_stride": 48 * 64}
+    one = half(8 * ROW).as_strided((1, 32, 64), (64, 64, 1))  # one row: any stride
+    call = launch(one, half(1, 4, 64), half(1, 4, 64), one.clone())
+    assert call["query"] == one.data_ptr() and call["query_stride"] == call["out_stride"] == ROW
+
+
+@pytest.mark.parametrize("query", [
+    half(1, 32, 64).expand(4, 32, 64),
+    half(8 * ROW).as_strided((4, 32, 64), (64, 64, 1)),
+    half(8 * ROW).as_strided((4, 32, 64), (ROW + 2, 64, 1)),
+], ids=["broadcast", "overlapping", "odd-stride"])
+def test_a_query_that_the_kernels_cannot_take_is_copied(launch, query) -> None:
+    call = launch(query, half(4, 4, 64), half(4, 4, 64), half(4, 32, 64))
+    assert call["query"] != query.data_ptr() and call["query"] % 16 == 0 and call["query_stride"] == ROW
+
+
+@pytest.mark.parametrize("out", [half(1, 32, 64).expand(4, 32, 64), half(8 * ROW).as_strided((4, 32, 64), (64, 64, 1))],
+                         ids=["broadcast", "overlapping"])
+def test_outputs_whose_rows_overlap_are_refused(launch, out) -> None:
+    with pytest.raises(ValueError, match="overlap"):
+        launch(half(4, 32, 64), half(4, 4, 64), half(4, 4, 64), out)
+
+
+@pytest.mark.gpu
+def test_a_decode_layer_and_attention_of_any_strides_give_the_same() -> None:
+    from tests.test_fp8_decoder_gpu import admit, make_allocator
+    from tests.test_fp8_gpu import randn
+
+    def step(shape):
+        allocator = make_allocator(20)
+        requests = admit(allocator, 3, 4, 3)
+        for i, (request, n) in enumerate(zip(requests, (20, 33, 16))):
+            allocator.append(request, randn(400 + i, 22, n, 4, 64).half(), randn(410 + i, 22, n, 4, 64).half(), rotate=True)
+        outs = []
+        with allocator.append_decode(requests):
+            for layer in range(22):
+                q = randn(420 + layer, 1, 32, 64).half().expand(3, 32, 64)
+                k, v = (randn(450 + layer + 30 * i, 3, 4, 64).half() for i in range(2))
+                arguments, out = shape(q, k, v)
+                result = allocator.decode_layer(layer, *arguments, out=out)
+                assert out is None or result is out
+                outs.append(result.clone())
+        batch = allocator.decode_batch(requests, layer_index=7)
+        query, out = shape(q, k, v)[0][0], shape(q, k, v)[1]
+        outs.append(allocator.attend(batch, query, layer_index=7, out=out).clone())
+        allocator.check_device_errors()
+        return outs
+
+    expected = step(lambda q, k, v: ((q.contiguous(), k, v), None))
+    shapes = {
+        "broadcast": lambda q, k, v: ((q, k, v), None),
+    }
+    for name, shape in shapes.items():
+        assert all(torch.equal(a, b) for a, b in zip(step(shape), expected)), name
