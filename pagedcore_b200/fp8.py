@@ -358,13 +358,29 @@ def _rows_ok(tensor: Tensor, strides: tuple[int, ...]) -> bool:
     )
 
 
+def _dense(tensor: Tensor) -> Tensor:
+    """A copy in contiguous, 16-byte aligned storage (``contiguous()`` keeps an unaligned tensor)."""
+    return tensor.clone(memory_format=torch.contiguous_format)
+
+
 def _aligned_pair(key: Tensor, value: Tensor) -> tuple[Tensor, Tensor, tuple[int, ...]]:
     """K and V with common strides that the kernels take (copies where they are not), and those strides."""
     strides = key.stride()
     if not (value.stride() == strides and _rows_ok(key, strides) and value.data_ptr() % 16 == 0):
-        key, value = key.contiguous(), value.contiguous()
+        key, value = _dense(key), _dense(value)
         strides = key.stride()
     return key, value, strides
+
+
+def _query_rows(query: Tensor) -> tuple[Tensor, int]:
+    """Query [rows, 32, 64] as the kernels take it (a copy where it is not), and its row stride."""
+    strides = query.stride()
+    if strides[1:] == (_HEAD_DIM, 1) and query.data_ptr() % 16 == 0:
+        if query.shape[0] == 1:
+            return query, _ROW  # of one row the stride may be anything
+        if strides[0] >= _ROW and strides[0] % 8 == 0:
+            return query, strides[0]
+    return _dense(query), _ROW
 
 
 def append_kv(
@@ -421,7 +437,7 @@ def append_kv(
         elif query_out.dtype not in (_HALF, _FLOAT) or query_out.get_device() != index:
             raise ValueError(f"query_out must be FP16 or FP32 on cuda:{index}")
         if not _rows_ok(query, query.stride()):
-            query = query.contiguous()
+            query = _dense(query)
         q_ptr, out_ptr = query.data_ptr(), query_out.data_ptr()
         q_strides, out_strides = query.stride()[:2], query_out.stride()[:2]
     if layers == 0 or tokens == 0:
@@ -465,15 +481,6 @@ def decode_workspace_bytes(batch: int, grid: int) -> int:
 def _attention_rows(name: str, tensor: Tensor, shape: tuple[int, ...], index: int) -> None:
     if tensor.shape != shape or tensor.dtype is not _HALF or tensor.get_device() != index:
         raise ValueError(f"{name} must be FP16 {list(shape)} on cuda:{index}")
-
-
-def _query_rows(query: Tensor) -> tuple[Tensor, int]:
-    """Query [rows, 32, 64] as the kernels take it (a copy where it is not), and its row stride."""
-    strides = query.stride()
-    if not _rows_ok(query, strides) or strides[0] < _ROW:
-        query = query.contiguous()
-        strides = query.stride()
-    return query, max(strides[0], _ROW)  # of one row it may be anything
 
 
 def _query_and_out(

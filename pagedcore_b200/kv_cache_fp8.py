@@ -76,10 +76,24 @@ class Fp8KVAllocator(KVAllocator):
         self._check_worker()
         if query.dtype == torch.float32:
             query = query.half()
-        return fp8.decode_attention(
+        to = self._aligned_out(out)
+        result = fp8.decode_attention(
             self._pool, layer_index, query, batch.lengths, batch.prefix, batch.flat, batch.total_blocks, self._error,
-            out,
+            to,
         )
+        return result if to is out else out.copy_(result)
+
+    @staticmethod
+    def _aligned_out(out: Tensor | None) -> Tensor | None:
+        """``out`` [rows, 32, 64], or rows to copy to it where its own are not what the kernels write."""
+        if out is None:
+            return None
+        if out.ndim != 3 or out.dtype != torch.float16 or out.stride()[1:] != (64, 1):
+            raise ValueError("out must be FP16 [batch, 32, 64] with contiguous rows")
+        fp8._row_stride("out", out, 32 * 64)
+        if fp8._rows_ok(out, out.stride()):
+            return out
+        return torch.empty_like(out, memory_format=torch.contiguous_format)
 
     def _decode_layer_args(self, batch: DecodeBatch, rows: int, grid: int) -> tuple:
         grid = fp8.decode_plan(self._pool.device.index, rows, batch.total_blocks)[0]
@@ -103,15 +117,18 @@ class Fp8KVAllocator(KVAllocator):
         flags: int, stream: int,
     ) -> None:
         cache, rope, lengths, prefix, flat, capacity, grid, workspace, workspace_bytes, error = fixed
-        out_stride = fp8._row_stride("out", out, 32 * 64)
         query, query_stride = fp8._query_rows(query)
+        key, value, strides = fp8._aligned_pair(key, value)
+        to = self._aligned_out(out)
         check(
             lib.pkv_fp8_decode_layer(
-                *cache, layer, query.data_ptr(), query_stride, key.data_ptr(), value.data_ptr(), key.stride(0), rope,
-                lengths, prefix, flat, rows, capacity, grid, out.data_ptr(), out_stride, workspace, workspace_bytes,
-                error, stream,
+                *cache, layer, query.data_ptr(), query_stride, key.data_ptr(), value.data_ptr(), strides[0], rope,
+                lengths, prefix, flat, rows, capacity, grid, to.data_ptr(), fp8._row_stride("out", to, 32 * 64),
+                workspace, workspace_bytes, error, stream,
             )
         )
+        if to is not out:
+            out.copy_(to)
 
     # -- reading back ----------------------------------------------------------------
     @torch.inference_mode()

@@ -1,11 +1,11 @@
-"""Strides of the 8-bit allocator's decode calls: what reaches the kernels, and the results."""
+"""Strides and alignments of the 8-bit allocator's decode calls: what reaches the kernels, and the results."""
 
 from __future__ import annotations
 
 import pytest
 import torch
 
-from pagedcore_b200 import kv_cache_fp8
+from pagedcore_b200 import fp8, kv_cache_fp8
 from pagedcore_b200.kv_cache_fp8 import Fp8KVAllocator
 
 ROW = 32 * 64
@@ -45,7 +45,7 @@ def test_rows_as_they_are_reach_the_kernels_as_they_are(launch) -> None:
     assert call == {"query": wide.data_ptr(), "query_stride": 2560, "key": wide[:, 32:].data_ptr(),
                     "value": wide[:, 36:].data_ptr(), "kv_stride": 2560, "out": out[:, 8:].data_ptr(),
                     "out_stride": 48 * 64}
-    one = half(8 * ROW).as_strided((1, 32, 64), (64, 64, 1))  # one row: any stride
+    one = half(1, ROW).expand(3, ROW)[:1].view(1, 32, 64)  # one row: any stride
     call = launch(one, half(1, 4, 64), half(1, 4, 64), one.clone())
     assert call["query"] == one.data_ptr() and call["query_stride"] == call["out_stride"] == ROW
 
@@ -54,10 +54,21 @@ def test_rows_as_they_are_reach_the_kernels_as_they_are(launch) -> None:
     half(1, 32, 64).expand(4, 32, 64),
     half(8 * ROW).as_strided((4, 32, 64), (64, 64, 1)),
     half(8 * ROW).as_strided((4, 32, 64), (ROW + 2, 64, 1)),
-], ids=["broadcast", "overlapping", "odd-stride"])
+    half(8 * ROW)[2 : 2 + 4 * ROW].view(4, 32, 64),
+], ids=["broadcast", "overlapping", "odd-stride", "unaligned"])
 def test_a_query_that_the_kernels_cannot_take_is_copied(launch, query) -> None:
     call = launch(query, half(4, 4, 64), half(4, 4, 64), half(4, 32, 64))
     assert call["query"] != query.data_ptr() and call["query"] % 16 == 0 and call["query_stride"] == ROW
+
+
+def test_unaligned_keys_values_and_outputs_are_copied(launch) -> None:
+    base = half(8 * ROW)
+    kv = base[2 : 2 + 1024].view(4, 4, 64)
+    for out in (base[2 : 2 + 4 * ROW].view(4, 32, 64), base.as_strided((3, 32, 64), (ROW + 2, 64, 1))):
+        rows = out.shape[0]
+        call = launch(half(rows, 32, 64), kv[:rows], kv[:rows], out)
+        assert call["key"] % 16 == 0 and call["value"] % 16 == 0 and call["kv_stride"] == 256
+        assert call["out"] % 16 == 0 and call["out"] != out.data_ptr() and call["out_stride"] == ROW
 
 
 @pytest.mark.parametrize("out", [half(1, 32, 64).expand(4, 32, 64), half(8 * ROW).as_strided((4, 32, 64), (64, 64, 1))],
@@ -92,9 +103,35 @@ def test_a_decode_layer_and_attention_of_any_strides_give_the_same() -> None:
         allocator.check_device_errors()
         return outs
 
+    def unaligned(tensor, gap):
+        """The tensor's values in rows `gap` more than contiguous ones apart, two values off alignment."""
+        rows, width = tensor.shape[0], tensor[0].numel()
+        base = torch.full((rows * (width + gap) + 8,), 7.0, dtype=torch.float16, device=tensor.device)
+        view = base.as_strided(tensor.shape, (width + gap, 64, 1), 2)
+        return view.copy_(tensor)
+
     expected = step(lambda q, k, v: ((q.contiguous(), k, v), None))
     shapes = {
         "broadcast": lambda q, k, v: ((q, k, v), None),
+        "unaligned": lambda q, k, v: ((unaligned(q, 0), unaligned(k, 0), unaligned(v, 0)), unaligned(torch.zeros_like(q), 0)),
+        "odd": lambda q, k, v: ((unaligned(q, 2), unaligned(k, 2), unaligned(v, 2)), unaligned(torch.zeros_like(q), 2)),
+        "kv": lambda q, k, v: ((q, unaligned(k, 6), v), None),
     }
     for name, shape in shapes.items():
         assert all(torch.equal(a, b) for a, b in zip(step(shape), expected)), name
+
+
+@pytest.mark.gpu
+def test_operators_copy_what_is_contiguous_but_not_aligned() -> None:
+    from tests.test_fp8_gpu import LAYER, CacheCase, randn
+
+    case = CacheCase(141, [40, 20])
+    lengths, prefix, flat, total = case.batch()
+    query = randn(142, 2, 32, 64).half()
+    moved = torch.zeros(2 * ROW + 8, dtype=torch.float16, device=query.device)[4 : 4 + 2 * ROW].view(2, 32, 64).copy_(query)
+    assert moved.is_contiguous() and moved.data_ptr() % 16
+    expected = fp8.decode_attention(case.cache, LAYER, query, lengths, prefix, flat, total, case.flag)
+    assert torch.equal(fp8.decode_attention(case.cache, LAYER, moved, lengths, prefix, flat, total, case.flag), expected)
+    expected = fp8.prefill_attention(case.cache, LAYER, query, flat, 20, case.flag)
+    assert torch.equal(fp8.prefill_attention(case.cache, LAYER, moved, flat, 20, case.flag), expected)
+    assert int(case.flag.item()) == 0
