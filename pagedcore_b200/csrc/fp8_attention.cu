@@ -168,6 +168,13 @@ __device__ __forceinline__ int total_blocks(const Args &a) {
     return 0;
 }
 
+// Whether row `row` breaks the order of the list: it begins at block 0 and no row ends
+// before it begins.  Such a list is reported, and no partial is written where the plan has
+// no room for one.
+__device__ __forceinline__ bool out_of_order(int row, int first, int last) {
+    return last < first || (row == 0 && first != 0);
+}
+
 // Pieces of a list of `total` blocks: at most one per CTA and per chunk, so
 // none is empty.  (A captured launch has a CTA for every resident slot.)
 __host__ __device__ __forceinline__ int pieces_of(int total, int grid) {
@@ -333,9 +340,11 @@ __global__ void __launch_bounds__(kThreads, 3) fp8_decode_kernel(const __grid_co
     int sample = lane * step < a.batch ? a.prefix[min((lane + 1) * step, a.batch)] : INT32_MAX;
     const int total = total_blocks(a);
     const int pieces = pieces_of(total, a.grid);
-    // Rows without blocks: zeros.
-    for (int b = blockIdx.x * kThreads + threadIdx.x; a.clear && b < a.batch; b += a.grid * kThreads) {
-        if (a.prefix[b + 1] <= a.prefix[b]) {
+    // Rows without blocks: zeros.  (The merge looks at the rows' order too, where there is one.)
+    for (int b = blockIdx.x * kThreads + threadIdx.x; (a.clear || a.grid == 1) && b < a.batch; b += a.grid * kThreads) {
+        const int first = a.prefix[b], last = a.prefix[b + 1];
+        if (out_of_order(b, first, last)) atomicOr(a.error_flag, PKV_DEVICE_BAD_BLOCK);
+        if (a.clear && last <= first) {
             for (int i = 0; i < kQueryHeads * kDim; ++i) a.out[b * a.out_stride + i] = __float2half_rn(0.f);
         }
     }
@@ -532,6 +541,8 @@ __global__ void __launch_bounds__(kThreads, 3) fp8_decode_kernel(const __grid_co
                 dst[head0 * kDim + d + 8] = __float2half_rn(l0 == 0.f ? 0.f : __fdiv_rn(o[mt][2], l0));
                 dst[(head0 + 1) * kDim + d + 8] = __float2half_rn(l1 == 0.f ? 0.f : __fdiv_rn(o[mt][3], l1));
             }
+        } else if (pieces == 1) {  // begins before the list or ends behind it
+            if (lane == 0) atomicOr(a.error_flag, PKV_DEVICE_BAD_BLOCK);
         } else {
             const int64_t index = static_cast<int64_t>(row) + blockIdx.x;
             float *po = a.part_o + index * kQueryHeads * kDim;
@@ -597,6 +608,7 @@ __global__ void __launch_bounds__(kMergeThreads) fp8_merge_kernel(const __grid_c
     if (row < a.batch) {
         const int first_block = a.prefix[row], last_block = a.prefix[row + 1] - 1;
         const int total = total_blocks(a);
+        if (lane == 0 && out_of_order(row, first_block, last_block + 1)) atomicOr(a.error_flag, PKV_DEVICE_BAD_BLOCK);
         if (last_block >= first_block && first_block >= 0 && last_block < total) {
             const int pieces = pieces_of(total, a.grid);
             first = piece_of(first_block, total, pieces);

@@ -1,0 +1,50 @@
+"""Block tables that are out of order or out of range in the 8-bit decode attention: reported, nothing else touched."""
+
+from __future__ import annotations
+
+import pytest
+import torch
+
+from pagedcore_b200 import fp8
+from pagedcore_b200._lib import DEVICE_BAD_BLOCK, check, lib
+from tests.test_fp8_gpu import LAYER, CacheCase, randn
+
+pytestmark = pytest.mark.gpu
+
+GUARD = 1 << 16  # bytes before and behind the workspace
+
+
+def guarded(size: int, device) -> torch.Tensor:
+    return torch.full((GUARD + size + GUARD,), 0x5A, dtype=torch.uint8, device=device)
+
+
+@pytest.mark.parametrize("prefix", [[0, 3, 2], [-1, 2], [1, 2], [0, -5, 2], [0, 1000000, 2], [0, 90, 40, 60],
+                                    [0, 10, 59, 58, 60], [5, 60], [-7, 30, 60], [0, 2**31 - 1, 60]], ids=str)
+@pytest.mark.parametrize("layer_call", [False, True])
+def test_rows_that_are_out_of_order_are_reported(prefix, layer_call) -> None:
+    total, batch = prefix[-1], len(prefix) - 1
+    case = CacheCase(151, [16 * 60])
+    flat = case.batch()[2][:total].contiguous()
+    lengths = torch.full((batch,), 20, dtype=torch.int32, device=case.device)
+    table = torch.tensor(prefix, dtype=torch.int32, device=case.device)
+    grid, size = fp8.decode_plan(case.device.index, batch, total)
+    assert (grid == 1) == (total == 2)
+    workspace = guarded(size, case.device)
+    out = torch.full((batch + 2, 32, 64), 3.0, dtype=torch.float16, device=case.device)
+    query, key, value = (randn(152 + heads, batch, heads, 64).half() for heads in (32, 4, 4))
+    new = (key.data_ptr(), value.data_ptr(), 256, case.rope.data_ptr()) if layer_call else ()
+    check((lib.pkv_fp8_decode_layer if layer_call else lib.pkv_fp8_decode_attention)(
+        *case.cache._args(), LAYER, query.data_ptr(), 2048, *new, lengths.data_ptr(), table.data_ptr(), flat.data_ptr(),
+        batch, total, grid, out[1:].data_ptr(), 2048, workspace[GUARD:].data_ptr(), size, case.flag.data_ptr(),
+        torch.cuda.current_stream().cuda_stream))
+    assert int(case.flag.item()) & DEVICE_BAD_BLOCK
+    assert bool((workspace[:GUARD] == 0x5A).all()) and bool((workspace[GUARD + size :] == 0x5A).all())
+    assert bool((out[0] == 3).all()) and bool((out[-1] == 3).all())
+
+
+def test_rows_in_order_are_not_reported() -> None:
+    for lengths in ([0, 5, 0, 300, 0], [0], [960], [16] * 60):
+        case = CacheCase(153, lengths)
+        query = randn(154, len(lengths), 32, 64).half()
+        case.check_attention(query, fp8.decode_attention(case.cache, LAYER, query, *case.batch(), case.flag))
+        assert int(case.flag.item()) == 0
