@@ -239,6 +239,11 @@ __device__ __forceinline__ bool wait_bounded(uint32_t bar, uint32_t parity) {
     return pkv::mbar_test_wait(bar, parity) || pkv::mbar_wait_bounded(bar, parity, kWaitPolls);
 }
 
+// What a block id outside the cache reads as: codes of zero with the smallest scale, so
+// that the block does not move the reference of the weights (the scale goes into it).
+__device__ __align__(16) const uint8_t kZeroTiles[kBlockBytes] = {};
+__device__ __align__(16) const float kLeastScales[kHeads] = {0x1p-15f, 0x1p-15f, 0x1p-15f, 0x1p-15f};
+
 // The producer warp: copies the blocks of [begin, end) chunk by chunk, a chunk
 // ending with its row.  `lo` is at most 32 rows before the piece's first; !ready:
 // rows' last blocks only after the grid before this one.
@@ -273,12 +278,9 @@ __device__ __forceinline__ void fill_ring(const Args &a, int begin, int end, int
         const int offset = at - ids_base + j;
         const int near = __shfl_sync(0xffffffffu, ids, offset & 31);
         const int far = __shfl_sync(0xffffffffu, ids_next, offset & 31);
-        int block = offset < 32 ? near : far;
-        if (j < n && (block < 0 || block >= a.cache.num_blocks)) {
-            // Reported; block 0 is read in its place (inside the cache).
-            atomicOr(a.error_flag, PKV_DEVICE_BAD_BLOCK);
-            block = 0;
-        }
+        const int block = offset < 32 ? near : far;
+        const bool bad = block < 0 || block >= a.cache.num_blocks;  // reported, and read as zeros
+        if (j < n && bad) atomicOr(a.error_flag, PKV_DEVICE_BAD_BLOCK);
         if (!ready && at + n >= row_end) {  // the row's last block
             pkv::pdl_wait();
             ready = true;
@@ -294,14 +296,14 @@ __device__ __forceinline__ void fill_ring(const Args &a, int begin, int end, int
         __syncwarp();
         if (j < n && lane < 16) {
             const int64_t tile = layer_tile + static_cast<int64_t>(block) * kHeads;
-            if (lane < 4) {
-                bulk_load(dst + j * kBlockBytes, a.cache.key_codes + tile * kTile, kBlockBytes, bar, policy);
-            } else if (lane < 8) {
-                bulk_load(dst + kValueAt + j * kValuePitch, a.cache.value_codes + tile * kTile, kBlockBytes, bar, policy);
-            } else if (lane < 12) {
-                bulk_load(dst + kScaleAt + j * 16, a.cache.key_scales + tile, 16, bar, policy);
+            if (lane < 8) {
+                const uint8_t *codes = lane < 4 ? a.cache.key_codes : a.cache.value_codes;
+                bulk_load(dst + (lane < 4 ? j * kBlockBytes : kValueAt + j * kValuePitch),
+                          bad ? kZeroTiles : codes + tile * kTile, kBlockBytes, bar, policy);
             } else {
-                bulk_load(dst + kScaleAt + (kChunk + j) * 16, a.cache.value_scales + tile, 16, bar, policy);
+                const float *scales = lane < 12 ? a.cache.key_scales : a.cache.value_scales;
+                bulk_load(dst + kScaleAt + (lane < 12 ? j : kChunk + j) * 16, bad ? kLeastScales : scales + tile, 16, bar,
+                          policy);
             }
         }
         at += n;

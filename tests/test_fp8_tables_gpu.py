@@ -7,6 +7,7 @@ import torch
 
 from pagedcore_b200 import fp8
 from pagedcore_b200._lib import DEVICE_BAD_BLOCK, check, lib
+from tests.fp8_reference import attend64, rope64
 from tests.test_fp8_gpu import LAYER, CacheCase, randn
 
 pytestmark = pytest.mark.gpu
@@ -48,3 +49,43 @@ def test_rows_in_order_are_not_reported() -> None:
         query = randn(154, len(lengths), 32, 64).half()
         case.check_attention(query, fp8.decode_attention(case.cache, LAYER, query, *case.batch(), case.flag))
         assert int(case.flag.item()) == 0
+
+
+@pytest.mark.parametrize("lengths, bad", [([40], [(0, 1)]), ([40], [(0, 0), (0, 1), (0, 2)]), ([3, 300, 17], [(1, 0), (1, 7), (2, 1)]),
+                                          ([1], [(0, 0)]), ([2048, 64], [(0, 127), (0, 64), (1, 3)]), ([130] * 9, [(4, 8), (8, 2)])],
+                         ids=lambda v: "-".join(map(str, v[:3])).replace(" ", ""))
+@pytest.mark.parametrize("layer_call", [False, True])
+def test_a_bad_block_reads_as_zeros(lengths, bad, layer_call) -> None:
+    """A block id outside the cache stands for 16 tokens of zero keys and values, whatever block 0 holds."""
+    case = CacheCase(155, lengths)
+    case.cache.key_codes.view(torch.uint8)[LAYER, 0] = 0x70  # recognisable: 128, with a scale of 4
+    case.cache.value_codes.view(torch.uint8)[LAYER, 0] = 0x70
+    case.cache.key_scales[LAYER, 0], case.cache.value_scales[LAYER, 0] = 4.0, 4.0
+    for table in case.tables:  # block 0 belongs to nobody
+        assert len(case.free) > 1
+        if 0 in table:
+            at, spare = table.index(0), case.free.pop()
+            table[at] = spare
+            for name in ("key_codes", "value_codes"):
+                getattr(case.cache, name).view(torch.uint8)[LAYER, spare] = 0
+            for name in ("key_scales", "value_scales"):
+                getattr(case.cache, name)[LAYER, spare] = 1.0
+            for oracle in (case.key, case.value):
+                oracle.values[spare] = 0.0
+    lengths_, prefix, flat, total = case.batch()
+    for index, (row, block) in enumerate(bad):
+        flat[int(prefix[row]) + block] = (-1, case.cache.num_blocks, 2**31 - 1)[index % 3]
+    query = 2 * randn(156, len(lengths), 32, 64).half()
+    if layer_call:  # the new token of a row whose last block is bad is not written
+        key, value = (randn(157 + i, len(lengths), 4, 64).half() for i in range(2))
+        out = fp8.decode_layer(case.cache, LAYER, query, key, value, case.rope, lengths_, prefix, flat, total, case.flag)
+        query = rope64(query, case.rope, lengths_.long() - 1)
+    else:
+        out = fp8.decode_attention(case.cache, LAYER, query, lengths_, prefix, flat, total, case.flag)
+    assert int(case.flag.item()) == DEVICE_BAD_BLOCK
+    for row, length in enumerate(lengths):
+        good = torch.tensor([b if (row, i) not in bad else -1 for i, b in enumerate(case.tables[row])], device=case.device)
+        read = fp8.read_blocks(case.cache, LAYER, good.int(), torch.zeros_like(case.flag))  # zeros for bad ids, too
+        k, v = (x.reshape(-1, 4, 64)[:length].double() for x in read)
+        exact, bound = attend64(query[row], k, v)
+        assert bool(((out[row].double() - exact).abs() <= bound).all()), row
