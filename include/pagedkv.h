@@ -442,6 +442,15 @@ int pkv_fp8_read_blocks(const void *key_codes, const void *value_codes, const vo
                         const int32_t *blocks, int32_t count, void *key_out, void *value_out, int32_t *error_flag,
                         void *stream);
 
+/* What undoes a step: codes and scales of the blocks of `slots` (device int32
+ * [count], the slots that the step writes first) in every layer, to `saved`
+ * (16-byte aligned, 8224 bytes for each layer and slot), or with `restore` back
+ * from it.  A slot that opens its block has nothing to keep; slots outside the
+ * cache are passed over. */
+int pkv_fp8_save_blocks(void *key_codes, void *value_codes, void *key_scales, void *value_scales, int32_t layers,
+                        int32_t num_blocks, const int32_t *slots, int32_t count, void *saved, int64_t saved_bytes,
+                        int32_t restore, void *stream);
+
 /* pkv_prefill_attention over the 8-bit cache: same arguments and result over the
  * values that the cache holds; the query FP16 or, with query_fp32, FP32 (taken
  * as it is; rows query_stride values apart).  The workspace (16-byte aligned,

@@ -127,6 +127,10 @@ SIGNATURES: dict[str, tuple[object, list[object]]] = {
         c_int,
         [*_FP8_CACHE, c_int32, c_void_p, c_int32, c_void_p, c_void_p, c_void_p, c_void_p],
     ),
+    "pkv_fp8_save_blocks": (
+        c_int,
+        [*_FP8_CACHE, c_void_p, c_int32, c_void_p, c_int64, c_int32, c_void_p],
+    ),
     "pkv_fp8_prefill_attention": (
         c_int,
         [

@@ -391,6 +391,32 @@ __global__ void __launch_bounds__(kReadThreads)
     }
 }
 
+// The open blocks of a step (those of `slots` that are not a block's first), all layers:
+// codes and scales to `saved` before the step, or back from it.  One CTA per (slot, layer),
+// 16 bytes of K and of V a thread.  256 slots of 22 layers are 46 MB each way.
+constexpr int kSavedBytes = 2 * kHeads * pkv::fp8::kTileBytes + 2 * kHeads * 4;  // K codes, V codes, K and V scales
+
+template <bool RESTORE>
+__global__ void __launch_bounds__(kReadThreads) fp8_save_kernel(const pkv::fp8::Cache cache, const int32_t *slots,
+                                                                uint8_t *saved) {
+    pkv::pdl_wait();
+    pkv::pdl_launch_dependents();
+    const int slot = slots[blockIdx.x];
+    if (slot < 0 || slot % kSlots == 0 || slot / kSlots >= cache.num_blocks) return;
+    const int64_t tile = pkv::fp8::tile_index(cache, blockIdx.y, slot / kSlots, 0);
+    uint4 *const held = reinterpret_cast<uint4 *>(saved + (static_cast<int64_t>(blockIdx.y) * gridDim.x + blockIdx.x) * kSavedBytes);
+    const auto copy = [&](void *block, int at, int i) {
+        uint4 *const stored = static_cast<uint4 *>(block);
+        if (RESTORE) stored[i] = held[at + i];
+        else held[at + i] = stored[i];
+    };
+    constexpr int kCodes = kHeads * pkv::fp8::kTileBytes / 16;  // of K or V
+    static_assert(kCodes == kReadThreads, "a thread takes 16 bytes of each");
+    copy(cache.key_codes + tile * pkv::fp8::kTileBytes, 0, threadIdx.x);
+    copy(cache.value_codes + tile * pkv::fp8::kTileBytes, kCodes, threadIdx.x);
+    if (threadIdx.x < 2) copy((threadIdx.x ? cache.value_scales : cache.key_scales) + tile, 2 * kCodes + threadIdx.x, 0);
+}
+
 pkv::fp8::Cache cache_of(const void *key_codes, const void *value_codes, const void *key_scales,
                          const void *value_scales, int32_t layers, int32_t num_blocks) {
     return {static_cast<uint8_t *>(const_cast<void *>(key_codes)), static_cast<uint8_t *>(const_cast<void *>(value_codes)),
@@ -551,6 +577,28 @@ extern "C" int pkv_fp8_read_blocks(const void *key_codes, const void *value_code
     pkv::clear_error();
     return read_blocks(key_codes, value_codes, key_scales, value_scales, layers, num_blocks, layer, blocks, count,
                        key_out, value_out, nullptr, error_flag, stream);
+}
+
+extern "C" int pkv_fp8_save_blocks(void *key_codes, void *value_codes, void *key_scales, void *value_scales,
+                                   int32_t layers, int32_t num_blocks, const int32_t *slots, int32_t count, void *saved,
+                                   int64_t saved_bytes, int32_t restore, void *stream) {
+    pkv::clear_error();
+    const int rc = pkv::fp8::check_cache(key_codes, value_codes, key_scales, value_scales, layers, num_blocks, 0, layers);
+    if (rc) return rc;
+    if (slots == nullptr || saved == nullptr || count < 0) {
+        return pkv::fail(PKV_VALUE_ERROR, "fp8 save: slots and a buffer are required");
+    }
+    if (layers > 65535) return pkv::fail(PKV_VALUE_ERROR, "fp8 save: layers out of range");
+    if (!aligned16(saved) || saved_bytes / kSavedBytes / layers < count) {
+        return pkv::fail(PKV_VALUE_ERROR, "fp8 save: the buffer must be 16-byte aligned, 8224 bytes for each layer and slot");
+    }
+    if (count == 0) return PKV_OK;
+    const cudaError_t e = pkv::launch_pdl(restore ? fp8_save_kernel<true> : fp8_save_kernel<false>, dim3(count, layers),
+                                          dim3(kReadThreads), static_cast<cudaStream_t>(stream),
+                                          cache_of(key_codes, value_codes, key_scales, value_scales, layers, num_blocks),
+                                          slots, static_cast<uint8_t *>(saved));
+    if (e != cudaSuccess) return pkv::fail(PKV_CUDA_ERROR, std::string("fp8 save launch failed: ") + cudaGetErrorString(e));
+    return PKV_OK;
 }
 
 // The request's blocks become an FP16 pool of one layer in the workspace (the values are

@@ -465,6 +465,33 @@ def read_blocks(cache: Fp8Cache, layer: int, blocks: Tensor, error_flag: Tensor)
     return key, value
 
 
+_SAVED_BYTES = 2 * _KV_HEADS * (_BLOCK_TOKENS * _HEAD_DIM + 4)  # of a block in one layer
+
+
+def save_blocks(cache: Fp8Cache, slots: Tensor) -> Tensor:
+    """What ``restore_blocks`` needs to undo writes that begin at ``slots`` (int32 [count], one a block).
+
+    A write inside a block may raise the block's scale and round its earlier
+    codes again; this keeps the blocks' codes and scales, of every layer.
+    """
+    index = cache.key_codes.get_device()
+    count = slots.numel()
+    saved = torch.empty(max(count, 1) * cache.layers * _SAVED_BYTES, dtype=torch.uint8, device=cache.device)
+    _call(index, lib.pkv_fp8_save_blocks, *cache._args(), _int_list(index, "slots", slots, count), count,
+          saved.data_ptr(), saved.numel(), 0)
+    return saved
+
+
+def restore_blocks(cache: Fp8Cache, slots: Tensor, saved: Tensor) -> None:
+    """The blocks of ``slots`` as they were when ``save_blocks`` returned ``saved``."""
+    index = cache.key_codes.get_device()
+    if saved.dtype is not torch.uint8 or saved.get_device() != index or not saved.is_contiguous():
+        raise ValueError("saved must be what save_blocks returned")
+    count = slots.numel()
+    _call(index, lib.pkv_fp8_save_blocks, *cache._args(), _int_list(index, "slots", slots, count), count,
+          saved.data_ptr(), saved.numel(), 1)
+
+
 @functools.lru_cache(maxsize=4096)
 def decode_plan(device_index: int, batch: int, total_blocks: int) -> tuple[int, int]:
     """Grid and workspace bytes of the decode attention (``pkv_fp8_decode_plan``)."""

@@ -338,6 +338,13 @@ class KVAllocator:
             rope_table=None if positions is None else self._rope, query_in=query_in, query_out=query_out,
         )
 
+    def _save_blocks(self, slots: Tensor) -> tuple | None:
+        """What a failed step that writes at ``slots`` (one a block) and on has to put back: nothing here."""
+        return None
+
+    def _restore_blocks(self, saved: tuple) -> None:
+        raise NotImplementedError
+
     def _attend_prompt(self, layer: int, query: Tensor, blocks: Tensor, start: int, out: Tensor) -> Tensor:
         return kernels.prefill_attention(self._pool, layer, query, blocks, start, out, self._error)
 
@@ -636,8 +643,15 @@ class KVAllocator:
         count = len(blocks)
         chunk = PrefillAppend(self, blocks, device[:count], device[count : count + tokens],
                               device[count + tokens :], start, tokens)
-        yield chunk
-        self._ledger.append_commit(handle, tokens)
+        saved = self._save_blocks(chunk.slots[:1]) if start % _BLOCK_TOKENS else None
+        try:
+            yield chunk
+            self._ledger.append_commit(handle, tokens)
+        except BaseException:
+            # Unless the request was released or grew by other calls meanwhile: its block is theirs.
+            if saved is not None and self._handles.get(request_id) == handle and self._ledger.length(handle) == start:
+                self._restore_blocks(saved)
+            raise
 
     @contextmanager
     def append_decode(
@@ -672,6 +686,7 @@ class KVAllocator:
             # decode layer reads; its tables travel with the slots in one copy.
             tables, total, plan = self._batch_tables(request_ids, handles, _VIEW_STAGED, layout)
             device, upload = self._uploads.upload((tables, slots, positions))
+            saved = self._save_blocks(device[len(tables) : len(tables) + count])
         except BaseException:
             self._ledger.decode_abort()
             raise
@@ -687,12 +702,17 @@ class KVAllocator:
             flat_capacity=upload.device.numel() - (4 * grid + 4 * rows + 1),
         )
         try:
-            yield
+            try:
+                yield
+            except BaseException:
+                self._ledger.decode_abort()
+                raise
+            self._ledger.decode_commit()
         except BaseException:
-            self._ledger.decode_abort()
+            if saved is not None:
+                self._restore_blocks(saved)
             raise
         else:
-            self._ledger.decode_commit()
             self._measure_slots(plan, count)
         finally:
             self._staged = None

@@ -11,7 +11,8 @@ and head (K rotated in FP32 and rounded once), a prompt chunk's rotated queries
 are FP32 (``prompt_query_dtype``) unless rotated in place, ``read_block`` and
 ``iter_layer_blocks`` return FP16 copies of what is stored instead of views,
 and a token that raises its block's scale may round the block's earlier codes
-again (an aborted step leaves a scale that it raised).
+again.  A step or prompt chunk that fails leaves the cache as it was: the open
+blocks are copied before it (8 KiB a row and layer) and put back.
 """
 
 from __future__ import annotations
@@ -129,6 +130,12 @@ class Fp8KVAllocator(KVAllocator):
         )
         if to is not out:
             out.copy_(to)
+
+    def _save_blocks(self, slots: Tensor) -> tuple[Tensor, Tensor]:
+        return slots, fp8.save_blocks(self._pool, slots)
+
+    def _restore_blocks(self, saved: tuple[Tensor, Tensor]) -> None:
+        fp8.restore_blocks(self._pool, *saved)
 
     # -- reading back ----------------------------------------------------------------
     @torch.inference_mode()
