@@ -35,7 +35,7 @@
 // w * 2^-e, in FP32.  The weights go into the MMA as two FP16 numbers, hi = fp16(w)
 // and lo = fp16(w - hi), 2^-22 of the weight together (one alone is off by 2^-11,
 // which showed in the output), and so do the queries of the decode layer, rotated
-// in FP32; scores, maxima, normaliser and sums are FP32.  The second products are
+// in FP32 and halved (two components near FP16's largest number rotate past it); scores, maxima, normaliser and sums are FP32.  The second products are
 // free: the tensor pipe was 13 % busy without them.
 
 #include <cuda_fp16.h>
@@ -91,7 +91,7 @@ struct Args {
     pkv::fp8::Cache cache;
     int32_t layer;
     const __half *query;
-    const __half *query_low;  // SPLIT_Q: what FP16 left of each query value
+    const __half *query_low;  // SPLIT_Q: query holds half of each value, this what FP16 left of it
     int64_t query_stride;
     const int32_t *lengths;
     const int32_t *prefix;
@@ -433,7 +433,7 @@ __global__ void __launch_bounds__(kThreads, 3) fp8_decode_kernel(const __grid_co
                 }
             }
             const float key_scale =
-                *reinterpret_cast<const float *>(src + kScaleAt + (g >> 1) * 16 + warp * 4) * kScaleLog2;
+                *reinterpret_cast<const float *>(src + kScaleAt + (g >> 1) * 16 + warp * 4) * (SPLIT_Q ? 2.f : 1.f) * kScaleLog2;
             const float value_scale =
                 *reinterpret_cast<const float *>(src + kScaleAt + (kChunk + (g >> 1)) * 16 + warp * 4);
             uint4 v[4][2];

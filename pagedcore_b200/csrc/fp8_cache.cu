@@ -50,7 +50,8 @@ struct AppendArgs {
     const __half *rope;  // FP16 cos [2048][32], sin [2048][32], or null
     const __half *query_in;
     __half *query_out;
-    __half *query_low;   // nullable, laid out as query_out: what FP16 left of each value
+    __half *query_low;   // nullable, laid out as query_out: then both hold halves of the values
+                         // (two FP16 components can rotate past FP16's range), and this what FP16 left of each
     float *query_out32;  // in place of query_out: the rotated queries in FP32
     int64_t q_layer_stride;
     int64_t q_token_stride;
@@ -278,8 +279,10 @@ __device__ void rotate_queries(const AppendArgs &a, int layer, int begin, int wa
             continue;
         }
         uint32_t r[4], low[4];
+        const float part = a.query_low != nullptr ? 0.5f : 1.f;
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
+            y[i].x *= part, y[i].y *= part;
             const __half2 h = __floats2half2_rn(y[i].x, y[i].y);
             const float2 f = __half22float2(h);
             r[i] = pkv::pack_half2(h);
@@ -456,7 +459,7 @@ int check_cache(const void *key_codes, const void *value_codes, const void *key_
 }
 
 // The new token of every row of a staged batch at `layer`: K rotated and V written, Q
-// rotated to query_out + query_low (FP16 numbers that add up to the FP32 value).
+// rotated to query_out + query_low (FP16 numbers that add up to half of the FP32 value).
 int launch_decode_append(const Cache &cache, int32_t layer, const void *key, const void *value, int64_t kv_stride,
                          const void *rope_table, const void *query, int64_t query_stride, void *query_out, void *query_low,
                          const int32_t *lengths, const int32_t *prefix, const int32_t *flat, int32_t batch,

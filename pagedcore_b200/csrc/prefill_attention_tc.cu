@@ -55,7 +55,8 @@
 //
 // An FP32 query (SPLIT_Q; the 8-bit cache's rotated query) becomes two Q tiles, its FP16
 // value and what that leaves, and S takes both: four more MMAs a step, mostly hidden behind
-// the softmax.  Over the 8-bit cache (FINE) so does P: what the FP16 weights leave goes over
+// the softmax.  A row is scaled by a power of two that brings its largest value to 2^14 ..
+// 2^15, whatever FP32 range it had, and the row's scores are scaled back.  Over the 8-bit cache (FINE) so does P: what the FP16 weights leave goes over
 // the second 32 columns of S_g's buffer, and P.V takes both, so that the output's own
 // rounding is the only one to FP16.  (One FP16 number for each weight was off by as much
 // again: relative error 2.9e-4 where the output's rounding alone gives 2.0e-4.)
@@ -74,6 +75,7 @@
 #include <atomic>
 #include <string>
 
+#include "fp8.cuh"
 #include "pagedkv.h"
 #include "pdl.h"
 #include "ptx.cuh"
@@ -228,17 +230,29 @@ __device__ __forceinline__ void load_q_row(uint32_t q_smem, const TcArgs &a, con
     pkv::cp_async_commit();
 }
 
-// The same from an FP32 query: two FP16 numbers that add up to each value, the high
-// halves at q_smem and the low ones a tile further.
-__device__ __forceinline__ void load_q_row_split(uint32_t q_smem, const TcArgs &a, const Item &it, int r) {
+// The same from an FP32 query: two FP16 numbers that add up to each value times 2^-e, the
+// high halves at q_smem and the low ones a tile further.  Returns 2^e.  (Few loads
+// at a time: the registers for a whole row are not there.  All at once before the first
+// step, where they are, saved 0.5 us of 70.)
+__device__ __forceinline__ float load_q_row_split(uint32_t q_smem, const TcArgs &a, const Item &it, int r) {
     const int t = min(it.t0 + (r >> 3), a.tokens - 1);
     const float4 *src = reinterpret_cast<const float4 *>(a.query32 + static_cast<int64_t>(t) * a.query_stride +
                                                          (it.kv * 8 + (r & 7)) * kHeadDim);
     const uint32_t row = q_smem + (r >> 3) * 1024 + (r & 7) * kRowBytes;
-#pragma unroll
+    float largest = 0.f;  // of the finite values
+#pragma unroll 4
+    for (int c = 0; c < 16; ++c) {
+        const float4 x = src[c];
+        largest = pkv::fp8::max_finite(pkv::fp8::max_finite(largest, x.x), x.y);
+        largest = pkv::fp8::max_finite(pkv::fp8::max_finite(largest, x.z), x.w);
+    }
+    // A row of zeros or of FP32's subnormals stays what it is (2^100 times).
+    const int e = max((__float_as_int(largest) >> 23) - 127 - 14, -100);
+    const float down = pkv::fp8::exp2_int(-e);
+#pragma unroll 2
     for (int c = 0; c < 8; ++c) {
         const float4 x = src[2 * c], y = src[2 * c + 1];
-        const float v[8] = {x.x, x.y, x.z, x.w, y.x, y.y, y.z, y.w};
+        const float v[8] = {x.x * down, x.y * down, x.z * down, x.w * down, y.x * down, y.y * down, y.z * down, y.w * down};
         uint32_t high[4], low[4];
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
@@ -251,14 +265,17 @@ __device__ __forceinline__ void load_q_row_split(uint32_t q_smem, const TcArgs &
         asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(at), "r"(high[0]), "r"(high[1]), "r"(high[2]), "r"(high[3]) : "memory");
         asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(at + kQBytes), "r"(low[0]), "r"(low[1]), "r"(low[2]), "r"(low[3]) : "memory");
     }
+    return pkv::fp8::exp2_int(e);
 }
 
+// Either, and the factor from the row's products to scores in base 2.
 template <bool SPLIT_Q>
-__device__ __forceinline__ void load_q(uint32_t q_smem, const TcArgs &a, const Item &it, int r) {
+__device__ __forceinline__ float load_q(uint32_t q_smem, const TcArgs &a, const Item &it, int r) {
     if constexpr (SPLIT_Q) {
-        load_q_row_split(q_smem, a, it, r);
+        return load_q_row_split(q_smem, a, it, r) * kScaleLog2;
     } else {
         load_q_row(q_smem, a, it, r);
+        return kScaleLog2;
     }
 }
 
@@ -493,8 +510,9 @@ __global__ void __maxnreg__(120)
         int g = 0;
         // The first item's Q tile; each later one is loaded during the last step
         // of the item before it, once every S MMA that read the tile has completed.
+        float next_scale = kScaleLog2;
         if (item_of(0, cta, ctas) < items) {
-            load_q<SPLIT_Q>(q_smem, a, item_info(item_of(0, cta, ctas), tiles, a), r);
+            next_scale = load_q<SPLIT_Q>(q_smem, a, item_info(item_of(0, cta, ctas), tiles, a), r);
             pkv::cp_async_wait<0>();
             pkv::fence_proxy_async_smem();  // generic-proxy copies -> the MMA's (async proxy) reads
             __syncwarp();
@@ -508,6 +526,7 @@ __global__ void __maxnreg__(120)
             const int t = it.t0 + (r >> 3);
             const int pos = a.start + min(t, a.tokens - 1);  // last position this row attends to
             const int head = it.kv * 8 + (r & 7);
+            const float scale = SPLIT_Q ? next_scale : kScaleLog2;
             float m = -INFINITY;  // the row maximum at its last rescale (log2 units)
             float l = 0.f;        // sum of this row's weights, relative to m
             for (int j = 0; j < it.steps; ++j, ++g) {
@@ -526,7 +545,7 @@ __global__ void __maxnreg__(120)
                 pkv::tc::tmem_wait_ld();
                 // s_full of the item's last step: every S MMA of the item has
                 // completed, so the next item's Q may replace this one's.
-                if (last && next < items) load_q<SPLIT_Q>(q_smem, a, item_info(next, tiles, a), r);
+                if (last && next < items) next_scale = load_q<SPLIT_Q>(q_smem, a, item_info(next, tiles, a), r);
 
                 float s[64];
 #pragma unroll
@@ -552,7 +571,7 @@ __global__ void __maxnreg__(120)
                 const float mx = pkv::fmax3(pkv::fmax3(mx8[0], mx8[1], mx8[2]), pkv::fmax3(mx8[3], mx8[4], mx8[5]),
                                             fmaxf(mx8[6], mx8[7]));
                 // Step 0 holds position 0, which every row attends to: m is finite from step 0 on.
-                const float m_blk = mx * kScaleLog2;
+                const float m_blk = mx * scale;
                 const float m_new = m_blk > m + kRescaleLog2 ? m_blk : m;  // m = -inf at step 0: always moves
                 // P_g as FP16 (x 2^7) over the first 32 columns of its S buffer,
                 // two keys to a column (the A operand of P.V from TMEM); l sums the
@@ -560,7 +579,7 @@ __global__ void __maxnreg__(120)
                 // Pairs of keys go through the packed FP32 instructions (the same
                 // rounding as two scalar ones, half the instructions).
                 const float shift = kWeightShift - m_new;
-                const uint64_t scale2 = pkv::f32x2(kScaleLog2, kScaleLog2);
+                const uint64_t scale2 = pkv::f32x2(scale, scale);
                 const uint64_t shift2 = pkv::f32x2(shift, shift);
                 uint64_t l4[4] = {0, 0, 0, 0};  // FP32 pairs: 8 independent chains
 #pragma unroll

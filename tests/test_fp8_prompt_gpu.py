@@ -128,3 +128,66 @@ def test_the_decoders_prompts_keep_the_rotated_query_in_fp32(kind, weights, monk
         recorded.check(allocator, (0, 11, 21))
         recorded.calls.clear()
     allocator.check_device_errors()
+
+
+
+def small_keys(seed: int, lengths: list[int], room: int = 0) -> CacheCase:
+    """A cache whose keys are 2^-14 of the usual size: queries 2^14 times as large give ordinary scores."""
+    case = CacheCase(seed, [0] * len(lengths), spare=sum(-(-(n + room) // 16) for n in lengths))
+    for row, length in enumerate(lengths):
+        case.tables[row] += [case.free.pop() for _ in range(-(-(length + room) // 16))]
+        if length:
+            case.append(row, randn(seed + 5 * row + 1, length, 4, 64) * 2.0**-14, randn(seed + 5 * row + 2, length, 4, 64), 0)
+        case.lengths[row] = length
+    return case
+
+
+@pytest.mark.parametrize("start, tokens", [(0, 33), (100, 70), (0, 2047)])
+def test_prompt_attention_takes_fp32_queries_of_any_size(start, tokens) -> None:
+    """Rows from 2^-140 to 2^24, beside one another: no range of FP16 shows."""
+    case = small_keys(133, [start + tokens])
+    size = torch.randint(-100, 25, (tokens, 1, 1), generator=torch.Generator().manual_seed(134)).to(case.device)
+    size[::2] = torch.randint(10, 20, (tokens, 1, 1), generator=torch.Generator().manual_seed(135)).to(case.device)[::2]
+    query = torch.ldexp(randn(136, tokens, 32, 64), size)
+    query[3] = 0.0
+    query[5] = torch.ldexp(randn(137, 32, 64), torch.tensor(-140, device=query.device))  # FP32 subnormals in part
+    query[7] = randn(138, 32, 64) * torch.tensor([1.0, 1e6] * 32, device=query.device)
+    out = fp8.prefill_attention(case.cache, LAYER, query, case.batch()[2], start, case.flag)
+    assert int(case.flag.item()) == 0 and bool(out.isfinite().all())
+    key, value = (oracle.tokens(case.tables[0], start + tokens) for oracle in (case.key, case.value))
+    check_prompt(out, query, key, value, start, sorted({*range(12), *range(12, tokens, max(1, tokens // 40)), tokens - 1}))
+
+
+def test_queries_that_rotate_past_fp16_stay_finite() -> None:
+    """Two components near FP16's largest number rotate to up to sqrt(2) times it."""
+    lengths = [1, 40, 17, 300]
+    case = small_keys(139, [n - 1 for n in lengths], room=1)
+    case.lengths = lengths
+    query = torch.where(randn(140, 4, 32, 64) > 0, 65504.0, -65504.0).half()
+    query[0] = randn(141, 32, 64).half() * 1000
+    key, value = randn(142, 4, 4, 64).half() * 2.0**-14, randn(143, 4, 4, 64).half()
+    exact_query = rope64(query, case.rope, torch.tensor(lengths, device=case.device) - 1)
+    assert bool((exact_query[1:].abs().amax((1, 2)) > 65520).all())
+    out = fp8.decode_layer(case.cache, LAYER, query, key, value, case.rope, *case.batch(), case.flag)
+    assert int(case.flag.item()) == 0 and bool(out.isfinite().all())
+    for row, length in enumerate(lengths):
+        blocks = torch.tensor(case.tables[row], dtype=torch.int32, device=case.device)
+        k, v = (x.reshape(-1, 4, 64)[:length].double() for x in fp8.read_blocks(case.cache, LAYER, blocks, case.flag))
+        check_prompt(out[row : row + 1], exact_query[row : row + 1], k, v, length - 1, [0])
+
+
+def test_a_prompt_that_rotates_past_fp16_stays_finite() -> None:
+    case = small_keys(144, [0], room=40)
+    query = torch.where(randn(145, 40, 32, 64) > 0, 65504.0, -65504.0).half()
+    key, value = randn(146, 40, 4, 64).half() * 2.0**-14, randn(147, 40, 4, 64).half()
+    at = torch.arange(40, device=case.device)
+    slots = torch.tensor(case.slots(0, 0, 40), dtype=torch.int32, device=case.device)
+    rotated = fp8.append_kv(case.cache, key[None], value[None], slots, layer_begin=LAYER, error_flag=case.flag,
+                            positions=at.int(), rope_table=case.rope, query=query[None])
+    blocks = torch.tensor(case.tables[0], dtype=torch.int32, device=case.device)
+    out = fp8.prefill_attention(case.cache, LAYER, rotated[0], blocks, 0, case.flag)
+    assert int(case.flag.item()) == 0 and bool(out.isfinite().all())
+    k, v = (x.reshape(-1, 4, 64)[:40].double() for x in fp8.read_blocks(case.cache, LAYER, blocks, case.flag))
+    exact_query = rope64(query, case.rope, at)
+    assert float(exact_query.abs().max()) > 65520
+    check_prompt(out, exact_query, k, v, 0, [0, 1, 17, 39])
