@@ -32,7 +32,8 @@
 // the exponent: the weight is w = 2^(s + e - M + 15) with M the running maximum
 // of s + e, so the largest contribution, not the largest probability, sits at
 // 2^15 and blocks of very different magnitude lose nothing; the normaliser adds
-// w * 2^-e, in FP32.  The weights go into the MMA as two FP16 numbers, hi = fp16(w)
+// w * 2^-e, in FP32.  (M is held as M - 15.  Past 2^20, where 15 would soon be lost in its
+// rounding and a weight pass FP16's range, as M itself.)  The weights go into the MMA as two FP16 numbers, hi = fp16(w)
 // and lo = fp16(w - hi), 2^-22 of the weight together (one alone is off by 2^-11,
 // which showed in the output), and so do the queries of the decode layer, rotated
 // in FP32 and halved (two components near FP16's largest number rotate past it); scores, maxima, normaliser and sums are FP32.  The second products are
@@ -84,6 +85,7 @@ constexpr int kSmem = kLowAt + kWarps * 32 * 32;
 constexpr uint32_t kWaitPolls = 1u << 24;
 constexpr float kScaleLog2 = 0.125f * 1.4426950408889634f;  // 64^-0.5 * log2(e)
 constexpr float kWeightShift = 15.0f;
+constexpr float kFarScore = 0x1p20f;
 constexpr float kLowest = -1e30f;  // below every finite score
 constexpr int kPartial = kQueryHeads * (kDim + 2);  // floats of a partial
 
@@ -473,21 +475,22 @@ __global__ void __launch_bounds__(kThreads, 3) fp8_decode_kernel(const __grid_co
                 top0 = fmaxf(top0, fmaxf(s[j][0], s[j][2]));
                 top1 = fmaxf(top1, fmaxf(s[j][1], s[j][3]));
             }
-            top0 = fmaxf(m0, max8(top0));
-            top1 = fmaxf(m1, max8(top1));
+            top0 = max8(top0);
+            top1 = max8(top1);
+            top0 = fmaxf(m0, fabsf(top0) > kFarScore ? top0 : top0 - kWeightShift);
+            top1 = fmaxf(m1, fabsf(top1) > kFarScore ? top1 : top1 - kWeightShift);
             const float alpha0 = pkv::exp2_approx(m0 - top0);
             const float alpha1 = pkv::exp2_approx(m1 - top1);
             m0 = top0;
             m1 = top1;
-            const float base0 = kWeightShift - m0, base1 = kWeightShift - m1;
             float add0 = 0.f, add1 = 0.f;
             uint32_t p[4][2], pl[4][2];
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
-                const float w0 = pkv::exp2_approx(s[j][0] + base0);
-                const float w1 = pkv::exp2_approx(s[j][1] + base1);
-                const float w2 = pkv::exp2_approx(s[j][2] + base0);
-                const float w3 = pkv::exp2_approx(s[j][3] + base1);
+                const float w0 = pkv::exp2_approx(s[j][0] - m0);
+                const float w1 = pkv::exp2_approx(s[j][1] - m1);
+                const float w2 = pkv::exp2_approx(s[j][2] - m0);
+                const float w3 = pkv::exp2_approx(s[j][3] - m1);
                 add0 += w0 + w2;
                 add1 += w1 + w3;
                 const __half2 h01 = __floats2half2_rn(w0, w1), h23 = __floats2half2_rn(w2, w3);

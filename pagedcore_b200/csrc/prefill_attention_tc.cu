@@ -53,13 +53,16 @@
 // TMEM: S/P buffers at columns 0, 64, 128, O at 192 (256 columns, two CTAs
 // per SM).  Shared memory: Q (16 KiB) and the K and V rings.
 //
-// An FP32 query (SPLIT_Q; the 8-bit cache's rotated query) becomes two Q tiles, its FP16
-// value and what that leaves, and S takes both: four more MMAs a step, mostly hidden behind
-// the softmax.  A row is scaled by a power of two that brings its largest value to 2^14 ..
-// 2^15, whatever FP32 range it had, and the row's scores are scaled back.  Over the 8-bit cache (FINE) so does P: what the FP16 weights leave goes over
-// the second 32 columns of S_g's buffer, and P.V takes both, so that the output's own
-// rounding is the only one to FP16.  (One FP16 number for each weight was off by as much
-// again: relative error 2.9e-4 where the output's rounding alone gives 2.0e-4.)
+// FINE, over the 8-bit cache, rounds nothing but the output to FP16:
+// - A query row (FP16, or FP32 as rotated) is multiplied by log2(e) / 8 and a power of two
+//   that brings its largest value to 2^14 .. 2^15, whatever FP32 range it had, and becomes
+//   two Q tiles, the FP16 values and what they leave.  S takes both (four more MMAs a step,
+//   mostly hidden behind the softmax) and is scaled back by the power of two, exactly.
+// - What the FP16 weights leave goes over the second 32 columns of S_g's buffer, and P.V
+//   takes both.  (One FP16 number for each weight: relative error 2.9e-4 where the output's
+//   rounding alone gives 2.0e-4.)
+// - The reference is m - 7 and moves when a weight would pass 2^15; past 2^20, where 7 would
+//   soon be lost in its rounding, it is m itself.
 //
 // Block ids outside the pool set PKV_DEVICE_BAD_BLOCK and read as zeros.
 // Every wait is bounded: on a timeout the thread sets
@@ -105,9 +108,9 @@ constexpr int kKCopyLag = 2;
 constexpr int kVCopyLag = 1;
 constexpr int kQBytes = kRows * kRowBytes;             // 16 KiB
 constexpr int kRingBytes = kStepBlocks * kBoxBytes;    // 8 KiB: one step's K (or V)
-// SPLIT_Q: a second Q tile, the low halves.  + alignment slack.
-template <bool SPLIT_Q>
-constexpr int kSmemBytes = (SPLIT_Q ? 2 : 1) * kQBytes + (kKStages + kVStages) * kRingBytes + 1024;
+// FINE: a second Q tile, the low halves.  + alignment slack.
+template <bool FINE>
+constexpr int kSmemBytes = (FINE ? 2 : 1) * kQBytes + (kKStages + kVStages) * kRingBytes + 1024;
 constexpr int kSoftmaxWarps = 4;           // thread r of warps 0-3 owns row r (TMEM lane r)
 constexpr int kSoftmaxThreads = kSoftmaxWarps * 32;
 constexpr int kThreads = kSoftmaxThreads + 128;
@@ -131,6 +134,7 @@ constexpr float kScaleLog2 = 0.125f * 1.4426950408889634f;  // 64^-0.5 * log2(e)
 // inside FP16 while O and l are rescaled at most a few times per row.
 constexpr float kWeightShift = 7.0f;
 constexpr float kRescaleLog2 = 8.0f;
+constexpr float kFarScore = 0x1p20f;
 static_assert(kRows == kTileTokens * (PKV_QUERY_HEADS / kKvHeads), "a tile's rows are its tokens x 8 heads");
 static_assert(kKCopyLag < kKStages && kVCopyLag < kVStages, "a producer would wait for a stage it has not published");
 
@@ -150,7 +154,7 @@ struct TcArgs {
     int32_t start;
     int32_t tokens;
     int32_t *error_flag;
-    const float *query32;  // SPLIT_Q, in place of query
+    const float *query32;  // FINE: in place of query, where it is not null
 };
 
 // Barriers of one CTA (8-byte mbarriers in static shared memory).
@@ -230,58 +234,73 @@ __device__ __forceinline__ void load_q_row(uint32_t q_smem, const TcArgs &a, con
     pkv::cp_async_commit();
 }
 
-// The same from an FP32 query: two FP16 numbers that add up to each value times 2^-e, the
-// high halves at q_smem and the low ones a tile further.  Returns 2^e.  (Few loads
-// at a time: the registers for a whole row are not there.  All at once before the first
-// step, where they are, saved 0.5 us of 70.)
-__device__ __forceinline__ float load_q_row_split(uint32_t q_smem, const TcArgs &a, const Item &it, int r) {
+// Eight values of the query, FP16 or FP32.
+__device__ __forceinline__ void load_q8(const TcArgs &a, int64_t at, float (&v)[8]) {
+    if (a.query32 != nullptr) {
+        const float4 *src = reinterpret_cast<const float4 *>(a.query32 + at);
+        const float4 x = src[0], y = src[1];
+        v[0] = x.x, v[1] = x.y, v[2] = x.z, v[3] = x.w, v[4] = y.x, v[5] = y.y, v[6] = y.z, v[7] = y.w;
+    } else {
+        const uint4 raw = *reinterpret_cast<const uint4 *>(a.query + at);
+        const __half2 *h = reinterpret_cast<const __half2 *>(&raw);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const float2 f = __half22float2(h[i]);
+            v[2 * i] = f.x, v[2 * i + 1] = f.y;
+        }
+    }
+}
+
+// FINE: the row times log2(e) / 8 and 2^-e as two FP16 numbers that add up to each value, the
+// high halves at q_smem and the low ones a tile further.  Returns 2^e.  (Few loads at a time:
+// the registers for a whole row are not there.  All at once before the first step, where they
+// are, saved 0.5 us of 70.)
+__device__ __forceinline__ float load_q_row_fine(uint32_t q_smem, const TcArgs &a, const Item &it, int r) {
     const int t = min(it.t0 + (r >> 3), a.tokens - 1);
-    const float4 *src = reinterpret_cast<const float4 *>(a.query32 + static_cast<int64_t>(t) * a.query_stride +
-                                                         (it.kv * 8 + (r & 7)) * kHeadDim);
+    const int64_t at = static_cast<int64_t>(t) * a.query_stride + (it.kv * 8 + (r & 7)) * kHeadDim;
     const uint32_t row = q_smem + (r >> 3) * 1024 + (r & 7) * kRowBytes;
     float largest = 0.f;  // of the finite values
-#pragma unroll 4
-    for (int c = 0; c < 16; ++c) {
-        const float4 x = src[c];
-        largest = pkv::fp8::max_finite(pkv::fp8::max_finite(largest, x.x), x.y);
-        largest = pkv::fp8::max_finite(pkv::fp8::max_finite(largest, x.z), x.w);
-    }
-    // A row of zeros or of FP32's subnormals stays what it is (2^100 times).
-    const int e = max((__float_as_int(largest) >> 23) - 127 - 14, -100);
-    const float down = pkv::fp8::exp2_int(-e);
 #pragma unroll 2
     for (int c = 0; c < 8; ++c) {
-        const float4 x = src[2 * c], y = src[2 * c + 1];
-        const float v[8] = {x.x * down, x.y * down, x.z * down, x.w * down, y.x * down, y.y * down, y.z * down, y.w * down};
+        float v[8];
+        load_q8(a, at + 8 * c, v);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) largest = pkv::fp8::max_finite(largest, v[i]);
+    }
+    // A row of zeros or of FP32's subnormals: 2^100.
+    const int e = max((__float_as_int(largest) >> 23) - 127 - 14, -100);
+    const float factor = pkv::fp8::exp2_int(-e) * kScaleLog2;
+#pragma unroll 2
+    for (int c = 0; c < 8; ++c) {
+        float v[8];
+        load_q8(a, at + 8 * c, v);
         uint32_t high[4], low[4];
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-            const __half2 h = __floats2half2_rn(v[2 * i], v[2 * i + 1]);
+            const float x = __fmul_rn(v[2 * i], factor), y = __fmul_rn(v[2 * i + 1], factor);
+            const __half2 h = __floats2half2_rn(x, y);
             const float2 f = __half22float2(h);
             high[i] = pkv::pack_half2(h);
-            low[i] = pack2(v[2 * i] - f.x, v[2 * i + 1] - f.y);
+            low[i] = pack2(x - f.x, y - f.y);
         }
-        const uint32_t at = row + ((c ^ (r & 7)) << 4);
-        asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(at), "r"(high[0]), "r"(high[1]), "r"(high[2]), "r"(high[3]) : "memory");
-        asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(at + kQBytes), "r"(low[0]), "r"(low[1]), "r"(low[2]), "r"(low[3]) : "memory");
+        const uint32_t to = row + ((c ^ (r & 7)) << 4);
+        asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(to), "r"(high[0]), "r"(high[1]), "r"(high[2]), "r"(high[3]) : "memory");
+        asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(to + kQBytes), "r"(low[0]), "r"(low[1]), "r"(low[2]), "r"(low[3]) : "memory");
     }
     return pkv::fp8::exp2_int(e);
 }
 
 // Either, and the factor from the row's products to scores in base 2.
-template <bool SPLIT_Q>
+template <bool FINE>
 __device__ __forceinline__ float load_q(uint32_t q_smem, const TcArgs &a, const Item &it, int r) {
-    if constexpr (SPLIT_Q) {
-        return load_q_row_split(q_smem, a, it, r) * kScaleLog2;
-    } else {
-        load_q_row(q_smem, a, it, r);
-        return kScaleLog2;
-    }
+    if constexpr (FINE) return load_q_row_fine(q_smem, a, it, r);
+    load_q_row(q_smem, a, it, r);
+    return kScaleLog2;
 }
 
 // At most 120 registers a thread: two CTAs of 256 threads then fit an SM
 // (the occupancy calculation gives one CTA at 125).
-template <bool SPLIT_Q, bool FINE>
+template <bool FINE>
 __global__ void __maxnreg__(120)
     prefill_tc_kernel(const TcArgs a) {
     extern __shared__ uint8_t dyn_smem[];
@@ -293,7 +312,7 @@ __global__ void __maxnreg__(120)
     const uint32_t raw = pkv::smem_addr(dyn_smem);
     const uint32_t base = (raw + 1023u) & ~1023u;  // 1024-aligned: swizzle atoms
     const uint32_t q_smem = base;
-    const uint32_t k_smem = base + (SPLIT_Q ? 2 : 1) * kQBytes;   // K ring, 8 KiB a stage
+    const uint32_t k_smem = base + (FINE ? 2 : 1) * kQBytes;   // K ring, 8 KiB a stage
     const uint32_t v_smem = k_smem + kKStages * kRingBytes;   // V ring, 8 KiB a stage
 
     const int tiles = (a.tokens + kTileTokens - 1) / kTileTokens;
@@ -441,7 +460,7 @@ __global__ void __maxnreg__(120)
                         pkv::tc::mma_f16_ss(tmem + (g % kSBuffers) * kStepKeys, q_desc + 2 * k, k_desc + 2 * k, kIdescS,
                                             k > 0);
                     }
-                    if constexpr (SPLIT_Q) {  // the low halves, a tile (kQBytes / 16 on the descriptor) further
+                    if constexpr (FINE) {  // the low halves, a tile (kQBytes / 16 on the descriptor) further
 #pragma unroll
                         for (int k = 0; k < kHeadDim / 16; ++k) {
                             pkv::tc::mma_f16_ss(tmem + (g % kSBuffers) * kStepKeys, q_desc + kQBytes / 16 + 2 * k,
@@ -512,7 +531,7 @@ __global__ void __maxnreg__(120)
         // of the item before it, once every S MMA that read the tile has completed.
         float next_scale = kScaleLog2;
         if (item_of(0, cta, ctas) < items) {
-            next_scale = load_q<SPLIT_Q>(q_smem, a, item_info(item_of(0, cta, ctas), tiles, a), r);
+            next_scale = load_q<FINE>(q_smem, a, item_info(item_of(0, cta, ctas), tiles, a), r);
             pkv::cp_async_wait<0>();
             pkv::fence_proxy_async_smem();  // generic-proxy copies -> the MMA's (async proxy) reads
             __syncwarp();
@@ -526,7 +545,7 @@ __global__ void __maxnreg__(120)
             const int t = it.t0 + (r >> 3);
             const int pos = a.start + min(t, a.tokens - 1);  // last position this row attends to
             const int head = it.kv * 8 + (r & 7);
-            const float scale = SPLIT_Q ? next_scale : kScaleLog2;
+            const float scale = FINE ? next_scale : kScaleLog2;
             float m = -INFINITY;  // the row maximum at its last rescale (log2 units)
             float l = 0.f;        // sum of this row's weights, relative to m
             for (int j = 0; j < it.steps; ++j, ++g) {
@@ -545,7 +564,7 @@ __global__ void __maxnreg__(120)
                 pkv::tc::tmem_wait_ld();
                 // s_full of the item's last step: every S MMA of the item has
                 // completed, so the next item's Q may replace this one's.
-                if (last && next < items) next_scale = load_q<SPLIT_Q>(q_smem, a, item_info(next, tiles, a), r);
+                if (last && next < items) next_scale = load_q<FINE>(q_smem, a, item_info(next, tiles, a), r);
 
                 float s[64];
 #pragma unroll
@@ -572,13 +591,18 @@ __global__ void __maxnreg__(120)
                                             fmaxf(mx8[6], mx8[7]));
                 // Step 0 holds position 0, which every row attends to: m is finite from step 0 on.
                 const float m_blk = mx * scale;
-                const float m_new = m_blk > m + kRescaleLog2 ? m_blk : m;  // m = -inf at step 0: always moves
+                float m_new = m;  // m = -inf at step 0: always moves
+                if constexpr (FINE) {  // m is the reference itself
+                    if (m_blk - m > kWeightShift + kRescaleLog2) m_new = fabsf(m_blk) > kFarScore ? m_blk : m_blk - kWeightShift;
+                } else {
+                    if (m_blk > m + kRescaleLog2) m_new = m_blk;
+                }
                 // P_g as FP16 (x 2^7) over the first 32 columns of its S buffer,
                 // two keys to a column (the A operand of P.V from TMEM); l sums the
                 // FP32 weights over 8 independent chains.
                 // Pairs of keys go through the packed FP32 instructions (the same
                 // rounding as two scalar ones, half the instructions).
-                const float shift = kWeightShift - m_new;
+                const float shift = FINE ? -m_new : kWeightShift - m_new;
                 const uint64_t scale2 = pkv::f32x2(scale, scale);
                 const uint64_t shift2 = pkv::f32x2(shift, shift);
                 uint64_t l4[4] = {0, 0, 0, 0};  // FP32 pairs: 8 independent chains
@@ -689,18 +713,18 @@ constexpr int kCtasPerSm = 2;
 
 // Per device, once: the kernel's dynamic shared-memory limit raised, and the
 // number of its CTAs that run at once (2 per SM) recorded in *ctas.
-template <bool SPLIT_Q, bool FINE>
+template <bool FINE>
 int prepare(int device, int *ctas) {
     static std::atomic<int> resident[kMaxDevices] = {};
     if (device >= 0 && device < kMaxDevices) {
         *ctas = resident[device].load(std::memory_order_acquire);
         if (*ctas > 0) return PKV_OK;
     }
-    cudaError_t e = cudaFuncSetAttribute(prefill_tc_kernel<SPLIT_Q, FINE>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                         kSmemBytes<SPLIT_Q>);
+    cudaError_t e = cudaFuncSetAttribute(prefill_tc_kernel<FINE>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                         kSmemBytes<FINE>);
     if (e == cudaSuccess) {
         // All of the SM's unified L1/shared memory as shared memory: two CTAs' worth.
-        e = cudaFuncSetAttribute(prefill_tc_kernel<SPLIT_Q, FINE>, cudaFuncAttributePreferredSharedMemoryCarveout,
+        e = cudaFuncSetAttribute(prefill_tc_kernel<FINE>, cudaFuncAttributePreferredSharedMemoryCarveout,
                                  cudaSharedmemCarveoutMaxShared);
     }
     if (e != cudaSuccess) {
@@ -721,21 +745,21 @@ int prepare(int device, int *ctas) {
     return PKV_OK;
 }
 
-template <bool SPLIT_Q, bool FINE>
+template <bool FINE>
 int launch(const TcArgs &args, cudaStream_t stream) {
     int device = 0;
     cudaError_t e = cudaGetDevice(&device);
     if (e != cudaSuccess) return pkv::fail(PKV_CUDA_ERROR, std::string("cudaGetDevice: ") + cudaGetErrorString(e));
     int resident = 0;
-    const int rc = prepare<SPLIT_Q, FINE>(device, &resident);
+    const int rc = prepare<FINE>(device, &resident);
     if (rc) return rc;
     // One CTA per resident slot at most; each walks its share of the items.
     const int items = (args.tokens + kTileTokens - 1) / kTileTokens * kKvHeads;
     if constexpr (FINE) {
-        e = pkv::launch_pdl_smem(prefill_tc_kernel<SPLIT_Q, FINE>, dim3(std::min(items, resident)), dim3(kThreads),
-                                 kSmemBytes<SPLIT_Q>, stream, args);
+        e = pkv::launch_pdl_smem(prefill_tc_kernel<FINE>, dim3(std::min(items, resident)), dim3(kThreads),
+                                 kSmemBytes<FINE>, stream, args);
     } else {
-        prefill_tc_kernel<SPLIT_Q, FINE><<<std::min(items, resident), kThreads, kSmemBytes<SPLIT_Q>, stream>>>(args);
+        prefill_tc_kernel<FINE><<<std::min(items, resident), kThreads, kSmemBytes<FINE>, stream>>>(args);
         e = cudaGetLastError();
     }
     if (e != cudaSuccess) {
@@ -750,7 +774,7 @@ namespace pkv {
 
 // Launch of the tcgen05 prefill attention (arguments checked by the caller); the query FP16
 // or, with query_fp32, FP32.  fine: over the 8-bit cache's values, behind the kernel that
-// reads them, with weights that are not rounded to FP16 (query_fp32 needs it).
+// reads them (query_fp32 needs it).
 int launch_prefill_attention_tc(const void *pool, int32_t num_blocks, int32_t layer, const void *query,
                                 bool query_fp32, bool fine, int64_t query_stride, const int32_t *blocks, int32_t start,
                                 int32_t tokens, void *out, int64_t out_stride, int32_t *error_flag,
@@ -768,8 +792,7 @@ int launch_prefill_attention_tc(const void *pool, int32_t num_blocks, int32_t la
     args.start = start;
     args.tokens = tokens;
     args.error_flag = error_flag;
-    if (query_fp32) return launch<true, true>(args, stream);
-    return fine ? launch<false, true>(args, stream) : launch<false, false>(args, stream);
+    return fine ? launch<true>(args, stream) : launch<false>(args, stream);
 }
 
 }  // namespace pkv

@@ -191,3 +191,57 @@ def test_a_prompt_that_rotates_past_fp16_stays_finite() -> None:
     exact_query = rope64(query, case.rope, at)
     assert float(exact_query.abs().max()) > 65520
     check_prompt(out, exact_query, k, v, 0, [0, 1, 17, 39])
+
+
+def check_far(out, query, key, value) -> None:
+    """``out`` [32, 64] where scores lie far apart: finite, and the value of the one that is clearly the largest."""
+    assert bool(out.isfinite().all())
+    scores = query.double().view(4, 8, 64) @ key.transpose(0, 1).transpose(1, 2) / 8
+    weight = torch.softmax(scores, -1)
+    # FP32 scores are off by some 2^-16 of their size: a lead of that and 40 more leaves the rest below 2^-40.
+    lead = scores.topk(min(2, len(key)), -1).values
+    clear = lead[..., 0] - lead[..., -1] > 40 + 2.0**-12 * scores.abs().amax(-1) if len(key) > 1 else lead[..., 0] == lead[..., 0]
+    best = (weight @ value.transpose(0, 1)).reshape(32, 64)
+    clear = clear.reshape(32)
+    assert int(clear.sum()) > 16
+    assert bool(((out.double() - best).abs() <= 2.0**-11 * best.abs() + 2.0**-25 + 2.0**-30 * value.abs().amax())[clear].all())
+
+
+@pytest.mark.parametrize("factor", [2.0**16, 2.0**21, 2.0**25, 2.0**31, 2.0**38])
+@pytest.mark.parametrize("layer_call", [False, True])
+def test_decode_attention_of_scores_far_out(factor, layer_call) -> None:
+    """Scores up to and past 2^24, where 1 is lost in FP32: the largest one's value, not NaN."""
+    lengths = [1, 40, 17, 300, 2048]
+    case = CacheCase(161, [0] * 5, spare=sum(-(-n // 16) for n in lengths))
+    size = min(factor, 2.0**15)
+    for row, n in enumerate(lengths):
+        case.tables[row] += [case.free.pop() for _ in range(-(-n // 16))]
+        case.lengths[row] = n
+        key = (randn(162 + row, n, 4, 64) * (factor / size / 64 if factor > size else 1.0)).clamp(-60000, 60000)
+        case.append(row, key, randn(170 + row, n, 4, 64), 0)
+    query = (randn(163, 5, 32, 64) * size / 2).clamp(-65504, 65504).half()
+    if layer_call:
+        key, value = randn(164, 5, 4, 64).half(), randn(165, 5, 4, 64).half()
+        out = fp8.decode_layer(case.cache, LAYER, query, key, value, case.rope, *case.batch(), case.flag)
+        query = rope64(query, case.rope, torch.tensor(lengths, device=case.device) - 1)
+    else:
+        out = fp8.decode_attention(case.cache, LAYER, query, *case.batch(), case.flag)
+    assert int(case.flag.item()) == 0
+    for row, n in enumerate(lengths):
+        blocks = torch.tensor(case.tables[row], dtype=torch.int32, device=case.device)
+        k, v = (x.reshape(-1, 4, 64)[:n].double() for x in fp8.read_blocks(case.cache, LAYER, blocks, case.flag))
+        check_far(out[row], query[row], k, v)
+
+
+@pytest.mark.parametrize("exponent", [16, 21, 24, 25, 27, 31, 60, 100])
+@pytest.mark.parametrize("start, tokens", [(0, 40), (300, 70), (0, 1300)])
+def test_prompt_attention_of_scores_far_out(exponent, start, tokens) -> None:
+    case = CacheCase(166, [start + tokens])
+    query = torch.ldexp(randn(167, tokens, 32, 64), torch.tensor(exponent, device=case.device))
+    query[1::3] *= 2.0**-exponent  # ordinary rows beside them
+    out = fp8.prefill_attention(case.cache, LAYER, query, case.batch()[2], start, case.flag)
+    assert int(case.flag.item()) == 0 and bool(out.isfinite().all())
+    key, value = (oracle.tokens(case.tables[0], start + tokens) for oracle in (case.key, case.value))
+    check_prompt(out, query, key, value, start, range(1, tokens, 3 * max(1, tokens // 60)))
+    for t in range(0, tokens, 3 * max(1, tokens // 60)):
+        check_far(out[t], query[t], key[: start + t + 1], value[: start + t + 1])
