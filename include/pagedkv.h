@@ -494,6 +494,14 @@ int pkv_fp8_decode_layer(void *key_codes, void *value_codes, void *key_scales, v
                          void *out, int64_t out_stride, void *workspace, int64_t workspace_bytes, int32_t *error_flag,
                          void *stream);
 
+/* The same, but a row without blocks gives zeros. */
+int pkv_fp8_decode_layer_zero(void *key_codes, void *value_codes, void *key_scales, void *value_scales, int32_t layers,
+                              int32_t num_blocks, int32_t layer, const void *query, int64_t query_stride,
+                              const void *key, const void *value, int64_t kv_stride, const void *rope_table,
+                              const int32_t *lengths, const int32_t *prefix, const int32_t *flat, int32_t batch,
+                              int32_t total_blocks, int32_t grid, void *out, int64_t out_stride, void *workspace,
+                              int64_t workspace_bytes, int32_t *error_flag, void *stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -197,6 +197,31 @@ SIGNATURES: dict[str, tuple[object, list[object]]] = {
             c_void_p,  # stream
         ],
     ),
+    "pkv_fp8_decode_layer_zero": (
+        c_int,
+        [
+            *_FP8_CACHE,
+            c_int32,  # layer
+            c_void_p,  # query
+            c_int64,  # query_stride
+            c_void_p,  # key
+            c_void_p,  # value
+            c_int64,  # kv_stride
+            c_void_p,  # rope_table
+            c_void_p,  # lengths
+            c_void_p,  # prefix
+            c_void_p,  # flat
+            c_int32,  # batch
+            c_int32,  # total_blocks
+            c_int32,  # grid
+            c_void_p,  # out
+            c_int64,  # out_stride
+            c_void_p,  # workspace
+            c_int64,  # workspace_bytes
+            c_void_p,  # error_flag
+            c_void_p,  # stream
+        ],
+    ),
     "pkv_append_kv": (
         c_int,
         [

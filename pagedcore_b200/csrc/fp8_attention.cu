@@ -737,9 +737,9 @@ namespace {
 
 // The attention of pkv_fp8_decode_attention, with the append of pkv_fp8_decode_layer before it when `key` is given.
 int decode(const pkv::fp8::Cache &cache, int32_t layer, const void *query, int64_t query_stride, const void *key,
-           const void *value, int64_t kv_stride, const void *rope_table, const int32_t *lengths, const int32_t *prefix,
-           const int32_t *flat, int32_t batch, int32_t total_blocks, int32_t grid, void *out, int64_t out_stride,
-           void *workspace, int64_t workspace_bytes, int32_t *error_flag, cudaStream_t stream) {
+           const void *value, int64_t kv_stride, const void *rope_table, bool clear, const int32_t *lengths,
+           const int32_t *prefix, const int32_t *flat, int32_t batch, int32_t total_blocks, int32_t grid, void *out,
+           int64_t out_stride, void *workspace, int64_t workspace_bytes, int32_t *error_flag, cudaStream_t stream) {
     int rc = pkv::fp8::check_cache(cache.key_codes, cache.value_codes, cache.key_scales, cache.value_scales,
                                    cache.layers, cache.num_blocks, layer, 1);
     if (rc) return rc;
@@ -787,7 +787,7 @@ int decode(const pkv::fp8::Cache &cache, int32_t layer, const void *query, int64
     a.batch = batch;
     a.capacity = total_blocks;
     a.grid = grid;
-    a.clear = key == nullptr;
+    a.clear = clear;
     a.early = key != nullptr;
     a.out = static_cast<__half *>(out);
     a.out_stride = out_stride;
@@ -825,6 +825,19 @@ pkv::fp8::Cache cache_of(const void *key_codes, const void *value_codes, const v
             layers, num_blocks};
 }
 
+// The same with the append before it; clear: rows without blocks give zeros.
+int decode_layer(const pkv::fp8::Cache &cache, int32_t layer, const void *query, int64_t query_stride, const void *key,
+                 const void *value, int64_t kv_stride, const void *rope_table, bool clear, const int32_t *lengths,
+                 const int32_t *prefix, const int32_t *flat, int32_t batch, int32_t total_blocks, int32_t grid, void *out,
+                 int64_t out_stride, void *workspace, int64_t workspace_bytes, int32_t *error_flag, cudaStream_t stream) {
+    pkv::clear_error();
+    if (key == nullptr || value == nullptr || rope_table == nullptr) {
+        return pkv::fail(PKV_VALUE_ERROR, "fp8 decode layer: key, value and rope_table are required");
+    }
+    return decode(cache, layer, query, query_stride, key, value, kv_stride, rope_table, clear, lengths, prefix, flat,
+                  batch, total_blocks, grid, out, out_stride, workspace, workspace_bytes, error_flag, stream);
+}
+
 }  // namespace
 
 extern "C" int pkv_fp8_decode_attention(const void *key_codes, const void *value_codes, const void *key_scales,
@@ -835,8 +848,8 @@ extern "C" int pkv_fp8_decode_attention(const void *key_codes, const void *value
                                         int64_t workspace_bytes, int32_t *error_flag, void *stream) {
     pkv::clear_error();
     return decode(cache_of(key_codes, value_codes, key_scales, value_scales, layers, num_blocks), layer, query,
-                  query_stride, nullptr, nullptr, 0, nullptr, lengths, prefix, flat, batch, total_blocks, grid, out,
-                  out_stride, workspace, workspace_bytes, error_flag, static_cast<cudaStream_t>(stream));
+                  query_stride, nullptr, nullptr, 0, nullptr, true, lengths, prefix, flat, batch, total_blocks, grid,
+                  out, out_stride, workspace, workspace_bytes, error_flag, static_cast<cudaStream_t>(stream));
 }
 
 extern "C" int pkv_fp8_decode_layer(void *key_codes, void *value_codes, void *key_scales, void *value_scales,
@@ -846,11 +859,19 @@ extern "C" int pkv_fp8_decode_layer(void *key_codes, void *value_codes, void *ke
                                     const int32_t *flat, int32_t batch, int32_t total_blocks, int32_t grid, void *out,
                                     int64_t out_stride, void *workspace, int64_t workspace_bytes, int32_t *error_flag,
                                     void *stream) {
-    pkv::clear_error();
-    if (key == nullptr || value == nullptr || rope_table == nullptr) {
-        return pkv::fail(PKV_VALUE_ERROR, "fp8 decode layer: key, value and rope_table are required");
-    }
-    return decode(cache_of(key_codes, value_codes, key_scales, value_scales, layers, num_blocks), layer, query,
-                  query_stride, key, value, kv_stride, rope_table, lengths, prefix, flat, batch, total_blocks, grid, out,
-                  out_stride, workspace, workspace_bytes, error_flag, static_cast<cudaStream_t>(stream));
+    return decode_layer(cache_of(key_codes, value_codes, key_scales, value_scales, layers, num_blocks), layer, query,
+                        query_stride, key, value, kv_stride, rope_table, false, lengths, prefix, flat, batch, total_blocks,
+                        grid, out, out_stride, workspace, workspace_bytes, error_flag, static_cast<cudaStream_t>(stream));
+}
+
+extern "C" int pkv_fp8_decode_layer_zero(void *key_codes, void *value_codes, void *key_scales, void *value_scales,
+                                         int32_t layers, int32_t num_blocks, int32_t layer, const void *query,
+                                         int64_t query_stride, const void *key, const void *value, int64_t kv_stride,
+                                         const void *rope_table, const int32_t *lengths, const int32_t *prefix,
+                                         const int32_t *flat, int32_t batch, int32_t total_blocks, int32_t grid, void *out,
+                                         int64_t out_stride, void *workspace, int64_t workspace_bytes, int32_t *error_flag,
+                                         void *stream) {
+    return decode_layer(cache_of(key_codes, value_codes, key_scales, value_scales, layers, num_blocks), layer, query,
+                        query_stride, key, value, kv_stride, rope_table, true, lengths, prefix, flat, batch, total_blocks,
+                        grid, out, out_stride, workspace, workspace_bytes, error_flag, static_cast<cudaStream_t>(stream));
 }

@@ -536,7 +536,7 @@ def _decode(cache, layer, query, new, lengths, prefix, flat, total_blocks, error
     grid, workspace_bytes = decode_plan(index, batch, total_blocks)
     workspace = torch.empty((workspace_bytes + 1) // 2, dtype=_HALF, device=query.device)
     _call(
-        index, lib.pkv_fp8_decode_attention if new is None else lib.pkv_fp8_decode_layer, *cache._args(), layer,
+        index, lib.pkv_fp8_decode_attention if new is None else lib.pkv_fp8_decode_layer_zero, *cache._args(), layer,
         query.data_ptr(), query_stride, *(new or ()), _int_list(index, "lengths", lengths, batch),
         _int_list(index, "prefix", prefix, batch + 1), _int_list(index, "flat", flat, total_blocks), batch,
         total_blocks, grid, out.data_ptr(), out_stride, workspace.data_ptr(), workspace_bytes,
@@ -584,7 +584,7 @@ def decode_layer(
     The new token of each row sits at position lengths - 1 in the row's last
     block: its K (rotated) and V [B, 4, 64] are written, query [B, 32, 64] is
     rotated, and attends to all of the row's tokens.  No two rows may share
-    a last block.
+    a last block.  A row without blocks gives zeros.
     """
     index = cache.key_codes.get_device()
     shape = (query.shape[0], _KV_HEADS, _HEAD_DIM)

@@ -89,3 +89,45 @@ def test_a_bad_block_reads_as_zeros(lengths, bad, layer_call) -> None:
         k, v = (x.reshape(-1, 4, 64)[:length].double() for x in read)
         exact, bound = attend64(query[row], k, v)
         assert bool(((out[row].double() - exact).abs() <= bound).all()), row
+
+
+@pytest.mark.parametrize("lengths", [[0], [5, 0, 40], [0, 0, 300, 0, 17, 0, 0], [0] * 70 + [2048], [1] + [0] * 300], ids=lambda v: f"{len(v)}rows{max(v)}")
+def test_a_decode_layer_row_without_blocks_gives_zeros(lengths) -> None:
+    case = CacheCase(158, [max(0, n - 1) for n in lengths])
+    for row, length in enumerate(lengths):
+        if len(case.tables[row]) * 16 < length:
+            case.tables[row].append(case.free.pop())
+        case.lengths[row] = length
+    rows = len(lengths)
+    query, key, value = (randn(159 + heads, rows, heads, 64).half() for heads in (32, 4, 4))
+    query[torch.tensor(lengths) == 0] = float("nan")
+    calls = []
+    for out in (None, torch.full((rows + 1, 40, 64), 7.0, dtype=torch.float16, device=case.device)):
+        torch.full((rows, 32, 64), 9.0, dtype=torch.float16, device=case.device)  # storage that the next call may get
+        calls.append(fp8.decode_layer(case.cache, LAYER, query, key, value, case.rope, *case.batch(), case.flag,
+                                      None if out is None else out[:rows, 4:36]))
+    assert int(case.flag.item()) == 0
+    assert bool((out[rows] == 7).all()) and bool((out[:, :4] == 7).all()) and bool((out[:, 36:] == 7).all())
+    exact_query = rope64(query.nan_to_num(), case.rope, (torch.tensor(lengths, device=case.device) - 1).clamp(min=0))
+    for result in calls:
+        for row, length in enumerate(lengths):
+            blocks = torch.tensor(case.tables[row], dtype=torch.int32, device=case.device)
+            k, v = (x.reshape(-1, 4, 64)[:length].double() for x in fp8.read_blocks(case.cache, LAYER, blocks, case.flag))
+            exact, bound = attend64(exact_query[row], k, v)
+            assert bool(((result[row].double() - exact).abs() <= bound).all()), row
+
+
+def test_rows_past_a_replayed_batch_are_left_alone() -> None:
+    """The entry point that step graphs launch: a row without blocks keeps its output."""
+    case = CacheCase(160, [20, 0])
+    lengths, prefix, flat, total = case.batch()
+    query, key, value = (randn(161 + heads, 2, heads, 64).half() for heads in (32, 4, 4))
+    grid, size = fp8.decode_plan(case.device.index, 2, total)
+    workspace = torch.empty(size, dtype=torch.uint8, device=case.device)
+    for function, kept in ((lib.pkv_fp8_decode_layer, 3.0), (lib.pkv_fp8_decode_layer_zero, 0.0)):
+        out = torch.full((2, 32, 64), 3.0, dtype=torch.float16, device=case.device)
+        check(function(*case.cache._args(), LAYER, query.data_ptr(), 2048, key.data_ptr(), value.data_ptr(), 256,
+                       case.rope.data_ptr(), lengths.data_ptr(), prefix.data_ptr(), flat.data_ptr(), 2, total, grid,
+                       out.data_ptr(), 2048, workspace.data_ptr(), size, case.flag.data_ptr(),
+                       torch.cuda.current_stream().cuda_stream))
+        assert bool((out[1] == kept).all()) and not bool((out[0] == 3.0).any())
