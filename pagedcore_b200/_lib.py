@@ -386,7 +386,7 @@ def check(status: int) -> None:
         raise error_for(status)
 
 
-def device_error_message(flag: int) -> str:
+def device_error_message(flag: int, kernel: str = "KV") -> str:
     parts = []
     if flag & DEVICE_BAD_BLOCK:
         parts.append("physical KV block outside the pool")
@@ -394,4 +394,4 @@ def device_error_message(flag: int) -> str:
         parts.append("RoPE position outside [0, 2048)")
     if flag & DEVICE_WAIT_TIMEOUT:
         parts.append("a bounded pipeline wait timed out")
-    return "KV kernel reported: " + ", ".join(parts or [f"flag {flag}"])
+    return f"{kernel} kernel reported: " + ", ".join(parts or [f"flag {flag}"])

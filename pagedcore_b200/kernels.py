@@ -16,7 +16,7 @@ import numpy as np
 import torch
 from torch import Tensor
 
-from pagedcore_b200._lib import check, lib
+from pagedcore_b200._lib import check, device_error_message, lib
 
 _LAYERS = 22
 _KV_HEADS = 4
@@ -471,16 +471,53 @@ GEMV_MAX_ROWS = 1
 TC_MAX_ROWS = 32
 
 _linear_errors: dict[int, Tensor] = {}
+_captured_errors: list[Tensor] = []  # made inside a capture: zero only once the graph has run, and kept for it
 
 
 def linear_error_flag(device: torch.device) -> Tensor:
-    """The device error flag of this device's ``pkv_linear`` launches (int32, zero when all is well)."""
+    """The device error flag of this device's linear layers, FP16 and 8-bit (int32, zero when all is well).
+
+    ``check_linear_errors`` and an allocator's ``check_device_errors`` read it.
+    (A flag whose first use is inside a graph capture is that graph's own, and
+    not read: ask for the flag before a capture, as the decoders do.)
+    """
     index = device.index if device.index is not None else torch.cuda.current_device()
     flag = _linear_errors.get(index)
     if flag is None:
         with torch.inference_mode(False):
-            flag = _linear_errors[index] = torch.zeros(1, dtype=torch.int32, device=torch.device("cuda", index))
+            flag = torch.zeros(1, dtype=torch.int32, device=torch.device("cuda", index))
+        if torch.cuda.is_current_stream_capturing():
+            _captured_errors.append(flag)
+        else:
+            _linear_errors[index] = flag
     return flag
+
+
+def device_linear_flag(device: torch.device) -> Tensor | None:
+    """``linear_error_flag`` if a linear layer of ``device`` has asked for it."""
+    return _linear_errors.get(device.index if device.index is not None else torch.cuda.current_device())
+
+
+def take_flags(*flags: Tensor) -> int:
+    """The bits set in device error flags (int32 [1], of one device), cleared; waits for the current stream."""
+    host = torch.empty(len(flags), dtype=torch.int32, pin_memory=True)
+    for at, flag in enumerate(flags):
+        host[at : at + 1].copy_(flag, non_blocking=True)
+    torch.cuda.current_stream(flags[0].device).synchronize()
+    bits = 0
+    for flag, value in zip(flags, host.tolist()):
+        if value:
+            bits |= value
+            flag.zero_()
+    return bits
+
+
+def check_linear_errors(device: torch.device | str = "cuda") -> None:
+    """Wait for the current stream and raise if a linear layer on ``device`` reported an error since the last check."""
+    flag = device_linear_flag(torch.device(device))
+    bits = 0 if flag is None else take_flags(flag)
+    if bits:
+        raise RuntimeError(device_error_message(bits, "linear"))
 
 
 def linear_splits(rows: int, n: int, k: int) -> int:

@@ -488,11 +488,21 @@ class KVAllocator:
         return {grid: state.weights.copy() for grid, state in self._speeds.items()}
 
     def check_device_errors(self) -> None:
-        """Synchronise and raise if a kernel flagged an out-of-range block or position."""
-        flag = int(self._error.item())
+        """Synchronise and raise if a kernel flagged an out-of-range block or position, or a wait that ran out.
+
+        Where linear layers ran on the pool's device, their flag is read too: a
+        projection that gave up has written part of its sums.
+        """
+        linear = kernels.device_linear_flag(self._pool.device)
+        if linear is None:
+            flag = int(self._error.item())
+            if flag:
+                self._error.zero_()
+                raise RuntimeError(device_error_message(flag))
+            return
+        flag = kernels.take_flags(self._error, linear)
         if flag:
-            self._error.zero_()
-            raise RuntimeError(device_error_message(flag))
+            raise RuntimeError(device_error_message(flag, "KV or linear"))
 
     # -- reference API ----------------------------------------------------------
     def create(self, reservation: KVReservation) -> None:
