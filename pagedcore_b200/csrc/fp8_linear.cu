@@ -1107,6 +1107,10 @@ extern "C" int pkv_fp8_linear(const void *x, int64_t x_stride, const void *x_sca
     if (rows < 0 || n < 1 || k < 16 || k % 16) {
         return pkv::fail(PKV_VALUE_ERROR, "fp8 linear: k must be a multiple of 16, n at least 1");
     }
+    // A tile past the last row or column still counts in 32 bits.
+    if (rows > INT32_MAX - 255 || n > INT32_MAX - 255 || k > INT32_MAX - 127) {
+        return pkv::fail(PKV_VALUE_ERROR, "fp8 linear: too many rows or columns");
+    }
     if ((reinterpret_cast<uintptr_t>(x) & 15) || (reinterpret_cast<uintptr_t>(w) & 15) || x_stride % 16 ||
         x_stride < k || (reinterpret_cast<uintptr_t>(out) & 1) || out_stride < n ||
         (reinterpret_cast<uintptr_t>(x_scales) & 3) || (reinterpret_cast<uintptr_t>(w_scales) & 3)) {

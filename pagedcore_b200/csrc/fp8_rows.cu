@@ -33,6 +33,7 @@ constexpr int kThreads = 256;
 constexpr int kChunk = 8;  // FP16 values per 16-byte access
 constexpr int kMaxChunks = 4;
 constexpr int kMaxDim = kThreads * kChunk * kMaxChunks;  // 8192
+constexpr int kMaxRows = INT32_MAX - 65535;  // the row loops step by up to 65535 rows past the last
 
 __device__ __forceinline__ void unpack8(const uint4 &raw, float (&v)[kChunk]) {
     const __half2 *h = reinterpret_cast<const __half2 *>(&raw);
@@ -208,6 +209,7 @@ extern "C" int pkv_fp8_add_rms_norm(const void *hidden, const void *delta, const
         (delta != nullptr && residual == nullptr)) {
         return pkv::fail(PKV_VALUE_ERROR, "fp8 rms norm: hidden, weight, codes and scales are required, and residual with delta");
     }
+    if (rows > kMaxRows) return pkv::fail(PKV_VALUE_ERROR, "fp8 rms norm: too many rows");
     if (rows < 0 || dim < kChunk || dim % kChunk || dim > kMaxDim) {
         return pkv::fail(PKV_VALUE_ERROR, "fp8 rms norm: dim must be a multiple of 8 up to 8192");
     }
@@ -232,6 +234,7 @@ extern "C" int pkv_fp8_quantize(const void *x, int64_t x_stride, int32_t silu_pa
     if (x == nullptr || codes == nullptr || scales == nullptr) {
         return pkv::fail(PKV_VALUE_ERROR, "fp8 rows: x, codes and scales are required");
     }
+    if (rows > kMaxRows) return pkv::fail(PKV_VALUE_ERROR, "fp8 rows: too many rows");
     if (rows < 0 || width < kChunk || width % kChunk || width > (1 << 28)) {
         return pkv::fail(PKV_VALUE_ERROR, "fp8 rows: the width must be a multiple of 8");
     }
@@ -253,6 +256,7 @@ extern "C" int pkv_fp8_to_half(const void *codes, const void *scales, int32_t ro
     if (out == nullptr || codes == nullptr || scales == nullptr) {
         return pkv::fail(PKV_VALUE_ERROR, "fp8 rows: codes, scales and out are required");
     }
+    if (rows > kMaxRows) return pkv::fail(PKV_VALUE_ERROR, "fp8 rows: too many rows");
     if (rows < 0 || width < kChunk || width % kChunk || width > (1 << 28)) {
         return pkv::fail(PKV_VALUE_ERROR, "fp8 rows: the width must be a multiple of 8");
     }

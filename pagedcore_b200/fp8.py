@@ -41,6 +41,15 @@ _current_device = torch._C._cuda_getDevice
 _raw_stream = torch._C._cuda_getCurrentRawStream
 
 
+_MOST = 2**31 - 2**16  # rows, columns and list entries: the C ABI's int32, and a step of a row loop
+
+
+def _fits(name: str, count: int) -> None:
+    """``count`` as the kernels take it (ctypes would cut it to 32 bits without a word)."""
+    if count > _MOST:
+        raise ValueError(f"{name} must be at most {_MOST}, not {count}")
+
+
 def _groups(width: int) -> int:
     return -(-width // GROUP)
 
@@ -130,6 +139,8 @@ def _check_rows(x: Fp8Rows) -> tuple[int, int]:
     if len(shape) != 2 or codes.dtype is not _CODES or codes.stride(1) != 1:
         raise ValueError("8-bit rows must be E4M3 [rows, width] with contiguous rows")
     rows, width = shape
+    _fits("rows", rows)
+    _fits("width", width)
     if scales.shape != (rows, -(-width // GROUP)) or scales.dtype is not _FLOAT or not scales.is_contiguous():
         raise ValueError("8-bit rows need contiguous FP32 scales [rows, ceil(width / 128)]")
     return rows, width
@@ -167,6 +178,8 @@ def add_rms_norm(
     if len(shape) != 2:
         raise ValueError("hidden must be contiguous FP16 [rows, dim]")
     rows, dim = shape
+    _fits("rows", rows)
+    _fits("dim", dim)
     _half_matrix("hidden", hidden, shape)
     _half_matrix("weight", weight, (dim,))
     delta_ptr = residual_ptr = None
@@ -188,8 +201,10 @@ def add_rms_norm(
 
 
 def _quantize(x: Tensor, width: int, silu_pairs: bool) -> Fp8Rows:
-    index = _device(x)
     rows, columns = x.shape
+    _fits("rows", rows)
+    _fits("width", columns)
+    index = _device(x)
     out = _empty_rows(x, rows, width)
     if rows:
         _call(index, lib.pkv_fp8_quantize, x.data_ptr(), _row_stride("x", x, columns), silu_pairs, rows, width,
@@ -243,6 +258,7 @@ def linear(x: Fp8Rows, weight: Fp8Weight, out: Tensor | None = None) -> Tensor:
     if len(shape) != 2 or shape[1] != k or codes.dtype is not _CODES or not codes.is_contiguous():
         raise ValueError(f"weight must be contiguous E4M3 [n, {k}]")
     n = shape[0]
+    _fits("n", n)
     if scales.shape != (_groups(n), _groups(k)) or scales.dtype is not _FLOAT or not scales.is_contiguous():
         raise ValueError("weight needs contiguous FP32 scales [ceil(n / 128), ceil(k / 128)]")
     index = _device(x.codes, x.scales, codes, scales)
@@ -331,6 +347,7 @@ def _half(name: str, tensor: Tensor, index: int) -> None:
 
 def _int_list(index: int, name: str, tensor: Tensor, count: int) -> int:
     """Address of ``count`` or more int32 values on the device."""
+    _fits(f"the entries of {name}", count)
     if tensor.dtype is _INT and tensor.numel() >= count and tensor.get_device() == index and tensor.is_contiguous():
         return tensor.data_ptr()
     raise ValueError(f"{name} must hold {count} contiguous int32 values on cuda:{index}")
@@ -411,6 +428,7 @@ def append_kv(
     _half("key", key, index)
     _half("value", value, index)
     layers, tokens = shape[0], shape[1]
+    _fits("layers", layers)
     slots_ptr = _int_list(index, "slots", slots, tokens)
     flag = _int_list(index, "error_flag", error_flag, 1)
     if (rope_table is None) != (positions is None) or (query is not None and rope_table is None):
