@@ -375,6 +375,31 @@ def _rows_ok(tensor: Tensor, strides: tuple[int, ...]) -> bool:
     )
 
 
+def _rows_apart(strides: tuple[int, ...], layers: int, tokens: int) -> bool:
+    """Whether the [32, 64] rows of [layers, tokens, 32, 64] do not overlap: one of the two dimensions within the other."""
+    over, within = strides[0], strides[1]
+    if layers < 2 or tokens < 2:
+        return (layers < 2 or over >= _ROW) and (tokens < 2 or within >= _ROW)
+    if over < within:
+        over, within, tokens = within, over, layers
+    return within >= _ROW and over >= (tokens - 1) * within + _ROW
+
+
+def _span(tensor: Tensor) -> tuple[int, int]:
+    """First address and the one past the last of a tensor without negative strides."""
+    reach = sum((n - 1) * stride for n, stride in zip(tensor.shape, tensor.stride())) + 1
+    return tensor.data_ptr(), tensor.data_ptr() + reach * tensor.element_size()
+
+
+def _mixes(query: Tensor, out: Tensor) -> bool:
+    """Whether a row of ``out`` may be written before another row of ``query`` that it overlaps is read."""
+    if query.data_ptr() == out.data_ptr() and query.stride() == out.stride() and query.dtype == out.dtype:
+        return False  # in place
+    first, last = _span(query)
+    begin, end = _span(out)
+    return begin < last and first < end
+
+
 def _dense(tensor: Tensor) -> Tensor:
     """A copy in contiguous, 16-byte aligned storage (``contiguous()`` keeps an unaligned tensor)."""
     return tensor.clone(memory_format=torch.contiguous_format)
@@ -448,13 +473,12 @@ def append_kv(
         elif (
             query_out.shape != query.shape
             or not _rows_ok(query_out, query_out.stride())
-            or (tokens > 1 and query_out.stride(1) < _ROW)
-            or (layers > 1 and query_out.stride(0) < _ROW)
+            or not _rows_apart(query_out.stride(), layers, tokens)
         ):
             raise ValueError("query_out must be [layers, tokens, 32, 64] with contiguous, 16-byte aligned rows")
         elif query_out.dtype not in (_HALF, _FLOAT) or query_out.get_device() != index:
             raise ValueError(f"query_out must be FP16 or FP32 on cuda:{index}")
-        if not _rows_ok(query, query.stride()):
+        if not _rows_ok(query, query.stride()) or _mixes(query, query_out):
             query = _dense(query)
         q_ptr, out_ptr = query.data_ptr(), query_out.data_ptr()
         q_strides, out_strides = query.stride()[:2], query_out.stride()[:2]
