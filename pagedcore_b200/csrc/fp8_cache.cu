@@ -351,9 +351,8 @@ constexpr int kReadThreads = 256;
 constexpr int64_t kBlockValues = kSlots * kHeads * kDim;
 
 __global__ void __launch_bounds__(kReadThreads)
-    fp8_read_kernel(const pkv::fp8::Cache cache, int layer, const int32_t *__restrict__ blocks,
-                    __half *__restrict__ key_out, __half *__restrict__ value_out, int32_t *__restrict__ index_out,
-                    int32_t *error_flag) {
+    fp8_read_kernel(const pkv::fp8::Cache cache, int layer, const int32_t *blocks, __half *key_out, __half *value_out,
+                    int32_t *index_out, int32_t *error_flag) {
     __shared__ __align__(16) __half turned[kHeads][kSlots][kDim + 8];
     pkv::pdl_launch_dependents();
     pkv::pdl_wait();

@@ -371,10 +371,11 @@ struct RowsShape {
     static constexpr int kSmem = kRing + kEpilogueWarps * kStoreBytes + 1024;
 };
 
-// v[j] = p[at + j] for the indexes below `count`.
+// v[j] = p[at + j] for the indexes below `count`.  (Plain loads: the kernel before this one,
+// which writes the scales of x, may still run while this one is set up.)
 __device__ __forceinline__ void load_group(const float *p, int at, int count, float (&v)[4]) {
 #pragma unroll
-    for (int j = 0; j < 4; ++j) v[j] = at + j < count ? __ldg(p + at + j) : 0.f;
+    for (int j = 0; j < 4; ++j) v[j] = at + j < count ? p[at + j] : 0.f;
 }
 
 // acc[j] += (d[2 j], d[2 j + 1]) * f for 32 columns.
@@ -856,14 +857,14 @@ __global__ void __launch_bounds__(PairShape::kThreads, 1)
             // Below 2^32: with more than one K block a row has 72 codes or more a scale.
             uint32_t sx = static_cast<uint32_t>(min(m0 + quarter * 32 + lane, a.rows - 1)) * count;
             uint32_t sw = static_cast<uint32_t>(min((n0 + first) / kTileRows, a.w_blocks - 1)) * count;
-            float x = __ldg(a.x_scales + sx), w = __ldg(a.w_scales + sw);  // a K block ahead
+            float x = a.x_scales[sx], w = a.w_scales[sw];  // a K block ahead
 #pragma unroll
             for (int c = 0; c < 32; ++c) acc[c] = 0;
 #pragma unroll 1
             for (int i = 1; i <= count; ++i) {
                 const float f = x * w;
                 const uint64_t f2 = pkv::f32x2(f, f);
-                if (i < count) x = __ldg(a.x_scales + ++sx), w = __ldg(a.w_scales + ++sw);
+                if (i < count) x = a.x_scales[++sx], w = a.w_scales[++sw];
                 const int buf = done & 1;
                 if (ok) ok = wait_bounded(pkv::smem_addr(&tmem_full[buf]), (done >> 1) & 1, a.error_flag);
                 ok = __all_sync(0xffffffffu, ok);

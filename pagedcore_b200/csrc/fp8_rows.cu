@@ -64,16 +64,18 @@ __device__ __forceinline__ uint2 encode_group(const float (&y)[kChunk], float &s
                       pkv::fp8::encode2(s[4], s[5]) | (pkv::fp8::encode2(s[6], s[7]) << 16));
 }
 
+// (No __restrict__ on the inputs below: it promises that they do not change while the kernel
+// runs, but a kernel launched early runs beside the one that writes them, and the norm's
+// residual may be hidden or delta itself.  A thread reads all of its row before it writes.)
+
 // One CTA per row; thread c holds chunk c (+ 256 ...) of the row.
 template <int CHUNKS>
-__global__ void __launch_bounds__(kThreads) norm_kernel(const __half *__restrict__ hidden,
-                                                        const __half *__restrict__ delta,
-                                                        const __half *__restrict__ weight, __half *__restrict__ residual,
-                                                        uint8_t *__restrict__ codes, float *__restrict__ scales,
-                                                        int dim, int groups, float eps) {
+__global__ void __launch_bounds__(kThreads) norm_kernel(const __half *hidden, const __half *delta, const __half *weight,
+                                                        __half *residual, uint8_t *codes, float *scales, int dim,
+                                                        int groups, float eps) {
     __shared__ float partial[kThreads / 32];
     const int chunks = dim / kChunk;
-    uint4 wraw[CHUNKS];
+    uint4 wraw[CHUNKS], hraw[CHUNKS], draw[CHUNKS];
     pkv::pdl_launch_dependents();
     pkv::pdl_wait();
     const int64_t base = static_cast<int64_t>(blockIdx.x) * dim;
@@ -82,12 +84,21 @@ __global__ void __launch_bounds__(kThreads) norm_kernel(const __half *__restrict
 #pragma unroll
     for (int j = 0; j < CHUNKS; ++j) {
         const int c = threadIdx.x + j * kThreads;
+        wraw[j] = hraw[j] = draw[j] = make_uint4(0, 0, 0, 0);
         if (c < chunks) {
             wraw[j] = *reinterpret_cast<const uint4 *>(weight + c * kChunk);
-            unpack8(*reinterpret_cast<const uint4 *>(hidden + base + c * kChunk), v[j]);
+            hraw[j] = *reinterpret_cast<const uint4 *>(hidden + base + c * kChunk);
+            if (delta != nullptr) draw[j] = *reinterpret_cast<const uint4 *>(delta + base + c * kChunk);
+        }
+    }
+#pragma unroll
+    for (int j = 0; j < CHUNKS; ++j) {
+        const int c = threadIdx.x + j * kThreads;
+        if (c < chunks) {
+            unpack8(hraw[j], v[j]);
             if (delta != nullptr) {
                 float d[kChunk];
-                unpack8(*reinterpret_cast<const uint4 *>(delta + base + c * kChunk), d);
+                unpack8(draw[j], d);
                 uint4 rraw;
                 __half2 *r = reinterpret_cast<__half2 *>(&rraw);
 #pragma unroll
@@ -101,7 +112,6 @@ __global__ void __launch_bounds__(kThreads) norm_kernel(const __half *__restrict
         } else {
 #pragma unroll
             for (int i = 0; i < kChunk; ++i) v[j][i] = 0.f;
-            wraw[j] = make_uint4(0, 0, 0, 0);
         }
     }
 #pragma unroll
@@ -132,9 +142,8 @@ __global__ void __launch_bounds__(kThreads) norm_kernel(const __half *__restrict
 // y = x, or with SILU y = silu(x[.., c]) * x[.., width + c]: 16 lanes a group,
 // groups of a row along x, rows along y.
 template <bool SILU>
-__global__ void __launch_bounds__(kThreads) encode_kernel(const __half *__restrict__ x, int64_t stride, int rows,
-                                                          int width, int groups, uint8_t *__restrict__ codes,
-                                                          float *__restrict__ scales) {
+__global__ void __launch_bounds__(kThreads) encode_kernel(const __half *x, int64_t stride, int rows, int width,
+                                                          int groups, uint8_t *codes, float *scales) {
     pkv::pdl_launch_dependents();
     pkv::pdl_wait();
     const int c = blockIdx.x * kThreads + threadIdx.x;
@@ -165,9 +174,8 @@ __global__ void __launch_bounds__(kThreads) encode_kernel(const __half *__restri
     }
 }
 
-__global__ void __launch_bounds__(kThreads) to_half_kernel(const uint8_t *__restrict__ codes,
-                                                           const float *__restrict__ scales, int rows, int width,
-                                                           int groups, __half *__restrict__ out, int64_t out_stride) {
+__global__ void __launch_bounds__(kThreads) to_half_kernel(const uint8_t *codes, const float *scales, int rows,
+                                                           int width, int groups, __half *out, int64_t out_stride) {
     pkv::pdl_launch_dependents();
     pkv::pdl_wait();
     const int c = blockIdx.x * kThreads + threadIdx.x;

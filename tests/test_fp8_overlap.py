@@ -63,3 +63,50 @@ def test_a_query_rotated_over_its_neighbours_is_rotated_right() -> None:
         fp8.append_kv(case.cache, two(key), two(value), slots, query=two(query), query_out=out, **(arguments | {"layer_begin": 0}))
         assert torch.equal(out[0], expected[0]) and torch.equal(out[1], expected[0])
     assert int(case.flag.item()) == 0
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("rows, dim", [(3, 200), (64, 2048), (5, 4104), (9, 8192)])
+def test_a_norms_residual_may_be_either_input(rows, dim) -> None:
+    from tests.test_fp8_gpu import randn
+
+    weight = randn(190, dim).half()
+    hidden, delta = randn(191, rows, dim).half(), randn(192, rows, dim).half()
+    expected = torch.empty_like(hidden)
+    out = fp8.add_rms_norm(hidden, delta, weight, residual=expected)
+    for which in (0, 1):
+        inputs = [hidden.clone(), delta.clone()]
+        again = fp8.add_rms_norm(*inputs, weight, residual=inputs[which])
+        assert torch.equal(inputs[which], expected) and torch.equal(inputs[1 - which], (hidden, delta)[1 - which])
+        assert torch.equal(again.codes.view(torch.uint8), out.codes.view(torch.uint8)) and torch.equal(again.scales, out.scales)
+
+
+@pytest.mark.gpu
+def test_a_chain_of_early_launches_reads_what_was_just_written() -> None:
+    """Norm, product, SwiGLU and product again in the same storage, step after step, back to back and apart."""
+    from tests.test_fp8_gpu import randn
+
+    weight = torch.ones(512, dtype=torch.float16, device="cuda")
+    up, down = fp8.quantize_weight(0.05 * randn(193, 2048, 512)), fp8.quantize_weight(0.05 * randn(194, 512, 1024))
+
+    def chain(hidden: torch.Tensor, steps: int, wait: bool) -> torch.Tensor:
+        hidden = hidden.clone()
+        delta = torch.zeros_like(hidden)
+        for _ in range(steps):
+            rows = fp8.add_rms_norm(hidden, delta, weight)
+            if wait:
+                torch.cuda.synchronize()
+            gate_up = fp8.linear(rows, up)
+            if wait:
+                torch.cuda.synchronize()
+            act = fp8.silu_mul(gate_up)
+            if wait:
+                torch.cuda.synchronize()
+            fp8.linear(act, down, delta)
+            if wait:
+                torch.cuda.synchronize()
+        return hidden
+
+    for count in (1, 20, 100, 700):
+        hidden = randn(195 + count, count, 512).half()
+        assert torch.equal(chain(hidden, 30, False), chain(hidden, 30, True))
