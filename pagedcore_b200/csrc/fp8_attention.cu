@@ -52,15 +52,6 @@
 #include "ptx.cuh"
 #include "status.h"
 
-namespace pkv::fp8 {
-int check_cache(const void *key_codes, const void *value_codes, const void *key_scales, const void *value_scales,
-                int32_t layers, int32_t num_blocks, int32_t layer_begin, int32_t layer_count);
-int launch_decode_append(const Cache &cache, int32_t layer, const void *key, const void *value, int64_t kv_stride,
-                         const void *rope_table, const void *query, int64_t query_stride, void *query_out, void *query_low,
-                         const int32_t *lengths, const int32_t *prefix, const int32_t *flat, int32_t batch,
-                         int32_t total_blocks, int32_t *error_flag, cudaStream_t stream);
-}
-
 namespace {
 
 constexpr int kDim = PKV_HEAD_DIM;
@@ -818,13 +809,6 @@ int decode(const pkv::fp8::Cache &cache, int32_t layer, const void *query, int64
     return PKV_OK;
 }
 
-pkv::fp8::Cache cache_of(const void *key_codes, const void *value_codes, const void *key_scales,
-                         const void *value_scales, int32_t layers, int32_t num_blocks) {
-    return {static_cast<uint8_t *>(const_cast<void *>(key_codes)), static_cast<uint8_t *>(const_cast<void *>(value_codes)),
-            static_cast<float *>(const_cast<void *>(key_scales)), static_cast<float *>(const_cast<void *>(value_scales)),
-            layers, num_blocks};
-}
-
 // The same with the append before it; clear: rows without blocks give zeros.
 int decode_layer(const pkv::fp8::Cache &cache, int32_t layer, const void *query, int64_t query_stride, const void *key,
                  const void *value, int64_t kv_stride, const void *rope_table, bool clear, const int32_t *lengths,
@@ -847,7 +831,7 @@ extern "C" int pkv_fp8_decode_attention(const void *key_codes, const void *value
                                         int32_t grid, void *out, int64_t out_stride, void *workspace,
                                         int64_t workspace_bytes, int32_t *error_flag, void *stream) {
     pkv::clear_error();
-    return decode(cache_of(key_codes, value_codes, key_scales, value_scales, layers, num_blocks), layer, query,
+    return decode(pkv::fp8::cache_of(key_codes, value_codes, key_scales, value_scales, layers, num_blocks), layer, query,
                   query_stride, nullptr, nullptr, 0, nullptr, true, lengths, prefix, flat, batch, total_blocks, grid,
                   out, out_stride, workspace, workspace_bytes, error_flag, static_cast<cudaStream_t>(stream));
 }
@@ -859,7 +843,7 @@ extern "C" int pkv_fp8_decode_layer(void *key_codes, void *value_codes, void *ke
                                     const int32_t *flat, int32_t batch, int32_t total_blocks, int32_t grid, void *out,
                                     int64_t out_stride, void *workspace, int64_t workspace_bytes, int32_t *error_flag,
                                     void *stream) {
-    return decode_layer(cache_of(key_codes, value_codes, key_scales, value_scales, layers, num_blocks), layer, query,
+    return decode_layer(pkv::fp8::cache_of(key_codes, value_codes, key_scales, value_scales, layers, num_blocks), layer, query,
                         query_stride, key, value, kv_stride, rope_table, false, lengths, prefix, flat, batch, total_blocks,
                         grid, out, out_stride, workspace, workspace_bytes, error_flag, static_cast<cudaStream_t>(stream));
 }
@@ -871,7 +855,7 @@ extern "C" int pkv_fp8_decode_layer_zero(void *key_codes, void *value_codes, voi
                                          const int32_t *flat, int32_t batch, int32_t total_blocks, int32_t grid, void *out,
                                          int64_t out_stride, void *workspace, int64_t workspace_bytes, int32_t *error_flag,
                                          void *stream) {
-    return decode_layer(cache_of(key_codes, value_codes, key_scales, value_scales, layers, num_blocks), layer, query,
+    return decode_layer(pkv::fp8::cache_of(key_codes, value_codes, key_scales, value_scales, layers, num_blocks), layer, query,
                         query_stride, key, value, kv_stride, rope_table, true, lengths, prefix, flat, batch, total_blocks,
                         grid, out, out_stride, workspace, workspace_bytes, error_flag, static_cast<cudaStream_t>(stream));
 }

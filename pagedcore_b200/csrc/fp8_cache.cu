@@ -26,6 +26,7 @@
 
 #include "fp8_cache.cuh"
 #include "pdl.h"
+#include "prefill_attention.h"
 #include "ptx.cuh"
 #include "status.h"
 
@@ -419,27 +420,12 @@ __global__ void __launch_bounds__(kReadThreads) fp8_save_kernel(const pkv::fp8::
     if (threadIdx.x < 2) copy((threadIdx.x ? cache.value_scales : cache.key_scales) + tile, 2 * kCodes + threadIdx.x, 0);
 }
 
-pkv::fp8::Cache cache_of(const void *key_codes, const void *value_codes, const void *key_scales,
-                         const void *value_scales, int32_t layers, int32_t num_blocks) {
-    return {static_cast<uint8_t *>(const_cast<void *>(key_codes)), static_cast<uint8_t *>(const_cast<void *>(value_codes)),
-            static_cast<float *>(const_cast<void *>(key_scales)), static_cast<float *>(const_cast<void *>(value_scales)),
-            layers, num_blocks};
-}
-
 bool aligned16(const void *p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
 
 }  // namespace
 
-namespace pkv {
-int launch_prefill_attention_tc(const void *pool, int32_t num_blocks, int32_t layer, const void *query,
-                                bool query_fp32, bool fine, int64_t query_stride, const int32_t *blocks,
-                                int32_t start, int32_t tokens, void *out, int64_t out_stride, int32_t *error_flag,
-                                cudaStream_t stream);
-}
-
 namespace pkv::fp8 {
 
-// The checks of a cache that every entry point makes.
 int check_cache(const void *key_codes, const void *value_codes, const void *key_scales, const void *value_scales,
                 int32_t layers, int32_t num_blocks, int32_t layer_begin, int32_t layer_count) {
     if (key_codes == nullptr || value_codes == nullptr || key_scales == nullptr || value_scales == nullptr) {
@@ -457,8 +443,6 @@ int check_cache(const void *key_codes, const void *value_codes, const void *key_
     return PKV_OK;
 }
 
-// The new token of every row of a staged batch at `layer`: K rotated and V written, Q
-// rotated to query_out + query_low (FP16 numbers that add up to half of the FP32 value).
 int launch_decode_append(const Cache &cache, int32_t layer, const void *key, const void *value, int64_t kv_stride,
                          const void *rope_table, const void *query, int64_t query_stride, void *query_out, void *query_low,
                          const int32_t *lengths, const int32_t *prefix, const int32_t *flat, int32_t batch,
@@ -518,8 +502,7 @@ extern "C" int pkv_fp8_append_kv(void *key_codes, void *value_codes, void *key_s
     if (layer_count > 65535) return pkv::fail(PKV_VALUE_ERROR, "fp8 append: layers out of range");
     if (tokens == 0) return PKV_OK;
     AppendArgs a = {};
-    a.cache = {static_cast<uint8_t *>(key_codes), static_cast<uint8_t *>(value_codes), static_cast<float *>(key_scales),
-               static_cast<float *>(value_scales), layers, num_blocks};
+    a.cache = pkv::fp8::cache_of(key_codes, value_codes, key_scales, value_scales, layers, num_blocks);
     a.layer_begin = layer_begin;
     a.key = static_cast<const __half *>(key);
     a.value = static_cast<const __half *>(value);
@@ -564,7 +547,7 @@ int read_blocks(const void *key_codes, const void *value_codes, const void *key_
     if (count == 0) return PKV_OK;
     const cudaError_t e = pkv::launch_pdl(
         fp8_read_kernel, dim3(count), dim3(kReadThreads), static_cast<cudaStream_t>(stream),
-        cache_of(key_codes, value_codes, key_scales, value_scales, layers, num_blocks), layer, blocks,
+        pkv::fp8::cache_of(key_codes, value_codes, key_scales, value_scales, layers, num_blocks), layer, blocks,
         static_cast<__half *>(key_out), static_cast<__half *>(value_out), index_out, error_flag);
     if (e != cudaSuccess) return pkv::fail(PKV_CUDA_ERROR, std::string("fp8 read launch failed: ") + cudaGetErrorString(e));
     return PKV_OK;
@@ -597,7 +580,7 @@ extern "C" int pkv_fp8_save_blocks(void *key_codes, void *value_codes, void *key
     if (count == 0) return PKV_OK;
     const cudaError_t e = pkv::launch_pdl(restore ? fp8_save_kernel<true> : fp8_save_kernel<false>, dim3(count, layers),
                                           dim3(kReadThreads), static_cast<cudaStream_t>(stream),
-                                          cache_of(key_codes, value_codes, key_scales, value_scales, layers, num_blocks),
+                                          pkv::fp8::cache_of(key_codes, value_codes, key_scales, value_scales, layers, num_blocks),
                                           slots, static_cast<uint8_t *>(saved));
     if (e != cudaSuccess) return pkv::fail(PKV_CUDA_ERROR, std::string("fp8 save launch failed: ") + cudaGetErrorString(e));
     return PKV_OK;

@@ -16,14 +16,8 @@
 #include <string>
 
 #include "pagedkv.h"
+#include "prefill_attention.h"
 #include "status.h"
-
-namespace pkv {
-int launch_prefill_attention_tc(const void *pool, int32_t num_blocks, int32_t layer, const void *query,
-                                bool query_fp32, bool fine, int64_t query_stride, const int32_t *blocks,
-                                int32_t start, int32_t tokens, void *out, int64_t out_stride, int32_t *error_flag,
-                                cudaStream_t stream);
-}
 
 extern "C" int pkv_prefill_attention(const void *pool, int32_t num_blocks, int32_t layer, const void *query,
                                      int64_t query_stride, const int32_t *blocks, int32_t start, int32_t tokens,

@@ -81,6 +81,7 @@
 #include "fp8.cuh"
 #include "pagedkv.h"
 #include "pdl.h"
+#include "prefill_attention.h"
 #include "ptx.cuh"
 #include "status.h"
 #include "tcgen05.cuh"
@@ -772,9 +773,6 @@ int launch(const TcArgs &args, cudaStream_t stream) {
 
 namespace pkv {
 
-// Launch of the tcgen05 prefill attention (arguments checked by the caller); the query FP16
-// or, with query_fp32, FP32.  fine: over the 8-bit cache's values, behind the kernel that
-// reads them (query_fp32 needs it).
 int launch_prefill_attention_tc(const void *pool, int32_t num_blocks, int32_t layer, const void *query,
                                 bool query_fp32, bool fine, int64_t query_stride, const int32_t *blocks, int32_t start,
                                 int32_t tokens, void *out, int64_t out_stride, int32_t *error_flag,
