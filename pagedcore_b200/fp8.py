@@ -385,18 +385,18 @@ def _rows_apart(strides: tuple[int, ...], layers: int, tokens: int) -> bool:
     return within >= _ROW and over >= (tokens - 1) * within + _ROW
 
 
-def _span(tensor: Tensor) -> tuple[int, int]:
-    """First address and the one past the last of a tensor without negative strides."""
-    reach = sum((n - 1) * stride for n, stride in zip(tensor.shape, tensor.stride())) + 1
-    return tensor.data_ptr(), tensor.data_ptr() + reach * tensor.element_size()
-
-
 def _mixes(query: Tensor, out: Tensor) -> bool:
-    """Whether a row of ``out`` may be written before another row of ``query`` that it overlaps is read."""
-    if query.data_ptr() == out.data_ptr() and query.stride() == out.stride() and query.dtype == out.dtype:
-        return False  # in place
-    first, last = _span(query)
-    begin, end = _span(out)
+    """Whether a row of ``out`` may be written before another row of ``query`` that it overlaps is read.
+
+    Both [layers, tokens, 32, 64] with contiguous rows, the query FP16; in place is fine.
+    """
+    layers, tokens = query.shape[0] - 1, query.shape[1] - 1
+    first, strides = query.data_ptr(), query.stride()
+    begin, over = out.data_ptr(), out.stride()
+    if first == begin and strides == over and out.dtype is _HALF:
+        return False
+    last = first + 2 * (layers * strides[0] + tokens * strides[1] + _ROW)
+    end = begin + out.element_size() * (layers * over[0] + tokens * over[1] + _ROW)
     return begin < last and first < end
 
 
@@ -468,7 +468,8 @@ def append_kv(
         if query.shape != (layers, tokens, _QUERY_HEADS, _HEAD_DIM):
             raise ValueError("query must be FP16 [layers, tokens, 32, 64]")
         _half("query", query, index)
-        if query_out is None:
+        given = query_out is not None
+        if not given:
             query_out = torch.empty_like(query, dtype=_FLOAT, memory_format=torch.contiguous_format)
         elif (
             query_out.shape != query.shape
@@ -478,7 +479,7 @@ def append_kv(
             raise ValueError("query_out must be [layers, tokens, 32, 64] with contiguous, 16-byte aligned rows")
         elif query_out.dtype not in (_HALF, _FLOAT) or query_out.get_device() != index:
             raise ValueError(f"query_out must be FP16 or FP32 on cuda:{index}")
-        if not _rows_ok(query, query.stride()) or _mixes(query, query_out):
+        if not _rows_ok(query, query.stride()) or (given and _mixes(query, query_out)):
             query = _dense(query)
         q_ptr, out_ptr = query.data_ptr(), query_out.data_ptr()
         q_strides, out_strides = query.stride()[:2], query_out.stride()[:2]
