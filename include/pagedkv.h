@@ -468,7 +468,10 @@ int pkv_fp8_decode_plan(int32_t device, int32_t batch, int32_t total_blocks, int
 
 /* pkv_decode_attention over the 8-bit cache: query (rotated), lengths, prefix,
  * flat and out as there; a row without blocks (prefix[b + 1] == prefix[b]) or
- * without valid tokens gives zeros.  The batch's blocks are prefix[batch], read
+ * without valid tokens gives zeros.  Block ids outside the cache set
+ * PKV_DEVICE_BAD_BLOCK and read as zeros; a prefix that falls or does not begin
+ * at 0 sets it too (the rows' outputs are then anything, and nothing else is
+ * written).  The batch's blocks are prefix[batch], read
  * on the device; total_blocks is the room of flat, which it must not exceed, so
  * a captured launch serves any batch within it.  grid: the plan's for this
  * batch and block count, or any other; workspace (16-byte aligned, of at least

@@ -296,7 +296,8 @@ __device__ void rotate_queries(const AppendArgs &a, int layer, int begin, int wa
     }
 }
 
-// The grid for `tokens`: eight tokens a CTA (of a prompt every sixteenth opens a run) once there are enough CTAs to fill the SMs.
+// The grid for `tokens`: eight tokens a CTA (of a prompt every sixteenth opens a run) from 512
+// tokens on, where a single layer still gives 64 CTAs or more; several layers have a grid row each.
 dim3 append_grid(AppendArgs &a, int layers) {
     a.span = a.lengths == nullptr && a.tokens >= 512 ? 8 : 1;
     a.tile_ctas = (a.tokens + a.span - 1) / a.span;
@@ -588,10 +589,10 @@ extern "C" int pkv_fp8_save_blocks(void *key_codes, void *value_codes, void *key
 
 // The request's blocks become an FP16 pool of one layer in the workspace (the values are
 // FP16 numbers: nothing is rounded), which the tensor-core prompt kernel attends to.  That
-// kernel reads every block once for each 16 queries, so the conversion is a small part: 2 us
-// at 2047 tokens.  (The prompt kernel's producers reading codes and converting them, every
-// block as often as there are 16 queries behind it: 74 to 85 us against 58 for append, attention
-// and read of 2047 tokens, 29 against 24 for 75 behind 601.)
+// kernel reads every block once for each 16 queries, so the conversion is a small part: 2 of
+// 53 us at 2047 tokens.  (The prompt kernel's producers reading codes and converting them, every
+// block as often as there are 16 queries behind it, took 16 to 27 us more for 2047 tokens, 5 for
+// 75 behind 601.)
 extern "C" int pkv_fp8_prefill_attention(const void *key_codes, const void *value_codes, const void *key_scales,
                                          const void *value_scales, int32_t layers, int32_t num_blocks, int32_t layer,
                                          const void *query, int32_t query_fp32, int64_t query_stride,

@@ -3,23 +3,22 @@
 // with E4M3 codes x [rows][k] and w [n][k] and FP32 scales per row of x and
 // 128 values, and per 128 x 128 block of w.
 //
-// The weight is the MMA's M side (128 weight rows a tile), the rows of x its N
-// side (NT a tile, 16 to 256): at decode the weight is the large operand and is
-// read once.  One K block of 128 is four tcgen05.mma (kind::f8f6f4, K = 32)
+// To 64 rows the weight is the MMA's M side (128 weight rows a tile) and the rows
+// of x its N side (all of them one tile of NT = 16, 32 or 64): at decode the weight
+// is the large operand and is read once.  (More rows: the two kernels below.)  One K block of 128 is four tcgen05.mma (kind::f8f6f4, K = 32)
 // into a TMEM buffer of its own; the scales differ from block to block, so a
 // block's sums are read back and added into FP32 registers times sx * sw (sw is
 // one number for the tile and block, sx one per column).  Two TMEM buffers let
 // the tensor cores work on the next block meanwhile.
 //
-// Work split: one CTA per (128 weight rows, NT rows of x); where that leaves
+// Work split: one CTA per 128 weight rows; where that leaves
 // SMs idle the K blocks of a tile are dealt to the 2, 4 or 8 CTAs of a cluster,
 // which add their FP32 sums through distributed shared memory in rank order and
 // write FP16: one launch, and results that do not depend on timing.
 //
-// Roles: warps 0 .. E-1 read TMEM, scale and add (warp w reads lanes
-// 32 (w % 4) .. and with E = 8 half of the columns); warp E loads by TMA (one
-// 128-byte swizzled box of each operand a stage, no multicast); warp E + 1 owns
-// the TMEM allocation and issues the MMAs.  Every wait is bounded; one that
+// Roles: warps 0 to 3 read TMEM, scale and add (warp w lanes 32 w ..); warp 4
+// loads by TMA (one 128-byte swizzled box of each operand a stage, no multicast);
+// warp 5 owns the TMEM allocation and issues the MMAs.  Every wait is bounded; one that
 // runs out sets PKV_DEVICE_WAIT_TIMEOUT, and the CTA goes on without waiting so
 // that no barrier is left short.
 
@@ -1142,9 +1141,11 @@ extern "C" int pkv_fp8_linear(const void *x, int64_t x_stride, const void *x_sca
     if (rows <= 32) return launch_few<32>(device, x, x_stride, w, k, sms, args, s);
     if (rows <= 64) return launch_few<64>(device, x, x_stride, w, k, sms, args, s);
     // Tile shape by the time of the busiest SM: rounds of tiles, times the K blocks of a
-    // CTA, times the clocks that a K block was measured to take (the chain of waits,
-    // TMEM reads and scaled sums, more than the MMAs' 2 N clocks): 700 / 800 / 1000 at
-    // N = 64 / 128 / 192, and 1100 for a pair's 256 x 256.
+    // CTA, times the clocks that a K block was measured to take: 700 / 800 / 1000 at
+    // N = 64 / 128 / 192, and 1100 for a pair's 256 x 256.  Up to 192 that is mostly the
+    // transfer of the block's 24 / 32 / 40 KiB from L2, 35 to 41 bytes a clock and SM: the
+    // loads alone, without MMAs, TMEM reads and sums, take 9.4 of 12.0 us at 256 x 11264 x
+    // 2048 (rows x n x k) and 15.6 of 20.5 at 512 rows.
     const int64_t m_tiles = (rows + kTileRows - 1) / kTileRows;
     const int64_t pair_rounds = (static_cast<int64_t>((rows + 255) / 256) * ((n + 255) / 256) + sms / 2 - 1) / (sms / 2);
     int best = 256;

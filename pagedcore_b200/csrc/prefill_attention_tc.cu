@@ -60,7 +60,7 @@
 //   mostly hidden behind the softmax) and is scaled back by the power of two, exactly.
 // - What the FP16 weights leave goes over the second 32 columns of S_g's buffer, and P.V
 //   takes both.  (One FP16 number for each weight: relative error 2.9e-4 where the output's
-//   rounding alone gives 2.0e-4.)
+//   rounding alone gives 2.0e-4, and 43 us for 2047 tokens with their read; 53 with two.)
 // - The reference is m - 7 and moves when a weight would pass 2^15; past 2^20, where 7 would
 //   soon be lost in its rounding, it is m itself.
 //

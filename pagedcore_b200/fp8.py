@@ -213,7 +213,10 @@ def _quantize(x: Tensor, width: int, silu_pairs: bool) -> Fp8Rows:
 
 
 def quantize_rows(x: Tensor) -> Fp8Rows:
-    """FP16 [rows, width] (rows contiguous, any row stride that is a multiple of 8) as 8-bit rows."""
+    """FP16 [rows, width] (rows contiguous, any row stride that is a multiple of 8) as 8-bit rows.
+
+    Any width that is a multiple of 8; ``linear`` takes those of 16.
+    """
     if x.ndim != 2 or x.dtype != torch.float16 or (x.numel() and x.stride(1) != 1):
         raise ValueError("x must be FP16 [rows, width] with contiguous rows")
     return _quantize(x, x.shape[1], False)
@@ -285,7 +288,9 @@ class Fp8Cache:
     """An 8-bit KV cache: E4M3 codes and FP32 scales.
 
     key_codes [layers, blocks, 4, 16, 64], value_codes [layers, blocks, 4, 64, 16]
-    (V is held transposed), key_scales and value_scales [layers, blocks, 4].
+    (V is held transposed), key_scales and value_scales [layers, blocks, 4],
+    powers of two from 2^-15 to 2^8 as ``append_kv`` makes them (the decode
+    attention takes V's scale as an exponent).
     A slot id is physical_block * 16 + slot_in_block, as in the FP16 pool.
     """
 
