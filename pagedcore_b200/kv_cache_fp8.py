@@ -121,6 +121,8 @@ class Fp8KVAllocator(KVAllocator):
         query, query_stride = fp8._query_rows(query)
         key, value, strides = fp8._aligned_pair(key, value)
         to = self._aligned_out(out)
+        if to is not out:
+            to.copy_(out)  # rows past the batch are left alone
         check(
             lib.pkv_fp8_decode_layer(
                 *cache, layer, query.data_ptr(), query_stride, key.data_ptr(), value.data_ptr(), strides[0], rope,

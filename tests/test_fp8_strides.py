@@ -122,6 +122,30 @@ def test_a_decode_layer_and_attention_of_any_strides_give_the_same() -> None:
 
 
 @pytest.mark.gpu
+def test_a_step_graph_leaves_rows_past_the_batch_alone_in_an_unaligned_output() -> None:
+    from pagedcore_b200.graph import DecodeStepGraph
+    from tests.test_fp8_decoder_gpu import admit, make_allocator
+    from tests.test_fp8_gpu import randn
+
+    outs = []
+    for offset in (0, 2):
+        allocator = make_allocator(12)
+        requests = admit(allocator, 3, 3)
+        for i, request in enumerate(requests):
+            allocator.append(request, randn(460 + i, 22, 20, 4, 64).half(), randn(465 + i, 22, 20, 4, 64).half())
+        q, k, v = (randn(470 + heads, 22, 5, heads, 64).half() for heads in (32, 4, 4))
+        out = torch.full((22 * 5 * ROW + 8,), 5.0, dtype=torch.float16, device=q.device)[offset : offset + 22 * 5 * ROW]
+        out = out.view(22, 5, 32, 64)
+        graph = DecodeStepGraph(allocator, rows=5)
+        for step in range(2):
+            graph.step(q, k, v, out, requests)
+            assert bool((out[:, 2:] == 5).all())
+        allocator.check_device_errors()
+        outs.append(out[:, :2])
+    assert torch.equal(*outs)
+
+
+@pytest.mark.gpu
 def test_operators_copy_what_is_contiguous_but_not_aligned() -> None:
     from tests.test_fp8_gpu import LAYER, CacheCase, randn
 
