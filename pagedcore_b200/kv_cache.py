@@ -821,8 +821,13 @@ class KVAllocator:
             key, value = key.contiguous(), value.contiguous()
         if out is None:
             out = torch.empty((count, 32, 64), dtype=torch.float16, device=self._pool.device)
-        elif out.shape != (count, 32, 64) or out.dtype != torch.float16 or out.stride()[1:] != (64, 1):
-            raise ValueError("out must be FP16 [batch, 32, 64] with contiguous rows")
+        elif (
+            out.shape != (count, 32, 64)
+            or out.dtype != torch.float16
+            or out.stride()[1:] != (64, 1)
+            or out.device != self._pool.device
+        ):
+            raise ValueError("out must be FP16 [batch, 32, 64] with contiguous rows, on the pool device")
         fixed = staged.launch_args
         if fixed is None:
             batch = self.staged_decode_batch()

@@ -146,6 +146,32 @@ def test_a_step_graph_leaves_rows_past_the_batch_alone_in_an_unaligned_output() 
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("kind", ["fp16", "fp8"])
+def test_a_decode_layers_output_elsewhere_is_refused(kind) -> None:
+    from pagedcore_b200.kv_cache import KVAllocator
+    from tests.test_fp8_decoder_gpu import admit, make_allocator
+    from tests.test_fp8_gpu import randn
+
+    if kind == "fp8":
+        allocator = make_allocator(4)
+    else:
+        allocator = KVAllocator(torch.zeros(22, 2, 4, 16, 4, 64, dtype=torch.float16, device="cuda:0"))
+    (request,) = admit(allocator, 2)
+    allocator.append(request, randn(480, 22, 5, 4, 64).half(), randn(481, 22, 5, 4, 64).half())
+    q, k, v = (randn(482 + heads, 1, heads, 64).half() for heads in (32, 4, 4))
+    with pytest.raises(ValueError, match="out must be"):
+        with allocator.append_decode((request,)):
+            allocator.decode_layer(0, q, k, v, out=half(1, 32, 64))
+    if kind == "fp8":
+        batch = allocator.decode_batch((request,), layer_index=0)
+        for out in (half(1, 32, 64), half(9 * ROW)[2 : 2 + ROW].view(1, 32, 64)):
+            with pytest.raises(ValueError, match="out must be"):
+                allocator.attend(batch, q, layer_index=0, out=out)
+    assert allocator.cached_length(request) == 5
+    allocator.check_device_errors()
+
+
+@pytest.mark.gpu
 def test_operators_copy_what_is_contiguous_but_not_aligned() -> None:
     from tests.test_fp8_gpu import LAYER, CacheCase, randn
 
