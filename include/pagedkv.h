@@ -505,6 +505,69 @@ int pkv_fp8_decode_layer_zero(void *key_codes, void *value_codes, void *key_scal
                               int32_t total_blocks, int32_t grid, void *out, int64_t out_stride, void *workspace,
                               int64_t workspace_bytes, int32_t *error_flag, void *stream);
 
+/* ---- 4-bit KV cache ------------------------------------------------------------
+ * Groups of 16 consecutive dims of one token and head: 16 codes of 4 bits, -7 .. 7, and one
+ * scale of 8 bits, an unsigned number with 5 exponent and 3 fraction bits (the FP16 number
+ * whose bits 14 .. 7 the byte is); a value is code times scale, an FP16 number.  Written, the
+ * scale is the number nearest to a seventh of the group's largest magnitude (ties to even;
+ * below 2^-14 the next multiple of 2^-17 up; at most 9216, so values past 64512 are held as
+ * that), the code the nearest to x / scale (ties to even, at most 7): no other value moves
+ * by more than half a scale.  A group with a value that is not finite reads as NaN.  No
+ * counterpart in the reference; each function is the 4-bit form of the FP16 one named.
+ *
+ * Storage: bytes [layers][num_blocks][PKV_INT4_BLOCK_BYTES], 16-byte aligned, a block being
+ * [4 heads][1152]: K codes [4 groups][16 tokens][8], V codes [8 chunks of 8 dims][16 tokens][4],
+ * K scales [4 groups][16 tokens], V scales alike.  Eight codes are a 32-bit word: dim 2 i + h of
+ * the eight is nibble i of its 16-bit half h, held as code + 8, each half then rotated left by
+ * two bits. */
+#define PKV_INT4_BLOCK_BYTES 4608
+
+/* pkv_append_kv into it, for layers layer_begin .. + layer_count of the cache.  With rope_table
+ * K and the query are rotated, in FP32 or better and rounded once (K to its codes, the query to
+ * FP16, or with query_out_fp32 not at all); with query_norm and key_norm (FP16 [layers][64], of
+ * the cache's layers, 16-byte aligned) each head is normed first:
+ * x * rsqrt(mean(x^2) + eps) * weight.  Tokens may go to any slots, in any order, but to no slot
+ * twice. */
+int pkv_int4_append_kv(void *storage, int32_t layers, int32_t num_blocks, int32_t layer_begin, int32_t layer_count,
+                       const void *key, const void *value, int64_t src_layer_stride, int64_t src_token_stride,
+                       const int32_t *slots, const int32_t *positions, int32_t tokens, const void *rope_table,
+                       const void *query_norm, const void *key_norm, double eps, const void *query_in,
+                       int64_t q_layer_stride, int64_t q_token_stride, void *query_out, int32_t query_out_fp32,
+                       int64_t q_out_layer_stride, int64_t q_out_token_stride, int32_t *error_flag, void *stream);
+
+/* K and V of `count` blocks (device int32) at `layer` as FP16 [count][16][4][64] each, 16-byte
+ * aligned. */
+int pkv_int4_read_blocks(const void *storage, int32_t layers, int32_t num_blocks, int32_t layer, const int32_t *blocks,
+                         int32_t count, void *key_out, void *value_out, int32_t *error_flag, void *stream);
+
+/* pkv_fp8_prefill_attention over the 4-bit cache: same arguments, workspace and result over the
+ * values that the cache holds. */
+int pkv_int4_prefill_attention(const void *storage, int32_t layers, int32_t num_blocks, int32_t layer,
+                               const void *query, int32_t query_fp32, int64_t query_stride, const int32_t *blocks,
+                               int32_t start, int32_t tokens, void *out, int64_t out_stride, void *workspace,
+                               int64_t workspace_bytes, int32_t *error_flag, void *stream);
+
+/* Grid and workspace of the two functions below on `device`. */
+int pkv_int4_decode_plan(int32_t device, int32_t batch, int32_t total_blocks, int32_t *out_grid,
+                         int64_t *out_workspace_bytes);
+
+/* pkv_fp8_decode_attention over the 4-bit cache, with its contracts; the workspace is
+ * 8448 * (batch + grid) bytes, none for a grid of 1.  Rows may have any number of tokens. */
+int pkv_int4_decode_attention(const void *storage, int32_t layers, int32_t num_blocks, int32_t layer, const void *query,
+                              int64_t query_stride, const int32_t *lengths, const int32_t *prefix, const int32_t *flat,
+                              int32_t batch, int32_t total_blocks, int32_t grid, void *out, int64_t out_stride,
+                              void *workspace, int64_t workspace_bytes, int32_t *error_flag, void *stream);
+
+/* pkv_fp8_decode_layer over the 4-bit cache, with its contracts: norm (query_norm and key_norm as
+ * above, or both null), rotation, write and attention.  Rows without blocks give zeros with
+ * `clear`, and are left alone without it. */
+int pkv_int4_decode_layer(void *storage, int32_t layers, int32_t num_blocks, int32_t layer, const void *query,
+                          int64_t query_stride, const void *key, const void *value, int64_t kv_stride,
+                          const void *rope_table, const void *query_norm, const void *key_norm, double eps,
+                          const int32_t *lengths, const int32_t *prefix, const int32_t *flat, int32_t batch,
+                          int32_t total_blocks, int32_t grid, int32_t clear, void *out, int64_t out_stride,
+                          void *workspace, int64_t workspace_bytes, int32_t *error_flag, void *stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -8,7 +8,7 @@ operation of this package goes through it and there is no fallback path.
 from __future__ import annotations
 
 import ctypes
-from ctypes import POINTER, c_char_p, c_float, c_int, c_int32, c_int64, c_void_p
+from ctypes import POINTER, c_char_p, c_double, c_float, c_int, c_int32, c_int64, c_void_p
 from pathlib import Path
 
 from pagedcore_b200 import build as _build
@@ -36,6 +36,9 @@ i64p = POINTER(c_int64)
 
 # key_codes, value_codes, key_scales, value_scales, layers, num_blocks
 _FP8_CACHE = (c_void_p, c_void_p, c_void_p, c_void_p, c_int32, c_int32)
+
+# storage, layers, num_blocks
+_INT4_CACHE = (c_void_p, c_int32, c_int32)
 
 # name -> (restype, argtypes); every symbol declared in include/pagedkv.h.
 SIGNATURES: dict[str, tuple[object, list[object]]] = {
@@ -214,6 +217,108 @@ SIGNATURES: dict[str, tuple[object, list[object]]] = {
             c_int32,  # batch
             c_int32,  # total_blocks
             c_int32,  # grid
+            c_void_p,  # out
+            c_int64,  # out_stride
+            c_void_p,  # workspace
+            c_int64,  # workspace_bytes
+            c_void_p,  # error_flag
+            c_void_p,  # stream
+        ],
+    ),
+    "pkv_int4_append_kv": (
+        c_int,
+        [
+            *_INT4_CACHE,
+            c_int32,  # layer_begin
+            c_int32,  # layer_count
+            c_void_p,  # key
+            c_void_p,  # value
+            c_int64,  # src_layer_stride
+            c_int64,  # src_token_stride
+            c_void_p,  # slots
+            c_void_p,  # positions
+            c_int32,  # tokens
+            c_void_p,  # rope_table
+            c_void_p,  # query_norm
+            c_void_p,  # key_norm
+            c_double,  # eps
+            c_void_p,  # query_in
+            c_int64,  # q_layer_stride
+            c_int64,  # q_token_stride
+            c_void_p,  # query_out
+            c_int32,  # query_out_fp32
+            c_int64,  # q_out_layer_stride
+            c_int64,  # q_out_token_stride
+            c_void_p,  # error_flag
+            c_void_p,  # stream
+        ],
+    ),
+    "pkv_int4_read_blocks": (
+        c_int,
+        [*_INT4_CACHE, c_int32, c_void_p, c_int32, c_void_p, c_void_p, c_void_p, c_void_p],
+    ),
+    "pkv_int4_prefill_attention": (
+        c_int,
+        [
+            *_INT4_CACHE,
+            c_int32,  # layer
+            c_void_p,  # query
+            c_int32,  # query_fp32
+            c_int64,  # query_stride
+            c_void_p,  # blocks
+            c_int32,  # start
+            c_int32,  # tokens
+            c_void_p,  # out
+            c_int64,  # out_stride
+            c_void_p,  # workspace
+            c_int64,  # workspace_bytes
+            c_void_p,  # error_flag
+            c_void_p,  # stream
+        ],
+    ),
+    "pkv_int4_decode_plan": (c_int, [c_int32, c_int32, c_int32, i32p, i64p]),
+    "pkv_int4_decode_attention": (
+        c_int,
+        [
+            *_INT4_CACHE,
+            c_int32,  # layer
+            c_void_p,  # query
+            c_int64,  # query_stride
+            c_void_p,  # lengths
+            c_void_p,  # prefix
+            c_void_p,  # flat
+            c_int32,  # batch
+            c_int32,  # total_blocks
+            c_int32,  # grid
+            c_void_p,  # out
+            c_int64,  # out_stride
+            c_void_p,  # workspace
+            c_int64,  # workspace_bytes
+            c_void_p,  # error_flag
+            c_void_p,  # stream
+        ],
+    ),
+    "pkv_int4_decode_layer": (
+        c_int,
+        [
+            *_INT4_CACHE,
+            c_int32,  # layer
+            c_void_p,  # query
+            c_int64,  # query_stride
+            c_void_p,  # key
+            c_void_p,  # value
+            c_int64,  # kv_stride
+            c_void_p,  # rope_table
+            c_void_p,  # query_norm
+            c_void_p,  # key_norm
+            c_double,  # eps
+            c_void_p,  # lengths
+            c_void_p,  # prefix
+            c_void_p,  # flat
+            c_int32,  # batch
+            c_int32,  # total_blocks
+            c_int32,  # grid
+            c_int32,  # clear
             c_void_p,  # out
             c_int64,  # out_stride
             c_void_p,  # workspace

@@ -48,12 +48,15 @@
 #include <initializer_list>
 #include <string>
 
+#include "block_list.cuh"
 #include "fp8_cache.cuh"
 #include "pdl.h"
 #include "ptx.cuh"
 #include "status.h"
 
 namespace {
+
+using pkv::advance_row, pkv::load_rows, pkv::max8, pkv::Merge, pkv::out_of_order, pkv::Rows, pkv::sum8, pkv::total_blocks;
 
 constexpr int kDim = PKV_HEAD_DIM;
 constexpr int kHeads = PKV_KV_HEADS;
@@ -127,18 +130,6 @@ __device__ __forceinline__ void mma(float (&d)[4], uint32_t a0, uint32_t a1, uin
         : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
 
-__device__ __forceinline__ float max8(float v) {
-    v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, 4));
-    v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, 8));
-    return fmaxf(v, __shfl_xor_sync(0xffffffffu, v, 16));
-}
-
-__device__ __forceinline__ float sum8(float v) {
-    v += __shfl_xor_sync(0xffffffffu, v, 4);
-    v += __shfl_xor_sync(0xffffffffu, v, 8);
-    return v + __shfl_xor_sync(0xffffffffu, v, 16);
-}
-
 __device__ __forceinline__ uint32_t word(const uint4 &v, int i) {
     return i == 0 ? v.x : i == 1 ? v.y : i == 2 ? v.z : v.w;
 }
@@ -154,47 +145,11 @@ __device__ __forceinline__ uint4 keep_bytes(const uint4 &v, int keep) {
     return make_uint4(v.x & m[0], v.y & m[1], v.z & m[2], v.w & m[3]);
 }
 
-// The batch's block count, from the device so that a captured launch serves changing batches.
-__device__ __forceinline__ int total_blocks(const Args &a) {
-    const int total = a.prefix[a.batch];
-    if (total >= 0 && total <= a.capacity) return total;
-    atomicOr(a.error_flag, PKV_DEVICE_BAD_BLOCK);
-    return 0;
-}
-
-// Whether row `row` breaks the order of the list: it begins at block 0 and no row ends
-// before it begins.  Such a list is reported, and no partial is written where the plan has
-// no room for one.
-__device__ __forceinline__ bool out_of_order(int row, int first, int last) {
-    return last < first || (row == 0 && first != 0);
-}
-
 // Pieces of a list of `total` blocks: at most one per CTA and per chunk, so
 // none is empty.  (A captured launch has a CTA for every resident slot.)
 __host__ __device__ __forceinline__ int pieces_of(int total, int grid) {
     const int chunks = (total + kChunk - 1) / kChunk;
     return chunks < 1 ? 1 : chunks < grid ? chunks : grid;
-}
-
-// Rows of the block list: where each begins and ends.  32 rows from `base` in registers.
-struct Rows {
-    int base, first, last, length;
-};
-
-__device__ __forceinline__ Rows load_rows(const Args &a, int base, int lane) {
-    const int r = base + lane;
-    if (r >= a.batch) return Rows{base, INT32_MAX, INT32_MAX, 0};
-    return Rows{base, a.prefix[r], a.prefix[r + 1], a.lengths[r]};
-}
-
-// The first row at or after `row` that has blocks past `block`, with its window.
-__device__ __forceinline__ int advance_row(const Args &a, Rows &w, int row, int block, int lane) {
-    while (true) {
-        if (row - w.base >= 32) w = load_rows(a, row, lane);
-        const unsigned past = __ballot_sync(0xffffffffu, w.base + lane >= row && w.last > block);
-        if (past != 0) return w.base + __ffs(past) - 1;
-        row = w.base + 32;
-    }
 }
 
 // A lane's 16 query dims of a head: the high halves to registers, the low ones to its
@@ -574,21 +529,6 @@ __global__ void __launch_bounds__(kThreads, 3) fp8_decode_kernel(const __grid_co
 // pieces.
 constexpr int kMergeWarps = 8;
 constexpr int kMergeThreads = kMergeWarps * 32;
-
-struct Merge {
-    float M, L, A[4];
-
-    __device__ __forceinline__ void add(float m, float l, const float4 &v) {
-        const float top = fmaxf(M, m);
-        const float x = pkv::exp2_approx(M - top), y = pkv::exp2_approx(m - top);
-        M = top;
-        L = fmaf(L, x, l * y);
-        A[0] = fmaf(A[0], x, v.x * y);
-        A[1] = fmaf(A[1], x, v.y * y);
-        A[2] = fmaf(A[2], x, v.z * y);
-        A[3] = fmaf(A[3], x, v.w * y);
-    }
-};
 
 template <bool SPREAD>
 __global__ void __launch_bounds__(kMergeThreads) fp8_merge_kernel(const __grid_constant__ Args a) {

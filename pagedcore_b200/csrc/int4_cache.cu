@@ -1,0 +1,336 @@
+// Writes to and reads from the 4-bit KV cache (numbers and layout: int4.cuh).
+//
+// pkv_int4_append_kv puts new K (with a norm of each head and the rotation, where asked for)
+// and V rows into their slots.  A warp takes K or V of one head of eight tokens, a lane 16
+// dims, which are a group: its scale and codes need no other lane.  Tokens are independent
+// of one another.  CTAs behind those rotate the queries.
+
+#include <cuda_fp16.h>
+#include <cuda_runtime.h>
+#include <stdint.h>
+
+#include <string>
+
+#include "int4.cuh"
+#include "pdl.h"
+#include "prefill_attention.h"
+#include "ptx.cuh"
+#include "status.h"
+
+namespace {
+
+constexpr int kDim = PKV_HEAD_DIM;
+constexpr int kHalf = kDim / 2;
+constexpr int kHeads = PKV_KV_HEADS;
+constexpr int kSlots = PKV_BLOCK_TOKENS;
+constexpr int kThreads = 2 * kHeads * 32;
+constexpr int kSpan = 8;       // tokens per CTA that writes K and V
+constexpr int kQuerySpan = 4;  // and per CTA that rotates queries
+
+struct AppendArgs {
+    pkv::int4::Cache cache;
+    int32_t layer_begin;
+    const __half *key;
+    const __half *value;
+    int64_t layer_stride;
+    int64_t token_stride;
+    const int32_t *slots;
+    const int32_t *positions;  // with rope
+    int32_t tokens;
+    const __half *rope;        // FP16 cos [2048][32], sin [2048][32], or null
+    const __half *query_norm;  // FP16 [layers][64], or null
+    const __half *key_norm;
+    double eps;
+    const __half *query_in;
+    void *query_out;
+    int32_t query_out_fp32;
+    int64_t q_layer_stride;
+    int64_t q_token_stride;
+    int64_t q_out_layer_stride;
+    int64_t q_out_token_stride;
+    int32_t *error_flag;
+    int32_t tile_ctas;  // CTAs that write K and V; those that rotate queries come after them in the grid
+};
+
+__device__ __forceinline__ int checked_position(const AppendArgs &a, int token) {
+    const int position = a.positions[token];
+    if (position >= 0 && position < PKV_CONTEXT_LIMIT) return position;
+    atomicOr(a.error_flag, PKV_DEVICE_BAD_POSITION);
+    return 0;
+}
+
+// Norm and RoPE of kQuerySpan tokens' queries, four heads a warp: eight lanes a head, eight
+// dims a lane; the partner's dims (32 away) come from the lane four further.
+__device__ void rotate_queries(const AppendArgs &a, int layer, int begin, int warp, int lane) {
+    const int chunk = lane & 7, at = (4 * warp + (lane >> 3)) * kDim + 8 * chunk;
+    const float sign = chunk < 4 ? -1.f : 1.f;
+    float weight[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) weight[i] = 1.f;
+    if (a.query_norm != nullptr) {
+        const __half *from = a.query_norm + static_cast<int64_t>(a.layer_begin + layer) * kDim + 8 * chunk;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) weight[i] = __half2float(from[i]);
+    }
+    for (int token = begin; token < min(begin + kQuerySpan, a.tokens); ++token) {
+        const uint4 own =
+            *reinterpret_cast<const uint4 *>(a.query_in + layer * a.q_layer_stride + token * a.q_token_stride + at);
+        const __half *factors = a.rope + checked_position(a, token) * kHalf + 8 * (chunk & 3);
+        const __half2 *h = reinterpret_cast<const __half2 *>(&own);
+        float x[8], y[8];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const float2 f = __half22float2(h[i]);
+            x[2 * i] = f.x, x[2 * i + 1] = f.y;
+        }
+        if (a.query_norm != nullptr) {
+            float sum = 0.f;
+#pragma unroll
+            for (int i = 0; i < 8; ++i) sum = fmaf(x[i], x[i], sum);
+#pragma unroll
+            for (int offset = 1; offset < 8; offset <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, offset);
+            const float inverse = rsqrtf(sum * (1.f / kDim) + static_cast<float>(a.eps));
+#pragma unroll
+            for (int i = 0; i < 8; ++i) x[i] *= inverse * weight[i];
+        }
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            const float partner = __shfl_xor_sync(0xffffffffu, x[i], 4);
+            y[i] = x[i] * __half2float(factors[i]) + sign * partner * __half2float(factors[PKV_CONTEXT_LIMIT * kHalf + i]);
+        }
+        const int64_t to = layer * a.q_out_layer_stride + token * a.q_out_token_stride + at;
+        if (a.query_out_fp32) {
+            float4 *dst = reinterpret_cast<float4 *>(static_cast<float *>(a.query_out) + to);
+            dst[0] = make_float4(y[0], y[1], y[2], y[3]);
+            dst[1] = make_float4(y[4], y[5], y[6], y[7]);
+        } else {
+            uint32_t r[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) r[i] = pkv::pack_half2(__floats2half2_rn(y[2 * i], y[2 * i + 1]));
+            *reinterpret_cast<uint4 *>(static_cast<__half *>(a.query_out) + to) = make_uint4(r[0], r[1], r[2], r[3]);
+        }
+    }
+}
+
+__global__ void __launch_bounds__(kThreads) int4_append_kernel(const __grid_constant__ AppendArgs a) {
+    pkv::pdl_wait();
+    pkv::pdl_launch_dependents();
+    const int layer = blockIdx.y;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    if (static_cast<int>(blockIdx.x) >= a.tile_ctas) {
+        rotate_queries(a, layer, (static_cast<int>(blockIdx.x) - a.tile_ctas) * kQuerySpan, warp, lane);
+        return;
+    }
+    const int token = static_cast<int>(blockIdx.x) * kSpan + (lane >> 2);
+    const int t = lane & 3, head = warp & 3;
+    int slot = token < a.tokens ? a.slots[token] : -1;
+    if (slot < 0 || slot >= static_cast<int64_t>(a.cache.num_blocks) * kSlots) {
+        if (token < a.tokens && t == 0 && warp == 0) atomicOr(a.error_flag, PKV_DEVICE_BAD_BLOCK);
+        slot = -1;
+    }
+    const bool here = slot >= 0;
+    const int64_t from = layer * a.layer_stride + token * a.token_stride + head * kDim;
+    float v[16];
+    uint32_t words[2], scale;
+    uint8_t *const to =
+        pkv::int4::block_at(a.cache, a.layer_begin + layer, here ? slot / kSlots : 0) + head * pkv::int4::kHeadBytes;
+    if (warp < kHeads) {
+        const int position = here && a.rope != nullptr ? checked_position(a, token) : 0;
+        const __half *weight =
+            a.key_norm != nullptr ? a.key_norm + static_cast<int64_t>(a.layer_begin + layer) * kDim : nullptr;
+        pkv::int4::key_group(a.key + from, t, here, weight, a.eps, a.rope, position, v);
+        if (!here) return;
+        pkv::int4::encode_group(v, words, scale);
+        pkv::int4::store_key(to, t, slot % kSlots, words, scale);
+    } else if (here) {
+        pkv::int4::load16(a.value + from + pkv::int4::kGroup * t, v);
+        pkv::int4::encode_group(v, words, scale);
+        pkv::int4::store_value(to, t, slot % kSlots, words, scale);
+    }
+}
+
+// K and V of `blocks` as FP16, each [i][slot][head][dim].  One CTA per block, a group a thread:
+// 32 consecutive bytes out, a token's row of 512 by 16 threads.  index_out (nullable) receives
+// 0 .. count - 1, the block table of the outputs as a pool.
+constexpr int kReadThreads = kSlots * kHeads * 4;
+constexpr int64_t kBlockValues = kSlots * kHeads * kDim;
+
+__device__ __forceinline__ void store_group(__half *to, uint32_t w0, uint32_t w1, uint32_t scale) {
+    const __half2 s = __half2half2(__ushort_as_half(static_cast<unsigned short>(scale << 7)));
+    __align__(16) __half2 v[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+        const uint32_t word = i < 4 ? w0 : w1;
+        const __half2 n = pkv::int4::nibble_pair(word, pkv::int4::swap_bytes(word), i & 3);
+        v[i] = __hmul2(__hsub2(n, __float2half2_rn(i & 1 ? 24.f : 264.f)), s);  // exact
+    }
+    reinterpret_cast<uint4 *>(to)[0] = reinterpret_cast<const uint4 *>(v)[0];
+    reinterpret_cast<uint4 *>(to)[1] = reinterpret_cast<const uint4 *>(v)[1];
+}
+
+__global__ void __launch_bounds__(kReadThreads)
+    int4_read_kernel(const pkv::int4::Cache cache, int layer, const int32_t *blocks, __half *key_out, __half *value_out,
+                     int32_t *index_out, int32_t *error_flag) {
+    pkv::pdl_launch_dependents();
+    pkv::pdl_wait();
+    const int block = blocks[blockIdx.x];
+    const bool bad = block < 0 || block >= cache.num_blocks;
+    if (bad && threadIdx.x == 0) atomicOr(error_flag, PKV_DEVICE_BAD_BLOCK);
+    if (index_out != nullptr && threadIdx.x == 0) index_out[blockIdx.x] = blockIdx.x;
+    const int t = threadIdx.x & 3, head = (threadIdx.x >> 2) & 3, token = threadIdx.x >> 4;
+    uint2 k = make_uint2(0, 0), v = k;
+    uint32_t ks = 0, vs = 0;
+    if (!bad) {
+        const uint8_t *from = pkv::int4::block_at(cache, layer, block) + head * pkv::int4::kHeadBytes;
+        k = *reinterpret_cast<const uint2 *>(from + pkv::int4::key_words(t, token));
+        v.x = *reinterpret_cast<const uint32_t *>(from + pkv::int4::value_word(2 * t, token));
+        v.y = *reinterpret_cast<const uint32_t *>(from + pkv::int4::value_word(2 * t + 1, token));
+        ks = from[pkv::int4::scale_at(pkv::int4::kKeyScaleAt, t, token)];
+        vs = from[pkv::int4::scale_at(pkv::int4::kValueScaleAt, t, token)];
+    }
+    const int64_t at = static_cast<int64_t>(blockIdx.x) * kBlockValues + threadIdx.x * pkv::int4::kGroup;
+    store_group(key_out + at, k.x, k.y, ks);
+    store_group(value_out + at, v.x, v.y, vs);
+}
+
+bool aligned16(const void *p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
+
+}  // namespace
+
+namespace pkv::int4 {
+
+int check_cache(const void *storage, int32_t layers, int32_t num_blocks, int32_t layer_begin, int32_t layer_count) {
+    if (storage == nullptr || !aligned16(storage)) {
+        return fail(PKV_VALUE_ERROR, "int4 cache: the storage is required and must be 16-byte aligned");
+    }
+    if (layers < 1 || num_blocks < 1 || num_blocks > INT32_MAX / PKV_BLOCK_TOKENS) {
+        return fail(PKV_VALUE_ERROR, "int4 cache: layer or block count out of range");
+    }
+    if (layer_begin < 0 || layer_count < 1 || layer_count > layers - layer_begin) {
+        return fail(PKV_VALUE_ERROR, "int4 cache: layers out of range");
+    }
+    return PKV_OK;
+}
+
+}  // namespace pkv::int4
+
+extern "C" int pkv_int4_append_kv(void *storage, int32_t layers, int32_t num_blocks, int32_t layer_begin,
+                                  int32_t layer_count, const void *key, const void *value, int64_t src_layer_stride,
+                                  int64_t src_token_stride, const int32_t *slots, const int32_t *positions,
+                                  int32_t tokens, const void *rope_table, const void *query_norm, const void *key_norm,
+                                  double eps, const void *query_in, int64_t q_layer_stride, int64_t q_token_stride,
+                                  void *query_out, int32_t query_out_fp32, int64_t q_out_layer_stride,
+                                  int64_t q_out_token_stride, int32_t *error_flag, void *stream) {
+    pkv::clear_error();
+    const int rc = pkv::int4::check_cache(storage, layers, num_blocks, layer_begin, layer_count);
+    if (rc) return rc;
+    if (key == nullptr || value == nullptr || slots == nullptr || error_flag == nullptr || tokens < 0) {
+        return pkv::fail(PKV_VALUE_ERROR, "int4 append: key, value, slots and error_flag are required");
+    }
+    if ((rope_table != nullptr) != (positions != nullptr) || (query_in != nullptr) != (query_out != nullptr) ||
+        (query_in != nullptr && rope_table == nullptr)) {
+        return pkv::fail(PKV_VALUE_ERROR, "int4 append: rope_table goes with positions, query with both and an output");
+    }
+    if ((query_norm != nullptr) != (key_norm != nullptr) || (key_norm != nullptr && rope_table == nullptr)) {
+        return pkv::fail(PKV_VALUE_ERROR, "int4 append: the norms go together and with rope_table");
+    }
+    if (!aligned16(key) || !aligned16(value) || src_layer_stride % 8 || src_token_stride % 8 || !aligned16(rope_table) ||
+        !aligned16(query_norm) || !aligned16(key_norm) ||
+        (query_in && (!aligned16(query_in) || !aligned16(query_out) || q_layer_stride % 8 || q_token_stride % 8 ||
+                      q_out_layer_stride % 8 || q_out_token_stride % 8))) {
+        return pkv::fail(PKV_VALUE_ERROR, "int4 append: rows must be 16-byte aligned with strides in multiples of 8");
+    }
+    if (layer_count > 65535) return pkv::fail(PKV_VALUE_ERROR, "int4 append: layers out of range");
+    if (tokens == 0) return PKV_OK;
+    AppendArgs a = {};
+    a.cache = pkv::int4::cache_of(storage, layers, num_blocks);
+    a.layer_begin = layer_begin;
+    a.key = static_cast<const __half *>(key);
+    a.value = static_cast<const __half *>(value);
+    a.layer_stride = src_layer_stride;
+    a.token_stride = src_token_stride;
+    a.slots = slots;
+    a.positions = positions;
+    a.tokens = tokens;
+    a.rope = static_cast<const __half *>(rope_table);
+    a.query_norm = static_cast<const __half *>(query_norm);
+    a.key_norm = static_cast<const __half *>(key_norm);
+    a.eps = eps;
+    a.query_in = static_cast<const __half *>(query_in);
+    a.query_out = query_out;
+    a.query_out_fp32 = query_out_fp32;
+    a.q_layer_stride = q_layer_stride;
+    a.q_token_stride = q_token_stride;
+    a.q_out_layer_stride = q_out_layer_stride;
+    a.q_out_token_stride = q_out_token_stride;
+    a.error_flag = error_flag;
+    a.tile_ctas = (tokens + kSpan - 1) / kSpan;
+    const dim3 grid(a.tile_ctas + (query_in != nullptr ? (tokens + kQuerySpan - 1) / kQuerySpan : 0), layer_count);
+    const cudaError_t e =
+        pkv::launch_pdl(int4_append_kernel, grid, dim3(kThreads), static_cast<cudaStream_t>(stream), a);
+    if (e != cudaSuccess) return pkv::fail(PKV_CUDA_ERROR, std::string("int4 append launch failed: ") + cudaGetErrorString(e));
+    return PKV_OK;
+}
+
+namespace {
+
+int read_blocks(const void *storage, int32_t layers, int32_t num_blocks, int32_t layer, const int32_t *blocks,
+                int32_t count, void *key_out, void *value_out, int32_t *index_out, int32_t *error_flag, void *stream) {
+    const int rc = pkv::int4::check_cache(storage, layers, num_blocks, layer, 1);
+    if (rc) return rc;
+    if (blocks == nullptr || key_out == nullptr || value_out == nullptr || error_flag == nullptr || count < 0) {
+        return pkv::fail(PKV_VALUE_ERROR, "int4 read: blocks, outputs and error_flag are required");
+    }
+    if (!aligned16(key_out) || !aligned16(value_out)) {
+        return pkv::fail(PKV_VALUE_ERROR, "int4 read: the outputs must be 16-byte aligned");
+    }
+    if (count == 0) return PKV_OK;
+    const cudaError_t e = pkv::launch_pdl(int4_read_kernel, dim3(count), dim3(kReadThreads), static_cast<cudaStream_t>(stream),
+                                          pkv::int4::cache_of(storage, layers, num_blocks), layer, blocks,
+                                          static_cast<__half *>(key_out), static_cast<__half *>(value_out), index_out,
+                                          error_flag);
+    if (e != cudaSuccess) return pkv::fail(PKV_CUDA_ERROR, std::string("int4 read launch failed: ") + cudaGetErrorString(e));
+    return PKV_OK;
+}
+
+}  // namespace
+
+extern "C" int pkv_int4_read_blocks(const void *storage, int32_t layers, int32_t num_blocks, int32_t layer,
+                                    const int32_t *blocks, int32_t count, void *key_out, void *value_out,
+                                    int32_t *error_flag, void *stream) {
+    pkv::clear_error();
+    return read_blocks(storage, layers, num_blocks, layer, blocks, count, key_out, value_out, nullptr, error_flag, stream);
+}
+
+// The request's blocks become an FP16 pool of one layer in the workspace (the values are
+// FP16 numbers: nothing is rounded), which the tensor-core prompt kernel attends to: that
+// kernel reads every block once for each 16 queries.
+extern "C" int pkv_int4_prefill_attention(const void *storage, int32_t layers, int32_t num_blocks, int32_t layer,
+                                          const void *query, int32_t query_fp32, int64_t query_stride,
+                                          const int32_t *blocks, int32_t start, int32_t tokens, void *out,
+                                          int64_t out_stride, void *workspace, int64_t workspace_bytes,
+                                          int32_t *error_flag, void *stream) {
+    pkv::clear_error();
+    if (query == nullptr || blocks == nullptr || out == nullptr || error_flag == nullptr) {
+        return pkv::fail(PKV_VALUE_ERROR, "prefill attention: null pointer argument");
+    }
+    if (tokens < 1 || start < 0 || static_cast<int64_t>(start) + tokens > PKV_CONTEXT_LIMIT) {
+        return pkv::fail(PKV_VALUE_ERROR, "prefill attention: the chunk must hold 1 or more tokens at positions below 2048");
+    }
+    constexpr int64_t kRow = PKV_QUERY_HEADS * PKV_HEAD_DIM;
+    if (!aligned16(query) || !aligned16(out) || query_stride % 8 || out_stride % 8 || query_stride < kRow ||
+        out_stride < kRow) {
+        return pkv::fail(PKV_VALUE_ERROR, "prefill attention: rows must be 16-byte aligned, 2048 or more values apart in multiples of 8");
+    }
+    const int count = (start + tokens + kSlots - 1) / kSlots;
+    const int64_t pool_bytes = static_cast<int64_t>(count) * 2 * kBlockValues * 2;
+    if (workspace == nullptr || !aligned16(workspace) || workspace_bytes < pool_bytes + 4 * count) {
+        return pkv::fail(PKV_VALUE_ERROR, "prefill attention: the workspace needs 16388 bytes per block of 16 tokens");
+    }
+    int32_t *const table = reinterpret_cast<int32_t *>(static_cast<uint8_t *>(workspace) + pool_bytes);
+    const int rc = read_blocks(storage, layers, num_blocks, layer, blocks, count, workspace,
+                               static_cast<__half *>(workspace) + count * kBlockValues, table, error_flag, stream);
+    if (rc) return rc;
+    return pkv::launch_prefill_attention_tc(workspace, count, 0, query, query_fp32 != 0, true, query_stride, table, start,
+                                            tokens, out, out_stride, error_flag, static_cast<cudaStream_t>(stream));
+}
