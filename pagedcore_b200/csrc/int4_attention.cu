@@ -30,6 +30,7 @@
 #include <stdint.h>
 
 #include <atomic>
+#include <initializer_list>
 #include <string>
 
 #include "block_list.cuh"
@@ -47,12 +48,21 @@ constexpr int kHeads = PKV_KV_HEADS;
 constexpr int kQueryHeads = PKV_QUERY_HEADS;
 constexpr int kHeadGroup = kQueryHeads / kHeads;
 constexpr int kSlots = PKV_BLOCK_TOKENS;
-constexpr int kWarps = kHeads;
-constexpr int kThreads = kWarps * 32;
-constexpr int kLeastPiece = 4;  // blocks
+constexpr int kWarps = kHeads;     // consumers, one per KV head
+constexpr int kProducer = kWarps;  // the warp that fills the ring
+constexpr int kThreads = (kWarps + 1) * 32;
+constexpr int kChunk = 4;  // blocks per stage, and the least of a piece
+constexpr int kStages = 2;
+constexpr int kStageBytes = kChunk * pkv::int4::kBlockBytes;
+constexpr int kFreshBytes = 320;  // a row's new token as it is stored: 72 bytes a head, and whether there is one
+constexpr int kFreshOk = 4 * 72;
+constexpr int kFreshAt = kStages * kStageBytes;
+constexpr int kSmem = kFreshAt + kStages * kFreshBytes;
+constexpr uint32_t kWaitPolls = 1u << 24;
 constexpr float kScaleLog2 = 0.125f * 1.4426950408889634f;  // 64^-0.5 * log2(e)
 constexpr float kValueFactor = 0x1p-6f;  // of the values in the MMAs
-constexpr float kWeightShift = 15.0f;
+constexpr float kMostWeight = 15.0f;  // log2 of the largest weight
+constexpr float kWeightShift = 11.0f;  // ... and of one at the reference when that is set
 constexpr float kFarScore = 0x1p20f;
 constexpr float kLowest = -1e30f;  // below every finite score
 constexpr int kPartial = kQueryHeads * (kDim + 2);  // floats of a partial
@@ -92,10 +102,10 @@ __device__ __forceinline__ int piece_of(int block, int total, int pieces) {
     return static_cast<int>(((static_cast<int64_t>(block) + 1) * pieces - 1) / total);
 }
 
-// Pieces of a list of `total` blocks: at most one per CTA and per kLeastPiece blocks, so
+// Pieces of a list of `total` blocks: at most one per CTA and per chunk, so
 // none is empty.  (A captured launch has a CTA for every resident slot.)
 __host__ __device__ __forceinline__ int pieces_of(int total, int grid) {
-    const int most = (total + kLeastPiece - 1) / kLeastPiece;
+    const int most = (total + kChunk - 1) / kChunk;
     return most < 1 ? 1 : most < grid ? most : grid;
 }
 
@@ -188,39 +198,295 @@ struct Query {
     }
 };
 
-// The new token of row `row` into its slot of the row's last block: K by lanes 0 .. 3 of the
-// head's warp, V by lanes 4 .. 7.
-__device__ __forceinline__ void write_new(const Args &a, int row, int length, int last_block, int warp, int lane) {
-    const int t = lane & 3;
-    const int block = a.flat[last_block];
-    const bool ok = block >= 0 && block < a.cache.num_blocks && length >= 1 && length <= PKV_CONTEXT_LIMIT;
-    if (!ok) {
-        if (warp == 0 && lane == 0) {
-            atomicOr(a.error_flag, PKV_DEVICE_BAD_BLOCK);
-            if (length < 1 || length > PKV_CONTEXT_LIMIT) atomicOr(a.error_flag, PKV_DEVICE_BAD_POSITION);
-        }
-        return;
+// Copies of memory that one CTA reads once.
+__device__ __forceinline__ void bulk_load(uint32_t dst, const void *src, uint32_t bytes, uint32_t bar, uint64_t policy) {
+    asm volatile(
+        "cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes.L2::cache_hint [%0], [%1], %2, [%3], %4;"
+        ::"r"(dst), "l"(src), "r"(bytes), "r"(bar), "l"(policy)
+        : "memory");
+}
+
+__device__ __forceinline__ void mbar_expect_tx(uint32_t bar, uint32_t bytes) {
+    asm volatile("mbarrier.expect_tx.relaxed.cta.shared::cta.b64 [%0], %1;" ::"r"(bar), "r"(bytes) : "memory");
+}
+
+__device__ __forceinline__ bool wait_bounded(uint32_t bar, uint32_t parity) {
+    return pkv::mbar_test_wait(bar, parity) || pkv::mbar_wait_bounded(bar, parity, kWaitPolls);
+}
+
+// What a block id outside the cache reads as.
+__device__ __align__(16) const uint8_t kZeroBlock[pkv::int4::kBlockBytes] = {};
+
+// The new token of row `row` into its slot of `block`, and into `fresh` in shared memory: per
+// head 32 bytes of K codes, 32 of V codes and their scales.  Lane (head, K or V, group).
+__device__ __forceinline__ void write_new(const Args &a, int row, int length, int block, int lane, uint8_t *fresh) {
+    const int head = lane >> 3, t = lane & 3;
+    const bool is_key = (lane & 4) == 0;
+    const bool in_range = length >= 1 && length <= PKV_CONTEXT_LIMIT;
+    const bool ok = in_range && block >= 0 && block < a.cache.num_blocks;
+    if (lane == 0) {
+        if (!ok) atomicOr(a.error_flag, PKV_DEVICE_BAD_BLOCK | (in_range ? 0 : PKV_DEVICE_BAD_POSITION));
+        *reinterpret_cast<int *>(fresh + kFreshOk) = ok;
     }
-    const int64_t from = row * a.kv_stride + warp * kDim;
-    uint8_t *const to = pkv::int4::block_at(a.cache, a.layer, block) + warp * pkv::int4::kHeadBytes;
-    const int slot = (length - 1) % kSlots;
+    if (!ok) return;
+    const int64_t from = row * a.kv_stride + head * kDim;
     float v[16];
     uint32_t words[2], scale;
-    pkv::int4::key_group(a.key + from, t, lane < 4, a.key_norm, a.eps, a.rope, length - 1, v);
-    if (lane >= 4 && lane < 8) pkv::int4::load16(a.value + from + 16 * t, v);
-    if (lane < 8) {
-        pkv::int4::encode_group(v, words, scale);
-        if (lane < 4) pkv::int4::store_key(to, t, slot, words, scale);
-        else pkv::int4::store_value(to, t, slot, words, scale);
+    pkv::int4::key_group(a.key + from, t, is_key, a.key_norm, a.eps, a.rope, length - 1, v);
+    if (!is_key) pkv::int4::load16(a.value + from + 16 * t, v);
+    pkv::int4::encode_group(v, words, scale);
+    uint8_t *const mine = fresh + head * 72;
+    *reinterpret_cast<uint2 *>(mine + (is_key ? 0 : 32) + 8 * t) = make_uint2(words[0], words[1]);
+    mine[(is_key ? 64 : 68) + t] = static_cast<uint8_t>(scale);
+    uint8_t *const to = pkv::int4::block_at(a.cache, a.layer, block) + head * pkv::int4::kHeadBytes;
+    const int slot = (length - 1) % kSlots;
+    if (is_key) pkv::int4::store_key(to, t, slot, words, scale);
+    else pkv::int4::store_value(to, t, slot, words, scale);
+}
+
+// The same token into the copy of its (block, head) at `head` in shared memory.
+__device__ __forceinline__ void put_fresh(const uint8_t *fresh, int warp, uint8_t *head, int slot, int lane) {
+    if (*reinterpret_cast<const int *>(fresh + kFreshOk) == 0) return;
+    const uint8_t *mine = fresh + warp * 72;
+    if (lane < 4) {
+        *reinterpret_cast<uint2 *>(head + pkv::int4::key_words(lane, slot)) = *reinterpret_cast<const uint2 *>(mine + 8 * lane);
+    } else if (lane < 12) {
+        *reinterpret_cast<uint32_t *>(head + pkv::int4::value_word(lane - 4, slot)) =
+            *reinterpret_cast<const uint32_t *>(mine + 32 + 4 * (lane - 4));
+    } else if (lane < 20) {
+        const int first = lane < 16 ? pkv::int4::kKeyScaleAt : pkv::int4::kValueScaleAt;
+        head[pkv::int4::scale_at(first, lane & 3, slot)] = mine[64 + lane - 12];
+    }
+    __syncwarp();
+}
+
+// The producer warp: copies the blocks of [begin, end) chunk by chunk, a chunk ending with its
+// row, and writes the new token of each row that ends here.
+template <bool NEW>
+__device__ __forceinline__ void fill_ring(const Args &a, int begin, int end, Rows rows, int row, int lane, uint8_t *smem,
+                                          uint64_t *full, uint64_t *empty) {
+    const uint64_t policy = pkv::l2_policy_evict_first();
+    const uint32_t ring = pkv::smem_addr(smem);
+    // The ids of the list's next 64 blocks, 32 at a time, a window ahead.
+    int ids_base = begin;
+    int ids = begin + lane < end ? a.flat[begin + lane] : 0;
+    int ids_next = begin + 32 + lane < end ? a.flat[begin + 32 + lane] : 0;
+    int row_end = __shfl_sync(0xffffffffu, rows.last, row - rows.base);
+    int issued = 0;
+    bool ok = true;
+    for (int at = begin; at < end;) {
+        if (at >= row_end) {
+            row = advance_row(a, rows, row + 1, at, lane);
+            row_end = __shfl_sync(0xffffffffu, rows.last, row - rows.base);
+        }
+        if (row >= a.batch) break;  // prefix does not grow from row to row: the consumers stop here too
+        const int n = min(kChunk, min(row_end, end) - at);
+        if (at - ids_base >= 32) {
+            ids = ids_next;
+            ids_base += 32;
+            const int ahead = ids_base + 32 + lane;
+            ids_next = ahead < end ? a.flat[ahead] : 0;
+        }
+        const int offset = at - ids_base + min(lane, n - 1);
+        const int near = __shfl_sync(0xffffffffu, ids, offset & 31);
+        const int far = __shfl_sync(0xffffffffu, ids_next, offset & 31);
+        const int block = offset < 32 ? near : far;  // of lane's copy; from lane n - 1 on the last one
+        const bool bad = block < 0 || block >= a.cache.num_blocks;  // reported, and read as zeros
+        if (bad && lane < n) atomicOr(a.error_flag, PKV_DEVICE_BAD_BLOCK);
+        const int stage = issued % kStages;
+        if (issued >= kStages) {
+            ok = wait_bounded(pkv::smem_addr(&empty[stage]), (issued / kStages - 1) & 1);
+            ok = __all_sync(0xffffffffu, ok);
+            if (!ok) break;  // a consumer gave up
+        }
+        const uint32_t bar = pkv::smem_addr(&full[stage]);
+        if (lane == 0) mbar_expect_tx(bar, n * pkv::int4::kBlockBytes);
+        __syncwarp();
+        if (lane < n) {
+            bulk_load(ring + stage * kStageBytes + lane * pkv::int4::kBlockBytes,
+                      bad ? kZeroBlock : pkv::int4::block_at(a.cache, a.layer, block), pkv::int4::kBlockBytes, bar, policy);
+        }
+        if (NEW && at + n == row_end) {
+            const int length = __shfl_sync(0xffffffffu, rows.length, row - rows.base);
+            write_new(a, row, length, __shfl_sync(0xffffffffu, block, n - 1), lane, smem + kFreshAt + stage * kFreshBytes);
+            __syncwarp();
+        }
+        if (lane == 0) pkv::mbar_arrive(bar);
+        at += n;
+        ++issued;
+    }
+    if (!ok && lane == 0) atomicOr(a.error_flag, PKV_DEVICE_WAIT_TIMEOUT);
+    // No copy may land after the CTA has left.
+    for (int c = max(0, issued - kStages); c < issued; ++c) {
+        wait_bounded(pkv::smem_addr(&full[c % kStages]), (c / kStages) & 1);
+    }
+}
+
+// One row's running softmax of heads 2 t and 2 t + 1, over the tokens of the lane's rows.
+struct Sums {
+    float m0, m1;  // the references: weights are 2^(score - m)
+    float l0, l1;
+    float o[4][4];
+    bool far;  // a reference of the warp's is so far out that a score's own rounding is not small
+
+    __device__ __forceinline__ void clear() {
+        m0 = m1 = kLowest;
+        far = false;
+        l0 = l1 = 0.f;
+#pragma unroll
+        for (int mt = 0; mt < 4; ++mt) o[mt][0] = o[mt][1] = o[mt][2] = o[mt][3] = 0.f;
+    }
+
+    // log2 of the weights of products s.  The product is rounded by itself only far out, where
+    // what a fused operation keeps of it could be large (2^-24 of 2^38 in the exponent).
+    __device__ __forceinline__ void exponents(const float (&s)[4], const Query &q, float (&x)[4]) const {
+        if (far) {
+            x[0] = __fmul_rn(s[0], q.factor0) - m0, x[1] = __fmul_rn(s[1], q.factor1) - m1;
+            x[2] = __fmul_rn(s[2], q.factor0) - m0, x[3] = __fmul_rn(s[3], q.factor1) - m1;
+        } else {
+            x[0] = fmaf(s[0], q.factor0, -m0), x[1] = fmaf(s[1], q.factor1, -m1);
+            x[2] = fmaf(s[2], q.factor0, -m0), x[3] = fmaf(s[3], q.factor1, -m1);
+        }
+    }
+
+    // References for scores that reach top0 and top1 in this lane.
+    __device__ __forceinline__ void raise(float top0, float top1) {
+        top0 = max8(top0);
+        top1 = max8(top1);
+        // Far out, where the shift would soon be lost in its rounding, the maximum itself.
+        top0 = fmaxf(m0, fabsf(top0) > kFarScore ? top0 : top0 - kWeightShift);
+        top1 = fmaxf(m1, fabsf(top1) > kFarScore ? top1 : top1 - kWeightShift);
+        const float alpha0 = pkv::exp2_approx(m0 - top0), alpha1 = pkv::exp2_approx(m1 - top1);
+        m0 = top0;
+        m1 = top1;
+        far = __any_sync(0xffffffffu, fmaxf(m0, m1) > kFarScore || (m0 < -kFarScore && m0 > kLowest) ||
+                                          (m1 < -kFarScore && m1 > kLowest));
+        l0 *= alpha0;
+        l1 *= alpha1;
+#pragma unroll
+        for (int mt = 0; mt < 4; ++mt) o[mt][0] *= alpha0, o[mt][1] *= alpha1, o[mt][2] *= alpha0, o[mt][3] *= alpha1;
+    }
+};
+
+// Bytes of a (block, head) as a lane reads them.
+struct Tile {
+    uint4 k, v;
+    uint32_t ks, vs;
+
+    __device__ __forceinline__ void load(const uint8_t *head, int lane) {
+        const int g = lane >> 2, t = lane & 3;
+        k = *reinterpret_cast<const uint4 *>(head + pkv::int4::key_words(t, 2 * g));
+        v = *reinterpret_cast<const uint4 *>(head + pkv::int4::kValueAt + lane * 16);
+        ks = *reinterpret_cast<const uint16_t *>(head + pkv::int4::scale_at(pkv::int4::kKeyScaleAt, t, 2 * g));
+        vs = *reinterpret_cast<const uint32_t *>(head + pkv::int4::scale_at(pkv::int4::kValueScaleAt, g >> 1, 4 * t));
+    }
+};
+
+template <bool NEW>
+__device__ __forceinline__ void score(const Tile &tile, const Query &q, float (&s)[4]) {
+    s[0] = s[1] = s[2] = s[3] = 0.f;
+    const Steps k0((tile.ks & 0xffu) * 0x00800080u), k1((tile.ks >> 8) * 0x00800080u);  // each scale twice
+#pragma unroll
+    for (int ks = 0; ks < 4; ++ks) {
+        const uint32_t x = ks < 2 ? tile.k.x : tile.k.y, y = ks < 2 ? tile.k.z : tile.k.w;
+        const uint32_t xs = pkv::int4::swap_bytes(x), ys = pkv::int4::swap_bytes(y);
+        const int i = 2 * (ks & 1);
+        const uint32_t a0 = value_pair(x, xs, i, k0), a1 = value_pair(y, ys, i, k1);
+        const uint32_t a2 = value_pair(x, xs, i + 1, k0), a3 = value_pair(y, ys, i + 1, k1);
+        mma(s, a0, a1, a2, a3, q.high[2 * ks], q.high[2 * ks + 1]);
+        if (NEW) mma(s, a0, a1, a2, a3, q.low[2 * ks], q.low[2 * ks + 1]);
+    }
+}
+
+// Adds the weights w of a block's tokens (rows g and g + 8 of heads 2 t, 2 t + 1) times its V.
+__device__ __forceinline__ void add_values(const Tile &tile, const float (&w)[4], Sums &sums) {
+    const __half2 h01 = __floats2half2_rn(w[0], w[1]), h23 = __floats2half2_rn(w[2], w[3]);
+    const float2 f01 = __half22float2(h01), f23 = __half22float2(h23);
+    const uint32_t p0 = pkv::movmatrix_trans(pack(h01)), p1 = pkv::movmatrix_trans(pack(h23));
+    const uint32_t r0 = pkv::movmatrix_trans(pack(__floats2half2_rn(w[0] - f01.x, w[1] - f01.y)));
+    const uint32_t r1 = pkv::movmatrix_trans(pack(__floats2half2_rn(w[2] - f23.x, w[3] - f23.y)));
+    // Tokens 4 t, 4 t + 2 in the first pair, 4 t + 1, 4 t + 3 in the second.
+    const Steps v0((tile.vs & 0x00ff00ffu) << 7), v1((tile.vs & 0xff00ff00u) >> 1);
+    const uint4 &v = tile.v;
+    uint32_t even[4], odd[4];  // a pair's low halves, straight and swapped, and its high ones
+    even[0] = __byte_perm(v.x, v.z, 0x5410), even[1] = __byte_perm(v.x, v.z, 0x4501);
+    even[2] = __byte_perm(v.x, v.z, 0x7632), even[3] = __byte_perm(v.x, v.z, 0x6723);
+    odd[0] = __byte_perm(v.y, v.w, 0x5410), odd[1] = __byte_perm(v.y, v.w, 0x4501);
+    odd[2] = __byte_perm(v.y, v.w, 0x7632), odd[3] = __byte_perm(v.y, v.w, 0x6723);
+#pragma unroll
+    for (int mt = 0; mt < 4; ++mt) {
+        const uint32_t a0 = value_pair(even[0], even[1], mt, v0), a1 = value_pair(even[2], even[3], mt, v0);
+        const uint32_t a2 = value_pair(odd[0], odd[1], mt, v1), a3 = value_pair(odd[2], odd[3], mt, v1);
+        mma(sums.o[mt], a0, a1, a2, a3, p0, p1);
+        mma(sums.o[mt], a0, a1, a2, a3, r0, r1);
+    }
+}
+
+// `count` blocks in shared memory, `valid` tokens from the first one's first on.
+template <bool NEW, int COUNT>
+__device__ __forceinline__ void attend(Tile (&tile)[COUNT], int valid, const Query &q, Sums &sums, int lane) {
+    const int g = lane >> 2, t = lane & 3;
+    float s[COUNT][4], x[COUNT][4];
+    const bool whole = valid >= COUNT * kSlots;
+#pragma unroll
+    for (int b = 0; b < COUNT; ++b) {
+        score<NEW>(tile[b], q, s[b]);
+        if (!whole) {
+            const int here = valid - b * kSlots;
+            if (2 * g >= here) s[b][0] = s[b][1] = -INFINITY;
+            if (2 * g + 1 >= here) s[b][2] = s[b][3] = -INFINITY;
+            const int keep = min(max(here - 4 * t, 0), 4);  // V of masked tokens: weight 0 times NaN is NaN
+            if (keep < 4) tile[b].vs &= (1u << (8 * keep)) - 1u;
+        }
+    }
+    bool over = false;
+#pragma unroll
+    for (int b = 0; b < COUNT; ++b) {
+        sums.exponents(s[b], q, x[b]);
+        over |= fmaxf(fmaxf(x[b][0], x[b][1]), fmaxf(x[b][2], x[b][3])) > kMostWeight;
+    }
+    if (__any_sync(0xffffffffu, over)) {
+        float top0 = -INFINITY, top1 = -INFINITY;
+#pragma unroll
+        for (int b = 0; b < COUNT; ++b) {
+            top0 = fmaxf(top0, fmaxf(__fmul_rn(s[b][0], q.factor0), __fmul_rn(s[b][2], q.factor0)));
+            top1 = fmaxf(top1, fmaxf(__fmul_rn(s[b][1], q.factor1), __fmul_rn(s[b][3], q.factor1)));
+        }
+        sums.raise(top0, top1);
+#pragma unroll
+        for (int b = 0; b < COUNT; ++b) sums.exponents(s[b], q, x[b]);
+    }
+#pragma unroll
+    for (int b = 0; b < COUNT; ++b) {
+        float w[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) w[j] = pkv::exp2_approx(x[b][j]);
+        sums.l0 += w[0] + w[2];
+        sums.l1 += w[1] + w[3];
+        add_values(tile[b], w, sums);
     }
 }
 
 template <bool NEW>
-__global__ void __launch_bounds__(kThreads) int4_decode_kernel(const __grid_constant__ Args a) {
+__global__ void __launch_bounds__(kThreads, 3) int4_decode_kernel(const __grid_constant__ Args a) {
+    extern __shared__ __align__(16) uint8_t smem[];
+    __shared__ __align__(8) uint64_t full[kStages], empty[kStages];
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int g = lane >> 2, t = lane & 3;
+    if (threadIdx.x == 0) {
+        for (int s = 0; s < kStages; ++s) {
+            pkv::mbar_init(pkv::smem_addr(&full[s]), 1);
+            pkv::mbar_init(pkv::smem_addr(&empty[s]), kWarps);
+        }
+        pkv::fence_barrier_init();
+    }
+    __syncthreads();
     pkv::pdl_wait();
     pkv::pdl_launch_dependents();
+
+    // The piece, and a first cut of the rows: 32 samples of prefix, `step` rows apart.
+    int step = (a.batch + 31) / 32;
+    int sample = lane * step < a.batch ? a.prefix[min((lane + 1) * step, a.batch)] : INT32_MAX;
     const int total = total_blocks(a);
     const int pieces = pieces_of(total, a.grid);
     // Rows without blocks: zeros.  (The merge looks at the rows' order too, where there is one.)
@@ -234,96 +500,73 @@ __global__ void __launch_bounds__(kThreads) int4_decode_kernel(const __grid_cons
     if (total == 0 || static_cast<int>(blockIdx.x) >= pieces) return;
     const int begin = piece_begin(blockIdx.x, total, pieces);
     const int end = piece_begin(blockIdx.x + 1, total, pieces);
-    Rows rows = load_rows(a, 0, lane);
-    int row = advance_row(a, rows, 0, begin, lane);
-    for (int i = begin; i < end;) {
+    // The first row with blocks past `begin`: the first sample past it, cut finer until
+    // the samples are rows.
+    int lo = 0;
+    while (true) {
+        const unsigned past = __ballot_sync(0xffffffffu, sample > begin);
+        lo += (past != 0 ? __ffs(past) - 1 : 31) * step;
+        if (step <= 32) break;
+        step = (step + 31) / 32;
+        sample = lo + lane * step < a.batch ? a.prefix[min(lo + (lane + 1) * step, a.batch)] : INT32_MAX;
+    }
+    Rows rows = load_rows(a, lo, lane);
+    int row = advance_row(a, rows, lo, begin, lane);
+    if (warp == kProducer) {
+        if (row < a.batch) fill_ring<NEW>(a, begin, end, rows, row, lane, smem, full, empty);
+        return;
+    }
+
+    int consumed = 0;
+    bool failed = false;
+    int i = begin;
+    while (i < end) {
         if (row >= a.batch) {  // prefix does not grow from row to row
             if (threadIdx.x == 0) atomicOr(a.error_flag, PKV_DEVICE_BAD_BLOCK);
-            return;
+            break;
         }
         const int row_first = __shfl_sync(0xffffffffu, rows.first, row - rows.base);
         const int row_last = __shfl_sync(0xffffffffu, rows.last, row - rows.base);
         const int length = __shfl_sync(0xffffffffu, rows.length, row - rows.base);
         const int seg_end = min(end, row_last);
-        if (NEW && row_last <= end) {
-            write_new(a, row, length, row_last - 1, warp, lane);
-            __syncwarp();
-        }
         Query q;
         q.load<NEW>(a, row, length, warp, lane);
-
-        float m0 = kLowest, m1 = kLowest, l0 = 0.f, l1 = 0.f;
-        float o[4][4];
-#pragma unroll
-        for (int mt = 0; mt < 4; ++mt) o[mt][0] = o[mt][1] = o[mt][2] = o[mt][3] = 0.f;
-        for (; i < seg_end; ++i) {
-            const int block = a.flat[i];
-            const bool bad = block < 0 || block >= a.cache.num_blocks;  // reported, and read as zeros
-            if (bad && threadIdx.x == 0) atomicOr(a.error_flag, PKV_DEVICE_BAD_BLOCK);
-            const uint8_t *from = pkv::int4::block_at(a.cache, a.layer, bad ? 0 : block) + warp * pkv::int4::kHeadBytes;
-            const uint4 k = *reinterpret_cast<const uint4 *>(from + pkv::int4::key_words(t, 2 * g));
-            const uint4 v = *reinterpret_cast<const uint4 *>(from + pkv::int4::kValueAt + lane * 16);
-            uint32_t ks = *reinterpret_cast<const uint16_t *>(from + pkv::int4::scale_at(pkv::int4::kKeyScaleAt, t, 2 * g));
-            uint32_t vs = *reinterpret_cast<const uint32_t *>(from + pkv::int4::scale_at(pkv::int4::kValueScaleAt, g >> 1, 4 * t));
-            if (bad) ks = vs = 0;
-            const int valid = min(max(length - (i - row_first) * kSlots, 0), kSlots);  // tokens of this block
-            if (valid < kSlots) {  // weight 0 times NaN is NaN
-                const int keep = min(max(valid - 4 * t, 0), 4);
-                vs = keep == 4 ? vs : vs & ((1u << (8 * keep)) - 1u);
+        Sums sums;
+        sums.clear();
+        while (i < seg_end) {
+            const int n = min(kChunk, seg_end - i);
+            const int stage = consumed % kStages;
+            failed = !wait_bounded(pkv::smem_addr(&full[stage]), (consumed / kStages) & 1);
+            failed = __any_sync(0xffffffffu, failed);
+            if (failed) break;
+            uint8_t *const src = smem + stage * kStageBytes + warp * pkv::int4::kHeadBytes;
+            if (NEW && i + n == row_last) {
+                put_fresh(smem + kFreshAt + stage * kFreshBytes, warp, src + (n - 1) * pkv::int4::kBlockBytes,
+                          (length - 1) & (kSlots - 1), lane);
             }
-
-            float s[4] = {0.f, 0.f, 0.f, 0.f};
-            const Steps k0((ks & 0xffu) * 0x00800080u), k1((ks >> 8) * 0x00800080u);  // each scale twice
-#pragma unroll
-            for (int ks4 = 0; ks4 < 4; ++ks4) {
-                const uint32_t x = ks4 < 2 ? k.x : k.y, y = ks4 < 2 ? k.z : k.w;
-                const uint32_t xs = pkv::int4::swap_bytes(x), ys = pkv::int4::swap_bytes(y);
-                const int i0 = 2 * (ks4 & 1);
-                const uint32_t a0 = value_pair(x, xs, i0, k0), a1 = value_pair(y, ys, i0, k1);
-                const uint32_t a2 = value_pair(x, xs, i0 + 1, k0), a3 = value_pair(y, ys, i0 + 1, k1);
-                mma(s, a0, a1, a2, a3, q.high[2 * ks4], q.high[2 * ks4 + 1]);
-                if (NEW) mma(s, a0, a1, a2, a3, q.low[2 * ks4], q.low[2 * ks4 + 1]);
+            const int tokens = min(max(length - (i - row_first) * kSlots, 0), n * kSlots);  // valid ones of the chunk
+            // Blocks past n hold an earlier chunk's bytes: their tokens are masked.
+#pragma unroll 1
+            for (int b = 0; b < n; b += 2) {
+                Tile tile[2];
+                tile[0].load(src + b * pkv::int4::kBlockBytes, lane);
+                tile[1].load(src + (b + 1) * pkv::int4::kBlockBytes, lane);
+                if (b + 2 >= n) {
+                    // Every lane has read the stage (the fence orders the reads before the copies,
+                    // the warp barrier the lanes): it may be filled again.
+                    pkv::fence_proxy_async_smem();
+                    __syncwarp();
+                    if (lane == 0) pkv::mbar_arrive(pkv::smem_addr(&empty[stage]));
+                }
+                attend<NEW, 2>(tile, tokens - b * kSlots, q, sums, lane);
             }
-            s[0] *= q.factor0, s[1] *= q.factor1, s[2] *= q.factor0, s[3] *= q.factor1;
-            if (2 * g >= valid) s[0] = s[1] = -INFINITY;
-            if (2 * g + 1 >= valid) s[2] = s[3] = -INFINITY;
-            float top0 = max8(fmaxf(s[0], s[2])), top1 = max8(fmaxf(s[1], s[3]));
-            // The reference is 15 below the maximum, so that weights reach 2^15; far out,
-            // where 15 would soon be lost in its rounding, the maximum itself.
-            top0 = fmaxf(m0, fabsf(top0) > kFarScore ? top0 : top0 - kWeightShift);
-            top1 = fmaxf(m1, fabsf(top1) > kFarScore ? top1 : top1 - kWeightShift);
-            const float alpha0 = pkv::exp2_approx(m0 - top0), alpha1 = pkv::exp2_approx(m1 - top1);
-            m0 = top0;
-            m1 = top1;
-            const float w0 = pkv::exp2_approx(s[0] - m0), w1 = pkv::exp2_approx(s[1] - m1);
-            const float w2 = pkv::exp2_approx(s[2] - m0), w3 = pkv::exp2_approx(s[3] - m1);
-            l0 = fmaf(l0, alpha0, w0 + w2);
-            l1 = fmaf(l1, alpha1, w1 + w3);
-            const __half2 h01 = __floats2half2_rn(w0, w1), h23 = __floats2half2_rn(w2, w3);
-            const float2 f01 = __half22float2(h01), f23 = __half22float2(h23);
-            const uint32_t p0 = pkv::movmatrix_trans(pack(h01)), p1 = pkv::movmatrix_trans(pack(h23));
-            const uint32_t r0 = pkv::movmatrix_trans(pack(__floats2half2_rn(w0 - f01.x, w1 - f01.y)));
-            const uint32_t r1 = pkv::movmatrix_trans(pack(__floats2half2_rn(w2 - f23.x, w3 - f23.y)));
-
-            // Tokens 4 t, 4 t + 2 in the first pair, 4 t + 1, 4 t + 3 in the second.
-            const Steps v0((vs & 0x00ff00ffu) << 7), v1((vs & 0xff00ff00u) >> 1);
-            uint32_t even[4], odd[4];  // the first pair's low and high halves, straight and swapped; the second's
-            even[0] = __byte_perm(v.x, v.z, 0x5410), even[1] = __byte_perm(v.x, v.z, 0x4501);
-            even[2] = __byte_perm(v.x, v.z, 0x7632), even[3] = __byte_perm(v.x, v.z, 0x6723);
-            odd[0] = __byte_perm(v.y, v.w, 0x5410), odd[1] = __byte_perm(v.y, v.w, 0x4501);
-            odd[2] = __byte_perm(v.y, v.w, 0x7632), odd[3] = __byte_perm(v.y, v.w, 0x6723);
-#pragma unroll
-            for (int mt = 0; mt < 4; ++mt) {
-                o[mt][0] *= alpha0, o[mt][1] *= alpha1, o[mt][2] *= alpha0, o[mt][3] *= alpha1;
-                const uint32_t a0 = value_pair(even[0], even[1], mt, v0), a1 = value_pair(even[2], even[3], mt, v0);
-                const uint32_t a2 = value_pair(odd[0], odd[1], mt, v1), a3 = value_pair(odd[2], odd[3], mt, v1);
-                mma(o[mt], a0, a1, a2, a3, p0, p1);
-                mma(o[mt], a0, a1, a2, a3, r0, r1);
-            }
+            i += n;
+            ++consumed;
         }
+        if (failed) break;
 
-        l0 = sum8(l0);
-        l1 = sum8(l1);
+        const float l0 = sum8(sums.l0), l1 = sum8(sums.l1);
+        const auto &o = sums.o;
         const int head0 = warp * kHeadGroup + 2 * t;
         if (row_first >= begin && row_last <= end) {
             // Normalise and round; a row whose every token is masked is zeros.
@@ -350,11 +593,14 @@ __global__ void __launch_bounds__(kThreads) int4_decode_kernel(const __grid_cons
                 dst[1] = make_float4(o[2][h] * kUndo, o[2][2 + h] * kUndo, o[3][h] * kUndo, o[3][2 + h] * kUndo);
             }
             if (g == 0) {
-                *reinterpret_cast<float4 *>(a.part_ml + index * kQueryHeads * 2 + head0 * 2) = make_float4(m0, l0, m1, l1);
+                *reinterpret_cast<float4 *>(a.part_ml + index * kQueryHeads * 2 + head0 * 2) =
+                    make_float4(sums.m0, l0, sums.m1, l1);
             }
         }
         if (row_last < end) row = advance_row(a, rows, row + 1, row_last, lane);
+        else break;
     }
+    if (failed && lane == 0) atomicOr(a.error_flag, PKV_DEVICE_WAIT_TIMEOUT);
 }
 
 // Merge of the rows that several pieces hold, sixteen lanes a head and four dims a lane.
@@ -432,6 +678,15 @@ struct DeviceInfo {
     int ctas_per_sm = 0;
 };
 
+cudaError_t prepare_kernel(void (*kernel)(Args), int *ctas_per_sm) {
+    cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem);
+    if (e == cudaSuccess) {
+        e = cudaFuncSetAttribute(kernel, cudaFuncAttributePreferredSharedMemoryCarveout, cudaSharedmemCarveoutMaxShared);
+    }
+    if (e == cudaSuccess) e = cudaOccupancyMaxActiveBlocksPerMultiprocessor(ctas_per_sm, kernel, kThreads, kSmem);
+    return e;
+}
+
 constexpr int kMaxDevices = 64;
 
 // SMs and resident CTAs of `device`, found out at its first use.
@@ -448,8 +703,14 @@ int device_info(int device, DeviceInfo *info) {
     if (e == cudaSuccess) e = cudaSetDevice(device);
     if (e != cudaSuccess) return pkv::fail(PKV_CUDA_ERROR, std::string("int4 decode: ") + cudaGetErrorString(e));
     e = cudaDeviceGetAttribute(&info->sms, cudaDevAttrMultiProcessorCount, device);
-    if (e == cudaSuccess) e = cudaOccupancyMaxActiveBlocksPerMultiprocessor(&plain, int4_decode_kernel<false>, kThreads, 0);
-    if (e == cudaSuccess) e = cudaOccupancyMaxActiveBlocksPerMultiprocessor(&fresh, int4_decode_kernel<true>, kThreads, 0);
+    if (e == cudaSuccess) e = prepare_kernel(int4_decode_kernel<false>, &plain);
+    if (e == cudaSuccess) e = prepare_kernel(int4_decode_kernel<true>, &fresh);
+    // The merge keeps the split kernel's partition of L1 and shared memory.
+    for (const auto merge : {int4_merge_kernel<false>, int4_merge_kernel<true>}) {
+        if (e == cudaSuccess) {
+            e = cudaFuncSetAttribute(merge, cudaFuncAttributePreferredSharedMemoryCarveout, cudaSharedmemCarveoutMaxShared);
+        }
+    }
     cudaSetDevice(previous);
     if (e != cudaSuccess) return pkv::fail(PKV_CUDA_ERROR, std::string("int4 decode: ") + cudaGetErrorString(e));
     const int least = plain < fresh ? plain : fresh;
@@ -491,8 +752,8 @@ int decode(Args a, void *workspace, int64_t workspace_bytes, cudaStream_t stream
         a.part_o = static_cast<float *>(workspace);
         a.part_ml = a.part_o + (static_cast<int64_t>(a.batch) + a.grid) * kQueryHeads * kDim;
     }
-    e = pkv::launch_pdl(a.key != nullptr ? int4_decode_kernel<true> : int4_decode_kernel<false>, dim3(a.grid),
-                        dim3(kThreads), stream, a);
+    e = pkv::launch_pdl_smem(a.key != nullptr ? int4_decode_kernel<true> : int4_decode_kernel<false>, dim3(a.grid),
+                             dim3(kThreads), kSmem, stream, a);
     if (e == cudaSuccess && a.grid > 1) {
         // A CTA per (row, two heads) while that is at most two waves of CTAs: beyond it rows
         // have few pieces each and a warp merges them as fast.
