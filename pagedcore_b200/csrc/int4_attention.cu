@@ -368,17 +368,29 @@ struct Sums {
     }
 };
 
-// Bytes of a (block, head) as a lane reads them.
+// Where a lane reads its bytes of a (block, head), as shared memory addresses for block 0 of stage 0.
+struct Places {
+    uint32_t k, v, ks, vs;
+
+    __device__ __forceinline__ Places(uint32_t head, int lane) {
+        const int g = lane >> 2, t = lane & 3;
+        k = head + pkv::int4::key_words(t, 2 * g);
+        v = head + pkv::int4::kValueAt + lane * 16;
+        ks = head + pkv::int4::scale_at(pkv::int4::kKeyScaleAt, t, 2 * g);
+        vs = head + pkv::int4::scale_at(pkv::int4::kValueScaleAt, g >> 1, 4 * t);
+    }
+};
+
 struct Tile {
     uint4 k, v;
     uint32_t ks, vs;
 
-    __device__ __forceinline__ void load(const uint8_t *head, int lane) {
-        const int g = lane >> 2, t = lane & 3;
-        k = *reinterpret_cast<const uint4 *>(head + pkv::int4::key_words(t, 2 * g));
-        v = *reinterpret_cast<const uint4 *>(head + pkv::int4::kValueAt + lane * 16);
-        ks = *reinterpret_cast<const uint16_t *>(head + pkv::int4::scale_at(pkv::int4::kKeyScaleAt, t, 2 * g));
-        vs = *reinterpret_cast<const uint32_t *>(head + pkv::int4::scale_at(pkv::int4::kValueScaleAt, g >> 1, 4 * t));
+    // Block at byte `at` of the ring.
+    __device__ __forceinline__ void load(const Places &p, uint32_t at) {
+        asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(k.x), "=r"(k.y), "=r"(k.z), "=r"(k.w) : "r"(p.k + at));
+        asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(p.v + at));
+        asm volatile("ld.shared.u16 %0, [%1];" : "=r"(ks) : "r"(p.ks + at));
+        asm volatile("ld.shared.u32 %0, [%1];" : "=r"(vs) : "r"(p.vs + at));
     }
 };
 
@@ -422,16 +434,15 @@ __device__ __forceinline__ void add_values(const Tile &tile, const float (&w)[4]
     }
 }
 
-// `count` blocks in shared memory, `valid` tokens from the first one's first on.
-template <bool NEW, int COUNT>
+// COUNT blocks, of which `valid` tokens count (MASKED; else all).
+template <bool NEW, int COUNT, bool MASKED>
 __device__ __forceinline__ void attend(Tile (&tile)[COUNT], int valid, const Query &q, Sums &sums, int lane) {
     const int g = lane >> 2, t = lane & 3;
     float s[COUNT][4], x[COUNT][4];
-    const bool whole = valid >= COUNT * kSlots;
 #pragma unroll
     for (int b = 0; b < COUNT; ++b) {
         score<NEW>(tile[b], q, s[b]);
-        if (!whole) {
+        if constexpr (MASKED) {
             const int here = valid - b * kSlots;
             if (2 * g >= here) s[b][0] = s[b][1] = -INFINITY;
             if (2 * g + 1 >= here) s[b][2] = s[b][3] = -INFINITY;
@@ -439,13 +450,13 @@ __device__ __forceinline__ void attend(Tile (&tile)[COUNT], int valid, const Que
             if (keep < 4) tile[b].vs &= (1u << (8 * keep)) - 1u;
         }
     }
-    bool over = false;
+    float most = -INFINITY;
 #pragma unroll
     for (int b = 0; b < COUNT; ++b) {
         sums.exponents(s[b], q, x[b]);
-        over |= fmaxf(fmaxf(x[b][0], x[b][1]), fmaxf(x[b][2], x[b][3])) > kMostWeight;
+        most = pkv::fmax3(pkv::fmax3(most, x[b][0], x[b][1]), x[b][2], x[b][3]);
     }
-    if (__any_sync(0xffffffffu, over)) {
+    if (__any_sync(0xffffffffu, most > kMostWeight)) {
         float top0 = -INFINITY, top1 = -INFINITY;
 #pragma unroll
         for (int b = 0; b < COUNT; ++b) {
@@ -517,6 +528,7 @@ __global__ void __launch_bounds__(kThreads, 3) int4_decode_kernel(const __grid_c
         return;
     }
 
+    const Places places(pkv::smem_addr(smem) + warp * pkv::int4::kHeadBytes, lane);
     int consumed = 0;
     bool failed = false;
     int i = begin;
@@ -539,26 +551,37 @@ __global__ void __launch_bounds__(kThreads, 3) int4_decode_kernel(const __grid_c
             failed = !wait_bounded(pkv::smem_addr(&full[stage]), (consumed / kStages) & 1);
             failed = __any_sync(0xffffffffu, failed);
             if (failed) break;
-            uint8_t *const src = smem + stage * kStageBytes + warp * pkv::int4::kHeadBytes;
             if (NEW && i + n == row_last) {
-                put_fresh(smem + kFreshAt + stage * kFreshBytes, warp, src + (n - 1) * pkv::int4::kBlockBytes,
+                put_fresh(smem + kFreshAt + stage * kFreshBytes, warp,
+                          smem + stage * kStageBytes + (n - 1) * pkv::int4::kBlockBytes + warp * pkv::int4::kHeadBytes,
                           (length - 1) & (kSlots - 1), lane);
             }
             const int tokens = min(max(length - (i - row_first) * kSlots, 0), n * kSlots);  // valid ones of the chunk
-            // Blocks past n hold an earlier chunk's bytes: their tokens are masked.
-#pragma unroll 1
-            for (int b = 0; b < n; b += 2) {
+            const uint32_t at = stage * kStageBytes;
+            const auto release = [&] {
+                // Every lane has read the stage (the fence orders the reads before the copies, the
+                // warp barrier the lanes): it may be filled again.
+                pkv::fence_proxy_async_smem();
+                __syncwarp();
+                if (lane == 0) pkv::mbar_arrive(pkv::smem_addr(&empty[stage]));
+            };
+            if (tokens == kChunk * kSlots) {
                 Tile tile[2];
-                tile[0].load(src + b * pkv::int4::kBlockBytes, lane);
-                tile[1].load(src + (b + 1) * pkv::int4::kBlockBytes, lane);
-                if (b + 2 >= n) {
-                    // Every lane has read the stage (the fence orders the reads before the copies,
-                    // the warp barrier the lanes): it may be filled again.
-                    pkv::fence_proxy_async_smem();
-                    __syncwarp();
-                    if (lane == 0) pkv::mbar_arrive(pkv::smem_addr(&empty[stage]));
+                tile[0].load(places, at);
+                tile[1].load(places, at + pkv::int4::kBlockBytes);
+                attend<NEW, 2, false>(tile, 0, q, sums, lane);
+                tile[0].load(places, at + 2 * pkv::int4::kBlockBytes);
+                tile[1].load(places, at + 3 * pkv::int4::kBlockBytes);
+                release();
+                attend<NEW, 2, false>(tile, 0, q, sums, lane);
+            } else {
+#pragma unroll 1
+                for (int b = 0; b < n; ++b) {
+                    Tile tile[1];
+                    tile[0].load(places, at + b * pkv::int4::kBlockBytes);
+                    if (b + 1 == n) release();
+                    attend<NEW, 1, true>(tile, tokens - b * kSlots, q, sums, lane);
                 }
-                attend<NEW, 2>(tile, tokens - b * kSlots, q, sums, lane);
             }
             i += n;
             ++consumed;
