@@ -126,7 +126,9 @@ __device__ __forceinline__ void store_value(uint8_t *head, int t, int token, con
 // with the bytes of each half swapped.
 __device__ __forceinline__ __half2 nibble_pair(uint32_t word, uint32_t swapped, int i) {
     const uint32_t from = i < 2 ? word : swapped;
-    const uint32_t bits = i & 1 ? (from & 0x03c003c0u) | 0x4c004c00u : (from & 0x003c003cu) | 0x5c005c00u;
+    uint32_t bits;  // (from & mask) | base as one instruction, which the compiler does not make of it
+    if (i & 1) asm("lop3.b32 %0, %1, %2, %3, 0xea;" : "=r"(bits) : "r"(from), "n"(0x03c003c0), "n"(0x4c004c00));
+    else asm("lop3.b32 %0, %1, %2, %3, 0xea;" : "=r"(bits) : "r"(from), "n"(0x003c003c), "n"(0x5c005c00));
     return *reinterpret_cast<const __half2 *>(&bits);
 }
 

@@ -327,26 +327,19 @@ struct Sums {
     float m0, m1;  // the references: weights are 2^(score - m)
     float l0, l1;
     float o[4][4];
-    bool far;  // a reference of the warp's is so far out that a score's own rounding is not small
 
     __device__ __forceinline__ void clear() {
         m0 = m1 = kLowest;
-        far = false;
         l0 = l1 = 0.f;
 #pragma unroll
         for (int mt = 0; mt < 4; ++mt) o[mt][0] = o[mt][1] = o[mt][2] = o[mt][3] = 0.f;
     }
 
-    // log2 of the weights of products s.  The product is rounded by itself only far out, where
-    // what a fused operation keeps of it could be large (2^-24 of 2^38 in the exponent).
+    // log2 of the weights of products s.  The product is rounded by itself, as raise does: far
+    // out, what a fused operation keeps of it would be large (2^-24 of 2^38, in the exponent).
     __device__ __forceinline__ void exponents(const float (&s)[4], const Query &q, float (&x)[4]) const {
-        if (far) {
-            x[0] = __fmul_rn(s[0], q.factor0) - m0, x[1] = __fmul_rn(s[1], q.factor1) - m1;
-            x[2] = __fmul_rn(s[2], q.factor0) - m0, x[3] = __fmul_rn(s[3], q.factor1) - m1;
-        } else {
-            x[0] = fmaf(s[0], q.factor0, -m0), x[1] = fmaf(s[1], q.factor1, -m1);
-            x[2] = fmaf(s[2], q.factor0, -m0), x[3] = fmaf(s[3], q.factor1, -m1);
-        }
+        x[0] = __fmul_rn(s[0], q.factor0) - m0, x[1] = __fmul_rn(s[1], q.factor1) - m1;
+        x[2] = __fmul_rn(s[2], q.factor0) - m0, x[3] = __fmul_rn(s[3], q.factor1) - m1;
     }
 
     // References for scores that reach top0 and top1 in this lane.
@@ -359,8 +352,6 @@ struct Sums {
         const float alpha0 = pkv::exp2_approx(m0 - top0), alpha1 = pkv::exp2_approx(m1 - top1);
         m0 = top0;
         m1 = top1;
-        far = __any_sync(0xffffffffu, fmaxf(m0, m1) > kFarScore || (m0 < -kFarScore && m0 > kLowest) ||
-                                          (m1 < -kFarScore && m1 > kLowest));
         l0 *= alpha0;
         l1 *= alpha1;
 #pragma unroll
@@ -368,7 +359,7 @@ struct Sums {
     }
 };
 
-// Where a lane reads its bytes of a (block, head), as shared memory addresses for block 0 of stage 0.
+// Where a lane reads its bytes of a (block, head), as shared memory addresses.
 struct Places {
     uint32_t k, v, ks, vs;
 
@@ -379,18 +370,28 @@ struct Places {
         ks = head + pkv::int4::scale_at(pkv::int4::kKeyScaleAt, t, 2 * g);
         vs = head + pkv::int4::scale_at(pkv::int4::kValueScaleAt, g >> 1, 4 * t);
     }
+
+    __device__ __forceinline__ Places at(uint32_t bytes) const {
+        Places p = *this;
+        p.k += bytes, p.v += bytes, p.ks += bytes, p.vs += bytes;
+        return p;
+    }
 };
 
 struct Tile {
     uint4 k, v;
     uint32_t ks, vs;
 
-    // Block at byte `at` of the ring.
-    __device__ __forceinline__ void load(const Places &p, uint32_t at) {
-        asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(k.x), "=r"(k.y), "=r"(k.z), "=r"(k.w) : "r"(p.k + at));
-        asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(p.v + at));
-        asm volatile("ld.shared.u16 %0, [%1];" : "=r"(ks) : "r"(p.ks + at));
-        asm volatile("ld.shared.u32 %0, [%1];" : "=r"(vs) : "r"(p.vs + at));
+    // Block BLOCK of the stage at `p`.
+    template <int BLOCK>
+    __device__ __forceinline__ void load(const Places &p) {
+        constexpr int kAt = BLOCK * pkv::int4::kBlockBytes;
+        asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4 + %5];"
+                     : "=r"(k.x), "=r"(k.y), "=r"(k.z), "=r"(k.w) : "r"(p.k), "n"(kAt));
+        asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4 + %5];"
+                     : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(p.v), "n"(kAt));
+        asm volatile("ld.shared.u16 %0, [%1 + %2];" : "=r"(ks) : "r"(p.ks), "n"(kAt));
+        asm volatile("ld.shared.u32 %0, [%1 + %2];" : "=r"(vs) : "r"(p.vs), "n"(kAt));
     }
 };
 
@@ -557,7 +558,7 @@ __global__ void __launch_bounds__(kThreads, 3) int4_decode_kernel(const __grid_c
                           (length - 1) & (kSlots - 1), lane);
             }
             const int tokens = min(max(length - (i - row_first) * kSlots, 0), n * kSlots);  // valid ones of the chunk
-            const uint32_t at = stage * kStageBytes;
+            const Places here = places.at(stage * kStageBytes);
             const auto release = [&] {
                 // Every lane has read the stage (the fence orders the reads before the copies, the
                 // warp barrier the lanes): it may be filled again.
@@ -567,18 +568,18 @@ __global__ void __launch_bounds__(kThreads, 3) int4_decode_kernel(const __grid_c
             };
             if (tokens == kChunk * kSlots) {
                 Tile tile[2];
-                tile[0].load(places, at);
-                tile[1].load(places, at + pkv::int4::kBlockBytes);
+                tile[0].load<0>(here);
+                tile[1].load<1>(here);
                 attend<NEW, 2, false>(tile, 0, q, sums, lane);
-                tile[0].load(places, at + 2 * pkv::int4::kBlockBytes);
-                tile[1].load(places, at + 3 * pkv::int4::kBlockBytes);
+                tile[0].load<2>(here);
+                tile[1].load<3>(here);
                 release();
                 attend<NEW, 2, false>(tile, 0, q, sums, lane);
             } else {
 #pragma unroll 1
                 for (int b = 0; b < n; ++b) {
                     Tile tile[1];
-                    tile[0].load(places, at + b * pkv::int4::kBlockBytes);
+                    tile[0].load<0>(here.at(b * pkv::int4::kBlockBytes));
                     if (b + 1 == n) release();
                     attend<NEW, 1, true>(tile, tokens - b * kSlots, q, sums, lane);
                 }
