@@ -1,9 +1,10 @@
-"""Build the native library ``libpagedkv.so`` in-tree for sm_100a.
+"""Build the native library ``libpagedkv.so`` and the extension ``_int4_ops.so`` in-tree for sm_100a.
 
 The library holds the C++ block ledger and the CUDA kernels behind the C ABI
 declared in ``include/pagedkv.h``.  It is compiled with nvcc for
 ``arch=compute_100a,code=sm_100a`` and links the CUDA runtime statically, so
-it loads (and the ledger runs) on machines without a GPU.
+it loads (and the ledger runs) on machines without a GPU.  The extension binds
+the 4-bit cache's operators of the library to torch tensors (host code only).
 
 Usage: ``python -m pagedcore_b200.build [--force]``.
 """
@@ -14,6 +15,7 @@ import os
 import shutil
 import subprocess
 import sys
+import sysconfig
 from pathlib import Path
 
 PACKAGE_DIR = Path(__file__).resolve().parent
@@ -21,6 +23,8 @@ REPO_ROOT = PACKAGE_DIR.parent
 CSRC = PACKAGE_DIR / "csrc"
 INCLUDE = REPO_ROOT / "include"
 LIBRARY = PACKAGE_DIR / "libpagedkv.so"
+BINDING = CSRC / "binding" / "int4_ops.cpp"
+EXTENSION = PACKAGE_DIR / "_int4_ops.so"
 
 ARCH_FLAGS = ["-gencode", "arch=compute_100a,code=sm_100a"]
 
@@ -33,11 +37,22 @@ def _inputs() -> list[Path]:
     return [*sources(), *CSRC.glob("*.h"), *CSRC.glob("*.cuh"), *INCLUDE.glob("*.h")]
 
 
-def up_to_date() -> bool:
+def _library_up_to_date() -> bool:
     if not LIBRARY.exists():
         return False
     built = LIBRARY.stat().st_mtime
     return all(path.stat().st_mtime <= built for path in _inputs())
+
+
+def _extension_up_to_date() -> bool:
+    if not EXTENSION.exists():
+        return False
+    built = EXTENSION.stat().st_mtime
+    return all(path.stat().st_mtime <= built for path in (BINDING, *INCLUDE.glob("*.h")))
+
+
+def up_to_date() -> bool:
+    return _library_up_to_date() and _extension_up_to_date()
 
 
 def nvcc() -> str:
@@ -51,9 +66,15 @@ def nvcc() -> str:
 
 
 def build(force: bool = False, verbose: bool = False) -> Path:
-    """Compile every source into ``libpagedkv.so`` (skipped when up to date)."""
-    if not force and up_to_date():
-        return LIBRARY
+    """Compile every source into ``libpagedkv.so``, then the extension (each skipped when up to date)."""
+    if force or not _library_up_to_date():
+        _build_library(verbose)
+    if force or not _extension_up_to_date():
+        _build_extension(verbose)
+    return LIBRARY
+
+
+def _build_library(verbose: bool) -> None:
     tmp = LIBRARY.with_suffix(".so.tmp")
     command = [
         nvcc(),
@@ -74,14 +95,54 @@ def build(force: bool = False, verbose: bool = False) -> Path:
     ]
     if verbose:
         command.insert(1, "-Xptxas=-v")
+    _run(command, tmp, LIBRARY, verbose)
+
+
+def _build_extension(verbose: bool) -> None:
+    import torch
+
+    root = Path(torch.__file__).resolve().parent
+    cuda = Path(nvcc()).resolve().parents[1]
+    tmp = EXTENSION.with_suffix(".so.tmp")
+    command = [
+        os.environ.get("CXX", "g++"),
+        "-O2",
+        "-std=c++17",
+        "-fPIC",
+        "-shared",
+        "-fvisibility=hidden",
+        f"-D_GLIBCXX_USE_CXX11_ABI={int(torch.compiled_with_cxx11_abi())}",
+        f"-I{INCLUDE}",
+        f"-I{root / 'include'}",
+        f"-I{root / 'include' / 'torch' / 'csrc' / 'api' / 'include'}",
+        f"-I{cuda / 'include'}",
+        f"-I{sysconfig.get_paths()['include']}",
+        str(BINDING),
+        "-o",
+        str(tmp),
+        f"-L{root / 'lib'}",
+        "-ltorch_python",
+        "-ltorch_cuda",
+        "-ltorch_cpu",
+        "-ltorch",
+        "-lc10",
+        "-lc10_cuda",
+        f"-L{PACKAGE_DIR}",
+        f"-l:{LIBRARY.name}",
+        "-Wl,-rpath,$ORIGIN",
+    ]
+    _run(command, tmp, EXTENSION, verbose)
+
+
+def _run(command: list[str], tmp: Path, target: Path, verbose: bool) -> None:
+    if verbose:
         print(" ".join(command), file=sys.stderr)
     result = subprocess.run(command, capture_output=True, text=True)
     if result.returncode != 0:
-        raise RuntimeError(f"building libpagedkv.so failed:\n{result.stdout}\n{result.stderr}")
+        raise RuntimeError(f"building {target.name} failed:\n{result.stdout}\n{result.stderr}")
     if verbose and result.stderr:
         print(result.stderr, file=sys.stderr)
-    os.replace(tmp, LIBRARY)
-    return LIBRARY
+    os.replace(tmp, target)
 
 
 if __name__ == "__main__":
