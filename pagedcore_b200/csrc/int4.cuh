@@ -90,14 +90,20 @@ __device__ __forceinline__ void encode_group(const float (&v)[16], uint32_t (&wo
 #pragma unroll
     for (int i = 0; i < 16; ++i) top = max(top, __float_as_uint(v[i]) & 0x7fffffffu);
     scale = scale_of(top);
-    const float s = scale == 0 ? 1.f : scale_value(scale);
+    // x / s rounded as a division rounds it, since ties must stay ties: from 1 / s, correctly
+    // rounded, a quotient within a unit of its last place takes one exact remainder (Markstein's
+    // theorem; nothing here is near the ends of FP32's range).
+    const float s = scale == 0 ? 1.f : scale_value(scale), inverse = __frcp_rn(s);
 #pragma unroll
     for (int w = 0; w < 2; ++w) {
         uint32_t word = 0;
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
-            const int code = __float2int_rn(fminf(fmaxf(__fdiv_rn(v[8 * w + i], s), -7.f), 7.f));
-            word |= static_cast<uint32_t>(code + 8) << (4 * (i >> 1) + 16 * (i & 1));
+            const float x = v[8 * w + i], q = x * inverse;
+            const float quotient = fmaf(fmaf(-q, s, x), inverse, q);
+            // The sum's unit is 1: the nearest integer, ties to even, plus 8, in its low bits.
+            const uint32_t code = __float_as_uint(fminf(fmaxf(quotient, -7.f), 7.f) + (0x1.8p23f + 8.f));
+            word |= (code & 15u) << (4 * (i >> 1) + 16 * (i & 1));
         }
         words[w] = ((word << 2) & 0xfffcfffcu) | ((word >> 14) & 0x00030003u);
     }
@@ -175,9 +181,10 @@ __device__ __forceinline__ void key_group(const __half *row, int t, bool here, c
         for (int i = 0; i < 16; ++i) v[i] = v[i] * cos[i] + other[i] * sin[i];
         return;
     }
-    double sum = 0;
+    double part[4] = {0, 0, 0, 0};  // four short chains
 #pragma unroll
-    for (int i = 0; i < 16; ++i) sum = fma(static_cast<double>(v[i]), static_cast<double>(v[i]), sum);
+    for (int i = 0; i < 16; ++i) part[i & 3] = fma(static_cast<double>(v[i]), static_cast<double>(v[i]), part[i & 3]);
+    double sum = (part[0] + part[1]) + (part[2] + part[3]);
     sum += __shfl_xor_sync(0xffffffffu, sum, 1);
     sum += __shfl_xor_sync(0xffffffffu, sum, 2);
     const double inverse = rsqrt(sum * (1.0 / PKV_HEAD_DIM) + eps);

@@ -57,8 +57,12 @@ constexpr int kStageBytes = kChunk * pkv::int4::kBlockBytes;
 constexpr int kFreshBytes = 320;  // a row's new token as it is stored: 72 bytes a head, and whether there is one
 constexpr int kFreshOk = 4 * 72;
 constexpr int kFreshAt = kStages * kStageBytes;
-constexpr int kSmem = kFreshAt + kStages * kFreshBytes;
+constexpr int kFresh = kStages + 1;  // rows whose last chunk is in the ring, and the one that is prepared
+constexpr int kSmem = kFreshAt + kFresh * kFreshBytes;
 constexpr uint32_t kWaitPolls = 1u << 24;
+constexpr int kRowCost = 3;  // below a chunk's blocks
+constexpr int kWeighedRows = 256;
+static_assert(kRowCost < kChunk, "a piece could lie in the cost of one row");
 constexpr float kScaleLog2 = 0.125f * 1.4426950408889634f;  // 64^-0.5 * log2(e)
 constexpr float kValueFactor = 0x1p-6f;  // of the values in the MMAs
 constexpr float kMostWeight = 15.0f;  // log2 of the largest weight
@@ -93,21 +97,86 @@ struct Args {
     int32_t *error_flag;
 };
 
-// Piece g covers blocks [g * total / pieces, (g + 1) * total / pieces).
-__device__ __forceinline__ int piece_begin(int g, int total, int pieces) {
-    return static_cast<int>(static_cast<int64_t>(g) * total / pieces);
-}
-
-__device__ __forceinline__ int piece_of(int block, int total, int pieces) {
-    return static_cast<int>(((static_cast<int64_t>(block) + 1) * pieces - 1) / total);
-}
-
-// Pieces of a list of `total` blocks: at most one per CTA and per chunk, so
-// none is empty.  (A captured launch has a CTA for every resident slot.)
+// Pieces of a list of `total` blocks: at most one per CTA and per chunk.  (A captured
+// launch has a CTA for every resident slot.)
 __host__ __device__ __forceinline__ int pieces_of(int total, int grid) {
     const int most = (total + kChunk - 1) / kChunk;
     return most < 1 ? 1 : most < grid ? most : grid;
 }
+
+// How the list is cut: a block weighs 1 and a row's first block kRowCost more, what it costs a
+// CTA to begin a row (its queries, its result); piece g holds the blocks whose weights, summed to
+// and without the block itself, lie in [g, g + 1) * weight / pieces.  A piece is at least a chunk
+// long, so none is without blocks.  Beyond kWeighedRows rows, where a CTA has several rows and
+// they even out, rows weigh nothing.  (256 rows of 1 to 2048 tokens: MEASURED.)
+struct Cut {
+    int total, pieces;
+    int64_t weight;
+
+    __device__ __forceinline__ Cut(const Args &a, int rows_with_blocks) {
+        total = total_blocks(a);
+        pieces = pieces_of(total, a.grid);
+        weight = static_cast<int64_t>(total) + kRowCost * rows_with_blocks;
+    }
+    // Of block `block` in the list's `rank`-th row with blocks (counted from 1).
+    __device__ __forceinline__ int piece_of(int block, int rank) const {
+        return static_cast<int>((static_cast<int64_t>(block) + kRowCost * rank) * pieces / weight);
+    }
+    // The least weight that is in piece g.
+    __device__ __forceinline__ int64_t begins(int g) const { return (g * weight + pieces - 1) / pieces; }
+};
+
+// The rows of a list of up to kWeighedRows rows, 32 k + lane in each lane.
+struct RowScan {
+    static constexpr int kParts = kWeighedRows / 32;
+    int first[kParts], last[kParts];
+    unsigned held[kParts];  // rows with blocks
+
+    __device__ __forceinline__ RowScan(const Args &a, int lane) {
+#pragma unroll
+        for (int k = 0; k < kParts; ++k) {
+            const int r = 32 * k + lane;
+            first[k] = last[k] = 0;
+            if (r < a.batch) first[k] = a.prefix[r], last[k] = a.prefix[r + 1];
+        }
+#pragma unroll
+        for (int k = 0; k < kParts; ++k) held[k] = __ballot_sync(0xffffffffu, last[k] > first[k]);
+    }
+    __device__ __forceinline__ int rows_with_blocks() const {
+        int count = 0;
+#pragma unroll
+        for (int k = 0; k < kParts; ++k) count += __popc(held[k]);
+        return count;
+    }
+    __device__ __forceinline__ int rank(int row) const {
+        int count = 0;
+#pragma unroll
+        for (int k = 0; k < kParts; ++k) {
+            const int upto = row - 32 * k;  // rows of this part that count
+            if (upto >= 0) count += __popc(upto >= 31 ? held[k] : held[k] & ((2u << upto) - 1u));
+        }
+        return count;
+    }
+    // The first block of weight `target` or more, and its row; `total` where there is none.
+    __device__ __forceinline__ int block_at(int64_t target, int total, int lane, int &row) const {
+        int before = 0;
+#pragma unroll
+        for (int k = 0; k < kParts; ++k) {
+            const int cost = kRowCost * (before + __popc(held[k] & ((2u << lane) - 1u)));
+            const bool past = last[k] > first[k] && static_cast<int64_t>(last[k]) - 1 + cost >= target;
+            const unsigned found = __ballot_sync(0xffffffffu, past);
+            if (found != 0) {
+                const int from = __ffs(found) - 1;
+                row = 32 * k + from;
+                const int64_t block = max(static_cast<int64_t>(first[k]), target - cost);
+                return __shfl_sync(0xffffffffu, static_cast<int>(min(max(block, int64_t{0}), static_cast<int64_t>(total))), from);
+            }
+            before += __popc(held[k]);
+        }
+        row = INT32_MAX;
+        return total;
+    }
+};
 
 // D = A(16x16, row) * B(16x8, col) + D, FP16 operands.
 __device__ __forceinline__ void mma(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
@@ -198,6 +267,12 @@ struct Query {
     }
 };
 
+// A head's queries of a row into L1.
+__device__ __forceinline__ void prefetch_query(const Args &a, int row, int warp, int lane) {
+    const __half *at = a.query + row * a.query_stride + warp * kHeadGroup * kDim + lane * 16;
+    asm volatile("prefetch.global.L1 [%0];" ::"l"(at));
+}
+
 // Copies of memory that one CTA reads once.
 __device__ __forceinline__ void bulk_load(uint32_t dst, const void *src, uint32_t bytes, uint32_t bar, uint64_t policy) {
     asm volatile(
@@ -261,9 +336,10 @@ __device__ __forceinline__ void put_fresh(const uint8_t *fresh, int warp, uint8_
 }
 
 // The producer warp: copies the blocks of [begin, end) chunk by chunk, a chunk ending with its
-// row, and writes the new token of each row that ends here.
+// row, and writes the new token of each row that ends here: while it would wait for a free
+// stage, or when the row's last chunk is on its way.
 template <bool NEW>
-__device__ __forceinline__ void fill_ring(const Args &a, int begin, int end, Rows rows, int row, int lane, uint8_t *smem,
+__device__ __forceinline__ void fill_ring(const Args &a, int begin, int end, int row, int lane, uint8_t *smem,
                                           uint64_t *full, uint64_t *empty) {
     const uint64_t policy = pkv::l2_policy_evict_first();
     const uint32_t ring = pkv::smem_addr(smem);
@@ -271,15 +347,23 @@ __device__ __forceinline__ void fill_ring(const Args &a, int begin, int end, Row
     int ids_base = begin;
     int ids = begin + lane < end ? a.flat[begin + lane] : 0;
     int ids_next = begin + 32 + lane < end ? a.flat[begin + 32 + lane] : 0;
-    int row_end = __shfl_sync(0xffffffffu, rows.last, row - rows.base);
+    Rows rows = load_rows(a, row, lane);
+    int row_end = __shfl_sync(0xffffffffu, rows.last, 0);
     int issued = 0;
     bool ok = true;
+    int prepared = -1, ended = 0;  // the row whose new token is in place, and rows that ended
+    const auto prepare = [&] {
+        const int length = __shfl_sync(0xffffffffu, rows.length, row - rows.base);
+        write_new(a, row, length, a.flat[row_end - 1], lane, smem + kFreshAt + ended % kFresh * kFreshBytes);
+        __syncwarp();
+        prepared = row;
+    };
     for (int at = begin; at < end;) {
         if (at >= row_end) {
             row = advance_row(a, rows, row + 1, at, lane);
+            if (row >= a.batch) break;  // prefix does not grow from row to row: the consumers stop here too
             row_end = __shfl_sync(0xffffffffu, rows.last, row - rows.base);
         }
-        if (row >= a.batch) break;  // prefix does not grow from row to row: the consumers stop here too
         const int n = min(kChunk, min(row_end, end) - at);
         if (at - ids_base >= 32) {
             ids = ids_next;
@@ -290,13 +374,15 @@ __device__ __forceinline__ void fill_ring(const Args &a, int begin, int end, Row
         const int offset = at - ids_base + min(lane, n - 1);
         const int near = __shfl_sync(0xffffffffu, ids, offset & 31);
         const int far = __shfl_sync(0xffffffffu, ids_next, offset & 31);
-        const int block = offset < 32 ? near : far;  // of lane's copy; from lane n - 1 on the last one
+        const int block = offset < 32 ? near : far;  // of lane's copy
         const bool bad = block < 0 || block >= a.cache.num_blocks;  // reported, and read as zeros
         if (bad && lane < n) atomicOr(a.error_flag, PKV_DEVICE_BAD_BLOCK);
         const int stage = issued % kStages;
+        const bool fresh = NEW && row_end <= end;  // the row ends here
         if (issued >= kStages) {
-            ok = wait_bounded(pkv::smem_addr(&empty[stage]), (issued / kStages - 1) & 1);
-            ok = __all_sync(0xffffffffu, ok);
+            const uint32_t bar = pkv::smem_addr(&empty[stage]), parity = (issued / kStages - 1) & 1;
+            if (fresh && prepared != row && !__all_sync(0xffffffffu, pkv::mbar_test_wait(bar, parity))) prepare();
+            ok = __all_sync(0xffffffffu, wait_bounded(bar, parity));
             if (!ok) break;  // a consumer gave up
         }
         const uint32_t bar = pkv::smem_addr(&full[stage]);
@@ -306,10 +392,9 @@ __device__ __forceinline__ void fill_ring(const Args &a, int begin, int end, Row
             bulk_load(ring + stage * kStageBytes + lane * pkv::int4::kBlockBytes,
                       bad ? kZeroBlock : pkv::int4::block_at(a.cache, a.layer, block), pkv::int4::kBlockBytes, bar, policy);
         }
-        if (NEW && at + n == row_end) {
-            const int length = __shfl_sync(0xffffffffu, rows.length, row - rows.base);
-            write_new(a, row, length, __shfl_sync(0xffffffffu, block, n - 1), lane, smem + kFreshAt + stage * kFreshBytes);
-            __syncwarp();
+        if (fresh && at + n == row_end) {
+            if (prepared != row) prepare();
+            ++ended;
         }
         if (lane == 0) pkv::mbar_arrive(bar);
         at += n;
@@ -496,11 +581,33 @@ __global__ void __launch_bounds__(kThreads, 3) int4_decode_kernel(const __grid_c
     pkv::pdl_wait();
     pkv::pdl_launch_dependents();
 
-    // The piece, and a first cut of the rows: 32 samples of prefix, `step` rows apart.
-    int step = (a.batch + 31) / 32;
-    int sample = lane * step < a.batch ? a.prefix[min((lane + 1) * step, a.batch)] : INT32_MAX;
-    const int total = total_blocks(a);
-    const int pieces = pieces_of(total, a.grid);
+    // The piece and the row that it begins in.
+    int begin, end, row;
+    int pieces;
+    if (a.batch <= kWeighedRows) {
+        const RowScan scan(a, lane);
+        const Cut cut(a, scan.rows_with_blocks());
+        pieces = cut.total > 0 ? cut.pieces : 0;
+        int other;
+        begin = scan.block_at(cut.begins(blockIdx.x), cut.total, lane, row);
+        end = scan.block_at(cut.begins(blockIdx.x + 1), cut.total, lane, other);
+    } else {
+        // Of 32 samples of prefix, `step` rows apart, the first past `begin`, cut finer until the
+        // samples are rows.
+        int step = (a.batch + 31) / 32;
+        int sample = lane * step < a.batch ? a.prefix[min((lane + 1) * step, a.batch)] : INT32_MAX;
+        const Cut cut(a, 0);
+        pieces = cut.total > 0 ? cut.pieces : 0;
+        begin = static_cast<int>(cut.begins(blockIdx.x)), end = static_cast<int>(cut.begins(blockIdx.x + 1));
+        row = 0;
+        while (true) {
+            const unsigned past = __ballot_sync(0xffffffffu, sample > begin);
+            row += (past != 0 ? __ffs(past) - 1 : 31) * step;
+            if (step == 1) break;
+            step = (step + 31) / 32;
+            sample = row + lane * step < a.batch ? a.prefix[min(row + (lane + 1) * step, a.batch)] : INT32_MAX;
+        }
+    }
     // Rows without blocks: zeros.  (The merge looks at the rows' order too, where there is one.)
     for (int b = blockIdx.x * kThreads + threadIdx.x; (a.clear || a.grid == 1) && b < a.batch; b += a.grid * kThreads) {
         const int first = a.prefix[b], last = a.prefix[b + 1];
@@ -509,28 +616,19 @@ __global__ void __launch_bounds__(kThreads, 3) int4_decode_kernel(const __grid_c
             for (int i = 0; i < kQueryHeads * kDim; ++i) a.out[b * a.out_stride + i] = __float2half_rn(0.f);
         }
     }
-    if (total == 0 || static_cast<int>(blockIdx.x) >= pieces) return;
-    const int begin = piece_begin(blockIdx.x, total, pieces);
-    const int end = piece_begin(blockIdx.x + 1, total, pieces);
-    // The first row with blocks past `begin`: the first sample past it, cut finer until
-    // the samples are rows.
-    int lo = 0;
-    while (true) {
-        const unsigned past = __ballot_sync(0xffffffffu, sample > begin);
-        lo += (past != 0 ? __ffs(past) - 1 : 31) * step;
-        if (step <= 32) break;
-        step = (step + 31) / 32;
-        sample = lo + lane * step < a.batch ? a.prefix[min(lo + (lane + 1) * step, a.batch)] : INT32_MAX;
-    }
-    Rows rows = load_rows(a, lo, lane);
-    int row = advance_row(a, rows, lo, begin, lane);
-    if (warp == kProducer) {
-        if (row < a.batch) fill_ring<NEW>(a, begin, end, rows, row, lane, smem, full, empty);
+    if (static_cast<int>(blockIdx.x) >= pieces || begin >= end) return;
+    if (row >= a.batch) {  // prefix does not grow from row to row
+        if (threadIdx.x == 0) atomicOr(a.error_flag, PKV_DEVICE_BAD_BLOCK);
         return;
     }
+    if (warp == kProducer) {
+        fill_ring<NEW>(a, begin, end, row, lane, smem, full, empty);
+        return;
+    }
+    Rows rows = load_rows(a, row, lane);
 
     const Places places(pkv::smem_addr(smem) + warp * pkv::int4::kHeadBytes, lane);
-    int consumed = 0;
+    int consumed = 0, ended = 0;
     bool failed = false;
     int i = begin;
     while (i < end) {
@@ -544,6 +642,11 @@ __global__ void __launch_bounds__(kThreads, 3) int4_decode_kernel(const __grid_c
         const int seg_end = min(end, row_last);
         Query q;
         q.load<NEW>(a, row, length, warp, lane);
+        int next = row;
+        if (row_last < end) {  // the next row's queries are brought near while this one streams
+            next = advance_row(a, rows, row + 1, row_last, lane);
+            if (next < a.batch) prefetch_query(a, next, warp, lane);
+        }
         Sums sums;
         sums.clear();
         while (i < seg_end) {
@@ -553,7 +656,7 @@ __global__ void __launch_bounds__(kThreads, 3) int4_decode_kernel(const __grid_c
             failed = __any_sync(0xffffffffu, failed);
             if (failed) break;
             if (NEW && i + n == row_last) {
-                put_fresh(smem + kFreshAt + stage * kFreshBytes, warp,
+                put_fresh(smem + kFreshAt + ended++ % kFresh * kFreshBytes, warp,
                           smem + stage * kStageBytes + (n - 1) * pkv::int4::kBlockBytes + warp * pkv::int4::kHeadBytes,
                           (length - 1) & (kSlots - 1), lane);
             }
@@ -621,8 +724,7 @@ __global__ void __launch_bounds__(kThreads, 3) int4_decode_kernel(const __grid_c
                     make_float4(sums.m0, l0, sums.m1, l1);
             }
         }
-        if (row_last < end) row = advance_row(a, rows, row + 1, row_last, lane);
-        else break;
+        row = next;
     }
     if (failed && lane == 0) atomicOr(a.error_flag, PKV_DEVICE_WAIT_TIMEOUT);
 }
@@ -645,14 +747,20 @@ __global__ void __launch_bounds__(kMergeThreads) int4_merge_kernel(const __grid_
     // The tables are older than the split kernel: it lets this one start only after
     // its own wait for what came before.
     int first = 0, last = 0;
+    const int row_at = min(row, a.batch - 1);
+    const int first_block = a.prefix[row_at], last_block = a.prefix[row_at + 1] - 1;
+    int rank = 0, rows_with_blocks = 0;
+    if (a.batch <= kWeighedRows) {
+        const RowScan scan(a, lane);
+        rank = scan.rank(row_at);
+        rows_with_blocks = scan.rows_with_blocks();
+    }
+    const Cut cut(a, rows_with_blocks);
     if (row < a.batch) {
-        const int first_block = a.prefix[row], last_block = a.prefix[row + 1] - 1;
-        const int total = total_blocks(a);
         if (lane == 0 && out_of_order(row, first_block, last_block + 1)) atomicOr(a.error_flag, PKV_DEVICE_BAD_BLOCK);
-        if (last_block >= first_block && first_block >= 0 && last_block < total) {
-            const int pieces = pieces_of(total, a.grid);
-            first = piece_of(first_block, total, pieces);
-            last = piece_of(last_block, total, pieces);
+        if (last_block >= first_block && first_block >= 0 && last_block < cut.total) {
+            first = cut.piece_of(first_block, rank);
+            last = min(cut.piece_of(last_block, rank), cut.pieces - 1);
         }
     }
     pkv::pdl_wait();
