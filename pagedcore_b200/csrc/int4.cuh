@@ -84,29 +84,55 @@ __device__ __forceinline__ float scale_value(uint32_t scale) {
     return __half2float(__ushort_as_half(static_cast<unsigned short>(scale << 7)));
 }
 
-// A group's 16 values to its two words of codes and its scale.
-__device__ __forceinline__ void encode_group(const float (&v)[16], uint32_t (&words)[2], uint32_t &scale) {
+// A group's scale as the divisor of its values.
+struct Divisor {
+    float scale, inverse;
+
+    __device__ __forceinline__ explicit Divisor(uint32_t byte) {
+        scale = byte == 0 ? 1.f : scale_value(byte);
+        inverse = __frcp_rn(scale);
+    }
+    // The code of x, plus 8.  x / s is rounded as a division rounds it, since ties must stay ties:
+    // from 1 / s, correctly rounded, a quotient within a unit of its last place takes one exact
+    // remainder (Markstein's theorem; nothing here is near the ends of FP32's range).
+    __device__ __forceinline__ uint32_t code(float x) const {
+        const float q = x * inverse;
+        const float quotient = fmaf(fmaf(-q, scale, x), inverse, q);
+        // The sum's unit is 1: the nearest integer, ties to even, plus 8, in its low bits.
+        return __float_as_uint(fminf(fmaxf(quotient, -7.f), 7.f) + (0x1.8p23f + 8.f)) & 15u;
+    }
+};
+
+__device__ __forceinline__ uint32_t rotate_halves(uint32_t word) {
+    return ((word << 2) & 0xfffcfffcu) | ((word >> 14) & 0x00030003u);
+}
+
+// Dims 2 l and 2 l + 1 of a token's 64, by the lanes l of a warp, to the word of codes of
+// the lane's eight dims (the same in the four lanes that share them) and its group's scale.
+__device__ __forceinline__ void encode_pair(float x, float y, int lane, uint32_t &word, uint32_t &scale) {
+    uint32_t top = max(__float_as_uint(x) & 0x7fffffffu, __float_as_uint(y) & 0x7fffffffu);
+#pragma unroll
+    for (int offset = 1; offset < 8; offset <<= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, offset));
+    scale = scale_of(top);
+    const Divisor by(scale);
+    word = (by.code(x) | by.code(y) << 16) << (4 * (lane & 3));
+    word |= __shfl_xor_sync(0xffffffffu, word, 1);
+    word |= __shfl_xor_sync(0xffffffffu, word, 2);
+    word = rotate_halves(word);
+}
+
+// Dims 8 c .. + 7 of a token, by lane c of its eight, to their word and their group's scale.
+__device__ __forceinline__ void encode_chunk(const float (&v)[8], uint32_t &word, uint32_t &scale) {
     uint32_t top = 0;
 #pragma unroll
-    for (int i = 0; i < 16; ++i) top = max(top, __float_as_uint(v[i]) & 0x7fffffffu);
+    for (int i = 0; i < 8; ++i) top = max(top, __float_as_uint(v[i]) & 0x7fffffffu);
+    top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
     scale = scale_of(top);
-    // x / s rounded as a division rounds it, since ties must stay ties: from 1 / s, correctly
-    // rounded, a quotient within a unit of its last place takes one exact remainder (Markstein's
-    // theorem; nothing here is near the ends of FP32's range).
-    const float s = scale == 0 ? 1.f : scale_value(scale), inverse = __frcp_rn(s);
+    const Divisor by(scale);
+    word = 0;
 #pragma unroll
-    for (int w = 0; w < 2; ++w) {
-        uint32_t word = 0;
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-            const float x = v[8 * w + i], q = x * inverse;
-            const float quotient = fmaf(fmaf(-q, s, x), inverse, q);
-            // The sum's unit is 1: the nearest integer, ties to even, plus 8, in its low bits.
-            const uint32_t code = __float_as_uint(fminf(fmaxf(quotient, -7.f), 7.f) + (0x1.8p23f + 8.f));
-            word |= (code & 15u) << (4 * (i >> 1) + 16 * (i & 1));
-        }
-        words[w] = ((word << 2) & 0xfffcfffcu) | ((word >> 14) & 0x00030003u);
-    }
+    for (int i = 0; i < 8; ++i) word |= by.code(v[i]) << (4 * (i >> 1) + 16 * (i & 1));
+    word = rotate_halves(word);
 }
 
 // Byte offsets in a (block, head) of one token's words and scale in group t.
@@ -116,16 +142,15 @@ __device__ __forceinline__ int value_word(int chunk, int token) {
 }
 __device__ __forceinline__ int scale_at(int first, int t, int token) { return first + t * PKV_BLOCK_TOKENS + token; }
 
-// One group of a token into the (block, head) at `head`, memory of either kind.
-__device__ __forceinline__ void store_key(uint8_t *head, int t, int token, const uint32_t (&words)[2], uint32_t scale) {
-    *reinterpret_cast<uint2 *>(head + key_words(t, token)) = make_uint2(words[0], words[1]);
-    head[scale_at(kKeyScaleAt, t, token)] = static_cast<uint8_t>(scale);
+// The word of chunk c of a token, and in even chunks its group's scale, into the (block, head) at `head`.
+__device__ __forceinline__ void store_key(uint8_t *head, int c, int token, uint32_t word, uint32_t scale) {
+    *reinterpret_cast<uint32_t *>(head + key_words(c >> 1, token) + 4 * (c & 1)) = word;
+    if ((c & 1) == 0) head[scale_at(kKeyScaleAt, c >> 1, token)] = static_cast<uint8_t>(scale);
 }
 
-__device__ __forceinline__ void store_value(uint8_t *head, int t, int token, const uint32_t (&words)[2], uint32_t scale) {
-    *reinterpret_cast<uint32_t *>(head + value_word(2 * t, token)) = words[0];
-    *reinterpret_cast<uint32_t *>(head + value_word(2 * t + 1, token)) = words[1];
-    head[scale_at(kValueScaleAt, t, token)] = static_cast<uint8_t>(scale);
+__device__ __forceinline__ void store_value(uint8_t *head, int c, int token, uint32_t word, uint32_t scale) {
+    *reinterpret_cast<uint32_t *>(head + value_word(c, token)) = word;
+    if ((c & 1) == 0) head[scale_at(kValueScaleAt, c >> 1, token)] = static_cast<uint8_t>(scale);
 }
 
 // The FP16 pairs 256 + n (nibbles 0, 2) and 16 + n (nibbles 1, 3) of a word; `swapped` is the word
@@ -155,48 +180,44 @@ __device__ __forceinline__ void load16(const __half *p, float (&v)[16]) {
     }
 }
 
-// Dims 16 t .. + 15 of a K row as it is stored: with `weight` the norm of the head
-// (x * rsqrt(mean(x^2) + eps) * weight) first, with `rope` the rotation at `position`.  The
-// four lanes of a row call it together; `here` says whether there is a row.  The norm is
-// taken in FP64: its result is rounded to codes next, and a value beside the border between
-// two must not depend on the order of a sum (60 such operations a lane, which cost nothing
-// beside the loads).  Without it FP32 is enough: products of FP16 numbers are exact in it, so
-// each rotated value is rounded once.
-__device__ __forceinline__ void key_group(const __half *row, int t, bool here, const __half *weight, double eps,
-                                          const __half *rope, int position, float (&v)[16]) {
-    constexpr int kHalf = PKV_HEAD_DIM / 2;
-    float other[16];  // the dims that rotate with these, 32 away
-#pragma unroll
-    for (int i = 0; i < 16; ++i) v[i] = other[i] = 0.f;
-    if (here) load16(row + kGroup * t, v);
-    if (rope == nullptr) return;
-    if (here) load16(row + kGroup * (t ^ 2), other);
-    float cos[16], sin[16];
-    load16(rope + position * kHalf + kGroup * (t & 1), cos);
-    load16(rope + (PKV_CONTEXT_LIMIT + position) * kHalf + kGroup * (t & 1), sin);
-#pragma unroll
-    for (int i = 0; i < 16; ++i) sin[i] = t < 2 ? -sin[i] : sin[i];
-    if (weight == nullptr) {
-#pragma unroll
-        for (int i = 0; i < 16; ++i) v[i] = v[i] * cos[i] + other[i] * sin[i];
-        return;
+// What turns a K row: dims 2 l and 2 l + 1 of the norm's weights and of the rotation, by lane.
+struct KeyTurn {
+    float2 weight, cos, sin;  // sin negative in the lower half of the dims
+
+    __device__ __forceinline__ KeyTurn(const __half *norm, const __half *rope, int position, int lane) {
+        constexpr int kHalf = PKV_HEAD_DIM / 2;
+        weight = cos = sin = make_float2(0.f, 0.f);
+        if (rope == nullptr) return;
+        const __half *at = rope + position * kHalf + (2 * lane) % kHalf;
+        cos = __half22float2(*reinterpret_cast<const __half2 *>(at));
+        sin = __half22float2(*reinterpret_cast<const __half2 *>(at + PKV_CONTEXT_LIMIT * kHalf));
+        if (lane < 16) sin = make_float2(-sin.x, -sin.y);
+        if (norm != nullptr) weight = __half22float2(*reinterpret_cast<const __half2 *>(norm + 2 * lane));
     }
-    double part[4] = {0, 0, 0, 0};  // four short chains
+};
+
+// Dims 2 l and 2 l + 1 of a K row as it is stored, by the lanes l of a warp: with NORM the norm
+// of the head (x * rsqrt(mean(x^2) + eps) * weight) first, then the rotation.  The norm is taken
+// in FP64: its result is rounded to codes next, and a value beside the border between two must
+// not depend on the order of a sum (it costs MEASURED).  Without it FP32 is enough: products of
+// FP16 numbers are exact in it, so each rotated value is rounded once.
+template <bool NORM>
+__device__ __forceinline__ float2 turn_key(__half2 row, const KeyTurn &turn, double eps) {
+    const float2 x = __half22float2(row);
+    if constexpr (!NORM) {
+        const uint32_t far = __shfl_xor_sync(0xffffffffu, pack_half2(row), 16);
+        const float2 y = __half22float2(*reinterpret_cast<const __half2 *>(&far));
+        return make_float2(x.x * turn.cos.x + y.x * turn.sin.x, x.y * turn.cos.y + y.y * turn.sin.y);
+    }
+    const double a = x.x, b = x.y;
+    double sum = fma(a, a, b * b);
 #pragma unroll
-    for (int i = 0; i < 16; ++i) part[i & 3] = fma(static_cast<double>(v[i]), static_cast<double>(v[i]), part[i & 3]);
-    double sum = (part[0] + part[1]) + (part[2] + part[3]);
-    sum += __shfl_xor_sync(0xffffffffu, sum, 1);
-    sum += __shfl_xor_sync(0xffffffffu, sum, 2);
+    for (int offset = 1; offset < 32; offset <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, offset);
     const double inverse = rsqrt(sum * (1.0 / PKV_HEAD_DIM) + eps);
-    float own[16], far[16];
-    load16(weight + kGroup * t, own);
-    load16(weight + kGroup * (t ^ 2), far);
-#pragma unroll
-    for (int i = 0; i < 16; ++i) {
-        const double x = v[i] * inverse * static_cast<double>(own[i]);
-        const double y = other[i] * inverse * static_cast<double>(far[i]);
-        v[i] = static_cast<float>(x * static_cast<double>(cos[i]) + y * static_cast<double>(sin[i]));
-    }
+    const double u = a * inverse * static_cast<double>(turn.weight.x), v = b * inverse * static_cast<double>(turn.weight.y);
+    const double far_u = __shfl_xor_sync(0xffffffffu, u, 16), far_v = __shfl_xor_sync(0xffffffffu, v, 16);
+    return make_float2(static_cast<float>(u * static_cast<double>(turn.cos.x) + far_u * static_cast<double>(turn.sin.x)),
+                       static_cast<float>(v * static_cast<double>(turn.cos.y) + far_v * static_cast<double>(turn.sin.y)));
 }
 
 }  // namespace pkv::int4

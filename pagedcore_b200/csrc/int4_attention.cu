@@ -54,11 +54,10 @@ constexpr int kThreads = (kWarps + 1) * 32;
 constexpr int kChunk = 4;  // blocks per stage, and the least of a piece
 constexpr int kStages = 2;
 constexpr int kStageBytes = kChunk * pkv::int4::kBlockBytes;
-constexpr int kFreshBytes = 320;  // a row's new token as it is stored: 72 bytes a head, and whether there is one
-constexpr int kFreshOk = 4 * 72;
+constexpr int kFreshBytes = 80;  // of a row's new token in one head, see write_new
+constexpr int kFreshOk = 72;
 constexpr int kFreshAt = kStages * kStageBytes;
-constexpr int kFresh = kStages + 1;  // rows whose last chunk is in the ring, and the one that is prepared
-constexpr int kSmem = kFreshAt + kFresh * kFreshBytes;
+constexpr int kSmem = kFreshAt + kWarps * kFreshBytes;
 constexpr uint32_t kWaitPolls = 1u << 24;
 constexpr int kRowCost = 3;  // below a chunk's blocks
 constexpr int kWeighedRows = 256;
@@ -281,10 +280,6 @@ __device__ __forceinline__ void bulk_load(uint32_t dst, const void *src, uint32_
         : "memory");
 }
 
-__device__ __forceinline__ void mbar_expect_tx(uint32_t bar, uint32_t bytes) {
-    asm volatile("mbarrier.expect_tx.relaxed.cta.shared::cta.b64 [%0], %1;" ::"r"(bar), "r"(bytes) : "memory");
-}
-
 __device__ __forceinline__ bool wait_bounded(uint32_t bar, uint32_t parity) {
     return pkv::mbar_test_wait(bar, parity) || pkv::mbar_wait_bounded(bar, parity, kWaitPolls);
 }
@@ -292,53 +287,59 @@ __device__ __forceinline__ bool wait_bounded(uint32_t bar, uint32_t parity) {
 // What a block id outside the cache reads as.
 __device__ __align__(16) const uint8_t kZeroBlock[pkv::int4::kBlockBytes] = {};
 
-// The new token of row `row` into its slot of `block`, and into `fresh` in shared memory: per
-// head 32 bytes of K codes, 32 of V codes and their scales.  Lane (head, K or V, group).
-__device__ __forceinline__ void write_new(const Args &a, int row, int length, int block, int lane, uint8_t *fresh) {
-    const int head = lane >> 3, t = lane & 3;
-    const bool is_key = (lane & 4) == 0;
+// The new token of row `row` into its slot of `block`, one head a warp, and into the warp's 80
+// bytes of shared memory at `fresh`: 32 of K codes, 32 of V codes, 4 + 4 scales, and whether there
+// is one.
+__device__ __forceinline__ void write_new(const Args &a, int row, int length, int block, int warp, int lane, uint8_t *fresh) {
     const bool in_range = length >= 1 && length <= PKV_CONTEXT_LIMIT;
     const bool ok = in_range && block >= 0 && block < a.cache.num_blocks;
-    if (lane == 0) {
-        if (!ok) atomicOr(a.error_flag, PKV_DEVICE_BAD_BLOCK | (in_range ? 0 : PKV_DEVICE_BAD_POSITION));
-        *reinterpret_cast<int *>(fresh + kFreshOk) = ok;
+    const int64_t from = row * a.kv_stride + warp * kDim + 2 * lane;
+    const __half2 k = *reinterpret_cast<const __half2 *>(a.key + from), v = *reinterpret_cast<const __half2 *>(a.value + from);
+    const pkv::int4::KeyTurn turn(a.key_norm, a.rope, in_range ? length - 1 : 0, lane);
+    const float2 key = a.key_norm != nullptr ? pkv::int4::turn_key<true>(k, turn, a.eps) : pkv::int4::turn_key<false>(k, turn, a.eps);
+    const float2 value = __half22float2(v);
+    uint32_t key_word, key_scale, value_word, value_scale;
+    pkv::int4::encode_pair(key.x, key.y, lane, key_word, key_scale);
+    pkv::int4::encode_pair(value.x, value.y, lane, value_word, value_scale);
+    if (lane % 4 == 0) {
+        reinterpret_cast<uint32_t *>(fresh)[lane >> 2] = key_word;
+        reinterpret_cast<uint32_t *>(fresh)[8 + (lane >> 2)] = value_word;
     }
-    if (!ok) return;
-    const int64_t from = row * a.kv_stride + head * kDim;
-    float v[16];
-    uint32_t words[2], scale;
-    pkv::int4::key_group(a.key + from, t, is_key, a.key_norm, a.eps, a.rope, length - 1, v);
-    if (!is_key) pkv::int4::load16(a.value + from + 16 * t, v);
-    pkv::int4::encode_group(v, words, scale);
-    uint8_t *const mine = fresh + head * 72;
-    *reinterpret_cast<uint2 *>(mine + (is_key ? 0 : 32) + 8 * t) = make_uint2(words[0], words[1]);
-    mine[(is_key ? 64 : 68) + t] = static_cast<uint8_t>(scale);
-    uint8_t *const to = pkv::int4::block_at(a.cache, a.layer, block) + head * pkv::int4::kHeadBytes;
-    const int slot = (length - 1) % kSlots;
-    if (is_key) pkv::int4::store_key(to, t, slot, words, scale);
-    else pkv::int4::store_value(to, t, slot, words, scale);
+    if (lane % 8 == 0) {
+        fresh[64 + (lane >> 3)] = static_cast<uint8_t>(key_scale);
+        fresh[68 + (lane >> 3)] = static_cast<uint8_t>(value_scale);
+    }
+    if (lane == 0) *reinterpret_cast<int *>(fresh + kFreshOk) = ok;
+    if (ok) {
+        uint8_t *const to = pkv::int4::block_at(a.cache, a.layer, block) + warp * pkv::int4::kHeadBytes;
+        const int slot = (length - 1) % kSlots;
+        if (lane % 4 == 0) {
+            pkv::int4::store_key(to, lane >> 2, slot, key_word, key_scale);
+            pkv::int4::store_value(to, lane >> 2, slot, value_word, value_scale);
+        }
+    } else if (warp == 0 && lane == 0) {
+        atomicOr(a.error_flag, PKV_DEVICE_BAD_BLOCK | (in_range ? 0 : PKV_DEVICE_BAD_POSITION));
+    }
+    __syncwarp();
 }
 
 // The same token into the copy of its (block, head) at `head` in shared memory.
-__device__ __forceinline__ void put_fresh(const uint8_t *fresh, int warp, uint8_t *head, int slot, int lane) {
+__device__ __forceinline__ void put_fresh(const uint8_t *fresh, uint8_t *head, int slot, int lane) {
     if (*reinterpret_cast<const int *>(fresh + kFreshOk) == 0) return;
-    const uint8_t *mine = fresh + warp * 72;
-    if (lane < 4) {
-        *reinterpret_cast<uint2 *>(head + pkv::int4::key_words(lane, slot)) = *reinterpret_cast<const uint2 *>(mine + 8 * lane);
-    } else if (lane < 12) {
-        *reinterpret_cast<uint32_t *>(head + pkv::int4::value_word(lane - 4, slot)) =
-            *reinterpret_cast<const uint32_t *>(mine + 32 + 4 * (lane - 4));
-    } else if (lane < 20) {
-        const int first = lane < 16 ? pkv::int4::kKeyScaleAt : pkv::int4::kValueScaleAt;
-        head[pkv::int4::scale_at(first, lane & 3, slot)] = mine[64 + lane - 12];
+    if (lane < 8) {
+        *reinterpret_cast<uint32_t *>(head + pkv::int4::key_words(lane >> 1, slot) + 4 * (lane & 1)) =
+            reinterpret_cast<const uint32_t *>(fresh)[lane];
+    } else if (lane < 16) {
+        *reinterpret_cast<uint32_t *>(head + pkv::int4::value_word(lane - 8, slot)) = reinterpret_cast<const uint32_t *>(fresh)[lane];
+    } else if (lane < 24) {
+        const int first = lane < 20 ? pkv::int4::kKeyScaleAt : pkv::int4::kValueScaleAt;
+        head[pkv::int4::scale_at(first, lane & 3, slot)] = fresh[64 + lane - 16];
     }
     __syncwarp();
 }
 
 // The producer warp: copies the blocks of [begin, end) chunk by chunk, a chunk ending with its
-// row, and writes the new token of each row that ends here: while it would wait for a free
-// stage, or when the row's last chunk is on its way.
-template <bool NEW>
+// row.
 __device__ __forceinline__ void fill_ring(const Args &a, int begin, int end, int row, int lane, uint8_t *smem,
                                           uint64_t *full, uint64_t *empty) {
     const uint64_t policy = pkv::l2_policy_evict_first();
@@ -351,13 +352,6 @@ __device__ __forceinline__ void fill_ring(const Args &a, int begin, int end, int
     int row_end = __shfl_sync(0xffffffffu, rows.last, 0);
     int issued = 0;
     bool ok = true;
-    int prepared = -1, ended = 0;  // the row whose new token is in place, and rows that ended
-    const auto prepare = [&] {
-        const int length = __shfl_sync(0xffffffffu, rows.length, row - rows.base);
-        write_new(a, row, length, a.flat[row_end - 1], lane, smem + kFreshAt + ended % kFresh * kFreshBytes);
-        __syncwarp();
-        prepared = row;
-    };
     for (int at = begin; at < end;) {
         if (at >= row_end) {
             row = advance_row(a, rows, row + 1, at, lane);
@@ -378,25 +372,17 @@ __device__ __forceinline__ void fill_ring(const Args &a, int begin, int end, int
         const bool bad = block < 0 || block >= a.cache.num_blocks;  // reported, and read as zeros
         if (bad && lane < n) atomicOr(a.error_flag, PKV_DEVICE_BAD_BLOCK);
         const int stage = issued % kStages;
-        const bool fresh = NEW && row_end <= end;  // the row ends here
         if (issued >= kStages) {
-            const uint32_t bar = pkv::smem_addr(&empty[stage]), parity = (issued / kStages - 1) & 1;
-            if (fresh && prepared != row && !__all_sync(0xffffffffu, pkv::mbar_test_wait(bar, parity))) prepare();
-            ok = __all_sync(0xffffffffu, wait_bounded(bar, parity));
+            ok = __all_sync(0xffffffffu, wait_bounded(pkv::smem_addr(&empty[stage]), (issued / kStages - 1) & 1));
             if (!ok) break;  // a consumer gave up
         }
         const uint32_t bar = pkv::smem_addr(&full[stage]);
-        if (lane == 0) mbar_expect_tx(bar, n * pkv::int4::kBlockBytes);
+        if (lane == 0) pkv::mbar_arrive_expect_tx(bar, n * pkv::int4::kBlockBytes);
         __syncwarp();
         if (lane < n) {
             bulk_load(ring + stage * kStageBytes + lane * pkv::int4::kBlockBytes,
                       bad ? kZeroBlock : pkv::int4::block_at(a.cache, a.layer, block), pkv::int4::kBlockBytes, bar, policy);
         }
-        if (fresh && at + n == row_end) {
-            if (prepared != row) prepare();
-            ++ended;
-        }
-        if (lane == 0) pkv::mbar_arrive(bar);
         at += n;
         ++issued;
     }
@@ -622,13 +608,14 @@ __global__ void __launch_bounds__(kThreads, 3) int4_decode_kernel(const __grid_c
         return;
     }
     if (warp == kProducer) {
-        fill_ring<NEW>(a, begin, end, row, lane, smem, full, empty);
+        fill_ring(a, begin, end, row, lane, smem, full, empty);
         return;
     }
     Rows rows = load_rows(a, row, lane);
 
     const Places places(pkv::smem_addr(smem) + warp * pkv::int4::kHeadBytes, lane);
-    int consumed = 0, ended = 0;
+    uint8_t *const fresh = smem + kFreshAt + warp * kFreshBytes;
+    int consumed = 0;
     bool failed = false;
     int i = begin;
     while (i < end) {
@@ -640,6 +627,7 @@ __global__ void __launch_bounds__(kThreads, 3) int4_decode_kernel(const __grid_c
         const int row_last = __shfl_sync(0xffffffffu, rows.last, row - rows.base);
         const int length = __shfl_sync(0xffffffffu, rows.length, row - rows.base);
         const int seg_end = min(end, row_last);
+        if (NEW && row_last <= end) write_new(a, row, length, a.flat[row_last - 1], warp, lane, fresh);
         Query q;
         q.load<NEW>(a, row, length, warp, lane);
         int next = row;
@@ -656,8 +644,7 @@ __global__ void __launch_bounds__(kThreads, 3) int4_decode_kernel(const __grid_c
             failed = __any_sync(0xffffffffu, failed);
             if (failed) break;
             if (NEW && i + n == row_last) {
-                put_fresh(smem + kFreshAt + ended++ % kFresh * kFreshBytes, warp,
-                          smem + stage * kStageBytes + (n - 1) * pkv::int4::kBlockBytes + warp * pkv::int4::kHeadBytes,
+                put_fresh(fresh, smem + stage * kStageBytes + (n - 1) * pkv::int4::kBlockBytes + warp * pkv::int4::kHeadBytes,
                           (length - 1) & (kSlots - 1), lane);
             }
             const int tokens = min(max(length - (i - row_first) * kSlots, 0), n * kSlots);  // valid ones of the chunk

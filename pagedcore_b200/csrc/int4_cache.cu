@@ -1,9 +1,9 @@
 // Writes to and reads from the 4-bit KV cache (numbers and layout: int4.cuh).
 //
 // pkv_int4_append_kv puts new K (with a norm of each head and the rotation, where asked for)
-// and V rows into their slots.  A warp takes K or V of one head of eight tokens, a lane 16
-// dims, which are a group: its scale and codes need no other lane.  Tokens are independent
-// of one another.  CTAs behind those rotate the queries.
+// and V rows into their slots.  A warp takes K or V of one head of four tokens, a lane eight
+// dims, which are a word of codes; consecutive tokens of a block fill whole sectors.  Tokens
+// are independent of one another.  CTAs behind those rotate the queries.
 
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
@@ -24,7 +24,7 @@ constexpr int kHalf = kDim / 2;
 constexpr int kHeads = PKV_KV_HEADS;
 constexpr int kSlots = PKV_BLOCK_TOKENS;
 constexpr int kThreads = 2 * kHeads * 32;
-constexpr int kSpan = 8;       // tokens per CTA that writes K and V
+constexpr int kSpan = 4;       // tokens per CTA that writes K and V
 constexpr int kQuerySpan = 4;  // and per CTA that rotates queries
 
 struct AppendArgs {
@@ -112,6 +112,51 @@ __device__ void rotate_queries(const AppendArgs &a, int layer, int begin, int wa
     }
 }
 
+// Eight FP16 values as FP32.
+__device__ __forceinline__ void halves(const uint4 &raw, float (&v)[8]) {
+    const __half2 *h = reinterpret_cast<const __half2 *>(&raw);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const float2 f = __half22float2(h[i]);
+        v[2 * i] = f.x, v[2 * i + 1] = f.y;
+    }
+}
+
+// turn_key of int4.cuh by the eight lanes c of a row: dims 8 c .. + 7, `raw` in FP16, to v.
+__device__ __forceinline__ void turn_chunk(const AppendArgs &a, int layer, int position, int c, const uint4 &raw, float (&v)[8]) {
+    const __half *factors = a.rope + position * kHalf + 8 * (c & 3);
+    float cos[8], sin[8], far[8];
+    halves(*reinterpret_cast<const uint4 *>(factors), cos);
+    halves(*reinterpret_cast<const uint4 *>(factors + PKV_CONTEXT_LIMIT * kHalf), sin);
+    uint4 other;  // the dims that rotate with these, 32 away
+    other.x = __shfl_xor_sync(0xffffffffu, raw.x, 4), other.y = __shfl_xor_sync(0xffffffffu, raw.y, 4);
+    other.z = __shfl_xor_sync(0xffffffffu, raw.z, 4), other.w = __shfl_xor_sync(0xffffffffu, raw.w, 4);
+    halves(other, far);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) sin[i] = c < 4 ? -sin[i] : sin[i];
+    if (a.key_norm == nullptr) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) v[i] = v[i] * cos[i] + far[i] * sin[i];
+        return;
+    }
+    double part[2] = {0, 0};
+#pragma unroll
+    for (int i = 0; i < 8; ++i) part[i & 1] = fma(static_cast<double>(v[i]), static_cast<double>(v[i]), part[i & 1]);
+    double sum = part[0] + part[1];
+#pragma unroll
+    for (int offset = 1; offset < 8; offset <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, offset);
+    const double inverse = rsqrt(sum * (1.0 / kDim) + a.eps);
+    const __half *norm = a.key_norm + static_cast<int64_t>(a.layer_begin + layer) * kDim;
+    float own[8], its[8];
+    halves(*reinterpret_cast<const uint4 *>(norm + 8 * c), own);
+    halves(*reinterpret_cast<const uint4 *>(norm + 8 * (c ^ 4)), its);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+        const double x = v[i] * inverse * static_cast<double>(own[i]), y = far[i] * inverse * static_cast<double>(its[i]);
+        v[i] = static_cast<float>(x * static_cast<double>(cos[i]) + y * static_cast<double>(sin[i]));
+    }
+}
+
 __global__ void __launch_bounds__(kThreads) int4_append_kernel(const __grid_constant__ AppendArgs a) {
     pkv::pdl_wait();
     pkv::pdl_launch_dependents();
@@ -121,32 +166,25 @@ __global__ void __launch_bounds__(kThreads) int4_append_kernel(const __grid_cons
         rotate_queries(a, layer, (static_cast<int>(blockIdx.x) - a.tile_ctas) * kQuerySpan, warp, lane);
         return;
     }
-    const int token = static_cast<int>(blockIdx.x) * kSpan + (lane >> 2);
-    const int t = lane & 3, head = warp & 3;
-    int slot = token < a.tokens ? a.slots[token] : -1;
-    if (slot < 0 || slot >= static_cast<int64_t>(a.cache.num_blocks) * kSlots) {
-        if (token < a.tokens && t == 0 && warp == 0) atomicOr(a.error_flag, PKV_DEVICE_BAD_BLOCK);
-        slot = -1;
-    }
-    const bool here = slot >= 0;
-    const int64_t from = layer * a.layer_stride + token * a.token_stride + head * kDim;
-    float v[16];
-    uint32_t words[2], scale;
-    uint8_t *const to =
-        pkv::int4::block_at(a.cache, a.layer_begin + layer, here ? slot / kSlots : 0) + head * pkv::int4::kHeadBytes;
-    if (warp < kHeads) {
-        const int position = here && a.rope != nullptr ? checked_position(a, token) : 0;
-        const __half *weight =
-            a.key_norm != nullptr ? a.key_norm + static_cast<int64_t>(a.layer_begin + layer) * kDim : nullptr;
-        pkv::int4::key_group(a.key + from, t, here, weight, a.eps, a.rope, position, v);
-        if (!here) return;
-        pkv::int4::encode_group(v, words, scale);
-        pkv::int4::store_key(to, t, slot % kSlots, words, scale);
-    } else if (here) {
-        pkv::int4::load16(a.value + from + pkv::int4::kGroup * t, v);
-        pkv::int4::encode_group(v, words, scale);
-        pkv::int4::store_value(to, t, slot % kSlots, words, scale);
-    }
+    // Lane c of a row's eight: dims 8 c .. + 7 of one token's K or V head.
+    const int c = lane & 7, head = warp & 3;
+    const bool is_key = warp < kHeads;
+    const int token = static_cast<int>(blockIdx.x) * kSpan + (lane >> 3);
+    const bool listed = token < a.tokens;
+    const int64_t from = layer * a.layer_stride + min(token, a.tokens - 1) * a.token_stride + head * kDim + 8 * c;
+    const uint4 raw = *reinterpret_cast<const uint4 *>((is_key ? a.key : a.value) + from);
+    const int slot = listed ? a.slots[token] : -1;
+    const bool ok = slot >= 0 && slot < static_cast<int64_t>(a.cache.num_blocks) * kSlots;
+    if (listed && !ok && c == 0 && warp == 0) atomicOr(a.error_flag, PKV_DEVICE_BAD_BLOCK);
+    float v[8];
+    halves(raw, v);
+    if (is_key && a.rope != nullptr) turn_chunk(a, layer, ok ? checked_position(a, token) : 0, c, raw, v);
+    uint32_t word, scale;
+    pkv::int4::encode_chunk(v, word, scale);
+    if (!ok) return;
+    uint8_t *const to = pkv::int4::block_at(a.cache, a.layer_begin + layer, slot / kSlots) + head * pkv::int4::kHeadBytes;
+    if (is_key) pkv::int4::store_key(to, c, slot % kSlots, word, scale);
+    else pkv::int4::store_value(to, c, slot % kSlots, word, scale);
 }
 
 // K and V of `blocks` as FP16, each [i][slot][head][dim].  One CTA per block, a group a thread:
