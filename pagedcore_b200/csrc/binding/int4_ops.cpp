@@ -256,6 +256,22 @@ PyObject *check_cache(PyObject *const *args) {
     Py_RETURN_NONE;
 }
 
+// (storage, query_norm, key_norm, eps)
+PyObject *check_norms(PyObject *const *args) {
+    const Cache cache = cache_of(args[0]);
+    tensor_of(args[1], "head norms");
+    norms_of(args + 1, cache);
+    Py_RETURN_NONE;
+}
+
+// (rows, out): whether [rows, heads, 64] lie where [rows, 32, 64] are written, other than as the same rows.
+PyObject *overlaps(PyObject *const *args) {
+    const at::Tensor &rows = tensor_of(args[0], "rows"), &out = tensor_of(args[1], "out");
+    if (rows.dim() != 3 || out.dim() != 3) refuse("rows and out must have three dimensions");
+    if (rows.numel() == 0 || out.numel() == 0 || !within(rows, out)) Py_RETURN_FALSE;
+    Py_RETURN_TRUE;
+}
+
 // Whether the rows of [layers, tokens, 32, 64] do not overlap: one of the two dimensions within the other.
 bool rows_apart(const at::Tensor &rows) {
     const int64_t layers = rows.size(0), tokens = rows.size(1), over = rows.stride(0), within_ = rows.stride(1);
@@ -521,8 +537,9 @@ PyObject *entry(PyObject *, PyObject *const *args, Py_ssize_t count) {
     {#name, reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(entry<name, count>)), METH_FASTCALL, nullptr}
 
 PyMethodDef methods[] = {
-    OPERATOR(check_cache, 1),      OPERATOR(append_kv, 13),    OPERATOR(read_blocks, 4),
-    OPERATOR(decode_attention, 9), OPERATOR(decode_layer, 15), OPERATOR(prefill_attention, 7),
+    OPERATOR(check_cache, 1),      OPERATOR(check_norms, 4),   OPERATOR(overlaps, 2),
+    OPERATOR(append_kv, 13),       OPERATOR(read_blocks, 4),   OPERATOR(decode_attention, 9),
+    OPERATOR(decode_layer, 15),    OPERATOR(prefill_attention, 7),
     {nullptr, nullptr, 0, nullptr},
 };
 

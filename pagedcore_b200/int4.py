@@ -90,6 +90,15 @@ class HeadNorms:
     key: Tensor
     eps: float = 1e-5
 
+    def check(self, cache: Int4Cache) -> None:
+        """Raise ValueError unless these are norms for the layers of ``cache``."""
+        _int4_ops.check_norms(cache.storage, self.query, self.key, self.eps)
+
+
+def overlaps(rows: Tensor, out: Tensor) -> bool:
+    """Whether ``rows`` [rows, heads, 64] lie where ``out`` [rows, 32, 64] is written, other than as the same rows."""
+    return _int4_ops.overlaps(rows, out)
+
 
 def append_kv(
     cache: Int4Cache,

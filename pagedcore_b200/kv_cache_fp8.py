@@ -17,42 +17,25 @@ blocks are copied before it (8 KiB a row and layer) and put back.
 
 from __future__ import annotations
 
-from collections.abc import Iterator
-
 import torch
 from torch import Tensor
 
 from pagedcore_b200 import fp8
 from pagedcore_b200._lib import check, lib
 from pagedcore_b200.config import PagedCoreConfig
-from pagedcore_b200.engine_types import RequestId
-from pagedcore_b200.kv_cache import _BLOCK_TOKENS, _LAYERS, DecodeBatch, KVAllocator
+from pagedcore_b200.kv_cache import _BLOCK_TOKENS, _LAYERS, DecodeBatch
+from pagedcore_b200.kv_cache_quantised import QuantisedKVAllocator, allocate_quantised
 
 _BLOCK_BYTES = _LAYERS * 2 * 4 * (_BLOCK_TOKENS * 64 + 4)  # codes and one FP32 scale per head
 
 
 def allocate_fp8_kv_pool(config: PagedCoreConfig, *, device: str | torch.device = "cuda:0") -> fp8.Fp8Cache:
     """``allocate_kv_pool`` for an 8-bit cache: as many blocks as ``kv_pool_mib`` holds."""
-    target = torch.device(device)
-    if target.type != "cuda":
-        raise ValueError("KV pool requires a CUDA device")
-    if not torch.cuda.is_available():
-        raise RuntimeError("KV pool requires an available CUDA runtime")
-    pool_bytes = config.kv_pool_mib * 2**20
-    margin_bytes = config.workspace_margin_mib * 2**20
-    if torch.cuda.mem_get_info(target)[0] < pool_bytes + margin_bytes:
-        raise RuntimeError("configured KV pool and workspace margin do not fit in GPU memory")
-    cache = fp8.Fp8Cache.empty(_LAYERS, pool_bytes // _BLOCK_BYTES, target)
-    if torch.cuda.mem_get_info(target)[0] < margin_bytes:
-        del cache
-        raise RuntimeError("KV pool allocation leaves less than the configured workspace margin")
-    return cache
+    return allocate_quantised(config, device, _BLOCK_BYTES, lambda blocks, on: fp8.Fp8Cache.empty(_LAYERS, blocks, on))
 
 
-class Fp8KVAllocator(KVAllocator):
+class Fp8KVAllocator(QuantisedKVAllocator):
     """Assign blocks within an 8-bit cache of 22 layers."""
-
-    prompt_query_dtype = torch.float32  # rotated in FP32 and not rounded
 
     def __init__(self, pool: fp8.Fp8Cache, *, validation: str = "full") -> None:
         if not isinstance(pool, fp8.Fp8Cache) or pool.layers != _LAYERS:
@@ -72,29 +55,10 @@ class Fp8KVAllocator(KVAllocator):
     def _attend_prompt(self, layer: int, query: Tensor, blocks: Tensor, start: int, out: Tensor) -> Tensor:
         return fp8.prefill_attention(self._pool, layer, query, blocks, start, self._error, out)
 
-    def attend(self, batch: DecodeBatch, query: Tensor, *, layer_index: int, out: Tensor | None = None) -> Tensor:
-        """Decode attention of FP16 query [B, 32, 64] over a :class:`DecodeBatch` (FP32 is rounded first)."""
-        self._check_worker()
-        if query.dtype == torch.float32:
-            query = query.half()
-        to = self._aligned_out(out)
-        result = fp8.decode_attention(
-            self._pool, layer_index, query, batch.lengths, batch.prefix, batch.flat, batch.total_blocks, self._error,
-            to,
+    def _attend_rows(self, layer: int, batch: DecodeBatch, query: Tensor, out: Tensor | None) -> Tensor:
+        return fp8.decode_attention(
+            self._pool, layer, query, batch.lengths, batch.prefix, batch.flat, batch.total_blocks, self._error, out
         )
-        return result if to is out else out.copy_(result)
-
-    @staticmethod
-    def _aligned_out(out: Tensor | None) -> Tensor | None:
-        """``out`` [rows, 32, 64], or rows to copy to it where its own are not what the kernels write."""
-        if out is None:
-            return None
-        if out.ndim != 3 or out.dtype != torch.float16 or out.stride()[1:] != (64, 1):
-            raise ValueError("out must be FP16 [batch, 32, 64] with contiguous rows")
-        fp8._row_stride("out", out, 32 * 64)
-        if fp8._rows_ok(out, out.stride()):
-            return out
-        return torch.empty_like(out, memory_format=torch.contiguous_format)
 
     def _decode_layer_args(self, batch: DecodeBatch, rows: int, grid: int) -> tuple:
         grid = fp8.decode_plan(self._pool.device.index, rows, batch.total_blocks)[0]
@@ -140,34 +104,6 @@ class Fp8KVAllocator(KVAllocator):
         fp8.restore_blocks(self._pool, *saved)
 
     # -- reading back ----------------------------------------------------------------
-    @torch.inference_mode()
-    def iter_layer_blocks(self, request_id: RequestId, *, layer_index: int) -> Iterator[tuple[Tensor, Tensor]]:
-        """FP16 copies of the valid [slots, 4, 64] pages, including a completed staged layer."""
-        self._check_worker()
-        if type(layer_index) is not int or not 0 <= layer_index < _LAYERS:
-            raise ValueError("layer_index must identify one of the 22 decoder layers")
-        blocks, length = self._call(self._ledger.view, request_id, self._handle(request_id), layer_index)
-        if length == 0:
-            raise ValueError("attention requires a nonempty cache")
-        for logical, physical in enumerate(blocks):
-            self._check_worker()
-            valid = min(_BLOCK_TOKENS, length - logical * _BLOCK_TOKENS)
-            key, value = self._read(layer_index, physical)
-            yield key[:valid], value[:valid]
-
-    @torch.inference_mode()
-    def read_block(self, request_id: RequestId, logical_block: int) -> tuple[Tensor, Tensor]:
-        """FP16 copies of K/V [22, valid slots, 4, 64] of one logical block."""
-        self._check_worker()
-        handle = self._handle(request_id)
-        blocks = self._call(self._ledger.table, request_id, handle)
-        length = self._ledger.length(handle)
-        if type(logical_block) is not int or not 0 <= logical_block < len(blocks):
-            raise ValueError("logical block must identify a cached block")
-        valid = min(_BLOCK_TOKENS, length - logical_block * _BLOCK_TOKENS)
-        layers = [self._read(layer, blocks[logical_block]) for layer in range(_LAYERS)]
-        return tuple(torch.stack([layer[kv][:valid] for layer in layers]) for kv in (0, 1))
-
     def _read(self, layer: int, physical: int) -> tuple[Tensor, Tensor]:
         block = torch.full((1,), physical, dtype=torch.int32, device=self._pool.device)
         key, value = fp8.read_blocks(self._pool, layer, block, self._error)
