@@ -716,19 +716,26 @@ __global__ void __launch_bounds__(kThreads, 3) int4_decode_kernel(const __grid_c
     if (failed && lane == 0) atomicOr(a.error_flag, PKV_DEVICE_WAIT_TIMEOUT);
 }
 
-// Merge of the rows that several pieces hold, sixteen lanes a head and four dims a lane.
-// With few rows a CTA's eight warps deal out the pieces of one (row, two heads) and the first
-// warp merges the warps' results in order; with many rows a warp merges a row's few pieces.
-constexpr int kMergeWarps = 8;
-constexpr int kMergeThreads = kMergeWarps * 32;
+// Merge of the rows that several pieces hold: H half warps a (row, head), whose sixteen lanes
+// hold its 64 dims, each with every H-th piece, four or eight read at a time; then the halves of a warp
+// are joined, and the warps' results in order.
+template <int H>
+constexpr int kMergeThreads = 16 * (H < 16 ? 16 : H);
 
-template <bool SPREAD>
-__global__ void __launch_bounds__(kMergeThreads) int4_merge_kernel(const __grid_constant__ Args a) {
-    __shared__ float part[kMergeWarps][32][6];
+__device__ __forceinline__ void join_halves(Merge &m) {
+    const float4 v = make_float4(__shfl_down_sync(0xffffffffu, m.A[0], 16), __shfl_down_sync(0xffffffffu, m.A[1], 16),
+                                 __shfl_down_sync(0xffffffffu, m.A[2], 16), __shfl_down_sync(0xffffffffu, m.A[3], 16));
+    const float top = __shfl_down_sync(0xffffffffu, m.M, 16), sum = __shfl_down_sync(0xffffffffu, m.L, 16);
+    m.add(top, sum, v);  // of use in the lower half
+}
+
+template <int H>
+__global__ void __launch_bounds__(kMergeThreads<H>) int4_merge_kernel(const __grid_constant__ Args a) {
+    __shared__ float part[H > 2 ? kMergeThreads<H> / 32 : 1][16][6];
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const int pair = SPREAD ? blockIdx.x : blockIdx.x * kMergeWarps + warp;
-    const int row = pair / (kQueryHeads / 2);
-    const int head = 2 * (pair % (kQueryHeads / 2)) + (lane >> 4);
+    const int half = threadIdx.x >> 4;
+    const int at = blockIdx.x * (kMergeThreads<H> / 16 / H) + half / H;
+    const int row = at / kQueryHeads, head = at % kQueryHeads;
     const int dim = 4 * (lane & 15);
     pkv::pdl_launch_dependents();
     // The tables are older than the split kernel: it lets this one start only after
@@ -751,11 +758,10 @@ __global__ void __launch_bounds__(kMergeThreads) int4_merge_kernel(const __grid_
         }
     }
     pkv::pdl_wait();
-    if (first == last) return;
-    constexpr int kStep = SPREAD ? kMergeWarps : 1;
+    if (H <= 2 && __all_sync(0xffffffffu, first >= last)) return;
     Merge merged{kLowest, 0.f, {0.f, 0.f, 0.f, 0.f}};
-    constexpr int kBatch = 4;
-    for (int c0 = first + (SPREAD ? warp : 0); c0 <= last; c0 += kBatch * kStep) {
+    constexpr int kBatch = H > 8 ? 8 : 4, kStep = H;
+    for (int c0 = first + half % H; c0 <= last && first < last; c0 += kBatch * kStep) {
         float2 ml[kBatch];
         float4 v[kBatch];
 #pragma unroll
@@ -772,22 +778,40 @@ __global__ void __launch_bounds__(kMergeThreads) int4_merge_kernel(const __grid_
             if (c0 + j * kStep <= last) merged.add(ml[j].x, ml[j].y, v[j]);
         }
     }
-    if constexpr (SPREAD) {
-        float *mine = part[warp][lane];
-        mine[0] = merged.M, mine[1] = merged.L;
-        mine[2] = merged.A[0], mine[3] = merged.A[1], mine[4] = merged.A[2], mine[5] = merged.A[3];
+    if constexpr (H > 1) {
+        __syncwarp();
+        join_halves(merged);
+    }
+    if constexpr (H > 2) {
+        constexpr int kWarpsAHead = H / 2;
+        if (lane < 16) {
+            float *mine = part[warp][lane];
+            mine[0] = merged.M, mine[1] = merged.L;
+            mine[2] = merged.A[0], mine[3] = merged.A[1], mine[4] = merged.A[2], mine[5] = merged.A[3];
+        }
         __syncthreads();
-        if (warp != 0) return;
-        for (int w = 1; w < kMergeWarps; ++w) {
-            const float *p = part[w][lane];
+        if (warp % kWarpsAHead != 0 || first >= last) return;
+        merged = Merge{kLowest, 0.f, {0.f, 0.f, 0.f, 0.f}};
+        for (int other = lane >> 4; other < kWarpsAHead; other += 2) {
+            const float *p = part[warp + other][lane & 15];
             merged.add(p[0], p[1], make_float4(p[2], p[3], p[4], p[5]));
         }
+        __syncwarp();
+        join_halves(merged);
     }
+    if (first >= last || (H > 1 && lane >= 16)) return;
 #pragma unroll
     for (int d = 0; d < 4; ++d) merged.A[d] = merged.L == 0.f ? 0.f : __fdiv_rn(merged.A[d], merged.L);
-    __half2 *dst = reinterpret_cast<__half2 *>(a.out + row * a.out_stride + head * kDim + dim);
-    dst[0] = __floats2half2_rn(merged.A[0], merged.A[1]);
-    dst[1] = __floats2half2_rn(merged.A[2], merged.A[3]);
+    const __half2 low = __floats2half2_rn(merged.A[0], merged.A[1]), high = __floats2half2_rn(merged.A[2], merged.A[3]);
+    *reinterpret_cast<uint2 *>(a.out + row * a.out_stride + head * kDim + dim) = make_uint2(pack(low), pack(high));
+}
+
+template <int H>
+cudaError_t launch_merge(const Args &a, cudaStream_t stream) {
+    constexpr int kHeadsPerCta = kMergeThreads<H> / 16 / H;
+    const int64_t heads = static_cast<int64_t>(a.batch) * kQueryHeads;
+    return pkv::launch_pdl(int4_merge_kernel<H>, dim3(static_cast<unsigned>((heads + kHeadsPerCta - 1) / kHeadsPerCta)),
+                           dim3(kMergeThreads<H>), stream, a);
 }
 
 int64_t workspace_of(int64_t batch, int64_t grid) { return grid > 1 ? (batch + grid) * kPartial * 4 : 0; }
@@ -825,7 +849,7 @@ int device_info(int device, DeviceInfo *info) {
     if (e == cudaSuccess) e = prepare_kernel(int4_decode_kernel<false>, &plain);
     if (e == cudaSuccess) e = prepare_kernel(int4_decode_kernel<true>, &fresh);
     // The merge keeps the split kernel's partition of L1 and shared memory.
-    for (const auto merge : {int4_merge_kernel<false>, int4_merge_kernel<true>}) {
+    for (const auto merge : {int4_merge_kernel<1>, int4_merge_kernel<2>, int4_merge_kernel<4>, int4_merge_kernel<8>, int4_merge_kernel<32>}) {
         if (e == cudaSuccess) {
             e = cudaFuncSetAttribute(merge, cudaFuncAttributePreferredSharedMemoryCarveout, cudaSharedmemCarveoutMaxShared);
         }
@@ -874,13 +898,17 @@ int decode(Args a, void *workspace, int64_t workspace_bytes, cudaStream_t stream
     e = pkv::launch_pdl_smem(a.key != nullptr ? int4_decode_kernel<true> : int4_decode_kernel<false>, dim3(a.grid),
                              dim3(kThreads), kSmem, stream, a);
     if (e == cudaSuccess && a.grid > 1) {
-        // A CTA per (row, two heads) while that is at most two waves of CTAs: beyond it rows
-        // have few pieces each and a warp merges them as fast.
-        const int64_t pairs = static_cast<int64_t>(a.batch) * (kQueryHeads / 2);
-        const bool spread = pairs <= 16 * info.sms;
-        const auto blocks = static_cast<unsigned>(spread ? pairs : (pairs + kMergeWarps - 1) / kMergeWarps);
-        e = pkv::launch_pdl(spread ? int4_merge_kernel<true> : int4_merge_kernel<false>, dim3(blocks), dim3(kMergeThreads),
-                            stream, a);
+        // Half warps a head by the pieces that a row has when the GPU is full, so that one round of
+        // loads or two are enough; by nothing else, for results must not depend on the room of a
+        // captured launch.  (Whole calls: 100 rows, 5 pieces each, 18.0 us with 2 and 19.9 with 4;
+        // 64 rows, 7 each, 26.1 and 25.8; 7 rows, 64 each, 6.7 with 8 and 7.8 with 16; 2 rows, 222
+        // each, 26.1 with 16 and 25.1 with 32.)
+        const int pieces = info.sms * info.ctas_per_sm / a.batch + 1;
+        e = pieces <= 4 ? launch_merge<1>(a, stream)
+            : pieces <= 6 ? launch_merge<2>(a, stream)
+            : pieces <= 16 ? launch_merge<4>(a, stream)
+            : pieces <= 96 ? launch_merge<8>(a, stream)
+                           : launch_merge<32>(a, stream);
     }
     if (e != cudaSuccess) return pkv::fail(PKV_CUDA_ERROR, std::string("int4 decode launch failed: ") + cudaGetErrorString(e));
     return PKV_OK;
