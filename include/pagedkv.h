@@ -540,8 +540,10 @@ int pkv_int4_append_kv(void *storage, int32_t layers, int32_t num_blocks, int32_
 int pkv_int4_read_blocks(const void *storage, int32_t layers, int32_t num_blocks, int32_t layer, const int32_t *blocks,
                          int32_t count, void *key_out, void *value_out, int32_t *error_flag, void *stream);
 
-/* pkv_fp8_prefill_attention over the 4-bit cache: same arguments, workspace and result over the
- * values that the cache holds. */
+/* pkv_fp8_prefill_attention over the 4-bit cache: same arguments and result over the values that
+ * the cache holds; the workspace (16-byte aligned, uninitialised) has pkv_int4_prefill_plan's bytes
+ * for the chunk on the current device. */
+int pkv_int4_prefill_plan(int32_t device, int32_t start, int32_t tokens, int64_t *out_workspace_bytes);
 int pkv_int4_prefill_attention(const void *storage, int32_t layers, int32_t num_blocks, int32_t layer,
                                const void *query, int32_t query_fp32, int64_t query_stride, const int32_t *blocks,
                                int32_t start, int32_t tokens, void *out, int64_t out_stride, void *workspace,

@@ -257,6 +257,7 @@ SIGNATURES: dict[str, tuple[object, list[object]]] = {
         c_int,
         [*_INT4_CACHE, c_int32, c_void_p, c_int32, c_void_p, c_void_p, c_void_p, c_void_p],
     ),
+    "pkv_int4_prefill_plan": (c_int, [c_int32, c_int32, c_int32, i64p]),
     "pkv_int4_prefill_attention": (
         c_int,
         [

@@ -31,7 +31,6 @@ constexpr int64_t kQueryHeads = PKV_QUERY_HEADS, kKvHeads = PKV_KV_HEADS, kDim =
 constexpr int64_t kRow = kQueryHeads * kDim;  // values of a query row
 constexpr int64_t kBlockTokens = PKV_BLOCK_TOKENS;
 constexpr int64_t kMost = INT32_MAX - (1 << 16);  // rows and list entries: the C ABI's int32, and a step of a row loop
-constexpr int64_t kPrefillBlockBytes = 2 * kBlockTokens * kKvHeads * kDim * 2 + 4;  // an FP16 block and its table entry
 
 struct Refusal {
     std::string message;
@@ -489,13 +488,15 @@ PyObject *prefill_attention(PyObject *const *args) {
     at::Tensor out = output(given, tokens, cache.index, "tokens");
     take_query(query);
     if (given != nullptr && within(query.get(), out)) query.make_dense();
-    const at::Tensor workspace = bytes(count * kPrefillBlockBytes, cache.index);
+    int64_t workspace_bytes = 0;
+    check_status(pkv_int4_prefill_plan(cache.index, static_cast<int32_t>(start), static_cast<int32_t>(tokens), &workspace_bytes));
+    const at::Tensor workspace = bytes(workspace_bytes, cache.index);
     const at::Tensor &q = query.get();
     launch(cache.index, [&](void *stream) {
         return pkv_int4_prefill_attention(cache.storage, cache.layers, cache.blocks, layer, q.data_ptr(),
                                           q.scalar_type() == at::kFloat, row_stride(q), list, static_cast<int32_t>(start),
                                           static_cast<int32_t>(tokens), out.data_ptr(), row_stride(out),
-                                          workspace.data_ptr(), count * kPrefillBlockBytes, flag, stream);
+                                          workspace.data_ptr(), workspace_bytes, flag, stream);
     });
     return given != nullptr ? Py_NewRef(args[6]) : THPVariable_Wrap(std::move(out));
 }

@@ -63,6 +63,13 @@ inline Cache cache_of(const void *storage, int32_t layers, int32_t num_blocks) {
     return {static_cast<uint8_t *>(const_cast<void *>(storage)), layers, num_blocks};
 }
 
+// The attention of a prompt chunk as rows of the decode attention (arguments checked by the
+// caller), and its workspace.
+int rows_workspace(int device, int start, int tokens, int64_t *bytes);
+int attend_rows(const Cache &cache, int32_t layer, const void *query, bool query_fp32, int64_t query_stride,
+                const int32_t *blocks, int32_t start, int32_t tokens, void *out, int64_t out_stride, void *workspace,
+                int64_t workspace_bytes, int32_t *error_flag, cudaStream_t stream);
+
 // The checks of a cache that every entry point makes.
 int check_cache(const void *storage, int32_t layers, int32_t num_blocks, int32_t layer_begin, int32_t layer_count);
 

@@ -70,10 +70,15 @@ constexpr float kFarScore = 0x1p20f;
 constexpr float kLowest = -1e30f;  // below every finite score
 constexpr int kPartial = kQueryHeads * (kDim + 2);  // floats of a partial
 
+// What the rows' queries are: rotated FP16 numbers; rotated FP32 numbers; or, with a new token a row
+// (a decode layer), to be normed and rotated here.
+enum Rotation { kHalf, kWide, kFresh };
+
 struct Args {
     pkv::int4::Cache cache;
     int32_t layer;
-    const __half *query;
+    const __half *query;    // kHalf, kFresh
+    const float *query32;   // kWide
     int64_t query_stride;
     const __half *key;  // the new tokens, with rope; null for the attention alone
     const __half *value;
@@ -211,19 +216,35 @@ struct Query {
     uint32_t high[8], low[8];
     float factor0, factor1;  // of the scores of heads 2 t and 2 t + 1
 
-    template <bool NEW>
+    template <Rotation R>
     __device__ __forceinline__ void load(const Args &a, int row, int length, int warp, int lane) {
         const int g = lane >> 2, t = lane & 3;
-        const __half *src = a.query + row * a.query_stride + (warp * kHeadGroup + g) * kDim;
-        if constexpr (!NEW) {
-            const uint4 *from = reinterpret_cast<const uint4 *>(src + 16 * t);
+        const int64_t at = row * a.query_stride + (warp * kHeadGroup + g) * kDim;
+        if constexpr (R == kHalf) {
+            const uint4 *from = reinterpret_cast<const uint4 *>(a.query + at + 16 * t);
             const uint4 x = from[0], y = from[1];
             high[0] = x.x, high[1] = x.y, high[2] = x.z, high[3] = x.w;
             high[4] = y.x, high[5] = y.y, high[6] = y.z, high[7] = y.w;
             factor0 = factor1 = kScaleLog2 / kValueFactor;
             return;
         }
-        float q[16], other[16], cos[16], sin[16];
+        float q[16];
+        if constexpr (R == kWide) {
+            const float4 *from = reinterpret_cast<const float4 *>(a.query32 + at + 16 * t);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const float4 v = from[i];
+                q[4 * i] = v.x, q[4 * i + 1] = v.y, q[4 * i + 2] = v.z, q[4 * i + 3] = v.w;
+            }
+        } else {
+            turn(a, a.query + at, length, t, q);
+        }
+        halve(q, t);
+    }
+
+    // Norm (where there is one) and rotation of a head's dims, 16 t .. + 15 in each of its four lanes.
+    static __device__ __forceinline__ void turn(const Args &a, const __half *src, int length, int t, float (&q)[16]) {
+        float other[16], cos[16], sin[16];
         pkv::int4::load16(src + 16 * t, q);
         pkv::int4::load16(src + 16 * (t ^ 2), other);
         if (a.query_norm != nullptr) {
@@ -242,10 +263,15 @@ struct Query {
         const __half *factors = a.rope + position * (kDim / 2) + 16 * (t & 1);
         pkv::int4::load16(factors, cos);
         pkv::int4::load16(factors + PKV_CONTEXT_LIMIT * (kDim / 2), sin);
+#pragma unroll
+        for (int i = 0; i < 16; ++i) q[i] = q[i] * cos[i] + (t < 2 ? -other[i] : other[i]) * sin[i];
+    }
+
+    // The head's values, scaled, as two FP16 numbers each.
+    __device__ __forceinline__ void halve(const float (&q)[16], int t) {
         float largest = 0.f;
 #pragma unroll
         for (int i = 0; i < 16; ++i) {
-            q[i] = q[i] * cos[i] + (t < 2 ? -other[i] : other[i]) * sin[i];
             if (fabsf(q[i]) < INFINITY) largest = fmaxf(largest, fabsf(q[i]));
         }
         largest = fmaxf(largest, __shfl_xor_sync(0xffffffffu, largest, 1));
@@ -267,9 +293,11 @@ struct Query {
 };
 
 // A head's queries of a row into L1.
+template <Rotation R>
 __device__ __forceinline__ void prefetch_query(const Args &a, int row, int warp, int lane) {
-    const __half *at = a.query + row * a.query_stride + warp * kHeadGroup * kDim + lane * 16;
-    asm volatile("prefetch.global.L1 [%0];" ::"l"(at));
+    const int64_t at = row * a.query_stride + warp * kHeadGroup * kDim + lane * 16;
+    if constexpr (R == kWide) asm volatile("prefetch.global.L1 [%0];" ::"l"(a.query32 + at));
+    else asm volatile("prefetch.global.L1 [%0];" ::"l"(a.query + at));
 }
 
 // Copies of memory that one CTA reads once.
@@ -466,7 +494,7 @@ struct Tile {
     }
 };
 
-template <bool NEW>
+template <Rotation R>
 __device__ __forceinline__ void score(const Tile &tile, const Query &q, float (&s)[4]) {
     s[0] = s[1] = s[2] = s[3] = 0.f;
     const Steps k0((tile.ks & 0xffu) * 0x00800080u), k1((tile.ks >> 8) * 0x00800080u);  // each scale twice
@@ -478,7 +506,7 @@ __device__ __forceinline__ void score(const Tile &tile, const Query &q, float (&
         const uint32_t a0 = value_pair(x, xs, i, k0), a1 = value_pair(y, ys, i, k1);
         const uint32_t a2 = value_pair(x, xs, i + 1, k0), a3 = value_pair(y, ys, i + 1, k1);
         mma(s, a0, a1, a2, a3, q.high[2 * ks], q.high[2 * ks + 1]);
-        if (NEW) mma(s, a0, a1, a2, a3, q.low[2 * ks], q.low[2 * ks + 1]);
+        if (R != kHalf) mma(s, a0, a1, a2, a3, q.low[2 * ks], q.low[2 * ks + 1]);
     }
 }
 
@@ -507,13 +535,13 @@ __device__ __forceinline__ void add_values(const Tile &tile, const float (&w)[4]
 }
 
 // COUNT blocks, of which `valid` tokens count (MASKED; else all).
-template <bool NEW, int COUNT, bool MASKED>
+template <Rotation R, int COUNT, bool MASKED>
 __device__ __forceinline__ void attend(Tile (&tile)[COUNT], int valid, const Query &q, Sums &sums, int lane) {
     const int g = lane >> 2, t = lane & 3;
     float s[COUNT][4], x[COUNT][4];
 #pragma unroll
     for (int b = 0; b < COUNT; ++b) {
-        score<NEW>(tile[b], q, s[b]);
+        score<R>(tile[b], q, s[b]);
         if constexpr (MASKED) {
             const int here = valid - b * kSlots;
             if (2 * g >= here) s[b][0] = s[b][1] = -INFINITY;
@@ -550,7 +578,7 @@ __device__ __forceinline__ void attend(Tile (&tile)[COUNT], int valid, const Que
     }
 }
 
-template <bool NEW>
+template <Rotation R>
 __global__ void __launch_bounds__(kThreads, 3) int4_decode_kernel(const __grid_constant__ Args a) {
     extern __shared__ __align__(16) uint8_t smem[];
     __shared__ __align__(8) uint64_t full[kStages], empty[kStages];
@@ -627,13 +655,13 @@ __global__ void __launch_bounds__(kThreads, 3) int4_decode_kernel(const __grid_c
         const int row_last = __shfl_sync(0xffffffffu, rows.last, row - rows.base);
         const int length = __shfl_sync(0xffffffffu, rows.length, row - rows.base);
         const int seg_end = min(end, row_last);
-        if (NEW && row_last <= end) write_new(a, row, length, a.flat[row_last - 1], warp, lane, fresh);
+        if (R == kFresh && row_last <= end) write_new(a, row, length, a.flat[row_last - 1], warp, lane, fresh);
         Query q;
-        q.load<NEW>(a, row, length, warp, lane);
+        q.load<R>(a, row, length, warp, lane);
         int next = row;
         if (row_last < end) {  // the next row's queries are brought near while this one streams
             next = advance_row(a, rows, row + 1, row_last, lane);
-            if (next < a.batch) prefetch_query(a, next, warp, lane);
+            if (next < a.batch) prefetch_query<R>(a, next, warp, lane);
         }
         Sums sums;
         sums.clear();
@@ -643,7 +671,7 @@ __global__ void __launch_bounds__(kThreads, 3) int4_decode_kernel(const __grid_c
             failed = !wait_bounded(pkv::smem_addr(&full[stage]), (consumed / kStages) & 1);
             failed = __any_sync(0xffffffffu, failed);
             if (failed) break;
-            if (NEW && i + n == row_last) {
+            if (R == kFresh && i + n == row_last) {
                 put_fresh(fresh, smem + stage * kStageBytes + (n - 1) * pkv::int4::kBlockBytes + warp * pkv::int4::kHeadBytes,
                           (length - 1) & (kSlots - 1), lane);
             }
@@ -660,18 +688,18 @@ __global__ void __launch_bounds__(kThreads, 3) int4_decode_kernel(const __grid_c
                 Tile tile[2];
                 tile[0].load<0>(here);
                 tile[1].load<1>(here);
-                attend<NEW, 2, false>(tile, 0, q, sums, lane);
+                attend<R, 2, false>(tile, 0, q, sums, lane);
                 tile[0].load<2>(here);
                 tile[1].load<3>(here);
                 release();
-                attend<NEW, 2, false>(tile, 0, q, sums, lane);
+                attend<R, 2, false>(tile, 0, q, sums, lane);
             } else {
 #pragma unroll 1
                 for (int b = 0; b < n; ++b) {
                     Tile tile[1];
                     tile[0].load<0>(here.at(b * pkv::int4::kBlockBytes));
                     if (b + 1 == n) release();
-                    attend<NEW, 1, true>(tile, tokens - b * kSlots, q, sums, lane);
+                    attend<R, 1, true>(tile, tokens - b * kSlots, q, sums, lane);
                 }
             }
             i += n;
@@ -841,13 +869,16 @@ int device_info(int device, DeviceInfo *info) {
         info->ctas_per_sm = ctas[device].load(std::memory_order_relaxed);
         return PKV_OK;
     }
-    int previous = 0, plain = 0, fresh = 0;
+    int previous = 0, least = 1 << 20;
     cudaError_t e = cudaGetDevice(&previous);
     if (e == cudaSuccess) e = cudaSetDevice(device);
     if (e != cudaSuccess) return pkv::fail(PKV_CUDA_ERROR, std::string("int4 decode: ") + cudaGetErrorString(e));
     e = cudaDeviceGetAttribute(&info->sms, cudaDevAttrMultiProcessorCount, device);
-    if (e == cudaSuccess) e = prepare_kernel(int4_decode_kernel<false>, &plain);
-    if (e == cudaSuccess) e = prepare_kernel(int4_decode_kernel<true>, &fresh);
+    for (const auto kernel : {int4_decode_kernel<kHalf>, int4_decode_kernel<kWide>, int4_decode_kernel<kFresh>}) {
+        int ctas = 0;
+        if (e == cudaSuccess) e = prepare_kernel(kernel, &ctas);
+        if (ctas < least) least = ctas;
+    }
     // The merge keeps the split kernel's partition of L1 and shared memory.
     for (const auto merge : {int4_merge_kernel<1>, int4_merge_kernel<2>, int4_merge_kernel<4>, int4_merge_kernel<8>, int4_merge_kernel<32>}) {
         if (e == cudaSuccess) {
@@ -856,7 +887,6 @@ int device_info(int device, DeviceInfo *info) {
     }
     cudaSetDevice(previous);
     if (e != cudaSuccess) return pkv::fail(PKV_CUDA_ERROR, std::string("int4 decode: ") + cudaGetErrorString(e));
-    const int least = plain < fresh ? plain : fresh;
     info->ctas_per_sm = least < 1 ? 1 : least;
     if (known) {
         sms[device].store(info->sms, std::memory_order_relaxed);
@@ -871,14 +901,15 @@ bool aligned16(const void *p) { return (reinterpret_cast<uintptr_t>(p) & 15u) ==
 int decode(Args a, void *workspace, int64_t workspace_bytes, cudaStream_t stream) {
     const int rc = pkv::int4::check_cache(a.cache.storage, a.cache.layers, a.cache.num_blocks, a.layer, 1);
     if (rc) return rc;
-    if (a.query == nullptr || a.lengths == nullptr || a.prefix == nullptr || (a.flat == nullptr && a.capacity > 0) ||
+    const void *const query = a.query32 != nullptr ? static_cast<const void *>(a.query32) : a.query;
+    if (query == nullptr || a.lengths == nullptr || a.prefix == nullptr || (a.flat == nullptr && a.capacity > 0) ||
         a.out == nullptr || a.error_flag == nullptr) {
         return pkv::fail(PKV_VALUE_ERROR, "int4 decode: null pointer argument");
     }
     if (a.batch < 1 || a.capacity < 0 || a.grid < 1) {
         return pkv::fail(PKV_VALUE_ERROR, "int4 decode: batch, block count or grid out of range");
     }
-    if (!aligned16(a.query) || !aligned16(a.out) || a.query_stride % 8 || a.out_stride % 8 ||
+    if (!aligned16(query) || !aligned16(a.out) || a.query_stride % 8 || a.out_stride % 8 ||
         a.query_stride < kQueryHeads * kDim || a.out_stride < kQueryHeads * kDim) {
         return pkv::fail(PKV_VALUE_ERROR, "int4 decode: rows must be 16-byte aligned, 2048 or more values apart in multiples of 8");
     }
@@ -895,7 +926,10 @@ int decode(Args a, void *workspace, int64_t workspace_bytes, cudaStream_t stream
         a.part_o = static_cast<float *>(workspace);
         a.part_ml = a.part_o + (static_cast<int64_t>(a.batch) + a.grid) * kQueryHeads * kDim;
     }
-    e = pkv::launch_pdl_smem(a.key != nullptr ? int4_decode_kernel<true> : int4_decode_kernel<false>, dim3(a.grid),
+    const auto kernel = a.key != nullptr       ? int4_decode_kernel<kFresh>
+                        : a.query32 != nullptr ? int4_decode_kernel<kWide>
+                                               : int4_decode_kernel<kHalf>;
+    e = pkv::launch_pdl_smem(kernel, dim3(a.grid),
                              dim3(kThreads), kSmem, stream, a);
     if (e == cudaSuccess && a.grid > 1) {
         // Half warps a head by the pieces that a row has when the GPU is full, so that one round of
@@ -936,6 +970,71 @@ Args args_of(const void *storage, int32_t layers, int32_t num_blocks, int32_t la
 }
 
 }  // namespace
+
+// -- a prompt chunk as rows ---------------------------------------------------------
+// Token t of a chunk is a row of start + t + 1 tokens over the first blocks of the request's
+// table.  Blocks of the rows before row r:
+namespace {
+
+__host__ __device__ __forceinline__ int blocks_before(int start, int r) {
+    const auto upto = [](int n) { return n + kSlots * (n / kSlots) * (n / kSlots - 1) / 2 + n / kSlots * (n % kSlots); };
+    return upto(start + r) - upto(start);
+}
+
+__global__ void int4_rows_kernel(const int32_t *blocks, int start, int tokens, int32_t *lengths, int32_t *prefix, int32_t *flat) {
+    pkv::pdl_launch_dependents();
+    pkv::pdl_wait();
+    const int row = blockIdx.x;
+    const int first = blocks_before(start, row), count = (start + row) / kSlots + 1;
+    for (int j = threadIdx.x; j < count; j += blockDim.x) flat[first + j] = blocks[j];
+    if (threadIdx.x == 0) {
+        lengths[row] = start + row + 1;
+        prefix[row] = first;
+        if (row == tokens - 1) prefix[tokens] = first + count;
+    }
+}
+
+int64_t tables_bytes(int start, int tokens) {
+    return (4 * (2 * static_cast<int64_t>(tokens) + 1 + blocks_before(start, tokens)) + 15) / 16 * 16;
+}
+
+}  // namespace
+
+namespace pkv::int4 {
+
+int rows_workspace(int device, int start, int tokens, int64_t *bytes) {
+    int32_t grid = 0;
+    int64_t partials = 0;
+    const int rc = pkv_int4_decode_plan(device, tokens, blocks_before(start, tokens), &grid, &partials);
+    *bytes = tables_bytes(start, tokens) + partials;
+    return rc;
+}
+
+int attend_rows(const Cache &cache, int32_t layer, const void *query, bool query_fp32, int64_t query_stride,
+                const int32_t *blocks, int32_t start, int32_t tokens, void *out, int64_t out_stride, void *workspace,
+                int64_t workspace_bytes, int32_t *error_flag, cudaStream_t stream) {
+    int device = 0;
+    cudaError_t e = cudaGetDevice(&device);
+    if (e != cudaSuccess) return fail(PKV_CUDA_ERROR, std::string("cudaGetDevice: ") + cudaGetErrorString(e));
+    const int total = blocks_before(start, tokens);
+    int32_t grid = 0;
+    int64_t partials = 0;
+    if (const int rc = pkv_int4_decode_plan(device, tokens, total, &grid, &partials)) return rc;
+    const int64_t tables = tables_bytes(start, tokens);
+    if (workspace_bytes < tables + partials) {
+        return fail(PKV_VALUE_ERROR, "prefill attention: the workspace is too small (see pkv_int4_prefill_plan)");
+    }
+    int32_t *const lengths = static_cast<int32_t *>(workspace), *const prefix = lengths + tokens;
+    int32_t *const flat = prefix + tokens + 1;
+    e = launch_pdl(int4_rows_kernel, dim3(tokens), dim3(128), stream, blocks, start, tokens, lengths, prefix, flat);
+    if (e != cudaSuccess) return fail(PKV_CUDA_ERROR, std::string("prefill attention launch failed: ") + cudaGetErrorString(e));
+    Args a = args_of(cache.storage, cache.layers, cache.num_blocks, layer, query_fp32 ? nullptr : query, query_stride, lengths,
+                     prefix, flat, tokens, total, grid, out, out_stride, error_flag);
+    if (query_fp32) a.query32 = static_cast<const float *>(query);
+    return decode(a, static_cast<uint8_t *>(workspace) + tables, partials, stream);
+}
+
+}  // namespace pkv::int4
 
 extern "C" int pkv_int4_decode_plan(int32_t device, int32_t batch, int32_t total_blocks, int32_t *out_grid,
                                     int64_t *out_workspace_bytes) {

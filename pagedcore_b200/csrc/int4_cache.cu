@@ -340,9 +340,48 @@ extern "C" int pkv_int4_read_blocks(const void *storage, int32_t layers, int32_t
     return read_blocks(storage, layers, num_blocks, layer, blocks, count, key_out, value_out, nullptr, error_flag, stream);
 }
 
-// The request's blocks become an FP16 pool of one layer in the workspace (the values are
-// FP16 numbers: nothing is rounded), which the tensor-core prompt kernel attends to: that
-// kernel reads every block once for each 16 queries.
+// Two ways to attend to a prompt chunk.
+//
+// By tiles: the request's blocks become an FP16 pool of one layer in the workspace (the values
+// are FP16 numbers: nothing is rounded), which the tensor-core prompt kernel attends to; that
+// kernel reads every block once for each 16 queries, but a tile's keys one after another.
+//
+// By rows: each token a row of the decode attention, which cuts the keys over the whole GPU but
+// reads a row's blocks for each token.  For a few tokens behind a long context.
+namespace {
+
+// Rows take about 8 us and 1.15 ns for each block of each row, tiles 8 us and 0.87 us for each 64
+// keys that the last tile walks (600 blocks a step is where they meet: 3 tokens behind 1900 take
+// 9.0 and 35.0 us, 75 behind 601 12.3 and 17.5, 150 behind 1500 25.7 and 31.7, 300 behind 256 18.0
+// and 15.8).  Rows of less than a chunk's blocks share pieces and take longer (16 tokens at the
+// beginning 18.9 and 9.2).
+bool by_rows(int start, int tokens) {
+    const int64_t blocks = static_cast<int64_t>(tokens) * (start + tokens / 2) / kSlots;
+    return tokens == 1 || (start >= 64 && blocks < 600ll * ((start + tokens) / 64));
+}
+
+int64_t tiles_workspace(int start, int tokens) {
+    return (start + tokens + kSlots - 1) / kSlots * (2 * kBlockValues * 2 + 4);
+}
+
+int check_chunk(int32_t start, int32_t tokens) {
+    if (tokens < 1 || start < 0 || static_cast<int64_t>(start) + tokens > PKV_CONTEXT_LIMIT) {
+        return pkv::fail(PKV_VALUE_ERROR, "prefill attention: the chunk must hold 1 or more tokens at positions below 2048");
+    }
+    return PKV_OK;
+}
+
+}  // namespace
+
+extern "C" int pkv_int4_prefill_plan(int32_t device, int32_t start, int32_t tokens, int64_t *out_workspace_bytes) {
+    pkv::clear_error();
+    if (out_workspace_bytes == nullptr) return pkv::fail(PKV_VALUE_ERROR, "prefill plan: null pointer argument");
+    if (const int rc = check_chunk(start, tokens)) return rc;
+    if (by_rows(start, tokens)) return pkv::int4::rows_workspace(device, start, tokens, out_workspace_bytes);
+    *out_workspace_bytes = tiles_workspace(start, tokens);
+    return PKV_OK;
+}
+
 extern "C" int pkv_int4_prefill_attention(const void *storage, int32_t layers, int32_t num_blocks, int32_t layer,
                                           const void *query, int32_t query_fp32, int64_t query_stride,
                                           const int32_t *blocks, int32_t start, int32_t tokens, void *out,
@@ -352,19 +391,27 @@ extern "C" int pkv_int4_prefill_attention(const void *storage, int32_t layers, i
     if (query == nullptr || blocks == nullptr || out == nullptr || error_flag == nullptr) {
         return pkv::fail(PKV_VALUE_ERROR, "prefill attention: null pointer argument");
     }
-    if (tokens < 1 || start < 0 || static_cast<int64_t>(start) + tokens > PKV_CONTEXT_LIMIT) {
-        return pkv::fail(PKV_VALUE_ERROR, "prefill attention: the chunk must hold 1 or more tokens at positions below 2048");
-    }
+    if (const int rc = check_chunk(start, tokens)) return rc;
     constexpr int64_t kRow = PKV_QUERY_HEADS * PKV_HEAD_DIM;
     if (!aligned16(query) || !aligned16(out) || query_stride % 8 || out_stride % 8 || query_stride < kRow ||
         out_stride < kRow) {
         return pkv::fail(PKV_VALUE_ERROR, "prefill attention: rows must be 16-byte aligned, 2048 or more values apart in multiples of 8");
     }
+    if (workspace == nullptr || !aligned16(workspace)) {
+        return pkv::fail(PKV_VALUE_ERROR, "prefill attention: the workspace is required and must be 16-byte aligned");
+    }
+    if (by_rows(start, tokens)) {
+        const int rc = pkv::int4::check_cache(storage, layers, num_blocks, layer, 1);
+        if (rc) return rc;
+        return pkv::int4::attend_rows(pkv::int4::cache_of(storage, layers, num_blocks), layer, query, query_fp32 != 0,
+                                      query_stride, blocks, start, tokens, out, out_stride, workspace, workspace_bytes,
+                                      error_flag, static_cast<cudaStream_t>(stream));
+    }
+    if (workspace_bytes < tiles_workspace(start, tokens)) {
+        return pkv::fail(PKV_VALUE_ERROR, "prefill attention: the workspace is too small (see pkv_int4_prefill_plan)");
+    }
     const int count = (start + tokens + kSlots - 1) / kSlots;
     const int64_t pool_bytes = static_cast<int64_t>(count) * 2 * kBlockValues * 2;
-    if (workspace == nullptr || !aligned16(workspace) || workspace_bytes < pool_bytes + 4 * count) {
-        return pkv::fail(PKV_VALUE_ERROR, "prefill attention: the workspace needs 16388 bytes per block of 16 tokens");
-    }
     int32_t *const table = reinterpret_cast<int32_t *>(static_cast<uint8_t *>(workspace) + pool_bytes);
     const int rc = read_blocks(storage, layers, num_blocks, layer, blocks, count, workspace,
                                static_cast<__half *>(workspace) + count * kBlockValues, table, error_flag, stream);

@@ -77,15 +77,20 @@ def test_attention() -> None:
     refused(function, *layer(norms=(P, None)), message=b"norms")
     refused(function, *layer(norms=(P, P + 2)), message=b"norms")
 
-    def prompt(start=0, tokens=16, stride=2048, size=16388, workspace=P):
+    def prompt(start=0, tokens=1000, stride=2048, size=63 * 16388, workspace=P):
         return (*CACHE, 0, P, 0, stride, P, start, tokens, P, 2048, workspace, size, P, None)
 
     function = lib.pkv_int4_prefill_attention
     refused(function, *prompt(tokens=0), message=b"positions below 2048")
-    refused(function, *prompt(start=2040), message=b"positions below 2048")
+    refused(function, *prompt(start=1049), message=b"positions below 2048")
     refused(function, *prompt(stride=2040), message=b"2048 or more")
-    refused(function, *prompt(size=16387), message=b"workspace")
+    refused(function, *prompt(size=63 * 16388 - 1), message=b"workspace")
     refused(function, *prompt(workspace=None), message=b"workspace")
+    refused(function, *prompt(workspace=P + 8), message=b"workspace")
+    size = ctypes.c_int64()
+    refused(lib.pkv_int4_prefill_plan, 0, 2040, 9, ctypes.byref(size), message=b"positions below 2048")
+    refused(lib.pkv_int4_prefill_plan, 0, 0, 16, None, message=b"null pointer")
+    assert lib.pkv_int4_prefill_plan(0, 0, 1000, ctypes.byref(size)) == _lib.PKV_OK and size.value == 63 * 16388
     refused(lib.pkv_int4_decode_plan, 0, 0, 4, ctypes.byref(ctypes.c_int32()), ctypes.byref(ctypes.c_int64()),
             message=b"nonempty batch")
 

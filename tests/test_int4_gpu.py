@@ -372,7 +372,7 @@ def test_decode_layer_reports_a_row_without_a_token() -> None:
 
 
 # -- a prompt chunk ----------------------------------------------------------------------
-@pytest.mark.parametrize("start, tokens", [(0, 1), (0, 15), (0, 130), (7, 40), (100, 64), (601, 75), (2000, 48), (0, 2047)])
+@pytest.mark.parametrize("start, tokens", [(0, 1), (0, 15), (0, 130), (7, 40), (64, 3), (100, 64), (601, 75), (300, 500), (2000, 48), (2047, 1), (0, 2047)])
 @pytest.mark.parametrize("dtype", [torch.float16, torch.float32])
 def test_prefill_attention(start, tokens, dtype) -> None:
     case = Case(31, [start + tokens])
