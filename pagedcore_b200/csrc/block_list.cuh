@@ -1,7 +1,7 @@
 // A decode batch as the split attention kernels over quantised caches walk it: the rows'
 // block tables form one flat list, and a CTA works on a contiguous piece of it.
 //
-// Args holds prefix, lengths, batch, capacity and error_flag.
+// Args holds batch, capacity and error_flag, and gives prefix_at(row) and length_at(row).
 #pragma once
 
 #include <cuda_runtime.h>
@@ -15,7 +15,7 @@ namespace pkv {
 // The batch's block count, from the device so that a captured launch serves changing batches.
 template <typename Args>
 __device__ __forceinline__ int total_blocks(const Args &a) {
-    const int total = a.prefix[a.batch];
+    const int total = a.prefix_at(a.batch);
     if (total >= 0 && total <= a.capacity) return total;
     atomicOr(a.error_flag, PKV_DEVICE_BAD_BLOCK);
     return 0;
@@ -37,7 +37,7 @@ template <typename Args>
 __device__ __forceinline__ Rows load_rows(const Args &a, int base, int lane) {
     const int r = base + lane;
     if (r >= a.batch) return Rows{base, INT32_MAX, INT32_MAX, 0};
-    return Rows{base, a.prefix[r], a.prefix[r + 1], a.lengths[r]};
+    return Rows{base, a.prefix_at(r), a.prefix_at(r + 1), a.length_at(r)};
 }
 
 // The first row at or after `row` that has blocks past `block`, with its window.

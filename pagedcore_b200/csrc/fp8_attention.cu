@@ -103,6 +103,9 @@ struct Args {
     float *part_o;   // [batch + grid][32][64]
     float *part_ml;  // [batch + grid][32][2]
     int32_t *error_flag;
+
+    __device__ __forceinline__ int prefix_at(int row) const { return prefix[row]; }
+    __device__ __forceinline__ int length_at(int row) const { return lengths[row]; }
 };
 
 // Piece g covers blocks [g * total / grid, (g + 1) * total / grid).

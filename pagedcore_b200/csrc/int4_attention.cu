@@ -70,15 +70,23 @@ constexpr float kFarScore = 0x1p20f;
 constexpr float kLowest = -1e30f;  // below every finite score
 constexpr int kPartial = kQueryHeads * (kDim + 2);  // floats of a partial
 
-// What the rows' queries are: rotated FP16 numbers; rotated FP32 numbers; or, with a new token a row
-// (a decode layer), to be normed and rotated here.
-enum Rotation { kHalf, kWide, kFresh };
+// What the rows are: sequences with rotated FP16 queries; sequences with a new token each (a
+// decode layer), whose queries are normed and rotated here; or the tokens of a prompt chunk, with
+// rotated FP16 or FP32 queries: token t is a row of start + t + 1 tokens over the first blocks of
+// the request's table.
+enum class Kind { kPlain, kFresh, kChunk };
+
+// Blocks of a chunk's rows before row r.
+__host__ __device__ __forceinline__ int blocks_before(int start, int r) {
+    const auto upto = [](int n) { return n + kSlots * (n / kSlots) * (n / kSlots - 1) / 2 + n / kSlots * (n % kSlots); };
+    return upto(start + r) - upto(start);
+}
 
 struct Args {
     pkv::int4::Cache cache;
     int32_t layer;
-    const __half *query;    // kHalf, kFresh
-    const float *query32;   // kWide
+    const __half *query;
+    const float *query32;  // of a chunk, in place of query where it is not null
     int64_t query_stride;
     const __half *key;  // the new tokens, with rope; null for the attention alone
     const __half *value;
@@ -87,9 +95,10 @@ struct Args {
     const __half *query_norm;  // of this layer, or null
     const __half *key_norm;
     double eps;
-    const int32_t *lengths;
-    const int32_t *prefix;
-    const int32_t *flat;
+    const int32_t *lengths;  // null for a chunk
+    const int32_t *prefix;   // null for a chunk
+    const int32_t *flat;     // of a chunk the request's table
+    int32_t start;           // of a chunk
     int32_t batch;
     int32_t capacity;  // of flat; the batch's blocks are prefix[batch]
     int32_t grid;
@@ -99,6 +108,17 @@ struct Args {
     float *part_o;   // [batch + grid][32][64]
     float *part_ml;  // [batch + grid][32][2]
     int32_t *error_flag;
+};
+
+// The arguments with the tables that the kind of rows has.
+template <Kind R>
+struct ArgsOf : Args {
+    explicit ArgsOf(const Args &args) : Args(args) {}
+
+    __device__ __forceinline__ int prefix_at(int row) const {
+        return R == Kind::kChunk ? blocks_before(start, row) : prefix[row];
+    }
+    __device__ __forceinline__ int length_at(int row) const { return R == Kind::kChunk ? start + row + 1 : lengths[row]; }
 };
 
 // Pieces of a list of `total` blocks: at most one per CTA and per chunk.  (A captured
@@ -117,7 +137,8 @@ struct Cut {
     int total, pieces;
     int64_t weight;
 
-    __device__ __forceinline__ Cut(const Args &a, int rows_with_blocks) {
+    template <Kind R>
+    __device__ __forceinline__ Cut(const ArgsOf<R> &a, int rows_with_blocks) {
         total = total_blocks(a);
         pieces = pieces_of(total, a.grid);
         weight = static_cast<int64_t>(total) + kRowCost * rows_with_blocks;
@@ -136,12 +157,13 @@ struct RowScan {
     int first[kParts], last[kParts];
     unsigned held[kParts];  // rows with blocks
 
-    __device__ __forceinline__ RowScan(const Args &a, int lane) {
+    template <Kind R>
+    __device__ __forceinline__ RowScan(const ArgsOf<R> &a, int lane) {
 #pragma unroll
         for (int k = 0; k < kParts; ++k) {
             const int r = 32 * k + lane;
             first[k] = last[k] = 0;
-            if (r < a.batch) first[k] = a.prefix[r], last[k] = a.prefix[r + 1];
+            if (r < a.batch) first[k] = a.prefix_at(r), last[k] = a.prefix_at(r + 1);
         }
 #pragma unroll
         for (int k = 0; k < kParts; ++k) held[k] = __ballot_sync(0xffffffffu, last[k] > first[k]);
@@ -216,11 +238,11 @@ struct Query {
     uint32_t high[8], low[8];
     float factor0, factor1;  // of the scores of heads 2 t and 2 t + 1
 
-    template <Rotation R>
+    template <Kind R>
     __device__ __forceinline__ void load(const Args &a, int row, int length, int warp, int lane) {
         const int g = lane >> 2, t = lane & 3;
         const int64_t at = row * a.query_stride + (warp * kHeadGroup + g) * kDim;
-        if constexpr (R == kHalf) {
+        if constexpr (R == Kind::kPlain) {
             const uint4 *from = reinterpret_cast<const uint4 *>(a.query + at + 16 * t);
             const uint4 x = from[0], y = from[1];
             high[0] = x.x, high[1] = x.y, high[2] = x.z, high[3] = x.w;
@@ -229,7 +251,9 @@ struct Query {
             return;
         }
         float q[16];
-        if constexpr (R == kWide) {
+        if constexpr (R == Kind::kFresh) {
+            turn(a, a.query + at, length, t, q);
+        } else if (a.query32 != nullptr) {
             const float4 *from = reinterpret_cast<const float4 *>(a.query32 + at + 16 * t);
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
@@ -237,7 +261,7 @@ struct Query {
                 q[4 * i] = v.x, q[4 * i + 1] = v.y, q[4 * i + 2] = v.z, q[4 * i + 3] = v.w;
             }
         } else {
-            turn(a, a.query + at, length, t, q);
+            pkv::int4::load16(a.query + at + 16 * t, q);
         }
         halve(q, t);
     }
@@ -293,10 +317,10 @@ struct Query {
 };
 
 // A head's queries of a row into L1.
-template <Rotation R>
+template <Kind R>
 __device__ __forceinline__ void prefetch_query(const Args &a, int row, int warp, int lane) {
     const int64_t at = row * a.query_stride + warp * kHeadGroup * kDim + lane * 16;
-    if constexpr (R == kWide) asm volatile("prefetch.global.L1 [%0];" ::"l"(a.query32 + at));
+    if (R == Kind::kChunk && a.query32 != nullptr) asm volatile("prefetch.global.L1 [%0];" ::"l"(a.query32 + at));
     else asm volatile("prefetch.global.L1 [%0];" ::"l"(a.query + at));
 }
 
@@ -368,14 +392,18 @@ __device__ __forceinline__ void put_fresh(const uint8_t *fresh, uint8_t *head, i
 
 // The producer warp: copies the blocks of [begin, end) chunk by chunk, a chunk ending with its
 // row.
-__device__ __forceinline__ void fill_ring(const Args &a, int begin, int end, int row, int lane, uint8_t *smem,
+template <Kind R>
+__device__ __forceinline__ void fill_ring(const ArgsOf<R> &a, int begin, int end, int row, int lane, uint8_t *smem,
                                           uint64_t *full, uint64_t *empty) {
     const uint64_t policy = pkv::l2_policy_evict_first();
     const uint32_t ring = pkv::smem_addr(smem);
     // The ids of the list's next 64 blocks, 32 at a time, a window ahead.
-    int ids_base = begin;
-    int ids = begin + lane < end ? a.flat[begin + lane] : 0;
-    int ids_next = begin + 32 + lane < end ? a.flat[begin + 32 + lane] : 0;
+    // (Of a chunk, whose rows share one short table, each id when it is needed.)
+    int ids_base = begin, ids = 0, ids_next = 0;
+    if constexpr (R != Kind::kChunk) {
+        if (begin + lane < end) ids = a.flat[begin + lane];
+        if (begin + 32 + lane < end) ids_next = a.flat[begin + 32 + lane];
+    }
     Rows rows = load_rows(a, row, lane);
     int row_end = __shfl_sync(0xffffffffu, rows.last, 0);
     int issued = 0;
@@ -387,16 +415,22 @@ __device__ __forceinline__ void fill_ring(const Args &a, int begin, int end, int
             row_end = __shfl_sync(0xffffffffu, rows.last, row - rows.base);
         }
         const int n = min(kChunk, min(row_end, end) - at);
-        if (at - ids_base >= 32) {
-            ids = ids_next;
-            ids_base += 32;
-            const int ahead = ids_base + 32 + lane;
-            ids_next = ahead < end ? a.flat[ahead] : 0;
+        int block;  // of lane's copy
+        if constexpr (R == Kind::kChunk) {
+            const int row_first = __shfl_sync(0xffffffffu, rows.first, row - rows.base);
+            block = a.flat[at - row_first + min(lane, n - 1)];
+        } else {
+            if (at - ids_base >= 32) {
+                ids = ids_next;
+                ids_base += 32;
+                const int ahead = ids_base + 32 + lane;
+                ids_next = ahead < end ? a.flat[ahead] : 0;
+            }
+            const int offset = at - ids_base + min(lane, n - 1);
+            const int near = __shfl_sync(0xffffffffu, ids, offset & 31);
+            const int far = __shfl_sync(0xffffffffu, ids_next, offset & 31);
+            block = offset < 32 ? near : far;
         }
-        const int offset = at - ids_base + min(lane, n - 1);
-        const int near = __shfl_sync(0xffffffffu, ids, offset & 31);
-        const int far = __shfl_sync(0xffffffffu, ids_next, offset & 31);
-        const int block = offset < 32 ? near : far;  // of lane's copy
         const bool bad = block < 0 || block >= a.cache.num_blocks;  // reported, and read as zeros
         if (bad && lane < n) atomicOr(a.error_flag, PKV_DEVICE_BAD_BLOCK);
         const int stage = issued % kStages;
@@ -494,7 +528,7 @@ struct Tile {
     }
 };
 
-template <Rotation R>
+template <Kind R>
 __device__ __forceinline__ void score(const Tile &tile, const Query &q, float (&s)[4]) {
     s[0] = s[1] = s[2] = s[3] = 0.f;
     const Steps k0((tile.ks & 0xffu) * 0x00800080u), k1((tile.ks >> 8) * 0x00800080u);  // each scale twice
@@ -506,7 +540,7 @@ __device__ __forceinline__ void score(const Tile &tile, const Query &q, float (&
         const uint32_t a0 = value_pair(x, xs, i, k0), a1 = value_pair(y, ys, i, k1);
         const uint32_t a2 = value_pair(x, xs, i + 1, k0), a3 = value_pair(y, ys, i + 1, k1);
         mma(s, a0, a1, a2, a3, q.high[2 * ks], q.high[2 * ks + 1]);
-        if (R != kHalf) mma(s, a0, a1, a2, a3, q.low[2 * ks], q.low[2 * ks + 1]);
+        if (R != Kind::kPlain) mma(s, a0, a1, a2, a3, q.low[2 * ks], q.low[2 * ks + 1]);
     }
 }
 
@@ -535,7 +569,7 @@ __device__ __forceinline__ void add_values(const Tile &tile, const float (&w)[4]
 }
 
 // COUNT blocks, of which `valid` tokens count (MASKED; else all).
-template <Rotation R, int COUNT, bool MASKED>
+template <Kind R, int COUNT, bool MASKED>
 __device__ __forceinline__ void attend(Tile (&tile)[COUNT], int valid, const Query &q, Sums &sums, int lane) {
     const int g = lane >> 2, t = lane & 3;
     float s[COUNT][4], x[COUNT][4];
@@ -578,8 +612,8 @@ __device__ __forceinline__ void attend(Tile (&tile)[COUNT], int valid, const Que
     }
 }
 
-template <Rotation R>
-__global__ void __launch_bounds__(kThreads, 3) int4_decode_kernel(const __grid_constant__ Args a) {
+template <Kind R>
+__global__ void __launch_bounds__(kThreads, 3) int4_decode_kernel(const __grid_constant__ ArgsOf<R> a) {
     extern __shared__ __align__(16) uint8_t smem[];
     __shared__ __align__(8) uint64_t full[kStages], empty[kStages];
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -609,7 +643,7 @@ __global__ void __launch_bounds__(kThreads, 3) int4_decode_kernel(const __grid_c
         // Of 32 samples of prefix, `step` rows apart, the first past `begin`, cut finer until the
         // samples are rows.
         int step = (a.batch + 31) / 32;
-        int sample = lane * step < a.batch ? a.prefix[min((lane + 1) * step, a.batch)] : INT32_MAX;
+        int sample = lane * step < a.batch ? a.prefix_at(min((lane + 1) * step, a.batch)) : INT32_MAX;
         const Cut cut(a, 0);
         pieces = cut.total > 0 ? cut.pieces : 0;
         begin = static_cast<int>(cut.begins(blockIdx.x)), end = static_cast<int>(cut.begins(blockIdx.x + 1));
@@ -619,12 +653,12 @@ __global__ void __launch_bounds__(kThreads, 3) int4_decode_kernel(const __grid_c
             row += (past != 0 ? __ffs(past) - 1 : 31) * step;
             if (step == 1) break;
             step = (step + 31) / 32;
-            sample = row + lane * step < a.batch ? a.prefix[min(row + (lane + 1) * step, a.batch)] : INT32_MAX;
+            sample = row + lane * step < a.batch ? a.prefix_at(min(row + (lane + 1) * step, a.batch)) : INT32_MAX;
         }
     }
     // Rows without blocks: zeros.  (The merge looks at the rows' order too, where there is one.)
     for (int b = blockIdx.x * kThreads + threadIdx.x; (a.clear || a.grid == 1) && b < a.batch; b += a.grid * kThreads) {
-        const int first = a.prefix[b], last = a.prefix[b + 1];
+        const int first = a.prefix_at(b), last = a.prefix_at(b + 1);
         if (out_of_order(b, first, last)) atomicOr(a.error_flag, PKV_DEVICE_BAD_BLOCK);
         if (a.clear && last <= first) {
             for (int i = 0; i < kQueryHeads * kDim; ++i) a.out[b * a.out_stride + i] = __float2half_rn(0.f);
@@ -636,7 +670,7 @@ __global__ void __launch_bounds__(kThreads, 3) int4_decode_kernel(const __grid_c
         return;
     }
     if (warp == kProducer) {
-        fill_ring(a, begin, end, row, lane, smem, full, empty);
+        fill_ring<R>(a, begin, end, row, lane, smem, full, empty);
         return;
     }
     Rows rows = load_rows(a, row, lane);
@@ -655,7 +689,7 @@ __global__ void __launch_bounds__(kThreads, 3) int4_decode_kernel(const __grid_c
         const int row_last = __shfl_sync(0xffffffffu, rows.last, row - rows.base);
         const int length = __shfl_sync(0xffffffffu, rows.length, row - rows.base);
         const int seg_end = min(end, row_last);
-        if (R == kFresh && row_last <= end) write_new(a, row, length, a.flat[row_last - 1], warp, lane, fresh);
+        if (R == Kind::kFresh && row_last <= end) write_new(a, row, length, a.flat[row_last - 1], warp, lane, fresh);
         Query q;
         q.load<R>(a, row, length, warp, lane);
         int next = row;
@@ -671,7 +705,7 @@ __global__ void __launch_bounds__(kThreads, 3) int4_decode_kernel(const __grid_c
             failed = !wait_bounded(pkv::smem_addr(&full[stage]), (consumed / kStages) & 1);
             failed = __any_sync(0xffffffffu, failed);
             if (failed) break;
-            if (R == kFresh && i + n == row_last) {
+            if (R == Kind::kFresh && i + n == row_last) {
                 put_fresh(fresh, smem + stage * kStageBytes + (n - 1) * pkv::int4::kBlockBytes + warp * pkv::int4::kHeadBytes,
                           (length - 1) & (kSlots - 1), lane);
             }
@@ -757,8 +791,8 @@ __device__ __forceinline__ void join_halves(Merge &m) {
     m.add(top, sum, v);  // of use in the lower half
 }
 
-template <int H>
-__global__ void __launch_bounds__(kMergeThreads<H>) int4_merge_kernel(const __grid_constant__ Args a) {
+template <int H, Kind R>
+__global__ void __launch_bounds__(kMergeThreads<H>) int4_merge_kernel(const __grid_constant__ ArgsOf<R> a) {
     __shared__ float part[H > 2 ? kMergeThreads<H> / 32 : 1][16][6];
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int half = threadIdx.x >> 4;
@@ -770,7 +804,7 @@ __global__ void __launch_bounds__(kMergeThreads<H>) int4_merge_kernel(const __gr
     // its own wait for what came before.
     int first = 0, last = 0;
     const int row_at = min(row, a.batch - 1);
-    const int first_block = a.prefix[row_at], last_block = a.prefix[row_at + 1] - 1;
+    const int first_block = a.prefix_at(row_at), last_block = a.prefix_at(row_at + 1) - 1;
     int rank = 0, rows_with_blocks = 0;
     if (a.batch <= kWeighedRows) {
         const RowScan scan(a, lane);
@@ -834,11 +868,11 @@ __global__ void __launch_bounds__(kMergeThreads<H>) int4_merge_kernel(const __gr
     *reinterpret_cast<uint2 *>(a.out + row * a.out_stride + head * kDim + dim) = make_uint2(pack(low), pack(high));
 }
 
-template <int H>
-cudaError_t launch_merge(const Args &a, cudaStream_t stream) {
+template <int H, Kind R>
+cudaError_t launch_merge(const ArgsOf<R> &a, cudaStream_t stream) {
     constexpr int kHeadsPerCta = kMergeThreads<H> / 16 / H;
     const int64_t heads = static_cast<int64_t>(a.batch) * kQueryHeads;
-    return pkv::launch_pdl(int4_merge_kernel<H>, dim3(static_cast<unsigned>((heads + kHeadsPerCta - 1) / kHeadsPerCta)),
+    return pkv::launch_pdl(int4_merge_kernel<H, R>, dim3(static_cast<unsigned>((heads + kHeadsPerCta - 1) / kHeadsPerCta)),
                            dim3(kMergeThreads<H>), stream, a);
 }
 
@@ -849,12 +883,29 @@ struct DeviceInfo {
     int ctas_per_sm = 0;
 };
 
-cudaError_t prepare_kernel(void (*kernel)(Args), int *ctas_per_sm) {
+template <Kind R>
+cudaError_t prepare_kernel(int *ctas_per_sm) {
+    const auto kernel = int4_decode_kernel<R>;
     cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem);
     if (e == cudaSuccess) {
         e = cudaFuncSetAttribute(kernel, cudaFuncAttributePreferredSharedMemoryCarveout, cudaSharedmemCarveoutMaxShared);
     }
-    if (e == cudaSuccess) e = cudaOccupancyMaxActiveBlocksPerMultiprocessor(ctas_per_sm, kernel, kThreads, kSmem);
+    int ctas = 0;
+    if (e == cudaSuccess) e = cudaOccupancyMaxActiveBlocksPerMultiprocessor(&ctas, kernel, kThreads, kSmem);
+    if (ctas < *ctas_per_sm) *ctas_per_sm = ctas;
+    return e;
+}
+
+// The merge keeps the split kernel's partition of L1 and shared memory.
+template <Kind R>
+cudaError_t prepare_merges() {
+    cudaError_t e = cudaSuccess;
+    for (const auto merge : {int4_merge_kernel<1, R>, int4_merge_kernel<2, R>, int4_merge_kernel<4, R>, int4_merge_kernel<8, R>,
+                             int4_merge_kernel<32, R>}) {
+        if (e == cudaSuccess) {
+            e = cudaFuncSetAttribute(merge, cudaFuncAttributePreferredSharedMemoryCarveout, cudaSharedmemCarveoutMaxShared);
+        }
+    }
     return e;
 }
 
@@ -874,17 +925,11 @@ int device_info(int device, DeviceInfo *info) {
     if (e == cudaSuccess) e = cudaSetDevice(device);
     if (e != cudaSuccess) return pkv::fail(PKV_CUDA_ERROR, std::string("int4 decode: ") + cudaGetErrorString(e));
     e = cudaDeviceGetAttribute(&info->sms, cudaDevAttrMultiProcessorCount, device);
-    for (const auto kernel : {int4_decode_kernel<kHalf>, int4_decode_kernel<kWide>, int4_decode_kernel<kFresh>}) {
-        int ctas = 0;
-        if (e == cudaSuccess) e = prepare_kernel(kernel, &ctas);
-        if (ctas < least) least = ctas;
-    }
-    // The merge keeps the split kernel's partition of L1 and shared memory.
-    for (const auto merge : {int4_merge_kernel<1>, int4_merge_kernel<2>, int4_merge_kernel<4>, int4_merge_kernel<8>, int4_merge_kernel<32>}) {
-        if (e == cudaSuccess) {
-            e = cudaFuncSetAttribute(merge, cudaFuncAttributePreferredSharedMemoryCarveout, cudaSharedmemCarveoutMaxShared);
-        }
-    }
+    if (e == cudaSuccess) e = prepare_kernel<Kind::kPlain>(&least);
+    if (e == cudaSuccess) e = prepare_kernel<Kind::kFresh>(&least);
+    if (e == cudaSuccess) e = prepare_kernel<Kind::kChunk>(&least);
+    if (e == cudaSuccess) e = prepare_merges<Kind::kPlain>();
+    if (e == cudaSuccess) e = prepare_merges<Kind::kChunk>();
     cudaSetDevice(previous);
     if (e != cudaSuccess) return pkv::fail(PKV_CUDA_ERROR, std::string("int4 decode: ") + cudaGetErrorString(e));
     info->ctas_per_sm = least < 1 ? 1 : least;
@@ -897,13 +942,32 @@ int device_info(int device, DeviceInfo *info) {
 
 bool aligned16(const void *p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
 
+template <Kind R>
+cudaError_t launch_split(const ArgsOf<R> &a, cudaStream_t stream) {
+    return pkv::launch_pdl_smem(int4_decode_kernel<R>, dim3(a.grid), dim3(kThreads), kSmem, stream, a);
+}
+
+template <Kind R>
+cudaError_t merge(const ArgsOf<R> &a, const DeviceInfo &info, cudaStream_t stream) {
+    // Half warps a head by the pieces that a row has when the GPU is full, so that one round of
+    // loads or two are enough; by nothing else, for results must not depend on the room of a
+    // captured launch.  (Whole calls: 100 rows, 5 pieces each, 18.0 us with 2 and 19.9 with 4;
+    // 64 rows, 7 each, 26.1 and 25.8; 7 rows, 64 each, 6.7 with 8 and 7.8 with 16; 2 rows, 222
+    // each, 26.1 with 16 and 25.1 with 32.)
+    const int pieces = info.sms * info.ctas_per_sm / a.batch + 1;
+    return pieces <= 4 ? launch_merge<1, R>(a, stream)
+        : pieces <= 6 ? launch_merge<2, R>(a, stream)
+        : pieces <= 16 ? launch_merge<4, R>(a, stream)
+        : pieces <= 96 ? launch_merge<8, R>(a, stream)
+                       : launch_merge<32, R>(a, stream);
+}
+
 // Checks and launches; `a` holds everything but the partials' addresses.
 int decode(Args a, void *workspace, int64_t workspace_bytes, cudaStream_t stream) {
     const int rc = pkv::int4::check_cache(a.cache.storage, a.cache.layers, a.cache.num_blocks, a.layer, 1);
     if (rc) return rc;
     const void *const query = a.query32 != nullptr ? static_cast<const void *>(a.query32) : a.query;
-    if (query == nullptr || a.lengths == nullptr || a.prefix == nullptr || (a.flat == nullptr && a.capacity > 0) ||
-        a.out == nullptr || a.error_flag == nullptr) {
+    if (query == nullptr || (a.flat == nullptr && a.capacity > 0) || a.out == nullptr || a.error_flag == nullptr) {
         return pkv::fail(PKV_VALUE_ERROR, "int4 decode: null pointer argument");
     }
     if (a.batch < 1 || a.capacity < 0 || a.grid < 1) {
@@ -926,23 +990,11 @@ int decode(Args a, void *workspace, int64_t workspace_bytes, cudaStream_t stream
         a.part_o = static_cast<float *>(workspace);
         a.part_ml = a.part_o + (static_cast<int64_t>(a.batch) + a.grid) * kQueryHeads * kDim;
     }
-    const auto kernel = a.key != nullptr       ? int4_decode_kernel<kFresh>
-                        : a.query32 != nullptr ? int4_decode_kernel<kWide>
-                                               : int4_decode_kernel<kHalf>;
-    e = pkv::launch_pdl_smem(kernel, dim3(a.grid),
-                             dim3(kThreads), kSmem, stream, a);
+    e = a.key != nullptr      ? launch_split(ArgsOf<Kind::kFresh>(a), stream)
+        : a.prefix != nullptr ? launch_split(ArgsOf<Kind::kPlain>(a), stream)
+                              : launch_split(ArgsOf<Kind::kChunk>(a), stream);
     if (e == cudaSuccess && a.grid > 1) {
-        // Half warps a head by the pieces that a row has when the GPU is full, so that one round of
-        // loads or two are enough; by nothing else, for results must not depend on the room of a
-        // captured launch.  (Whole calls: 100 rows, 5 pieces each, 18.0 us with 2 and 19.9 with 4;
-        // 64 rows, 7 each, 26.1 and 25.8; 7 rows, 64 each, 6.7 with 8 and 7.8 with 16; 2 rows, 222
-        // each, 26.1 with 16 and 25.1 with 32.)
-        const int pieces = info.sms * info.ctas_per_sm / a.batch + 1;
-        e = pieces <= 4 ? launch_merge<1>(a, stream)
-            : pieces <= 6 ? launch_merge<2>(a, stream)
-            : pieces <= 16 ? launch_merge<4>(a, stream)
-            : pieces <= 96 ? launch_merge<8>(a, stream)
-                           : launch_merge<32>(a, stream);
+        e = a.prefix != nullptr ? merge(ArgsOf<Kind::kPlain>(a), info, stream) : merge(ArgsOf<Kind::kChunk>(a), info, stream);
     }
     if (e != cudaSuccess) return pkv::fail(PKV_CUDA_ERROR, std::string("int4 decode launch failed: ") + cudaGetErrorString(e));
     return PKV_OK;
@@ -971,67 +1023,28 @@ Args args_of(const void *storage, int32_t layers, int32_t num_blocks, int32_t la
 
 }  // namespace
 
-// -- a prompt chunk as rows ---------------------------------------------------------
-// Token t of a chunk is a row of start + t + 1 tokens over the first blocks of the request's
-// table.  Blocks of the rows before row r:
-namespace {
-
-__host__ __device__ __forceinline__ int blocks_before(int start, int r) {
-    const auto upto = [](int n) { return n + kSlots * (n / kSlots) * (n / kSlots - 1) / 2 + n / kSlots * (n % kSlots); };
-    return upto(start + r) - upto(start);
-}
-
-__global__ void int4_rows_kernel(const int32_t *blocks, int start, int tokens, int32_t *lengths, int32_t *prefix, int32_t *flat) {
-    pkv::pdl_launch_dependents();
-    pkv::pdl_wait();
-    const int row = blockIdx.x;
-    const int first = blocks_before(start, row), count = (start + row) / kSlots + 1;
-    for (int j = threadIdx.x; j < count; j += blockDim.x) flat[first + j] = blocks[j];
-    if (threadIdx.x == 0) {
-        lengths[row] = start + row + 1;
-        prefix[row] = first;
-        if (row == tokens - 1) prefix[tokens] = first + count;
-    }
-}
-
-int64_t tables_bytes(int start, int tokens) {
-    return (4 * (2 * static_cast<int64_t>(tokens) + 1 + blocks_before(start, tokens)) + 15) / 16 * 16;
-}
-
-}  // namespace
-
 namespace pkv::int4 {
 
 int rows_workspace(int device, int start, int tokens, int64_t *bytes) {
     int32_t grid = 0;
-    int64_t partials = 0;
-    const int rc = pkv_int4_decode_plan(device, tokens, blocks_before(start, tokens), &grid, &partials);
-    *bytes = tables_bytes(start, tokens) + partials;
-    return rc;
+    return pkv_int4_decode_plan(device, tokens, blocks_before(start, tokens), &grid, bytes);
 }
 
 int attend_rows(const Cache &cache, int32_t layer, const void *query, bool query_fp32, int64_t query_stride,
                 const int32_t *blocks, int32_t start, int32_t tokens, void *out, int64_t out_stride, void *workspace,
                 int64_t workspace_bytes, int32_t *error_flag, cudaStream_t stream) {
     int device = 0;
-    cudaError_t e = cudaGetDevice(&device);
+    const cudaError_t e = cudaGetDevice(&device);
     if (e != cudaSuccess) return fail(PKV_CUDA_ERROR, std::string("cudaGetDevice: ") + cudaGetErrorString(e));
     const int total = blocks_before(start, tokens);
     int32_t grid = 0;
-    int64_t partials = 0;
-    if (const int rc = pkv_int4_decode_plan(device, tokens, total, &grid, &partials)) return rc;
-    const int64_t tables = tables_bytes(start, tokens);
-    if (workspace_bytes < tables + partials) {
-        return fail(PKV_VALUE_ERROR, "prefill attention: the workspace is too small (see pkv_int4_prefill_plan)");
-    }
-    int32_t *const lengths = static_cast<int32_t *>(workspace), *const prefix = lengths + tokens;
-    int32_t *const flat = prefix + tokens + 1;
-    e = launch_pdl(int4_rows_kernel, dim3(tokens), dim3(128), stream, blocks, start, tokens, lengths, prefix, flat);
-    if (e != cudaSuccess) return fail(PKV_CUDA_ERROR, std::string("prefill attention launch failed: ") + cudaGetErrorString(e));
-    Args a = args_of(cache.storage, cache.layers, cache.num_blocks, layer, query_fp32 ? nullptr : query, query_stride, lengths,
-                     prefix, flat, tokens, total, grid, out, out_stride, error_flag);
+    int64_t needed = 0;
+    if (const int rc = pkv_int4_decode_plan(device, tokens, total, &grid, &needed)) return rc;
+    Args a = args_of(cache.storage, cache.layers, cache.num_blocks, layer, query_fp32 ? nullptr : query, query_stride, nullptr,
+                     nullptr, blocks, tokens, total, grid, out, out_stride, error_flag);
     if (query_fp32) a.query32 = static_cast<const float *>(query);
-    return decode(a, static_cast<uint8_t *>(workspace) + tables, partials, stream);
+    a.start = start;
+    return decode(a, workspace, workspace_bytes, stream);
 }
 
 }  // namespace pkv::int4
@@ -1057,6 +1070,7 @@ extern "C" int pkv_int4_decode_attention(const void *storage, int32_t layers, in
                                          int32_t total_blocks, int32_t grid, void *out, int64_t out_stride,
                                          void *workspace, int64_t workspace_bytes, int32_t *error_flag, void *stream) {
     pkv::clear_error();
+    if (lengths == nullptr || prefix == nullptr) return pkv::fail(PKV_VALUE_ERROR, "int4 decode: null pointer argument");
     return decode(args_of(storage, layers, num_blocks, layer, query, query_stride, lengths, prefix, flat, batch,
                           total_blocks, grid, out, out_stride, error_flag),
                   workspace, workspace_bytes, static_cast<cudaStream_t>(stream));
@@ -1069,6 +1083,7 @@ extern "C" int pkv_int4_decode_layer(void *storage, int32_t layers, int32_t num_
                                      int32_t total_blocks, int32_t grid, int32_t clear, void *out, int64_t out_stride,
                                      void *workspace, int64_t workspace_bytes, int32_t *error_flag, void *stream) {
     pkv::clear_error();
+    if (lengths == nullptr || prefix == nullptr) return pkv::fail(PKV_VALUE_ERROR, "int4 decode: null pointer argument");
     if (key == nullptr || value == nullptr || rope_table == nullptr) {
         return pkv::fail(PKV_VALUE_ERROR, "int4 decode layer: key, value and rope_table are required");
     }

@@ -397,9 +397,6 @@ extern "C" int pkv_int4_prefill_attention(const void *storage, int32_t layers, i
         out_stride < kRow) {
         return pkv::fail(PKV_VALUE_ERROR, "prefill attention: rows must be 16-byte aligned, 2048 or more values apart in multiples of 8");
     }
-    if (workspace == nullptr || !aligned16(workspace)) {
-        return pkv::fail(PKV_VALUE_ERROR, "prefill attention: the workspace is required and must be 16-byte aligned");
-    }
     if (by_rows(start, tokens)) {
         const int rc = pkv::int4::check_cache(storage, layers, num_blocks, layer, 1);
         if (rc) return rc;
@@ -407,7 +404,7 @@ extern "C" int pkv_int4_prefill_attention(const void *storage, int32_t layers, i
                                       query_stride, blocks, start, tokens, out, out_stride, workspace, workspace_bytes,
                                       error_flag, static_cast<cudaStream_t>(stream));
     }
-    if (workspace_bytes < tiles_workspace(start, tokens)) {
+    if (workspace == nullptr || !aligned16(workspace) || workspace_bytes < tiles_workspace(start, tokens)) {
         return pkv::fail(PKV_VALUE_ERROR, "prefill attention: the workspace is too small (see pkv_int4_prefill_plan)");
     }
     const int count = (start + tokens + kSlots - 1) / kSlots;
