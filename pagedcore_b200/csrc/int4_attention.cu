@@ -455,15 +455,22 @@ __device__ __forceinline__ void fill_ring(const ArgsOf<R> &a, int begin, int end
     }
 }
 
+// a * b per lane, round to nearest.
+__device__ __forceinline__ uint64_t mul_f32x2(uint64_t a, uint64_t b) {
+    uint64_t d;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+    return d;
+}
+
 // One row's running softmax of heads 2 t and 2 t + 1, over the tokens of the lane's rows.
 struct Sums {
     float m0, m1;  // the references: weights are 2^(score - m)
-    float l0, l1;
+    uint64_t l;    // the normalisers, an FP32 pair
     float o[4][4];
 
     __device__ __forceinline__ void clear() {
         m0 = m1 = kLowest;
-        l0 = l1 = 0.f;
+        l = 0;
 #pragma unroll
         for (int mt = 0; mt < 4; ++mt) o[mt][0] = o[mt][1] = o[mt][2] = o[mt][3] = 0.f;
     }
@@ -471,8 +478,12 @@ struct Sums {
     // log2 of the weights of products s.  The product is rounded by itself, as raise does: far
     // out, what a fused operation keeps of it would be large (2^-24 of 2^38, in the exponent).
     __device__ __forceinline__ void exponents(const float (&s)[4], const Query &q, float (&x)[4]) const {
-        x[0] = __fmul_rn(s[0], q.factor0) - m0, x[1] = __fmul_rn(s[1], q.factor1) - m1;
-        x[2] = __fmul_rn(s[2], q.factor0) - m0, x[3] = __fmul_rn(s[3], q.factor1) - m1;
+        const uint64_t reference = pkv::f32x2(-m0, -m1);  // (a packed product would be fused with the sum)
+        const uint64_t p = pkv::f32x2(__fmul_rn(s[0], q.factor0), __fmul_rn(s[1], q.factor1));
+        const uint64_t r = pkv::f32x2(__fmul_rn(s[2], q.factor0), __fmul_rn(s[3], q.factor1));
+        const float2 first = pkv::unpack_f32x2(pkv::add_f32x2(p, reference));
+        const float2 second = pkv::unpack_f32x2(pkv::add_f32x2(r, reference));
+        x[0] = first.x, x[1] = first.y, x[2] = second.x, x[3] = second.y;
     }
 
     // References for scores that reach top0 and top1 in this lane.
@@ -485,8 +496,7 @@ struct Sums {
         const float alpha0 = pkv::exp2_approx(m0 - top0), alpha1 = pkv::exp2_approx(m1 - top1);
         m0 = top0;
         m1 = top1;
-        l0 *= alpha0;
-        l1 *= alpha1;
+        l = mul_f32x2(l, pkv::f32x2(alpha0, alpha1));
 #pragma unroll
         for (int mt = 0; mt < 4; ++mt) o[mt][0] *= alpha0, o[mt][1] *= alpha1, o[mt][2] *= alpha0, o[mt][3] *= alpha1;
     }
@@ -531,7 +541,8 @@ struct Tile {
 template <Kind R>
 __device__ __forceinline__ void score(const Tile &tile, const Query &q, float (&s)[4]) {
     s[0] = s[1] = s[2] = s[3] = 0.f;
-    const Steps k0((tile.ks & 0xffu) * 0x00800080u), k1((tile.ks >> 8) * 0x00800080u);  // each scale twice
+    // Each scale twice.
+    const Steps k0(__byte_perm(tile.ks, 0, 0x0404) >> 1), k1(__byte_perm(tile.ks, 0, 0x1414) >> 1);
 #pragma unroll
     for (int ks = 0; ks < 4; ++ks) {
         const uint32_t x = ks < 2 ? tile.k.x : tile.k.y, y = ks < 2 ? tile.k.z : tile.k.w;
@@ -546,11 +557,18 @@ __device__ __forceinline__ void score(const Tile &tile, const Query &q, float (&
 
 // Adds the weights w of a block's tokens (rows g and g + 8 of heads 2 t, 2 t + 1) times its V.
 __device__ __forceinline__ void add_values(const Tile &tile, const float (&w)[4], Sums &sums) {
-    const __half2 h01 = __floats2half2_rn(w[0], w[1]), h23 = __floats2half2_rn(w[2], w[3]);
-    const float2 f01 = __half22float2(h01), f23 = __half22float2(h23);
-    const uint32_t p0 = pkv::movmatrix_trans(pack(h01)), p1 = pkv::movmatrix_trans(pack(h23));
-    const uint32_t r0 = pkv::movmatrix_trans(pack(__floats2half2_rn(w[0] - f01.x, w[1] - f01.y)));
-    const uint32_t r1 = pkv::movmatrix_trans(pack(__floats2half2_rn(w[2] - f23.x, w[3] - f23.y)));
+    // hi: the first 11 bits, cut off by the integer pipe (the FP16 and FP32 ones are the busy ones);
+    // lo: the rest.
+    float hi[4], lo[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+        hi[j] = __uint_as_float(__float_as_uint(w[j]) & 0xffffe000u);
+        lo[j] = w[j] - hi[j];
+    }
+    const uint32_t p0 = pkv::movmatrix_trans(pack(__floats2half2_rn(hi[0], hi[1])));
+    const uint32_t p1 = pkv::movmatrix_trans(pack(__floats2half2_rn(hi[2], hi[3])));
+    const uint32_t r0 = pkv::movmatrix_trans(pack(__floats2half2_rn(lo[0], lo[1])));
+    const uint32_t r1 = pkv::movmatrix_trans(pack(__floats2half2_rn(lo[2], lo[3])));
     // Tokens 4 t, 4 t + 2 in the first pair, 4 t + 1, 4 t + 3 in the second.
     const Steps v0((tile.vs & 0x00ff00ffu) << 7), v1((tile.vs & 0xff00ff00u) >> 1);
     const uint4 &v = tile.v;
@@ -606,8 +624,7 @@ __device__ __forceinline__ void attend(Tile (&tile)[COUNT], int valid, const Que
         float w[4];
 #pragma unroll
         for (int j = 0; j < 4; ++j) w[j] = pkv::exp2_approx(x[b][j]);
-        sums.l0 += w[0] + w[2];
-        sums.l1 += w[1] + w[3];
+        sums.l = pkv::add_f32x2(sums.l, pkv::add_f32x2(pkv::f32x2(w[0], w[1]), pkv::f32x2(w[2], w[3])));
         add_values(tile[b], w, sums);
     }
 }
@@ -741,7 +758,8 @@ __global__ void __launch_bounds__(kThreads, 3) int4_decode_kernel(const __grid_c
         }
         if (failed) break;
 
-        const float l0 = sum8(sums.l0), l1 = sum8(sums.l1);
+        const float2 l = pkv::unpack_f32x2(sums.l);
+        const float l0 = sum8(l.x), l1 = sum8(l.y);
         const auto &o = sums.o;
         const int head0 = warp * kHeadGroup + 2 * t;
         if (row_first >= begin && row_last <= end) {
