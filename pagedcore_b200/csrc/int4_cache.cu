@@ -25,7 +25,7 @@ constexpr int kHeads = PKV_KV_HEADS;
 constexpr int kSlots = PKV_BLOCK_TOKENS;
 constexpr int kThreads = 2 * kHeads * 32;
 constexpr int kSpan = 4;       // tokens per CTA that writes K and V
-constexpr int kQuerySpan = 4;  // and per CTA that rotates queries
+constexpr int kQuerySpan = 2;  // and per CTA that rotates queries
 
 struct AppendArgs {
     pkv::int4::Cache cache;
@@ -59,55 +59,55 @@ __device__ __forceinline__ int checked_position(const AppendArgs &a, int token) 
     return 0;
 }
 
-// Norm and RoPE of kQuerySpan tokens' queries, four heads a warp: eight lanes a head, eight
-// dims a lane; the partner's dims (32 away) come from the lane four further.
+__device__ __forceinline__ float4 four(const uint2 &raw) {
+    const float2 x = __half22float2(*reinterpret_cast<const __half2 *>(&raw.x));
+    const float2 y = __half22float2(*reinterpret_cast<const __half2 *>(&raw.y));
+    return make_float4(x.x, x.y, y.x, y.y);
+}
+
+// Norm and RoPE of kQuerySpan tokens' queries: sixteen lanes a head, four dims a lane, so that
+// each store of FP32 fills whole sectors; the partner's dims (32 away) come from the lane eight
+// further.  A warp has two pairs of heads of each token in flight.
 __device__ void rotate_queries(const AppendArgs &a, int layer, int begin, int warp, int lane) {
-    const int chunk = lane & 7, at = (4 * warp + (lane >> 3)) * kDim + 8 * chunk;
-    const float sign = chunk < 4 ? -1.f : 1.f;
-    float weight[8];
-#pragma unroll
-    for (int i = 0; i < 8; ++i) weight[i] = 1.f;
+    constexpr int kPairs = kQuerySpan * 2;  // (token, pair of heads) of a warp
+    const int c = lane & 15;
+    const float sign = c < 8 ? -1.f : 1.f;
+    float4 weight = make_float4(1.f, 1.f, 1.f, 1.f);
     if (a.query_norm != nullptr) {
-        const __half *from = a.query_norm + static_cast<int64_t>(a.layer_begin + layer) * kDim + 8 * chunk;
-#pragma unroll
-        for (int i = 0; i < 8; ++i) weight[i] = __half2float(from[i]);
+        weight = four(*reinterpret_cast<const uint2 *>(a.query_norm + static_cast<int64_t>(a.layer_begin + layer) * kDim + 4 * c));
     }
-    for (int token = begin; token < min(begin + kQuerySpan, a.tokens); ++token) {
-        const uint4 own =
-            *reinterpret_cast<const uint4 *>(a.query_in + layer * a.q_layer_stride + token * a.q_token_stride + at);
-        const __half *factors = a.rope + checked_position(a, token) * kHalf + 8 * (chunk & 3);
-        const __half2 *h = reinterpret_cast<const __half2 *>(&own);
-        float x[8], y[8];
+    uint2 own[kPairs], cos[kPairs], sin[kPairs];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const float2 f = __half22float2(h[i]);
-            x[2 * i] = f.x, x[2 * i + 1] = f.y;
-        }
+    for (int j = 0; j < kPairs; ++j) {
+        const int token = min(begin + j / 2, a.tokens - 1), head = 4 * warp + 2 * (j & 1) + (lane >> 4);
+        own[j] = *reinterpret_cast<const uint2 *>(a.query_in + layer * a.q_layer_stride + token * a.q_token_stride + head * kDim + 4 * c);
+        const __half *factors = a.rope + checked_position(a, token) * kHalf + 4 * (c & 7);
+        cos[j] = *reinterpret_cast<const uint2 *>(factors);
+        sin[j] = *reinterpret_cast<const uint2 *>(factors + PKV_CONTEXT_LIMIT * kHalf);
+    }
+#pragma unroll
+    for (int j = 0; j < kPairs; ++j) {
+        float4 x = four(own[j]);
         if (a.query_norm != nullptr) {
-            float sum = 0.f;
+            float sum = fmaf(x.x, x.x, x.y * x.y) + fmaf(x.z, x.z, x.w * x.w);
 #pragma unroll
-            for (int i = 0; i < 8; ++i) sum = fmaf(x[i], x[i], sum);
-#pragma unroll
-            for (int offset = 1; offset < 8; offset <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, offset);
+            for (int offset = 1; offset < 16; offset <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, offset);
             const float inverse = rsqrtf(sum * (1.f / kDim) + static_cast<float>(a.eps));
-#pragma unroll
-            for (int i = 0; i < 8; ++i) x[i] *= inverse * weight[i];
+            x.x *= inverse * weight.x, x.y *= inverse * weight.y, x.z *= inverse * weight.z, x.w *= inverse * weight.w;
         }
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-            const float partner = __shfl_xor_sync(0xffffffffu, x[i], 4);
-            y[i] = x[i] * __half2float(factors[i]) + sign * partner * __half2float(factors[PKV_CONTEXT_LIMIT * kHalf + i]);
-        }
-        const int64_t to = layer * a.q_out_layer_stride + token * a.q_out_token_stride + at;
+        const float4 p = make_float4(__shfl_xor_sync(0xffffffffu, x.x, 8), __shfl_xor_sync(0xffffffffu, x.y, 8),
+                                     __shfl_xor_sync(0xffffffffu, x.z, 8), __shfl_xor_sync(0xffffffffu, x.w, 8));
+        const float4 k = four(cos[j]), s = four(sin[j]);
+        const float4 y = make_float4(x.x * k.x + sign * p.x * s.x, x.y * k.y + sign * p.y * s.y,
+                                     x.z * k.z + sign * p.z * s.z, x.w * k.w + sign * p.w * s.w);
+        const int token = begin + j / 2, head = 4 * warp + 2 * (j & 1) + (lane >> 4);
+        if (token >= a.tokens) continue;
+        const int64_t to = layer * a.q_out_layer_stride + token * a.q_out_token_stride + head * kDim + 4 * c;
         if (a.query_out_fp32) {
-            float4 *dst = reinterpret_cast<float4 *>(static_cast<float *>(a.query_out) + to);
-            dst[0] = make_float4(y[0], y[1], y[2], y[3]);
-            dst[1] = make_float4(y[4], y[5], y[6], y[7]);
+            *reinterpret_cast<float4 *>(static_cast<float *>(a.query_out) + to) = y;
         } else {
-            uint32_t r[4];
-#pragma unroll
-            for (int i = 0; i < 4; ++i) r[i] = pkv::pack_half2(__floats2half2_rn(y[2 * i], y[2 * i + 1]));
-            *reinterpret_cast<uint4 *>(static_cast<__half *>(a.query_out) + to) = make_uint4(r[0], r[1], r[2], r[3]);
+            const uint32_t low = pkv::pack_half2(__floats2half2_rn(y.x, y.y)), high = pkv::pack_half2(__floats2half2_rn(y.z, y.w));
+            *reinterpret_cast<uint2 *>(static_cast<__half *>(a.query_out) + to) = make_uint2(low, high);
         }
     }
 }
@@ -187,23 +187,23 @@ __global__ void __launch_bounds__(kThreads) int4_append_kernel(const __grid_cons
     else pkv::int4::store_value(to, c, slot % kSlots, word, scale);
 }
 
-// K and V of `blocks` as FP16, each [i][slot][head][dim].  One CTA per block, a group a thread:
-// 32 consecutive bytes out, a token's row of 512 by 16 threads.  index_out (nullable) receives
+// K and V of `blocks` as FP16, each [i][slot][head][dim].  One CTA per block, a word of codes a
+// thread: 16 consecutive bytes out, a warp whole rows (a thread with a group of 32 bytes filled
+// half of each sector at a time: 256 blocks MEASURED).  index_out (nullable) receives
 // 0 .. count - 1, the block table of the outputs as a pool.
-constexpr int kReadThreads = kSlots * kHeads * 4;
+constexpr int kReadThreads = kSlots * kHeads * 8;
 constexpr int64_t kBlockValues = kSlots * kHeads * kDim;
 
-__device__ __forceinline__ void store_group(__half *to, uint32_t w0, uint32_t w1, uint32_t scale) {
+__device__ __forceinline__ uint4 decode_word(uint32_t word, uint32_t scale) {
     const __half2 s = __half2half2(__ushort_as_half(static_cast<unsigned short>(scale << 7)));
-    __align__(16) __half2 v[8];
+    const uint32_t swapped = pkv::int4::swap_bytes(word);
+    uint32_t v[4];
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-        const uint32_t word = i < 4 ? w0 : w1;
-        const __half2 n = pkv::int4::nibble_pair(word, pkv::int4::swap_bytes(word), i & 3);
-        v[i] = __hmul2(__hsub2(n, __float2half2_rn(i & 1 ? 24.f : 264.f)), s);  // exact
+    for (int i = 0; i < 4; ++i) {
+        const __half2 n = pkv::int4::nibble_pair(word, swapped, i);
+        v[i] = pkv::pack_half2(__hmul2(__hsub2(n, __float2half2_rn(i & 1 ? 24.f : 264.f)), s));  // exact
     }
-    reinterpret_cast<uint4 *>(to)[0] = reinterpret_cast<const uint4 *>(v)[0];
-    reinterpret_cast<uint4 *>(to)[1] = reinterpret_cast<const uint4 *>(v)[1];
+    return make_uint4(v[0], v[1], v[2], v[3]);
 }
 
 __global__ void __launch_bounds__(kReadThreads)
@@ -215,20 +215,18 @@ __global__ void __launch_bounds__(kReadThreads)
     const bool bad = block < 0 || block >= cache.num_blocks;
     if (bad && threadIdx.x == 0) atomicOr(error_flag, PKV_DEVICE_BAD_BLOCK);
     if (index_out != nullptr && threadIdx.x == 0) index_out[blockIdx.x] = blockIdx.x;
-    const int t = threadIdx.x & 3, head = (threadIdx.x >> 2) & 3, token = threadIdx.x >> 4;
-    uint2 k = make_uint2(0, 0), v = k;
-    uint32_t ks = 0, vs = 0;
+    const int c = threadIdx.x & 7, head = (threadIdx.x >> 3) & 3, token = threadIdx.x >> 5;
+    uint32_t k = 0, v = 0, ks = 0, vs = 0;
     if (!bad) {
         const uint8_t *from = pkv::int4::block_at(cache, layer, block) + head * pkv::int4::kHeadBytes;
-        k = *reinterpret_cast<const uint2 *>(from + pkv::int4::key_words(t, token));
-        v.x = *reinterpret_cast<const uint32_t *>(from + pkv::int4::value_word(2 * t, token));
-        v.y = *reinterpret_cast<const uint32_t *>(from + pkv::int4::value_word(2 * t + 1, token));
-        ks = from[pkv::int4::scale_at(pkv::int4::kKeyScaleAt, t, token)];
-        vs = from[pkv::int4::scale_at(pkv::int4::kValueScaleAt, t, token)];
+        k = *reinterpret_cast<const uint32_t *>(from + pkv::int4::key_words(c >> 1, token) + 4 * (c & 1));
+        v = *reinterpret_cast<const uint32_t *>(from + pkv::int4::value_word(c, token));
+        ks = from[pkv::int4::scale_at(pkv::int4::kKeyScaleAt, c >> 1, token)];
+        vs = from[pkv::int4::scale_at(pkv::int4::kValueScaleAt, c >> 1, token)];
     }
-    const int64_t at = static_cast<int64_t>(blockIdx.x) * kBlockValues + threadIdx.x * pkv::int4::kGroup;
-    store_group(key_out + at, k.x, k.y, ks);
-    store_group(value_out + at, v.x, v.y, vs);
+    const int64_t at = static_cast<int64_t>(blockIdx.x) * (kBlockValues / 8) + threadIdx.x;
+    reinterpret_cast<uint4 *>(key_out)[at] = decode_word(k, ks);
+    reinterpret_cast<uint4 *>(value_out)[at] = decode_word(v, vs);
 }
 
 bool aligned16(const void *p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
