@@ -125,7 +125,7 @@ struct Norms {
 
 // From three arguments: both weights (or None) and eps.
 Norms norms_of(PyObject *const *args, const Cache &cache) {
-    if (args[0] == Py_None) return {};
+    if (args[0] == Py_None && args[1] == Py_None) return {};
     Norms norms;
     for (int i = 0; i < 2; ++i) {
         const at::Tensor &weight = tensor_of(args[i], "head norms");
@@ -213,10 +213,30 @@ at::Tensor output(const at::Tensor *out, int64_t rows, int index, const char *wh
     return *out;
 }
 
-// First byte and the byte behind the last of rows [rows, heads, 64].
-std::pair<uintptr_t, uintptr_t> span(const at::Tensor &rows) {
-    const auto first = reinterpret_cast<uintptr_t>(rows.data_ptr());
-    return {first, first + rows.element_size() * ((rows.size(0) - 1) * rows.stride(0) + rows.size(1) * kDim)};
+// Whether rows of `a` and of `b`, [..., rows, heads, 64] with contiguous [heads, 64], share memory.
+// Exact where the rows of both lie in the same pattern (views of one projection), else by the
+// ranges that they span.
+bool share(const at::Tensor &a, const at::Tensor &b) {
+    const auto reach = [](const at::Tensor &t) {  // bytes from the first to the end of the last
+        const int64_t n = t.dim();
+        int64_t values = t.size(n - 2) * kDim;
+        for (int64_t d = 0; d < n - 2; ++d) values += (t.size(d) - 1) * t.stride(d);
+        return static_cast<int64_t>(t.element_size()) * values;
+    };
+    if (a.numel() == 0 || b.numel() == 0) return false;
+    const int64_t apart = static_cast<int64_t>(reinterpret_cast<uintptr_t>(b.data_ptr()) - reinterpret_cast<uintptr_t>(a.data_ptr()));
+    if (apart >= reach(a) || -apart >= reach(b)) return false;
+    const int64_t n = a.dim();
+    const auto pitch = [n](const at::Tensor &t) { return static_cast<int64_t>(t.element_size()) * t.stride(n - 3); };
+    bool same = b.dim() == n && pitch(a) == pitch(b) && pitch(a) > 0;
+    if (n == 4) {
+        const auto layer = [](const at::Tensor &t) { return static_cast<int64_t>(t.element_size()) * t.stride(0); };
+        same = same && layer(a) == layer(b) && layer(a) % pitch(a) == 0;
+    }
+    if (!same) return true;
+    const int64_t at = (apart % pitch(a) + pitch(a)) % pitch(a);  // where rows of b begin within those of a
+    const auto width = [n](const at::Tensor &t) { return static_cast<int64_t>(t.element_size()) * t.size(n - 2) * kDim; };
+    return at < width(a) || at + width(b) > pitch(a);
 }
 
 // Whether `rows` lie where `out` is written, other than as the same rows.
@@ -225,8 +245,7 @@ bool within(const at::Tensor &rows, const at::Tensor &out) {
         rows.scalar_type() == out.scalar_type()) {
         return false;
     }
-    const auto a = span(rows), b = span(out);
-    return b.first < a.second && a.first < b.second;
+    return share(rows, out);
 }
 
 void check_status(int status) {
@@ -279,16 +298,6 @@ bool rows_apart(const at::Tensor &rows) {
     return within_ >= kRow && over >= (tokens - 1) * within_ + kRow;
 }
 
-// Whether a row of `out` may be written before another row of `query` that it overlaps is read.
-bool mixes(const at::Tensor &query, const at::Tensor &out) {
-    if (query.data_ptr() == out.data_ptr() && query.strides() == out.strides() && out.scalar_type() == at::kHalf) return false;
-    const auto reach = [](const at::Tensor &rows) {
-        return rows.element_size() * ((rows.size(0) - 1) * rows.stride(0) + (rows.size(1) - 1) * rows.stride(1) + kRow);
-    };
-    const auto first = reinterpret_cast<uintptr_t>(query.data_ptr()), begin = reinterpret_cast<uintptr_t>(out.data_ptr());
-    return begin < first + reach(query) && first < begin + reach(out);
-}
-
 // (storage, key, value, slots, layer_begin, error_flag, positions, rope_table, query, query_out, query_norm, key_norm, eps)
 PyObject *append_kv(PyObject *const *args) {
     const Cache cache = cache_of(args[0]);
@@ -311,7 +320,7 @@ PyObject *append_kv(PyObject *const *args) {
         refuse("rope_table goes with positions, query with both");
     }
     if (out != nullptr && given == nullptr) refuse("query_out goes with query");
-    if (args[10] != Py_None && table == nullptr) refuse("norms go with rope_table");
+    if ((args[10] != Py_None || args[11] != Py_None) && table == nullptr) refuse("norms go with rope_table");
     const void *const rope = table != nullptr ? rope_of(*table, index) : nullptr;
     const int32_t *const at_positions = table != nullptr ? int_list(*positions, "positions", tokens, index) : nullptr;
     const Norms norms = norms_of(args + 10, cache);
@@ -333,10 +342,14 @@ PyObject *append_kv(PyObject *const *args) {
             }
             result = *out;
         }
-        query = given->numel() != 0 && (!rows_ok(*given) || (out != nullptr && mixes(*given, *out))) ? dense(*given) : *given;
+        query = given->numel() != 0 && (!rows_ok(*given) || (out != nullptr && within(*given, *out))) ? dense(*given) : *given;
     }
     if (layers != 0 && tokens != 0) {
         take_pair(key, value);
+        if (out != nullptr && (share(key.get(), *out) || share(value.get(), *out))) {  // read while queries are written
+            key.make_dense();
+            value.make_dense();
+        }
         const bool rotates = query.defined();
         launch(index, [&](void *stream) {
             return pkv_int4_append_kv(

@@ -673,12 +673,15 @@ __global__ void __launch_bounds__(kThreads, 3) int4_decode_kernel(const __grid_c
             sample = row + lane * step < a.batch ? a.prefix_at(min(row + (lane + 1) * step, a.batch)) : INT32_MAX;
         }
     }
-    // Rows without blocks: zeros.  (The merge looks at the rows' order too, where there is one.)
-    for (int b = blockIdx.x * kThreads + threadIdx.x; (a.clear || a.grid == 1) && b < a.batch; b += a.grid * kThreads) {
-        const int first = a.prefix_at(b), last = a.prefix_at(b + 1);
-        if (out_of_order(b, first, last)) atomicOr(a.error_flag, PKV_DEVICE_BAD_BLOCK);
-        if (a.clear && last <= first) {
-            for (int i = 0; i < kQueryHeads * kDim; ++i) a.out[b * a.out_stride + i] = __float2half_rn(0.f);
+    // Rows without blocks: zeros, a warp looking at 32 rows.  (The merge looks at the rows' order
+    // too, where there is one.)
+    for (int b = (blockIdx.x * (kWarps + 1) + warp) * 32; (a.clear || a.grid == 1) && b < a.batch; b += a.grid * kThreads) {
+        const int r = b + lane;
+        const int first = r < a.batch ? a.prefix_at(r) : 0, last = r < a.batch ? a.prefix_at(r + 1) : 1;
+        if (r < a.batch && out_of_order(r, first, last)) atomicOr(a.error_flag, PKV_DEVICE_BAD_BLOCK);
+        for (unsigned none = __ballot_sync(0xffffffffu, last <= first); a.clear && none != 0; none &= none - 1) {
+            uint4 *const out = reinterpret_cast<uint4 *>(a.out + (b + __ffs(none) - 1) * a.out_stride);
+            for (int i = lane; i < kQueryHeads * kDim / 8; i += 32) out[i] = make_uint4(0, 0, 0, 0);
         }
     }
     if (static_cast<int>(blockIdx.x) >= pieces || begin >= end) return;

@@ -401,6 +401,39 @@ def test_a_prompt_a_bad_block_and_its_report() -> None:
     assert bool(((out[99].double() - exact).abs() <= bound).all())
 
 
+@pytest.mark.parametrize("start, tokens", [(64, 40), (700, 9)])
+def test_a_few_prompt_tokens_behind_a_long_context_and_a_bad_block(start, tokens) -> None:
+    case = Case(35, [start + tokens])
+    blocks, query = case.batch()[2].clone(), randn(36, tokens, 32, 64)
+    blocks[2] = case.cache.num_blocks + 5
+    out = int4.prefill_attention(case.cache, LAYER, query, blocks, start, case.flag)
+    assert int(case.flag.item()) == 1
+    for t in (0, tokens - 1):
+        key, value = (x.clone() for x in case.tokens(0, start + t + 1))
+        key[32:48] = value[32:48] = 0
+        exact, bound = attend64(query[t], key, value)
+        assert bool(((out[t].double() - exact).abs() <= bound).all())
+
+
+@pytest.mark.parametrize("exponent", [-60, 16, 24, 31, 60, 100])
+@pytest.mark.parametrize("start, tokens", [(0, 40), (300, 70), (1000, 3)])
+def test_prompt_queries_of_any_size(exponent, start, tokens) -> None:
+    """Far out the largest score's value alone is left; scores within their rounding of it may take its place."""
+    case = Case(37, [start + tokens])
+    query = torch.ldexp(randn(38, tokens, 32, 64), torch.tensor(exponent, device=case.device))
+    out = int4.prefill_attention(case.cache, LAYER, query, case.batch()[2], start, case.flag)
+    assert bool(out.isfinite().all()) and int(case.flag.item()) == 0
+    for t in (0, tokens - 1):
+        key, value = case.tokens(0, start + t + 1)
+        exact, bound = attend64(query[t], key, value, HALF_FP16)
+        scores = (query[t].double().view(4, 8, 64) @ key.transpose(0, 1).transpose(1, 2) / 8).topk(min(2, key.shape[0]), -1)[0]
+        gap = scores[..., 0] - scores[..., -1]
+        off = 4 * 65 * F32 * (query[t].double().abs().view(4, 8, 64) @ key.abs().transpose(0, 1).transpose(1, 2) / 8).amax(-1)
+        clear = ((gap > 2 * off + 50) | (off < 1)).reshape(32) if key.shape[0] > 1 else torch.ones(32, dtype=torch.bool, device=out.device)
+        bound = torch.where((off < 1).reshape(32, 1), bound, HALF_FP16 * exact.abs() + 2.0**-20)
+        assert bool(((out[t].double() - exact).abs() <= bound)[clear].all())
+
+
 # -- together, elsewhere, captured -----------------------------------------------------------
 def test_a_prompt_then_tokens_as_they_are_used() -> None:
     """Two requests: prompts written and attended to, then steps; each against the values in the cache."""
@@ -450,6 +483,24 @@ def test_an_output_may_be_the_query_and_overlaps_are_read_first() -> None:
     expected = int4.decode_layer(case.cache, LAYER, fused[:, :32], fused[:, 32:36], fused[:, 36:], *args)
     got = int4.decode_layer(case.cache, LAYER, fused[:, :32], fused[:, 32:36], fused[:, 36:], *args, fused[:, 8:])
     assert torch.equal(got, expected)
+
+
+def test_rotated_queries_written_over_keys_and_values() -> None:
+    """An output over K and V of other tokens, and one beside them in the same rows."""
+    sides = []
+    for how in ("new", "over", "beside"):
+        case = Case(43, [0], spare=8)
+        case.tables[0] = case.free[:4]
+        fused = randn(44, 1, 50, 48, 64).half()
+        query, key, value = fused[:, :, :32], fused[:, :, 32:36], fused[:, :, 36:40]
+        out = {"new": torch.empty(1, 50, 32, 64, dtype=torch.float16, device=case.device), "over": fused[:, :, 8:40],
+               "beside": fused[:, :, :32]}[how]
+        positions = torch.arange(50, device=case.device).int()
+        got = int4.append_kv(case.cache, key, value, case.slots(0, 0, 50), layer_begin=LAYER, error_flag=case.flag,
+                             positions=positions, rope_table=case.rope, query=query, query_out=out)
+        sides.append((got.clone(), case.cache.storage.clone()))
+    for got, storage in sides[1:]:
+        assert torch.equal(got, sides[0][0]) and torch.equal(storage, sides[0][1])
 
 
 def test_a_cache_past_32_bits_of_offset() -> None:
@@ -555,6 +606,8 @@ def test_refusals() -> None:
     refused("head norms", append, norms=int4.HeadNorms(good.query.cpu(), good.key), **both)
     refused("eps", append, norms=int4.HeadNorms(good.query, good.key, -1.0), **both)
     refused("eps", append, norms=int4.HeadNorms(good.query, good.key, math.nan), **both)
+    with pytest.raises(TypeError, match="head norms"):
+        append(norms=int4.HeadNorms(None, good.key), **both)
     refused("layers out of range", int4.read_blocks, cache, LAYERS, flat, flag)
     refused("blocks", int4.read_blocks, cache, LAYER, flat.long(), flag)
     refused("error_flag", int4.read_blocks, cache, LAYER, flat, flag.cpu())
