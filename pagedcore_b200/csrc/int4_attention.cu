@@ -151,7 +151,8 @@ struct Cut {
     __device__ __forceinline__ int64_t begins(int g) const { return (g * weight + pieces - 1) / pieces; }
 };
 
-// The rows of a list of up to kWeighedRows rows, 32 k + lane in each lane.
+// The rows of a list of up to kWeighedRows rows, 32 k + lane in each lane; what they list before
+// block 0 (of a list that is out of order) is left out, so that a row found ends past its block.
 struct RowScan {
     static constexpr int kParts = kWeighedRows / 32;
     int first[kParts], last[kParts];
@@ -163,7 +164,7 @@ struct RowScan {
         for (int k = 0; k < kParts; ++k) {
             const int r = 32 * k + lane;
             first[k] = last[k] = 0;
-            if (r < a.batch) first[k] = a.prefix_at(r), last[k] = a.prefix_at(r + 1);
+            if (r < a.batch) first[k] = max(a.prefix_at(r), 0), last[k] = a.prefix_at(r + 1);
         }
 #pragma unroll
         for (int k = 0; k < kParts; ++k) held[k] = __ballot_sync(0xffffffffu, last[k] > first[k]);

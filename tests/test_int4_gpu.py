@@ -304,7 +304,9 @@ def test_a_block_outside_the_cache_reads_as_zeros() -> None:
         assert bool(((out[row].double() - exact).abs() <= bound).all())
 
 
-@pytest.mark.parametrize("prefix", [[0, 3, 2], [-1, 2], [1, 2], [0, -5, 2], [0, 1000000, 2], [0, 90, 40, 60]], ids=str)
+@pytest.mark.parametrize(
+    "prefix", [[0, 3, 2], [-1, 2], [1, 2], [0, -5, 2], [-5, -2, 2], [-9, -1, 0, 2], [0, 1000000, 2], [0, 90, 40, 60]], ids=str
+)
 @pytest.mark.parametrize("layer_call", [False, True])
 def test_rows_out_of_order_are_reported(prefix, layer_call) -> None:
     case = Case(18, [16 * 60])
