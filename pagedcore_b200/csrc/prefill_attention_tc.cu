@@ -235,66 +235,63 @@ __device__ __forceinline__ void load_q_row(uint32_t q_smem, const TcArgs &a, con
     pkv::cp_async_commit();
 }
 
-// Eight values of the query, FP16 or FP32.
-__device__ __forceinline__ void load_q8(const TcArgs &a, int64_t at, float (&v)[8]) {
-    if (a.query32 != nullptr) {
-        const float4 *src = reinterpret_cast<const float4 *>(a.query32 + at);
-        const float4 x = src[0], y = src[1];
-        v[0] = x.x, v[1] = x.y, v[2] = x.z, v[3] = x.w, v[4] = y.x, v[5] = y.y, v[6] = y.z, v[7] = y.w;
-    } else {
-        const uint4 raw = *reinterpret_cast<const uint4 *>(a.query + at);
-        const __half2 *h = reinterpret_cast<const __half2 *>(&raw);
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const float2 f = __half22float2(h[i]);
-            v[2 * i] = f.x, v[2 * i + 1] = f.y;
-        }
-    }
+// Four values of the query, FP16 or FP32.
+__device__ __forceinline__ float4 load_q4(const TcArgs &a, int64_t at) {
+    if (a.query32 != nullptr) return *reinterpret_cast<const float4 *>(a.query32 + at);
+    const uint2 raw = *reinterpret_cast<const uint2 *>(a.query + at);
+    const float2 x = __half22float2(*reinterpret_cast<const __half2 *>(&raw.x));
+    const float2 y = __half22float2(*reinterpret_cast<const __half2 *>(&raw.y));
+    return make_float4(x.x, x.y, y.x, y.y);
 }
 
-// FINE: the row times log2(e) / 8 and 2^-e as two FP16 numbers that add up to each value, the
-// high halves at q_smem and the low ones a tile further.  Returns 2^e.  (Few loads at a time:
-// the registers for a whole row are not there.  All at once before the first step, where they
-// are, saved 0.5 us of 70.)
-__device__ __forceinline__ float load_q_row_fine(uint32_t q_smem, const TcArgs &a, const Item &it, int r) {
-    const int t = min(it.t0 + (r >> 3), a.tokens - 1);
-    const int64_t at = static_cast<int64_t>(t) * a.query_stride + (it.kv * 8 + (r & 7)) * kHeadDim;
-    const uint32_t row = q_smem + (r >> 3) * 1024 + (r & 7) * kRowBytes;
-    float largest = 0.f;  // of the finite values
-#pragma unroll 2
-    for (int c = 0; c < 8; ++c) {
-        float v[8];
-        load_q8(a, at + 8 * c, v);
+// FINE: the rows of a warp times log2(e) / 8 and 2^-e, e a row's own, as two FP16 numbers that add
+// up to each value, the high halves at q_smem and the low ones a tile further.  Returns 2^e of row
+// r.  Sixteen lanes a row, so that a load takes two whole rows, and eight loads at a time (a
+// thread that read its own row, few loads at a time and twice for its maximum, took 11,000 clocks,
+// a fifth of the kernel).
+__device__ __forceinline__ float load_q_rows_fine(uint32_t q_smem, const TcArgs &a, const Item &it, int r) {
+    const int lane = r & 31, base = r - lane, c = lane & 15;
+    float mine = 0.f;
+#pragma unroll 1
+    for (int batch = 0; batch < 4; ++batch) {
+        float4 v[4];
 #pragma unroll
-        for (int i = 0; i < 8; ++i) largest = pkv::fp8::max_finite(largest, v[i]);
-    }
-    // A row of zeros or of FP32's subnormals: 2^100.
-    const int e = max((__float_as_int(largest) >> 23) - 127 - 14, -100);
-    const float factor = pkv::fp8::exp2_int(-e) * kScaleLog2;
-#pragma unroll 2
-    for (int c = 0; c < 8; ++c) {
-        float v[8];
-        load_q8(a, at + 8 * c, v);
-        uint32_t high[4], low[4];
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const float x = __fmul_rn(v[2 * i], factor), y = __fmul_rn(v[2 * i + 1], factor);
-            const __half2 h = __floats2half2_rn(x, y);
-            const float2 f = __half22float2(h);
-            high[i] = pkv::pack_half2(h);
-            low[i] = pack2(x - f.x, y - f.y);
+        for (int p = 0; p < 4; ++p) {
+            const int row = base + 8 * batch + 2 * p + (lane >> 4);
+            const int t = min(it.t0 + (row >> 3), a.tokens - 1);
+            v[p] = load_q4(a, static_cast<int64_t>(t) * a.query_stride + (it.kv * 8 + (row & 7)) * kHeadDim + 4 * c);
         }
-        const uint32_t to = row + ((c ^ (r & 7)) << 4);
-        asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(to), "r"(high[0]), "r"(high[1]), "r"(high[2]), "r"(high[3]) : "memory");
-        asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(to + kQBytes), "r"(low[0]), "r"(low[1]), "r"(low[2]), "r"(low[3]) : "memory");
+#pragma unroll
+        for (int p = 0; p < 4; ++p) {
+            const int row = base + 8 * batch + 2 * p + (lane >> 4);
+            float largest = 0.f;  // of the finite values
+            largest = pkv::fp8::max_finite(pkv::fp8::max_finite(largest, v[p].x), v[p].y);
+            largest = pkv::fp8::max_finite(pkv::fp8::max_finite(largest, v[p].z), v[p].w);
+#pragma unroll
+            for (int offset = 1; offset < 16; offset <<= 1) {
+                largest = fmaxf(largest, __shfl_xor_sync(0xffffffffu, largest, offset));
+            }
+            // A row of zeros or of FP32's subnormals: 2^100.
+            const int e = max((__float_as_int(largest) >> 23) - 127 - 14, -100);
+            const float factor = pkv::fp8::exp2_int(-e) * kScaleLog2;
+            const float x = __fmul_rn(v[p].x, factor), y = __fmul_rn(v[p].y, factor);
+            const float z = __fmul_rn(v[p].z, factor), w = __fmul_rn(v[p].w, factor);
+            const __half2 h0 = __floats2half2_rn(x, y), h1 = __floats2half2_rn(z, w);
+            const float2 f0 = __half22float2(h0), f1 = __half22float2(h1);
+            const uint32_t to = q_smem + (row >> 3) * 1024 + (row & 7) * kRowBytes + (((c >> 1) ^ (row & 7)) << 4) + 8 * (c & 1);
+            asm volatile("st.shared.v2.b32 [%0], {%1, %2};" ::"r"(to), "r"(pkv::pack_half2(h0)), "r"(pkv::pack_half2(h1)) : "memory");
+            asm volatile("st.shared.v2.b32 [%0], {%1, %2};" ::"r"(to + kQBytes), "r"(pack2(x - f0.x, y - f0.y)), "r"(pack2(z - f1.x, w - f1.y)) : "memory");
+            const float scale = __shfl_sync(0xffffffffu, pkv::fp8::exp2_int(e), 16 * (lane & 1));
+            if ((lane >> 1) == 4 * batch + p) mine = scale;
+        }
     }
-    return pkv::fp8::exp2_int(e);
+    return mine;
 }
 
 // Either, and the factor from the row's products to scores in base 2.
 template <bool FINE>
 __device__ __forceinline__ float load_q(uint32_t q_smem, const TcArgs &a, const Item &it, int r) {
-    if constexpr (FINE) return load_q_row_fine(q_smem, a, it, r);
+    if constexpr (FINE) return load_q_rows_fine(q_smem, a, it, r);
     load_q_row(q_smem, a, it, r);
     return kScaleLog2;
 }
@@ -565,7 +562,7 @@ __global__ void __maxnreg__(120)
                 pkv::tc::tmem_wait_ld();
                 // s_full of the item's last step: every S MMA of the item has
                 // completed, so the next item's Q may replace this one's.
-                if (last && next < items) next_scale = load_q<FINE>(q_smem, a, item_info(next, tiles, a), r);
+                if (!FINE && last && next < items) next_scale = load_q<FINE>(q_smem, a, item_info(next, tiles, a), r);
 
                 float s[64];
 #pragma unroll
@@ -662,7 +659,7 @@ __global__ void __maxnreg__(120)
                 }
                 pkv::tc::tmem_wait_st();  // P_g (and a rescaled O) written
                 m = m_new;
-                if (last && next < items) {
+                if (!FINE && last && next < items) {
                     pkv::cp_async_wait<0>();         // the next item's Q row landed
                     pkv::fence_proxy_async_smem();   // and is ordered before the MMA's (async proxy) reads
                 }
@@ -670,7 +667,13 @@ __global__ void __maxnreg__(120)
                 __syncwarp();
                 if (lane == 0) {
                     pkv::mbar_arrive(bar_addr(bars.p_full[g % kSBuffers]));
-                    if (last && next < items) pkv::mbar_arrive(bar_addr(bars.q_full));
+                    if (!FINE && last && next < items) pkv::mbar_arrive(bar_addr(bars.q_full));
+                }
+                if (FINE && last && next < items) {  // (here the registers are free, and P.V runs)
+                    next_scale = load_q<FINE>(q_smem, a, item_info(next, tiles, a), r);
+                    pkv::fence_proxy_async_smem();
+                    __syncwarp();
+                    if (lane == 0) pkv::mbar_arrive(bar_addr(bars.q_full));
                 }
             }
             if (!ok) break;
