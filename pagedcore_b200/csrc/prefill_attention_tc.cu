@@ -53,14 +53,15 @@
 // TMEM: S/P buffers at columns 0, 64, 128, O at 192 (256 columns, two CTAs
 // per SM).  Shared memory: Q (16 KiB) and the K and V rings.
 //
-// FINE, over the 8-bit cache, rounds nothing but the output to FP16:
+// FINE, over a quantised cache's values, rounds nothing but the output to FP16:
 // - A query row (FP16, or FP32 as rotated) is multiplied by log2(e) / 8 and a power of two
 //   that brings its largest value to 2^14 .. 2^15, whatever FP32 range it had, and becomes
 //   two Q tiles, the FP16 values and what they leave.  S takes both (four more MMAs a step,
 //   mostly hidden behind the softmax) and is scaled back by the power of two, exactly.
 // - What the FP16 weights leave goes over the second 32 columns of S_g's buffer, and P.V
 //   takes both.  (One FP16 number for each weight: relative error 2.9e-4 where the output's
-//   rounding alone gives 2.0e-4, and 43 us for 2047 tokens with their read; 53 with two.)
+//   rounding alone gives 2.0e-4.  Making the second costs 3.4 us of the 47.6 that 2047 tokens
+//   take with the read of their values.)
 // - The reference is m - 7 and moves when a weight would pass 2^15; past 2^20, where 7 would
 //   soon be lost in its rounding, it is m itself.
 //
@@ -296,10 +297,11 @@ __device__ __forceinline__ float load_q(uint32_t q_smem, const TcArgs &a, const 
     return kScaleLog2;
 }
 
-// At most 120 registers a thread: two CTAs of 256 threads then fit an SM
-// (the occupancy calculation gives one CTA at 125).
+// At most 128 registers a thread: two CTAs of 256 threads then fill an SM's (the occupancy
+// calculation gives one CTA from 119 on, clock stamps show two; 2047 tokens in FINE: 48.6 us at
+// 120, with spills, 47.6 at 128).
 template <bool FINE>
-__global__ void __maxnreg__(120)
+__global__ void __maxnreg__(128)
     prefill_tc_kernel(const TcArgs a) {
     extern __shared__ uint8_t dyn_smem[];
     __shared__ Barriers bars;
@@ -742,7 +744,7 @@ int prepare(int device, int *ctas) {
                                              cudaGetErrorString(e));
     }
     // Two CTAs fit an SM: 2 x (at most 105 KiB + static) of shared memory, 2 x 256
-    // columns of TMEM, 2 x 256 threads at 120 registers.
+    // columns of TMEM, 2 x 256 threads at 128 registers.
     const int per_sm = kCtasPerSm;
     *ctas = sms * per_sm;
     if (device >= 0 && device < kMaxDevices) resident[device].store(*ctas, std::memory_order_release);
