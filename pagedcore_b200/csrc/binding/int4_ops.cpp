@@ -256,11 +256,16 @@ void check_status(int status) {
     throw PythonError{};
 }
 
-// Runs `call` with the current stream of device `index`, whatever the current device is.
+// Runs `call` with the current stream of device `index`, whatever the current device is.  Other
+// threads run meanwhile: a launch waits where the stream's queue is full.
 template <typename Call>
 void launch(int index, Call call) {
     const c10::cuda::OptionalCUDAGuard guard(at::Device(at::kCUDA, index));
-    check_status(call(static_cast<void *>(c10::cuda::getCurrentCUDAStream(index).stream())));
+    void *const stream = c10::cuda::getCurrentCUDAStream(index).stream();
+    PyThreadState *const thread = PyEval_SaveThread();
+    const int status = call(stream);  // throws nothing
+    PyEval_RestoreThread(thread);
+    check_status(status);
 }
 
 at::Tensor bytes(int64_t count, int index) {
