@@ -44,6 +44,7 @@
 #include <stdint.h>
 
 #include <atomic>
+#include <cfloat>
 #include <initializer_list>
 #include <string>
 
@@ -82,7 +83,7 @@ constexpr float kValueFactor = 0x1p-6f;  // of the values in the MMAs
 constexpr float kMostWeight = 15.0f;  // log2 of the largest weight
 constexpr float kWeightShift = 11.0f;  // ... and of one at the reference when that is set
 constexpr float kFarScore = 0x1p20f;
-constexpr float kLowest = -1e30f;  // below every finite score
+constexpr float kLowest = -FLT_MAX;  // no finite score is below
 constexpr int kPartial = kQueryHeads * (kDim + 2);  // floats of a partial
 
 // What the rows are: sequences with rotated FP16 queries; sequences with a new token each (a

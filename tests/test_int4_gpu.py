@@ -418,7 +418,7 @@ def test_a_few_prompt_tokens_behind_a_long_context_and_a_bad_block(start, tokens
 
 
 @pytest.mark.parametrize("exponent", [-60, 16, 24, 31, 60, 100])
-@pytest.mark.parametrize("start, tokens", [(0, 40), (300, 70), (1000, 3)])
+@pytest.mark.parametrize("start, tokens", [(0, 1), (0, 40), (300, 70), (1000, 3)])
 def test_prompt_queries_of_any_size(exponent, start, tokens) -> None:
     """Far out the largest score's value alone is left; scores within their rounding of it may take its place."""
     case = Case(37, [start + tokens])
