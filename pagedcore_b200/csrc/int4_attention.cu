@@ -77,7 +77,8 @@ constexpr uint32_t kWaitPolls = 1u << 24;
 constexpr int kRowCost = 3;  // below a chunk's blocks
 constexpr int kWeighedRows = 256;
 constexpr int kMostGrid = 65535;
-static_assert(kRowCost < kChunk, "a piece could lie in the cost of one row");
+constexpr int kShortRow = 8;
+static_assert(kRowCost < kChunk, "a piece could lie in the cost of one row");  // pieces are kRowCost + 1 long or more
 constexpr float kScaleLog2 = 0.125f * 1.4426950408889634f;  // 64^-0.5 * log2(e)
 constexpr float kValueFactor = 0x1p-6f;  // of the values in the MMAs
 constexpr float kMostWeight = 15.0f;  // log2 of the largest weight
@@ -137,41 +138,13 @@ struct ArgsOf : Args {
     __device__ __forceinline__ int length_at(int row) const { return R == Kind::kChunk ? start + row + 1 : lengths[row]; }
 };
 
-// Pieces of a list of `total` blocks: at most one per CTA and per chunk.  (A captured
-// launch has a CTA for every resident slot.)
-__host__ __device__ __forceinline__ int pieces_of(int total, int grid) {
-    const int most = (total + kChunk - 1) / kChunk;
+// Most pieces of a list of `total` blocks in `rows` rows with blocks: one per CTA, and one per
+// chunk or per row, whichever are more.  (A captured launch has a CTA for every resident slot.)
+__host__ __device__ __forceinline__ int pieces_of(int total, int rows, int grid) {
+    const int chunks = (total + kChunk - 1) / kChunk, rows_most = rows < total ? rows : total;
+    const int most = chunks > rows_most ? chunks : rows_most;
     return most < 1 ? 1 : most < grid ? most : grid;
 }
-
-// How the list is cut: a block weighs 1 and a row's first block kRowCost more, what it costs a
-// CTA to begin a row (its queries, its result); piece g holds the blocks whose weights, summed to
-// and without the block itself, lie in [g, g + 1) * weight / pieces.  A piece is at least a chunk
-// long, so none is without blocks.  Beyond kWeighedRows rows, where a CTA has several rows and
-// they even out, rows weigh nothing.  (A decode layer of 256 rows of 1 to 2048 tokens takes 34.0,
-// 33.2, 32.3 and 32.0 us with a cost of 0, 1, 2 and 3.)
-struct Cut {
-    int total, pieces;
-    uint32_t weight, whole, rest;  // weight = whole * pieces + rest
-
-    template <Kind R>
-    __device__ __forceinline__ Cut(const ArgsOf<R> &a, int rows_with_blocks) {
-        total = total_blocks(a);
-        pieces = pieces_of(total, a.grid);
-        weight = static_cast<uint32_t>(total) + kRowCost * rows_with_blocks;
-        whole = weight / pieces;
-        rest = weight % pieces;
-    }
-    // Of block `block` in the list's `rank`-th row with blocks (counted from 1).
-    __device__ __forceinline__ int piece_of(int block, int rank) const {
-        return static_cast<int>((static_cast<int64_t>(block) + kRowCost * rank) * pieces / weight);
-    }
-    // The least weight that is in piece g.  (No product passes 32 bits, for pieces <= kMostGrid:
-    // divisions of 64 bits cost a small call 0.2 us.)
-    __device__ __forceinline__ int64_t begins(int g) const {
-        return static_cast<int64_t>(whole) * g + (rest * g + pieces - 1) / static_cast<uint32_t>(pieces);
-    }
-};
 
 // The rows of a list of up to kWeighedRows rows, 32 k + lane in each lane; what they list before
 // block 0 (of a list that is out of order) is left out, so that a row found ends past its block.
@@ -179,51 +152,101 @@ struct RowScan {
     static constexpr int kParts = kWeighedRows / 32;
     int first[kParts], last[kParts];
     unsigned held[kParts];  // rows with blocks
+    int count;    // ... how many
+    bool short_rows;  // none has more than kShortRow
 
     template <Kind R>
     __device__ __forceinline__ RowScan(const ArgsOf<R> &a, int lane) {
+        bool long_row = false;
 #pragma unroll
         for (int k = 0; k < kParts; ++k) {
             const int r = 32 * k + lane;
             first[k] = last[k] = 0;
             if (r < a.batch) first[k] = max(a.prefix_at(r), 0), last[k] = a.prefix_at(r + 1);
+            long_row |= last[k] > first[k] && last[k] - first[k] > kShortRow;
         }
-#pragma unroll
-        for (int k = 0; k < kParts; ++k) held[k] = __ballot_sync(0xffffffffu, last[k] > first[k]);
-    }
-    __device__ __forceinline__ int rows_with_blocks() const {
-        int count = 0;
-#pragma unroll
-        for (int k = 0; k < kParts; ++k) count += __popc(held[k]);
-        return count;
-    }
-    __device__ __forceinline__ int rank(int row) const {
-        int count = 0;
+        short_rows = !__any_sync(0xffffffffu, long_row);
+        count = 0;
 #pragma unroll
         for (int k = 0; k < kParts; ++k) {
-            const int upto = row - 32 * k;  // rows of this part that count
-            if (upto >= 0) count += __popc(upto >= 31 ? held[k] : held[k] & ((2u << upto) - 1u));
+            held[k] = __ballot_sync(0xffffffffu, last[k] > first[k]);
+            count += __popc(held[k]);
         }
-        return count;
     }
-    // The first block of weight `target` or more, and its row; `total` where there is none.
-    __device__ __forceinline__ int block_at(int64_t target, int total, int lane, int &row) const {
+    // Rows with blocks up to row `row`.
+    __device__ __forceinline__ int rank(int row) const {
+        int upto = 0;
+#pragma unroll
+        for (int k = 0; k < kParts; ++k) {
+            const int n = row - 32 * k;  // the last row of this part that counts
+            if (n >= 0) upto += __popc(n >= 31 ? held[k] : held[k] & ((2u << n) - 1u));
+        }
+        return upto;
+    }
+    // The first block of weight `target` or more, and its row, which ends past it in any list;
+    // `total` where there is none.
+    __device__ __forceinline__ int block_at(uint32_t target, int total, int lane, int &row) const {
         int before = 0;
 #pragma unroll
         for (int k = 0; k < kParts; ++k) {
-            const int cost = kRowCost * (before + __popc(held[k] & ((2u << lane) - 1u)));
-            const bool past = last[k] > first[k] && static_cast<int64_t>(last[k]) - 1 + cost >= target;
-            const unsigned found = __ballot_sync(0xffffffffu, past);
+            const uint32_t cost = kRowCost * (before + __popc(held[k] & ((2u << lane) - 1u)));
+            const unsigned found = __ballot_sync(0xffffffffu, last[k] > first[k] && last[k] - 1 + cost >= target);
             if (found != 0) {
                 const int from = __ffs(found) - 1;
                 row = 32 * k + from;
-                const int64_t block = max(static_cast<int64_t>(first[k]), target - cost);
-                return __shfl_sync(0xffffffffu, static_cast<int>(min(max(block, int64_t{0}), static_cast<int64_t>(total))), from);
+                const int block = max(first[k], target > cost ? static_cast<int>(target - cost) : 0);
+                return __shfl_sync(0xffffffffu, min(block, total), from);
             }
             before += __popc(held[k]);
         }
         row = INT32_MAX;
         return total;
+    }
+    // Where the `index`-th row with blocks begins and ends, cut at `total`, and the row.  (With an exit
+    // per part, as above, the rows of both searches land in local memory: 0.6 us a call.)
+    __device__ __forceinline__ void row_at(int index, int total, int lane, int &begin, int &end, int &row) const {
+        int found = INT32_MAX, from = 0, to = 0;
+#pragma unroll
+        for (int k = 0; k < kParts; ++k) {
+            if (last[k] > first[k] && __popc(held[k] & ((1u << lane) - 1u)) == index) found = 32 * k + lane, from = first[k], to = last[k];
+            index -= __popc(held[k]);
+        }
+        row = __reduce_min_sync(0xffffffffu, found);
+        begin = min(__shfl_sync(0xffffffffu, from, row & 31), total);
+        end = row == INT32_MAX ? begin : min(__shfl_sync(0xffffffffu, to, row & 31), total);
+    }
+};
+
+// How the list is cut.  Short rows (kShortRow blocks or less, a CTA for each): one piece a row.
+// Else a block weighs 1 and a row's first block kRowCost more, what it costs a CTA to begin a row
+// (its queries, its result); piece g holds the blocks whose weights, summed to and without the
+// block itself, lie in [g, g + 1) * weight / pieces.  A piece is kRowCost + 1 long or more, so none
+// is without blocks.  Beyond kWeighedRows rows, where a CTA has several rows and they even out, rows
+// weigh nothing.  (A decode layer of 256 rows of 1 to 2048 tokens takes 34.0, 33.2, 32.3 and 32.0 us
+// with a cost of 0, 1, 2 and 3.  Pieces of a chunk or more made short rows wait for one another: 8
+// rows of 5 tokens took 8.7 us and their layer with norms 16.3, a piece each 4.0 and 5.8.)
+struct Cut {
+    int total, pieces;
+    bool by_row;
+    uint32_t weight, whole, rest;  // weight = whole * pieces + rest
+
+    template <Kind R>
+    __device__ __forceinline__ Cut(const ArgsOf<R> &a, int rows_with_blocks, bool short_rows) {
+        total = total_blocks(a);
+        by_row = short_rows && rows_with_blocks > 0 && rows_with_blocks <= a.grid;
+        pieces = by_row ? rows_with_blocks : pieces_of(total, a.batch <= kWeighedRows ? rows_with_blocks : total, a.grid);
+        weight = static_cast<uint32_t>(total) + kRowCost * rows_with_blocks;
+        whole = weight / pieces;
+        rest = weight % pieces;
+    }
+    // Of block `block` in the list's `rank`-th row with blocks (counted from 1).
+    __device__ __forceinline__ int piece_of(int block, int rank) const {
+        return by_row ? rank - 1 : static_cast<int>((static_cast<int64_t>(block) + kRowCost * rank) * pieces / weight);
+    }
+    // The least weight that is in piece g, g <= pieces.  (No product passes 32 bits, for pieces <=
+    // kMostGrid: divisions of 64 bits cost a small call 0.2 us.)
+    __device__ __forceinline__ uint32_t begins(int g) const {
+        return whole * g + (rest * g + pieces - 1) / static_cast<uint32_t>(pieces);
     }
 };
 
@@ -673,23 +696,28 @@ __global__ void __launch_bounds__(kThreads, 3) int4_decode_kernel(const __grid_c
     pkv::pdl_launch_dependents();
 
     // The piece and the row that it begins in.
+    const int piece = blockIdx.x;
     int begin, end, row;
     int pieces;
     if (a.batch <= kWeighedRows) {
         const RowScan scan(a, lane);
-        const Cut cut(a, scan.rows_with_blocks());
+        const Cut cut(a, scan.count, scan.short_rows);
         pieces = cut.total > 0 ? cut.pieces : 0;
-        int other;
-        begin = scan.block_at(cut.begins(blockIdx.x), cut.total, lane, row);
-        end = scan.block_at(cut.begins(blockIdx.x + 1), cut.total, lane, other);
+        if (cut.by_row) {
+            scan.row_at(piece, cut.total, lane, begin, end, row);
+        } else {
+            int other;
+            begin = scan.block_at(cut.begins(min(piece, cut.pieces)), cut.total, lane, row);
+            end = scan.block_at(cut.begins(min(piece + 1, cut.pieces)), cut.total, lane, other);
+        }
     } else {
         // Of 32 samples of prefix, `step` rows apart, the first past `begin`, cut finer until the
         // samples are rows.
         int step = (a.batch + 31) / 32;
         int sample = lane * step < a.batch ? a.prefix_at(min((lane + 1) * step, a.batch)) : INT32_MAX;
-        const Cut cut(a, 0);
+        const Cut cut(a, 0, false);
         pieces = cut.total > 0 ? cut.pieces : 0;
-        begin = static_cast<int>(cut.begins(blockIdx.x)), end = static_cast<int>(cut.begins(blockIdx.x + 1));
+        begin = static_cast<int>(cut.begins(min(piece, cut.pieces))), end = static_cast<int>(cut.begins(min(piece + 1, cut.pieces)));
         row = 0;
         while (true) {
             const unsigned past = __ballot_sync(0xffffffffu, sample > begin);
@@ -710,7 +738,7 @@ __global__ void __launch_bounds__(kThreads, 3) int4_decode_kernel(const __grid_c
             for (int i = lane; i < kQueryHeads * kDim / 8; i += 32) out[i] = make_uint4(0, 0, 0, 0);
         }
     }
-    if (static_cast<int>(blockIdx.x) >= pieces || begin >= end) return;
+    if (piece >= pieces || begin >= end) return;
     if (row >= a.batch) {  // prefix does not grow from row to row
         if (threadIdx.x == 0) atomicOr(a.error_flag, PKV_DEVICE_BAD_BLOCK);
         return;
@@ -854,12 +882,14 @@ __global__ void __launch_bounds__(kMergeThreads<H>) int4_merge_kernel(const __gr
     const int row_at = min(row, a.batch - 1);
     const int first_block = a.prefix_at(row_at), last_block = a.prefix_at(row_at + 1) - 1;
     int rank = 0, rows_with_blocks = 0;
+    bool short_rows = false;
     if (a.batch <= kWeighedRows) {
         const RowScan scan(a, lane);
         rank = scan.rank(row_at);
-        rows_with_blocks = scan.rows_with_blocks();
+        rows_with_blocks = scan.count;
+        short_rows = scan.short_rows;
     }
-    const Cut cut(a, rows_with_blocks);
+    const Cut cut(a, rows_with_blocks, short_rows);
     if (row < a.batch) {
         if (lane == 0 && out_of_order(row, first_block, last_block + 1)) atomicOr(a.error_flag, PKV_DEVICE_BAD_BLOCK);
         if (last_block >= first_block && first_block >= 0 && last_block < cut.total) {
@@ -1106,7 +1136,10 @@ extern "C" int pkv_int4_decode_plan(int32_t device, int32_t batch, int32_t total
     DeviceInfo info;
     const int rc = device_info(device, &info);
     if (rc) return rc;
-    const int grid = pieces_of(total_blocks, info.sms * info.ctas_per_sm);  // at most one CTA per resident slot
+    // At most one CTA per resident slot.  (A short row alone is one piece and needs no merge: 5 blocks
+    // 4.7 us, in two pieces 5.8.)
+    const int grid = batch == 1 && total_blocks <= kShortRow
+        ? 1 : pieces_of(total_blocks, batch <= kWeighedRows ? batch : total_blocks, info.sms * info.ctas_per_sm);
     *out_grid = grid;
     *out_workspace_bytes = workspace_of(batch, grid);
     return PKV_OK;

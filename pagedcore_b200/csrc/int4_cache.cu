@@ -351,14 +351,14 @@ extern "C" int pkv_int4_read_blocks(const void *storage, int32_t layers, int32_t
 // reads a row's blocks for each token.  For a few tokens behind a long context.
 namespace {
 
-// Rows take about 8 us and 1.15 ns for each block of each row, tiles 8 us and 0.87 us for each 64
-// keys that the last tile walks (600 blocks a step is where they meet: 3 tokens behind 1900 take
-// 9.0 and 35.0 us, 75 behind 601 12.3 and 17.5, 150 behind 1500 25.7 and 31.7, 300 behind 256 18.0
-// and 15.8).  Rows of less than a chunk's blocks share pieces and take longer (16 tokens at the
-// beginning 18.9 and 9.2).
+// Rows take about 6.5 us and 1.2 ns for each block of each row, tiles 7 us and 0.87 us for each 64
+// keys that the last tile walks: 600 blocks a step is where they meet (3 tokens behind 1900 take 8.4
+// and 33.4 us, 75 behind 601 11.7 and 16.4, 150 behind 1500 25.1 and 30.1, 220 behind 256 15.3 and
+// 13.4).  At the beginning it is short rows, a piece each, against the first tiles: 16 tokens 6.4 and
+// 7.4 us, 75 tokens 8.0 and 8.3, 110 tokens 10.3 and 8.7.
 bool by_rows(int start, int tokens) {
     const int64_t blocks = static_cast<int64_t>(tokens) * (start + tokens / 2) / kSlots;
-    return tokens == 1 || (start >= 64 && blocks < 600ll * ((start + tokens) / 64));
+    return start >= 64 ? blocks < 600ll * ((start + tokens) / 64) : tokens <= 80 && start + tokens <= 8 * kSlots;
 }
 
 int64_t tiles_workspace(int start, int tokens) {

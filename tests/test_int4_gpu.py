@@ -206,7 +206,8 @@ def test_appends_outside_the_cache_and_the_rotation_table_are_reported() -> None
 
 # -- one token a row -------------------------------------------------------------------
 LENGTHS = [[1], [15], [16], [17], [64], [65], [0], [0, 0, 5, 0], [3, 0, 200, 64, 1, 0], [2048], [100, 513, 2048, 17],
-           [1] * 70, [33, 64, 1, 128, 127, 129] * 11, [0] * 40 + [700], [9000, 3], [40000]]
+           [1] * 70, [33, 64, 1, 128, 127, 129] * 11, [0] * 40 + [700], [9000, 3], [40000],
+           [5, 0] * 49, [16 * n + 1 for n in range(8)] * 12, [129] + [3] * 60, [128] * 256, [20] * 300, [128], [129]]
 
 
 @pytest.mark.parametrize("lengths", LENGTHS, ids=lambda v: f"{len(v)}rows{max(v)}")
@@ -219,8 +220,9 @@ def test_decode_attention(lengths) -> None:
     assert torch.equal(int4.decode_attention(case.cache, LAYER, query, *case.batch(), case.flag), out)
 
 
-def test_decode_attention_does_not_depend_on_the_room_of_the_block_list() -> None:
-    case = Case(16, [300, 5, 64])
+@pytest.mark.parametrize("rows", [[300, 5, 64], [5, 100, 128], [65, 0, 0], [40, 200, 3]], ids=str)
+def test_decode_attention_does_not_depend_on_the_room_of_the_block_list(rows) -> None:
+    case = Case(16, rows)
     lengths, prefix, flat, total = case.batch()
     query = randn(3, 3, 32, 64).half()
     expected = int4.decode_attention(case.cache, LAYER, query, lengths, prefix, flat, total, case.flag)
@@ -322,7 +324,7 @@ def test_rows_out_of_order_are_reported(prefix, layer_call) -> None:
     assert int(case.flag.item()) & 1
 
 
-@pytest.mark.parametrize("lengths", [[1], [16, 17], [1, 15, 16, 48, 700, 65], [2048, 3], [33] * 300], ids=lambda v: f"{len(v)}rows{max(v)}")
+@pytest.mark.parametrize("lengths", [[1], [16, 17], [1, 15, 16, 48, 700, 65], [2048, 3], [33] * 300, [5] * 49, [130] + [3] * 60], ids=lambda v: f"{len(v)}rows{max(v)}")
 @pytest.mark.parametrize("normed", [False, True])
 def test_decode_layer_writes_as_append_does_and_attends(lengths, normed) -> None:
     whole, parts = (Case(21, [n - 1 for n in lengths], spare=len(lengths) + 3) for _ in range(2))
@@ -374,7 +376,7 @@ def test_decode_layer_reports_a_row_without_a_token() -> None:
 
 
 # -- a prompt chunk ----------------------------------------------------------------------
-@pytest.mark.parametrize("start, tokens", [(0, 1), (0, 15), (0, 130), (7, 40), (64, 3), (100, 64), (601, 75), (300, 500), (2000, 48), (2047, 1), (0, 2047)])
+@pytest.mark.parametrize("start, tokens", [(0, 1), (0, 15), (0, 130), (7, 40), (64, 3), (100, 64), (601, 75), (300, 500), (2000, 48), (2047, 1), (0, 2047), (0, 75), (20, 90)])
 @pytest.mark.parametrize("dtype", [torch.float16, torch.float32])
 def test_prefill_attention(start, tokens, dtype) -> None:
     case = Case(31, [start + tokens])
@@ -418,7 +420,7 @@ def test_a_few_prompt_tokens_behind_a_long_context_and_a_bad_block(start, tokens
 
 
 @pytest.mark.parametrize("exponent", [-60, 16, 24, 31, 60, 100])
-@pytest.mark.parametrize("start, tokens", [(0, 1), (0, 40), (300, 70), (1000, 3)])
+@pytest.mark.parametrize("start, tokens", [(0, 1), (0, 40), (0, 200), (300, 70), (1000, 3)])
 def test_prompt_queries_of_any_size(exponent, start, tokens) -> None:
     """Far out the largest score's value alone is left; scores within their rounding of it may take its place."""
     case = Case(37, [start + tokens])
