@@ -345,24 +345,40 @@ extern "C" int pkv_int4_read_blocks(const void *storage, int32_t layers, int32_t
 //
 // By tiles: the request's blocks become an FP16 pool of one layer in the workspace (the values
 // are FP16 numbers: nothing is rounded), which the tensor-core prompt kernel attends to; that
-// kernel reads every block once for each 16 queries, but a tile's keys one after another.
+// kernel reads every block once for each 16 queries, and a tile's keys one after another, in several
+// parts where there are few tiles.
 //
 // By rows: each token a row of the decode attention, which cuts the keys over the whole GPU but
 // reads a row's blocks for each token.  For a few tokens behind a long context.
 namespace {
 
 // Rows take about 6.5 us and 1.2 ns for each block of each row, tiles 7 us and 0.87 us for each 64
-// keys that the last tile walks: 600 blocks a step is where they meet (3 tokens behind 1900 take 8.4
-// and 33.4 us, 75 behind 601 11.7 and 16.4, 150 behind 1500 25.1 and 30.1, 220 behind 256 15.3 and
-// 13.4).  At the beginning it is short rows, a piece each, against the first tiles: 16 tokens 6.4 and
-// 7.4 us, 75 tokens 8.0 and 8.3, 110 tokens 10.3 and 8.7.
+// keys that the last tile walks, where its keys are not cut into parts: 600 blocks a step is where
+// they meet, and 7500 blocks with parts (3 tokens behind 1900 take 8.4 us by rows and 16 by tiles, 75
+// behind 601 11.7 and 14.3, 150 behind 256 11.9 and 12.6, 110 behind 1000 16.7 and 18.0, 150 behind
+// 1000 19.8 and 18.1, 220 behind 256 15.3 and 13.6).  At the beginning it is short rows, a piece each,
+// against the first tiles: 16 tokens 6.4 and 7.4 us, 75 tokens 8.0 and 8.3, 110 tokens 10.3 and 8.7.
 bool by_rows(int start, int tokens) {
     const int64_t blocks = static_cast<int64_t>(tokens) * (start + tokens / 2) / kSlots;
-    return start >= 64 ? blocks < 600ll * ((start + tokens) / 64) : tokens <= 80 && start + tokens <= 8 * kSlots;
+    if (start < 64) return tokens <= 80 && start + tokens <= 8 * kSlots;
+    return blocks < 7500 && blocks < 600 * ((start + tokens) / 64);
 }
 
-int64_t tiles_workspace(int start, int tokens) {
-    return (start + tokens + kSlots - 1) / kSlots * (2 * kBlockValues * 2 + 4);
+// Of the tiles: an FP16 pool of one layer, its table, the partial results.
+struct TilesWorkspace {
+    int blocks, splits;
+    int64_t table_at, partials_at, bytes;
+};
+
+int tiles_workspace(int device, int start, int tokens, TilesWorkspace *w) {
+    if (const int rc = pkv::prefill_splits(device, start, tokens, &w->splits)) return rc;
+    w->blocks = (start + tokens + kSlots - 1) / kSlots;
+    w->table_at = static_cast<int64_t>(w->blocks) * 2 * kBlockValues * 2;
+    w->bytes = w->table_at + static_cast<int64_t>(w->blocks) * 4;
+    w->partials_at = (w->bytes + 15) / 16 * 16;
+    const int64_t partials = pkv::prefill_splits_bytes(tokens, w->splits);
+    if (partials > 0) w->bytes = w->partials_at + partials;
+    return PKV_OK;
 }
 
 int check_chunk(int32_t start, int32_t tokens) {
@@ -379,7 +395,9 @@ extern "C" int pkv_int4_prefill_plan(int32_t device, int32_t start, int32_t toke
     if (out_workspace_bytes == nullptr) return pkv::fail(PKV_VALUE_ERROR, "prefill plan: null pointer argument");
     if (const int rc = check_chunk(start, tokens)) return rc;
     if (by_rows(start, tokens)) return pkv::int4::rows_workspace(device, start, tokens, out_workspace_bytes);
-    *out_workspace_bytes = tiles_workspace(start, tokens);
+    TilesWorkspace tiles;
+    if (const int rc = tiles_workspace(device, start, tokens, &tiles)) return rc;
+    *out_workspace_bytes = tiles.bytes;
     return PKV_OK;
 }
 
@@ -405,15 +423,23 @@ extern "C" int pkv_int4_prefill_attention(const void *storage, int32_t layers, i
                                       query_stride, blocks, start, tokens, out, out_stride, workspace, workspace_bytes,
                                       error_flag, static_cast<cudaStream_t>(stream));
     }
-    if (workspace == nullptr || !aligned16(workspace) || workspace_bytes < tiles_workspace(start, tokens)) {
+    int device = 0;
+    if (start > 0) {  // (at the beginning the plan asks for no device)
+        const cudaError_t e = cudaGetDevice(&device);
+        if (e != cudaSuccess) return pkv::fail(PKV_CUDA_ERROR, std::string("cudaGetDevice: ") + cudaGetErrorString(e));
+    }
+    TilesWorkspace tiles;
+    if (const int rc = tiles_workspace(device, start, tokens, &tiles)) return rc;
+    if (workspace == nullptr || !aligned16(workspace) || workspace_bytes < tiles.bytes) {
         return pkv::fail(PKV_VALUE_ERROR, "prefill attention: the workspace is too small (see pkv_int4_prefill_plan)");
     }
-    const int count = (start + tokens + kSlots - 1) / kSlots;
-    const int64_t pool_bytes = static_cast<int64_t>(count) * 2 * kBlockValues * 2;
-    int32_t *const table = reinterpret_cast<int32_t *>(static_cast<uint8_t *>(workspace) + pool_bytes);
-    const int rc = read_blocks(storage, layers, num_blocks, layer, blocks, count, workspace,
-                               static_cast<__half *>(workspace) + count * kBlockValues, table, error_flag, stream);
+    uint8_t *const base = static_cast<uint8_t *>(workspace);
+    int32_t *const table = reinterpret_cast<int32_t *>(base + tiles.table_at);
+    const int rc = read_blocks(storage, layers, num_blocks, layer, blocks, tiles.blocks, workspace,
+                               static_cast<__half *>(workspace) + tiles.blocks * kBlockValues, table, error_flag, stream);
     if (rc) return rc;
-    return pkv::launch_prefill_attention_tc(workspace, count, 0, query, query_fp32 != 0, true, query_stride, table, start,
-                                            tokens, out, out_stride, error_flag, static_cast<cudaStream_t>(stream));
+    return pkv::launch_prefill_attention_tc(workspace, tiles.blocks, 0, query, query_fp32 != 0, true, query_stride, table,
+                                            start, tokens, out, out_stride, error_flag, static_cast<cudaStream_t>(stream),
+                                            tiles.splits,
+                                            tiles.splits > 1 ? reinterpret_cast<float *>(base + tiles.partials_at) : nullptr);
 }

@@ -11,6 +11,11 @@ namespace pkv {
 int launch_prefill_attention_tc(const void *pool, int32_t num_blocks, int32_t layer, const void *query,
                                 bool query_fp32, bool fine, int64_t query_stride, const int32_t *blocks,
                                 int32_t start, int32_t tokens, void *out, int64_t out_stride, int32_t *error_flag,
-                                cudaStream_t stream);
+                                cudaStream_t stream, int splits = 1, float *partials = nullptr);
+
+// fine alone: parts that each tile's keys are cut into where the tiles are too few for the GPU, and
+// the bytes of their partial results (16-byte aligned `partials`).
+int prefill_splits(int device, int32_t start, int32_t tokens, int *splits);
+int64_t prefill_splits_bytes(int32_t tokens, int splits);
 
 }  // namespace pkv

@@ -65,6 +65,11 @@
 // - The reference is m - 7 and moves when a weight would pass 2^15; past 2^20, where 7 would
 //   soon be lost in its rounding, it is m itself.
 //
+// SPLIT, for a chunk behind a context: where the items are less than half of the resident CTAs,
+// an item's keys are cut into as many parts as fill them, an item of work each, whose sums, references
+// and normalisers a second kernel merges (FP32; 300 tokens behind 1500, 76 items in 3 parts, take 25.2
+// us with the read of their values, whole 32.9; 512 behind 1000 26.2 and 36).
+//
 // Block ids outside the pool set PKV_DEVICE_BAD_BLOCK and read as zeros.
 // Every wait is bounded: on a timeout the thread sets
 // PKV_DEVICE_WAIT_TIMEOUT, the CTA stops issuing work, waits (bounded) for
@@ -77,8 +82,10 @@
 
 #include <algorithm>
 #include <atomic>
+#include <cfloat>
 #include <string>
 
+#include "block_list.cuh"
 #include "fp8.cuh"
 #include "pagedkv.h"
 #include "pdl.h"
@@ -137,6 +144,8 @@ constexpr float kScaleLog2 = 0.125f * 1.4426950408889634f;  // 64^-0.5 * log2(e)
 constexpr float kWeightShift = 7.0f;
 constexpr float kRescaleLog2 = 8.0f;
 constexpr float kFarScore = 0x1p20f;
+constexpr int kMostSplits = 8;
+constexpr int kLeastSaved = 6;  // steps of an item that parts must save: the merge takes about 5 us
 static_assert(kRows == kTileTokens * (PKV_QUERY_HEADS / kKvHeads), "a tile's rows are its tokens x 8 heads");
 static_assert(kKCopyLag < kKStages && kVCopyLag < kVStages, "a producer would wait for a stage it has not published");
 
@@ -157,6 +166,9 @@ struct TcArgs {
     int32_t tokens;
     int32_t *error_flag;
     const float *query32;  // FINE: in place of query, where it is not null
+    int32_t splits;        // SPLIT: parts of an item's keys
+    float *part_o;         // SPLIT: [tokens][splits][32][64], sums of weights times V
+    float *part_ml;        // SPLIT: [tokens][splits][32][2], references and normalisers
 };
 
 // Barriers of one CTA (8-byte mbarriers in static shared memory).
@@ -213,15 +225,24 @@ struct Item {
     int kv;       // KV head
     int nblocks;  // pool blocks up to the tile's last token
     int steps;    // 64-key steps over them
+    int split;    // SPLIT: the part of the keys
+    int before;   // SPLIT: steps before it
 };
 
+template <bool SPLIT>
 __device__ __forceinline__ Item item_info(int w, int tiles, const TcArgs &a) {
     Item it;
+    it.split = it.before = 0;
+    if constexpr (SPLIT) it.split = w % a.splits, w /= a.splits;
     it.kv = w % kKvHeads;
     it.t0 = (tiles - 1 - w / kKvHeads) * kTileTokens;
     const int last_t = min(it.t0 + kTileTokens - 1, a.tokens - 1);
     it.nblocks = (a.start + last_t) / kBlockTokens + 1;
     it.steps = (it.nblocks + kStepBlocks - 1) / kStepBlocks;
+    if constexpr (SPLIT) {
+        it.before = it.split * it.steps / a.splits;
+        it.steps = (it.split + 1) * it.steps / a.splits - it.before;
+    }
     return it;
 }
 
@@ -300,7 +321,7 @@ __device__ __forceinline__ float load_q(uint32_t q_smem, const TcArgs &a, const 
 // At most 128 registers a thread: two CTAs of 256 threads then fill an SM's (the occupancy
 // calculation gives one CTA from 119 on, clock stamps show two; 2047 tokens in FINE: 48.6 us at
 // 120, with spills, 47.6 at 128).
-template <bool FINE>
+template <bool FINE, bool SPLIT>
 __global__ void __maxnreg__(128)
     prefill_tc_kernel(const TcArgs a) {
     extern __shared__ uint8_t dyn_smem[];
@@ -316,7 +337,7 @@ __global__ void __maxnreg__(128)
     const uint32_t v_smem = k_smem + kKStages * kRingBytes;   // V ring, 8 KiB a stage
 
     const int tiles = (a.tokens + kTileTokens - 1) / kTileTokens;
-    const int items = tiles * kKvHeads;
+    const int items = tiles * kKvHeads * (SPLIT ? a.splits : 1);
     const int cta = static_cast<int>(blockIdx.x);
     const int ctas = static_cast<int>(gridDim.x);
     const int written = a.start + a.tokens;  // positions below hold K/V
@@ -349,6 +370,7 @@ __global__ void __maxnreg__(128)
         pkv::fence_barrier_init();
     }
     if constexpr (FINE) pkv::pdl_wait();  // a programmatic dependent of the read that fills its pool
+    if constexpr (SPLIT) pkv::pdl_launch_dependents();  // the merge
     // Every item reads the same block table (the chunk's request).
     for (int j = threadIdx.x; j <= (written - 1) / kBlockTokens; j += kThreads) table[j] = a.blocks[j];
     pkv::tc::fence_before_sync();
@@ -381,7 +403,7 @@ __global__ void __maxnreg__(128)
         for (int round = 0; !stop; ++round) {
             const int w = item_of(round, cta, ctas);
             if (w >= items) break;
-            const Item it = item_info(w, tiles, a);
+            const Item it = item_info<SPLIT>(w, tiles, a);
             const __half *const plane = layer_plane + it.kv * kHeadDim;
             for (int j = 0; j < it.steps; ++j, ++g) {
                 if (__any_sync(0xffffffffu, abort_flag)) {  // one decision for the warp
@@ -395,11 +417,11 @@ __global__ void __maxnreg__(128)
                     break;
                 }
                 const uint32_t dst = ring + st * kRingBytes;
-                const int nb = min(kStepBlocks, it.nblocks - j * kStepBlocks);
+                const int nb = min(kStepBlocks, it.nblocks - (it.before + j) * kStepBlocks);
 #pragma unroll
                 for (int kb = 0; kb < kStepBlocks; ++kb) {
                     if (kb >= nb) break;
-                    const int index = j * kStepBlocks + kb;
+                    const int index = (it.before + j) * kStepBlocks + kb;
                     const int32_t block = table[index];
                     const bool valid = block >= 0 && block < a.num_blocks;
                     if (!valid && lane == 0) atomicOr(a.error_flag, PKV_DEVICE_BAD_BLOCK);
@@ -439,7 +461,7 @@ __global__ void __maxnreg__(128)
             for (int round = 0; !stop; ++round) {
                 const int w = item_of(round, cta, ctas);
                 if (w >= items) break;
-                const Item it = item_info(w, tiles, a);
+                const Item it = item_info<SPLIT>(w, tiles, a);
                 // The item's Q tile is in place (the softmax loads it).
                 if (!wait_or_abort(bar_addr(bars.q_full), round & 1, &abort_flag, a.error_flag)) break;
                 for (int j = 0; j < it.steps; ++j, ++g) {
@@ -487,7 +509,7 @@ __global__ void __maxnreg__(128)
             for (int round = 0; !stop; ++round) {
                 const int w = item_of(round, cta, ctas);
                 if (w >= items) break;
-                const Item it = item_info(w, tiles, a);
+                const Item it = item_info<SPLIT>(w, tiles, a);
                 for (int j = 0; j < it.steps; ++j, ++g) {
                     const int st = g % kVStages;
                     if (!wait_or_abort(bar_addr(bars.p_full[g % kSBuffers]), (g / kSBuffers) & 1, &abort_flag,
@@ -501,7 +523,7 @@ __global__ void __maxnreg__(128)
                     // slices are 8 TMEM columns apart.
                     const uint64_t v_desc = pkv::tc::desc_mn_major_sw128(v_smem + st * kRingBytes);
                     const uint32_t p_tmem = tmem + (g % kSBuffers) * kStepKeys;
-                    const int nb = min(kStepBlocks, it.nblocks - j * kStepBlocks);
+                    const int nb = min(kStepBlocks, it.nblocks - (it.before + j) * kStepBlocks);
                     for (int kb = 0; kb < nb; ++kb) {
                         // The item's first MMA overwrites O (read out by the softmax
                         // before it published P_g).
@@ -531,7 +553,7 @@ __global__ void __maxnreg__(128)
         // of the item before it, once every S MMA that read the tile has completed.
         float next_scale = kScaleLog2;
         if (item_of(0, cta, ctas) < items) {
-            next_scale = load_q<FINE>(q_smem, a, item_info(item_of(0, cta, ctas), tiles, a), r);
+            next_scale = load_q<FINE>(q_smem, a, item_info<SPLIT>(item_of(0, cta, ctas), tiles, a), r);
             pkv::cp_async_wait<0>();
             pkv::fence_proxy_async_smem();  // generic-proxy copies -> the MMA's (async proxy) reads
             __syncwarp();
@@ -540,13 +562,14 @@ __global__ void __maxnreg__(128)
         for (int round = 0; ok; ++round) {
             const int w = item_of(round, cta, ctas);
             if (w >= items) break;
-            const Item it = item_info(w, tiles, a);
+            const Item it = item_info<SPLIT>(w, tiles, a);
             const int next = item_of(round + 1, cta, ctas);
             const int t = it.t0 + (r >> 3);
             const int pos = a.start + min(t, a.tokens - 1);  // last position this row attends to
             const int head = it.kv * 8 + (r & 7);
             const float scale = FINE ? next_scale : kScaleLog2;
-            float m = -INFINITY;  // the row maximum at its last rescale (log2 units)
+            // The row maximum at its last rescale (log2 units).  (A part may hold none of a row's keys.)
+            float m = SPLIT ? -FLT_MAX : -INFINITY;
             float l = 0.f;        // sum of this row's weights, relative to m
             for (int j = 0; j < it.steps; ++j, ++g) {
                 const uint32_t sbuf = lanes + (g % kSBuffers) * kStepKeys;  // S_g, then P_g
@@ -564,12 +587,12 @@ __global__ void __maxnreg__(128)
                 pkv::tc::tmem_wait_ld();
                 // s_full of the item's last step: every S MMA of the item has
                 // completed, so the next item's Q may replace this one's.
-                if (!FINE && last && next < items) next_scale = load_q<FINE>(q_smem, a, item_info(next, tiles, a), r);
+                if (!FINE && last && next < items) next_scale = load_q<FINE>(q_smem, a, item_info<SPLIT>(next, tiles, a), r);
 
                 float s[64];
 #pragma unroll
                 for (int c = 0; c < 64; ++c) s[c] = __uint_as_float(sr[c >> 5][c & 31]);
-                const int key0 = j * kStepKeys;
+                const int key0 = (it.before + j) * kStepKeys;
                 if (key0 + kStepKeys - 1 > a.start + it.t0) {  // the diagonal: mask positions past the row
 #pragma unroll
                     for (int c = 0; c < 64; ++c) {
@@ -672,7 +695,7 @@ __global__ void __maxnreg__(128)
                     if (!FINE && last && next < items) pkv::mbar_arrive(bar_addr(bars.q_full));
                 }
                 if (FINE && last && next < items) {  // (here the registers are free, and P.V runs)
-                    next_scale = load_q<FINE>(q_smem, a, item_info(next, tiles, a), r);
+                    next_scale = load_q<FINE>(q_smem, a, item_info<SPLIT>(next, tiles, a), r);
                     pkv::fence_proxy_async_smem();
                     __syncwarp();
                     if (lane == 0) pkv::mbar_arrive(bar_addr(bars.q_full));
@@ -689,6 +712,19 @@ __global__ void __maxnreg__(128)
             pkv::tc::tmem_ld32(lanes + kTmemO, o[0]);
             pkv::tc::tmem_ld32(lanes + kTmemO + 32, o[1]);
             pkv::tc::tmem_wait_ld();
+            if constexpr (SPLIT) {
+                if (t < a.tokens) {
+                    const int64_t at = (static_cast<int64_t>(t) * a.splits + it.split) * PKV_QUERY_HEADS + head;
+                    float4 *dst = reinterpret_cast<float4 *>(a.part_o + at * kHeadDim);
+#pragma unroll
+                    for (int c = 0; c < 64; c += 4) {
+                        dst[c / 4] = make_float4(__uint_as_float(o[c >> 5][c & 31]), __uint_as_float(o[c >> 5][(c + 1) & 31]),
+                                                 __uint_as_float(o[c >> 5][(c + 2) & 31]), __uint_as_float(o[c >> 5][(c + 3) & 31]));
+                    }
+                    *reinterpret_cast<float2 *>(a.part_ml + at * 2) = make_float2(m, l);
+                }
+                continue;
+            }
             if (t < a.tokens) {
                 uint4 *dst = reinterpret_cast<uint4 *>(a.out + static_cast<int64_t>(t) * a.out_stride +
                                                        head * kHeadDim);
@@ -714,58 +750,108 @@ __global__ void __maxnreg__(128)
     }
 }
 
+// Merge of an item's parts: sixteen lanes a (token, head), four dims each, four parts read at a time.
+constexpr int kMergeThreads = 256;
+
+__global__ void __launch_bounds__(kMergeThreads) prefill_merge_kernel(const __grid_constant__ TcArgs a) {
+    pkv::pdl_launch_dependents();
+    pkv::pdl_wait();
+    const int64_t at = static_cast<int64_t>(blockIdx.x) * (kMergeThreads / 16) + (threadIdx.x >> 4);
+    const int t = static_cast<int>(at / PKV_QUERY_HEADS), head = static_cast<int>(at % PKV_QUERY_HEADS);
+    const int dim = 4 * (threadIdx.x & 15);
+    if (t >= a.tokens) return;
+    pkv::Merge merged{-FLT_MAX, 0.f, {0.f, 0.f, 0.f, 0.f}};
+    for (int s0 = 0; s0 < a.splits; s0 += 4) {
+        float2 ml[4];
+        float4 v[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            if (s0 + i < a.splits) {
+                const int64_t part = (static_cast<int64_t>(t) * a.splits + s0 + i) * PKV_QUERY_HEADS + head;
+                ml[i] = *reinterpret_cast<const float2 *>(a.part_ml + part * 2);
+                v[i] = *reinterpret_cast<const float4 *>(a.part_o + part * kHeadDim + dim);
+            }
+        }
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            if (s0 + i < a.splits) merged.add(ml[i].x, ml[i].y, v[i]);
+        }
+    }
+    const float inv = __frcp_rn(merged.L);
+    *reinterpret_cast<uint2 *>(a.out + t * a.out_stride + head * kHeadDim + dim) =
+        make_uint2(pack2(merged.A[0] * inv, merged.A[1] * inv), pack2(merged.A[2] * inv, merged.A[3] * inv));
+}
+
 constexpr int kMaxDevices = 64;
 constexpr int kCtasPerSm = 2;
 
+// CTAs that run at once on `device`, whatever the current device is.
+int resident_ctas(int device, int *ctas) {
+    static std::atomic<int> known[kMaxDevices] = {};
+    if (device >= 0 && device < kMaxDevices) {
+        *ctas = known[device].load(std::memory_order_relaxed);
+        if (*ctas > 0) return PKV_OK;
+    }
+    int sms = 0;
+    const cudaError_t e = cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, device);
+    if (e != cudaSuccess || sms < 1) {
+        return pkv::fail(PKV_CUDA_ERROR, std::string("prefill attention: SM count query failed: ") +
+                                             cudaGetErrorString(e));
+    }
+    *ctas = sms * kCtasPerSm;
+    if (device >= 0 && device < kMaxDevices) known[device].store(*ctas, std::memory_order_relaxed);
+    return PKV_OK;
+}
+
 // Per device, once: the kernel's dynamic shared-memory limit raised, and the
 // number of its CTAs that run at once (2 per SM) recorded in *ctas.
-template <bool FINE>
+template <bool FINE, bool SPLIT>
 int prepare(int device, int *ctas) {
     static std::atomic<int> resident[kMaxDevices] = {};
     if (device >= 0 && device < kMaxDevices) {
         *ctas = resident[device].load(std::memory_order_acquire);
         if (*ctas > 0) return PKV_OK;
     }
-    cudaError_t e = cudaFuncSetAttribute(prefill_tc_kernel<FINE>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+    cudaError_t e = cudaFuncSetAttribute(prefill_tc_kernel<FINE, SPLIT>, cudaFuncAttributeMaxDynamicSharedMemorySize,
                                          kSmemBytes<FINE>);
     if (e == cudaSuccess) {
         // All of the SM's unified L1/shared memory as shared memory: two CTAs' worth.
-        e = cudaFuncSetAttribute(prefill_tc_kernel<FINE>, cudaFuncAttributePreferredSharedMemoryCarveout,
+        e = cudaFuncSetAttribute(prefill_tc_kernel<FINE, SPLIT>, cudaFuncAttributePreferredSharedMemoryCarveout,
                                  cudaSharedmemCarveoutMaxShared);
     }
     if (e != cudaSuccess) {
         return pkv::fail(PKV_CUDA_ERROR, std::string("prefill attention: cudaFuncSetAttribute: ") +
                                              cudaGetErrorString(e));
     }
-    int sms = 0;
-    e = cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, device);
-    if (e != cudaSuccess || sms < 1) {
-        return pkv::fail(PKV_CUDA_ERROR, std::string("prefill attention: SM count query failed: ") +
-                                             cudaGetErrorString(e));
-    }
     // Two CTAs fit an SM: 2 x (at most 105 KiB + static) of shared memory, 2 x 256
     // columns of TMEM, 2 x 256 threads at 128 registers.
-    const int per_sm = kCtasPerSm;
-    *ctas = sms * per_sm;
+    if (const int rc = resident_ctas(device, ctas)) return rc;
     if (device >= 0 && device < kMaxDevices) resident[device].store(*ctas, std::memory_order_release);
     return PKV_OK;
 }
 
-template <bool FINE>
+template <bool FINE, bool SPLIT>
 int launch(const TcArgs &args, cudaStream_t stream) {
     int device = 0;
     cudaError_t e = cudaGetDevice(&device);
     if (e != cudaSuccess) return pkv::fail(PKV_CUDA_ERROR, std::string("cudaGetDevice: ") + cudaGetErrorString(e));
     int resident = 0;
-    const int rc = prepare<FINE>(device, &resident);
+    const int rc = prepare<FINE, SPLIT>(device, &resident);
     if (rc) return rc;
     // One CTA per resident slot at most; each walks its share of the items.
-    const int items = (args.tokens + kTileTokens - 1) / kTileTokens * kKvHeads;
+    const int items = (args.tokens + kTileTokens - 1) / kTileTokens * kKvHeads * (SPLIT ? args.splits : 1);
     if constexpr (FINE) {
-        e = pkv::launch_pdl_smem(prefill_tc_kernel<FINE>, dim3(std::min(items, resident)), dim3(kThreads),
+        e = pkv::launch_pdl_smem(prefill_tc_kernel<FINE, SPLIT>, dim3(std::min(items, resident)), dim3(kThreads),
                                  kSmemBytes<FINE>, stream, args);
+        if constexpr (SPLIT) {
+            const int64_t heads = static_cast<int64_t>(args.tokens) * PKV_QUERY_HEADS;
+            if (e == cudaSuccess) {
+                e = pkv::launch_pdl(prefill_merge_kernel, dim3(static_cast<unsigned>(heads * 16 / kMergeThreads)),
+                                    dim3(kMergeThreads), stream, args);
+            }
+        }
     } else {
-        prefill_tc_kernel<FINE><<<std::min(items, resident), kThreads, kSmemBytes<FINE>, stream>>>(args);
+        prefill_tc_kernel<FINE, SPLIT><<<std::min(items, resident), kThreads, kSmemBytes<FINE>, stream>>>(args);
         e = cudaGetLastError();
     }
     if (e != cudaSuccess) {
@@ -778,10 +864,27 @@ int launch(const TcArgs &args, cudaStream_t stream) {
 
 namespace pkv {
 
+// Parts of each item's keys (see the header).
+int prefill_splits(int device, int32_t start, int32_t tokens, int *splits) {
+    *splits = 1;
+    const int items = (tokens + kTileTokens - 1) / kTileTokens * kKvHeads;
+    const int steps = (start + tokens + kStepKeys - 1) / kStepKeys, fewest = start / kStepKeys + 1;
+    if (fewest < kLeastSaved) return PKV_OK;
+    int resident = 0;
+    if (const int rc = resident_ctas(device, &resident)) return rc;
+    const int most = std::min({resident / items, fewest, kMostSplits});
+    if (most > 1 && steps - steps / most >= kLeastSaved) *splits = most;
+    return PKV_OK;
+}
+
+int64_t prefill_splits_bytes(int32_t tokens, int splits) {
+    return splits > 1 ? static_cast<int64_t>(tokens) * splits * PKV_QUERY_HEADS * (kHeadDim + 2) * 4 : 0;
+}
+
 int launch_prefill_attention_tc(const void *pool, int32_t num_blocks, int32_t layer, const void *query,
                                 bool query_fp32, bool fine, int64_t query_stride, const int32_t *blocks, int32_t start,
                                 int32_t tokens, void *out, int64_t out_stride, int32_t *error_flag,
-                                cudaStream_t stream) {
+                                cudaStream_t stream, int splits, float *partials) {
     TcArgs args;
     args.pool = static_cast<const __half *>(pool);
     args.query = query_fp32 ? nullptr : static_cast<const __half *>(query);
@@ -795,7 +898,11 @@ int launch_prefill_attention_tc(const void *pool, int32_t num_blocks, int32_t la
     args.start = start;
     args.tokens = tokens;
     args.error_flag = error_flag;
-    return fine ? launch<true>(args, stream) : launch<false>(args, stream);
+    args.splits = splits;
+    args.part_o = partials;
+    args.part_ml = partials != nullptr ? partials + static_cast<int64_t>(tokens) * splits * PKV_QUERY_HEADS * kHeadDim : nullptr;
+    if (splits > 1) return launch<true, true>(args, stream);
+    return fine ? launch<true, false>(args, stream) : launch<false, false>(args, stream);
 }
 
 }  // namespace pkv

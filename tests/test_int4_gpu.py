@@ -376,7 +376,7 @@ def test_decode_layer_reports_a_row_without_a_token() -> None:
 
 
 # -- a prompt chunk ----------------------------------------------------------------------
-@pytest.mark.parametrize("start, tokens", [(0, 1), (0, 15), (0, 130), (7, 40), (64, 3), (100, 64), (601, 75), (300, 500), (2000, 48), (2047, 1), (0, 2047), (0, 75), (20, 90)])
+@pytest.mark.parametrize("start, tokens", [(0, 1), (0, 15), (0, 130), (7, 40), (64, 3), (100, 64), (601, 75), (300, 500), (2000, 48), (2047, 1), (0, 2047), (0, 75), (20, 90), (700, 330), (1500, 220), (1024, 512), (1039, 701)])
 @pytest.mark.parametrize("dtype", [torch.float16, torch.float32])
 def test_prefill_attention(start, tokens, dtype) -> None:
     case = Case(31, [start + tokens])
@@ -420,7 +420,7 @@ def test_a_few_prompt_tokens_behind_a_long_context_and_a_bad_block(start, tokens
 
 
 @pytest.mark.parametrize("exponent", [-60, 16, 24, 31, 60, 100])
-@pytest.mark.parametrize("start, tokens", [(0, 1), (0, 40), (0, 200), (300, 70), (1000, 3)])
+@pytest.mark.parametrize("start, tokens", [(0, 1), (0, 40), (0, 200), (300, 70), (1000, 3), (1100, 300)])
 def test_prompt_queries_of_any_size(exponent, start, tokens) -> None:
     """Far out the largest score's value alone is left; scores within their rounding of it may take its place."""
     case = Case(37, [start + tokens])
