@@ -554,7 +554,8 @@ int pkv_int4_decode_plan(int32_t device, int32_t batch, int32_t total_blocks, in
                          int64_t *out_workspace_bytes);
 
 /* pkv_fp8_decode_attention over the 4-bit cache, with its contracts; the workspace is
- * 8448 * (batch + grid) bytes, none for a grid of 1.  Rows may have any number of tokens. */
+ * 8448 * (batch + grid) bytes, none for a grid of 1, nor for 8 blocks or less in up to 256 rows
+ * with the plan's grid.  Rows may have any number of tokens. */
 int pkv_int4_decode_attention(const void *storage, int32_t layers, int32_t num_blocks, int32_t layer, const void *query,
                               int64_t query_stride, const int32_t *lengths, const int32_t *prefix, const int32_t *flat,
                               int32_t batch, int32_t total_blocks, int32_t grid, void *out, int64_t out_stride,

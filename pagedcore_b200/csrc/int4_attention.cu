@@ -43,6 +43,7 @@
 #include <cuda_runtime.h>
 #include <stdint.h>
 
+#include <algorithm>
 #include <atomic>
 #include <cfloat>
 #include <initializer_list>
@@ -729,7 +730,7 @@ __global__ void __launch_bounds__(kThreads, 3) int4_decode_kernel(const __grid_c
     }
     // Rows without blocks: zeros, a warp looking at 32 rows.  (The merge looks at the rows' order
     // too, where there is one.)
-    for (int b = (blockIdx.x * (kWarps + 1) + warp) * 32; (a.clear || a.grid == 1) && b < a.batch; b += a.grid * kThreads) {
+    for (int b = (blockIdx.x * (kWarps + 1) + warp) * 32; (a.clear || a.part_o == nullptr) && b < a.batch; b += a.grid * kThreads) {
         const int r = b + lane;
         const int first = r < a.batch ? a.prefix_at(r) : 0, last = r < a.batch ? a.prefix_at(r + 1) : 1;
         if (r < a.batch && out_of_order(r, first, last)) atomicOr(a.error_flag, PKV_DEVICE_BAD_BLOCK);
@@ -831,7 +832,7 @@ __global__ void __launch_bounds__(kThreads, 3) int4_decode_kernel(const __grid_c
             }
             *reinterpret_cast<uint4 *>(dst) = make_uint4(x[0], x[1], x[2], x[3]);
             *reinterpret_cast<uint4 *>(dst + kDim) = make_uint4(y[0], y[1], y[2], y[3]);
-        } else if (pieces == 1) {  // begins before the list or ends behind it
+        } else if (a.part_o == nullptr) {  // begins before the list or ends behind it
             if (lane == 0) atomicOr(a.error_flag, PKV_DEVICE_BAD_BLOCK);
         } else {
             const int64_t index = static_cast<int64_t>(row) + blockIdx.x;
@@ -954,7 +955,15 @@ cudaError_t launch_merge(const ArgsOf<R> &a, cudaStream_t stream) {
                            dim3(kMergeThreads<H>), stream, a);
 }
 
-int64_t workspace_of(int64_t batch, int64_t grid) { return grid > 1 ? (batch + grid) * kPartial * 4 : 0; }
+// Whether rows may be split: not one piece, nor a list so short that all of its rows are, with a
+// piece for each.
+bool splits_rows(int64_t batch, int64_t total, int64_t grid) {
+    return grid > 1 && (total > kShortRow || batch > kWeighedRows || grid < (batch < total ? batch : total));
+}
+
+int64_t workspace_of(int64_t batch, int64_t total, int64_t grid) {
+    return splits_rows(batch, total, grid) ? (batch + grid) * kPartial * 4 : 0;
+}
 
 struct DeviceInfo {
     int sms = 0;
@@ -1055,7 +1064,7 @@ int decode(Args a, void *workspace, int64_t workspace_bytes, cudaStream_t stream
         a.query_stride < kQueryHeads * kDim || a.out_stride < kQueryHeads * kDim) {
         return pkv::fail(PKV_VALUE_ERROR, "int4 decode: rows must be 16-byte aligned, 2048 or more values apart in multiples of 8");
     }
-    const int64_t needed = workspace_of(a.batch, a.grid);
+    const int64_t needed = workspace_of(a.batch, a.capacity, a.grid);
     if (needed > 0 && (workspace == nullptr || !aligned16(workspace) || workspace_bytes < needed)) {
         return pkv::fail(PKV_VALUE_ERROR, "int4 decode: the workspace is too small (see pkv_int4_decode_plan)");
     }
@@ -1071,7 +1080,7 @@ int decode(Args a, void *workspace, int64_t workspace_bytes, cudaStream_t stream
     e = a.key != nullptr      ? launch_split(ArgsOf<Kind::kFresh>(a), stream)
         : a.prefix != nullptr ? launch_split(ArgsOf<Kind::kPlain>(a), stream)
                               : launch_split(ArgsOf<Kind::kChunk>(a), stream);
-    if (e == cudaSuccess && a.grid > 1) {
+    if (e == cudaSuccess && needed > 0) {
         e = a.prefix != nullptr ? merge(ArgsOf<Kind::kPlain>(a), info, stream) : merge(ArgsOf<Kind::kChunk>(a), info, stream);
     }
     if (e != cudaSuccess) return pkv::fail(PKV_CUDA_ERROR, std::string("int4 decode launch failed: ") + cudaGetErrorString(e));
@@ -1136,12 +1145,14 @@ extern "C" int pkv_int4_decode_plan(int32_t device, int32_t batch, int32_t total
     DeviceInfo info;
     const int rc = device_info(device, &info);
     if (rc) return rc;
-    // At most one CTA per resident slot.  (A short row alone is one piece and needs no merge: 5 blocks
+    // At most one CTA per resident slot.  (A list of short rows needs no merge: one of 5 blocks takes
     // 4.7 us, in two pieces 5.8.)
-    const int grid = batch == 1 && total_blocks <= kShortRow
-        ? 1 : pieces_of(total_blocks, batch <= kWeighedRows ? batch : total_blocks, info.sms * info.ctas_per_sm);
+    const int slots = info.sms * info.ctas_per_sm;
+    const int grid = total_blocks > kShortRow || batch > kWeighedRows
+        ? pieces_of(total_blocks, batch <= kWeighedRows ? batch : total_blocks, slots)
+        : std::max(1, std::min({batch, total_blocks, slots}));
     *out_grid = grid;
-    *out_workspace_bytes = workspace_of(batch, grid);
+    *out_workspace_bytes = workspace_of(batch, total_blocks, grid);
     return PKV_OK;
 }
 

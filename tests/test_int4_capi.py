@@ -64,8 +64,11 @@ def test_attention() -> None:
     refused(function, *decode(out=P + 8), message=b"16-byte")
     refused(function, *decode(flag=None), message=b"null pointer")
     refused(function, *decode(layer=2), message=b"layers out of range")
-    refused(function, *decode(grid=4, workspace=None), message=b"workspace")
-    refused(function, *decode(grid=4, size=5 * 8448 - 1), message=b"workspace")
+    refused(function, *decode(total=40, grid=4, workspace=None), message=b"workspace")
+    refused(function, *decode(total=40, grid=4, size=5 * 8448 - 1), message=b"workspace")
+
+    refused(function, *decode(batch=4, grid=3, workspace=None), message=b"workspace")  # fewer pieces than rows
+    refused(function, *decode(batch=300, grid=4, workspace=None), message=b"workspace")
 
     def layer(key=P, kv_stride=256, rope=P, norms=(None, None)):
         return (*CACHE, 0, P, 2048, key, P, kv_stride, rope, *norms, 1e-5, P, P, P, 1, 4, 1, 1, P, 2048, None, 0, P, None)

@@ -309,13 +309,14 @@ def test_a_block_outside_the_cache_reads_as_zeros() -> None:
 @pytest.mark.parametrize(
     "prefix", [[0, 3, 2], [-1, 2], [1, 2], [0, -5, 2], [-5, -2, 2], [-9, -1, 0, 2], [0, 1000000, 2], [0, 90, 40, 60]], ids=str
 )
+@pytest.mark.parametrize("exact", [False, True])
 @pytest.mark.parametrize("layer_call", [False, True])
-def test_rows_out_of_order_are_reported(prefix, layer_call) -> None:
+def test_rows_out_of_order_are_reported(prefix, layer_call, exact) -> None:
     case = Case(18, [16 * 60])
     count = len(prefix) - 1
     as_int = lambda x: torch.tensor(x, dtype=torch.int32, device=case.device)  # noqa: E731
     flat = case.batch()[2]
-    args = (as_int([20] * count), as_int(prefix), flat, flat.numel(), case.flag)
+    args = (as_int([20] * count), as_int(prefix), flat, prefix[-1] if exact else flat.numel(), case.flag)
     q, k, v = (randn(i, count, h, 64).half() for i, h in ((1, 32), (2, 4), (3, 4)))
     if layer_call:
         int4.decode_layer(case.cache, LAYER, q, k, v, case.rope, *args)
