@@ -225,7 +225,7 @@ struct RowScan {
 // is without blocks.  Beyond kWeighedRows rows, where a CTA has several rows and they even out, rows
 // weigh nothing.  (A decode layer of 256 rows of 1 to 2048 tokens takes 34.0, 33.2, 32.3 and 32.0 us
 // with a cost of 0, 1, 2 and 3.  Pieces of a chunk or more made short rows wait for one another: 8
-// rows of 5 tokens took 8.7 us and their layer with norms 16.3, a piece each 4.0 and 5.8.)
+// rows of 5 tokens took 8.7 us and their layer with norms 16.3, a piece each 3.3 and 5.2.)
 struct Cut {
     int total, pieces;
     bool by_row;
