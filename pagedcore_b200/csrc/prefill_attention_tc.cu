@@ -268,7 +268,7 @@ __device__ __forceinline__ float4 load_q4(const TcArgs &a, int64_t at) {
 
 // FINE: the rows of a warp times log2(e) / 8 and 2^-e, e a row's own, as two FP16 numbers that add
 // up to each value, the high halves at q_smem and the low ones a tile further.  Returns 2^e of row
-// r.  Sixteen lanes a row, so that a load takes two whole rows, and eight loads at a time (a
+// r.  Sixteen lanes a row, so that a load takes two whole rows, and four loads at a time (a
 // thread that read its own row, few loads at a time and twice for its maximum, took 11,000 clocks,
 // a fifth of the kernel).
 __device__ __forceinline__ float load_q_rows_fine(uint32_t q_smem, const TcArgs &a, const Item &it, int r) {
