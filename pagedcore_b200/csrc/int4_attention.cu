@@ -723,7 +723,12 @@ __global__ void __launch_bounds__(kThreads, 3) int4_decode_kernel(const __grid_c
         while (true) {
             const unsigned past = __ballot_sync(0xffffffffu, sample > begin);
             row += (past != 0 ? __ffs(past) - 1 : 31) * step;
-            if (step == 1) break;
+            if (step == 1) {
+                // In a list that is out of order the last samples may all lie before `begin`: no row
+                // is taken that does not end past it.
+                if (past == 0) row = INT32_MAX;
+                break;
+            }
             step = (step + 31) / 32;
             sample = row + lane * step < a.batch ? a.prefix_at(min(row + (lane + 1) * step, a.batch)) : INT32_MAX;
         }
