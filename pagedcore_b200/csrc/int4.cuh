@@ -52,6 +52,10 @@ constexpr int kBlockBytes = PKV_KV_HEADS * kHeadBytes;
 static_assert(kBlockBytes == PKV_INT4_BLOCK_BYTES, "the header gives the bytes of a block");
 constexpr uint32_t kLargestScale = 225;  // 9216
 constexpr uint32_t kNanScale = 255;
+// Tokens, list entries and rows of a call: a loop over them looks up to 64 entries, or one step of
+// a row loop over the largest grid (65535 CTAs of 160 threads), past the last within 32 bits.
+constexpr int32_t kMostEntries = INT32_MAX - (1 << 16);
+constexpr int32_t kMostRows = INT32_MAX - (1 << 24);
 
 struct Cache {
     uint8_t *storage;

@@ -78,6 +78,7 @@ constexpr uint32_t kWaitPolls = 1u << 24;
 constexpr int kRowCost = 3;  // below a chunk's blocks
 constexpr int kWeighedRows = 256;
 constexpr int kMostGrid = 65535;
+static_assert(static_cast<int64_t>(kMostGrid) * kThreads < INT32_MAX - pkv::int4::kMostRows, "a row loop steps past 32 bits");
 constexpr int kShortRow = 8;
 static_assert(kRowCost < kChunk, "a piece could lie in the cost of one row");  // pieces are kRowCost + 1 long or more
 constexpr float kScaleLog2 = 0.125f * 1.4426950408889634f;  // 64^-0.5 * log2(e)
@@ -1062,7 +1063,8 @@ int decode(Args a, void *workspace, int64_t workspace_bytes, cudaStream_t stream
     if (query == nullptr || (a.flat == nullptr && a.capacity > 0) || a.out == nullptr || a.error_flag == nullptr) {
         return pkv::fail(PKV_VALUE_ERROR, "int4 decode: null pointer argument");
     }
-    if (a.batch < 1 || a.capacity < 0 || a.grid < 1 || a.grid > kMostGrid) {
+    if (a.batch < 1 || a.batch > pkv::int4::kMostRows || a.capacity < 0 || a.capacity > pkv::int4::kMostEntries ||
+        a.grid < 1 || a.grid > kMostGrid) {
         return pkv::fail(PKV_VALUE_ERROR, "int4 decode: batch, block count or grid out of range");
     }
     if (!aligned16(query) || !aligned16(a.out) || a.query_stride % 8 || a.out_stride % 8 ||
@@ -1146,6 +1148,9 @@ extern "C" int pkv_int4_decode_plan(int32_t device, int32_t batch, int32_t total
     pkv::clear_error();
     if (out_grid == nullptr || out_workspace_bytes == nullptr || batch < 1 || total_blocks < 0) {
         return pkv::fail(PKV_VALUE_ERROR, "int4 decode plan: needs a nonempty batch");
+    }
+    if (batch > pkv::int4::kMostRows || total_blocks > pkv::int4::kMostEntries) {
+        return pkv::fail(PKV_VALUE_ERROR, "int4 decode plan: batch or block count out of range");
     }
     DeviceInfo info;
     const int rc = device_info(device, &info);

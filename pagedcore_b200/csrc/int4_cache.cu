@@ -279,6 +279,7 @@ extern "C" int pkv_int4_append_kv(void *storage, int32_t layers, int32_t num_blo
                       q_out_layer_stride % 8 || q_out_token_stride % 8))) {
         return pkv::fail(PKV_VALUE_ERROR, "int4 append: rows must be 16-byte aligned with strides in multiples of 8");
     }
+    if (tokens > pkv::int4::kMostEntries) return pkv::fail(PKV_VALUE_ERROR, "int4 append: too many tokens");
     if (layer_count > 65535) return pkv::fail(PKV_VALUE_ERROR, "int4 append: layers out of range");
     if (tokens == 0) return PKV_OK;
     AppendArgs a = {};
