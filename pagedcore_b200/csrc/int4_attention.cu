@@ -780,6 +780,10 @@ __global__ void __launch_bounds__(kThreads, 3) int4_decode_kernel(const __grid_c
         }
         Sums sums;
         sums.clear();
+        // The row's tokens from block i on.  (Behind its length a row may list any number of blocks: times
+        // 16 they may pass 32 bits.)
+        const int before = i - row_first;
+        int left = before > (length >> 4) ? 0 : length - before * kSlots;
         while (i < seg_end) {
             const int n = min(kChunk, seg_end - i);
             const int stage = consumed % kStages;
@@ -790,7 +794,8 @@ __global__ void __launch_bounds__(kThreads, 3) int4_decode_kernel(const __grid_c
                 put_fresh(fresh, smem + stage * kStageBytes + (n - 1) * pkv::int4::kBlockBytes + warp * pkv::int4::kHeadBytes,
                           (length - 1) & (kSlots - 1), lane);
             }
-            const int tokens = min(max(length - (i - row_first) * kSlots, 0), n * kSlots);  // valid ones of the chunk
+            const int tokens = min(left, n * kSlots);  // valid ones of the chunk
+            left -= tokens;
             const Places here = places.at(stage * kStageBytes);
             const auto release = [&] {
                 // Every lane has read the stage (the fence orders the reads before the copies, the
