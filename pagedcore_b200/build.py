@@ -25,6 +25,7 @@ INCLUDE = REPO_ROOT / "include"
 LIBRARY = PACKAGE_DIR / "libpagedkv.so"
 BINDING = CSRC / "binding" / "int4_ops.cpp"
 EXTENSION = PACKAGE_DIR / "_int4_ops.so"
+EXTENSION_STAMP = PACKAGE_DIR / "_int4_ops.built_for"  # built_for() of the build that made it
 
 ARCH_FLAGS = ["-gencode", "arch=compute_100a,code=sm_100a"]
 
@@ -44,8 +45,15 @@ def _library_up_to_date() -> bool:
     return all(path.stat().st_mtime <= built for path in _inputs())
 
 
+def built_for() -> str:
+    """What a build of the extension is tied to: this Python's and this torch's binary interfaces."""
+    import torch
+
+    return f"{sysconfig.get_config_var('SOABI')}, torch {torch.__version__}, C++11 ABI {int(torch.compiled_with_cxx11_abi())}"
+
+
 def _extension_up_to_date() -> bool:
-    if not EXTENSION.exists():
+    if not EXTENSION.exists() or not EXTENSION_STAMP.exists() or EXTENSION_STAMP.read_text() != built_for():
         return False
     built = EXTENSION.stat().st_mtime
     return all(path.stat().st_mtime <= built for path in (BINDING, *INCLUDE.glob("*.h")))
@@ -112,6 +120,7 @@ def _build_extension(verbose: bool) -> None:
         "-shared",
         "-fvisibility=hidden",
         f"-D_GLIBCXX_USE_CXX11_ABI={int(torch.compiled_with_cxx11_abi())}",
+        f'-DPKV_BUILT_FOR="{built_for()}"',
         f"-I{INCLUDE}",
         f"-I{root / 'include'}",
         f"-I{root / 'include' / 'torch' / 'csrc' / 'api' / 'include'}",
@@ -132,6 +141,7 @@ def _build_extension(verbose: bool) -> None:
         "-Wl,-rpath,$ORIGIN",
     ]
     _run(command, tmp, EXTENSION, verbose)
+    EXTENSION_STAMP.write_text(built_for())
 
 
 def _run(command: list[str], tmp: Path, target: Path, verbose: bool) -> None:

@@ -567,4 +567,9 @@ PyModuleDef module = {PyModuleDef_HEAD_INIT, "_int4_ops", "Operators of the 4-bi
 
 }  // namespace
 
-PyMODINIT_FUNC PyInit__int4_ops() { return PyModule_Create(&module); }
+PyMODINIT_FUNC PyInit__int4_ops() {
+    PyObject *const created = PyModule_Create(&module);
+    if (created == nullptr || PyModule_AddStringConstant(created, "built_for", PKV_BUILT_FOR) == 0) return created;
+    Py_DECREF(created);
+    return nullptr;
+}

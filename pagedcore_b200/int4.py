@@ -26,13 +26,17 @@ from dataclasses import dataclass
 import torch
 from torch import Tensor
 
+from pagedcore_b200 import build
 from pagedcore_b200._lib import check, lib
 
 try:
     from pagedcore_b200 import _int4_ops
+
+    if _int4_ops.built_for != build.built_for():
+        raise ImportError(f"it was built for {_int4_ops.built_for}, not for {build.built_for()}")
 except ImportError as error:
     raise ImportError(
-        "pagedcore_b200/_int4_ops.so is missing or was built for another torch: "
+        "pagedcore_b200/_int4_ops.so is missing or was built for another torch or Python: "
         "build it with `python -m pagedcore_b200.build`"
     ) from error
 
