@@ -4,7 +4,8 @@ The library holds the C++ block ledger and the CUDA kernels behind the C ABI
 declared in ``include/pagedkv.h``.  It is compiled with nvcc for
 ``arch=compute_100a,code=sm_100a`` and links the CUDA runtime statically, so
 it loads (and the ledger runs) on machines without a GPU.  The extension binds
-the 4-bit cache's operators of the library to torch tensors (host code only).
+the 4-bit cache's operators of the library to torch tensors (host code only); where
+torch with CUDA or Python's headers are missing, the library is built without it.
 
 Usage: ``python -m pagedcore_b200.build [--force]``.
 """
@@ -52,6 +53,21 @@ def built_for() -> str:
     return f"{sysconfig.get_config_var('SOABI')}, torch {torch.__version__}, C++11 ABI {int(torch.compiled_with_cxx11_abi())}"
 
 
+def extension_lacks() -> str | None:
+    """What the extension's build needs and this machine has not, or None."""
+    try:
+        import torch
+    except ImportError:
+        return "torch"
+    root = Path(torch.__file__).resolve().parent
+    needed = {
+        "Python's headers": Path(sysconfig.get_paths()["include"]) / "Python.h",
+        "torch's headers": root / "include" / "ATen" / "ATen.h",
+        "torch with CUDA": root / "lib" / "libtorch_cuda.so",
+    }
+    return next((name for name, path in needed.items() if not path.exists()), None)
+
+
 def _extension_up_to_date() -> bool:
     if not EXTENSION.exists() or not EXTENSION_STAMP.exists() or EXTENSION_STAMP.read_text() != built_for():
         return False
@@ -60,7 +76,7 @@ def _extension_up_to_date() -> bool:
 
 
 def up_to_date() -> bool:
-    return _library_up_to_date() and _extension_up_to_date()
+    return _library_up_to_date() and (extension_lacks() is not None or _extension_up_to_date())
 
 
 def nvcc() -> str:
@@ -74,10 +90,17 @@ def nvcc() -> str:
 
 
 def build(force: bool = False, verbose: bool = False) -> Path:
-    """Compile every source into ``libpagedkv.so``, then the extension (each skipped when up to date)."""
+    """Compile every source into ``libpagedkv.so``, then the extension (each skipped when up to date).
+
+    The extension is left out, with a line on stderr, where what it needs is missing: only
+    :mod:`pagedcore_b200.int4` is without it then.
+    """
     if force or not _library_up_to_date():
         _build_library(verbose)
-    if force or not _extension_up_to_date():
+    lacks = extension_lacks()
+    if lacks is not None:
+        print(f"{EXTENSION.name} (the 4-bit cache's operators) is not built: {lacks} not found", file=sys.stderr)
+    elif force or not _extension_up_to_date():
         _build_extension(verbose)
     return LIBRARY
 

@@ -52,3 +52,25 @@ def test_an_extension_of_another_torch_is_not_taken() -> None:
     )
     done = subprocess.run([sys.executable, "-c", code], cwd=ROOT, capture_output=True, text=True, timeout=120)
     assert "python -m pagedcore_b200.build" in done.stdout and "torch 9.9.9" in done.stdout, done.stdout + done.stderr
+
+
+@pytest.mark.parametrize("lacks", ["Python's headers", "torch", "CUDA"])
+def test_the_library_is_built_without_what_only_the_extension_needs(lacks, tmp_path, monkeypatch, capsys) -> None:
+    import torch
+
+    if lacks == "Python's headers":
+        monkeypatch.setattr(build.sysconfig, "get_paths", lambda: {"include": str(tmp_path)})
+    elif lacks == "torch":
+        monkeypatch.setitem(sys.modules, "torch", None)  # importing it raises ImportError
+    else:
+        (tmp_path / "include" / "ATen").mkdir(parents=True)
+        (tmp_path / "include" / "ATen" / "ATen.h").touch()
+        monkeypatch.setattr(torch, "__file__", str(tmp_path / "__init__.py"))
+    library = tmp_path / "libpagedkv.so"
+    monkeypatch.setattr(build, "LIBRARY", library)
+    monkeypatch.setattr(build, "EXTENSION", tmp_path / "_int4_ops.so")
+    monkeypatch.setattr(build, "EXTENSION_STAMP", tmp_path / "_int4_ops.built_for")
+    monkeypatch.setattr(build, "_run", lambda command, tmp, target, verbose: target.write_bytes(b""))
+    assert not build.up_to_date()
+    assert build.build() == library and library.exists() and not build.EXTENSION.exists()
+    assert lacks in capsys.readouterr().err and build.up_to_date()
