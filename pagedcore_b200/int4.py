@@ -45,9 +45,9 @@ _QUERY_HEADS = 32
 _HEAD_DIM = 64
 
 
-@dataclass(slots=True)
+@dataclass(frozen=True, slots=True)
 class Int4Cache:
-    """A 4-bit KV cache: bytes [layers, blocks, 4608].
+    """A 4-bit KV cache: bytes [layers, blocks, 4608].  Its tensor is checked once and stays.
 
     A block holds 16 tokens: for each of the 4 heads 512 bytes of K codes [4 groups,
     16 tokens, 8], 512 of V codes [8 chunks of 8 dims, 16 tokens, 4], 64 of K scales
@@ -83,11 +83,12 @@ class Int4Cache:
         return storage.data_ptr(), shape[0], shape[1]
 
 
-@dataclass(slots=True)
+@dataclass(frozen=True, slots=True)
 class HeadNorms:
     """Weights of the RMS norms of each query and key head, FP16 [layers, 64] each, for a cache's layers.
 
-    x * rsqrt(mean(x^2) + eps) * weight over the 64 dims of a head, before the rotation.
+    x * rsqrt(mean(x^2) + eps) * weight over the 64 dims of a head, before the rotation.  An allocator
+    and its step graphs keep the weights' addresses: values may change in place, the tensors stay.
     """
 
     query: Tensor
