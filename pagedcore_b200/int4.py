@@ -11,7 +11,7 @@ one scale of 8 bits (5 exponent and 3 fraction bits, no sign), a value being cod
 times scale, an FP16 number.  A written value moves by at most half its group's
 scale, which is about a seventh of the group's largest magnitude (values past
 64512 are held as that); a group with a value that is not finite reads as NaN.
-A token takes 288 bytes a layer, FP16 2048 and E4M3 1026.
+A token takes 288 bytes a layer, FP16 1024 and E4M3 514.
 
 With :class:`HeadNorms`, queries and keys are normed head by head before they
 are rotated, in the same pass.

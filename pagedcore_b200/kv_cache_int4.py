@@ -2,8 +2,8 @@
 
 ``Int4KVAllocator`` is :class:`KVAllocator` (same bookkeeping, calls, errors and
 transactions) whose storage is an :class:`pagedcore_b200.int4.Int4Cache`: 288 bytes
-a token and layer where the FP16 pool has 2048, so seven times the tokens in the
-same memory.  The decoder functions, the step graphs and the scheduler take it in
+a token and layer where the FP16 pool has 1024, so 3.56 times the tokens in the
+same memory (1.78 times the 8-bit cache's).  The decoder functions, the step graphs and the scheduler take it in
 place of a ``KVAllocator``.
 
 What differs: K and V are rounded to 4 bits with a scale per 16 dims (K rotated in
