@@ -25,8 +25,9 @@
 // minus 264 s is one rounding, exact); the factor of the scores and the last product undo it.
 // Weights and the layer's queries go in as two FP16 numbers each, hi = x to 11 bits and
 // lo = fp16(x - hi), at most 2^-21 of x off (one alone shows in the output beside its own
-// rounding); a query head is scaled by the power of two that brings its largest value to
-// 2^14 .. 2^15 first, whatever its range.  Scores, references, normaliser and sums are FP32.
+// rounding), below FP16's normal numbers 2^-24 (of a weight 2^-35 of the row's largest); a query
+// head is scaled by the power of two that brings its largest value to 2^14 .. 2^15 first,
+// whatever its range.  Scores, references, normaliser and sums are FP32.
 //
 // The softmax's reference is raised only when a weight would pass 2^15, and then to 2^11 below the
 // largest score, so that most blocks touch neither it nor the sums; a row's weights are relative to

@@ -62,6 +62,7 @@
 //   takes both.  (One FP16 number for each weight: relative error 2.9e-4 where the output's
 //   rounding alone gives 2.0e-4.  Making the second costs 3.4 us of the 47.6 that 2047 tokens
 //   take with the read of their values.)
+// - Weights below FP16's normal numbers are off by up to 2^-25, 2^-32 of their row's largest.
 // - The reference is m - 7 and moves when a weight would pass 2^15; past 2^20, where 7 would
 //   soon be lost in its rounding, it is m itself.
 //
@@ -568,8 +569,7 @@ __global__ void __maxnreg__(128)
             const int pos = a.start + min(t, a.tokens - 1);  // last position this row attends to
             const int head = it.kv * 8 + (r & 7);
             const float scale = FINE ? next_scale : kScaleLog2;
-            // The row maximum at its last rescale (log2 units).  (A part may hold none of a row's keys.)
-            float m = SPLIT ? -FLT_MAX : -INFINITY;
+            float m = -INFINITY;  // the row maximum at its last rescale (log2 units)
             float l = 0.f;        // sum of this row's weights, relative to m
             for (int j = 0; j < it.steps; ++j, ++g) {
                 const uint32_t sbuf = lanes + (g % kSBuffers) * kStepKeys;  // S_g, then P_g
@@ -612,7 +612,9 @@ __global__ void __maxnreg__(128)
                 for (int e = 0; e < 8; ++e) mx8[e] = fmaxf(mx8[e], s[e + 56]);
                 const float mx = pkv::fmax3(pkv::fmax3(mx8[0], mx8[1], mx8[2]), pkv::fmax3(mx8[3], mx8[4], mx8[5]),
                                             fmaxf(mx8[6], mx8[7]));
-                // Step 0 holds position 0, which every row attends to: m is finite from step 0 on.
+                // Step 0 holds position 0, which every row attends to: m is finite from step 0 on.  So it is
+                // for a part: there are no more parts than steps up to the first token of the chunk, so that
+                // a tile over the end of a step has its last two steps in one part.
                 const float m_blk = mx * scale;
                 float m_new = m;  // m = -inf at step 0: always moves
                 if constexpr (FINE) {  // m is the reference itself
