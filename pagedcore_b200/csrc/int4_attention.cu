@@ -35,9 +35,10 @@
 //
 // What bounds it: 256 rows of 1 to 2048 tokens (16,500 blocks, 76 MB) take 25 us, 11.7 of them at
 // the copy rate.  A (block, head) is 183 instructions, 266 clocks of its SM's quarter: 12 MMAs at 8
-// clocks, 48 FP16 operations at 2 and about 24 FP32 ones share the FMA pipe for 216 of them.  The
-// rest, about 9 us, is fixed: 3.4 to the first data, 3.4 between an SM's first and last CTA, the
-// merge.  (tcgen05 would read V from shared memory as FP16: 488 bytes a token and head there and
+// clocks, 48 FP16 operations at 2 and about 24 FP32 ones, 216 in all, for timed together they take as
+// long as one after the other.  (No counter shows a full pipe: over the whole kernel ALU 43 %, FMA
+// 32 %, tensor 27 %, issue slots 52 %.)  The rest, about 9 us, is fixed: 3.4 to the first data, 3.4
+// between an SM's first and last CTA, the merge.  (tcgen05 would read V from shared memory as FP16: 488 bytes a token and head there and
 // back, 14 us of the 16.5 that the stream takes now.)
 
 #include <cuda_fp16.h>
