@@ -32,8 +32,9 @@ from pagedcore_b200._lib import check, lib
 try:
     from pagedcore_b200 import _int4_ops
 
-    if _int4_ops.built_for != build.built_for():
-        raise ImportError(f"it was built for {_int4_ops.built_for}, not for {build.built_for()}")
+    _built_for = getattr(_int4_ops, "built_for", "an earlier form of this package")
+    if _built_for != build.built_for():
+        raise ImportError(f"it was built for {_built_for}, not for {build.built_for()}")
 except ImportError as error:
     raise ImportError(
         "pagedcore_b200/_int4_ops.so is missing or was built for another torch or Python: "

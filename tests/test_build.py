@@ -74,3 +74,14 @@ def test_the_library_is_built_without_what_only_the_extension_needs(lacks, tmp_p
     assert not build.up_to_date()
     assert build.build() == library and library.exists() and not build.EXTENSION.exists()
     assert lacks in capsys.readouterr().err and build.up_to_date()
+
+
+def test_an_extension_that_does_not_say_what_it_was_built_for_is_not_taken() -> None:
+    code = (
+        "import sys, types, pagedcore_b200\n"
+        "pagedcore_b200._int4_ops = sys.modules['pagedcore_b200._int4_ops'] = types.ModuleType('_int4_ops')\n"
+        "try:\n    import pagedcore_b200.int4\n"
+        "except ImportError as error:\n    print(error, '|', error.__cause__)\n"
+    )
+    done = subprocess.run([sys.executable, "-c", code], cwd=ROOT, capture_output=True, text=True, timeout=120)
+    assert "python -m pagedcore_b200.build" in done.stdout and "earlier form" in done.stdout, done.stdout + done.stderr
