@@ -38,8 +38,8 @@
 // clocks, 48 FP16 operations at 2 and about 24 FP32 ones, 216 in all, for timed together they take as
 // long as one after the other.  (No counter shows a full pipe: over the whole kernel ALU 43 %, FMA
 // 32 %, tensor 27 %, issue slots 52 %.)  The rest, about 9 us, is fixed: 3.4 to the first data, 3.4
-// between an SM's first and last CTA, the merge.  (tcgen05 would read V from shared memory as FP16: 488 bytes a token and head there and
-// back, 14 us of the 16.5 that the stream takes now.)
+// between an SM's first and last CTA, the merge.  (tcgen05 would read V from shared memory as FP16:
+// 488 bytes a token and head there and back, 14 us of the 16.5 that the stream takes now.)
 
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
